@@ -194,6 +194,10 @@ void register_policy_tc_ops(py::module& m);
 void register_tc_gemm_ops(py::module& m);
 void register_attention_ops(py::module& m);
 void register_layernorm_ops(py::module& m);
+void register_rmsnorm_ops(py::module& m);
+void register_fp8_quant_ops(py::module& m);
+void register_fp8_gemm_ops(py::module& m);
+void register_token_logprobs_ops(py::module& m);
 void register_adstar_cpu(py::module& m);
 void register_sha256_ops(py::module& m);
 void register_plan_a_ops(py::module& m);
@@ -254,6 +258,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_tc_gemm_ops(m);
   register_attention_ops(m);
   register_layernorm_ops(m);
+  register_rmsnorm_ops(m);
+  register_fp8_quant_ops(m);
+  register_fp8_gemm_ops(m);
+  register_token_logprobs_ops(m);
   register_adstar_cpu(m);
   register_sha256_ops(m);
   register_plan_a_ops(m);

@@ -1,0 +1,219 @@
+// Quantisation to e4m3 with fp32 scales for the 8-bit product: rows with one
+// scale for each 128 columns (activations and gradients), and matrices with
+// one scale for each 128 x 128 block (weights), optionally with the transposed
+// copy that the input gradient's product reads.
+//
+// The values are exactly rounded (lm_vec.h), so a quantised tensor depends on
+// its input's values alone, not on the kernel's order of operations. Bound by
+// memory: one read of each element, one byte written (two with the
+// transposed copy).
+#include <torch/extension.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "lm_vec.h"
+
+namespace py = pybind11;
+
+namespace {
+
+// A half-warp quantises one group of 128 columns, eight columns a lane.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+quant_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale,
+                  int64_t rows, int k, int groups) {
+  const int sub = threadIdx.x & 15;
+  const int64_t total = rows * groups;
+  // both halves of a warp stay in the loop together (the shuffles are whole-warp)
+  for (int64_t g0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 32 * 2; g0 < total; g0 += (int64_t)gridDim.x * 16) {
+    const int64_t g = g0 + ((threadIdx.x >> 4) & 1);
+    const bool live = g < total;
+    const int64_t r = live ? g / groups : 0;
+    const int grp = live ? (int)(g - r * groups) : 0;
+    const T* row = x + r * ldx;
+    float v[8];
+    if constexpr (VEC) {
+      const int c = grp * 128 + sub * 8;
+      if (live && c < k) {
+        lm::load8(row + c, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = grp * 128 + e * 16 + sub;
+        v[e] = live && c < k ? lm::to_f<T>(row[c]) : 0.f;
+      }
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, lm::abs_bits(v[e]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (!live) continue;
+    const float s = lm::group_scale(m);
+    const lm::Divisor dv = lm::divisor(s);
+    uint8_t* out = q + r * ldq;
+    if constexpr (VEC) {
+      const int c = grp * 128 + sub * 8;
+      if (c < k) *reinterpret_cast<uint2*>(out + c) = lm::quantize8(v, dv);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = grp * 128 + e * 16 + sub;
+        if (c < k) out[c] = (uint8_t)(lm::e4m3x2(lm::quotient_to_odd(v[e], dv), 0.f) & 0xff);
+      }
+    }
+    if (sub == 0) scale[g] = s;
+  }
+}
+
+// One CTA per 128 x 128 block, held in registers: warp w has the rows 8 i + w,
+// 32 neighbouring columns an access. The values go out through shared memory,
+// the transposed copy read down its columns.
+template <typename T>
+__global__ void __launch_bounds__(256)
+quant_blocks_kernel(const T* __restrict__ w, int64_t ldw, uint8_t* __restrict__ q, int64_t ldq,
+                    uint8_t* __restrict__ qt, int64_t ldqt, float* __restrict__ scale, float* __restrict__ scale_t,
+                    int n, int k) {
+  __shared__ uint8_t tile[128][132];
+  __shared__ uint32_t red[8];
+  const int bn = blockIdx.y, bk = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float v[16][4];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int row = bn * 128 + i * 8 + warp;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = bk * 128 + j * 32 + lane;
+      v[i][j] = row < n && col < k ? lm::to_f<T>(w[(int64_t)row * ldw + col]) : 0.f;
+      m = max(m, lm::abs_bits(v[i][j]));
+    }
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (lane == 0) red[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, red[i]);
+  const float s = lm::group_scale(m);
+  const lm::Divisor dv = lm::divisor(s);
+  if (threadIdx.x == 0) {
+    scale[bn * gridDim.x + bk] = s;
+    if (scale_t) scale_t[bk * gridDim.y + bn] = s;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      tile[i * 8 + warp][j * 32 + lane] = (uint8_t)(lm::e4m3x2(lm::quotient_to_odd(v[i][j], dv), 0.f) & 0xff);
+  __syncthreads();
+  // four columns per thread and store; the last store of a row may run into its padding (rows are 16 bytes apart)
+  for (int e = threadIdx.x; e < 128 * 32; e += 256) {
+    const int r = e >> 5, c = (e & 31) * 4;
+    if (bn * 128 + r < n && bk * 128 + c < k)
+      *reinterpret_cast<uint32_t*>(q + (int64_t)(bn * 128 + r) * ldq + bk * 128 + c) =
+          *reinterpret_cast<const uint32_t*>(&tile[r][c]);
+  }
+  if (!qt) return;
+  for (int e = threadIdx.x; e < 128 * 32; e += 256) {
+    const int r = e >> 5, c = (e & 31) * 4;   // row r of the transposed block is column r of the tile
+    if (bk * 128 + r < k && bn * 128 + c < n) {
+      const uint32_t u = tile[c][r] | (uint32_t)tile[c + 1][r] << 8 | (uint32_t)tile[c + 2][r] << 16 |
+                         (uint32_t)tile[c + 3][r] << 24;
+      *reinterpret_cast<uint32_t*>(qt + (int64_t)(bk * 128 + r) * ldqt + bn * 128 + c) = u;
+    }
+  }
+}
+
+bool known_type(torch::ScalarType t) {
+  return t == torch::kFloat32 || t == torch::kBFloat16 || t == torch::kHalf;
+}
+
+template <typename F>
+void for_type(torch::ScalarType t, F&& f) {
+  if (t == torch::kFloat32) f(float{});
+  else if (t == torch::kBFloat16) f(__nv_bfloat16{});
+  else f(__half{});
+}
+
+void check_matrix(const torch::Tensor& x, const char* what) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && known_type(x.scalar_type()), what,
+              ": needs a CUDA fp32, bf16 or fp16 matrix");
+  TORCH_CHECK(x.numel() == 0 || x.size(1) == 1 || x.stride(1) == 1, what, ": columns must be contiguous");
+  TORCH_CHECK(x.size(1) < (1ll << 31) - 256, what, ": too many columns");
+}
+
+// e4m3 [rows][cols] whose rows start 16 bytes apart, as the TMA unit reads them.
+torch::Tensor empty_q(int64_t rows, int64_t cols, const torch::Tensor& like) {
+  return torch::empty({rows, (cols + 15) / 16 * 16}, like.options().dtype(torch::kFloat8_e4m3fn)).narrow(1, 0, cols);
+}
+
+std::vector<torch::Tensor> quantize_rows(torch::Tensor x) {
+  check_matrix(x, "quantize_rows");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t rows = x.size(0), k = x.size(1), groups = (k + 127) / 128;
+  auto q = empty_q(rows, k, x);
+  auto scale = torch::empty({rows, groups}, x.options().dtype(torch::kFloat32));
+  if (rows == 0 || k == 0) return {q, scale};
+  const int64_t ldx = rows > 1 ? x.stride(0) : k;
+  const bool vec = k % 8 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  int dev = 0, sms = 0;
+  TORCH_CHECK(cudaGetDevice(&dev) == cudaSuccess &&
+              cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess,
+              "quantize_rows: device query failed");
+  const int grid = (int)std::min<int64_t>((rows * groups + 15) / 16, (int64_t)sms * 32);
+  auto st = c10::cuda::getCurrentCUDAStream().stream();
+  for_type(x.scalar_type(), [&](auto t) {
+    using T = decltype(t);
+    auto* out = reinterpret_cast<uint8_t*>(q.data_ptr());
+    const T* in = reinterpret_cast<const T*>(x.data_ptr());
+    if (vec) quant_rows_kernel<T, true><<<grid, 256, 0, st>>>(in, ldx, out, q.stride(0), scale.data_ptr<float>(), rows, (int)k, (int)groups);
+    else quant_rows_kernel<T, false><<<grid, 256, 0, st>>>(in, ldx, out, q.stride(0), scale.data_ptr<float>(), rows, (int)k, (int)groups);
+  });
+  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "quantize_rows launch failed");
+  return {q, scale};
+}
+
+// {q, scale} or, with `transposed`, {q, scale, q^T, scale^T}.
+std::vector<torch::Tensor> quantize_blocks(torch::Tensor w, bool transposed) {
+  check_matrix(w, "quantize_blocks");
+  const c10::cuda::CUDAGuard guard(w.device());
+  const int64_t n = w.size(0), k = w.size(1), bn = (n + 127) / 128, bk = (k + 127) / 128;
+  TORCH_CHECK(n < (1ll << 23), "quantize_blocks: too many rows");   // grid.y holds n / 128
+  auto q = empty_q(n, k, w);
+  auto scale = torch::empty({bn, bk}, w.options().dtype(torch::kFloat32));
+  std::vector<torch::Tensor> out = {q, scale};
+  if (transposed) {
+    out.push_back(empty_q(k, n, w));
+    out.push_back(torch::empty({bk, bn}, scale.options()));
+  }
+  if (n == 0 || k == 0) return out;
+  auto st = c10::cuda::getCurrentCUDAStream().stream();
+  for_type(w.scalar_type(), [&](auto t) {
+    using T = decltype(t);
+    quant_blocks_kernel<T><<<dim3((unsigned)bk, (unsigned)bn), 256, 0, st>>>(
+        reinterpret_cast<const T*>(w.data_ptr()), n > 1 ? w.stride(0) : k, reinterpret_cast<uint8_t*>(q.data_ptr()),
+        q.stride(0), transposed ? reinterpret_cast<uint8_t*>(out[2].data_ptr()) : nullptr,
+        transposed ? out[2].stride(0) : 0, scale.data_ptr<float>(), transposed ? out[3].data_ptr<float>() : nullptr,
+        (int)n, (int)k);
+  });
+  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "quantize_blocks launch failed");
+  return out;
+}
+
+}  // namespace
+
+void register_fp8_quant_ops(py::module& m) {
+  m.def("quantize_rows", &quantize_rows, "e4m3 rows with a scale for each 128 columns: q, scale", py::arg("x"));
+  m.def("quantize_blocks", &quantize_blocks,
+        "e4m3 matrix with a scale for each 128 x 128 block: q, scale (and their transposes)", py::arg("w"),
+        py::arg("transposed"));
+}

@@ -1,5 +1,5 @@
-// Host-side TMA tensor maps for 2-D bf16 matrices (shared by the tcgen05
-// GEMM and attention kernels).
+// Host-side TMA tensor maps for 2-D bf16 and 8-bit matrices (shared by the
+// tcgen05 GEMM and attention kernels).
 #pragma once
 
 #include <cuda.h>
@@ -38,6 +38,24 @@ inline CUtensorMap bf16_sw128(const void* ptr, int64_t rows, int64_t cols, int64
   cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1u, 1u};
   CUresult r = encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (", (int)r, ")");
+  return m;
+}
+
+// 2-D map over a row-major [rows][cols] matrix of bytes with row stride `ld`;
+// box = 128 columns x box_rows rows with 128-byte swizzle. Bytes past either
+// end read as zero.
+inline CUtensorMap u8_sw128(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && ld % 16 == 0,
+              "TMA operands need 16-byte aligned bases and row strides");
+  CUtensorMap m;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1u, 1u};
+  CUresult r = encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (", (int)r, ")");

@@ -1,0 +1,604 @@
+// Log-probabilities of given tokens under masked logits, with the entropy of
+// each row's distribution, its most probable alternatives, and the gradient.
+//
+//   z = x / T over the valid entries      lse = log sum exp z
+//   log_prob = z[token] - lse             entropy = -sum p log p
+//   dx_j = (g_l ([j = token] - p_j) - g_e p_j (log p_j + entropy)) / T
+//
+// The forward reads the logits once: every thread keeps a running maximum m,
+// s = sum e and t = sum e (x - m), e = exp((x - m) / T), of its share of a row,
+// and rescales s and t when m grows; the shares are joined with the same rule.
+// Then lse = m / T + log s and entropy = log s - t / (T s), both terms of which
+// are positive, so nothing cancels. The row's m, log s and entropy are kept for
+// the backward, which reads the logits once more and writes the gradient.
+// Masked entries are never used, whatever they hold; entries that are -inf have
+// no probability. A row without any entry left has log_prob -inf, entropy 0 and
+// no gradient; a NaN or +inf among its entries makes a row's results NaN.
+//
+// Alternatives (the `top` largest logits, equal ones by their index): at least
+// `top` entries are as large as the top-th largest of the threads' maxima, so
+// only the few threads whose maximum reaches that bound have their entries
+// looked at again, and the entries that reach it are ranked.
+//
+// Bound by memory for long rows. Rows of up to 1024 entries are held in the
+// registers of one warp or of a part of one; longer ones take a CTA each.
+#include <torch/extension.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+#include <vector>
+
+#include "lm_vec.h"
+
+namespace py = pybind11;
+
+namespace {
+
+constexpr int kMaxTop = 64;
+constexpr int kSmall = 1024;        // longest row held in one warp's registers
+constexpr int kThreads = 512;       // threads of a long row's CTA
+constexpr int kCandidates = 1024;   // entries ranked in shared memory
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Args {
+  const void* x;
+  const uint8_t* mask;     // null without one
+  const int64_t* tokens;
+  int64_t rows, ldx, ldm;
+  int v, top;
+  float inv_t;             // 1 / T
+  float* log_prob;
+  float* entropy;
+  float* top_value;        // [rows][top]
+  int64_t* top_token;      // [rows][top]
+  float* stats;            // [rows][3]: m, log s, entropy; null when no backward follows
+};
+
+// Running maximum, sum and first moment of a set of entries.
+struct Stat {
+  float m, s, t;
+};
+__device__ __forceinline__ Stat empty_stat() { return Stat{-INFINITY, 0.f, 0.f}; }
+
+// The sums of `a` for the maximum m >= a.m.
+__device__ __forceinline__ Stat rescaled(const Stat& a, float m, float c) {
+  if (a.s == 0.f) return Stat{m, 0.f, 0.f};
+  const float d = a.m - m;
+  if (!(d < 0.f)) return Stat{m, a.s, a.t};   // the same maximum (NaN sums stay NaN)
+  const float f = exp2f(d * c);
+  const float s = a.s * f;                    // a NaN stays one, even times zero
+  return Stat{m, s, f > 0.f ? (a.t + a.s * d) * f : s};
+}
+__device__ __forceinline__ Stat joined(const Stat& a, const Stat& b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  const Stat p = rescaled(a, m, c), q = rescaled(b, m, c);
+  return Stat{m, p.s + q.s, p.t + q.t};
+}
+// Adds an entry that is at most st.m.
+__device__ __forceinline__ void add_entry(Stat& st, float x, float c) {
+  const float d = x - st.m;
+  const float e = exp2f(d * c);
+  st.s += e;
+  if (e != 0.f) st.t += e * d;   // not 0 * -inf
+}
+
+template <int G>
+__device__ __forceinline__ Stat group_join(Stat st, float c) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) {
+    Stat u;
+    u.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+    u.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+    u.t = __shfl_xor_sync(0xffffffffu, st.t, o);
+    st = joined(st, u, c);
+  }
+  return st;
+}
+
+// Bits that order like the values. Both zeros, and subnormal values (which the
+// compiler's fast-math mode compares as zeros), are one value. Not for NaN.
+__device__ __forceinline__ uint32_t order_bits(float x) {
+  const uint32_t u = fabsf(x) < 0x1p-126f ? 0u : __float_as_uint(x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float from_order_bits(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+// Larger values first, then smaller indices; 0 is "none".
+__device__ __forceinline__ uint64_t entry_key(float x, int idx) {
+  return (uint64_t)order_bits(x) << 32 | (uint32_t)~(uint32_t)idx;
+}
+__device__ __forceinline__ int key_index(uint64_t k) { return (int)~(uint32_t)k; }
+
+// Whether an entry can be an alternative: it has a probability.
+__device__ __forceinline__ bool ranked(float x) { return x > -INFINITY; }
+
+template <int G>
+__device__ __forceinline__ uint64_t group_max(uint64_t k) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) {
+    const uint64_t u = __shfl_xor_sync(0xffffffffu, k, o);
+    k = u > k ? u : k;
+  }
+  return k;
+}
+
+// The row's results, by one thread.
+__device__ __forceinline__ void write_row(const Args& a, int64_t r, const Stat& st, float logit, bool valid) {
+  const bool none = st.m == -INFINITY;
+  const float logs = none ? 0.f : logf(st.s);
+  const float ent = none ? 0.f : logs - st.t / st.s * a.inv_t;
+  const int64_t tok = a.tokens[r];
+  float lp;
+  if (tok < 0) lp = 0.f;                                        // ignored
+  else if (tok >= a.v) lp = __uint_as_float(0x7fffffffu);       // no such token
+  else if (none || !valid) lp = -INFINITY;
+  else lp = (logit - st.m) * a.inv_t - logs;
+  a.log_prob[r] = lp;
+  a.entropy[r] = ent;
+  if (a.stats) {
+    a.stats[3 * r] = st.m;
+    a.stats[3 * r + 1] = logs;
+    a.stats[3 * r + 2] = ent;
+  }
+}
+
+__device__ __forceinline__ void write_top(const Args& a, int64_t r, int place, uint64_t key, const Stat& st) {
+  const bool none = key == 0;
+  a.top_token[r * a.top + place] = none ? -1 : key_index(key);
+  a.top_value[r * a.top + place] =
+      none ? -INFINITY : (from_order_bits((uint32_t)(key >> 32)) - st.m) * a.inv_t - logf(st.s);
+}
+
+// ---- short rows: G lanes per row, E entries per lane, 32 / G rows per warp ----
+template <typename T, int G, int E>
+__global__ void __launch_bounds__(256) small_fwd_kernel(const Args a) {
+  const int lane = threadIdx.x & 31, sub = lane % G;
+  const int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) / G;
+  const bool live = r < a.rows;
+  const float c = a.inv_t * kLog2e;
+  const T* row = reinterpret_cast<const T*>(a.x) + (live ? r : 0) * a.ldx;
+  const uint8_t* mrow = a.mask ? a.mask + (live ? r : 0) * a.ldm : nullptr;
+  float x[E];
+  uint32_t ok = 0;
+  Stat st = empty_stat();
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int col = e * G + sub;
+    const bool in = live && col < a.v && (!mrow || mrow[col]);
+    x[e] = in ? lm::to_f<T>(row[col]) : -INFINITY;
+    if (in) ok |= 1u << e;
+    st.m = fmaxf(st.m, x[e]);
+    if (x[e] != x[e]) st.t = x[e];   // a NaN makes the row NaN (fmaxf passes it over)
+  }
+  if (st.m != -INFINITY) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (ok >> e & 1) add_entry(st, x[e], c);
+  } else if (st.t != st.t) {
+    st = Stat{0.f, st.t, st.t};
+  }
+  st = group_join<G>(st, c);
+  const int64_t tok = live ? a.tokens[r] : -1;
+  // the taken token's logit, from the lane that has it
+  float logit = 0.f;
+  bool valid = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (tok == e * G + sub) logit = x[e], valid = ok >> e & 1;
+  const int src = (lane & ~(G - 1)) + (tok < 0 ? 0 : (int)(tok % G));
+  logit = __shfl_sync(0xffffffffu, logit, src);
+  valid = __shfl_sync(0xffffffffu, (int)valid, src) != 0;
+  if (live && sub == 0) write_row(a, r, st, logit, valid);
+  for (int k = 0; k < a.top; ++k) {
+    uint64_t best = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (ok >> e & 1 && ranked(x[e])) {
+        const uint64_t key = entry_key(x[e], e * G + sub);
+        best = key > best ? key : best;
+      }
+    best = group_max<G>(best);
+#pragma unroll
+    for (int e = 0; e < E; ++e)   // taken
+      if (best && key_index(best) == e * G + sub) ok &= ~(1u << e);
+    if (live && sub == 0) write_top(a, r, k, best, st);
+  }
+}
+
+template <typename T, int G, int E>
+__global__ void __launch_bounds__(256)
+small_bwd_kernel(const Args a, const float* __restrict__ g_lp, const float* __restrict__ g_ent, T* __restrict__ dx) {
+  const int sub = threadIdx.x % G;
+  const int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) / G;
+  if (r >= a.rows) return;
+  const T* row = reinterpret_cast<const T*>(a.x) + r * a.ldx;
+  const uint8_t* mrow = a.mask ? a.mask + r * a.ldm : nullptr;
+  const float m = a.stats[3 * r], logs = a.stats[3 * r + 1], ent = a.stats[3 * r + 2];
+  const int64_t tok = a.tokens[r];
+  const float gl = g_lp && tok >= 0 && tok < a.v ? g_lp[r] : 0.f, ge = g_ent ? g_ent[r] : 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int col = e * G + sub;
+    if (col >= a.v) break;
+    float d = 0.f;
+    if ((!mrow || mrow[col]) && m != -INFINITY) {
+      const float lp = (lm::to_f<T>(row[col]) - m) * a.inv_t - logs;
+      const float p = exp2f(lp * kLog2e);
+      d = p == 0.f ? 0.f : p * (-gl - ge * (lp + ent));
+      if (col == tok) d += gl;
+      d *= a.inv_t;
+    }
+    dx[r * a.v + col] = lm::from_f<T>(d);
+  }
+}
+
+// ---- long rows ---------------------------------------------------------------
+// A row is read in vectors of eight entries on 16-byte boundaries, whatever the
+// boundary it starts on: vector i covers the columns 8 i - shift .. + 7, where
+// `shift` entries lie before the row between the boundary and its start. The
+// first and the last vector may run out of the row and are read one by one.
+template <typename T>
+struct RowView {
+  const T* row;
+  const uint8_t* mask;
+  int v, shift, vectors;
+  bool mask_aligned;   // the mask's bytes of a vector lie on an 8-byte boundary
+  __device__ __forceinline__ RowView(const Args& a, int64_t r) {
+    row = reinterpret_cast<const T*>(a.x) + r * a.ldx;
+    mask = a.mask ? a.mask + r * a.ldm : nullptr;
+    v = a.v;
+    shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    vectors = (v + shift + 7) / 8;
+    mask_aligned = mask && ((reinterpret_cast<uintptr_t>(mask) - shift) & 7) == 0;
+  }
+  // The entries of vector i and which of them are valid (bit e).
+  __device__ __forceinline__ uint32_t load(int i, float (&x)[8]) const {
+    const int c0 = 8 * i - shift;
+    uint32_t ok = 0xff;
+    if (c0 >= 0 && c0 + 8 <= v) {
+      lm::load8(row + c0, x);
+      if (mask) {
+        if (mask_aligned) {
+          const uint2 b = *reinterpret_cast<const uint2*>(mask + c0);
+          ok = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            ok |= (b.x >> 8 * e & 0xff ? 1u : 0u) << e;
+            ok |= (b.y >> 8 * e & 0xff ? 1u : 0u) << (e + 4);
+          }
+        } else {
+          ok = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ok |= (mask[c0 + e] ? 1u : 0u) << e;
+        }
+      }
+    } else {
+      ok = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = c0 + e;
+        x[e] = 0.f;
+        if (c >= 0 && c < v && (!mask || mask[c])) {
+          x[e] = lm::to_f<T>(row[c]);
+          ok |= 1u << e;
+        }
+      }
+    }
+    return ok;
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) long_fwd_kernel(const Args a) {
+  constexpr int W = kThreads / 32;
+  __shared__ Stat red[W];
+  __shared__ uint64_t keys[kThreads], cand[kCandidates], found[kMaxTop];
+  __shared__ uint64_t bound_s;
+  __shared__ int count_s;
+  const int64_t r = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float c = a.inv_t * kLog2e;
+  const RowView<T> view(a, r);
+  Stat st = empty_stat();
+  int first = 0;   // the vector in which this thread's maximum was first met
+  for (int i = threadIdx.x; i < view.vectors; i += kThreads) {
+    float x[8];
+    const uint32_t ok = view.load(i, x);
+    float m = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (!(ok >> e & 1)) x[e] = -INFINITY;
+      m = fmaxf(m, x[e]);
+    }
+    if (m > st.m) {
+      st = rescaled(st, m, c);
+      first = i;
+    }
+    if (st.m != -INFINITY) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) add_entry(st, x[e], c);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (x[e] != x[e]) st.s = x[e];   // a NaN makes the row NaN
+  }
+  // NaN alone: any finite maximum carries it through the joining
+  const bool nan_only = st.m == -INFINITY && st.s != st.s;
+  Stat mine = nan_only ? Stat{0.f, st.s, st.s} : st;
+  mine = group_join<32>(mine, c);
+  if (lane == 0) red[warp] = mine;
+  if (a.top) {
+    keys[threadIdx.x] = st.m == -INFINITY ? 0 : entry_key(st.m, first);
+    if (threadIdx.x == 0) count_s = 0;
+  }
+  __syncthreads();
+  Stat all = red[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) all = joined(all, red[w], c);
+  if (threadIdx.x == 0) {
+    const int64_t tok = a.tokens[r];
+    float logit = 0.f;
+    bool valid = false;
+    if (tok >= 0 && tok < a.v) {
+      valid = !view.mask || view.mask[tok];
+      if (valid) logit = lm::to_f<T>(view.row[tok]);
+    }
+    write_row(a, r, all, logit, valid);
+  }
+  if (!a.top) return;
+  // the top-th largest of the threads' maxima, by the first warp
+  if (warp == 0) {
+    uint64_t k[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) k[i] = keys[i * 32 + lane];
+    uint64_t best = 0;
+    for (int n = 0; n < a.top; ++n) {
+      uint64_t own = 0;
+#pragma unroll
+      for (int i = 0; i < W; ++i) own = k[i] > own ? k[i] : own;
+      best = group_max<32>(own);
+      if (!best) break;
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (k[i] == best) k[i] = 0;
+    }
+    if (lane == 0) bound_s = best;   // 0: fewer than `top` threads have an entry, so every entry counts
+  }
+  __syncthreads();
+  const uint64_t bound = bound_s;
+  // entries at or above the bound: a larger value, or the same value in no later vector
+  for (int owner = warp; owner < kThreads; owner += W) {
+    if (keys[owner] == 0 || keys[owner] < bound) continue;
+    for (int i0 = owner; i0 < view.vectors; i0 += kThreads * 32) {
+      const int i = i0 + lane * kThreads;
+      if (i >= view.vectors) continue;
+      float x[8];
+      const uint32_t ok = view.load(i, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (!(ok >> e & 1) || !ranked(x[e])) continue;
+        if (entry_key(x[e], i) < bound) continue;
+        const int at = atomicAdd(&count_s, 1);
+        if (at < kCandidates) cand[at] = entry_key(x[e], 8 * i - view.shift + e);
+      }
+    }
+  }
+  __syncthreads();
+  const int count = count_s;
+  if (count <= kCandidates) {
+    // an entry's place is the number of entries above it
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+      const uint64_t key = cand[i];
+      int place = 0;
+      for (int j = 0; j < count; ++j) place += cand[j] > key;
+      if (place < a.top) found[place] = key;
+    }
+    for (int i = count + threadIdx.x; i < a.top; i += kThreads) found[i] = 0;
+    __syncthreads();
+  } else {
+    // too many for shared memory (many equal or clustered maxima): one pass over the row for each place
+    uint64_t last = ~0ull;
+    for (int n = 0; n < a.top; ++n) {
+      uint64_t best = 0;
+      for (int i = threadIdx.x; i < view.vectors; i += kThreads) {
+        float x[8];
+        const uint32_t ok = view.load(i, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (!(ok >> e & 1) || !ranked(x[e])) continue;
+          const uint64_t key = entry_key(x[e], 8 * i - view.shift + e);
+          if (key < last && key > best) best = key;
+        }
+      }
+      best = group_max<32>(best);
+      __syncthreads();
+      if (lane == 0) cand[warp] = best;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < W; ++w) best = cand[w] > best ? cand[w] : best;
+      last = best;
+      if (threadIdx.x == 0) found[n] = best;
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < a.top; i += kThreads) write_top(a, r, i, found[i], all);
+}
+
+// The gradient: a CTA takes 256 x kBwdVectors vectors of one row.
+constexpr int kBwdVectors = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+long_bwd_kernel(const Args a, const float* __restrict__ g_lp, const float* __restrict__ g_ent, T* __restrict__ dx,
+                int parts) {
+  const int64_t r = blockIdx.x / parts;
+  const int part = (int)(blockIdx.x - r * parts);
+  const RowView<T> view(a, r);
+  const float m = a.stats[3 * r], logs = a.stats[3 * r + 1], ent = a.stats[3 * r + 2];
+  const int64_t tok = a.tokens[r];
+  const float gl = g_lp && tok >= 0 && tok < a.v ? g_lp[r] : 0.f, ge = g_ent ? g_ent[r] : 0.f;
+  const bool none = m == -INFINITY;
+  T* out = dx + r * a.v;
+  const bool same = ((reinterpret_cast<uintptr_t>(out) - view.shift * sizeof(T)) & 15) == 0;
+#pragma unroll
+  for (int j = 0; j < kBwdVectors; ++j) {
+    const int i = (part * kBwdVectors + j) * 256 + threadIdx.x;
+    if (i >= view.vectors) continue;
+    float x[8];
+    const uint32_t ok = view.load(i, x);
+    const int c0 = 8 * i - view.shift;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float d = 0.f;
+      if (ok >> e & 1 && !none) {
+        const float lp = (x[e] - m) * a.inv_t - logs;
+        const float p = exp2f(lp * kLog2e);
+        d = p == 0.f ? 0.f : p * (-gl - ge * (lp + ent));
+        if (c0 + e == tok) d += gl;
+        d *= a.inv_t;
+      }
+      x[e] = d;
+    }
+    if (same && c0 >= 0 && c0 + 8 <= a.v) {
+      lm::store8(out + c0, x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c0 + e >= 0 && c0 + e < a.v) out[c0 + e] = lm::from_f<T>(x[e]);
+    }
+  }
+}
+
+template <typename F>
+void for_type(torch::ScalarType t, F&& f) {
+  if (t == torch::kFloat32) f(float{});
+  else if (t == torch::kBFloat16) f(__nv_bfloat16{});
+  else f(__half{});
+}
+
+// Lanes per row and entries per lane of a short row.
+template <typename F>
+void for_small(int v, F&& f) {
+  auto go = [&](auto g, auto e) { f(g, e); };
+  using std::integral_constant;
+  if (v <= 8) go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+  else if (v <= 32) go(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+  else if (v <= 128) go(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+  else if (v <= 512) go(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+  else go(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+}
+
+Args common_args(const torch::Tensor& x, const torch::Tensor& tokens, const c10::optional<torch::Tensor>& mask,
+                 double temperature) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 &&
+                  (x.scalar_type() == torch::kFloat32 || x.scalar_type() == torch::kBFloat16 ||
+                   x.scalar_type() == torch::kHalf),
+              "token_log_probs: logits must be a CUDA fp32, bf16 or fp16 [rows, V] tensor");
+  TORCH_CHECK(x.size(1) >= 1 && x.size(1) < (1ll << 30), "token_log_probs: V must be in 1..2^30 - 1");
+  TORCH_CHECK(x.numel() == 0 || x.size(1) == 1 || x.stride(1) == 1, "token_log_probs: the logits of a row must be contiguous");
+  TORCH_CHECK(x.size(0) < (1ll << 31) - 1, "token_log_probs: too many rows");
+  TORCH_CHECK(tokens.is_cuda() && tokens.device() == x.device() && tokens.scalar_type() == torch::kInt64 &&
+                  tokens.dim() == 1 && tokens.size(0) == x.size(0) && tokens.is_contiguous(),
+              "token_log_probs: tokens must be a contiguous int64 [rows] on the logits' device");
+  TORCH_CHECK(temperature > 0., "token_log_probs: the temperature must be positive");
+  Args a{};
+  a.x = x.data_ptr();
+  a.rows = x.size(0);
+  a.v = (int)x.size(1);
+  a.ldx = a.rows > 1 ? x.stride(0) : a.v;
+  if (mask) {
+    TORCH_CHECK(mask->is_cuda() && mask->device() == x.device() && mask->scalar_type() == torch::kBool &&
+                    mask->sizes() == x.sizes() && (x.numel() == 0 || a.v == 1 || mask->stride(1) == 1),
+                "token_log_probs: mask must be bool [rows, V] with contiguous rows on the logits' device");
+    a.mask = reinterpret_cast<const uint8_t*>(mask->data_ptr());
+    a.ldm = a.rows > 1 ? mask->stride(0) : a.v;
+  }
+  a.tokens = tokens.data_ptr<int64_t>();
+  a.inv_t = (float)(1. / temperature);
+  return a;
+}
+
+// Returns {log_prob, entropy, top_value, top_token, stats (empty unless keep)}.
+std::vector<torch::Tensor> token_log_probs_fwd(torch::Tensor x, torch::Tensor tokens, c10::optional<torch::Tensor> mask,
+                                               double temperature, int64_t top, bool keep) {
+  Args a = common_args(x, tokens, mask, temperature);
+  TORCH_CHECK(top >= 0 && top <= kMaxTop, "token_log_probs: top must be in 0..", kMaxTop);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const auto f32 = x.options().dtype(torch::kFloat32);
+  auto lp = torch::empty({a.rows}, f32), ent = torch::empty({a.rows}, f32);
+  auto tv = torch::empty({a.rows, top}, f32);
+  auto tt = torch::empty({a.rows, top}, x.options().dtype(torch::kInt64));
+  auto stats = torch::empty({keep ? a.rows : 0, 3}, f32);
+  if (a.rows == 0) return {lp, ent, tv, tt, stats};
+  a.top = (int)top;
+  a.log_prob = lp.data_ptr<float>();
+  a.entropy = ent.data_ptr<float>();
+  a.top_value = tv.data_ptr<float>();
+  a.top_token = tt.data_ptr<int64_t>();
+  a.stats = keep ? stats.data_ptr<float>() : nullptr;
+  auto st = c10::cuda::getCurrentCUDAStream().stream();
+  for_type(x.scalar_type(), [&](auto t) {
+    using T = decltype(t);
+    if (a.v <= kSmall) {
+      for_small(a.v, [&](auto g, auto e) {
+        constexpr int G = decltype(g)::value, E = decltype(e)::value;
+        small_fwd_kernel<T, G, E><<<(unsigned)((a.rows * G + 255) / 256), 256, 0, st>>>(a);
+      });
+    } else {
+      long_fwd_kernel<T><<<(unsigned)a.rows, kThreads, 0, st>>>(a);
+    }
+  });
+  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "token_log_probs launch failed");
+  return {lp, ent, tv, tt, stats};
+}
+
+torch::Tensor token_log_probs_bwd(torch::Tensor x, torch::Tensor tokens, c10::optional<torch::Tensor> mask,
+                                  double temperature, torch::Tensor stats, c10::optional<torch::Tensor> g_lp,
+                                  c10::optional<torch::Tensor> g_ent) {
+  Args a = common_args(x, tokens, mask, temperature);
+  TORCH_CHECK(stats.is_cuda() && stats.device() == x.device() && stats.scalar_type() == torch::kFloat32 &&
+                  stats.numel() == 3 * a.rows && stats.is_contiguous(), "token_log_probs: stats must be fp32 [rows, 3]");
+  for (auto* g : {&g_lp, &g_ent})
+    if (*g)
+      TORCH_CHECK((*g)->is_cuda() && (*g)->device() == x.device() && (*g)->scalar_type() == torch::kFloat32 &&
+                      (*g)->numel() == a.rows && (*g)->is_contiguous(), "token_log_probs: gradients must be fp32 [rows]");
+  const c10::cuda::CUDAGuard guard(x.device());
+  auto dx = torch::empty({a.rows, (int64_t)a.v}, x.options());
+  if (a.rows == 0) return dx;
+  a.stats = stats.data_ptr<float>();
+  const float* gl = g_lp ? g_lp->data_ptr<float>() : nullptr;
+  const float* ge = g_ent ? g_ent->data_ptr<float>() : nullptr;
+  auto st = c10::cuda::getCurrentCUDAStream().stream();
+  for_type(x.scalar_type(), [&](auto t) {
+    using T = decltype(t);
+    T* out = reinterpret_cast<T*>(dx.data_ptr());
+    if (a.v <= kSmall) {
+      for_small(a.v, [&](auto g, auto e) {
+        constexpr int G = decltype(g)::value, E = decltype(e)::value;
+        small_bwd_kernel<T, G, E><<<(unsigned)((a.rows * G + 255) / 256), 256, 0, st>>>(a, gl, ge, out);
+      });
+    } else {
+      const int parts = (int)(((int64_t)a.v + 14) / 8 / (256 * kBwdVectors) + 1);   // a row may start inside a vector
+      TORCH_CHECK(a.rows * parts < (1ll << 31), "token_log_probs: too many logits");
+      long_bwd_kernel<T><<<(unsigned)(a.rows * parts), 256, 0, st>>>(a, gl, ge, out, parts);
+    }
+  });
+  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "token_log_probs backward launch failed");
+  return dx;
+}
+
+}  // namespace
+
+void register_token_logprobs_ops(py::module& m) {
+  m.def("token_log_probs_fwd", &token_log_probs_fwd,
+        "log-probabilities of given tokens: log_prob, entropy, top values, top tokens, stats", py::arg("logits"),
+        py::arg("tokens"), py::arg("mask"), py::arg("temperature"), py::arg("top"), py::arg("keep"));
+  m.def("token_log_probs_bwd", &token_log_probs_bwd, "gradient of the log-probabilities and entropies",
+        py::arg("logits"), py::arg("tokens"), py::arg("mask"), py::arg("temperature"), py::arg("stats"),
+        py::arg("g_log_prob"), py::arg("g_entropy"));
+  m.attr("TOKEN_LOG_PROBS_MAX_TOP") = kMaxTop;
+}

@@ -1,0 +1,288 @@
+"""8-bit floating-point products with a scale for each block of 128 on the
+sm_100a tensor cores (``csrc/fp8_gemm.cu``, ``csrc/fp8_quant.cu``).
+
+Operands are e4m3 with fp32 scales, a value being its 8-bit number times its
+scale:
+
+* rows (activations, gradients): one scale for each row and 128 columns,
+  ``quantize_rows(x) -> (q [..., K], scale [..., ceil(K / 128)])``;
+* matrices (weights): one scale for each 128 x 128 block,
+  ``quantize_blocks(w) -> (q [N, K], scale [ceil(N / 128), ceil(K / 128)])``.
+
+A scale is the largest magnitude of its group divided by 448, rounded to fp32,
+and the 8-bit number is the one nearest to the exact quotient. A group that
+holds a NaN or an infinity becomes NaN.
+
+``fp8_matmul(a, a_scale, b, b_scale, bias, out_dtype)`` is the product of rows
+with a weight matrix, a b^T, with fp32 sums. It has no gradient.
+
+``fp8_linear(x, weight, bias)`` is a linear layer for training: both operands
+are quantised on the way in; the backward takes the quantised gradient through
+the same quantised weight (rounding counts as the identity), and the weight's
+gradient as a bf16 product of the unquantised gradient and input.
+``Fp8Linear`` is the module (a drop-in ``nn.Linear``, beside ``TcLinear``), and
+``FrozenFp8Linear`` the one for acting and serving, which holds 8-bit weights
+only. ``freeze_fp8(module)`` swaps a module's linear layers for frozen ones.
+
+On CPU all of them compute the same values in plain PyTorch. The product's
+kernel reports timed-out waits through the status word of the bf16 GEMM
+(``ops.tc_linear.check_gemm_status``).
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor, nn
+from torch.autograd.function import once_differentiable
+
+from ..utils import launches
+from .ext import require_extension
+from .rmsnorm import from_rows
+from .tc_linear import _bf16_padded, _pad8, _result_dtype, _Status, gemm
+
+GROUP = 128
+E4M3 = torch.float8_e4m3fn
+E4M3_MAX = 448.
+_MIN_AMAX = E4M3_MAX * 2. ** -126
+_INPUTS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _groups(k: int) -> int:
+    return (k + GROUP - 1) // GROUP
+
+
+def _padded_q(values: Tensor) -> Tensor:
+    """`values` in storage whose rows start 16 bytes apart."""
+    m, k = values.shape
+    buf = torch.zeros((m, (k + 15) // 16 * 16), dtype=torch.uint8, device=values.device)
+    buf[:, :k] = values.view(torch.uint8)
+    return buf.view(E4M3)[:, :k]
+
+
+def _round_e4m3(t: Tensor) -> Tensor:
+    """The nearest e4m3 number of each fp64 value (ties to even), in fp64."""
+    _, exponent = torch.frexp(t)
+    step = torch.ldexp(torch.ones_like(t), exponent.clamp_min(-5) - 4)
+    return torch.round(t / step) * step
+
+
+def _scales(amax: Tensor) -> Tensor:
+    return (amax.double().clamp_min(_MIN_AMAX) / E4M3_MAX).float()
+
+
+def reference_quantize_rows(x: Tensor) -> tuple[Tensor, Tensor]:
+    """``quantize_rows`` of a matrix in plain PyTorch."""
+    m, k = x.shape
+    g = _groups(k)
+    padded = torch.zeros((m, g * GROUP), dtype=torch.float32, device=x.device)
+    padded[:, :k] = x
+    padded = padded.view(m, g, GROUP)
+    scale = _scales(padded.abs().amax(-1)) if g else padded.new_zeros((m, 0))
+    q = _round_e4m3(padded.double() / scale[..., None].double())
+    return _padded_q(q.view(m, -1)[:, :k].to(torch.float32).to(E4M3)), scale
+
+
+def reference_quantize_blocks(w: Tensor) -> tuple[Tensor, Tensor]:
+    """``quantize_blocks`` in plain PyTorch."""
+    n, k = w.shape
+    bn, bk = _groups(n), _groups(k)
+    padded = torch.zeros((bn * GROUP, bk * GROUP), dtype=torch.float32, device=w.device)
+    padded[:n, :k] = w
+    padded = padded.view(bn, GROUP, bk, GROUP)
+    scale = _scales(padded.abs().amax((1, 3))) if bn and bk else padded.new_zeros((bn, bk))
+    q = _round_e4m3(padded.double() / scale[:, None, :, None].double())
+    return _padded_q(q.view(bn * GROUP, bk * GROUP)[:n, :k].to(torch.float32).to(E4M3)), scale
+
+
+def dequantize_rows(q: Tensor, scale: Tensor) -> Tensor:
+    """The fp32 values of quantised rows."""
+    return q.float() * scale.repeat_interleave(GROUP, -1)[..., :q.shape[-1]]
+
+
+def dequantize_blocks(q: Tensor, scale: Tensor) -> Tensor:
+    """The fp32 values of a matrix quantised in blocks."""
+    n, k = q.shape
+    return q.float() * scale.repeat_interleave(GROUP, 0)[:n].repeat_interleave(GROUP, 1)[:, :k]
+
+
+def _check_input(x: Tensor, dims: int, what: str) -> None:
+    if x.dtype not in _INPUTS or x.dim() < dims:
+        raise ValueError(f"{what} takes fp32, bf16 or fp16 tensors of at least {dims} dimension(s)")
+
+
+def _matrix(x: Tensor) -> Tensor:
+    y = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.reshape(x.shape[:-1].numel(), 0)
+    return y if y.stride(-1) == 1 and (y.shape[0] <= 1 or y.stride(0) >= y.shape[1]) else y.contiguous()
+
+
+def quantize_rows(x: Tensor) -> tuple[Tensor, Tensor]:
+    """`x` [..., K] as e4m3 with one fp32 scale for each row and 128 columns
+    (see the module docstring). No gradient."""
+    _check_input(x, 1, "quantize_rows")
+    x2 = _matrix(x.detach())
+    if x.is_cuda:
+        launches.add(1)
+        q, scale = require_extension().quantize_rows(x2)
+    else:
+        q, scale = reference_quantize_rows(x2)
+    return from_rows(q, x.shape[:-1]), from_rows(scale, x.shape[:-1])
+
+
+def quantize_blocks(w: Tensor, transposed: bool = False):
+    """`w` [N, K] as e4m3 with one fp32 scale for each 128 x 128 block: (q,
+    scale), with `transposed` (q, scale, q^T, scale^T), the transposes being
+    matrices of their own. No gradient."""
+    _check_input(w, 2, "quantize_blocks")
+    if w.dim() != 2:
+        raise ValueError("quantize_blocks takes a matrix")
+    w2 = _matrix(w.detach())
+    if w.is_cuda:
+        launches.add(1)
+        return tuple(require_extension().quantize_blocks(w2, bool(transposed)))
+    q, scale = reference_quantize_blocks(w2)
+    return (q, scale, _padded_q(q.view(torch.uint8).t().view(E4M3)), scale.t().contiguous()) if transposed \
+        else (q, scale)
+
+
+def _operand(q: Tensor) -> Tensor:
+    """`q` as the kernel reads it: rows 16 bytes apart on a 16-byte aligned base (a copy only where they are not)."""
+    ok = (q.shape[1] <= 1 or q.stride(1) == 1) and (q.shape[0] <= 1 or (q.stride(0) % 16 == 0
+                                                                        and q.stride(0) >= q.shape[1]))
+    return q if ok and q.data_ptr() % 16 == 0 else _padded_q(q)
+
+
+def reference_fp8_matmul(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Tensor | None = None,
+                         out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """``fp8_matmul`` of matrices in plain fp32 PyTorch."""
+    y = dequantize_rows(a, a_scale) @ dequantize_blocks(b, b_scale).t()
+    return (y if bias is None else y + bias.float()).to(out_dtype)
+
+
+def fp8_matmul(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Tensor | None = None,
+               out_dtype: torch.dtype = torch.bfloat16, wait_ns: int = 2_000_000_000) -> Tensor:
+    """a b^T of quantised rows `a` [..., K] and a quantised matrix `b` [N, K]
+    with their scales, plus `bias` [N]: [..., N] in `out_dtype` (fp32, bf16 or
+    fp16). `wait_ns` bounds every pipeline wait inside the kernel."""
+    if a.dtype != E4M3 or b.dtype != E4M3 or a.dim() < 1 or b.dim() != 2:
+        raise ValueError("fp8_matmul takes e4m3 rows [..., K] and an e4m3 matrix [N, K]")
+    k, n, lead = a.shape[-1], b.shape[0], a.shape[:-1]
+    if b.shape[1] != k:
+        raise ValueError(f"fp8_matmul: a has {k} columns and b {b.shape[1]}")
+    if a_scale.shape != (*lead, _groups(k)) or b_scale.shape != (_groups(n), _groups(k)):
+        raise ValueError(f"fp8_matmul needs scales {(*lead, _groups(k))} and {(_groups(n), _groups(k))}, "
+                         f"not {tuple(a_scale.shape)} and {tuple(b_scale.shape)}")
+    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
+        raise ValueError("fp8_matmul needs fp32 scales")
+    if bias is not None and bias.shape != (n,):
+        raise ValueError(f"fp8_matmul needs a bias [{n}]")
+    if out_dtype not in _INPUTS:
+        raise ValueError("fp8_matmul gives fp32, bf16 or fp16")
+    if any(t is not None and t.device != a.device for t in (a_scale, b, b_scale, bias)):
+        raise ValueError("fp8_matmul needs all of its tensors on one device")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (a_scale, b_scale, bias)):
+        raise ValueError("fp8_matmul has no gradient: use fp8_linear, or call it under torch.no_grad()")
+    rows = lead.numel()
+    a2, s2 = a.reshape(rows, k), a_scale.reshape(rows, _groups(k))
+    if not a.is_cuda:
+        return reference_fp8_matmul(a2, s2, b, b_scale, bias, out_dtype).view(*lead, n)
+    b32 = None if bias is None else bias.detach().float().contiguous()
+    y = require_extension().fp8_matmul(_operand(a2), s2.contiguous(), _operand(b), b_scale.contiguous(), b32,
+                                       out_dtype, _Status.get(a.device), int(wait_ns))
+    launches.add(1)
+    _Status.after_launch(a.device)
+    return y.view(*lead, n)
+
+
+class _Fp8LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        x2 = _matrix(x)
+        xq, xs = quantize_rows(x2)
+        # the input gradient reads the weight down its columns: its transposed copy is written by the same pass
+        wq, ws, *t = quantize_blocks(weight, transposed=ctx.needs_input_grad[0])
+        target = _result_dtype(x)
+        b = None if bias is None else bias.detach()
+        y = fp8_matmul(xq, xs, wq, ws, b, target)
+        keep = x2 if ctx.needs_input_grad[1] else None
+        if keep is not None and x.is_cuda and keep.dtype != torch.bfloat16:
+            keep = keep.to(torch.bfloat16)   # the weight gradient's product takes bf16 operands
+        ctx.save_for_backward(keep, *t)
+        ctx.meta = (x.shape, x.dtype, weight.shape, weight.dtype, None if bias is None else bias.dtype)
+        return y.view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        keep, *t = ctx.saved_tensors
+        x_shape, x_dtype, (n, k), w_dtype, b_dtype = ctx.meta
+        g = gy.reshape(-1, n)
+        gx = gw = gb = None
+        if ctx.needs_input_grad[0]:
+            gq, gs = quantize_rows(g)
+            gx = fp8_matmul(gq, gs, t[0], t[1], out_dtype=x_dtype).view(x_shape)
+        if ctx.needs_input_grad[1]:
+            if g.is_cuda:
+                gw = gemm(_bf16_padded(g, _pad8(n)), _bf16_padded(keep, _pad8(k)), a_mn=True, b_mn=True)[:n, :k]
+            else:
+                gw = g.float().t() @ keep.float()
+            gw = gw.to(w_dtype)
+        if ctx.needs_input_grad[2]:
+            gb = g.sum(0, dtype=torch.float32).to(b_dtype)
+        return gx, gw, gb
+
+
+def fp8_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tensor:
+    """x weight^T + bias with both operands quantised to e4m3 (see the module
+    docstring), with autograd. The result has x's dtype, or the autocast dtype
+    inside a CUDA autocast region."""
+    _check_input(x, 1, "fp8_linear")
+    _check_input(weight, 2, "fp8_linear")
+    if weight.dim() != 2 or x.shape[-1] != weight.shape[1] or (bias is not None and bias.shape != weight.shape[:1]):
+        raise ValueError(f"fp8_linear: x {tuple(x.shape)}, weight {tuple(weight.shape)} and bias do not fit")
+    if any(t is not None and t.device != x.device for t in (weight, bias)):
+        raise ValueError("fp8_linear needs all of its tensors on one device")
+    return _Fp8LinearFn.apply(x, weight, bias)
+
+
+class Fp8Linear(nn.Linear):
+    """nn.Linear whose products run in 8 bits; its parameters stay as they are
+    (fp32 masters) and are quantised by every call."""
+
+    def forward(self, x: Tensor) -> Tensor:
+        return fp8_linear(x, self.weight, self.bias)
+
+
+class FrozenFp8Linear(nn.Module):
+    """A linear layer that holds its weight in 8 bits (buffers ``weight_q``,
+    ``weight_scale`` and ``bias``): for acting and serving, no gradient."""
+
+    def __init__(self, weight: Tensor, bias: Tensor | None = None):
+        super().__init__()
+        q, scale = quantize_blocks(weight)
+        self.out_features, self.in_features = weight.shape
+        self.register_buffer("weight_q", q)
+        self.register_buffer("weight_scale", scale)
+        self.register_buffer("bias", None if bias is None else bias.detach().float().clone())
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear) -> "FrozenFp8Linear":
+        return cls(linear.weight, linear.bias)
+
+    def forward(self, x: Tensor) -> Tensor:
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise ValueError("FrozenFp8Linear has no gradient: call it under torch.no_grad()")
+        xq, xs = quantize_rows(x)
+        return fp8_matmul(xq, xs, self.weight_q, self.weight_scale, self.bias, _result_dtype(x))
+
+
+def freeze_fp8(module: nn.Module, min_features: int = GROUP) -> nn.Module:
+    """Replace, in place, every plain nn.Linear of `module` (recursively) whose
+    two widths are at least `min_features` with a FrozenFp8Linear of its
+    current weight: narrower layers, such as the policy heads, are not bound
+    by their weights and keep their precision. Returns the module."""
+    for name, child in list(module.named_children()):
+        if type(child) in (nn.Linear, Fp8Linear):
+            if min(child.in_features, child.out_features) >= min_features:
+                setattr(module, name, FrozenFp8Linear.from_linear(child))
+        else:
+            freeze_fp8(child, min_features)
+    return module

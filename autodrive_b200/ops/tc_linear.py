@@ -82,6 +82,9 @@ class _Status:
         key = str(device)
         e = cls._state.get(key)
         if e is None:
+            if torch.cuda.is_current_stream_capturing():
+                # a word made here would live in the graph's memory and be cleared by its replays alone
+                raise RuntimeError("make one tensor-core call on this device before capturing a graph of them")
             word = torch.zeros(1, dtype=torch.int32, device=device)
             host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
             e = {"word": word, "host": host, "event": None, "launches": 0}
@@ -117,6 +120,8 @@ class _Status:
 
     @classmethod
     def after_launch(cls, device) -> None:
+        if torch.cuda.is_current_stream_capturing():   # an event query would end the capture
+            return
         e = cls._entry(device)
         e["launches"] += 1
         if e["event"] is not None:

@@ -1,0 +1,359 @@
+"""8-bit products with a scale for each block of 128 against 64-bit arithmetic.
+
+Quantisation is exact: values and scales equal the plain implementation's bit
+for bit. A product of K columns is a sum of K exact terms; whichever order and
+whether the adders round or truncate, fp32 sums are off by at most (K + 8)
+times 2^-23 of the sum of the terms' magnitudes, to which the rounding to the
+output's type adds eps / 2 of the result.
+"""
+import pytest
+import torch
+from torch import nn
+
+from autodrive_b200.ops import fp8
+from autodrive_b200.ops.fp8 import (Fp8Linear, FrozenFp8Linear, dequantize_blocks, dequantize_rows, fp8_linear, fp8_matmul,
+                                    freeze_fp8, quantize_blocks, quantize_rows, reference_quantize_blocks,
+                                    reference_quantize_rows)
+from autodrive_b200.ops.tc_linear import TensorCoreTimeout, check_gemm_status
+
+E = 2. ** -23
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _values(rows, k, seed, dtype=torch.float32, device="cpu"):
+    g = _gen(seed)
+    x = torch.randn(rows, k, generator=g) * (.7 * torch.randn(rows, 1, generator=g)).exp()
+    return x.to(dtype).to(device)
+
+
+def _slow_e4m3():
+    """All finite e4m3 magnitudes with their bits."""
+    v = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    return v
+
+
+def test_reference_rounds_to_the_nearest_e4m3():
+    table = _slow_e4m3()
+    x = torch.cat((torch.rand(3000, generator=_gen(0), dtype=torch.float64) * 448, table, (table[1:] + table[:-1]) / 2,
+                   torch.rand(300, generator=_gen(1), dtype=torch.float64) * 2 ** -6))
+    got = fp8._round_e4m3(x)
+    dist = (x[:, None] - table).abs()
+    best = dist.amin(1)
+    assert torch.equal((x - got).abs(), best)
+    # ties go to the even code
+    tie = (dist == best[:, None]).sum(1) == 2
+    code = got.float().to(torch.float8_e4m3fn).view(torch.uint8)
+    assert tie.sum() >= 126 and (code[tie] % 2 == 0).all()
+
+
+def test_cpu_linear_and_frozen_agree_with_dequantised_products():
+    x, w = _values(6, 200, 0), _values(130, 200, 1)
+    b = torch.randn(130, generator=_gen(2))
+    x.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)
+    y = fp8_linear(x.view(2, 3, 200), w, b)
+    xd, wd = dequantize_rows(*reference_quantize_rows(x.detach())), dequantize_blocks(*reference_quantize_blocks(w.detach()))
+    want = xd.double() @ wd.double().t() + b.double()
+    assert y.shape == (2, 3, 130)
+    assert ((y.view(6, 130) - want).abs() <= 210 * E * (xd.abs().double() @ wd.abs().double().t() + b.abs())).all()
+    dy = torch.randn(6, 130, generator=_gen(3))
+    y.backward(dy.view(2, 3, 130))
+    gd = dequantize_rows(*reference_quantize_rows(dy))
+    assert torch.allclose(x.grad, gd @ wd, atol=1e-4) and torch.allclose(w.grad, dy.t() @ x.detach(), atol=1e-4)
+    assert torch.allclose(b.grad, dy.sum(0), atol=1e-5)
+    lin = Fp8Linear(200, 130)
+    with torch.no_grad():
+        lin.weight.copy_(w), lin.bias.copy_(b)
+        assert torch.equal(FrozenFp8Linear.from_linear(lin)(x), lin(x))
+
+
+def test_freeze_keeps_narrow_layers():
+    net = nn.Sequential(nn.Linear(256, 128), nn.GELU(), nn.Sequential(nn.Linear(128, 8)), Fp8Linear(300, 128))
+    freeze_fp8(net)
+    assert isinstance(net[0], FrozenFp8Linear) and isinstance(net[3], FrozenFp8Linear) and type(net[2][0]) is nn.Linear
+    assert set(net[0].state_dict()) == {"weight_q", "weight_scale", "bias"}
+
+
+def _refusals(dev):
+    xq, xs = quantize_rows(torch.randn(4, 256, device=dev))
+    wq, ws = quantize_blocks(torch.randn(130, 256, device=dev))
+    for bad in (lambda: fp8_matmul(xq.float(), xs, wq, ws), lambda: fp8_matmul(xq[:, :128], xs, wq, ws),
+                lambda: fp8_matmul(xq, xs[:, :1], wq, ws), lambda: fp8_matmul(xq, xs, wq, ws[:1]),
+                lambda: fp8_matmul(xq, xs.double(), wq, ws), lambda: fp8_matmul(xq, xs, wq, ws, torch.zeros(3, device=dev)),
+                lambda: fp8_matmul(xq, xs, wq, ws, out_dtype=torch.float64),
+                lambda: fp8_matmul(xq, xs.clone().requires_grad_(True), wq, ws),
+                lambda: quantize_rows(torch.zeros(3, 4, device=dev, dtype=torch.int32)),
+                lambda: quantize_blocks(torch.zeros(3, device=dev)), lambda: quantize_blocks(torch.zeros(3, 4, 5, device=dev)),
+                lambda: fp8_linear(torch.randn(4, 255, device=dev), torch.randn(130, 256, device=dev)),
+                lambda: FrozenFp8Linear(torch.randn(8, 256, device=dev))(torch.randn(2, 256, device=dev, requires_grad=True))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_refusals_cpu():
+    _refusals("cpu")
+
+
+@pytest.mark.gpu
+def test_refusals_gpu():
+    _refusals("cuda")
+    xq, xs = quantize_rows(torch.randn(4, 256, device="cuda"))
+    wq, ws = quantize_blocks(torch.randn(130, 256))
+    with pytest.raises(ValueError):
+        fp8_matmul(xq, xs, wq, ws)
+
+
+def _same(got, want):
+    return torch.equal(got.contiguous().view(torch.uint8), want.contiguous().view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k", [(1, 1), (1, 16), (3, 127), (5, 128), (4, 136), (7, 2008), (300, 257), (2, 16640), (1000, 64)])
+def test_quantised_rows_are_exact(dtype, rows, k):
+    x = _values(rows, k, rows + k, dtype, "cuda")
+    q, s = quantize_rows(x)
+    rq, rs = reference_quantize_rows(x)
+    assert torch.equal(s, rs) and _same(q, rq) and q.stride(0) % 16 == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k", [(1, 1), (8, 128), (128, 128), (130, 257), (1000, 2008), (3, 16640)])
+def test_quantised_blocks_are_exact(dtype, n, k):
+    w = _values(n, k, n + k, dtype, "cuda")
+    q, s, qt, st = quantize_blocks(w, transposed=True)
+    rq, rs = reference_quantize_blocks(w)
+    assert torch.equal(s, rs) and _same(q, rq) and torch.equal(st, s.t()) and _same(qt, q.t())
+    q2, s2 = quantize_blocks(w)
+    assert _same(q2, q) and torch.equal(s2, s)
+
+
+@pytest.mark.gpu
+def test_quantised_ties_and_ends_of_the_range():
+    """Quotients that lie on the middle of two e4m3 numbers, or next to it: multiples of an odd scale, and all of the
+    group's bf16 neighbours of such middles; rows near both ends of fp32; subnormal inputs; zeros."""
+    mid = (_slow_e4m3()[1:] + _slow_e4m3()[:-1]) / 2
+    rows = []
+    for amax in (448., 1., 3., 7.3, 2. ** -100, 2. ** 100, 3e38, 1e-30, 2e-38):
+        v = (mid * amax / 448).float()
+        for x in (v, torch.nextafter(v, torch.tensor(0.)), torch.nextafter(v, torch.tensor(1e38)), v.bfloat16().float()):
+            rows.append(torch.cat((torch.tensor([amax], dtype=torch.float64).float(), x, torch.zeros(1))))
+    rows.append(torch.full((128,), 1e-40))
+    rows.append(torch.zeros(128))
+    x = torch.stack(rows)
+    x[::2] *= -1
+    q, s = quantize_rows(x.cuda())
+    rq, rs = reference_quantize_rows(x)
+    assert torch.equal(s.cpu(), rs)
+    assert torch.equal(q.float().cpu(), rq.float())
+
+
+@pytest.mark.gpu
+def test_non_finite_groups_become_nan():
+    x = torch.randn(3, 300, device="cuda")
+    x[0, 5], x[1, 200], x[2, 299] = torch.nan, torch.inf, -torch.inf
+    q, s = quantize_rows(x)
+    bad = torch.zeros(3, 300, dtype=torch.bool, device="cuda")
+    bad[0, :128] = bad[1, 128:256] = bad[2, 256:] = True
+    assert torch.equal(q.float().isnan(), bad)
+    wq, ws = quantize_blocks(torch.randn(40, 300, device="cuda"))
+    assert fp8_matmul(q, s, wq, ws).isnan().all()
+
+
+@pytest.mark.gpu
+def test_strided_inputs():
+    big = torch.randn(40, 3, 520, device="cuda")
+    for x in (big[:, 1], big[:, 1, 4:300], big[..., 1:257][:, 2], big.transpose(0, 2)[..., 0], big[0, 0].expand(7, 520),
+              big.bfloat16()[:, 0, 1:130]):
+        q, s = quantize_rows(x)
+        rq, rs = reference_quantize_rows(x)
+        assert torch.equal(s, rs) and _same(q, rq)
+        q, s = quantize_blocks(x)
+        rq, rs = reference_quantize_blocks(x)
+        assert torch.equal(s, rs) and _same(q, rq)
+
+
+def _check_product(y, a, a_s, b, b_s, bias, out):
+    ad, bd = dequantize_rows(a, a_s).double(), dequantize_blocks(b, b_s).double()
+    want, size = ad @ bd.t(), ad.abs() @ bd.abs().t()
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    tol = (a.shape[1] + 8) * E * size + torch.finfo(out).eps / 2 * want.abs() + torch.finfo(out).tiny
+    assert y.dtype == out and ((y.double() - want).abs() <= tol).all(), ((y.double() - want).abs() / tol).max()
+
+
+SHAPES = [(1, 1, 1), (1, 8, 128), (3, 130, 100), (16, 128, 128), (17, 200, 264), (33, 1408, 1000), (64, 64, 2008),
+          (128, 128, 4096), (129, 257, 513), (300, 1000, 136), (1, 1408, 16640), (8, 4096, 1024), (1000, 136, 2000),
+          (2500, 1500, 640), (130, 3000, 256), (20000, 300, 384)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("out", TYPES)
+def test_product_matches_64_bits(m, n, k, out):
+    a, a_s = quantize_rows(_values(m, k, m + k, device="cuda"))
+    b, b_s = quantize_blocks(_values(n, k, n + k + 1, device="cuda") * k ** -.5)
+    bias = torch.randn(n, generator=_gen(5)).cuda() if (m + n) % 2 else None
+    with torch.no_grad():
+        y = fp8_matmul(a, a_s, b, b_s, bias, out)
+    check_gemm_status(torch.device("cuda", 0))
+    _check_product(y, a, a_s, b, b_s, bias, out)
+
+
+@pytest.mark.gpu
+def test_product_of_any_scales():
+    """Scales need not come from the quantisers: zero, negative, tiny and large ones."""
+    a, a_s = quantize_rows(_values(200, 700, 1, device="cuda"))
+    b, b_s = quantize_blocks(_values(300, 700, 2, device="cuda"))
+    a_s[::3] *= -1e6
+    a_s[:, 2] = 0.
+    b_s[1] *= 1e-6
+    _check_product(fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32), a, a_s, b, b_s, None, torch.float32)
+    _check_product(fp8_matmul(a[:3], a_s[:3], b, b_s, out_dtype=torch.float32), a[:3], a_s[:3], b, b_s, None, torch.float32)
+
+
+@pytest.mark.gpu
+def test_product_of_unaligned_and_strided_operands():
+    a, a_s = quantize_rows(_values(60, 700, 1, device="cuda"))
+    b, b_s = quantize_blocks(_values(300, 700, 2, device="cuda"))
+    want = fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32)
+    ac, bc = a.contiguous(), b.contiguous()          # 700-byte rows
+    assert ac.stride(0) == 700
+    assert torch.equal(fp8_matmul(ac, a_s, bc, b_s, out_dtype=torch.float32), want)
+    off = torch.zeros(60 * 704 + 1, dtype=torch.uint8, device="cuda")[1:].view(60, 704)
+    off[:, :700] = a.view(torch.uint8)
+    assert torch.equal(fp8_matmul(off.view(torch.float8_e4m3fn)[:, :700], a_s, b, b_s, out_dtype=torch.float32), want)
+    at = a.view(torch.uint8).t().contiguous().t().view(torch.float8_e4m3fn)
+    ast = a_s.t().contiguous().t()
+    assert torch.equal(fp8_matmul(at, ast, b, b_s, out_dtype=torch.float32), want)
+    y = fp8_matmul(a.unflatten(0, (3, 4, 5)), a_s.view(3, 4, 5, 6), b, b_s, out_dtype=torch.float32)
+    assert torch.equal(y.view(60, 300), want)
+    one = fp8_matmul(a[7], a_s[7], b, b_s, out_dtype=torch.float32)   # a vector
+    _check_product(one[None], a[7:8], a_s[7:8], b, b_s, None, torch.float32)
+
+
+@pytest.mark.gpu
+def test_empty_products():
+    for m, n, k in ((0, 5, 64), (4, 0, 64), (4, 5, 0)):
+        a, a_s = quantize_rows(torch.randn(m, k, device="cuda"))
+        b, b_s = quantize_blocks(torch.randn(n, k, device="cuda"))
+        bias = torch.arange(n, device="cuda").float()
+        y = fp8_matmul(a, a_s, b, b_s, bias)
+        assert y.shape == (m, n) and (k or torch.equal(y.float(), bias.expand(m, n)))
+
+
+@pytest.mark.gpu
+def test_results_do_not_depend_on_the_run():
+    a, a_s = quantize_rows(_values(5, 16640, 1, device="cuda"))
+    b, b_s = quantize_blocks(_values(1408, 16640, 2, device="cuda"))
+    first = fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32)
+    for _ in range(5):
+        assert torch.equal(fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(1, 64, 64), (257, 130, 200), (1024, 256, 520), (33, 1000, 127)])
+def test_linear_gradients_match_the_formula(dtype, m, n, k):
+    x = _values(m, k, 1, torch.bfloat16, "cuda").to(dtype).requires_grad_(True)
+    w = (_values(n, k, 2, device="cuda") * k ** -.5).requires_grad_(True)
+    b = torch.randn(n, generator=_gen(4)).cuda().requires_grad_(True)
+    dy = torch.randn(m, n, generator=_gen(3)).bfloat16().to(dtype).cuda()
+    y = fp8_linear(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    xq, xs = quantize_rows(x)
+    wq, ws = quantize_blocks(w)
+    _check_product(y, xq, xs, wq, ws, b.detach(), dtype)
+    gq, gs = quantize_rows(dy)
+    _check_product(dx, gq, gs, *quantize_blocks(w.detach().t().contiguous()), None, dtype)
+    # bf16 values, so the bf16 operands are exact (an fp16 x holds them but for its own rounding, 2^-11)
+    terms = dy.double().abs().t() @ x.detach().double().abs()
+    op = 2. ** -8 if dtype == torch.float16 else 0.   # fp16 values are rounded to bf16 operands
+    assert ((dw.double() - dy.double().t() @ x.detach().double()).abs() <= ((m + 8) * E + 2.1 * op) * terms).all()
+    assert ((db.double() - dy.double().sum(0)).abs() <= (m + 8) * E * dy.double().abs().sum(0)).all()
+
+
+@pytest.mark.gpu
+def test_linear_input_gradient_is_the_difference_quotient():
+    """With the group's largest value fixed at 448 the scale is 1 and e4m3 inputs are held exactly, so the layer is
+    linear in them and its differences, sums of few small integers, are exact."""
+    g = _gen(9)
+    x = torch.randint(-8, 9, (3, 128), generator=g).float()
+    w = torch.randint(-4, 5, (128, 128), generator=g).float()
+    x[:, 0], w[0, 0] = 448., 448.
+    x, w = x.cuda().requires_grad_(True), w.cuda()
+    c = torch.zeros(3, 128, device="cuda")
+    c[0, 5] = c[1, 77] = c[2, 127] = 1.
+    gx, = torch.autograd.grad(fp8_linear(x, w), x, c)
+    for i, n in ((0, 5), (1, 77), (2, 127)):
+        for j in (1, 64, 127):
+            e = torch.zeros_like(x)
+            e[i, j] = 1.
+            with torch.no_grad():
+                up, down = x.clamp(-7, 7), None
+                up[:, 0] = 448.
+                d = (fp8_linear(up + e, w) - fp8_linear(up - e, w))[i, n] / 2
+            assert d == w[n, j]
+            # the gradient 1 is held as 448 times fp32(1 / 448)
+            assert abs(gx[i, j] - w[n, j]) <= 2. ** -22 * abs(w[n, j])
+
+
+@pytest.mark.gpu
+def test_modules_under_autocast_and_frozen():
+    lin = Fp8Linear(256, 384).cuda()
+    x = torch.randn(70, 256, device="cuda")
+    with torch.autocast("cuda", dtype=torch.bfloat16), torch.no_grad():
+        y = lin(x)
+        z = FrozenFp8Linear.from_linear(lin)(x)
+    assert y.dtype == torch.bfloat16 and torch.equal(y, z)
+    state = FrozenFp8Linear.from_linear(lin).state_dict()
+    other = FrozenFp8Linear(torch.zeros(384, 256, device="cuda"), torch.zeros(384, device="cuda"))
+    other.load_state_dict(state)
+    # the fp32 input itself is quantised, inside the region as outside
+    with torch.autocast("cuda", dtype=torch.bfloat16), torch.no_grad():
+        assert torch.equal(other(x), z)
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed_on_a_side_stream():
+    lin = Fp8Linear(520, 300).cuda()
+    x = torch.randn(77, 520, device="cuda").requires_grad_(True)
+    dy = torch.randn(77, 300, device="cuda")
+
+    def step():
+        y = lin(x)
+        return (y, *torch.autograd.grad(y, (x, lin.weight, lin.bias), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.no_grad():
+        x.copy_(torch.randn_like(x))
+    graph.replay()
+    for a, b in zip(out, step()):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [300, 4])
+def test_a_wait_that_runs_out_is_reported(m):
+    dev = torch.device("cuda", 0)
+    a, a_s = quantize_rows(_values(m, 4096, 1, device="cuda"))
+    b, b_s = quantize_blocks(_values(512, 4096, 2, device="cuda"))
+    fp8_matmul(a, a_s, b, b_s)
+    check_gemm_status(dev)
+    with pytest.raises(TensorCoreTimeout):
+        fp8_matmul(a, a_s, b, b_s, wait_ns=0)
+        check_gemm_status(dev)
+    y = fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32)   # the next call is sound
+    check_gemm_status(dev)
+    _check_product(y, a, a_s, b, b_s, None, torch.float32)
