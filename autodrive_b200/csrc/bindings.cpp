@@ -10,6 +10,7 @@
 #include <string>
 #include <vector>
 
+#include "lm_host.h"
 #include "sim.h"
 
 namespace py = pybind11;
@@ -197,6 +198,7 @@ void register_layernorm_ops(py::module& m);
 void register_rmsnorm_ops(py::module& m);
 void register_fp8_quant_ops(py::module& m);
 void register_fp8_gemm_ops(py::module& m);
+void register_fp8_linear_ops(py::module& m);
 void register_token_logprobs_ops(py::module& m);
 void register_adstar_cpu(py::module& m);
 void register_sha256_ops(py::module& m);
@@ -252,6 +254,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("set_seed", &Sim::set_seed)
       .def_readwrite("threads", &Sim::threads)
       .def_property_readonly("cuda", [](const Sim& s) { return s.cuda; });
+  m.def("native_launches", [] { return lm::launch_counter().load(); },
+        "kernels launched so far by the operators that count in C++");
   register_policy_ops(m);
   register_comm_ops(m);
   register_policy_tc_ops(m);
@@ -261,6 +265,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_rmsnorm_ops(m);
   register_fp8_quant_ops(m);
   register_fp8_gemm_ops(m);
+  register_fp8_linear_ops(m);
   register_token_logprobs_ops(m);
   register_adstar_cpu(m);
   register_sha256_ops(m);

@@ -1,0 +1,32 @@
+// The 8-bit quantisers and product as C++ functions (fp8_quant.cu,
+// fp8_gemm.cu), for the linear layer that joins them (fp8_linear.cpp), and the
+// bf16 product of its weight gradient (tc_gemm.cu). Operands are checked by
+// their callers' entry points.
+#pragma once
+
+#include <torch/extension.h>
+
+#include <utility>
+#include <vector>
+
+namespace fp8 {
+
+// A matrix [rows, K] with contiguous columns -> {q, scale}.
+std::pair<torch::Tensor, torch::Tensor> quantize_rows(const torch::Tensor& x);
+// A matrix with contiguous columns -> {q, scale}, or with `transposed` {q, scale, q^T, scale^T}.
+std::vector<torch::Tensor> quantize_blocks(const torch::Tensor& w, bool transposed);
+// a b^T (+ bias, fp32 or undefined) of operands whose rows start 16 bytes apart.
+torch::Tensor matmul(const torch::Tensor& a, const torch::Tensor& a_scale, const torch::Tensor& b,
+                     const torch::Tensor& b_scale, const torch::Tensor& bias, torch::ScalarType out_dtype,
+                     const torch::Tensor& status, int64_t wait_ns);
+// `t` as a matrix with contiguous columns: a view where its layout allows one.
+torch::Tensor as_matrix(const torch::Tensor& t);
+// 1: fp32, bf16 or fp16.
+bool known_type(torch::ScalarType t);
+
+constexpr int64_t kWaitNs = 2000000000ll;
+
+}  // namespace fp8
+
+// g^T x in fp32 for bf16 g [M, N] and x [M, K] with row strides that are multiples of 8.
+torch::Tensor tc_weight_gradient(const torch::Tensor& g, const torch::Tensor& x, const torch::Tensor& status);

@@ -26,6 +26,8 @@
 
 #include <algorithm>
 
+#include "fp8.h"
+#include "lm_host.h"
 #include "lm_vec.h"
 #include "smem_opt_in.h"
 #include "tc_sm100.h"
@@ -238,14 +240,6 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
   }
 }
 
-int sm_count() {
-  int dev = 0, sms = 0;
-  TORCH_CHECK(cudaGetDevice(&dev) == cudaSuccess &&
-                  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess,
-              "fp8_matmul: device query failed");
-  return sms;
-}
-
 template <int BN>
 void launch(const CUtensorMap& ta, const CUtensorMap& tb, const Args& g, cudaStream_t st) {
   static size_t configured[dynsmem::kMaxDevices] = {};
@@ -253,60 +247,46 @@ void launch(const CUtensorMap& ta, const CUtensorMap& tb, const Args& g, cudaStr
               "fp8_matmul shared-memory attribute");
   const int64_t total = (int64_t)((g.N + BN - 1) / BN) * ((g.M + kBM - 1) / kBM);
   TORCH_CHECK(total < (1ll << 31), "fp8_matmul: too many output tiles");
-  fp8_gemm_kernel<BN><<<(int)std::min<int64_t>(total, sm_count()), kThreads, Config<BN>::smem_bytes, st>>>(ta, tb, g);
+  fp8_gemm_kernel<BN><<<(int)std::min<int64_t>(total, lm::sm_count()), kThreads, Config<BN>::smem_bytes, st>>>(ta, tb, g);
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "fp8_matmul launch failed");
 }
 
-void check_operand(const torch::Tensor& q, const torch::Tensor& a, const char* name) {
-  TORCH_CHECK(q.is_cuda() && q.device() == a.device(), "fp8_matmul: ", name, " must be on a's device");
-  TORCH_CHECK(q.scalar_type() == torch::kFloat8_e4m3fn && q.dim() == 2, "fp8_matmul: ", name, " must be an e4m3 matrix");
-  TORCH_CHECK(q.numel() == 0 || q.size(1) == 1 || q.stride(1) == 1, "fp8_matmul: ", name, "'s columns must be contiguous");
-  TORCH_CHECK((q.size(0) <= 1 || q.size(1) == 0 || (q.stride(0) % 16 == 0 && q.stride(0) >= q.size(1))) &&
-                  reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
-              "fp8_matmul: ", name, "'s rows must start 16 bytes apart");
-  TORCH_CHECK(q.size(0) < (1ll << 30) && q.size(1) < (1ll << 30), "fp8_matmul: ", name, " is too large");
+// `q` as the TMA unit reads it: rows that start 16 bytes apart on a 16-byte
+// aligned base (a copy only where they do not).
+torch::Tensor operand(const torch::Tensor& q) {
+  const int64_t rows = q.size(0), k = q.size(1);
+  const bool ok = (k <= 1 || q.stride(1) == 1) && (rows <= 1 || (q.stride(0) % 16 == 0 && q.stride(0) >= k)) &&
+                  reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0;
+  if (ok || q.numel() == 0) return q;
+  auto buf = torch::empty({rows, (k + 15) / 16 * 16}, q.options()).narrow(1, 0, k);
+  buf.view(torch::kUInt8).copy_(q.view(torch::kUInt8));
+  return buf;
 }
 
-void check_scale(const torch::Tensor& s, const torch::Tensor& a, int64_t rows, int64_t groups, const char* name) {
-  TORCH_CHECK(s.is_cuda() && s.device() == a.device() && s.scalar_type() == torch::kFloat32 && s.dim() == 2 &&
-                  s.size(0) == rows && s.size(1) == groups && s.is_contiguous(),
-              "fp8_matmul: ", name, " must be a contiguous fp32 [", rows, ", ", groups, "] on a's device");
-}
+}  // namespace
 
-torch::Tensor fp8_matmul(torch::Tensor a, torch::Tensor a_scale, torch::Tensor b, torch::Tensor b_scale,
-                         c10::optional<torch::Tensor> bias, torch::ScalarType out_dtype, torch::Tensor status,
-                         int64_t wait_ns) {
-  check_operand(a, a, "a");
-  check_operand(b, a, "b");
-  const int64_t M = a.size(0), K = a.size(1), N = b.size(0);
-  TORCH_CHECK(b.size(1) == K, "fp8_matmul: inner dimensions differ");
-  const int64_t groups = (K + kGroup - 1) / kGroup;
-  check_scale(a_scale, a, M, groups, "a_scale");
-  check_scale(b_scale, a, (N + kGroup - 1) / kGroup, groups, "b_scale");
-  TORCH_CHECK(out_dtype == torch::kFloat32 || out_dtype == torch::kBFloat16 || out_dtype == torch::kHalf,
-              "fp8_matmul: the result is fp32, bf16 or fp16");
-  TORCH_CHECK(status.is_cuda() && status.device() == a.device() && status.scalar_type() == torch::kInt32,
-              "fp8_matmul: status must be int32 on a's device");
-  TORCH_CHECK(wait_ns >= 0, "wait_ns must be non-negative");
-  if (bias)
-    TORCH_CHECK(bias->is_cuda() && bias->device() == a.device() && bias->scalar_type() == torch::kFloat32 &&
-                    bias->dim() == 1 && bias->size(0) == N && bias->is_contiguous(),
-                "fp8_matmul: bias must be a contiguous fp32 [", N, "] on a's device");
+namespace fp8 {
+
+torch::Tensor matmul(const torch::Tensor& a, const torch::Tensor& a_scale, const torch::Tensor& b,
+                     const torch::Tensor& b_scale, const torch::Tensor& bias, torch::ScalarType out_dtype,
+                     const torch::Tensor& status, int64_t wait_ns) {
   const c10::cuda::CUDAGuard guard(a.device());
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(0);
   auto c = torch::empty({M, N}, a.options().dtype(out_dtype));
   if (M == 0 || N == 0) return c;
   if (K == 0) {
     c.zero_();
-    if (bias) c += *bias;
+    if (bias.defined()) c.add_(bias);
     return c;
   }
+  LM_CHECK_VALUE(M < (1ll << 30) && N < (1ll << 30) && K < (1ll << 30), "fp8_matmul: too large");
   Args g{};
   g.M = (int)M;
   g.N = (int)N;
-  g.groups = (int)groups;
+  g.groups = (int)((K + kGroup - 1) / kGroup);
   g.a_scale = a_scale.data_ptr<float>();
   g.b_scale = b_scale.data_ptr<float>();
-  g.bias = bias ? bias->data_ptr<float>() : nullptr;
+  g.bias = bias.defined() ? bias.data_ptr<float>() : nullptr;
   g.c = c.data_ptr();
   g.ldc = N;
   g.out_kind = out_dtype == torch::kFloat32 ? 0 : (out_dtype == torch::kBFloat16 ? 1 : 2);
@@ -317,19 +297,54 @@ torch::Tensor fp8_matmul(torch::Tensor a, torch::Tensor a_scale, torch::Tensor b
   const CUtensorMap ta = tma::u8_sw128(a.data_ptr(), M, K, M > 1 ? a.stride(0) : one_row, kBM);
   const CUtensorMap tb = tma::u8_sw128(b.data_ptr(), N, K, N > 1 ? b.stride(0) : one_row, BN);
   launch<BN>(ta, tb, g, c10::cuda::getCurrentCUDAStream().stream());
+  lm::count_launches(1);
   return c;
+}
+
+}  // namespace fp8
+
+namespace {
+
+torch::Tensor fp8_matmul(torch::Tensor a, torch::Tensor a_scale, torch::Tensor b, torch::Tensor b_scale,
+                         c10::optional<torch::Tensor> bias, py::object dtype, torch::Tensor status, int64_t wait_ns) {
+  const auto out_dtype = torch::python::detail::py_object_to_dtype(dtype);
+  LM_CHECK_VALUE(a.is_cuda() && a.scalar_type() == torch::kFloat8_e4m3fn && a.dim() >= 1 &&
+                        b.scalar_type() == torch::kFloat8_e4m3fn && b.dim() == 2,
+                    "fp8_matmul takes e4m3 rows [..., K] and an e4m3 matrix [N, K]");
+  const int64_t K = a.size(-1), N = b.size(0), groups = (K + kGroup - 1) / kGroup;
+  LM_CHECK_VALUE(b.size(1) == K, "fp8_matmul: a has ", K, " columns and b ", b.size(1));
+  auto want = a.sizes().vec();
+  want.back() = groups;
+  LM_CHECK_VALUE(a_scale.sizes() == c10::IntArrayRef(want) && b_scale.dim() == 2 &&
+                        b_scale.size(0) == (N + kGroup - 1) / kGroup && b_scale.size(1) == groups,
+                    "fp8_matmul needs scales ", c10::IntArrayRef(want), " and [", (N + kGroup - 1) / kGroup, ", ", groups,
+                    "], not ", a_scale.sizes(), " and ", b_scale.sizes());
+  LM_CHECK_VALUE(a_scale.scalar_type() == torch::kFloat32 && b_scale.scalar_type() == torch::kFloat32,
+                    "fp8_matmul needs fp32 scales");
+  LM_CHECK_VALUE(!bias || (bias->dim() == 1 && bias->size(0) == N && fp8::known_type(bias->scalar_type())),
+                    "fp8_matmul needs a bias [", N, "]");
+  LM_CHECK_VALUE(fp8::known_type(out_dtype), "fp8_matmul gives fp32, bf16 or fp16");
+  for (const auto* t : {&a_scale, &b, &b_scale, &status})
+    LM_CHECK_VALUE(t->device() == a.device(), "fp8_matmul needs all of its tensors on one device");
+  LM_CHECK_VALUE(!bias || bias->device() == a.device(), "fp8_matmul needs all of its tensors on one device");
+  TORCH_CHECK(status.scalar_type() == torch::kInt32, "fp8_matmul: status must be int32");
+  LM_CHECK_VALUE(wait_ns >= 0, "wait_ns must not be negative");
+  LM_CHECK_VALUE(!(at::GradMode::is_enabled() &&
+                      (a_scale.requires_grad() || b_scale.requires_grad() || (bias && bias->requires_grad()))),
+                    "fp8_matmul has no gradient: use fp8_linear, or call it under torch.no_grad()");
+  const int64_t rows = c10::multiply_integers(a.sizes().slice(0, a.dim() - 1));
+  const auto a2 = a.dim() == 2 ? a : a.reshape({rows, K});
+  const auto s2 = a_scale.dim() == 2 ? a_scale : a_scale.reshape({rows, groups});
+  torch::Tensor bf;
+  if (bias) bf = (bias->scalar_type() == torch::kFloat32 ? *bias : bias->to(torch::kFloat32)).contiguous();
+  const auto y = fp8::matmul(operand(a2), s2.contiguous(), operand(b), b_scale.contiguous(), bf, out_dtype, status, wait_ns);
+  return a.dim() == 2 ? y : lm::from_rows(y, a);
 }
 
 }  // namespace
 
 void register_fp8_gemm_ops(py::module& m) {
-  m.def("fp8_matmul",
-        [](torch::Tensor a, torch::Tensor a_scale, torch::Tensor b, torch::Tensor b_scale,
-           c10::optional<torch::Tensor> bias, py::object out_dtype, torch::Tensor status, int64_t wait_ns) {
-          return fp8_matmul(a, a_scale, b, b_scale, bias, torch::python::detail::py_object_to_dtype(out_dtype), status,
-                            wait_ns);
-        },
-        "e4m3 x e4m3 product with a scale for each block of 128 (+ bias): fp32, bf16 or fp16",
+  m.def("fp8_matmul", &fp8_matmul, "e4m3 x e4m3 product with a scale for each block of 128 (+ bias): fp32, bf16 or fp16",
         py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"), py::arg("bias"), py::arg("out_dtype"),
-        py::arg("status"), py::arg("wait_ns") = 2000000000ll);
+        py::arg("status"), py::arg("wait_ns") = fp8::kWaitNs);
 }

@@ -1,0 +1,115 @@
+// Linear layer with both operands in 8 bits, for training:
+//
+//   y  = Q(x) Q(w)^T + b      Q: e4m3 with scales for blocks of 128
+//   dx = Q(dy) Q(w)           rounding counts as the identity
+//   dw = dy^T x               bf16 operands, fp32 sums
+//   db = sum of dy's rows     in fp32
+//
+// One call runs the quantisers and the product, and one backward its four
+// kernels, so that no Python runs between the launches.
+#include <torch/extension.h>
+#include <c10/core/DeviceGuard.h>
+
+#include <algorithm>
+
+#include "fp8.h"
+#include "lm_host.h"
+
+namespace py = pybind11;
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// `x` [M, K] as a bf16 operand of the weight gradient: columns a multiple of 8, zeros behind the last.
+torch::Tensor bf16_operand(const torch::Tensor& x) {
+  const int64_t k = x.size(1), kp = (k + 7) / 8 * 8;
+  if (k == kp) {
+    const auto y = x.to(torch::kBFloat16).contiguous();
+    return reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 == 0 ? y : y.clone();
+  }
+  auto y = torch::empty({x.size(0), kp}, x.options().dtype(torch::kBFloat16));
+  y.narrow(1, k, kp - k).zero_();
+  y.narrow(1, 0, k).copy_(x);
+  return y;
+}
+
+struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& weight,
+                               const c10::optional<torch::Tensor>& bias_, int64_t out_dtype, const torch::Tensor& status) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::DeviceGuard guard(x.device());
+    const torch::Tensor bias = bias_ ? *bias_ : torch::Tensor();
+    const auto x2 = fp8::as_matrix(x);
+    const bool need_x = x.requires_grad(), need_w = weight.requires_grad();
+    const auto xq = fp8::quantize_rows(x2);
+    // the input gradient reads the weight down its columns: its transposed copy is written by the same pass
+    const auto wq = fp8::quantize_blocks(fp8::as_matrix(weight), need_x);
+    torch::Tensor b;
+    if (bias.defined()) b = bias.to(torch::kFloat32).contiguous();
+    const auto y = fp8::matmul(xq.first, xq.second, wq[0], wq[1], b, static_cast<torch::ScalarType>(out_dtype), status,
+                               fp8::kWaitNs);
+    torch::Tensor keep;   // what the weight gradient reads: the caller's x where it can be read as it is
+    if (need_w) keep = x2.scalar_type() == torch::kBFloat16 && x2.is_alias_of(x) ? x : x2.to(torch::kBFloat16);
+    ctx->save_for_backward({keep, need_x ? wq[2] : torch::Tensor(), need_x ? wq[3] : torch::Tensor(), status});
+    ctx->saved_data["x_sizes"] = x.sizes().vec();
+    ctx->saved_data["n"] = weight.size(0);
+    ctx->saved_data["x_type"] = static_cast<int64_t>(x.scalar_type());
+    ctx->saved_data["w_type"] = static_cast<int64_t>(weight.scalar_type());
+    ctx->saved_data["b_type"] = bias.defined() ? static_cast<int64_t>(bias.scalar_type()) : -1;
+    auto sizes = x.sizes().vec();
+    sizes.back() = weight.size(0);
+    return y.view(sizes);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "fp8_linear has no second derivative (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const auto x_sizes = ctx->saved_data["x_sizes"].toIntVector();
+    const int64_t n = ctx->saved_data["n"].toInt(), k = x_sizes.back();
+    const c10::DeviceGuard guard(grads[0].device());
+    const auto g = fp8::as_matrix(grads[0]);
+    const auto& status = saved[3];
+    variable_list out(5);
+    if (ctx->needs_input_grad(0)) {
+      const auto gq = fp8::quantize_rows(g);
+      out[0] = fp8::matmul(gq.first, gq.second, saved[1], saved[2], {},
+                           static_cast<torch::ScalarType>(ctx->saved_data["x_type"].toInt()), status, fp8::kWaitNs)
+                   .view(x_sizes);
+    }
+    if (ctx->needs_input_grad(1)) {
+      auto dw = tc_weight_gradient(bf16_operand(g), bf16_operand(fp8::as_matrix(saved[0])), status);
+      if (dw.size(0) != n || dw.size(1) != k) dw = dw.narrow(0, 0, n).narrow(1, 0, k);
+      out[1] = dw.to(static_cast<torch::ScalarType>(ctx->saved_data["w_type"].toInt()));
+    }
+    const int64_t b_type = ctx->saved_data["b_type"].toInt();
+    if (b_type >= 0 && ctx->needs_input_grad(2))
+      out[2] = g.sum(0, false, torch::kFloat32).to(static_cast<torch::ScalarType>(b_type));
+    return out;
+  }
+};
+
+torch::Tensor fp8_linear(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> bias, py::object dtype,
+                         torch::Tensor status) {
+  LM_CHECK_VALUE(x.is_cuda() && fp8::known_type(x.scalar_type()) && x.dim() >= 1 &&
+                        fp8::known_type(weight.scalar_type()) && weight.dim() == 2,
+                    "fp8_linear takes fp32, bf16 or fp16 rows [..., K] and a weight [N, K]");
+  LM_CHECK_VALUE(x.size(-1) == weight.size(1) &&
+                        (!bias || (bias->dim() == 1 && bias->size(0) == weight.size(0) &&
+                                   fp8::known_type(bias->scalar_type()))),
+                    "fp8_linear: x ", x.sizes(), ", weight ", weight.sizes(), " and bias do not fit");
+  LM_CHECK_VALUE(weight.device() == x.device() && status.device() == x.device() &&
+                        (!bias || bias->device() == x.device()),
+                    "fp8_linear needs all of its tensors on one device");
+  TORCH_CHECK(status.scalar_type() == torch::kInt32, "fp8_linear: status must be int32");
+  return Fp8LinearFn::apply(x, weight, bias,
+                            static_cast<int64_t>(torch::python::detail::py_object_to_dtype(dtype)), status);
+}
+
+}  // namespace
+
+void register_fp8_linear_ops(py::module& m) {
+  m.def("fp8_linear", &fp8_linear, "linear layer with both operands quantised to e4m3, with autograd", py::arg("x"),
+        py::arg("weight"), py::arg("bias"), py::arg("out_dtype"), py::arg("status"));
+}

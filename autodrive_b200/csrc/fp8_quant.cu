@@ -15,6 +15,8 @@
 #include <algorithm>
 #include <vector>
 
+#include "fp8.h"
+#include "lm_host.h"
 #include "lm_vec.h"
 
 namespace py = pybind11;
@@ -133,10 +135,6 @@ quant_blocks_kernel(const T* __restrict__ w, int64_t ldw, uint8_t* __restrict__ 
   }
 }
 
-bool known_type(torch::ScalarType t) {
-  return t == torch::kFloat32 || t == torch::kBFloat16 || t == torch::kHalf;
-}
-
 template <typename F>
 void for_type(torch::ScalarType t, F&& f) {
   if (t == torch::kFloat32) f(float{});
@@ -144,20 +142,35 @@ void for_type(torch::ScalarType t, F&& f) {
   else f(__half{});
 }
 
-void check_matrix(const torch::Tensor& x, const char* what) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && known_type(x.scalar_type()), what,
-              ": needs a CUDA fp32, bf16 or fp16 matrix");
-  TORCH_CHECK(x.numel() == 0 || x.size(1) == 1 || x.stride(1) == 1, what, ": columns must be contiguous");
-  TORCH_CHECK(x.size(1) < (1ll << 31) - 256, what, ": too many columns");
-}
-
 // e4m3 [rows][cols] whose rows start 16 bytes apart, as the TMA unit reads them.
 torch::Tensor empty_q(int64_t rows, int64_t cols, const torch::Tensor& like) {
-  return torch::empty({rows, (cols + 15) / 16 * 16}, like.options().dtype(torch::kFloat8_e4m3fn)).narrow(1, 0, cols);
+  const int64_t ld = (cols + 15) / 16 * 16;
+  auto q = torch::empty({rows, ld}, like.options().dtype(torch::kFloat8_e4m3fn));
+  return ld == cols ? q : q.narrow(1, 0, cols);
 }
 
-std::vector<torch::Tensor> quantize_rows(torch::Tensor x) {
-  check_matrix(x, "quantize_rows");
+void check_input(const torch::Tensor& x, int64_t dims, const char* what) {
+  LM_CHECK_VALUE(x.is_cuda() && fp8::known_type(x.scalar_type()) && x.dim() >= dims, what,
+                    " takes fp32, bf16 or fp16 tensors of at least ", dims, " dimension(s)");
+  LM_CHECK_VALUE(x.size(-1) < (1ll << 30), what, ": too many columns");
+}
+
+}  // namespace
+
+namespace fp8 {
+
+bool known_type(torch::ScalarType t) {
+  return t == torch::kFloat32 || t == torch::kBFloat16 || t == torch::kHalf;
+}
+
+torch::Tensor as_matrix(const torch::Tensor& t) {
+  const int64_t k = t.size(-1);
+  const auto y = t.dim() == 2 ? t : t.reshape({c10::multiply_integers(t.sizes().slice(0, t.dim() - 1)), k});
+  const bool ok = y.numel() == 0 || ((k == 1 || y.stride(1) == 1) && (y.size(0) == 1 || y.stride(0) >= k));
+  return ok ? y : y.contiguous();
+}
+
+std::pair<torch::Tensor, torch::Tensor> quantize_rows(const torch::Tensor& x) {
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t rows = x.size(0), k = x.size(1), groups = (k + 127) / 128;
   auto q = empty_q(rows, k, x);
@@ -165,29 +178,24 @@ std::vector<torch::Tensor> quantize_rows(torch::Tensor x) {
   if (rows == 0 || k == 0) return {q, scale};
   const int64_t ldx = rows > 1 ? x.stride(0) : k;
   const bool vec = k % 8 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
-  int dev = 0, sms = 0;
-  TORCH_CHECK(cudaGetDevice(&dev) == cudaSuccess &&
-              cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess,
-              "quantize_rows: device query failed");
-  const int grid = (int)std::min<int64_t>((rows * groups + 15) / 16, (int64_t)sms * 32);
+  const int grid = (int)std::min<int64_t>((rows * groups + 15) / 16, (int64_t)lm::sm_count() * 32);
   auto st = c10::cuda::getCurrentCUDAStream().stream();
   for_type(x.scalar_type(), [&](auto t) {
     using T = decltype(t);
     auto* out = reinterpret_cast<uint8_t*>(q.data_ptr());
     const T* in = reinterpret_cast<const T*>(x.data_ptr());
-    if (vec) quant_rows_kernel<T, true><<<grid, 256, 0, st>>>(in, ldx, out, q.stride(0), scale.data_ptr<float>(), rows, (int)k, (int)groups);
-    else quant_rows_kernel<T, false><<<grid, 256, 0, st>>>(in, ldx, out, q.stride(0), scale.data_ptr<float>(), rows, (int)k, (int)groups);
+    const auto kernel = vec ? quant_rows_kernel<T, true> : quant_rows_kernel<T, false>;
+    kernel<<<grid, 256, 0, st>>>(in, ldx, out, q.stride(0), scale.data_ptr<float>(), rows, (int)k, (int)groups);
   });
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "quantize_rows launch failed");
+  lm::count_launches(1);
   return {q, scale};
 }
 
-// {q, scale} or, with `transposed`, {q, scale, q^T, scale^T}.
-std::vector<torch::Tensor> quantize_blocks(torch::Tensor w, bool transposed) {
-  check_matrix(w, "quantize_blocks");
+std::vector<torch::Tensor> quantize_blocks(const torch::Tensor& w, bool transposed) {
   const c10::cuda::CUDAGuard guard(w.device());
   const int64_t n = w.size(0), k = w.size(1), bn = (n + 127) / 128, bk = (k + 127) / 128;
-  TORCH_CHECK(n < (1ll << 23), "quantize_blocks: too many rows");   // grid.y holds n / 128
+  LM_CHECK_VALUE(n < (1ll << 22), "quantize_blocks: too many rows");   // grid.y holds n / 128
   auto q = empty_q(n, k, w);
   auto scale = torch::empty({bn, bk}, w.options().dtype(torch::kFloat32));
   std::vector<torch::Tensor> out = {q, scale};
@@ -206,14 +214,26 @@ std::vector<torch::Tensor> quantize_blocks(torch::Tensor w, bool transposed) {
         (int)n, (int)k);
   });
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "quantize_blocks launch failed");
+  lm::count_launches(1);
   return out;
 }
 
-}  // namespace
+}  // namespace fp8
 
 void register_fp8_quant_ops(py::module& m) {
-  m.def("quantize_rows", &quantize_rows, "e4m3 rows with a scale for each 128 columns: q, scale", py::arg("x"));
-  m.def("quantize_blocks", &quantize_blocks,
-        "e4m3 matrix with a scale for each 128 x 128 block: q, scale (and their transposes)", py::arg("w"),
-        py::arg("transposed"));
+  m.def("quantize_rows",
+        [](torch::Tensor x) {
+          check_input(x, 1, "quantize_rows");
+          const auto r = fp8::quantize_rows(fp8::as_matrix(x.detach()));
+          return py::make_tuple(lm::from_rows(r.first, x), lm::from_rows(r.second, x));
+        },
+        "e4m3 rows with a scale for each 128 columns: (q, scale)", py::arg("x"));
+  m.def("quantize_blocks",
+        [](torch::Tensor w, bool transposed) {
+          check_input(w, 2, "quantize_blocks");
+          LM_CHECK_VALUE(w.dim() == 2, "quantize_blocks takes a matrix");
+          return py::tuple(py::cast(fp8::quantize_blocks(fp8::as_matrix(w.detach()), transposed)));
+        },
+        "e4m3 matrix with a scale for each 128 x 128 block: (q, scale), with its transpose (q, scale, q^T, scale^T)",
+        py::arg("w"), py::arg("transposed"));
 }

@@ -23,8 +23,10 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
+#include "lm_host.h"
 #include "lm_vec.h"
 
 namespace py = pybind11;
@@ -279,19 +281,11 @@ __global__ void __launch_bounds__(1024) rms_dw_kernel(const float* part, int par
   if (threadIdx.x == 0 && col < d) dw[col] = lm::from_f<W>(s);
 }
 
-int sm_count() {
-  int dev = 0, sms = 0;
-  TORCH_CHECK(cudaGetDevice(&dev) == cudaSuccess &&
-                  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess,
-              "rms_norm: device query failed");
-  return sms;
-}
-
 // Persistent CTAs: as many as fit on the SMs at once (2048 threads each).
 int grid_for(int64_t rows, int tpr) {
   const int rpb = rows_per_cta(tpr), threads = tpr * rpb;
   const int64_t want = (rows + rpb - 1) / rpb;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)sm_count() * std::max(1, 1024 / threads)));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)lm::sm_count() * std::max(1, 1024 / threads)));
 }
 
 // Threads and 256-column chunks per row (see the file's comment).
@@ -321,113 +315,112 @@ bool known_type(torch::ScalarType t) {
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-void check_rows(const torch::Tensor& t, const torch::Tensor& x, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.device() == x.device(), "rms_norm: ", name, " must be on x's device");
-  TORCH_CHECK(t.scalar_type() == x.scalar_type(), "rms_norm: ", name, " must have x's dtype");
-  TORCH_CHECK(t.dim() == 2 && t.sizes() == x.sizes(), "rms_norm: ", name, " must have x's shape");
-  TORCH_CHECK(t.numel() == 0 || t.size(1) == 1 || t.stride(1) == 1, "rms_norm: ", name, "'s columns must be contiguous");
+// `t` as rows of x's width: a view where its layout allows one.
+torch::Tensor as_rows(const torch::Tensor& t) {
+  const int64_t d = t.size(-1);
+  torch::Tensor y = t.dim() == 2 ? t : t.reshape({t.numel() / d, d});
+  const bool ok = y.numel() == 0 || ((d == 1 || y.stride(1) == 1) && (y.size(0) == 1 || y.stride(0) >= d));
+  return ok ? y : y.contiguous();
 }
 
-WeightPtr check_weight(const torch::Tensor& w, const torch::Tensor& x) {
-  TORCH_CHECK(w.is_cuda() && w.device() == x.device(), "rms_norm: weight must be on x's device");
-  TORCH_CHECK(known_type(w.scalar_type()) && w.dim() == 1 && w.size(0) == x.size(1) && w.is_contiguous(),
-              "rms_norm: weight must be a contiguous fp32, bf16 or fp16 [D]");
-  const int kind = w.scalar_type() == torch::kFloat32 ? 0 : (w.scalar_type() == torch::kBFloat16 ? 1 : 2);
-  return WeightPtr{w.data_ptr(), kind};
+void check_args(const torch::Tensor& x, const torch::Tensor& weight, const c10::optional<torch::Tensor>& residual) {
+  LM_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && known_type(x.scalar_type()),
+                    "rms_norm takes fp32, bf16 or fp16 rows");
+  const int64_t d = x.size(-1);
+  LM_CHECK_VALUE(d >= 1 && d <= kMaxWidth, "rms_norm rows are 1 to ", kMaxWidth, " wide, not ", d);
+  LM_CHECK_VALUE(weight.dim() == 1 && weight.size(0) == d && known_type(weight.scalar_type()) &&
+                        weight.device() == x.device(),
+                    "rms_norm needs an fp32, bf16 or fp16 weight [", d, "] on ", x.device());
+  if (residual)
+    LM_CHECK_VALUE(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type() &&
+                          residual->device() == x.device(),
+                      "rms_norm needs a residual of x's shape, dtype and device");
 }
 
-void check_x(const torch::Tensor& x) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && known_type(x.scalar_type()),
-              "rms_norm: x must be a CUDA fp32, bf16 or fp16 [rows, D] tensor");
-  TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= kMaxWidth, "rms_norm: D must be in 1..", kMaxWidth);
+WeightPtr weight_ptr(const torch::Tensor& w) {
+  return WeightPtr{w.data_ptr(), w.scalar_type() == torch::kFloat32 ? 0 : (w.scalar_type() == torch::kBFloat16 ? 1 : 2)};
 }
 
-// Returns {y or q, h or undefined, rstd or undefined, scale or undefined}.
-std::vector<c10::optional<torch::Tensor>> rms_norm_fwd(torch::Tensor x, c10::optional<torch::Tensor> residual,
-                                                       torch::Tensor weight, double eps, bool fp8, bool keep_rstd) {
-  check_x(x);
-  check_rows(x, x, "x");
+struct Forward {
+  torch::Tensor y, h, rstd, q, scale;   // undefined where not asked for
+};
+
+// x [rows, D] and the residual are rows as as_rows() gives them; a contiguous weight.
+Forward forward(const torch::Tensor& x, const torch::Tensor& residual, const torch::Tensor& weight, double eps, bool fp8,
+                bool keep_rstd) {
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t rows = x.size(0), d = x.size(1);
+  Forward out;
   FwdArgs a{};
   a.x = x.data_ptr();
   a.rows = rows;
   a.d = (int)d;
   a.ldx = rows > 1 ? x.stride(0) : d;
-  a.w = check_weight(weight, x);
+  a.w = weight_ptr(weight);
   a.eps = (float)eps;
   a.groups = (int)((d + 127) / 128);
-  c10::optional<torch::Tensor> out, h, rstd, scale;
   bool vec = d % 8 == 0 && a.ldx % 8 == 0 && aligned(a.x);
-  if (residual) {
-    check_rows(*residual, x, "residual");
-    a.res = residual->data_ptr();
-    a.ldres = rows > 1 ? residual->stride(0) : d;
-    h = torch::empty({rows, d}, x.options());
-    a.h = h->data_ptr();
+  if (residual.defined()) {
+    a.res = residual.data_ptr();
+    a.ldres = rows > 1 ? residual.stride(0) : d;
+    out.h = torch::empty({rows, d}, x.options());
+    a.h = out.h.data_ptr();
     vec = vec && a.ldres % 8 == 0 && aligned(a.res);
   }
   if (keep_rstd) {
-    rstd = torch::empty({rows}, x.options().dtype(torch::kFloat32));
-    a.rstd = rstd->data_ptr<float>();
+    out.rstd = torch::empty({rows}, x.options().dtype(torch::kFloat32));
+    a.rstd = out.rstd.data_ptr<float>();
   }
   if (fp8) {
     a.ldq = (d + 15) / 16 * 16;
-    out = torch::empty({rows, a.ldq}, x.options().dtype(torch::kFloat8_e4m3fn)).narrow(1, 0, d);
-    scale = torch::empty({rows, (int64_t)a.groups}, x.options().dtype(torch::kFloat32));
-    a.q = reinterpret_cast<uint8_t*>(out->data_ptr());
-    a.scale = scale->data_ptr<float>();
+    out.q = torch::empty({rows, a.ldq}, x.options().dtype(torch::kFloat8_e4m3fn));
+    if (a.ldq != d) out.q = out.q.narrow(1, 0, d);
+    out.scale = torch::empty({rows, (int64_t)a.groups}, x.options().dtype(torch::kFloat32));
+    a.q = reinterpret_cast<uint8_t*>(out.q.data_ptr());
+    a.scale = out.scale.data_ptr<float>();
   } else {
-    out = torch::empty({rows, d}, x.options());
-    a.y = out->data_ptr();
+    out.y = torch::empty({rows, d}, x.options());
+    a.y = out.y.data_ptr();
   }
-  if (rows > 0) {
-    auto st = c10::cuda::getCurrentCUDAStream().stream();
-    for_type(x.scalar_type(), [&](auto t) {
-      using T = decltype(t);
-      for_width(d, [&](auto tpr, auto nv) {
-        constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
-        const int grid = grid_for(rows, TPR), threads = TPR * rows_per_cta(TPR);
-        if (vec && fp8) rms_fwd_kernel<T, true, true, TPR, NV><<<grid, threads, 0, st>>>(a);
-        else if (vec) rms_fwd_kernel<T, true, false, TPR, NV><<<grid, threads, 0, st>>>(a);
-        else if (fp8) rms_fwd_kernel<T, false, true, TPR, NV><<<grid, threads, 0, st>>>(a);
-        else rms_fwd_kernel<T, false, false, TPR, NV><<<grid, threads, 0, st>>>(a);
-      });
+  if (rows == 0) return out;
+  auto st = c10::cuda::getCurrentCUDAStream().stream();
+  for_type(x.scalar_type(), [&](auto t) {
+    using T = decltype(t);
+    for_width(d, [&](auto tpr, auto nv) {
+      constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
+      const int grid = grid_for(rows, TPR), threads = TPR * rows_per_cta(TPR);
+      if (vec && fp8) rms_fwd_kernel<T, true, true, TPR, NV><<<grid, threads, 0, st>>>(a);
+      else if (vec) rms_fwd_kernel<T, true, false, TPR, NV><<<grid, threads, 0, st>>>(a);
+      else if (fp8) rms_fwd_kernel<T, false, true, TPR, NV><<<grid, threads, 0, st>>>(a);
+      else rms_fwd_kernel<T, false, false, TPR, NV><<<grid, threads, 0, st>>>(a);
     });
-    TORCH_CHECK(cudaGetLastError() == cudaSuccess, "rms_norm forward launch failed");
-  }
-  return {out, h, rstd, scale};
+  });
+  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "rms_norm forward launch failed");
+  lm::count_launches(1);
+  return out;
 }
 
-// Returns {dx, dweight}.
-std::vector<torch::Tensor> rms_norm_bwd(torch::Tensor dy, c10::optional<torch::Tensor> dh, torch::Tensor h,
-                                        torch::Tensor weight, torch::Tensor rstd) {
-  check_x(h);
-  check_rows(h, h, "h");
-  check_rows(dy, h, "dy");
-  TORCH_CHECK(dy.is_contiguous(), "rms_norm: dy must be contiguous");
-  TORCH_CHECK(rstd.is_cuda() && rstd.device() == h.device() && rstd.scalar_type() == torch::kFloat32 &&
-                  rstd.numel() == h.size(0) && rstd.is_contiguous(), "rms_norm: rstd must be fp32 [rows]");
+// {dx, dweight} of contiguous gradients; an undefined dh is zero.
+std::pair<torch::Tensor, torch::Tensor> backward(const torch::Tensor& dy, const torch::Tensor& dh, const torch::Tensor& h,
+                                                 const torch::Tensor& weight, const torch::Tensor& rstd) {
   const c10::cuda::CUDAGuard guard(h.device());
   const int64_t rows = h.size(0), d = h.size(1);
+  auto dx = torch::empty({rows, d}, h.options());
+  auto dw = rows > 0 ? torch::empty_like(weight) : torch::zeros_like(weight);
+  if (rows == 0) return {dx, dw};
   BwdArgs a{};
   a.dy = dy.data_ptr();
   a.h = h.data_ptr();
-  a.w = check_weight(weight, h);
+  a.w = weight_ptr(weight);
   a.rstd = rstd.data_ptr<float>();
   a.rows = rows;
   a.ldh = rows > 1 ? h.stride(0) : d;
   a.d = (int)d;
   bool vec = d % 8 == 0 && a.ldh % 8 == 0 && aligned(a.h) && aligned(a.dy);
-  if (dh) {
-    check_rows(*dh, h, "dh");
-    TORCH_CHECK(dh->is_contiguous(), "rms_norm: dh must be contiguous");
-    a.dh_out = dh->data_ptr();
+  if (dh.defined()) {
+    a.dh_out = dh.data_ptr();
     vec = vec && aligned(a.dh_out);
   }
-  auto dx = torch::empty({rows, d}, h.options());
-  auto dw = rows > 0 ? torch::empty_like(weight) : torch::zeros_like(weight);
-  if (rows == 0) return {dx, dw};
   a.dx = dx.data_ptr();
   auto st = c10::cuda::getCurrentCUDAStream().stream();
   torch::Tensor part;
@@ -451,16 +444,86 @@ std::vector<torch::Tensor> rms_norm_bwd(torch::Tensor dy, c10::optional<torch::T
                                                                   reinterpret_cast<W*>(dw.data_ptr()));
   });
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "rms_norm weight gradient launch failed");
+  lm::count_launches(2);
   return {dx, dw};
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct RmsNormFn : torch::autograd::Function<RmsNormFn> {
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& weight,
+                               const c10::optional<torch::Tensor>& res, double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const torch::Tensor residual = res ? *res : torch::Tensor();
+    const auto x2 = as_rows(x), w = weight.contiguous();
+    const Forward f = ::forward(x2, residual.defined() ? as_rows(residual) : residual, w, eps, false, true);
+    ctx->set_materialize_grads(false);
+    const auto y = f.y.view(x.sizes());
+    // What the backward reads again is saved as the very tensor that the caller
+    // holds (x, or the returned h), so that a change of it in place is noticed.
+    if (!residual.defined()) {
+      ctx->save_for_backward({x2.is_alias_of(x) ? x : x2, w, f.rstd});
+      return {y};
+    }
+    const auto h = f.h.view(x.sizes());
+    ctx->save_for_backward({h, w, f.rstd});
+    return {y, h};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "rms_norm has no second derivative (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const auto h = as_rows(saved[0]);
+    const auto& dy = grads[0];
+    const torch::Tensor dh = grads.size() > 1 ? grads[1] : torch::Tensor();
+    const bool has_residual = grads.size() > 1;
+    torch::Tensor dx, dw;
+    if (dy.defined()) {
+      const auto rows = [&](const torch::Tensor& g) { return g.reshape(h.sizes()).to(h.scalar_type()).contiguous(); };
+      std::tie(dx, dw) = ::backward(rows(dy), dh.defined() ? rows(dh) : dh, h, saved[1], saved[2]);
+      dx = dx.view(dy.sizes());
+    } else {
+      dx = dh;   // only the residual stream was used, or nothing at all
+    }
+    return {dx, dw, has_residual ? dx : torch::Tensor(), torch::Tensor()};
+  }
+};
+
+// y, or (y, h) with a residual.
+py::object rms_norm(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual, double eps) {
+  check_args(x, weight, residual);
+  const torch::Tensor res = residual ? *residual : torch::Tensor();
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || weight.requires_grad() || (res.defined() && res.requires_grad()))) {
+    const auto out = RmsNormFn::apply(x, weight, residual, eps);
+    return residual ? py::object(py::make_tuple(out[0], out[1])) : py::cast(out[0]);
+  }
+  const Forward f = forward(as_rows(x), res.defined() ? as_rows(res) : res, weight.contiguous(), eps, false, false);
+  const auto y = x.dim() == 2 ? f.y : f.y.view(x.sizes());
+  if (!residual) return py::cast(y);
+  return py::make_tuple(y, x.dim() == 2 ? f.h : f.h.view(x.sizes()));
+}
+
+// (q, scale), or (q, scale, h) with a residual.
+py::tuple rms_norm_fp8(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual, double eps) {
+  check_args(x, weight, residual);
+  LM_CHECK_VALUE(!(at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() ||
+                                                     (residual && residual->requires_grad()))),
+                    "rms_norm_fp8 has no gradient: call it under torch.no_grad()");
+  const Forward f = forward(as_rows(x), residual ? as_rows(*residual) : torch::Tensor(), weight.contiguous(), eps, true,
+                            false);
+  const auto q = lm::from_rows(f.q, x), scale = lm::from_rows(f.scale, x);
+  if (!residual) return py::make_tuple(q, scale);
+  return py::make_tuple(q, scale, f.h.view(x.sizes()));
 }
 
 }  // namespace
 
 void register_rmsnorm_ops(py::module& m) {
-  m.def("rms_norm_fwd", &rms_norm_fwd,
-        "RMS norm forward with the residual's addition: y (or 8-bit values), h, rstd, scales",
-        py::arg("x"), py::arg("residual"), py::arg("weight"), py::arg("eps"), py::arg("fp8"), py::arg("keep_rstd"));
-  m.def("rms_norm_bwd", &rms_norm_bwd, "RMS norm backward: dx, dweight", py::arg("dy"), py::arg("dh"), py::arg("h"),
-        py::arg("weight"), py::arg("rstd"));
+  m.def("rms_norm", &rms_norm, "RMS norm of the last dimension with the residual's addition: y or (y, h), with autograd",
+        py::arg("x"), py::arg("weight"), py::arg("residual"), py::arg("eps"));
+  m.def("rms_norm_fp8", &rms_norm_fp8, "RMS norm with an e4m3 result: (q, scale) or (q, scale, h)", py::arg("x"),
+        py::arg("weight"), py::arg("residual"), py::arg("eps"));
   m.attr("RMS_NORM_MAX_WIDTH") = kMaxWidth;
 }

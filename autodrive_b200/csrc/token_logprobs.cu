@@ -23,14 +23,17 @@
 // Bound by memory for long rows. Rows of up to 1024 entries are held in the
 // registers of one warp or of a part of one; longer ones take a CTA each.
 #include <torch/extension.h>
+#include <ATen/ExpandUtils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include <vector>
 
+#include "lm_host.h"
 #include "lm_vec.h"
 
 namespace py = pybind11;
@@ -492,54 +495,44 @@ void for_small(int v, F&& f) {
   else go(integral_constant<int, 32>{}, integral_constant<int, 32>{});
 }
 
-Args common_args(const torch::Tensor& x, const torch::Tensor& tokens, const c10::optional<torch::Tensor>& mask,
-                 double temperature) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 &&
-                  (x.scalar_type() == torch::kFloat32 || x.scalar_type() == torch::kBFloat16 ||
-                   x.scalar_type() == torch::kHalf),
-              "token_log_probs: logits must be a CUDA fp32, bf16 or fp16 [rows, V] tensor");
-  TORCH_CHECK(x.size(1) >= 1 && x.size(1) < (1ll << 30), "token_log_probs: V must be in 1..2^30 - 1");
-  TORCH_CHECK(x.numel() == 0 || x.size(1) == 1 || x.stride(1) == 1, "token_log_probs: the logits of a row must be contiguous");
-  TORCH_CHECK(x.size(0) < (1ll << 31) - 1, "token_log_probs: too many rows");
-  TORCH_CHECK(tokens.is_cuda() && tokens.device() == x.device() && tokens.scalar_type() == torch::kInt64 &&
-                  tokens.dim() == 1 && tokens.size(0) == x.size(0) && tokens.is_contiguous(),
-              "token_log_probs: tokens must be a contiguous int64 [rows] on the logits' device");
-  TORCH_CHECK(temperature > 0., "token_log_probs: the temperature must be positive");
+// Logits [rows, V] and mask (bool, or undefined) with contiguous rows.
+Args common_args(const torch::Tensor& x, const torch::Tensor& tokens, const torch::Tensor& mask, double temperature) {
   Args a{};
   a.x = x.data_ptr();
   a.rows = x.size(0);
   a.v = (int)x.size(1);
   a.ldx = a.rows > 1 ? x.stride(0) : a.v;
-  if (mask) {
-    TORCH_CHECK(mask->is_cuda() && mask->device() == x.device() && mask->scalar_type() == torch::kBool &&
-                    mask->sizes() == x.sizes() && (x.numel() == 0 || a.v == 1 || mask->stride(1) == 1),
-                "token_log_probs: mask must be bool [rows, V] with contiguous rows on the logits' device");
-    a.mask = reinterpret_cast<const uint8_t*>(mask->data_ptr());
-    a.ldm = a.rows > 1 ? mask->stride(0) : a.v;
+  if (mask.defined()) {
+    a.mask = reinterpret_cast<const uint8_t*>(mask.data_ptr());
+    a.ldm = a.rows > 1 ? mask.stride(0) : a.v;
   }
   a.tokens = tokens.data_ptr<int64_t>();
   a.inv_t = (float)(1. / temperature);
   return a;
 }
 
-// Returns {log_prob, entropy, top_value, top_token, stats (empty unless keep)}.
-std::vector<torch::Tensor> token_log_probs_fwd(torch::Tensor x, torch::Tensor tokens, c10::optional<torch::Tensor> mask,
-                                               double temperature, int64_t top, bool keep) {
-  Args a = common_args(x, tokens, mask, temperature);
-  TORCH_CHECK(top >= 0 && top <= kMaxTop, "token_log_probs: top must be in 0..", kMaxTop);
+struct Results {
+  torch::Tensor lp, ent, tv, tt, stats;   // stats only where a backward follows
+};
+
+Results forward(const torch::Tensor& x, const torch::Tensor& tokens, const torch::Tensor& mask, double temperature,
+                int64_t top, bool keep) {
   const c10::cuda::CUDAGuard guard(x.device());
+  Args a = common_args(x, tokens, mask, temperature);
   const auto f32 = x.options().dtype(torch::kFloat32);
-  auto lp = torch::empty({a.rows}, f32), ent = torch::empty({a.rows}, f32);
-  auto tv = torch::empty({a.rows, top}, f32);
-  auto tt = torch::empty({a.rows, top}, x.options().dtype(torch::kInt64));
-  auto stats = torch::empty({keep ? a.rows : 0, 3}, f32);
-  if (a.rows == 0) return {lp, ent, tv, tt, stats};
+  Results r;
+  r.lp = torch::empty({a.rows}, f32);
+  r.ent = torch::empty({a.rows}, f32);
+  r.tv = torch::empty({a.rows, top}, f32);
+  r.tt = torch::empty({a.rows, top}, x.options().dtype(torch::kInt64));
+  if (keep) r.stats = torch::empty({a.rows, 3}, f32);
+  if (a.rows == 0) return r;
   a.top = (int)top;
-  a.log_prob = lp.data_ptr<float>();
-  a.entropy = ent.data_ptr<float>();
-  a.top_value = tv.data_ptr<float>();
-  a.top_token = tt.data_ptr<int64_t>();
-  a.stats = keep ? stats.data_ptr<float>() : nullptr;
+  a.log_prob = r.lp.data_ptr<float>();
+  a.entropy = r.ent.data_ptr<float>();
+  a.top_value = r.tv.data_ptr<float>();
+  a.top_token = r.tt.data_ptr<int64_t>();
+  a.stats = keep ? r.stats.data_ptr<float>() : nullptr;
   auto st = c10::cuda::getCurrentCUDAStream().stream();
   for_type(x.scalar_type(), [&](auto t) {
     using T = decltype(t);
@@ -553,25 +546,19 @@ std::vector<torch::Tensor> token_log_probs_fwd(torch::Tensor x, torch::Tensor to
     }
   });
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "token_log_probs launch failed");
-  return {lp, ent, tv, tt, stats};
+  lm::count_launches(1);
+  return r;
 }
 
-torch::Tensor token_log_probs_bwd(torch::Tensor x, torch::Tensor tokens, c10::optional<torch::Tensor> mask,
-                                  double temperature, torch::Tensor stats, c10::optional<torch::Tensor> g_lp,
-                                  c10::optional<torch::Tensor> g_ent) {
-  Args a = common_args(x, tokens, mask, temperature);
-  TORCH_CHECK(stats.is_cuda() && stats.device() == x.device() && stats.scalar_type() == torch::kFloat32 &&
-                  stats.numel() == 3 * a.rows && stats.is_contiguous(), "token_log_probs: stats must be fp32 [rows, 3]");
-  for (auto* g : {&g_lp, &g_ent})
-    if (*g)
-      TORCH_CHECK((*g)->is_cuda() && (*g)->device() == x.device() && (*g)->scalar_type() == torch::kFloat32 &&
-                      (*g)->numel() == a.rows && (*g)->is_contiguous(), "token_log_probs: gradients must be fp32 [rows]");
+torch::Tensor backward(const torch::Tensor& x, const torch::Tensor& tokens, const torch::Tensor& mask, double temperature,
+                       const torch::Tensor& stats, const torch::Tensor& g_lp, const torch::Tensor& g_ent) {
   const c10::cuda::CUDAGuard guard(x.device());
+  Args a = common_args(x, tokens, mask, temperature);
   auto dx = torch::empty({a.rows, (int64_t)a.v}, x.options());
   if (a.rows == 0) return dx;
   a.stats = stats.data_ptr<float>();
-  const float* gl = g_lp ? g_lp->data_ptr<float>() : nullptr;
-  const float* ge = g_ent ? g_ent->data_ptr<float>() : nullptr;
+  const float* gl = g_lp.defined() ? g_lp.data_ptr<float>() : nullptr;
+  const float* ge = g_ent.defined() ? g_ent.data_ptr<float>() : nullptr;
   auto st = c10::cuda::getCurrentCUDAStream().stream();
   for_type(x.scalar_type(), [&](auto t) {
     using T = decltype(t);
@@ -588,17 +575,99 @@ torch::Tensor token_log_probs_bwd(torch::Tensor x, torch::Tensor tokens, c10::op
     }
   });
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "token_log_probs backward launch failed");
+  lm::count_launches(1);
   return dx;
+}
+
+// `t` as [rows, V] whose rows are contiguous (a row may be repeated).
+torch::Tensor as_rows(const torch::Tensor& t) {
+  const int64_t v = t.size(-1);
+  const auto y = t.dim() == 2 ? t : t.reshape({t.numel() / v, v});
+  return y.numel() == 0 || v == 1 || y.stride(1) == 1 ? y : y.contiguous();
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct TokenLogProbsFn : torch::autograd::Function<TokenLogProbsFn> {
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& logits, const torch::Tensor& tokens,
+                               const c10::optional<torch::Tensor>& m, double temperature, int64_t top) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const torch::Tensor mask = m ? *m : torch::Tensor();
+    const auto x = as_rows(logits);
+    const Results r = ::forward(x, tokens, mask, temperature, top, true);
+    // saved as the caller's tensors where they are read again, so that a change in place is noticed
+    ctx->save_for_backward({x.is_alias_of(logits) ? logits : x, tokens, mask, r.stats});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["sizes"] = logits.sizes().vec();
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({r.tv, r.tt});
+    return {r.lp, r.ent, r.tv, r.tt};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "token_log_probs has no second derivative (create_graph)");
+    variable_list out(5);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const auto f32 = [](const torch::Tensor& g) {
+      return g.defined() ? g.to(torch::kFloat32).contiguous() : g;
+    };
+    out[0] = ::backward(as_rows(saved[0]), saved[1], saved[2], ctx->saved_data["temperature"].toDouble(), saved[3],
+                        f32(grads[0]), f32(grads[1])).view(ctx->saved_data["sizes"].toIntVector());
+    return out;
+  }
+};
+
+// (log_prob, entropy, top_log_prob, top_token).
+py::tuple token_log_probs(torch::Tensor logits, torch::Tensor tokens, c10::optional<torch::Tensor> mask,
+                          double temperature, int64_t top) {
+  const auto type = logits.scalar_type();
+  LM_CHECK_VALUE(logits.is_cuda() && logits.dim() >= 1 && logits.size(-1) >= 1 && logits.size(-1) < (1ll << 30) &&
+                        (type == torch::kFloat32 || type == torch::kBFloat16 || type == torch::kHalf),
+                    "token_log_probs takes fp32, bf16 or fp16 logits [..., V]");
+  const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+  LM_CHECK_VALUE(tokens.sizes() == lead && tokens.device() == logits.device() &&
+                        (tokens.scalar_type() == torch::kInt64 || tokens.scalar_type() == torch::kInt32),
+                    "token_log_probs needs integer tokens ", lead, " on ", logits.device());
+  LM_CHECK_VALUE(tokens.numel() < (1ll << 31) - 1, "token_log_probs: too many rows");
+  LM_CHECK_VALUE(temperature > 0. && std::isfinite(temperature),
+                    "the temperature must be positive and finite, not ", temperature);
+  LM_CHECK_VALUE(top >= 0 && top <= kMaxTop, "top must be in 0..", kMaxTop, ", not ", top);
+  torch::Tensor m, t = tokens;
+  if (mask) {
+    LM_CHECK_VALUE(mask->scalar_type() == torch::kBool && mask->device() == logits.device(),
+                      "the mask must be boolean (true: valid) on the logits' device");
+    m = *mask;
+    if (m.sizes() != logits.sizes()) {
+      LM_CHECK_VALUE(at::is_expandable_to(m.sizes(), logits.sizes()), "the mask ", m.sizes(),
+                        " does not broadcast to ", logits.sizes());
+      m = m.expand(logits.sizes());
+    }
+    m = as_rows(m);
+  }
+  if (t.dim() != 1) t = t.reshape({t.numel()});
+  if (t.scalar_type() != torch::kInt64) t = t.to(torch::kInt64);
+  t = t.contiguous();
+  Results r;
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    const auto o = TokenLogProbsFn::apply(logits, t, mask ? c10::optional<torch::Tensor>(m) : c10::nullopt, temperature, top);
+    r = Results{o[0], o[1], o[2], o[3], {}};
+  } else {
+    r = forward(as_rows(logits), t, m, temperature, top, false);
+  }
+  if (lead.size() == 1) return py::make_tuple(r.lp, r.ent, r.tv, r.tt);
+  auto sizes = lead.vec();
+  const auto lp = r.lp.view(sizes), ent = r.ent.view(sizes);
+  sizes.push_back(top);
+  return py::make_tuple(lp, ent, r.tv.view(sizes), r.tt.view(sizes));
 }
 
 }  // namespace
 
 void register_token_logprobs_ops(py::module& m) {
-  m.def("token_log_probs_fwd", &token_log_probs_fwd,
-        "log-probabilities of given tokens: log_prob, entropy, top values, top tokens, stats", py::arg("logits"),
-        py::arg("tokens"), py::arg("mask"), py::arg("temperature"), py::arg("top"), py::arg("keep"));
-  m.def("token_log_probs_bwd", &token_log_probs_bwd, "gradient of the log-probabilities and entropies",
-        py::arg("logits"), py::arg("tokens"), py::arg("mask"), py::arg("temperature"), py::arg("stats"),
-        py::arg("g_log_prob"), py::arg("g_entropy"));
+  m.def("token_log_probs", &token_log_probs,
+        "log-probabilities of given tokens, with autograd: (log_prob, entropy, top_log_prob, top_token)",
+        py::arg("logits"), py::arg("tokens"), py::arg("mask"), py::arg("temperature"), py::arg("top"));
   m.attr("TOKEN_LOG_PROBS_MAX_TOP") = kMaxTop;
 }

@@ -34,10 +34,9 @@ import torch
 from torch import Tensor, nn
 from torch.autograd.function import once_differentiable
 
-from ..utils import launches
 from .ext import require_extension
 from .rmsnorm import from_rows
-from .tc_linear import _bf16_padded, _pad8, _result_dtype, _Status, gemm
+from .tc_linear import _result_dtype, _Status
 
 GROUP = 128
 E4M3 = torch.float8_e4m3fn
@@ -109,21 +108,13 @@ def _check_input(x: Tensor, dims: int, what: str) -> None:
         raise ValueError(f"{what} takes fp32, bf16 or fp16 tensors of at least {dims} dimension(s)")
 
 
-def _matrix(x: Tensor) -> Tensor:
-    y = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.reshape(x.shape[:-1].numel(), 0)
-    return y if y.stride(-1) == 1 and (y.shape[0] <= 1 or y.stride(0) >= y.shape[1]) else y.contiguous()
-
-
 def quantize_rows(x: Tensor) -> tuple[Tensor, Tensor]:
     """`x` [..., K] as e4m3 with one fp32 scale for each row and 128 columns
     (see the module docstring). No gradient."""
-    _check_input(x, 1, "quantize_rows")
-    x2 = _matrix(x.detach())
     if x.is_cuda:
-        launches.add(1)
-        q, scale = require_extension().quantize_rows(x2)
-    else:
-        q, scale = reference_quantize_rows(x2)
+        return require_extension().quantize_rows(x)
+    _check_input(x, 1, "quantize_rows")
+    q, scale = reference_quantize_rows(x.detach().reshape(x.shape[:-1].numel(), x.shape[-1]))
     return from_rows(q, x.shape[:-1]), from_rows(scale, x.shape[:-1])
 
 
@@ -131,23 +122,14 @@ def quantize_blocks(w: Tensor, transposed: bool = False):
     """`w` [N, K] as e4m3 with one fp32 scale for each 128 x 128 block: (q,
     scale), with `transposed` (q, scale, q^T, scale^T), the transposes being
     matrices of their own. No gradient."""
+    if w.is_cuda:
+        return require_extension().quantize_blocks(w, transposed)
     _check_input(w, 2, "quantize_blocks")
     if w.dim() != 2:
         raise ValueError("quantize_blocks takes a matrix")
-    w2 = _matrix(w.detach())
-    if w.is_cuda:
-        launches.add(1)
-        return tuple(require_extension().quantize_blocks(w2, bool(transposed)))
-    q, scale = reference_quantize_blocks(w2)
+    q, scale = reference_quantize_blocks(w.detach())
     return (q, scale, _padded_q(q.view(torch.uint8).t().view(E4M3)), scale.t().contiguous()) if transposed \
         else (q, scale)
-
-
-def _operand(q: Tensor) -> Tensor:
-    """`q` as the kernel reads it: rows 16 bytes apart on a 16-byte aligned base (a copy only where they are not)."""
-    ok = (q.shape[1] <= 1 or q.stride(1) == 1) and (q.shape[0] <= 1 or (q.stride(0) % 16 == 0
-                                                                        and q.stride(0) >= q.shape[1]))
-    return q if ok and q.data_ptr() % 16 == 0 else _padded_q(q)
 
 
 def reference_fp8_matmul(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Tensor | None = None,
@@ -162,6 +144,10 @@ def fp8_matmul(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Ten
     """a b^T of quantised rows `a` [..., K] and a quantised matrix `b` [N, K]
     with their scales, plus `bias` [N]: [..., N] in `out_dtype` (fp32, bf16 or
     fp16). `wait_ns` bounds every pipeline wait inside the kernel."""
+    if a.is_cuda:
+        y = require_extension().fp8_matmul(a, a_scale, b, b_scale, bias, out_dtype, _Status.get(a.device), wait_ns)
+        _Status.after_launch(a.device)
+        return y
     if a.dtype != E4M3 or b.dtype != E4M3 or a.dim() < 1 or b.dim() != 2:
         raise ValueError("fp8_matmul takes e4m3 rows [..., K] and an e4m3 matrix [N, K]")
     k, n, lead = a.shape[-1], b.shape[0], a.shape[:-1]
@@ -181,50 +167,31 @@ def fp8_matmul(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Ten
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (a_scale, b_scale, bias)):
         raise ValueError("fp8_matmul has no gradient: use fp8_linear, or call it under torch.no_grad()")
     rows = lead.numel()
-    a2, s2 = a.reshape(rows, k), a_scale.reshape(rows, _groups(k))
-    if not a.is_cuda:
-        return reference_fp8_matmul(a2, s2, b, b_scale, bias, out_dtype).view(*lead, n)
-    b32 = None if bias is None else bias.detach().float().contiguous()
-    y = require_extension().fp8_matmul(_operand(a2), s2.contiguous(), _operand(b), b_scale.contiguous(), b32,
-                                       out_dtype, _Status.get(a.device), int(wait_ns))
-    launches.add(1)
-    _Status.after_launch(a.device)
-    return y.view(*lead, n)
+    return reference_fp8_matmul(a.reshape(rows, k), a_scale.reshape(rows, _groups(k)), b, b_scale, bias,
+                                out_dtype).view(*lead, n)
 
 
-class _Fp8LinearFn(torch.autograd.Function):
+class _Fp8LinearCpuFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        x2 = _matrix(x)
-        xq, xs = quantize_rows(x2)
-        # the input gradient reads the weight down its columns: its transposed copy is written by the same pass
-        wq, ws, *t = quantize_blocks(weight, transposed=ctx.needs_input_grad[0])
-        target = _result_dtype(x)
-        b = None if bias is None else bias.detach()
-        y = fp8_matmul(xq, xs, wq, ws, b, target)
-        keep = x2 if ctx.needs_input_grad[1] else None
-        if keep is not None and x.is_cuda and keep.dtype != torch.bfloat16:
-            keep = keep.to(torch.bfloat16)   # the weight gradient's product takes bf16 operands
-        ctx.save_for_backward(keep, *t)
-        ctx.meta = (x.shape, x.dtype, weight.shape, weight.dtype, None if bias is None else bias.dtype)
+        x2 = x.reshape(x.shape[:-1].numel(), x.shape[-1])
+        wq, ws = reference_quantize_blocks(weight)
+        y = reference_fp8_matmul(*reference_quantize_rows(x2), wq, ws, bias, x.dtype)
+        ctx.save_for_backward(x, wq, ws)
+        ctx.meta = (weight.dtype, None if bias is None else bias.dtype)
         return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        keep, *t = ctx.saved_tensors
-        x_shape, x_dtype, (n, k), w_dtype, b_dtype = ctx.meta
-        g = gy.reshape(-1, n)
-        gx = gw = gb = None
+        x, wq, ws = ctx.saved_tensors
+        w_dtype, b_dtype = ctx.meta
+        n, k = wq.shape
+        g, gx, gw, gb = gy.reshape(-1, n), None, None, None
         if ctx.needs_input_grad[0]:
-            gq, gs = quantize_rows(g)
-            gx = fp8_matmul(gq, gs, t[0], t[1], out_dtype=x_dtype).view(x_shape)
+            gx = (dequantize_rows(*reference_quantize_rows(g)) @ dequantize_blocks(wq, ws)).to(x.dtype).view(x.shape)
         if ctx.needs_input_grad[1]:
-            if g.is_cuda:
-                gw = gemm(_bf16_padded(g, _pad8(n)), _bf16_padded(keep, _pad8(k)), a_mn=True, b_mn=True)[:n, :k]
-            else:
-                gw = g.float().t() @ keep.float()
-            gw = gw.to(w_dtype)
+            gw = (g.float().t() @ x.reshape(-1, k).float()).to(w_dtype)
         if ctx.needs_input_grad[2]:
             gb = g.sum(0, dtype=torch.float32).to(b_dtype)
         return gx, gw, gb
@@ -234,13 +201,17 @@ def fp8_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tensor:
     """x weight^T + bias with both operands quantised to e4m3 (see the module
     docstring), with autograd. The result has x's dtype, or the autocast dtype
     inside a CUDA autocast region."""
+    if x.is_cuda:
+        y = require_extension().fp8_linear(x, weight, bias, _result_dtype(x), _Status.get(x.device))
+        _Status.after_launch(x.device)
+        return y
     _check_input(x, 1, "fp8_linear")
     _check_input(weight, 2, "fp8_linear")
     if weight.dim() != 2 or x.shape[-1] != weight.shape[1] or (bias is not None and bias.shape != weight.shape[:1]):
         raise ValueError(f"fp8_linear: x {tuple(x.shape)}, weight {tuple(weight.shape)} and bias do not fit")
     if any(t is not None and t.device != x.device for t in (weight, bias)):
         raise ValueError("fp8_linear needs all of its tensors on one device")
-    return _Fp8LinearFn.apply(x, weight, bias)
+    return _Fp8LinearCpuFn.apply(x, weight, bias)
 
 
 class Fp8Linear(nn.Linear):

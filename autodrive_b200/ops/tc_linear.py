@@ -79,8 +79,7 @@ class _Status:
 
     @classmethod
     def _entry(cls, device):
-        key = str(device)
-        e = cls._state.get(key)
+        e = cls._state.get(device)
         if e is None:
             if torch.cuda.is_current_stream_capturing():
                 # a word made here would live in the graph's memory and be cleared by its replays alone
@@ -88,7 +87,7 @@ class _Status:
             word = torch.zeros(1, dtype=torch.int32, device=device)
             host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
             e = {"word": word, "host": host, "event": None, "launches": 0}
-            cls._state[key] = e
+            cls._state[device] = e
         return e
 
     @classmethod

@@ -30,7 +30,6 @@ import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
-from ..utils import launches
 from .ext import require_extension
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
@@ -97,17 +96,11 @@ def reference_token_log_probs_grad(logits: Tensor, tokens: Tensor, mask: Tensor 
     return torch.where(dead, 0., d)
 
 
-class _TokenLogProbsFn(torch.autograd.Function):
+class _TokenLogProbsCpuFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, mask, temperature, top):
-        if logits.is_cuda:
-            launches.add(1)
-            lp, ent, tv, tt, stats = require_extension().token_log_probs_fwd(logits, tokens, mask, temperature, top,
-                                                                            True)
-        else:
-            lp, ent, tv, tt = reference_token_log_probs(logits, tokens, mask, temperature, top)
-            stats = None
-        ctx.save_for_backward(logits, tokens, mask, stats)
+        lp, ent, tv, tt = reference_token_log_probs(logits, tokens, mask, temperature, top)
+        ctx.save_for_backward(logits, tokens, mask)
         ctx.temperature = temperature
         ctx.mark_non_differentiable(tv, tt)
         ctx.set_materialize_grads(False)
@@ -118,26 +111,17 @@ class _TokenLogProbsFn(torch.autograd.Function):
     def backward(ctx, g_lp, g_ent, _tv, _tt):
         if g_lp is None and g_ent is None:
             return None, None, None, None, None
-        logits, tokens, mask, stats = ctx.saved_tensors
-        g_lp, g_ent = (None if g is None else g.float().contiguous() for g in (g_lp, g_ent))
-        if logits.is_cuda:
-            launches.add(1)
-            dx = require_extension().token_log_probs_bwd(logits, tokens, mask, ctx.temperature, stats, g_lp, g_ent)
-        else:
-            dx = reference_token_log_probs_grad(logits, tokens, mask, ctx.temperature, g_lp, g_ent).to(logits.dtype)
-        return dx, None, None, None, None
-
-
-def _rows(x: Tensor) -> Tensor:
-    """`x` as [rows, V] whose rows are contiguous (a row may be repeated)."""
-    y = x.reshape(-1, x.shape[-1])
-    return y if y.shape[1] == 1 or y.stride(1) == 1 else y.contiguous()
+        logits, tokens, mask = ctx.saved_tensors
+        dx = reference_token_log_probs_grad(logits, tokens, mask, ctx.temperature, g_lp, g_ent)
+        return dx.to(logits.dtype), None, None, None, None
 
 
 def token_log_probs(logits: Tensor, tokens: Tensor, mask: Tensor | None = None, temperature: float = 1.,
                     top: int = 0) -> TokenLogProbs:
     """Log-probabilities of `tokens`, entropies and alternatives of the rows of
     `logits` (see the module docstring)."""
+    if logits.is_cuda:
+        return TokenLogProbs._make(require_extension().token_log_probs(logits, tokens, mask, temperature, top))
     if logits.dim() < 1 or logits.shape[-1] < 1 or logits.dtype not in DTYPES:
         raise ValueError("token_log_probs takes fp32, bf16 or fp16 logits [..., V]")
     lead, v = logits.shape[:-1], logits.shape[-1]
@@ -151,17 +135,9 @@ def token_log_probs(logits: Tensor, tokens: Tensor, mask: Tensor | None = None, 
         if mask.dtype != torch.bool or mask.device != logits.device:
             raise ValueError("the mask must be boolean (true: valid) on the logits' device")
         try:
-            mask = _rows(mask.expand(logits.shape))
+            mask = mask.expand(logits.shape).reshape(-1, v)
         except RuntimeError as exc:
             raise ValueError(f"the mask {tuple(mask.shape)} does not broadcast to {tuple(logits.shape)}") from exc
-    x, t = _rows(logits), tokens.reshape(-1).long().contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        lp, ent, tv, tt = _TokenLogProbsFn.apply(x, t, mask, float(temperature), int(top))
-    elif x.is_cuda:
-        launches.add(1)
-        lp, ent, tv, tt, _ = require_extension().token_log_probs_fwd(x, t, mask, float(temperature), int(top), False)
-    else:
-        lp, ent, tv, tt = reference_token_log_probs(x.detach(), t, mask, temperature, top)
-    if len(lead) == 1:
-        return TokenLogProbs(lp, ent, tv, tt)
+    lp, ent, tv, tt = _TokenLogProbsCpuFn.apply(logits.reshape(-1, v), tokens.reshape(-1).long(), mask, float(temperature),
+                                                int(top))
     return TokenLogProbs(lp.view(lead), ent.view(lead), tv.view(*lead, top), tt.view(*lead, top))

@@ -12,7 +12,7 @@ ext = CUDAExtension(
     name="autodrive_b200._C",
     sources=[os.path.join(CSRC, f) for f in (
         "bindings.cpp", "adstar_cpu.cpp", "sim.cu", "policy_ops.cu", "policy_tc.cu", "tc_gemm.cu", "comm_ops.cu", "noalloc_adam.cu", "sha256.cu", "plan_a.cu", "layernorm.cu", "rmsnorm.cu",
-        "fp8_quant.cu", "fp8_gemm.cu", "token_logprobs.cu", "attention.cu")],
+        "fp8_quant.cu", "fp8_gemm.cu", "fp8_linear.cpp", "token_logprobs.cu", "attention.cu")],
     include_dirs=[os.path.join(HERE, CSRC)],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],

@@ -357,3 +357,16 @@ def test_a_wait_that_runs_out_is_reported(m):
     y = fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32)   # the next call is sound
     check_gemm_status(dev)
     _check_product(y, a, a_s, b, b_s, None, torch.float32)
+
+
+@pytest.mark.gpu
+def test_changes_in_place_and_second_derivatives_are_refused():
+    x = torch.randn(8, 64, device="cuda").bfloat16()
+    w = torch.randn(32, 64, device="cuda", requires_grad=True)
+    y = fp8_linear(x, w)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y.sum(), w, create_graph=True)
+    y = fp8_linear(x, w)
+    x += 1.   # the weight gradient would read it
+    with pytest.raises(RuntimeError):
+        y.sum().backward()

@@ -271,3 +271,18 @@ def test_captured_and_replayed():
     want = step()
     for a, b in zip(out, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_changes_in_place_and_second_derivatives_are_refused():
+    x, r, w = _inputs(4, 64, torch.float32, "cuda")
+    x.requires_grad_(True)
+    y, h = rms_norm(x, w, r)
+    h.data_ptr()
+    with torch.no_grad():
+        h += 1.   # the backward would read it
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+    y = rms_norm(x, w)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y.sum(), x, create_graph=True)

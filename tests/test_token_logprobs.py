@@ -338,3 +338,17 @@ def test_reference_pads_and_breaks_ties_by_index():
     x = torch.tensor([[1., 3., 3., -torch.inf]])
     r = reference_token_log_probs(x, torch.tensor([1]), top=5)
     assert r.top_token.tolist() == [[1, 2, 0, -1, -1]]
+
+
+@pytest.mark.gpu
+def test_changes_in_place_and_second_derivatives_are_refused():
+    x, t, _ = _make(4, 64, torch.float32, "cuda")
+    x.requires_grad_(True)
+    r = token_log_probs(x, t)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(r.log_prob.sum(), x, create_graph=True)
+    r = token_log_probs(x, t)
+    with torch.no_grad():
+        x += 1.
+    with pytest.raises(RuntimeError):
+        r.entropy.sum().backward()
