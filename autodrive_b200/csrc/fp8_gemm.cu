@@ -12,8 +12,10 @@
 //   warp 0     TMA producer: the 128-byte wide A and B tiles of each group into
 //              a shared-memory ring that runs on across output tiles;
 //   warp 1     allocates TMEM; one lane issues the four K = 32 products of a
-//              group into the next buffer, then commits the stage back to the
-//              producer and the buffer to the epilogue;
+//              group into the next buffer and commits them to one barrier, on
+//              which the producer waits for the stage and the epilogue for the
+//              buffer (there are more stages than buffers, so neither can be
+//              a whole round behind);
 //   warps 2-9  two per TMEM lane quadrant: thread = one row, half the columns.
 // Waits are bounded and reported as in the bf16 GEMM (tc_gemm.cu), with the
 // same status bits and the same drains before the CTA gives up its TMEM.
@@ -54,6 +56,20 @@ struct Args {
   uint64_t wait_ns;
 };
 
+// Records that a wait of the role with this status bit ran out.
+__device__ __forceinline__ void give_up(const Args& g, int bit, int* s_fail) {
+  atomicOr(g.status, bit);
+  atomicExch(s_fail, 1);
+}
+
+// A place in a ring of N slots and the parity of its current round.
+template <int N> struct Ring {
+  uint32_t slot = 0, round = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) slot = 0, round ^= 1;
+  }
+};
+
 template <int BN> struct Config {
   static constexpr int stages = BN == 128 ? 6 : 4;
   static constexpr uint32_t a_bytes = kBM * kGroup, stage_bytes = a_bytes + BN * kGroup;
@@ -78,6 +94,197 @@ __device__ __forceinline__ void store32(T* dst, const float (&v)[32], int n, boo
   }
 }
 
+// The sums of a CTA's rows over one group: acc += sc * TMEM, `chunks` times 32
+// columns from `base`, the next chunk's load in flight while one is added. The
+// buffer is handed back (release()) once its last chunk is in registers.
+template <int CHUNKS, typename F>
+__device__ __forceinline__ void add_group(uint32_t base, float sc, float (&acc)[CHUNKS][32], F&& release) {
+  float v[2][32];
+  tc::tmem_ld32_issue(base, v[0]);
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    tc::tmem_ld_wait();
+    tc::tmem_regs_ready(v[c & 1]);
+    if (c + 1 < CHUNKS) tc::tmem_ld32_issue(base + 32 * (c + 1), v[(c + 1) & 1]);
+    else release();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) acc[c][i] = fmaf(v[c & 1][i], sc, acc[c][i]);
+  }
+}
+
+// The scales of one row of A and one row block of B, loaded four groups ahead
+// and multiplied only when they are used: a load has four groups' time to
+// arrive.
+struct Scales {
+  const float* a;
+  const float* b;
+  int groups;
+  float cur[4], na[4], nb[4];
+  __device__ __forceinline__ void load(int kb) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = min(kb + j, groups - 1);
+      na[j] = __ldg(a + k);
+      nb[j] = __ldg(b + k);
+    }
+  }
+  __device__ __forceinline__ Scales(const float* pa, const float* pb, int g) : a(pa), b(pb), groups(g) { load(0); }
+  // Call for kb = 0, 1, 2, ...
+  __device__ __forceinline__ float at(int kb) {
+    if ((kb & 3) == 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) cur[j] = na[j] * nb[j];
+      if (kb + 4 < groups) load(kb + 4);
+    }
+    const float lo = kb & 1 ? cur[1] : cur[0], hi = kb & 1 ? cur[3] : cur[2];
+    return kb & 2 ? hi : lo;
+  }
+};
+
+// bias and the store of `acc`, `CHUNKS` times 32 columns from n0 of one row.
+template <int CHUNKS>
+__device__ __forceinline__ void store_row(const Args& g, float (&acc)[CHUNKS][32], int row, int n0) {
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int col = n0 + 32 * c, n = g.N - col;
+    if (n <= 0) break;
+    if (g.bias) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) acc[c][i] += i < n ? g.bias[col + i] : 0.f;
+    }
+    const int64_t off = (int64_t)row * g.ldc + col;
+    const bool vec = n >= 32 && g.ldc % 8 == 0;   // the output's base is 16-byte aligned (host)
+    if (g.out_kind == 0) store32(reinterpret_cast<float*>(g.c) + off, acc[c], n, vec);
+    else if (g.out_kind == 1) store32(reinterpret_cast<__nv_bfloat16*>(g.c) + off, acc[c], n, vec);
+    else store32(reinterpret_cast<__half*>(g.c) + off, acc[c], n, vec);
+  }
+}
+
+// An epilogue warp: TMEM lanes 32 q .. + 31 and half of the tile's COLS columns,
+// which lie inside one block of 128 rows of B. `walk` calls tile(first row,
+// first column) for one of the CTA's tiles after the other. `tempty0` may lie
+// in another CTA (a mapped address).
+template <int STAGES, int BUFFERS, int COLS, typename F>
+__device__ __forceinline__ void epilogue(const Args& g, uint32_t tmem, uint32_t done0, uint32_t tempty0, int* s_fail,
+                                         int q, int half, F&& walk) {
+  constexpr int kChunks = COLS / 64;   // 32-column chunks per warp
+  const int lane = threadIdx.x & 31, G = g.groups;
+  const uint32_t lanes = tmem + half * (COLS / 2) + ((uint32_t)(32 * q) << 16);
+  Ring<STAGES> st;
+  Ring<BUFFERS> buf;
+  walk([&](int m0, int n0) {
+    const int row = m0 + 32 * q + lane;
+    n0 += half * (COLS / 2);
+    float acc[kChunks][32];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) acc[c][i] = 0.f;
+    Scales sc(g.a_scale + (int64_t)min(row, g.M - 1) * G,
+              g.b_scale + (int64_t)min(n0 / kGroup, (g.N - 1) / kGroup) * G, G);
+    for (int kb = 0; kb < G; ++kb) {
+      const float scale = sc.at(kb);
+      const bool got = tc::mbar_wait(done0 + 8 * st.slot, st.round, g.wait_ns);
+      if (!__all_sync(0xffffffffu, got)) {   // the loads below are whole-warp
+        give_up(g, 4, s_fail);
+        return false;
+      }
+      tc::tc_fence_after();
+      add_group<kChunks>(lanes + buf.slot * COLS, scale, acc, [&] {
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_cluster(tempty0 + 8 * buf.slot);
+      });
+      st.next();
+      buf.next();
+    }
+    if (row < g.M) store_row<kChunks>(g, acc, row, n0);
+    return true;
+  });
+}
+
+// The producer's thread: `walk` calls load(k, row of A, row of B) for one
+// group's tiles after the other, until it answers false. Before it returns,
+// every load has landed and the products of every stage are complete: the
+// CTA's shared memory must not be given away before.
+template <int STAGES, typename F>
+__device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, const CUtensorMap* tb, uint32_t smem0,
+                                        uint32_t stage_bytes, uint32_t a_bytes, uint32_t full0, uint32_t done0,
+                                        int* s_fail, F&& walk) {
+  Ring<STAGES> st;
+  uint32_t issued = 0;
+  bool ok = true;
+  walk([&](int k, int row_a, int row_b) {
+    if (issued >= STAGES && !tc::mbar_wait(done0 + 8 * st.slot, st.round ^ 1, g.wait_ns)) {
+      give_up(g, 1, s_fail);
+      return ok = false;
+    }
+    const uint32_t sa = smem0 + st.slot * stage_bytes, full = full0 + 8 * st.slot;
+    tc::mbar_arrive_expect_tx(full, stage_bytes);
+    tc::tma_load_2d(sa, ta, k, row_a, full);
+    tc::tma_load_2d(sa + a_bytes, tb, k, row_b, full);
+    st.next();
+    ++issued;
+    return true;
+  });
+  for (uint32_t i = issued > (uint32_t)STAGES ? issued - STAGES : 0u; i < issued; ++i) {
+    const uint32_t slot = i % STAGES, round = (i / STAGES) & 1;
+    if (ok && !tc::mbar_wait(done0 + 8 * slot, round, g.wait_ns)) {
+      give_up(g, 1, s_fail);
+      ok = false;
+    }
+    if (!ok && !tc::mbar_wait(full0 + 8 * slot, round, kDrainNs)) atomicOr(g.status, 16);
+  }
+}
+
+// The product thread: for each of `count` groups, once its tiles are loaded (in
+// both CTAs of a pair) and the TMEM buffer is read out, issue its four products
+// and one commit, for the producer and the epilogue alike. Products take 48
+// cycles to issue, commits 59 and successful waits 40, one after the other, so
+// the next group's barriers are looked at between the products.
+template <int STAGES, int BUFFERS, int COLS, bool PAIR>
+__device__ __forceinline__ void multiply(const Args& g, uint32_t count, uint32_t smem0, uint32_t stage_bytes,
+                                         uint32_t a_bytes, uint32_t tmem, uint32_t full0, uint32_t peer0,
+                                         uint32_t done0, uint32_t tempty0, uint32_t drain, int* s_fail) {
+  const uint32_t id = tc::idesc_e4m3(PAIR ? 256 : 128, COLS), lo = tc::kmajor_desc_lo(smem0);
+  Ring<STAGES> st;
+  Ring<BUFFERS> buf;
+  bool loaded = false, read = true, peer = !PAIR;   // the buffers' first round needs no waiting
+  for (uint32_t it = 0; it < count; ++it) {
+    if (!read && !tc::mbar_wait(tempty0 + 8 * buf.slot, buf.round ^ 1, g.wait_ns)) {
+      give_up(g, 8, s_fail);
+      break;
+    }
+    if ((!loaded && !tc::mbar_wait(full0 + 8 * st.slot, st.round, g.wait_ns)) ||
+        (!peer && !tc::mbar_wait(peer0 + 8 * st.slot, st.round, g.wait_ns))) {
+      give_up(g, 2, s_fail);
+      break;
+    }
+    tc::tc_fence_after();
+    const uint32_t la = lo + st.slot * (stage_bytes >> 4), lb = la + (a_bytes >> 4), d = tmem + buf.slot * COLS;
+    const uint32_t done = done0 + 8 * st.slot;
+    st.next();
+    buf.next();
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      if constexpr (PAIR) tc::mma_e4m3_pair(d, tc::kmajor_desc(la + 2 * ks), tc::kmajor_desc(lb + 2 * ks), id, ks > 0);
+      else tc::mma_e4m3(d, tc::kmajor_desc(la + 2 * ks), tc::kmajor_desc(lb + 2 * ks), id, ks > 0);
+      if (ks == 1) {
+        read = it + 1 < (uint32_t)BUFFERS || tc::mbar_try_wait(tempty0 + 8 * buf.slot, buf.round ^ 1);
+        loaded = tc::mbar_try_wait(full0 + 8 * st.slot, st.round);
+        if constexpr (PAIR) peer = tc::mbar_try_wait(peer0 + 8 * st.slot, st.round);
+      }
+    }
+    if constexpr (PAIR) tc::mma_commit_pair(done);
+    else tc::mma_commit(done);
+  }
+  if (*(volatile int*)s_fail) {   // products issued so far may still read shared memory and write TMEM
+    if constexpr (PAIR) tc::mma_commit_pair(drain);
+    else tc::mma_commit(drain);
+    if (!tc::mbar_wait(drain, 0, kDrainNs)) atomicOr(g.status, 32);
+  }
+}
+
 template <int BN>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const Args g) {
@@ -86,13 +293,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* misc = smem + C::stages * C::stage_bytes;
   const uint32_t full0 = tc::smem_u32(misc);                    // stage loaded
-  const uint32_t empty0 = full0 + 8 * C::stages;                // stage consumed
-  const uint32_t tfull0 = empty0 + 8 * C::stages;               // TMEM buffer complete
-  const uint32_t tempty0 = tfull0 + 8 * C::buffers;             // TMEM buffer read out
+  const uint32_t done0 = full0 + 8 * C::stages;                 // stage's products complete
+  const uint32_t tempty0 = done0 + 8 * C::stages;               // TMEM buffer read out
   const uint32_t drain = tempty0 + 8 * C::buffers;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (2 * C::stages + 2 * C::buffers + 1));
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (2 * C::stages + C::buffers + 1));
   int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
-  volatile int* fail = s_fail;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles_n = (g.N + BN - 1) / BN, tiles_m = (g.M + kBM - 1) / kBM;
@@ -101,12 +306,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::stages; ++s) {
       tc::mbar_init(full0 + 8 * s, 1);
-      tc::mbar_init(empty0 + 8 * s, 1);
+      tc::mbar_init(done0 + 8 * s, 1);
     }
-    for (int b = 0; b < C::buffers; ++b) {
-      tc::mbar_init(tfull0 + 8 * b, 1);
-      tc::mbar_init(tempty0 + 8 * b, 32 * kEpiWarps);
-    }
+    for (int b = 0; b < C::buffers; ++b) tc::mbar_init(tempty0 + 8 * b, kEpiWarps);   // one lane of every epilogue warp
     tc::mbar_init(drain, 1);
     tc::mbar_init_fence();
     *s_fail = 0;
@@ -118,125 +320,128 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  const uint32_t tmem = *s_tmem;
+  const uint32_t tmem = *s_tmem, smem0 = tc::smem_u32(smem);
 
   if (warp == 0 && lane == 0) {
-    uint32_t it = 0;
-    for (int w = blockIdx.x; w < total && !*fail; w += gridDim.x) {
-      const int n0 = (w % tiles_n) * BN, m0 = (w / tiles_n) * kBM;
-      for (int kb = 0; kb < G; ++kb, ++it) {
-        const uint32_t s = it % C::stages;
-        if (it >= C::stages && !tc::mbar_wait(empty0 + 8 * s, ((it / C::stages) - 1) & 1, g.wait_ns)) {
-          atomicOr(g.status, 1);
-          atomicExch(s_fail, 1);
-        }
-        if (*fail) break;
-        const uint32_t sa = tc::smem_u32(smem + s * C::stage_bytes), full = full0 + 8 * s;
-        tc::mbar_arrive_expect_tx(full, C::stage_bytes);
-        tc::tma_load_2d(sa, &ta, kb * kGroup, m0, full);
-        tc::tma_load_2d(sa + C::a_bytes, &tb, kb * kGroup, n0, full);
-      }
-    }
-    if (*fail) {   // every stage's latest load may still be in flight
-      for (uint32_t i = it > (uint32_t)C::stages ? it - C::stages : 0u; i < it; ++i)
-        if (!tc::mbar_wait(full0 + 8 * (i % C::stages), (i / C::stages) & 1, kDrainNs)) atomicOr(g.status, 16);
-    }
+    produce<C::stages>(g, &ta, &tb, smem0, C::stage_bytes, C::a_bytes, full0, done0, s_fail, [&](auto&& load) {
+      for (int w = blockIdx.x; w < total; w += gridDim.x)
+        for (int kb = 0; kb < G; ++kb)
+          if (!load(kb * kGroup, (w / tiles_n) * kBM, (w % tiles_n) * BN)) return;
+    });
   } else if (warp == 1 && lane == 0) {
-    const uint32_t id = tc::idesc_e4m3(kBM, BN);
-    uint32_t it = 0;
-    for (int w = blockIdx.x; w < total && !*fail; w += gridDim.x) {
-      for (int kb = 0; kb < G; ++kb, ++it) {
-        const uint32_t s = it % C::stages, b = it % C::buffers;
-        if (it >= C::buffers && !tc::mbar_wait(tempty0 + 8 * b, ((it / C::buffers) - 1) & 1, g.wait_ns)) {
-          atomicOr(g.status, 8);
-          atomicExch(s_fail, 1);
-        } else if (!tc::mbar_wait(full0 + 8 * s, (it / C::stages) & 1, g.wait_ns)) {
-          atomicOr(g.status, 2);
-          atomicExch(s_fail, 1);
-        }
-        if (*fail) break;
-        tc::tc_fence_after();
-        const uint32_t sa = tc::smem_u32(smem + s * C::stage_bytes), sb = sa + C::a_bytes;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-          tc::mma_e4m3(tmem + b * BN, tc::sw128_desc(sa + 32 * ks, 16, 1024), tc::sw128_desc(sb + 32 * ks, 16, 1024),
-                       id, ks > 0);
-        tc::mma_commit(empty0 + 8 * s);
-        tc::mma_commit(tfull0 + 8 * b);
-      }
-    }
-    if (*fail) {   // products issued so far may still read shared memory and write TMEM
-      tc::mma_commit(drain);
-      if (!tc::mbar_wait(drain, 0, kDrainNs)) atomicOr(g.status, 32);
-    }
-  }
-
-  if (warp >= 2) {
-    constexpr int kChunks = BN / 64;   // 32-column chunks per warp
+    const uint32_t tiles = (total - 1 - (int)blockIdx.x) / (int)gridDim.x + 1;   // never more CTAs than tiles
+    multiply<C::stages, C::buffers, BN, false>(g, tiles * G, smem0, C::stage_bytes, C::a_bytes, tmem, full0, 0, done0,
+                                               tempty0, drain, s_fail);
+  } else if (warp >= 2) {
     const int q = warp & 3, half = (warp - 2) >> 2;
-    uint32_t it = 0;
-    for (int w = blockIdx.x; w < total; w += gridDim.x) {
-      const int n0 = (w % tiles_n) * BN + half * (BN / 2), row = (w / tiles_n) * kBM + 32 * q + lane;
-      float acc[kChunks][32];
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-        for (int i = 0; i < 32; ++i) acc[c][i] = 0.f;
-      // this half of the tile lies inside one block of 128 rows of B
-      const float* as = g.a_scale + (int64_t)min(row, g.M - 1) * G;
-      const float* bs = g.b_scale + (int64_t)min(n0 / kGroup, (g.N - 1) / kGroup) * G;
-      for (int kb = 0; kb < G; ++kb, ++it) {
-        const uint32_t b = it % C::buffers;
-        const float sc = as[kb] * bs[kb];
-        if (!tc::mbar_wait(tfull0 + 8 * b, (it / C::buffers) & 1, g.wait_ns)) {
-          atomicOr(g.status, 4);
-          atomicExch(s_fail, 1);
-        }
-        if (__any_sync(0xffffffffu, *fail)) break;   // the loads below are whole-warp
-        tc::tc_fence_after();
-        const uint32_t base = tmem + b * BN + half * (BN / 2) + ((uint32_t)(32 * q) << 16);
-#pragma unroll
-        for (int c = 0; c < kChunks; c += 2) {
-          float v[2][32];
-          tc::tmem_ld32_issue(base + 32 * c, v[0]);
-          tc::tmem_ld32_issue(base + 32 * (c + 1), v[1]);
-          tc::tmem_ld_wait();
-          tc::tmem_regs_ready(v[0]);
-          tc::tmem_regs_ready(v[1]);
-          if (c + 2 >= kChunks) {
-            tc::tc_fence_before();
-            tc::mbar_arrive(tempty0 + 8 * b);
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) acc[c + j][i] = fmaf(v[j][i], sc, acc[c + j][i]);
-        }
-      }
-      if (__any_sync(0xffffffffu, *fail)) break;
-      if (row < g.M) {
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const int col = n0 + 32 * c, n = g.N - col;
-          if (n <= 0) continue;
-          if (g.bias) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) acc[c][i] += i < n ? g.bias[col + i] : 0.f;
-          }
-          const int64_t off = (int64_t)row * g.ldc + col;
-          const bool vec = n >= 32 && g.ldc % 8 == 0;   // the output's base is 16-byte aligned (host)
-          if (g.out_kind == 0) store32(reinterpret_cast<float*>(g.c) + off, acc[c], n, vec);
-          else if (g.out_kind == 1) store32(reinterpret_cast<__nv_bfloat16*>(g.c) + off, acc[c], n, vec);
-          else store32(reinterpret_cast<__half*>(g.c) + off, acc[c], n, vec);
-        }
-      }
-    }
+    epilogue<C::stages, C::buffers, BN>(g, tmem, done0, tempty0, s_fail, q, half, [&](auto&& tile) {
+      for (int w = blockIdx.x; w < total; w += gridDim.x)
+        if (!tile((w / tiles_n) * kBM, (w % tiles_n) * BN)) return;
+    });
   }
   tc::tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- 256 x 256 tiles by pairs of CTAs ------------------------------------------
+// Each CTA loads 128 rows of A and 128 rows of B a group and keeps 128 x 256
+// sums; the pair's tensor cores share B, so that shared memory moves 64 KB per
+// 128 x 256 x 128 products instead of 96 KB for one CTA with such a tile, or
+// 128 KB with two of 128 x 128.
+//   warp 0      producer of the CTA's own tiles, into its own ring;
+//   warp 1      first CTA: issues the pair's products once both CTAs' tiles are
+//               there; second CTA: tells the first when its tiles have arrived;
+//   warps 4-11  epilogue, as above; warps 2 and 3 only complete the warpgroup
+//               that gives up its registers to the epilogue's 128 sums a thread.
+// Every CTA waits for its own loads before it ends, and both meet at a cluster
+// barrier before either frees its TMEM or shared memory.
+constexpr int kPairThreads = 384, kPairStages = 6, kPairBuffers = 2;
+constexpr uint32_t kPairTile = 128 * kGroup, kPairStage = 2 * kPairTile;
+constexpr uint32_t kPairSmem = kPairStages * kPairStage + 1024 + 256;
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const Args g) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* misc = smem + kPairStages * kPairStage;
+  const uint32_t full0 = tc::smem_u32(misc);                  // own tiles loaded
+  const uint32_t peer0 = full0 + 8 * kPairStages;             // first CTA: the second one's tiles loaded
+  const uint32_t done0 = peer0 + 8 * kPairStages;             // stage's products complete
+  const uint32_t tempty0 = done0 + 8 * kPairStages;           // first CTA: TMEM buffer read out by both
+  const uint32_t drain = tempty0 + 8 * kPairBuffers;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (3 * kPairStages + kPairBuffers + 1));
+  int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = tc::cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles_n = (g.N + 255) / 256, tiles_m = (g.M + 255) / 256;
+  const int total = tiles_n * tiles_m, G = g.groups;
+  const uint32_t tiles = (total - 1 - pair) / pairs + 1;      // never more pairs than tiles
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      tc::mbar_init(full0 + 8 * s, 1);
+      tc::mbar_init(peer0 + 8 * s, 1);
+      tc::mbar_init(done0 + 8 * s, 1);
+    }
+    for (int b = 0; b < kPairBuffers; ++b)
+      tc::mbar_init(tempty0 + 8 * b, 2 * kEpiWarps);   // one lane of every epilogue warp of both CTAs
+    tc::mbar_init(drain, 1);
+    tc::mbar_init_fence();
+    *s_fail = 0;
+  }
+  if (warp == 1) {
+    tc::tmem_alloc_pair(tc::smem_u32(s_tmem), 512);
+    tc::tmem_relinquish_pair();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::cluster_sync();
+  tc::tc_fence_after();
+  const uint32_t tmem = *s_tmem, smem0 = tc::smem_u32(smem);
+
+  if (warp < 4) {
+    tc::regs_dec<40>();
+    if (warp == 0 && lane == 0) {
+      produce<kPairStages>(g, &ta, &tb, smem0, kPairStage, kPairTile, full0, done0, s_fail, [&](auto&& load) {
+        for (int w = pair; w < total; w += pairs)
+          for (int kb = 0; kb < G; ++kb)
+            if (!load(kb * kGroup, (w / tiles_n) * 256 + (int)rank * 128, (w % tiles_n) * 256 + (int)rank * 128)) return;
+      });
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      multiply<kPairStages, kPairBuffers, 256, true>(g, tiles * G, smem0, kPairStage, kPairTile, tmem, full0, peer0, done0,
+                                                     tempty0, drain, s_fail);
+    } else if (warp == 1 && lane == 0) {
+      const uint32_t peer = tc::cluster_map(peer0, 0);
+      Ring<kPairStages> st;
+      for (uint32_t it = 0; it < tiles * G; ++it, st.next()) {
+        if (!tc::mbar_wait(full0 + 8 * st.slot, st.round, g.wait_ns)) {
+          give_up(g, 2, s_fail);
+          break;
+        }
+        tc::mbar_arrive_cluster(peer + 8 * st.slot);
+      }
+    }
+    __syncwarp();
+  } else {
+    tc::regs_inc<216>();
+    epilogue<kPairStages, kPairBuffers, 256>(
+        g, tmem, done0, tc::cluster_map(tempty0, 0), s_fail, warp & 3, (warp - 4) >> 2, [&](auto&& tile) {
+          for (int w = pair; w < total; w += pairs)
+            if (!tile((w / tiles_n) * 256 + (int)rank * 128, (w % tiles_n) * 256)) return;
+        });
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::cluster_sync();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc_pair(tmem, 512);
   }
 }
 
@@ -248,6 +453,15 @@ void launch(const CUtensorMap& ta, const CUtensorMap& tb, const Args& g, cudaStr
   const int64_t total = (int64_t)((g.N + BN - 1) / BN) * ((g.M + kBM - 1) / kBM);
   TORCH_CHECK(total < (1ll << 31), "fp8_matmul: too many output tiles");
   fp8_gemm_kernel<BN><<<(int)std::min<int64_t>(total, lm::sm_count()), kThreads, Config<BN>::smem_bytes, st>>>(ta, tb, g);
+  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "fp8_matmul launch failed");
+}
+
+void launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const Args& g, int64_t tiles, cudaStream_t st) {
+  static size_t configured[dynsmem::kMaxDevices] = {};
+  TORCH_CHECK(dynsmem::opt_in(fp8_gemm_pair_kernel, kPairSmem, configured) == cudaSuccess,
+              "fp8_matmul shared-memory attribute");
+  TORCH_CHECK(tiles < (1ll << 31), "fp8_matmul: too many output tiles");
+  fp8_gemm_pair_kernel<<<2 * (int)std::min<int64_t>(tiles, lm::sm_count() / 2), kPairThreads, kPairSmem, st>>>(ta, tb, g);
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "fp8_matmul launch failed");
 }
 
@@ -292,11 +506,13 @@ torch::Tensor matmul(const torch::Tensor& a, const torch::Tensor& a_scale, const
   g.out_kind = out_dtype == torch::kFloat32 ? 0 : (out_dtype == torch::kBFloat16 ? 1 : 2);
   g.status = status.data_ptr<int>();
   g.wait_ns = (uint64_t)wait_ns;
-  constexpr int BN = 128;
   const int64_t one_row = (K + 15) / 16 * 16;   // a single row's stride says nothing
   const CUtensorMap ta = tma::u8_sw128(a.data_ptr(), M, K, M > 1 ? a.stride(0) : one_row, kBM);
-  const CUtensorMap tb = tma::u8_sw128(b.data_ptr(), N, K, N > 1 ? b.stride(0) : one_row, BN);
-  launch<BN>(ta, tb, g, c10::cuda::getCurrentCUDAStream().stream());
+  const CUtensorMap tb = tma::u8_sw128(b.data_ptr(), N, K, N > 1 ? b.stride(0) : one_row, 128);
+  auto st = c10::cuda::getCurrentCUDAStream().stream();
+  const int64_t pair_tiles = ((M + 255) / 256) * ((N + 255) / 256);
+  if (pair_tiles >= lm::sm_count() / 2) launch_pair(ta, tb, g, pair_tiles, st);
+  else launch<128>(ta, tb, g, st);
   lm::count_launches(1);
   return c;
 }

@@ -172,6 +172,15 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo_byte
   return d;
 }
 
+// A descriptor of the same kind from its low word, (leading byte offset >> 4)
+// << 16 | address >> 4, for K-major operands whose 8-row groups are 1024 bytes
+// apart: a step along the operand adds to the low word alone.
+__device__ __forceinline__ uint32_t kmajor_desc_lo(uint32_t saddr) { return (1u << 16) | ((saddr >> 4) & 0x3FFFu); }
+__device__ __forceinline__ uint64_t kmajor_desc(uint32_t lo) {
+  constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+  return (uint64_t)hi << 32 | lo;
+}
+
 // K-major operand, contraction along image columns: 16-wide k-slice `ks` of an
 // image with `rows` rows. The leading byte offset is unused for swizzled
 // K-major layouts; 8-row groups are 1024 bytes apart.
@@ -224,6 +233,61 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint6
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
                :: "r"(bar) : "memory");
+}
+
+// ---- CTA pairs (cta_group::2): two CTAs of a cluster of two work on one 256-row tile ----
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Address of the same shared-memory location in the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t cluster_map(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrive on a barrier of any CTA of the cluster (an address from cluster_map).
+// For handing over what the tensor cores and the TMA unit read and write; with
+// cluster-scope release semantics an arrival takes 320 cycles instead of 16.
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t mapped) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(mapped) : "memory");
+}
+// Whole-warp operations, by one warp of each CTA of the pair.
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+               :: "r"(dst_smem), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish_pair() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(taddr), "r"(ncols) : "memory");
+}
+// Issued by one thread of the pair's first CTA: both CTAs hold 128 rows of A
+// and half of B's rows at the descriptors' offsets, and get 128 rows of D.
+__device__ __forceinline__ void mma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                              bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
+      :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u) : "memory");
+}
+// Arrive on `bar` in both CTAs of the pair once all tcgen05 ops issued so far complete.
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+      :: "r"(bar), "h"((uint16_t)3) : "memory");
+}
+
+template <int N> __device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N));
+}
+template <int N> __device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N));
 }
 
 #endif  // __CUDACC__

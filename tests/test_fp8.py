@@ -188,7 +188,8 @@ def _check_product(y, a, a_s, b, b_s, bias, out):
 
 SHAPES = [(1, 1, 1), (1, 8, 128), (3, 130, 100), (16, 128, 128), (17, 200, 264), (33, 1408, 1000), (64, 64, 2008),
           (128, 128, 4096), (129, 257, 513), (300, 1000, 136), (1, 1408, 16640), (8, 4096, 1024), (1000, 136, 2000),
-          (2500, 1500, 640), (130, 3000, 256), (20000, 300, 384)]
+          (2500, 1500, 640), (130, 3000, 256), (20000, 300, 384),
+          (6000, 900, 1000), (2050, 4100, 520), (5000, 1030, 2000)]
 
 
 @pytest.mark.gpu
@@ -344,7 +345,7 @@ def test_captured_and_replayed_on_a_side_stream():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m", [300, 4])
+@pytest.mark.parametrize("m", [20000, 300, 4])
 def test_a_wait_that_runs_out_is_reported(m):
     dev = torch.device("cuda", 0)
     a, a_s = quantize_rows(_values(m, 4096, 1, device="cuda"))
