@@ -52,6 +52,7 @@ struct Args {
   void* c;
   int64_t ldc;
   int out_kind;           // 0 fp32, 1 bf16, 2 fp16
+  int splits;             // CTAs of a cluster that share one tile's groups (1: none do)
   int* status;
   uint64_t wait_ns;
 };
@@ -162,17 +163,18 @@ __device__ __forceinline__ void store_row(const Args& g, float (&acc)[CHUNKS][32
 
 // An epilogue warp: TMEM lanes 32 q .. + 31 and half of the tile's COLS columns,
 // which lie inside one block of 128 rows of B. `walk` calls tile(first row,
-// first column) for one of the CTA's tiles after the other. `tempty0` may lie
-// in another CTA (a mapped address).
-template <int STAGES, int BUFFERS, int COLS, typename F>
+// first column, first group, last group) for one of the CTA's tiles after the
+// other; sink(sums, row, first column) gets each tile's sums. `tempty0` may
+// lie in another CTA (a mapped address).
+template <int STAGES, int BUFFERS, int COLS, typename F, typename S>
 __device__ __forceinline__ void epilogue(const Args& g, uint32_t tmem, uint32_t done0, uint32_t tempty0, int* s_fail,
-                                         int q, int half, F&& walk) {
+                                         int q, int half, F&& walk, S&& sink) {
   constexpr int kChunks = COLS / 64;   // 32-column chunks per warp
   const int lane = threadIdx.x & 31, G = g.groups;
   const uint32_t lanes = tmem + half * (COLS / 2) + ((uint32_t)(32 * q) << 16);
   Ring<STAGES> st;
   Ring<BUFFERS> buf;
-  walk([&](int m0, int n0) {
+  walk([&](int m0, int n0, int kb0, int kb1) {
     const int row = m0 + 32 * q + lane;
     n0 += half * (COLS / 2);
     float acc[kChunks][32];
@@ -180,10 +182,10 @@ __device__ __forceinline__ void epilogue(const Args& g, uint32_t tmem, uint32_t 
     for (int c = 0; c < kChunks; ++c)
 #pragma unroll
       for (int i = 0; i < 32; ++i) acc[c][i] = 0.f;
-    Scales sc(g.a_scale + (int64_t)min(row, g.M - 1) * G,
-              g.b_scale + (int64_t)min(n0 / kGroup, (g.N - 1) / kGroup) * G, G);
-    for (int kb = 0; kb < G; ++kb) {
-      const float scale = sc.at(kb);
+    Scales sc(g.a_scale + (int64_t)min(row, g.M - 1) * G + kb0,
+              g.b_scale + (int64_t)min(n0 / kGroup, (g.N - 1) / kGroup) * G + kb0, max(kb1 - kb0, 1));
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const float scale = sc.at(kb - kb0);
       const bool got = tc::mbar_wait(done0 + 8 * st.slot, st.round, g.wait_ns);
       if (!__all_sync(0xffffffffu, got)) {   // the loads below are whole-warp
         give_up(g, 4, s_fail);
@@ -198,9 +200,55 @@ __device__ __forceinline__ void epilogue(const Args& g, uint32_t tmem, uint32_t 
       st.next();
       buf.next();
     }
-    if (row < g.M) store_row<kChunks>(g, acc, row, n0);
+    sink(acc, row, n0);
     return true;
   });
+}
+
+// ---- tiles whose groups are shared by a cluster --------------------------------
+// Few tiles leave most SMs idle, so the CTAs of a cluster take a part of one
+// tile's groups each, leave their sums in shared memory, and after a cluster
+// barrier each adds up, in the order of the ranks, an equal part of the rows.
+constexpr int kMaxSplits = 8;
+
+__device__ __forceinline__ float4 load_cluster(uint32_t mapped) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mapped) : "memory");
+  return v;
+}
+
+// Row strides of the sums in shared memory: 16 bytes more than the row, so that
+// the lanes' 16-byte accesses of neighbouring rows fall on different banks.
+__host__ __device__ constexpr int sum_stride(int cols) { return cols + 4; }
+
+template <int CHUNKS>
+__device__ __forceinline__ void keep_sums(float* sums, int stride, const float (&acc)[CHUNKS][32], int row, int col) {
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+      *reinterpret_cast<float4*>(sums + row * stride + col + 32 * c + i) =
+          make_float4(acc[c][i], acc[c][i + 1], acc[c][i + 2], acc[c][i + 3]);
+}
+
+// Sums of four columns of one row over the cluster's CTAs.
+__device__ __forceinline__ float4 cluster_sum(uint32_t sums, int stride, int splits, int row, int col) {
+  const uint32_t at = sums + 4 * (row * stride + col);
+  float4 s = load_cluster(tc::cluster_map(at, 0));
+  for (int r = 1; r < splits; ++r) {
+    const float4 v = load_cluster(tc::cluster_map(at, r));
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  return s;
+}
+
+__device__ __forceinline__ void store_one(const Args& g, int row, int col, float v) {
+  if (g.bias) v += g.bias[col];
+  const int64_t off = (int64_t)row * g.ldc + col;
+  if (g.out_kind == 0) reinterpret_cast<float*>(g.c)[off] = v;
+  else if (g.out_kind == 1) reinterpret_cast<__nv_bfloat16*>(g.c)[off] = __float2bfloat16_rn(v);
+  else reinterpret_cast<__half*>(g.c)[off] = __float2half_rn(v);
 }
 
 // The producer's thread: `walk` calls load(k, row of A, row of B) for one
@@ -322,28 +370,194 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
   tc::tc_fence_after();
   const uint32_t tmem = *s_tmem, smem0 = tc::smem_u32(smem);
 
+  // this CTA's tiles, and its part of their groups
+  const int splits = g.splits, rank = splits > 1 ? (int)tc::cluster_rank() : 0;
+  const int first = blockIdx.x / splits, step = gridDim.x / splits;
+  const int part = (G + splits - 1) / splits, kb0 = min(G, rank * part), kb1 = min(G, kb0 + part);
+  float* sums = reinterpret_cast<float*>(smem);   // the stages, once the one tile of a shared CTA is done
+  constexpr int kStride = sum_stride(BN);
+  static_assert(kBM * kStride * 4 <= C::stages * C::stage_bytes, "the sums take the stages' place");
+
   if (warp == 0 && lane == 0) {
     produce<C::stages>(g, &ta, &tb, smem0, C::stage_bytes, C::a_bytes, full0, done0, s_fail, [&](auto&& load) {
-      for (int w = blockIdx.x; w < total; w += gridDim.x)
-        for (int kb = 0; kb < G; ++kb)
+      for (int w = first; w < total; w += step)
+        for (int kb = kb0; kb < kb1; ++kb)
           if (!load(kb * kGroup, (w / tiles_n) * kBM, (w % tiles_n) * BN)) return;
     });
   } else if (warp == 1 && lane == 0) {
-    const uint32_t tiles = (total - 1 - (int)blockIdx.x) / (int)gridDim.x + 1;   // never more CTAs than tiles
-    multiply<C::stages, C::buffers, BN, false>(g, tiles * G, smem0, C::stage_bytes, C::a_bytes, tmem, full0, 0, done0,
-                                               tempty0, drain, s_fail);
+    const uint32_t tiles = (total - 1 - first) / step + 1;   // never more CTAs than tiles
+    multiply<C::stages, C::buffers, BN, false>(g, tiles * (kb1 - kb0), smem0, C::stage_bytes, C::a_bytes, tmem, full0, 0,
+                                               done0, tempty0, drain, s_fail);
   } else if (warp >= 2) {
     const int q = warp & 3, half = (warp - 2) >> 2;
-    epilogue<C::stages, C::buffers, BN>(g, tmem, done0, tempty0, s_fail, q, half, [&](auto&& tile) {
-      for (int w = blockIdx.x; w < total; w += gridDim.x)
-        if (!tile((w / tiles_n) * kBM, (w % tiles_n) * BN)) return;
-    });
+    epilogue<C::stages, C::buffers, BN>(
+        g, tmem, done0, tempty0, s_fail, q, half,
+        [&](auto&& tile) {
+          for (int w = first; w < total; w += step)
+            if (!tile((w / tiles_n) * kBM, (w % tiles_n) * BN, kb0, kb1)) return;
+        },
+        [&](auto& acc, int row, int n0) {
+          if (splits > 1) keep_sums<BN / 64>(sums, kStride, acc, 32 * q + lane, half * (BN / 2));
+          else if (row < g.M) store_row<BN / 64>(g, acc, row, n0);
+        });
+  }
+  if (splits > 1) {
+    __syncwarp();
+    tc::cluster_sync();
+    const int m0 = (first / tiles_n) * kBM, n0 = (first % tiles_n) * BN, rows = kBM / splits;
+    for (int e = threadIdx.x; e < rows * (BN / 4); e += kThreads) {
+      const int r = rank * rows + e / (BN / 4), c = (e % (BN / 4)) * 4;
+      if (m0 + r >= g.M || n0 + c >= g.N) continue;
+      const float4 v = cluster_sum(smem0, kStride, splits, r, c);
+      store_one(g, m0 + r, n0 + c, v.x);
+      if (n0 + c + 1 < g.N) store_one(g, m0 + r, n0 + c + 1, v.y);
+      if (n0 + c + 2 < g.N) store_one(g, m0 + r, n0 + c + 2, v.z);
+      if (n0 + c + 3 < g.N) store_one(g, m0 + r, n0 + c + 3, v.w);
+    }
+    __syncwarp();
+    tc::cluster_sync();   // the sums stay until every CTA has read them
   }
   tc::tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- few rows --------------------------------------------------------------------
+// Up to 64 rows of A: bound by reading B. The operands change places, 128 rows
+// of B against COLS = 16, 32 or 64 rows of A, so that no tensor work is spent
+// on rows that are not there, and a cluster shares a tile's groups. A thread's
+// sums are one row of B against all rows of A, with a scale for each: the
+// products of the scales of the CTA's groups lie in shared memory.
+//   warp 0  producer, warp 1  products (as above), warps 2-5  epilogue
+constexpr int kRowsThreads = 192, kRowsStages = 8, kRowsBuffers = 4, kRowsScales = 8192;
+template <int COLS> __host__ __device__ constexpr uint32_t rows_stage_bytes() { return kBM * kGroup + COLS * kGroup; }
+template <int COLS> __host__ __device__ constexpr uint32_t rows_smem_bytes() {
+  return kRowsStages * rows_stage_bytes<COLS>() + 1024 + 256 + 4 * kRowsScales;
+}
+
+template <int COLS>
+__global__ void __launch_bounds__(kRowsThreads, 1)
+fp8_gemm_rows_kernel(const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap ta, const Args g) {
+  constexpr uint32_t kStage = rows_stage_bytes<COLS>();
+  constexpr int kStride = sum_stride(COLS), kTmem = kRowsBuffers * COLS;
+  static_assert(kBM * kStride * 4 <= kRowsStages * kStage, "the sums take the stages' place");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* scales = reinterpret_cast<float*>(smem + kRowsStages * kStage);   // [group][COLS]
+  uint8_t* misc = reinterpret_cast<uint8_t*>(scales + kRowsScales);
+  const uint32_t full0 = tc::smem_u32(misc), done0 = full0 + 8 * kRowsStages, tempty0 = done0 + 8 * kRowsStages;
+  const uint32_t drain = tempty0 + 8 * kRowsBuffers;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (2 * kRowsStages + kRowsBuffers + 1));
+  int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = g.groups;
+  const int splits = g.splits, rank = splits > 1 ? (int)tc::cluster_rank() : 0, n0 = (blockIdx.x / splits) * kBM;
+  const int part = (G + splits - 1) / splits, kb0 = min(G, rank * part), kb1 = min(G, kb0 + part);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kRowsStages; ++s) {
+      tc::mbar_init(full0 + 8 * s, 1);
+      tc::mbar_init(done0 + 8 * s, 1);
+    }
+    for (int b = 0; b < kRowsBuffers; ++b) tc::mbar_init(tempty0 + 8 * b, 4);
+    tc::mbar_init(drain, 1);
+    tc::mbar_init_fence();
+    *s_fail = 0;
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tc::smem_u32(s_tmem), kTmem);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *s_tmem, smem0 = tc::smem_u32(smem);
+  float* sums = reinterpret_cast<float*>(smem);
+
+  if (warp == 0 && lane == 0) {
+    produce<kRowsStages>(g, &tb, &ta, smem0, kStage, kBM * kGroup, full0, done0, s_fail, [&](auto&& load) {
+      for (int kb = kb0; kb < kb1; ++kb)
+        if (!load(kb * kGroup, n0, 0)) return;
+    });
+  } else if (warp == 1 && lane == 0) {
+    multiply<kRowsStages, kRowsBuffers, COLS, false>(g, kb1 - kb0, smem0, kStage, kBM * kGroup, tmem, full0, 0, done0,
+                                                     tempty0, drain, s_fail);
+  } else if (warp >= 2) {
+    const int q = warp & 3;
+    const float* bs = g.b_scale + (int64_t)(n0 / kGroup) * G;
+    for (int e = threadIdx.x - 64; e < (kb1 - kb0) * COLS; e += 128) {
+      // neighbouring threads read neighbouring groups of one row
+      const int j = e / (kb1 - kb0), kb = kb0 + e - j * (kb1 - kb0);
+      scales[(kb - kb0) * COLS + j] = j < g.M ? g.a_scale[(int64_t)j * G + kb] * bs[kb] : 0.f;
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");   // the four epilogue warps
+    float acc[COLS / 16][16];
+#pragma unroll
+    for (int c = 0; c < COLS / 16; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[c][i] = 0.f;
+    Ring<kRowsStages> st;
+    Ring<kRowsBuffers> buf;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const bool got = tc::mbar_wait(done0 + 8 * st.slot, st.round, g.wait_ns);
+      if (!__all_sync(0xffffffffu, got)) {
+        give_up(g, 4, s_fail);
+        break;
+      }
+      tc::tc_fence_after();
+      const uint32_t base = tmem + buf.slot * COLS + ((uint32_t)(32 * q) << 16);
+      const float4* sc = reinterpret_cast<const float4*>(scales + (kb - kb0) * COLS);
+      float v[COLS / 16][16];
+#pragma unroll
+      for (int c = 0; c < COLS / 16; ++c) tc::tmem_ld16_issue(base + 16 * c, v[c]);
+      tc::tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < COLS / 16; ++c) tc::tmem_regs_ready16(v[c]);
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(tempty0 + 8 * buf.slot);
+#pragma unroll
+      for (int c = 0; c < COLS / 16; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const float4 f = sc[c * 4 + i / 4];
+          acc[c][i] = fmaf(v[c][i], f.x, acc[c][i]);
+          acc[c][i + 1] = fmaf(v[c][i + 1], f.y, acc[c][i + 1]);
+          acc[c][i + 2] = fmaf(v[c][i + 2], f.z, acc[c][i + 2]);
+          acc[c][i + 3] = fmaf(v[c][i + 3], f.w, acc[c][i + 3]);
+        }
+      st.next();
+      buf.next();
+    }
+    // every stage is read by now: the sums take the stages' place
+#pragma unroll
+    for (int c = 0; c < COLS / 16; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4*>(sums + (32 * q + lane) * kStride + 16 * c + i) =
+            make_float4(acc[c][i], acc[c][i + 1], acc[c][i + 2], acc[c][i + 3]);
+  }
+  __syncwarp();
+  tc::cluster_sync();
+  const int rows = kBM / splits, quads = (min(g.M, COLS) + 3) / 4;
+  for (int e = threadIdx.x; e < rows * quads; e += kRowsThreads) {
+    const int r = rank * rows + e % rows, m = (e / rows) * 4;   // neighbouring threads: neighbouring columns of C
+    if (n0 + r >= g.N) continue;
+    const float4 v = cluster_sum(smem0, kStride, splits, r, m);
+    store_one(g, m, n0 + r, v.x);
+    if (m + 1 < g.M) store_one(g, m + 1, n0 + r, v.y);
+    if (m + 2 < g.M) store_one(g, m + 2, n0 + r, v.z);
+    if (m + 3 < g.M) store_one(g, m + 3, n0 + r, v.w);
+  }
+  __syncwarp();
+  tc::tc_fence_before();
+  tc::cluster_sync();   // the sums stay until every CTA has read them
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, kTmem);
   }
 }
 
@@ -433,7 +647,10 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_consta
     epilogue<kPairStages, kPairBuffers, 256>(
         g, tmem, done0, tc::cluster_map(tempty0, 0), s_fail, warp & 3, (warp - 4) >> 2, [&](auto&& tile) {
           for (int w = pair; w < total; w += pairs)
-            if (!tile((w / tiles_n) * 256 + (int)rank * 128, (w % tiles_n) * 256)) return;
+            if (!tile((w / tiles_n) * 256 + (int)rank * 128, (w % tiles_n) * 256, 0, G)) return;
+        },
+        [&](auto& acc, int row, int n0) {
+          if (row < g.M) store_row<4>(g, acc, row, n0);
         });
   }
   tc::tc_fence_before();
@@ -445,15 +662,51 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_consta
   }
 }
 
+// CTAs that share a tile: enough to give most SMs one, a power of two that
+// divides a tile's rows, and a part of at least two groups each.
+int splits_for(int64_t tiles, int groups) {
+  int s = 1;
+  while (s < kMaxSplits && tiles * s * 2 <= lm::sm_count() + lm::sm_count() / 4 && groups >= 4 * s) s *= 2;
+  return s;
+}
+
+template <typename K, typename... A>
+void launch_cluster(K* kernel, int grid, int threads, size_t smem, int cluster, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  TORCH_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess, "fp8_matmul launch failed");
+}
+
 template <int BN>
-void launch(const CUtensorMap& ta, const CUtensorMap& tb, const Args& g, cudaStream_t st) {
+void launch(const CUtensorMap& ta, const CUtensorMap& tb, Args g, cudaStream_t st) {
   static size_t configured[dynsmem::kMaxDevices] = {};
   TORCH_CHECK(dynsmem::opt_in(fp8_gemm_kernel<BN>, Config<BN>::smem_bytes, configured) == cudaSuccess,
               "fp8_matmul shared-memory attribute");
-  const int64_t total = (int64_t)((g.N + BN - 1) / BN) * ((g.M + kBM - 1) / kBM);
-  TORCH_CHECK(total < (1ll << 31), "fp8_matmul: too many output tiles");
-  fp8_gemm_kernel<BN><<<(int)std::min<int64_t>(total, lm::sm_count()), kThreads, Config<BN>::smem_bytes, st>>>(ta, tb, g);
-  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "fp8_matmul launch failed");
+  const int64_t tiles = (int64_t)((g.N + BN - 1) / BN) * ((g.M + kBM - 1) / kBM);
+  TORCH_CHECK(tiles < (1ll << 31), "fp8_matmul: too many output tiles");
+  g.splits = splits_for(tiles, g.groups);
+  const int grid = g.splits > 1 ? (int)tiles * g.splits : (int)std::min<int64_t>(tiles, lm::sm_count());
+  launch_cluster(fp8_gemm_kernel<BN>, grid, kThreads, Config<BN>::smem_bytes, g.splits, st, ta, tb, g);
+}
+
+template <int COLS>
+void launch_rows(const CUtensorMap& tb, const torch::Tensor& a, int64_t lda, Args g, int splits, cudaStream_t st) {
+  static size_t configured[dynsmem::kMaxDevices] = {};
+  TORCH_CHECK(dynsmem::opt_in(fp8_gemm_rows_kernel<COLS>, rows_smem_bytes<COLS>(), configured) == cudaSuccess,
+              "fp8_matmul shared-memory attribute");
+  g.splits = splits;
+  const CUtensorMap ta = tma::u8_sw128(a.data_ptr(), a.size(0), a.size(1), lda, COLS);
+  launch_cluster(fp8_gemm_rows_kernel<COLS>, (g.N + kBM - 1) / kBM * splits, kRowsThreads, rows_smem_bytes<COLS>(), splits,
+                 st, tb, ta, g);
 }
 
 void launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const Args& g, int64_t tiles, cudaStream_t st) {
@@ -507,12 +760,20 @@ torch::Tensor matmul(const torch::Tensor& a, const torch::Tensor& a_scale, const
   g.status = status.data_ptr<int>();
   g.wait_ns = (uint64_t)wait_ns;
   const int64_t one_row = (K + 15) / 16 * 16;   // a single row's stride says nothing
-  const CUtensorMap ta = tma::u8_sw128(a.data_ptr(), M, K, M > 1 ? a.stride(0) : one_row, kBM);
+  const int64_t lda = M > 1 ? a.stride(0) : one_row;
   const CUtensorMap tb = tma::u8_sw128(b.data_ptr(), N, K, N > 1 ? b.stride(0) : one_row, 128);
   auto st = c10::cuda::getCurrentCUDAStream().stream();
-  const int64_t pair_tiles = ((M + 255) / 256) * ((N + 255) / 256);
-  if (pair_tiles >= lm::sm_count() / 2) launch_pair(ta, tb, g, pair_tiles, st);
-  else launch<128>(ta, tb, g, st);
+  const int cols = M <= 16 ? 16 : (M <= 32 ? 32 : 64), splits = splits_for((N + kBM - 1) / kBM, g.groups);
+  if (M <= 64 && (g.groups + splits - 1) / splits * cols <= kRowsScales) {
+    if (cols == 16) launch_rows<16>(tb, a, lda, g, splits, st);
+    else if (cols == 32) launch_rows<32>(tb, a, lda, g, splits, st);
+    else launch_rows<64>(tb, a, lda, g, splits, st);
+  } else {
+    const CUtensorMap ta = tma::u8_sw128(a.data_ptr(), M, K, lda, kBM);
+    const int64_t pair_tiles = ((M + 255) / 256) * ((N + 255) / 256);
+    if (pair_tiles >= lm::sm_count() / 2) launch_pair(ta, tb, g, pair_tiles, st);
+    else launch<128>(ta, tb, g, st);
+  }
   lm::count_launches(1);
   return c;
 }

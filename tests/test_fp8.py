@@ -189,7 +189,8 @@ def _check_product(y, a, a_s, b, b_s, bias, out):
 SHAPES = [(1, 1, 1), (1, 8, 128), (3, 130, 100), (16, 128, 128), (17, 200, 264), (33, 1408, 1000), (64, 64, 2008),
           (128, 128, 4096), (129, 257, 513), (300, 1000, 136), (1, 1408, 16640), (8, 4096, 1024), (1000, 136, 2000),
           (2500, 1500, 640), (130, 3000, 256), (20000, 300, 384),
-          (6000, 900, 1000), (2050, 4100, 520), (5000, 1030, 2000)]
+          (6000, 900, 1000), (2050, 4100, 520), (5000, 1030, 2000),
+          (64, 130, 5000), (65, 300, 5000), (31, 20000, 300), (7, 128, 100000), (60, 100, 40000)]
 
 
 @pytest.mark.gpu
