@@ -69,7 +69,7 @@ quant_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int c = grp * 128 + e * 16 + sub;
-        if (c < k) out[c] = (uint8_t)(lm::e4m3x2(lm::quotient_to_odd(v[e], dv), 0.f) & 0xff);
+        if (c < k) out[c] = (uint8_t)(lm::e4m3x2(lm::e4m3_quotient(v[e], dv), 0.f) & 0xff);
       }
     }
     if (sub == 0) scale[g] = s;
@@ -115,7 +115,7 @@ quant_blocks_kernel(const T* __restrict__ w, int64_t ldw, uint8_t* __restrict__ 
   for (int i = 0; i < 16; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      tile[i * 8 + warp][j * 32 + lane] = (uint8_t)(lm::e4m3x2(lm::quotient_to_odd(v[i][j], dv), 0.f) & 0xff);
+      tile[i * 8 + warp][j * 32 + lane] = (uint8_t)(lm::e4m3x2(lm::e4m3_quotient(v[i][j], dv), 0.f) & 0xff);
   __syncthreads();
   // four columns per thread and store; the last store of a row may run into its padding (rows are 16 bytes apart)
   for (int e = threadIdx.x; e < 128 * 32; e += 256) {

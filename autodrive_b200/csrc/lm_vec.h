@@ -60,24 +60,32 @@ __device__ __forceinline__ int slice_col(int chunk, int lane, int e) {
   return chunk * 256 + (VEC ? lane * 8 + e : e * 32 + lane);
 }
 
+// A slice as it lies in memory, to be loaded a row ahead.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_slice(const T* row, int chunk, int lane, int d, float (&v)[8]) {
-  if constexpr (VEC) {
-    const int c = slice_col<true>(chunk, lane, 0);
-    if (c < d) {
-      load8(row + c, v);
+struct RawSlice {
+  alignas(16) T e[8];
+  __device__ __forceinline__ void load(const T* row, int chunk, int lane, int d) {
+    if constexpr (VEC) {
+      constexpr int kVectors = sizeof(T) * 8 / 16;
+      const int c = slice_col<true>(chunk, lane, 0);
+      uint4* u = reinterpret_cast<uint4*>(e);
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j)
+        u[j] = c < d ? reinterpret_cast<const uint4*>(row + c)[j] : make_uint4(0, 0, 0, 0);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = slice_col<false>(chunk, lane, e);
-      v[e] = c < d ? to_f<T>(row[c]) : 0.f;
+      for (int i = 0; i < 8; ++i) {
+        const int c = slice_col<false>(chunk, lane, i);
+        e[i] = from_f<T>(0.f);
+        if (c < d) e[i] = row[c];
+      }
     }
   }
-}
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f<T>(e[i]);
+  }
+};
 
 template <typename T, bool VEC>
 __device__ __forceinline__ void store_slice(T* row, int chunk, int lane, int d, const float (&v)[8]) {
@@ -115,22 +123,26 @@ __device__ __forceinline__ float group_scale(uint32_t amax_bits) {
 }
 
 // x / scale rounded to e4m3 once. A quotient rounded to fp32 first can land
-// on the middle between two e4m3 numbers and then be rounded to the wrong
-// one, so it is rounded to odd instead: truncated, with the last bit set when
-// the remainder is not zero (Boldo & Melquiond, "When double rounding is
-// odd", 2005); the conversion that follows then rounds as if from the exact
-// quotient. The remainder of the quotient's correction step is exact in an
-// fma. `lift` (a power of two) keeps it out of the subnormal range for tiny
-// scales. Written without the flush-to-zero that the compiler's fast-math
-// mode adds, so subnormal inputs keep their value.
+// on the middle between two e4m3 numbers, or on its wrong side, and then be
+// rounded to the wrong one. x times the rounded reciprocal is within two units
+// in the last place, so only values within four of a middle (the last 20 bits
+// tell, among e4m3's normal numbers) and those below them take the exact way:
+// there the quotient is rounded to odd (truncated, with the last bit set when
+// the remainder is not zero; Boldo & Melquiond, "When double rounding is odd",
+// 2005), from which the conversion rounds as if from the exact quotient. The
+// remainder of the quotient's correction step is exact in an fma; `lift` (a
+// power of two) keeps it out of the subnormal range for tiny scales. Written
+// without the flush-to-zero that the compiler's fast-math mode adds, so
+// subnormal inputs keep their value.
 struct Divisor {
-  float scale, inv, lift;
+  float scale, inv, lift, direct;   // scale and 1 / scale, lifted; 1 / scale
 };
 __device__ __forceinline__ Divisor divisor(float scale) {
   Divisor d;
   d.lift = scale < 0x1p-60f ? 0x1p64f : 1.f;
   d.scale = scale * d.lift;
   d.inv = __frcp_rn(d.scale);
+  d.direct = scale < __uint_as_float(0x7f800000u) ? d.inv * d.lift : __uint_as_float(0x7fffffffu);   // inf, NaN: NaN
   return d;
 }
 __device__ __forceinline__ float mul_nf(float a, float b) {
@@ -144,7 +156,8 @@ __device__ __forceinline__ float fma_nf(float a, float b, float c) {
   return r;
 }
 __device__ __forceinline__ float quotient_to_odd(float x, const Divisor& d) {
-  const float y = mul_nf(x, d.lift);
+  float y;
+  asm volatile("mul.rn.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(d.lift));   // volatile: a branch, not computed for all
   const float q0 = mul_nf(y, d.inv);
   const float q = fma_nf(fma_nf(-q0, d.scale, y), d.inv, q0);
   const float rem = fma_nf(-q, d.scale, y);                  // exact; its sign says on which side q lies
@@ -156,6 +169,14 @@ __device__ __forceinline__ float quotient_to_odd(float x, const Divisor& d) {
   }
   return __uint_as_float(b);
 }
+// A number that converts to e4m3 as the exact quotient would.
+__device__ __forceinline__ float e4m3_quotient(float x, const Divisor& d) {
+  const float q = mul_nf(x, d.direct);
+  const uint32_t u = __float_as_uint(q);
+  const bool middle = (u & 0xfffffu) - 0x7fffcu <= 8u;
+  const bool below = (u << 1) - 1u < (0x3c800000u << 1) - 1u;   // 0 < |q| < 2^-6
+  return middle || below ? quotient_to_odd(x, d) : q;
+}
 __device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
@@ -165,7 +186,7 @@ __device__ __forceinline__ uint2 quantize8(const float (&v)[8], const Divisor& d
   uint32_t h[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    h[i] = e4m3x2(quotient_to_odd(v[2 * i], d), quotient_to_odd(v[2 * i + 1], d));
+    h[i] = e4m3x2(e4m3_quotient(v[2 * i], d), e4m3_quotient(v[2 * i + 1], d));
   return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 

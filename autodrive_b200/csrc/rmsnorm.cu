@@ -13,15 +13,17 @@
 // Bound by memory: every element is read and written once. A row is held in
 // registers between the sum and the scaling, by as many threads as give each
 // about 16 elements (32 lanes up to 512 columns, 1024 threads from 8193 on);
-// CTAs are persistent, so that the weight is loaded once for many rows and
-// the backward sums the weight's gradient in registers, one partial row for
-// each CTA, added up in a fixed order by a second kernel.
+// CTAs are persistent, so that the weight is loaded once for many rows, the
+// next row's loads are in flight while a row is worked on, and the backward
+// sums the weight's gradient in registers, one partial row for each CTA, added
+// up in a fixed order by a second kernel.
 #include <torch/extension.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -96,24 +98,42 @@ rms_fwd_kernel(const FwdArgs a) {
       const int c = lm::slice_col<VEC>(i * W + part, lane, e);
       w[i][e] = c < a.d ? a.w.at(c) : 0.f;
     }
+  // the next row is loaded while this one is worked on
+  lm::RawSlice<T, VEC> next_x[NV], next_r[NV];
+  const auto load = [&](int64_t r) {
+    if (r >= a.rows) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) next_x[i].load(x + r * a.ldx, i * W + part, lane, a.d);
+    if (res) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) next_r[i].load(res + r * a.ldres, i * W + part, lane, a.d);
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  load((int64_t)blockIdx.x * RPB + threadIdx.x / TPR);
   int buf = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB, buf ^= 1) {
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += step, buf ^= 1) {
     const int64_t r = r0 + threadIdx.x / TPR;
     const bool live = r < a.rows;
     float v[NV][8];
     float s = 0.f;
     if (live) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) lm::load_slice<T, VEC>(x + r * a.ldx, i * W + part, lane, a.d, v[i]);
+      for (int i = 0; i < NV; ++i) next_x[i].get(v[i]);
       if (res) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           float u[8];
-          lm::load_slice<T, VEC>(res + r * a.ldres, i * W + part, lane, a.d, u);
+          next_r[i].get(u);
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[i][e] = lm::to_f<T>(lm::from_f<T>(v[i][e] + u[e]));
-          lm::store_slice<T, VEC>(reinterpret_cast<T*>(a.h) + r * a.d, i * W + part, lane, a.d, v[i]);
         }
+      }
+      load(r + step);
+      if (res) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          lm::store_slice<T, VEC>(reinterpret_cast<T*>(a.h) + r * a.d, i * W + part, lane, a.d, v[i]);
       }
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -163,7 +183,7 @@ rms_fwd_kernel(const FwdArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int c = lm::slice_col<false>(chunk, lane, 4 * g + e);
-              if (c < a.d) q[c] = (uint8_t)(lm::e4m3x2(lm::quotient_to_odd(v[i][4 * g + e], dv), 0.f) & 0xff);
+              if (c < a.d) q[c] = (uint8_t)(lm::e4m3x2(lm::e4m3_quotient(v[i][4 * g + e], dv), 0.f) & 0xff);
             }
             if (lane == 0) sc[g] = gs;
           }
@@ -201,19 +221,35 @@ rms_bwd_kernel(const BwdArgs a) {
       w[i][e] = c < a.d ? a.w.at(c) : 0.f;
       dw[i][e] = 0.f;
     }
+  lm::RawSlice<T, VEC> next_g[NV], next_h[NV], next_u[NV];
+  float next_rstd = 0.f;
+  const auto load = [&](int64_t r) {
+    if (r >= a.rows) return;
+    next_rstd = a.rstd[r];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      next_g[i].load(reinterpret_cast<const T*>(a.dy) + r * a.d, i * W + part, lane, a.d);
+      next_h[i].load(reinterpret_cast<const T*>(a.h) + r * a.ldh, i * W + part, lane, a.d);
+    }
+    if (a.dh_out) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) next_u[i].load(reinterpret_cast<const T*>(a.dh_out) + r * a.d, i * W + part, lane, a.d);
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  load((int64_t)blockIdx.x * RPB + threadIdx.x / TPR);
   int buf = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB, buf ^= 1) {
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += step, buf ^= 1) {
     const int64_t r = r0 + threadIdx.x / TPR;
     const bool live = r < a.rows;
     float g[NV][8], n[NV][8];
+    lm::RawSlice<T, VEC> u[NV];
     float s = 0.f, rstd = 0.f;
     if (live) {
-      rstd = a.rstd[r];
+      rstd = next_rstd;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        lm::load_slice<T, VEC>(reinterpret_cast<const T*>(a.dy) + r * a.d, i * W + part, lane, a.d, g[i]);
-        lm::load_slice<T, VEC>(reinterpret_cast<const T*>(a.h) + r * a.ldh, i * W + part, lane, a.d, n[i]);
-      }
+      for (int i = 0; i < NV; ++i) next_g[i].get(g[i]), next_h[i].get(n[i]), u[i] = next_u[i];
+      load(r + step);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -231,10 +267,10 @@ rms_bwd_kernel(const BwdArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) g[i][e] = rstd * (g[i][e] - n[i][e] * s);
       if (a.dh_out) {
-        float u[8];
-        lm::load_slice<T, VEC>(reinterpret_cast<const T*>(a.dh_out) + r * a.d, i * W + part, lane, a.d, u);
+        float f[8];
+        u[i].get(f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[i][e] += u[e];
+        for (int e = 0; e < 8; ++e) g[i][e] += f[e];
       }
       lm::store_slice<T, VEC>(reinterpret_cast<T*>(a.dx) + r * a.d, i * W + part, lane, a.d, g[i]);
     }
@@ -272,8 +308,10 @@ __global__ void __launch_bounds__(1024) rms_dw_kernel(const float* part, int par
   __shared__ float red[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
   float s = 0.f;
-  if (c < d)
+  if (c < d) {
+#pragma unroll 8
     for (int p = threadIdx.y; p < parts; p += 32) s += part[(int64_t)p * d + c];
+  }
   red[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   s = lm::warp_sum(red[threadIdx.x][threadIdx.y]);
@@ -281,11 +319,22 @@ __global__ void __launch_bounds__(1024) rms_dw_kernel(const float* part, int par
   if (threadIdx.x == 0 && col < d) dw[col] = lm::from_f<W>(s);
 }
 
-// Persistent CTAs: as many as fit on the SMs at once (2048 threads each).
-int grid_for(int64_t rows, int tpr) {
-  const int rpb = rows_per_cta(tpr), threads = tpr * rpb;
-  const int64_t want = (rows + rpb - 1) / rpb;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)lm::sm_count() * std::max(1, 1024 / threads)));
+// Persistent CTAs: as many as fit on the SMs at once, so that none waits for a
+// second round.
+template <typename T, auto... V, typename K>
+int grid_for(K* kernel, int64_t rows, int tpr) {
+  static std::atomic<int> fits[64];   // one array for each kernel: T and V are its template arguments
+  const int rpb = rows_per_cta(tpr);
+  int dev = 0;
+  TORCH_CHECK(cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64, "rms_norm: device query failed");
+  int n = fits[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    TORCH_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, tpr * rpb, 0) == cudaSuccess,
+                "rms_norm: occupancy query failed");
+    n = std::max(1, n);
+    fits[dev].store(n, std::memory_order_relaxed);
+  }
+  return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rpb - 1) / rpb, (int64_t)lm::sm_count() * n));
 }
 
 // Threads and 256-column chunks per row (see the file's comment).
@@ -388,11 +437,15 @@ Forward forward(const torch::Tensor& x, const torch::Tensor& residual, const tor
     using T = decltype(t);
     for_width(d, [&](auto tpr, auto nv) {
       constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
-      const int grid = grid_for(rows, TPR), threads = TPR * rows_per_cta(TPR);
-      if (vec && fp8) rms_fwd_kernel<T, true, true, TPR, NV><<<grid, threads, 0, st>>>(a);
-      else if (vec) rms_fwd_kernel<T, true, false, TPR, NV><<<grid, threads, 0, st>>>(a);
-      else if (fp8) rms_fwd_kernel<T, false, true, TPR, NV><<<grid, threads, 0, st>>>(a);
-      else rms_fwd_kernel<T, false, false, TPR, NV><<<grid, threads, 0, st>>>(a);
+      const auto launch = [&](auto v8, auto q8) {
+        constexpr bool VEC = decltype(v8)::value, FP8 = decltype(q8)::value;
+        const int grid = grid_for<T, VEC, FP8, TPR, NV>(rms_fwd_kernel<T, VEC, FP8, TPR, NV>, rows, TPR);
+        rms_fwd_kernel<T, VEC, FP8, TPR, NV><<<grid, TPR * rows_per_cta(TPR), 0, st>>>(a);
+      };
+      if (vec && fp8) launch(std::true_type{}, std::true_type{});
+      else if (vec) launch(std::true_type{}, std::false_type{});
+      else if (fp8) launch(std::false_type{}, std::true_type{});
+      else launch(std::false_type{}, std::false_type{});
     });
   });
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "rms_norm forward launch failed");
@@ -429,12 +482,15 @@ std::pair<torch::Tensor, torch::Tensor> backward(const torch::Tensor& dy, const 
     using T = decltype(t);
     for_width(d, [&](auto tpr, auto nv) {
       constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
-      grid = grid_for(rows, TPR);
-      part = torch::empty({grid, d}, h.options().dtype(torch::kFloat32));
-      a.part = part.data_ptr<float>();
-      const int threads = TPR * rows_per_cta(TPR);
-      if (vec) rms_bwd_kernel<T, true, TPR, NV><<<grid, threads, 0, st>>>(a);
-      else rms_bwd_kernel<T, false, TPR, NV><<<grid, threads, 0, st>>>(a);
+      const auto launch = [&](auto v8) {
+        constexpr bool VEC = decltype(v8)::value;
+        grid = grid_for<T, VEC, TPR, NV>(rms_bwd_kernel<T, VEC, TPR, NV>, rows, TPR);
+        part = torch::empty({grid, d}, h.options().dtype(torch::kFloat32));
+        a.part = part.data_ptr<float>();
+        rms_bwd_kernel<T, VEC, TPR, NV><<<grid, TPR * rows_per_cta(TPR), 0, st>>>(a);
+      };
+      if (vec) launch(std::true_type{});
+      else launch(std::false_type{});
     });
   });
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "rms_norm backward launch failed");

@@ -21,7 +21,8 @@
 // looked at again, and the entries that reach it are ranked.
 //
 // Bound by memory for long rows. Rows of up to 1024 entries are held in the
-// registers of one warp or of a part of one; longer ones take a CTA each.
+// registers of one warp or of a part of one; longer ones take a CTA each, or a
+// cluster of CTAs where there are few rows.
 #include <torch/extension.h>
 #include <ATen/ExpandUtils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -42,7 +43,9 @@ namespace {
 
 constexpr int kMaxTop = 64;
 constexpr int kSmall = 1024;        // longest row held in one warp's registers
-constexpr int kThreads = 512;       // threads of a long row's CTA
+constexpr int kThreads = 256;       // threads of a long row's CTA
+constexpr int kAhead = 4;           // vectors of eight that a thread loads before it uses the first
+constexpr int kMaxSplits = 8;       // CTAs of a cluster that share a row
 constexpr int kCandidates = 1024;   // entries ranked in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -53,6 +56,7 @@ struct Args {
   int64_t rows, ldx, ldm;
   int v, top;
   float inv_t;             // 1 / T
+  int splits;              // CTAs that share a long row
   float* log_prob;
   float* entropy;
   float* top_value;        // [rows][top]
@@ -80,12 +84,14 @@ __device__ __forceinline__ Stat joined(const Stat& a, const Stat& b, float c) {
   const Stat p = rescaled(a, m, c), q = rescaled(b, m, c);
   return Stat{m, p.s + q.s, p.t + q.t};
 }
-// Adds an entry that is at most st.m.
+// Adds an entry that is at most st.m. The difference is kept finite, so that an
+// entry without weight adds 0 times a number; NaN passes through.
 __device__ __forceinline__ void add_entry(Stat& st, float x, float c) {
-  const float d = x - st.m;
+  float d = x - st.m;
+  asm("max.NaN.f32 %0, %0, 0fFF000000;" : "+f"(d));   // -2^127
   const float e = exp2f(d * c);
   st.s += e;
-  if (e != 0.f) st.t += e * d;   // not 0 * -inf
+  st.t = fmaf(e, d, st.t);
 }
 
 template <int G>
@@ -295,39 +301,86 @@ struct RowView {
   }
 };
 
+// One vector's entries into the running sums.
+__device__ __forceinline__ void add_vector(Stat& st, int& first, int i, uint32_t ok, float (&x)[8], float c) {
+  if (ok != 0xff) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (!(ok >> e & 1)) x[e] = -INFINITY;
+  }
+  float m = x[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) m = fmaxf(m, x[e]);
+  if (m > st.m) {
+    st = rescaled(st, m, c);
+    first = i;
+  }
+  if (st.m != -INFINITY) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) add_entry(st, x[e], c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (x[e] != x[e]) st.s = x[e];   // NaN and nothing else so far: the row is NaN
+  }
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same shared variable in the cluster's CTA `rank`.
+template <typename V>
+__device__ __forceinline__ const V* cluster_peer(const V* p, int rank) {
+  uint64_t r;
+  asm volatile("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"(p), "r"(rank));
+  return reinterpret_cast<const V*>(r);
+}
+
+// The `top` largest of `count` different keys, in order, into out (0: none).
+__device__ __forceinline__ void rank_keys(const uint64_t* keys, int count, int top, uint64_t* out) {
+  for (int i = threadIdx.x; i < count; i += kThreads) {
+    const uint64_t key = keys[i];
+    if (!key) continue;
+    int place = 0;   // the number of keys above it
+    for (int j = 0; j < count; ++j) place += keys[j] > key;
+    if (place < top) out[place] = key;
+  }
+}
+
+// A cluster of a.splits CTAs takes one row, each CTA an equal part of its vectors.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) long_fwd_kernel(const Args a) {
   constexpr int W = kThreads / 32;
-  __shared__ Stat red[W];
+  __shared__ Stat red[W], part_s;
   __shared__ uint64_t keys[kThreads], cand[kCandidates], found[kMaxTop];
   __shared__ uint64_t bound_s;
   __shared__ int count_s;
-  const int64_t r = blockIdx.x;
+  const int64_t r = blockIdx.x / a.splits;
+  const int rank = a.splits > 1 ? (int)cluster_rank() : 0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float c = a.inv_t * kLog2e;
   const RowView<T> view(a, r);
+  const int share = (view.vectors + a.splits - 1) / a.splits, i0 = rank * share, i1 = min(view.vectors, i0 + share);
   Stat st = empty_stat();
   int first = 0;   // the vector in which this thread's maximum was first met
-  for (int i = threadIdx.x; i < view.vectors; i += kThreads) {
+  int i = i0 + threadIdx.x;
+  for (; i + (kAhead - 1) * kThreads < i1; i += kAhead * kThreads) {
+    float x[kAhead][8];
+    uint32_t ok[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) ok[j] = view.load(i + j * kThreads, x[j]);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) add_vector(st, first, i + j * kThreads, ok[j], x[j], c);
+  }
+  for (; i < i1; i += kThreads) {
     float x[8];
     const uint32_t ok = view.load(i, x);
-    float m = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (!(ok >> e & 1)) x[e] = -INFINITY;
-      m = fmaxf(m, x[e]);
-    }
-    if (m > st.m) {
-      st = rescaled(st, m, c);
-      first = i;
-    }
-    if (st.m != -INFINITY) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) add_entry(st, x[e], c);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (x[e] != x[e]) st.s = x[e];   // a NaN makes the row NaN
+    add_vector(st, first, i, ok, x, c);
   }
   // NaN alone: any finite maximum carries it through the joining
   const bool nan_only = st.m == -INFINITY && st.s != st.s;
@@ -337,11 +390,99 @@ __global__ void __launch_bounds__(kThreads) long_fwd_kernel(const Args a) {
   if (a.top) {
     keys[threadIdx.x] = st.m == -INFINITY ? 0 : entry_key(st.m, first);
     if (threadIdx.x == 0) count_s = 0;
+    for (int k = threadIdx.x; k < a.top; k += kThreads) found[k] = 0;
   }
   __syncthreads();
   Stat all = red[0];
 #pragma unroll
   for (int w = 1; w < W; ++w) all = joined(all, red[w], c);
+  if (a.top) {
+    // the top-th largest of the threads' maxima, by the first warp
+    if (warp == 0) {
+      uint64_t k[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) k[j] = keys[j * 32 + lane];
+      uint64_t best = 0;
+      for (int n = 0; n < a.top; ++n) {
+        uint64_t own = 0;
+#pragma unroll
+        for (int j = 0; j < W; ++j) own = k[j] > own ? k[j] : own;
+        best = group_max<32>(own);
+        if (!best) break;
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+          if (k[j] == best) k[j] = 0;
+      }
+      if (lane == 0) bound_s = best;   // 0: fewer than `top` threads have an entry, so every entry counts
+    }
+    __syncthreads();
+    const uint64_t bound = bound_s;
+    // entries at or above the bound: a larger value, or the same value in no later vector
+    for (int owner = warp; owner < kThreads; owner += W) {
+      if (keys[owner] == 0 || keys[owner] < bound) continue;
+      for (int v = i0 + owner + lane * kThreads; v < i1; v += kThreads * 32) {
+        float x[8];
+        const uint32_t ok = view.load(v, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (!(ok >> e & 1) || !ranked(x[e])) continue;
+          if (entry_key(x[e], v) < bound) continue;
+          const int at = atomicAdd(&count_s, 1);
+          if (at < kCandidates) cand[at] = entry_key(x[e], 8 * v - view.shift + e);
+        }
+      }
+    }
+    __syncthreads();
+    const int count = count_s;
+    if (count <= kCandidates) {
+      rank_keys(cand, count, a.top, found);
+    } else {
+      // too many for shared memory (many equal or clustered maxima): one pass over the row for each place
+      uint64_t last = ~0ull;
+      for (int n = 0; n < a.top; ++n) {
+        uint64_t best = 0;
+        for (int v = i0 + threadIdx.x; v < i1; v += kThreads) {
+          float x[8];
+          const uint32_t ok = view.load(v, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (!(ok >> e & 1) || !ranked(x[e])) continue;
+            const uint64_t key = entry_key(x[e], 8 * v - view.shift + e);
+            if (key < last && key > best) best = key;
+          }
+        }
+        best = group_max<32>(best);
+        __syncthreads();
+        if (lane == 0) cand[warp] = best;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) best = cand[w] > best ? cand[w] : best;
+        last = best;
+        if (threadIdx.x == 0) found[n] = best;
+      }
+    }
+  }
+  const uint64_t* list = found;
+  if (a.splits > 1) {
+    if (threadIdx.x == 0) part_s = all;
+    __syncthreads();
+    cluster_sync();
+    if (rank == 0) {
+      // join the parts in the order of the ranks, and rank their lists once more
+      for (int p = 1; p < a.splits; ++p) all = joined(all, *cluster_peer(&part_s, p), c);
+      const int n = a.splits * a.top;   // at most 8 x 64
+      for (int k = threadIdx.x; k < n; k += kThreads) cand[k] = cluster_peer(found, k / a.top)[k % a.top];
+      for (int k = threadIdx.x; k < a.top; k += kThreads) keys[k] = 0;
+      __syncthreads();
+      rank_keys(cand, n, a.top, keys);
+      list = keys;
+    }
+    __syncthreads();
+    cluster_sync();   // the parts stay until they have been read
+    if (rank != 0) return;
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < a.top; k += kThreads) write_top(a, r, k, list[k], all);
   if (threadIdx.x == 0) {
     const int64_t tok = a.tokens[r];
     float logit = 0.f;
@@ -352,83 +493,6 @@ __global__ void __launch_bounds__(kThreads) long_fwd_kernel(const Args a) {
     }
     write_row(a, r, all, logit, valid);
   }
-  if (!a.top) return;
-  // the top-th largest of the threads' maxima, by the first warp
-  if (warp == 0) {
-    uint64_t k[W];
-#pragma unroll
-    for (int i = 0; i < W; ++i) k[i] = keys[i * 32 + lane];
-    uint64_t best = 0;
-    for (int n = 0; n < a.top; ++n) {
-      uint64_t own = 0;
-#pragma unroll
-      for (int i = 0; i < W; ++i) own = k[i] > own ? k[i] : own;
-      best = group_max<32>(own);
-      if (!best) break;
-#pragma unroll
-      for (int i = 0; i < W; ++i)
-        if (k[i] == best) k[i] = 0;
-    }
-    if (lane == 0) bound_s = best;   // 0: fewer than `top` threads have an entry, so every entry counts
-  }
-  __syncthreads();
-  const uint64_t bound = bound_s;
-  // entries at or above the bound: a larger value, or the same value in no later vector
-  for (int owner = warp; owner < kThreads; owner += W) {
-    if (keys[owner] == 0 || keys[owner] < bound) continue;
-    for (int i0 = owner; i0 < view.vectors; i0 += kThreads * 32) {
-      const int i = i0 + lane * kThreads;
-      if (i >= view.vectors) continue;
-      float x[8];
-      const uint32_t ok = view.load(i, x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (!(ok >> e & 1) || !ranked(x[e])) continue;
-        if (entry_key(x[e], i) < bound) continue;
-        const int at = atomicAdd(&count_s, 1);
-        if (at < kCandidates) cand[at] = entry_key(x[e], 8 * i - view.shift + e);
-      }
-    }
-  }
-  __syncthreads();
-  const int count = count_s;
-  if (count <= kCandidates) {
-    // an entry's place is the number of entries above it
-    for (int i = threadIdx.x; i < count; i += kThreads) {
-      const uint64_t key = cand[i];
-      int place = 0;
-      for (int j = 0; j < count; ++j) place += cand[j] > key;
-      if (place < a.top) found[place] = key;
-    }
-    for (int i = count + threadIdx.x; i < a.top; i += kThreads) found[i] = 0;
-    __syncthreads();
-  } else {
-    // too many for shared memory (many equal or clustered maxima): one pass over the row for each place
-    uint64_t last = ~0ull;
-    for (int n = 0; n < a.top; ++n) {
-      uint64_t best = 0;
-      for (int i = threadIdx.x; i < view.vectors; i += kThreads) {
-        float x[8];
-        const uint32_t ok = view.load(i, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (!(ok >> e & 1) || !ranked(x[e])) continue;
-          const uint64_t key = entry_key(x[e], 8 * i - view.shift + e);
-          if (key < last && key > best) best = key;
-        }
-      }
-      best = group_max<32>(best);
-      __syncthreads();
-      if (lane == 0) cand[warp] = best;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < W; ++w) best = cand[w] > best ? cand[w] : best;
-      last = best;
-      if (threadIdx.x == 0) found[n] = best;
-    }
-    __syncthreads();
-  }
-  for (int i = threadIdx.x; i < a.top; i += kThreads) write_top(a, r, i, found[i], all);
 }
 
 // The gradient: a CTA takes 256 x kBwdVectors vectors of one row.
@@ -447,12 +511,19 @@ long_bwd_kernel(const Args a, const float* __restrict__ g_lp, const float* __res
   const bool none = m == -INFINITY;
   T* out = dx + r * a.v;
   const bool same = ((reinterpret_cast<uintptr_t>(out) - view.shift * sizeof(T)) & 15) == 0;
+  float xs[kBwdVectors][8];
+  uint32_t oks[kBwdVectors];
+#pragma unroll
+  for (int j = 0; j < kBwdVectors; ++j) {
+    const int i = (part * kBwdVectors + j) * 256 + threadIdx.x;
+    oks[j] = i < view.vectors ? view.load(i, xs[j]) : 0;
+  }
 #pragma unroll
   for (int j = 0; j < kBwdVectors; ++j) {
     const int i = (part * kBwdVectors + j) * 256 + threadIdx.x;
     if (i >= view.vectors) continue;
-    float x[8];
-    const uint32_t ok = view.load(i, x);
+    float(&x)[8] = xs[j];
+    const uint32_t ok = oks[j];
     const int c0 = 8 * i - view.shift;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -542,7 +613,22 @@ Results forward(const torch::Tensor& x, const torch::Tensor& tokens, const torch
         small_fwd_kernel<T, G, E><<<(unsigned)((a.rows * G + 255) / 256), 256, 0, st>>>(a);
       });
     } else {
-      long_fwd_kernel<T><<<(unsigned)a.rows, kThreads, 0, st>>>(a);
+      // few rows: as many CTAs for each as give the SMs two, with a vector at least for every thread
+      a.splits = 1;
+      while (a.splits < kMaxSplits && a.rows * a.splits * 2 <= 2 * lm::sm_count() && a.v / 8 >= 2 * a.splits * kThreads)
+        a.splits *= 2;
+      TORCH_CHECK(a.rows * a.splits < (1ll << 31), "token_log_probs: too many rows");
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)(a.rows * a.splits));
+      cfg.blockDim = dim3(kThreads);
+      cfg.stream = st;
+      cudaLaunchAttribute attr = {};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = a.splits;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      TORCH_CHECK(cudaLaunchKernelEx(&cfg, long_fwd_kernel<T>, a) == cudaSuccess, "token_log_probs launch failed");
     }
   });
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "token_log_probs launch failed");
@@ -631,8 +717,8 @@ py::tuple token_log_probs(torch::Tensor logits, torch::Tensor tokens, c10::optio
                         (tokens.scalar_type() == torch::kInt64 || tokens.scalar_type() == torch::kInt32),
                     "token_log_probs needs integer tokens ", lead, " on ", logits.device());
   LM_CHECK_VALUE(tokens.numel() < (1ll << 31) - 1, "token_log_probs: too many rows");
-  LM_CHECK_VALUE(temperature > 0. && std::isfinite(temperature),
-                    "the temperature must be positive and finite, not ", temperature);
+  // far enough inside fp32's range for 1 / T, and for the difference of any two logits over T to be told from zero
+  LM_CHECK_VALUE(temperature >= 1e-30 && temperature <= 1e30, "the temperature must be in 1e-30..1e30, not ", temperature);
   LM_CHECK_VALUE(top >= 0 && top <= kMaxTop, "top must be in 0..", kMaxTop, ", not ", top);
   torch::Tensor m, t = tokens;
   if (mask) {

@@ -127,8 +127,8 @@ def token_log_probs(logits: Tensor, tokens: Tensor, mask: Tensor | None = None, 
     lead, v = logits.shape[:-1], logits.shape[-1]
     if tokens.shape != lead or tokens.dtype not in (torch.int64, torch.int32) or tokens.device != logits.device:
         raise ValueError(f"token_log_probs needs integer tokens {tuple(lead)} on {logits.device}")
-    if not temperature > 0. or temperature == float("inf"):
-        raise ValueError(f"the temperature must be positive and finite, not {temperature}")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"the temperature must be in 1e-30..1e30, not {temperature}")
     if not 0 <= top <= MAX_TOP:
         raise ValueError(f"top must be in 0..{MAX_TOP}, not {top}")
     if mask is not None:
