@@ -15,6 +15,8 @@ namespace fp8 {
 std::pair<torch::Tensor, torch::Tensor> quantize_rows(const torch::Tensor& x);
 // A matrix with contiguous columns -> {q, scale}, or with `transposed` {q, scale, q^T, scale^T}.
 std::vector<torch::Tensor> quantize_blocks(const torch::Tensor& w, bool transposed);
+// Sums of a matrix's columns, in fp32, as `out_type`.
+torch::Tensor column_sums(const torch::Tensor& x, torch::ScalarType out_type);
 // a b^T (+ bias, fp32 or undefined) of operands whose rows start 16 bytes apart.
 torch::Tensor matmul(const torch::Tensor& a, const torch::Tensor& a_scale, const torch::Tensor& b,
                      const torch::Tensor& b_scale, const torch::Tensor& bias, torch::ScalarType out_dtype,

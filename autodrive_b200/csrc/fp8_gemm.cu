@@ -74,26 +74,9 @@ template <int N> struct Ring {
 template <int BN> struct Config {
   static constexpr int stages = BN == 128 ? 6 : 4;
   static constexpr uint32_t a_bytes = kBM * kGroup, stage_bytes = a_bytes + BN * kGroup;
-  static constexpr uint32_t smem_bytes = stages * stage_bytes + 1024 + 256;
+  static constexpr uint32_t smem_bytes = stages * stage_bytes + kEpiWarps * 4096 + 1024 + 256;   // ring, stores, barriers
   static constexpr int buffers = 512 / BN;   // TMEM has 512 columns
 };
-
-template <typename T>
-__device__ __forceinline__ void store32(T* dst, const float (&v)[32], int n, bool vec) {
-  if (vec) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float u[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] = v[8 * j + i];
-      lm::store8(dst + 8 * j, u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) dst[i] = lm::from_f<T>(v[i]);
-  }
-}
 
 // The sums of a CTA's rows over one group: acc += sc * TMEM, `chunks` times 32
 // columns from `base`, the next chunk's load in flight while one is added. The
@@ -142,22 +125,58 @@ struct Scales {
   }
 };
 
-// bias and the store of `acc`, `CHUNKS` times 32 columns from n0 of one row.
+// The store of 32 columns of a warp's 32 rows, one row a lane. Full columns of
+// aligned rows go through `stage` (4 KB of the warp's own), from where
+// neighbouring lanes write neighbouring 16 bytes of a row; with each lane
+// writing its own row a 128 x 256 tile took twice as long to store. 16-byte
+// pieces of a row are swapped by its number, so that neither side's accesses
+// share banks.
+template <typename T>
+__device__ __forceinline__ void store32(const Args& g, const float (&v)[32], int row0, int col, uint8_t* stage) {
+  constexpr int kPieces = 32 * sizeof(T) / 16, kShift = sizeof(T) == 4 ? 0 : 1, kRows = 32 / kPieces;
+  const int lane = threadIdx.x & 31, n = g.N - col;
+  T* c = reinterpret_cast<T*>(g.c);
+  if (n >= 32 && g.ldc % 8 == 0) {   // the output's base is 16-byte aligned (host)
+    uint4* s = reinterpret_cast<uint4*>(stage);
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      alignas(16) T e[16 / sizeof(T)];
+#pragma unroll
+      for (int i = 0; i < (int)(16 / sizeof(T)); ++i) e[i] = lm::from_f<T>(v[p * (16 / sizeof(T)) + i]);
+      s[lane * kPieces + (p ^ ((lane >> kShift) & (kPieces - 1)))] = *reinterpret_cast<const uint4*>(e);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      const int r = k * kRows + lane / kPieces, p = lane % kPieces;
+      if (row0 + r < g.M)
+        *reinterpret_cast<uint4*>(c + (int64_t)(row0 + r) * g.ldc + col + p * (16 / sizeof(T))) =
+            s[r * kPieces + (p ^ ((r >> kShift) & (kPieces - 1)))];
+    }
+    __syncwarp();
+  } else if (row0 + lane < g.M) {
+    T* dst = c + (int64_t)(row0 + lane) * g.ldc + col;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n) dst[i] = lm::from_f<T>(v[i]);
+  }
+}
+
+// bias and the store of `acc`, `CHUNKS` times 32 columns from n0 of the warp's rows.
+constexpr uint32_t kStoreStage = 4096;
 template <int CHUNKS>
-__device__ __forceinline__ void store_row(const Args& g, float (&acc)[CHUNKS][32], int row, int n0) {
+__device__ __forceinline__ void store_rows(const Args& g, float (&acc)[CHUNKS][32], int row0, int n0, uint8_t* stage) {
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
     const int col = n0 + 32 * c, n = g.N - col;
     if (n <= 0) break;
     if (g.bias) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) acc[c][i] += i < n ? g.bias[col + i] : 0.f;
+      for (int i = 0; i < 32; ++i) acc[c][i] += i < n ? __ldg(g.bias + col + i) : 0.f;
     }
-    const int64_t off = (int64_t)row * g.ldc + col;
-    const bool vec = n >= 32 && g.ldc % 8 == 0;   // the output's base is 16-byte aligned (host)
-    if (g.out_kind == 0) store32(reinterpret_cast<float*>(g.c) + off, acc[c], n, vec);
-    else if (g.out_kind == 1) store32(reinterpret_cast<__nv_bfloat16*>(g.c) + off, acc[c], n, vec);
-    else store32(reinterpret_cast<__half*>(g.c) + off, acc[c], n, vec);
+    if (g.out_kind == 0) store32<float>(g, acc[c], row0, col, stage);
+    else if (g.out_kind == 1) store32<__nv_bfloat16>(g, acc[c], row0, col, stage);
+    else store32<__half>(g, acc[c], row0, col, stage);
   }
 }
 
@@ -339,7 +358,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
   using C = Config<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* misc = smem + C::stages * C::stage_bytes;
+  uint8_t* stage0 = smem + C::stages * C::stage_bytes;
+  uint8_t* misc = stage0 + kEpiWarps * kStoreStage;
   const uint32_t full0 = tc::smem_u32(misc);                    // stage loaded
   const uint32_t done0 = full0 + 8 * C::stages;                 // stage's products complete
   const uint32_t tempty0 = done0 + 8 * C::stages;               // TMEM buffer read out
@@ -398,7 +418,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
         },
         [&](auto& acc, int row, int n0) {
           if (splits > 1) keep_sums<BN / 64>(sums, kStride, acc, 32 * q + lane, half * (BN / 2));
-          else if (row < g.M) store_row<BN / 64>(g, acc, row, n0);
+          else store_rows<BN / 64>(g, acc, row - lane, n0, stage0 + (warp - 2) * kStoreStage);
         });
   }
   if (splits > 1) {
@@ -575,13 +595,14 @@ fp8_gemm_rows_kernel(const __grid_constant__ CUtensorMap tb, const __grid_consta
 // barrier before either frees its TMEM or shared memory.
 constexpr int kPairThreads = 384, kPairStages = 6, kPairBuffers = 2;
 constexpr uint32_t kPairTile = 128 * kGroup, kPairStage = 2 * kPairTile;
-constexpr uint32_t kPairSmem = kPairStages * kPairStage + 1024 + 256;
+constexpr uint32_t kPairSmem = kPairStages * kPairStage + kEpiWarps * kStoreStage + 1024 + 256;
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const Args g) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* misc = smem + kPairStages * kPairStage;
+  uint8_t* stage0 = smem + kPairStages * kPairStage;
+  uint8_t* misc = stage0 + kEpiWarps * kStoreStage;
   const uint32_t full0 = tc::smem_u32(misc);                  // own tiles loaded
   const uint32_t peer0 = full0 + 8 * kPairStages;             // first CTA: the second one's tiles loaded
   const uint32_t done0 = peer0 + 8 * kPairStages;             // stage's products complete
@@ -650,7 +671,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_consta
             if (!tile((w / tiles_n) * 256 + (int)rank * 128, (w % tiles_n) * 256, 0, G)) return;
         },
         [&](auto& acc, int row, int n0) {
-          if (row < g.M) store_row<4>(g, acc, row, n0);
+          store_rows<4>(g, acc, row - lane, n0, stage0 + (warp - 4) * kStoreStage);
         });
   }
   tc::tc_fence_before();

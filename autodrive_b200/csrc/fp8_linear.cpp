@@ -5,7 +5,7 @@
 //   dw = dy^T x               bf16 operands, fp32 sums
 //   db = sum of dy's rows     in fp32
 //
-// One call runs the quantisers and the product, and one backward its four
+// One call runs the quantisers and the product, and one backward its
 // kernels, so that no Python runs between the launches.
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
@@ -85,7 +85,7 @@ struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
     }
     const int64_t b_type = ctx->saved_data["b_type"].toInt();
     if (b_type >= 0 && ctx->needs_input_grad(2))
-      out[2] = g.sum(0, false, torch::kFloat32).to(static_cast<torch::ScalarType>(b_type));
+      out[2] = fp8::column_sums(g, static_cast<torch::ScalarType>(b_type));
     return out;
   }
 };

@@ -135,6 +135,39 @@ quant_blocks_kernel(const T* __restrict__ w, int64_t ldw, uint8_t* __restrict__ 
   }
 }
 
+// Partial column sums: a CTA takes 256 columns and every gridDim.y-th group of
+// eight rows, one row a warp.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+column_sums_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int d, float* __restrict__ part) {
+  __shared__ float red[8][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float acc[8] = {};
+  const int64_t step = (int64_t)gridDim.y * 8;
+  for (int64_t r = (int64_t)blockIdx.y * 8 + warp; r < rows; r += 4 * step) {
+    lm::RawSlice<T, VEC> s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (r + j * step < rows) s[j].load(x + (r + j * step) * ldx, blockIdx.x, lane, d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (r + j * step >= rows) continue;
+      float v[8];
+      s[j].get(v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += v[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) red[warp][lm::slice_col<VEC>(0, lane, e)] = acc[e];
+  __syncthreads();
+  float t = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) t += red[w][threadIdx.x];
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c < d) part[(int64_t)blockIdx.y * d + c] = t;
+}
+
 template <typename F>
 void for_type(torch::ScalarType t, F&& f) {
   if (t == torch::kFloat32) f(float{});
@@ -190,6 +223,34 @@ std::pair<torch::Tensor, torch::Tensor> quantize_rows(const torch::Tensor& x) {
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "quantize_rows launch failed");
   lm::count_launches(1);
   return {q, scale};
+}
+
+torch::Tensor column_sums(const torch::Tensor& x, torch::ScalarType out_type) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t rows = x.size(0), d = x.size(1);
+  auto out = torch::empty({d}, x.options().dtype(out_type));
+  if (d == 0) return out;
+  if (rows == 0) return out.zero_();
+  const int64_t blocks = (d + 255) / 256;
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>((rows + 31) / 32, 4 * lm::sm_count() / blocks));
+  const int64_t ldx = rows > 1 ? x.stride(0) : d;
+  const bool vec = d % 8 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  auto part = torch::empty({parts, d}, x.options().dtype(torch::kFloat32));
+  auto st = c10::cuda::getCurrentCUDAStream().stream();
+  for_type(x.scalar_type(), [&](auto t) {
+    using T = decltype(t);
+    const auto kernel = vec ? column_sums_kernel<T, true> : column_sums_kernel<T, false>;
+    kernel<<<dim3((unsigned)blocks, (unsigned)parts), 256, 0, st>>>(reinterpret_cast<const T*>(x.data_ptr()), ldx, rows,
+                                                                   (int)d, part.data_ptr<float>());
+  });
+  for_type(out_type, [&](auto t) {
+    using W = decltype(t);
+    lm::sum_parts_kernel<W><<<(unsigned)((d + lm::kSumColumns - 1) / lm::kSumColumns), 64 * lm::kSumColumns, 0, st>>>(
+        part.data_ptr<float>(), (int)parts, (int)d, reinterpret_cast<W*>(out.data_ptr()));
+  });
+  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "column_sums launch failed");
+  lm::count_launches(2);
+  return out;
 }
 
 std::vector<torch::Tensor> quantize_blocks(const torch::Tensor& w, bool transposed) {

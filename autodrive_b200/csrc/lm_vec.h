@@ -107,6 +107,28 @@ __device__ __forceinline__ float warp_sum(float s) {
   return s;
 }
 
+// out[c] = sum of the rows of part [parts][d]: eight columns per CTA (a sector
+// of each row), 64 threads down each, in an order that depends on the sizes
+// alone.
+constexpr int kSumColumns = 8;
+template <typename W>
+__global__ void __launch_bounds__(64 * kSumColumns) sum_parts_kernel(const float* part, int parts, int d, W* out) {
+  __shared__ float red[64][kSumColumns + 1];
+  const int tx = threadIdx.x % kSumColumns, ty = threadIdx.x / kSumColumns, c = blockIdx.x * kSumColumns + tx;
+  float s = 0.f;
+  if (c < d) {
+#pragma unroll 8
+    for (int p = ty; p < parts; p += 64) s += part[(int64_t)p * d + c];
+  }
+  red[ty][tx] = s;
+  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (warp >= kSumColumns) return;
+  s = warp_sum(red[lane][warp] + red[lane + 32][warp]);
+  const int col = blockIdx.x * kSumColumns + warp;
+  if (lane == 0 && col < d) out[col] = from_f<W>(s);
+}
+
 // ---- 8-bit quantisation ---------------------------------------------------------
 // A group's scale is max(amax, 448 * 2^-126) / 448, rounded to fp32 once: the
 // largest value becomes 448, the largest e4m3 number, and a group of zeros

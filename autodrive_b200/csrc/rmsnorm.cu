@@ -61,18 +61,22 @@ struct FwdArgs {
   float eps;
 };
 
-// Sum over the row's TPR threads; every thread gets it. `red` holds one value
-// per warp, twice, so that one barrier per row is enough.
+// Warps of a row: TPR / 32, but of wide rows as many as the row needs.
+template <int TPR>
+__device__ __forceinline__ int row_warps() { return TPR >= 512 ? blockDim.x >> 5 : TPR / 32; }
+
+// Sum over the row's threads; every thread gets it. `red` holds one value per
+// warp, twice, so that one barrier per row is enough.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float s, float* red, int buf) {
   s = lm::warp_sum(s);
   if constexpr (TPR > 32) {
-    constexpr int W = TPR / 32;
+    constexpr int W = TPR / 32;   // a row's share of `red`: zeros where it has fewer warps
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float* r = red + buf * 32;
     if (lane == 0) r[warp] = s;
     __syncthreads();
-    const int first = warp / W * W;
+    const int first = TPR >= 256 ? 0 : warp / W * W;
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < W; ++i) s += r[first + i];
@@ -85,9 +89,12 @@ constexpr int rows_per_cta(int tpr) { return tpr >= 256 ? 1 : 256 / tpr; }
 template <typename T, bool VEC, bool FP8, int TPR, int NV>
 __global__ void __launch_bounds__(TPR * rows_per_cta(TPR))
 rms_fwd_kernel(const FwdArgs a) {
-  constexpr int RPB = rows_per_cta(TPR), W = TPR / 32;
-  __shared__ float red[64];
-  const int lane = threadIdx.x & 31, part = (threadIdx.x >> 5) % W;   // this warp's part of the row
+  constexpr int RPB = rows_per_cta(TPR);
+  __shared__ __align__(16) float red[64];
+  if (threadIdx.x < 32) red[threadIdx.x] = red[threadIdx.x + 32] = 0.f;
+  __syncthreads();
+  const int W = row_warps<TPR>();
+  const int lane = threadIdx.x & 31, part = TPR >= 256 ? threadIdx.x >> 5 : (threadIdx.x >> 5) % W;   // of the row
   const T* x = reinterpret_cast<const T*>(a.x);
   const T* res = reinterpret_cast<const T*>(a.res);
   float w[NV][8];
@@ -208,10 +215,13 @@ struct BwdArgs {
 template <typename T, bool VEC, int TPR, int NV>
 __global__ void __launch_bounds__(TPR * rows_per_cta(TPR))
 rms_bwd_kernel(const BwdArgs a) {
-  constexpr int RPB = rows_per_cta(TPR), W = TPR / 32;
-  __shared__ float red[64];
+  constexpr int RPB = rows_per_cta(TPR);
+  __shared__ __align__(16) float red[64];
+  if (threadIdx.x < 32) red[threadIdx.x] = red[threadIdx.x + 32] = 0.f;
+  __syncthreads();
   __shared__ float cols[RPB > 1 ? RPB * TPR * NV * 8 : 1];
-  const int lane = threadIdx.x & 31, part = (threadIdx.x >> 5) % W;
+  const int W = row_warps<TPR>();
+  const int lane = threadIdx.x & 31, part = TPR >= 256 ? threadIdx.x >> 5 : (threadIdx.x >> 5) % W;
   float w[NV][8], dw[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -221,6 +231,7 @@ rms_bwd_kernel(const BwdArgs a) {
       w[i][e] = c < a.d ? a.w.at(c) : 0.f;
       dw[i][e] = 0.f;
     }
+  // aligned rows are loaded one ahead; element by element that would cost too many registers
   lm::RawSlice<T, VEC> next_g[NV], next_h[NV], next_u[NV];
   float next_rstd = 0.f;
   const auto load = [&](int64_t r) {
@@ -237,7 +248,7 @@ rms_bwd_kernel(const BwdArgs a) {
     }
   };
   const int64_t step = (int64_t)gridDim.x * RPB;
-  load((int64_t)blockIdx.x * RPB + threadIdx.x / TPR);
+  if (VEC) load((int64_t)blockIdx.x * RPB + threadIdx.x / TPR);
   int buf = 0;
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += step, buf ^= 1) {
     const int64_t r = r0 + threadIdx.x / TPR;
@@ -246,10 +257,11 @@ rms_bwd_kernel(const BwdArgs a) {
     lm::RawSlice<T, VEC> u[NV];
     float s = 0.f, rstd = 0.f;
     if (live) {
+      if (!VEC) load(r);
       rstd = next_rstd;
 #pragma unroll
       for (int i = 0; i < NV; ++i) next_g[i].get(g[i]), next_h[i].get(n[i]), u[i] = next_u[i];
-      load(r + step);
+      if (VEC) load(r + step);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -302,37 +314,20 @@ rms_bwd_kernel(const BwdArgs a) {
   }
 }
 
-// dw[c] = sum of the partial rows: 32 columns per CTA, 32 threads down each.
-template <typename W>
-__global__ void __launch_bounds__(1024) rms_dw_kernel(const float* part, int parts, int d, W* dw) {
-  __shared__ float red[32][33];
-  const int c = blockIdx.x * 32 + threadIdx.x;
-  float s = 0.f;
-  if (c < d) {
-#pragma unroll 8
-    for (int p = threadIdx.y; p < parts; p += 32) s += part[(int64_t)p * d + c];
-  }
-  red[threadIdx.y][threadIdx.x] = s;
-  __syncthreads();
-  s = lm::warp_sum(red[threadIdx.x][threadIdx.y]);
-  const int col = blockIdx.x * 32 + threadIdx.y;
-  if (threadIdx.x == 0 && col < d) dw[col] = lm::from_f<W>(s);
-}
-
 // Persistent CTAs: as many as fit on the SMs at once, so that none waits for a
 // second round.
 template <typename T, auto... V, typename K>
-int grid_for(K* kernel, int64_t rows, int tpr) {
-  static std::atomic<int> fits[64];   // one array for each kernel: T and V are its template arguments
-  const int rpb = rows_per_cta(tpr);
+int grid_for(K* kernel, int64_t rows, int rpb, int threads) {
+  static std::atomic<int> fits[64][33];   // of each kernel (T and V are its template arguments): by device and warps
   int dev = 0;
   TORCH_CHECK(cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64, "rms_norm: device query failed");
-  int n = fits[dev].load(std::memory_order_relaxed);
+  auto& fit = fits[dev][threads / 32];
+  int n = fit.load(std::memory_order_relaxed);
   if (n == 0) {
-    TORCH_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, tpr * rpb, 0) == cudaSuccess,
+    TORCH_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) == cudaSuccess,
                 "rms_norm: occupancy query failed");
     n = std::max(1, n);
-    fits[dev].store(n, std::memory_order_relaxed);
+    fit.store(n, std::memory_order_relaxed);
   }
   return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rpb - 1) / rpb, (int64_t)lm::sm_count() * n));
 }
@@ -349,6 +344,11 @@ void for_width(int64_t d, F&& f) {
   else if (chunks <= 32) f(std::integral_constant<int, 512>{}, std::integral_constant<int, 2>{});
   else if (chunks <= 64) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
   else f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
+}
+
+// A CTA's threads: for wide rows no more warps than the row has chunks for.
+int threads_for(int tpr, int nv, int64_t d) {
+  return tpr < 512 ? tpr * rows_per_cta(tpr) : 32 * (int)(((d + 255) / 256 + nv - 1) / nv);
 }
 
 template <typename F>
@@ -439,8 +439,9 @@ Forward forward(const torch::Tensor& x, const torch::Tensor& residual, const tor
       constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
       const auto launch = [&](auto v8, auto q8) {
         constexpr bool VEC = decltype(v8)::value, FP8 = decltype(q8)::value;
-        const int grid = grid_for<T, VEC, FP8, TPR, NV>(rms_fwd_kernel<T, VEC, FP8, TPR, NV>, rows, TPR);
-        rms_fwd_kernel<T, VEC, FP8, TPR, NV><<<grid, TPR * rows_per_cta(TPR), 0, st>>>(a);
+        const int threads = threads_for(TPR, NV, d);
+        const int grid = grid_for<T, VEC, FP8, TPR, NV>(rms_fwd_kernel<T, VEC, FP8, TPR, NV>, rows, rows_per_cta(TPR), threads);
+        rms_fwd_kernel<T, VEC, FP8, TPR, NV><<<grid, threads, 0, st>>>(a);
       };
       if (vec && fp8) launch(std::true_type{}, std::true_type{});
       else if (vec) launch(std::true_type{}, std::false_type{});
@@ -484,10 +485,11 @@ std::pair<torch::Tensor, torch::Tensor> backward(const torch::Tensor& dy, const 
       constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
       const auto launch = [&](auto v8) {
         constexpr bool VEC = decltype(v8)::value;
-        grid = grid_for<T, VEC, TPR, NV>(rms_bwd_kernel<T, VEC, TPR, NV>, rows, TPR);
+        const int threads = threads_for(TPR, NV, d);
+        grid = grid_for<T, VEC, TPR, NV>(rms_bwd_kernel<T, VEC, TPR, NV>, rows, rows_per_cta(TPR), threads);
         part = torch::empty({grid, d}, h.options().dtype(torch::kFloat32));
         a.part = part.data_ptr<float>();
-        rms_bwd_kernel<T, VEC, TPR, NV><<<grid, TPR * rows_per_cta(TPR), 0, st>>>(a);
+        rms_bwd_kernel<T, VEC, TPR, NV><<<grid, threads, 0, st>>>(a);
       };
       if (vec) launch(std::true_type{});
       else launch(std::false_type{});
@@ -496,8 +498,8 @@ std::pair<torch::Tensor, torch::Tensor> backward(const torch::Tensor& dy, const 
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "rms_norm backward launch failed");
   for_type(weight.scalar_type(), [&](auto t) {
     using W = decltype(t);
-    rms_dw_kernel<W><<<(int)((d + 31) / 32), dim3(32, 32), 0, st>>>(part.data_ptr<float>(), grid, (int)d,
-                                                                  reinterpret_cast<W*>(dw.data_ptr()));
+    lm::sum_parts_kernel<W><<<(int)((d + lm::kSumColumns - 1) / lm::kSumColumns), 64 * lm::kSumColumns, 0, st>>>(part.data_ptr<float>(), grid, (int)d,
+                                                                         reinterpret_cast<W*>(dw.data_ptr()));
   });
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "rms_norm weight gradient launch failed");
   lm::count_launches(2);
