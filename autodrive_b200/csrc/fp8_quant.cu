@@ -23,56 +23,55 @@ namespace py = pybind11;
 
 namespace {
 
-// A half-warp quantises one group of 128 columns, eight columns a lane.
+// A warp takes 256 columns of a row, eight a lane: two groups of 128, the
+// halves of the warp for aligned rows, the halves of every lane's columns
+// otherwise. gridDim.y splits long rows between the CTAs.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 quant_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale,
                   int64_t rows, int k, int groups) {
-  const int sub = threadIdx.x & 15;
-  const int64_t total = rows * groups;
-  // both halves of a warp stay in the loop together (the shuffles are whole-warp)
-  for (int64_t g0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 32 * 2; g0 < total; g0 += (int64_t)gridDim.x * 16) {
-    const int64_t g = g0 + ((threadIdx.x >> 4) & 1);
-    const bool live = g < total;
-    const int64_t r = live ? g / groups : 0;
-    const int grp = live ? (int)(g - r * groups) : 0;
+  const int lane = threadIdx.x & 31, chunks = (groups + 1) / 2;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
     const T* row = x + r * ldx;
-    float v[8];
-    if constexpr (VEC) {
-      const int c = grp * 128 + sub * 8;
-      if (live && c < k) {
-        lm::load8(row + c, v);
+    uint8_t* out = q + r * ldq;
+    float* sc = scale + r * groups;
+    lm::RawSlice<T, VEC> next;
+    next.load(row, blockIdx.y, lane, k);
+    for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
+      float v[8];
+      next.get(v);
+      next.load(row, chunk + gridDim.y, lane, k);   // beyond the row: zeros
+      if constexpr (VEC) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max(m, lm::abs_bits(v[e]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float s = lm::group_scale(m);
+        const int c = lm::slice_col<true>(chunk, lane, 0);
+        if (c < k) {
+          *reinterpret_cast<uint2*>(out + c) = lm::quantize8(v, lm::divisor(s));
+          if ((lane & 15) == 0) sc[2 * chunk + (lane >> 4)] = s;
+        }
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      }
-    } else {
+        for (int g = 0; g < 2; ++g) {
+          uint32_t m = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = grp * 128 + e * 16 + sub;
-        v[e] = live && c < k ? lm::to_f<T>(row[c]) : 0.f;
-      }
-    }
-    uint32_t m = 0;
+          for (int e = 0; e < 4; ++e) m = max(m, lm::abs_bits(v[4 * g + e]));
+          m = __reduce_max_sync(0xffffffffu, m);
+          if (2 * chunk + g >= groups) continue;
+          const float s = lm::group_scale(m);
+          const lm::Divisor dv = lm::divisor(s);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = max(m, lm::abs_bits(v[e]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (!live) continue;
-    const float s = lm::group_scale(m);
-    const lm::Divisor dv = lm::divisor(s);
-    uint8_t* out = q + r * ldq;
-    if constexpr (VEC) {
-      const int c = grp * 128 + sub * 8;
-      if (c < k) *reinterpret_cast<uint2*>(out + c) = lm::quantize8(v, dv);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = grp * 128 + e * 16 + sub;
-        if (c < k) out[c] = (uint8_t)(lm::e4m3x2(lm::e4m3_quotient(v[e], dv), 0.f) & 0xff);
+          for (int e = 0; e < 4; ++e) {
+            const int c = lm::slice_col<false>(chunk, lane, 4 * g + e);
+            if (c < k) out[c] = (uint8_t)(lm::e4m3x2(lm::e4m3_quotient(v[4 * g + e], dv), 0.f) & 0xff);
+          }
+          if (lane == 0) sc[2 * chunk + g] = s;
+        }
       }
     }
-    if (sub == 0) scale[g] = s;
   }
 }
 
@@ -211,7 +210,10 @@ std::pair<torch::Tensor, torch::Tensor> quantize_rows(const torch::Tensor& x) {
   if (rows == 0 || k == 0) return {q, scale};
   const int64_t ldx = rows > 1 ? x.stride(0) : k;
   const bool vec = k % 8 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
-  const int grid = (int)std::min<int64_t>((rows * groups + 15) / 16, (int64_t)lm::sm_count() * 32);
+  // eight warps a CTA, one row each; few rows are split between CTAs
+  const int64_t ctas = (rows + 7) / 8, chunks = (groups + 1) / 2, room = (int64_t)lm::sm_count() * 8;
+  const dim3 grid((unsigned)std::min<int64_t>(ctas, room),
+                  (unsigned)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(chunks, 65535), room / ctas)));
   auto st = c10::cuda::getCurrentCUDAStream().stream();
   for_type(x.scalar_type(), [&](auto t) {
     using T = decltype(t);

@@ -251,6 +251,19 @@ small_bwd_kernel(const Args a, const float* __restrict__ g_lp, const float* __re
 // `shift` entries lie before the row between the boundary and its start. The
 // first and the last vector may run out of the row and are read one by one.
 template <typename T>
+struct Raw {   // eight entries as they lie in memory
+  alignas(16) T e[8];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(T) / 2); ++j) reinterpret_cast<uint4*>(e)[j] = reinterpret_cast<const uint4*>(p)[j];
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = lm::to_f<T>(e[i]);
+  }
+};
+
+template <typename T>
 struct RowView {
   const T* row;
   const uint8_t* mask;
@@ -264,6 +277,9 @@ struct RowView {
     vectors = (v + shift + 7) / 8;
     mask_aligned = mask && ((reinterpret_cast<uintptr_t>(mask) - shift) & 7) == 0;
   }
+  // Vectors from..to - 1 lie wholly inside the row and have no masked entries.
+  __device__ __forceinline__ int plain_from() const { return shift ? 1 : 0; }
+  __device__ __forceinline__ int plain_to() const { return mask ? 0 : (v + shift) / 8; }
   // The entries of vector i and which of them are valid (bit e).
   __device__ __forceinline__ uint32_t load(int i, float (&x)[8]) const {
     const int c0 = 8 * i - shift;
@@ -356,10 +372,11 @@ __device__ __forceinline__ void rank_keys(const uint64_t* keys, int count, int t
 template <typename T>
 __global__ void __launch_bounds__(kThreads) long_fwd_kernel(const Args a) {
   constexpr int W = kThreads / 32;
-  __shared__ Stat red[W], part_s;
+  __shared__ Stat red[W], part_s, part_s2;
   __shared__ uint64_t keys[kThreads], cand[kCandidates], found[kMaxTop];
   __shared__ uint64_t bound_s;
-  __shared__ int count_s;
+  __shared__ int count_s, owners_s;
+  __shared__ uint16_t owners[kThreads];
   const int64_t r = blockIdx.x / a.splits;
   const int rank = a.splits > 1 ? (int)cluster_rank() : 0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -369,13 +386,24 @@ __global__ void __launch_bounds__(kThreads) long_fwd_kernel(const Args a) {
   Stat st = empty_stat();
   int first = 0;   // the vector in which this thread's maximum was first met
   int i = i0 + threadIdx.x;
-  for (; i + (kAhead - 1) * kThreads < i1; i += kAhead * kThreads) {
-    float x[kAhead][8];
-    uint32_t ok[kAhead];
+  const int plain0 = view.plain_from(), plain1 = min(i1, view.plain_to());
+  if (i < plain0) {   // the row's first vector, where the row starts inside it
+    float x[8];
+    const uint32_t ok = view.load(i, x);
+    add_vector(st, first, i, ok, x, c);
+    i += kThreads;
+  }
+  const T* base = view.row - view.shift;
+  for (; i + (kAhead - 1) * kThreads < plain1; i += kAhead * kThreads) {
+    Raw<T> raw[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) ok[j] = view.load(i + j * kThreads, x[j]);
+    for (int j = 0; j < kAhead; ++j) raw[j].load(base + 8 * (int64_t)(i + j * kThreads));
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) add_vector(st, first, i + j * kThreads, ok[j], x[j], c);
+    for (int j = 0; j < kAhead; ++j) {
+      float x[8];
+      raw[j].get(x);
+      add_vector(st, first, i + j * kThreads, 0xffu, x, c);
+    }
   }
   for (; i < i1; i += kThreads) {
     float x[8];
@@ -389,7 +417,7 @@ __global__ void __launch_bounds__(kThreads) long_fwd_kernel(const Args a) {
   if (lane == 0) red[warp] = mine;
   if (a.top) {
     keys[threadIdx.x] = st.m == -INFINITY ? 0 : entry_key(st.m, first);
-    if (threadIdx.x == 0) count_s = 0;
+    if (threadIdx.x == 0) count_s = owners_s = 0, bound_s = 0;
     for (int k = threadIdx.x; k < a.top; k += kThreads) found[k] = 0;
   }
   __syncthreads();
@@ -397,39 +425,29 @@ __global__ void __launch_bounds__(kThreads) long_fwd_kernel(const Args a) {
 #pragma unroll
   for (int w = 1; w < W; ++w) all = joined(all, red[w], c);
   if (a.top) {
-    // the top-th largest of the threads' maxima, by the first warp
-    if (warp == 0) {
-      uint64_t k[W];
-#pragma unroll
-      for (int j = 0; j < W; ++j) k[j] = keys[j * 32 + lane];
-      uint64_t best = 0;
-      for (int n = 0; n < a.top; ++n) {
-        uint64_t own = 0;
-#pragma unroll
-        for (int j = 0; j < W; ++j) own = k[j] > own ? k[j] : own;
-        best = group_max<32>(own);
-        if (!best) break;
-#pragma unroll
-        for (int j = 0; j < W; ++j)
-          if (k[j] == best) k[j] = 0;
-      }
-      if (lane == 0) bound_s = best;   // 0: fewer than `top` threads have an entry, so every entry counts
-    }
+    // the top-th largest of the threads' maxima: the one with top - 1 above it
+    const uint64_t own = keys[threadIdx.x];
+    int place = 0;
+#pragma unroll 8
+    for (int j = 0; j < kThreads; ++j) place += keys[j] > own;
+    if (own && place == a.top - 1) bound_s = own;
     __syncthreads();
-    const uint64_t bound = bound_s;
-    // entries at or above the bound: a larger value, or the same value in no later vector
-    for (int owner = warp; owner < kThreads; owner += W) {
-      if (keys[owner] == 0 || keys[owner] < bound) continue;
-      for (int v = i0 + owner + lane * kThreads; v < i1; v += kThreads * 32) {
-        float x[8];
-        const uint32_t ok = view.load(v, x);
+    const uint64_t bound = bound_s;   // 0: fewer than `top` threads have an entry, so every entry counts
+    if (own && own >= bound) owners[atomicAdd(&owners_s, 1)] = threadIdx.x;
+    __syncthreads();
+    // the owners' entries at or above the bound: a larger value, or the same value in no later vector
+    const int per = (i1 - i0 + kThreads - 1) / kThreads, items = owners_s * per;
+    for (int item = threadIdx.x; item < items; item += kThreads) {
+      const int v = i0 + owners[item / per] + item % per * kThreads;
+      if (v >= i1) continue;
+      float x[8];
+      const uint32_t ok = view.load(v, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (!(ok >> e & 1) || !ranked(x[e])) continue;
-          if (entry_key(x[e], v) < bound) continue;
-          const int at = atomicAdd(&count_s, 1);
-          if (at < kCandidates) cand[at] = entry_key(x[e], 8 * v - view.shift + e);
-        }
+      for (int e = 0; e < 8; ++e) {
+        if (!(ok >> e & 1) || !ranked(x[e])) continue;
+        if (entry_key(x[e], v) < bound) continue;
+        const int at = atomicAdd(&count_s, 1);
+        if (at < kCandidates) cand[at] = entry_key(x[e], 8 * v - view.shift + e);
       }
     }
     __syncthreads();
@@ -468,12 +486,17 @@ __global__ void __launch_bounds__(kThreads) long_fwd_kernel(const Args a) {
     __syncthreads();
     cluster_sync();
     if (rank == 0) {
-      // join the parts in the order of the ranks, and rank their lists once more
-      for (int p = 1; p < a.splits; ++p) all = joined(all, *cluster_peer(&part_s, p), c);
+      // join the parts, and rank their lists once more
+      if (warp == 0) {
+        all = lane < a.splits ? *cluster_peer(&part_s, lane) : empty_stat();
+        all = group_join<kMaxSplits>(all, c);
+      }
+      if (threadIdx.x == 0) part_s2 = all;
       const int n = a.splits * a.top;   // at most 8 x 64
       for (int k = threadIdx.x; k < n; k += kThreads) cand[k] = cluster_peer(found, k / a.top)[k % a.top];
       for (int k = threadIdx.x; k < a.top; k += kThreads) keys[k] = 0;
       __syncthreads();
+      all = part_s2;
       rank_keys(cand, n, a.top, keys);
       list = keys;
     }
@@ -511,29 +534,49 @@ long_bwd_kernel(const Args a, const float* __restrict__ g_lp, const float* __res
   const bool none = m == -INFINITY;
   T* out = dx + r * a.v;
   const bool same = ((reinterpret_cast<uintptr_t>(out) - view.shift * sizeof(T)) & 15) == 0;
-  float xs[kBwdVectors][8];
-  uint32_t oks[kBwdVectors];
+  // d = p (k0 + k1 log p), plus `hot` at the token; without weight 0 times a finite number
+  const float k0 = (-gl - ge * ent) * a.inv_t, k1 = -ge * a.inv_t, hot = gl * a.inv_t;
+  const auto entry = [&](float x) {
+    float lp = fmaf(x - m, a.inv_t, -logs);
+    asm("max.NaN.f32 %0, %0, 0fC3480000;" : "+f"(lp));   // -200: the weight is zero from -88 on
+    return exp2f(lp * kLog2e) * fmaf(k1, lp, k0);
+  };
+  const int first = part * kBwdVectors * 256 + threadIdx.x, hot_vector = (int)((tok + view.shift) >> 3);
+  if (same && !none && part * kBwdVectors * 256 >= view.plain_from() &&
+      (part + 1) * kBwdVectors * 256 <= view.plain_to()) {   // the whole CTA's vectors are plain
+    Raw<T> raw[kBwdVectors];
+    const T* in = view.row - view.shift;
 #pragma unroll
-  for (int j = 0; j < kBwdVectors; ++j) {
-    const int i = (part * kBwdVectors + j) * 256 + threadIdx.x;
-    oks[j] = i < view.vectors ? view.load(i, xs[j]) : 0;
+    for (int j = 0; j < kBwdVectors; ++j) raw[j].load(in + 8 * (int64_t)(first + j * 256));
+#pragma unroll
+    for (int j = 0; j < kBwdVectors; ++j) {
+      const int i = first + j * 256;
+      float x[8];
+      raw[j].get(x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = entry(x[e]);
+      if (i == hot_vector && hot != 0.f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (8 * i - view.shift + e == tok) x[e] += hot;
+      }
+      lm::store8(out + 8 * (int64_t)i - view.shift, x);
+    }
+    return;
   }
-#pragma unroll
+#pragma unroll 1
   for (int j = 0; j < kBwdVectors; ++j) {
-    const int i = (part * kBwdVectors + j) * 256 + threadIdx.x;
-    if (i >= view.vectors) continue;
-    float(&x)[8] = xs[j];
-    const uint32_t ok = oks[j];
+    const int i = first + j * 256;
+    if (i >= view.vectors) return;
+    float x[8];
+    const uint32_t ok = view.load(i, x);
     const int c0 = 8 * i - view.shift;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float d = 0.f;
       if (ok >> e & 1 && !none) {
-        const float lp = (x[e] - m) * a.inv_t - logs;
-        const float p = exp2f(lp * kLog2e);
-        d = p == 0.f ? 0.f : p * (-gl - ge * (lp + ent));
-        if (c0 + e == tok) d += gl;
-        d *= a.inv_t;
+        d = entry(x[e]);
+        if (c0 + e == tok) d += hot;
       }
       x[e] = d;
     }
