@@ -1,6 +1,5 @@
 // The 8-bit quantisers and product as C++ functions (fp8_quant.cu,
-// fp8_gemm.cu), for the linear layer that joins them (fp8_linear.cpp), and the
-// bf16 product of its weight gradient (tc_gemm.cu). Operands are checked by
+// fp8_gemm.cu), for the linear layer that joins them (fp8_linear.cpp). Operands are checked by
 // their callers' entry points.
 #pragma once
 
@@ -21,6 +20,9 @@ torch::Tensor column_sums(const torch::Tensor& x, torch::ScalarType out_type);
 torch::Tensor matmul(const torch::Tensor& a, const torch::Tensor& a_scale, const torch::Tensor& b,
                      const torch::Tensor& b_scale, const torch::Tensor& bias, torch::ScalarType out_dtype,
                      const torch::Tensor& status, int64_t wait_ns);
+// a^T b of bf16 matrices [K, M] and [K, N] with 16-byte aligned rows, fp32 sums.
+torch::Tensor weight_gradient(const torch::Tensor& a, const torch::Tensor& b, torch::ScalarType out_type,
+                              const torch::Tensor& status);
 // `t` as a matrix with contiguous columns: a view where its layout allows one.
 torch::Tensor as_matrix(const torch::Tensor& t);
 // 1: fp32, bf16 or fp16.
@@ -29,6 +31,3 @@ bool known_type(torch::ScalarType t);
 constexpr int64_t kWaitNs = 2000000000ll;
 
 }  // namespace fp8
-
-// g^T x in fp32 for bf16 g [M, N] and x [M, K] with row strides that are multiples of 8.
-torch::Tensor tc_weight_gradient(const torch::Tensor& g, const torch::Tensor& x, const torch::Tensor& status);

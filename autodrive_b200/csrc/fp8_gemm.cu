@@ -52,7 +52,8 @@ struct Args {
   void* c;
   int64_t ldc;
   int out_kind;           // 0 fp32, 1 bf16, 2 fp16
-  int splits;             // CTAs of a cluster that share one tile's groups (1: none do)
+  int splits;             // CTAs of a cluster that share one tile's groups (1: none do); bf16: parts of the rows
+  int64_t part;           // bf16: elements between the results of two parts
   int* status;
   uint64_t wait_ns;
 };
@@ -112,7 +113,9 @@ struct Scales {
       nb[j] = __ldg(b + k);
     }
   }
-  __device__ __forceinline__ Scales(const float* pa, const float* pb, int g) : a(pa), b(pb), groups(g) { load(0); }
+  __device__ __forceinline__ Scales(const float* pa, const float* pb, int g) : a(pa), b(pb), groups(g) {
+    if (a && g > 0) load(0);
+  }
   // Call for kb = 0, 1, 2, ...
   __device__ __forceinline__ float at(int kb) {
     if ((kb & 3) == 0) {
@@ -185,7 +188,7 @@ __device__ __forceinline__ void store_rows(const Args& g, float (&acc)[CHUNKS][3
 // first column, first group, last group) for one of the CTA's tiles after the
 // other; sink(sums, row, first column) gets each tile's sums. `tempty0` may
 // lie in another CTA (a mapped address).
-template <int STAGES, int BUFFERS, int COLS, typename F, typename S>
+template <int STAGES, int BUFFERS, int COLS, bool SCALED = true, typename F, typename S>
 __device__ __forceinline__ void epilogue(const Args& g, uint32_t tmem, uint32_t done0, uint32_t tempty0, int* s_fail,
                                          int q, int half, F&& walk, S&& sink) {
   constexpr int kChunks = COLS / 64;   // 32-column chunks per warp
@@ -201,10 +204,10 @@ __device__ __forceinline__ void epilogue(const Args& g, uint32_t tmem, uint32_t 
     for (int c = 0; c < kChunks; ++c)
 #pragma unroll
       for (int i = 0; i < 32; ++i) acc[c][i] = 0.f;
-    Scales sc(g.a_scale + (int64_t)min(row, g.M - 1) * G + kb0,
-              g.b_scale + (int64_t)min(n0 / kGroup, (g.N - 1) / kGroup) * G + kb0, max(kb1 - kb0, 1));
+    Scales sc(SCALED ? g.a_scale + (int64_t)min(row, g.M - 1) * G + kb0 : nullptr,
+              SCALED ? g.b_scale + (int64_t)min(n0 / kGroup, (g.N - 1) / kGroup) * G + kb0 : nullptr, kb1 - kb0);
     for (int kb = kb0; kb < kb1; ++kb) {
-      const float scale = sc.at(kb - kb0);
+      const float scale = SCALED ? sc.at(kb - kb0) : 1.f;
       const bool got = tc::mbar_wait(done0 + 8 * st.slot, st.round, g.wait_ns);
       if (!__all_sync(0xffffffffu, got)) {   // the loads below are whole-warp
         give_up(g, 4, s_fail);
@@ -274,7 +277,7 @@ __device__ __forceinline__ void store_one(const Args& g, int row, int col, float
 // group's tiles after the other, until it answers false. Before it returns,
 // every load has landed and the products of every stage are complete: the
 // CTA's shared memory must not be given away before.
-template <int STAGES, typename F>
+template <int STAGES, bool BF16 = false, typename F>
 __device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, const CUtensorMap* tb, uint32_t smem0,
                                         uint32_t stage_bytes, uint32_t a_bytes, uint32_t full0, uint32_t done0,
                                         int* s_fail, F&& walk) {
@@ -288,8 +291,15 @@ __device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, co
     }
     const uint32_t sa = smem0 + st.slot * stage_bytes, full = full0 + 8 * st.slot;
     tc::mbar_arrive_expect_tx(full, stage_bytes);
-    tc::tma_load_2d(sa, ta, k, row_a, full);
-    tc::tma_load_2d(sa + a_bytes, tb, k, row_b, full);
+    if constexpr (BF16) {   // 64 rows by 128 columns, as two boxes of 64 columns
+      tc::tma_load_2d(sa, ta, row_a, k, full);
+      tc::tma_load_2d(sa + 8192, ta, row_a + 64, k, full);
+      tc::tma_load_2d(sa + a_bytes, tb, row_b, k, full);
+      tc::tma_load_2d(sa + a_bytes + 8192, tb, row_b + 64, k, full);
+    } else {
+      tc::tma_load_2d(sa, ta, k, row_a, full);
+      tc::tma_load_2d(sa + a_bytes, tb, k, row_b, full);
+    }
     st.next();
     ++issued;
     return true;
@@ -309,11 +319,13 @@ __device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, co
 // and one commit, for the producer and the epilogue alike. Products take 48
 // cycles to issue, commits 59 and successful waits 40, one after the other, so
 // the next group's barriers are looked at between the products.
-template <int STAGES, int BUFFERS, int COLS, bool PAIR>
+template <int STAGES, int BUFFERS, int COLS, bool PAIR, bool BF16 = false>
 __device__ __forceinline__ void multiply(const Args& g, uint32_t count, uint32_t smem0, uint32_t stage_bytes,
                                          uint32_t a_bytes, uint32_t tmem, uint32_t full0, uint32_t peer0,
                                          uint32_t done0, uint32_t tempty0, uint32_t drain, int* s_fail) {
-  const uint32_t id = tc::idesc_e4m3(PAIR ? 256 : 128, COLS), lo = tc::kmajor_desc_lo(smem0);
+  static_assert(!BF16 || PAIR, "bf16 tiles are the pairs' alone");
+  const uint32_t id = BF16 ? tc::idesc_bf16(256, COLS, true, true) : tc::idesc_e4m3(PAIR ? 256 : 128, COLS);
+  const uint32_t lo = BF16 ? tc::mnmajor64_desc_lo(smem0) : tc::kmajor_desc_lo(smem0);
   Ring<STAGES> st;
   Ring<BUFFERS> buf;
   bool loaded = false, read = true, peer = !PAIR;   // the buffers' first round needs no waiting
@@ -334,7 +346,9 @@ __device__ __forceinline__ void multiply(const Args& g, uint32_t count, uint32_t
     buf.next();
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      if constexpr (PAIR) tc::mma_e4m3_pair(d, tc::kmajor_desc(la + 2 * ks), tc::kmajor_desc(lb + 2 * ks), id, ks > 0);
+      if constexpr (BF16)
+        tc::mma_bf16_pair(d, tc::kmajor_desc(la + 128 * ks), tc::kmajor_desc(lb + 128 * ks), id, ks > 0);
+      else if constexpr (PAIR) tc::mma_e4m3_pair(d, tc::kmajor_desc(la + 2 * ks), tc::kmajor_desc(lb + 2 * ks), id, ks > 0);
       else tc::mma_e4m3(d, tc::kmajor_desc(la + 2 * ks), tc::kmajor_desc(lb + 2 * ks), id, ks > 0);
       if (ks == 1) {
         read = it + 1 < (uint32_t)BUFFERS || tc::mbar_try_wait(tempty0 + 8 * buf.slot, buf.round ^ 1);
@@ -597,8 +611,15 @@ constexpr int kPairThreads = 384, kPairStages = 6, kPairBuffers = 2;
 constexpr uint32_t kPairTile = 128 * kGroup, kPairStage = 2 * kPairTile;
 constexpr uint32_t kPairSmem = kPairStages * kPairStage + kEpiWarps * kStoreStage + 1024 + 256;
 
+// BF16: the weight gradient's product instead, C = A^T B in fp32 of bf16 A
+// [K,M] and B [K,N]. A stage holds 64 rows of both (as many bytes), read down
+// their columns by the tensor cores, and without scales the epilogue adds up
+// every 64 rows in fp32 with round-to-nearest, which the tensor cores' own long
+// sums do not; g.splits parts of the rows give as many partial results, `part`
+// elements apart.
+template <bool BF16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const Args g) {
+gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const Args g) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* stage0 = smem + kPairStages * kPairStage;
@@ -615,8 +636,14 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_consta
   const uint32_t rank = tc::cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int tiles_n = (g.N + 255) / 256, tiles_m = (g.M + 255) / 256;
-  const int total = tiles_n * tiles_m, G = g.groups;
-  const uint32_t tiles = (total - 1 - pair) / pairs + 1;      // never more pairs than tiles
+  const int tiles = tiles_n * tiles_m, splits = BF16 ? g.splits : 1, total = tiles * splits, G = g.groups;
+  const int share = (G + splits - 1) / splits;                // groups of a part of the rows
+  const auto range = [&](int w) {
+    const int kb0 = BF16 ? w / tiles * share : 0;
+    return make_int2(min(G, kb0), min(G, kb0 + share));
+  };
+  uint32_t count = 0;                                         // of this pair's groups
+  for (int w = pair; w < total; w += pairs) count += range(w).y - range(w).x;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kPairStages; ++s) {
@@ -643,18 +670,21 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_consta
   if (warp < 4) {
     tc::regs_dec<40>();
     if (warp == 0 && lane == 0) {
-      produce<kPairStages>(g, &ta, &tb, smem0, kPairStage, kPairTile, full0, done0, s_fail, [&](auto&& load) {
-        for (int w = pair; w < total; w += pairs)
-          for (int kb = 0; kb < G; ++kb)
-            if (!load(kb * kGroup, (w / tiles_n) * 256 + (int)rank * 128, (w % tiles_n) * 256 + (int)rank * 128)) return;
+      produce<kPairStages, BF16>(g, &ta, &tb, smem0, kPairStage, kPairTile, full0, done0, s_fail, [&](auto&& load) {
+        for (int w = pair; w < total; w += pairs) {
+          const int2 kb = range(w);
+          const int m0 = (w % tiles / tiles_n) * 256 + (int)rank * 128, n0 = (w % tiles_n) * 256 + (int)rank * 128;
+          for (int k = kb.x; k < kb.y; ++k)
+            if (!load(k * (BF16 ? 64 : kGroup), m0, n0)) return;
+        }
       });
     } else if (warp == 1 && lane == 0 && rank == 0) {
-      multiply<kPairStages, kPairBuffers, 256, true>(g, tiles * G, smem0, kPairStage, kPairTile, tmem, full0, peer0, done0,
-                                                     tempty0, drain, s_fail);
+      multiply<kPairStages, kPairBuffers, 256, true, BF16>(g, count, smem0, kPairStage, kPairTile, tmem, full0, peer0, done0,
+                                                           tempty0, drain, s_fail);
     } else if (warp == 1 && lane == 0) {
       const uint32_t peer = tc::cluster_map(peer0, 0);
       Ring<kPairStages> st;
-      for (uint32_t it = 0; it < tiles * G; ++it, st.next()) {
+      for (uint32_t it = 0; it < count; ++it, st.next()) {
         if (!tc::mbar_wait(full0 + 8 * st.slot, st.round, g.wait_ns)) {
           give_up(g, 2, s_fail);
           break;
@@ -665,13 +695,18 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_consta
     __syncwarp();
   } else {
     tc::regs_inc<216>();
-    epilogue<kPairStages, kPairBuffers, 256>(
-        g, tmem, done0, tc::cluster_map(tempty0, 0), s_fail, warp & 3, (warp - 4) >> 2, [&](auto&& tile) {
-          for (int w = pair; w < total; w += pairs)
-            if (!tile((w / tiles_n) * 256 + (int)rank * 128, (w % tiles_n) * 256, 0, G)) return;
+    Args out = g;
+    epilogue<kPairStages, kPairBuffers, 256, !BF16>(
+        g, tmem, done0, tc::cluster_map(tempty0, 0), s_fail, warp & 3, (warp - 4) >> 2,
+        [&](auto&& tile) {
+          for (int w = pair; w < total; w += pairs) {
+            const int2 kb = range(w);
+            if (BF16) out.c = reinterpret_cast<float*>(g.c) + (int64_t)(w / tiles) * g.part;
+            if (!tile((w % tiles / tiles_n) * 256 + (int)rank * 128, (w % tiles_n) * 256, kb.x, kb.y)) return;
+          }
         },
         [&](auto& acc, int row, int n0) {
-          store_rows<4>(g, acc, row - lane, n0, stage0 + (warp - 4) * kStoreStage);
+          store_rows<4>(out, acc, row - lane, n0, stage0 + (warp - 4) * kStoreStage);
         });
   }
   tc::tc_fence_before();
@@ -680,6 +715,30 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_consta
   if (warp == 1) {
     tc::tc_fence_after();
     tc::tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// out = sum of `splits` slices of `count` elements, in their order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+sum_slices_kernel(const float* __restrict__ parts, int splits, int64_t count, T* __restrict__ out) {
+  const int64_t step = (int64_t)gridDim.x * 1024;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += step) {
+    if (i + 4 <= count && count % 4 == 0) {
+      float4 s = *reinterpret_cast<const float4*>(parts + i);
+      for (int k = 1; k < splits; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(parts + k * count + i);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+      }
+      out[i] = lm::from_f<T>(s.x), out[i + 1] = lm::from_f<T>(s.y);
+      out[i + 2] = lm::from_f<T>(s.z), out[i + 3] = lm::from_f<T>(s.w);
+    } else {
+      for (int64_t j = i; j < min(count, i + 4); ++j) {
+        float s = 0.f;
+        for (int k = 0; k < splits; ++k) s += parts[k * count + j];
+        out[j] = lm::from_f<T>(s);
+      }
+    }
   }
 }
 
@@ -730,12 +789,13 @@ void launch_rows(const CUtensorMap& tb, const torch::Tensor& a, int64_t lda, Arg
                  st, tb, ta, g);
 }
 
+template <bool BF16>
 void launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const Args& g, int64_t tiles, cudaStream_t st) {
   static size_t configured[dynsmem::kMaxDevices] = {};
-  TORCH_CHECK(dynsmem::opt_in(fp8_gemm_pair_kernel, kPairSmem, configured) == cudaSuccess,
+  TORCH_CHECK(dynsmem::opt_in(gemm_pair_kernel<BF16>, kPairSmem, configured) == cudaSuccess,
               "fp8_matmul shared-memory attribute");
   TORCH_CHECK(tiles < (1ll << 31), "fp8_matmul: too many output tiles");
-  fp8_gemm_pair_kernel<<<2 * (int)std::min<int64_t>(tiles, lm::sm_count() / 2), kPairThreads, kPairSmem, st>>>(ta, tb, g);
+  gemm_pair_kernel<BF16><<<2 * (int)std::min<int64_t>(tiles, lm::sm_count() / 2), kPairThreads, kPairSmem, st>>>(ta, tb, g);
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "fp8_matmul launch failed");
 }
 
@@ -792,11 +852,52 @@ torch::Tensor matmul(const torch::Tensor& a, const torch::Tensor& a_scale, const
   } else {
     const CUtensorMap ta = tma::u8_sw128(a.data_ptr(), M, K, lda, kBM);
     const int64_t pair_tiles = ((M + 255) / 256) * ((N + 255) / 256);
-    if (pair_tiles >= lm::sm_count() / 2) launch_pair(ta, tb, g, pair_tiles, st);
+    if (pair_tiles >= lm::sm_count() / 2) launch_pair<false>(ta, tb, g, pair_tiles, st);
     else launch<128>(ta, tb, g, st);
   }
   lm::count_launches(1);
   return c;
+}
+
+torch::Tensor weight_gradient(const torch::Tensor& a, const torch::Tensor& b, torch::ScalarType out_type,
+                              const torch::Tensor& status) {
+  const c10::cuda::CUDAGuard guard(a.device());
+  const int64_t K = a.size(0), M = a.size(1), N = b.size(1);
+  auto out = torch::empty({M, N}, a.options().dtype(out_type));
+  if (M == 0 || N == 0) return out;
+  if (K == 0) return out.zero_();
+  LM_CHECK_VALUE(M < (1ll << 30) && N < (1ll << 30) && K < (1ll << 30), "weight gradient: too large");
+  Args g{};
+  g.M = (int)M;
+  g.N = (int)N;
+  g.groups = (int)((K + 63) / 64);
+  g.ldc = N;
+  g.status = status.data_ptr<int>();
+  g.wait_ns = kWaitNs;
+  // Few tiles over many rows: as many parts of the rows as the SM pairs have room for, four stages each at least.
+  const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256), pairs = lm::sm_count() / 2;
+  g.splits = (int)std::max<int64_t>(1, std::min<int64_t>(pairs / tiles, g.groups / 4));
+  g.part = M * N;
+  const bool direct = g.splits == 1 && out_type == torch::kFloat32;
+  torch::Tensor parts = direct ? out : torch::empty({g.splits, M, N}, a.options().dtype(torch::kFloat32));
+  g.c = parts.data_ptr();
+  const CUtensorMap ta = tma::bf16_sw128(a.data_ptr(), K, M, a.stride(0), 64);
+  const CUtensorMap tb = tma::bf16_sw128(b.data_ptr(), K, N, b.stride(0), 64);
+  auto st = c10::cuda::getCurrentCUDAStream().stream();
+  launch_pair<true>(ta, tb, g, tiles * g.splits, st);
+  lm::count_launches(1);
+  if (direct) return out;
+  const auto sum = [&](auto t) {
+    using T = decltype(t);
+    sum_slices_kernel<T><<<(unsigned)std::min<int64_t>((M * N + 1023) / 1024, lm::sm_count() * 16), 256, 0, st>>>(
+        parts.data_ptr<float>(), g.splits, M * N, reinterpret_cast<T*>(out.data_ptr()));
+  };
+  if (out_type == torch::kFloat32) sum(float{});
+  else if (out_type == torch::kBFloat16) sum(__nv_bfloat16{});
+  else sum(__half{});
+  TORCH_CHECK(cudaGetLastError() == cudaSuccess, "weight gradient launch failed");
+  lm::count_launches(1);
+  return out;
 }
 
 }  // namespace fp8

@@ -22,16 +22,15 @@ namespace {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// `x` [M, K] as a bf16 operand of the weight gradient: columns a multiple of 8, zeros behind the last.
+// `x` as a bf16 operand of the weight gradient: rows that start 16 bytes apart
+// on an aligned base (a copy only where they do not).
 torch::Tensor bf16_operand(const torch::Tensor& x) {
-  const int64_t k = x.size(1), kp = (k + 7) / 8 * 8;
-  if (k == kp) {
-    const auto y = x.to(torch::kBFloat16).contiguous();
-    return reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 == 0 ? y : y.clone();
-  }
-  auto y = torch::empty({x.size(0), kp}, x.options().dtype(torch::kBFloat16));
-  y.narrow(1, k, kp - k).zero_();
-  y.narrow(1, 0, k).copy_(x);
+  const int64_t rows = x.size(0), k = x.size(1);
+  if (x.scalar_type() == torch::kBFloat16 && (rows <= 1 || x.stride(0) % 8 == 0) && (k <= 1 || x.stride(1) == 1) &&
+      reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && rows != 1)
+    return x;
+  auto y = torch::empty({rows, (k + 7) / 8 * 8}, x.options().dtype(torch::kBFloat16)).narrow(1, 0, k);
+  y.copy_(x);
   return y;
 }
 
@@ -79,9 +78,8 @@ struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
                    .view(x_sizes);
     }
     if (ctx->needs_input_grad(1)) {
-      auto dw = tc_weight_gradient(bf16_operand(g), bf16_operand(fp8::as_matrix(saved[0])), status);
-      if (dw.size(0) != n || dw.size(1) != k) dw = dw.narrow(0, 0, n).narrow(1, 0, k);
-      out[1] = dw.to(static_cast<torch::ScalarType>(ctx->saved_data["w_type"].toInt()));
+      out[1] = fp8::weight_gradient(bf16_operand(g), bf16_operand(fp8::as_matrix(saved[0])),
+                                    static_cast<torch::ScalarType>(ctx->saved_data["w_type"].toInt()), status);
     }
     const int64_t b_type = ctx->saved_data["b_type"].toInt();
     if (b_type >= 0 && ctx->needs_input_grad(2))

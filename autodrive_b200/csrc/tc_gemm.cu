@@ -44,7 +44,6 @@
 #include <algorithm>
 #include <cmath>
 
-#include "fp8.h"
 #include "tc_sm100.h"
 #include "tma_map.h"
 #include "smem_opt_in.h"
@@ -596,12 +595,6 @@ void tc_gemm(torch::Tensor a, bool a_mn, torch::Tensor b, bool b_mn, torch::Tens
 }
 
 }  // namespace
-
-torch::Tensor tc_weight_gradient(const torch::Tensor& g, const torch::Tensor& x, const torch::Tensor& status) {
-  auto out = torch::empty({g.size(1), x.size(1)}, g.options().dtype(torch::kFloat32));
-  tc_gemm(g, true, x, true, out, c10::nullopt, 0, false, status, 2000000000ll, c10::nullopt);
-  return out;
-}
 
 void register_tc_gemm_ops(py::module& m) {
   m.def("tc_gemm", &tc_gemm, "bf16 tcgen05 GEMM C = op(A) op(B)^T (+bias, activation), TMA-fed, fp32 accumulate",

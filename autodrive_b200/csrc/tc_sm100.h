@@ -195,6 +195,12 @@ __device__ __forceinline__ uint64_t kmajor_desc(uint32_t lo) {
   return (uint64_t)hi << 32 | lo;
 }
 
+// The low word of an MN-major bf16 operand's descriptor: an image of 64 rows,
+// its 64-wide column blocks 8192 bytes apart.
+__device__ __forceinline__ uint32_t mnmajor64_desc_lo(uint32_t saddr) {
+  return ((8192u >> 4) << 16) | ((saddr >> 4) & 0x3FFFu);
+}
+
 // K-major operand, contraction along image columns: 16-wide k-slice `ks` of an
 // image with `rows` rows. The leading byte offset is unused for swizzled
 // K-major layouts; 8-row groups are 1024 bytes apart.
@@ -288,6 +294,14 @@ __device__ __forceinline__ void mma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc, 
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
       " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
+      :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u) : "memory");
+}
+// The same over 16 bf16 columns.
+__device__ __forceinline__ void mma_bf16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                              bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
       :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u) : "memory");
 }
 // Arrive on `bar` in both CTAs of the pair once all tcgen05 ops issued so far complete.

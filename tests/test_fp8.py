@@ -259,7 +259,8 @@ def test_results_do_not_depend_on_the_run():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("m,n,k", [(1, 64, 64), (257, 130, 200), (1024, 256, 520), (33, 1000, 127)])
+@pytest.mark.parametrize("m,n,k", [(1, 64, 64), (257, 130, 200), (1024, 256, 520), (33, 1000, 127), (9000, 520, 264),
+                                   (300, 5000, 4100)])
 def test_linear_gradients_match_the_formula(dtype, m, n, k):
     x = _values(m, k, 1, torch.bfloat16, "cuda").to(dtype).requires_grad_(True)
     w = (_values(n, k, 2, device="cuda") * k ** -.5).requires_grad_(True)
