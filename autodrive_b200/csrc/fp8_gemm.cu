@@ -386,6 +386,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
   const int total = tiles_n * tiles_m, G = g.groups;
 
   if (threadIdx.x == 0) {
+    tc::tma_prefetch_map(&ta);
+    tc::tma_prefetch_map(&tb);
     for (int s = 0; s < C::stages; ++s) {
       tc::mbar_init(full0 + 8 * s, 1);
       tc::mbar_init(done0 + 8 * s, 1);
@@ -492,6 +494,8 @@ fp8_gemm_rows_kernel(const __grid_constant__ CUtensorMap tb, const __grid_consta
   const int part = (G + splits - 1) / splits, kb0 = min(G, rank * part), kb1 = min(G, kb0 + part);
 
   if (threadIdx.x == 0) {
+    tc::tma_prefetch_map(&ta);
+    tc::tma_prefetch_map(&tb);
     for (int s = 0; s < kRowsStages; ++s) {
       tc::mbar_init(full0 + 8 * s, 1);
       tc::mbar_init(done0 + 8 * s, 1);
@@ -646,6 +650,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
   for (int w = pair; w < total; w += pairs) count += range(w).y - range(w).x;
 
   if (threadIdx.x == 0) {
+    tc::tma_prefetch_map(&ta);
+    tc::tma_prefetch_map(&tb);
     for (int s = 0; s < kPairStages; ++s) {
       tc::mbar_init(full0 + 8 * s, 1);
       tc::mbar_init(peer0 + 8 * s, 1);

@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace lm {
 
@@ -43,9 +44,17 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
     reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
   } else {
     uint4 u;
-    T* e = reinterpret_cast<T*>(&u);
+    uint32_t* w = &u.x;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f<T>(v[i]);
+    for (int i = 0; i < 4; ++i) {   // two at a time
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
     *reinterpret_cast<uint4*>(p) = u;
   }
 }
@@ -140,14 +149,31 @@ constexpr uint32_t kMinAmaxBits = 0x04e00000u;   // 448 * 2^-126
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+__device__ __forceinline__ float mul_nf(float a, float b) {
+  float r;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float fma_nf(float a, float b, float c) {
+  float r;
+  asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// amax / 448, correctly rounded by one correction of the product with the
+// rounded reciprocal (Markstein, "Computation of elementary functions on the IBM
+// RISC System/6000 processor", 1990): the remainder is exact in an fma.
 __device__ __forceinline__ float group_scale(uint32_t amax_bits) {
-  return __fdiv_rn(__uint_as_float(max(amax_bits, kMinAmaxBits)), 448.f);
+  constexpr float r = 1.f / 448.f;
+  const float a = __uint_as_float(max(amax_bits, kMinAmaxBits));
+  const float q = mul_nf(a, r);
+  const float s = fma_nf(fma_nf(-q, 448.f, a), r, q);
+  return amax_bits < 0x7f800000u ? s : a;
 }
 
 // x / scale rounded to e4m3 once. A quotient rounded to fp32 first can land
 // on the middle between two e4m3 numbers, or on its wrong side, and then be
-// rounded to the wrong one. x times the rounded reciprocal is within two units
-// in the last place, so only values within four of a middle (the last 20 bits
+// rounded to the wrong one. x times the reciprocal is within three units in
+// the last place, so only values within four of a middle (the last 20 bits
 // tell, among e4m3's normal numbers) and those below them take the exact way:
 // there the quotient is rounded to odd (truncated, with the last bit set when
 // the remainder is not zero; Boldo & Melquiond, "When double rounding is odd",
@@ -163,19 +189,9 @@ __device__ __forceinline__ Divisor divisor(float scale) {
   Divisor d;
   d.lift = scale < 0x1p-60f ? 0x1p64f : 1.f;
   d.scale = scale * d.lift;
-  d.inv = __frcp_rn(d.scale);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d.inv) : "f"(d.scale));   // within one unit in the last place
   d.direct = scale < __uint_as_float(0x7f800000u) ? d.inv * d.lift : __uint_as_float(0x7fffffffu);   // inf, NaN: NaN
   return d;
-}
-__device__ __forceinline__ float mul_nf(float a, float b) {
-  float r;
-  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float fma_nf(float a, float b, float c) {
-  float r;
-  asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
 }
 __device__ __forceinline__ float quotient_to_odd(float x, const Divisor& d) {
   float y;

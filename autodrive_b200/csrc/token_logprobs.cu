@@ -16,9 +16,9 @@
 // no gradient; a NaN or +inf among its entries makes a row's results NaN.
 //
 // Alternatives (the `top` largest logits, equal ones by their index): at least
-// `top` entries are as large as the top-th largest of the threads' maxima, so
-// only the few threads whose maximum reaches that bound have their entries
-// looked at again, and the entries that reach it are ranked.
+// `top` entries are as large as the top-th largest of the maxima of groups of
+// threads, so only the few threads whose maximum reaches that bound have their
+// entries looked at again, and the entries that reach it are ranked.
 //
 // Bound by memory for long rows. Rows of up to 1024 entries are held in the
 // registers of one warp or of a part of one; longer ones take a CTA each, or a
@@ -421,18 +421,30 @@ __global__ void __launch_bounds__(kThreads) long_fwd_kernel(const Args a) {
     for (int k = threadIdx.x; k < a.top; k += kThreads) found[k] = 0;
   }
   __syncthreads();
-  Stat all = red[0];
-#pragma unroll
-  for (int w = 1; w < W; ++w) all = joined(all, red[w], c);
+  if (warp == 0) {
+    const Stat s = group_join<W>(lane < W ? red[lane] : empty_stat(), c);
+    if (lane == 0) part_s = s;
+  }
   if (a.top) {
-    // the top-th largest of the threads' maxima: the one with top - 1 above it
-    const uint64_t own = keys[threadIdx.x];
-    int place = 0;
-#pragma unroll 8
-    for (int j = 0; j < kThreads; ++j) place += keys[j] > own;
-    if (own && place == a.top - 1) bound_s = own;
+    // the top-th largest maximum of groups of threads, at least `top` of them
+    int lanes = 32;
+    while (kThreads / lanes < a.top) lanes /= 2;
+    uint64_t best = keys[threadIdx.x];
+    for (int o = lanes / 2; o > 0; o >>= 1) {
+      const uint64_t u = __shfl_xor_sync(0xffffffffu, best, o);
+      best = u > best ? u : best;
+    }
+    if (lane % lanes == 0) cand[threadIdx.x / lanes] = best;
     __syncthreads();
-    const uint64_t bound = bound_s;   // 0: fewer than `top` threads have an entry, so every entry counts
+    if (threadIdx.x < kThreads / lanes) {
+      const uint64_t own = cand[threadIdx.x];
+      int place = 0;
+      for (int j = 0; j < kThreads / lanes; ++j) place += cand[j] > own;
+      if (own && place == a.top - 1) bound_s = own;
+    }
+    const uint64_t own = keys[threadIdx.x];
+    __syncthreads();
+    const uint64_t bound = bound_s;   // 0: fewer than `top` groups have an entry, so every entry counts
     if (own && own >= bound) owners[atomicAdd(&owners_s, 1)] = threadIdx.x;
     __syncthreads();
     // the owners' entries at or above the bound: a larger value, or the same value in no later vector
@@ -482,21 +494,18 @@ __global__ void __launch_bounds__(kThreads) long_fwd_kernel(const Args a) {
   }
   const uint64_t* list = found;
   if (a.splits > 1) {
-    if (threadIdx.x == 0) part_s = all;
     __syncthreads();
     cluster_sync();
     if (rank == 0) {
       // join the parts, and rank their lists once more
       if (warp == 0) {
-        all = lane < a.splits ? *cluster_peer(&part_s, lane) : empty_stat();
-        all = group_join<kMaxSplits>(all, c);
+        const Stat s = group_join<kMaxSplits>(lane < a.splits ? *cluster_peer(&part_s, lane) : empty_stat(), c);
+        if (lane == 0) part_s2 = s;
       }
-      if (threadIdx.x == 0) part_s2 = all;
       const int n = a.splits * a.top;   // at most 8 x 64
       for (int k = threadIdx.x; k < n; k += kThreads) cand[k] = cluster_peer(found, k / a.top)[k % a.top];
       for (int k = threadIdx.x; k < a.top; k += kThreads) keys[k] = 0;
       __syncthreads();
-      all = part_s2;
       rank_keys(cand, n, a.top, keys);
       list = keys;
     }
@@ -505,6 +514,7 @@ __global__ void __launch_bounds__(kThreads) long_fwd_kernel(const Args a) {
     if (rank != 0) return;
   }
   __syncthreads();
+  const Stat all = a.splits > 1 ? part_s2 : part_s;
   for (int k = threadIdx.x; k < a.top; k += kThreads) write_top(a, r, k, list[k], all);
   if (threadIdx.x == 0) {
     const int64_t tok = a.tokens[r];
