@@ -79,41 +79,60 @@ template <int BN> struct Config {
   static constexpr int buffers = 512 / BN;   // TMEM has 512 columns
 };
 
-// The sums of a CTA's rows over one group: acc += sc * TMEM, `chunks` times 32
-// columns from `base`, the next chunk's load in flight while one is added. The
-// buffer is handed back (release()) once its last chunk is in registers.
+// The sums of a CTA's rows over one group: acc += sc * TMEM, `CHUNKS` times 32
+// columns from `base`. Two chunks are loaded at a time, and the next ones into
+// the registers of those that are added already. The buffer is handed back
+// (release()) once its last chunks are in registers.
 template <int CHUNKS, typename F>
 __device__ __forceinline__ void add_group(uint32_t base, float sc, float (&acc)[CHUNKS][32], F&& release) {
+  static_assert(CHUNKS % 2 == 0, "chunks are loaded in pairs");
   float v[2][32];
   tc::tmem_ld32_issue(base, v[0]);
+  tc::tmem_ld32_issue(base + 32, v[1]);
 #pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
+  for (int c = 0; c < CHUNKS; c += 2) {
     tc::tmem_ld_wait();
-    tc::tmem_regs_ready(v[c & 1]);
-    if (c + 1 < CHUNKS) tc::tmem_ld32_issue(base + 32 * (c + 1), v[(c + 1) & 1]);
-    else release();
+    tc::tmem_regs_ready(v[0]);
+    tc::tmem_regs_ready(v[1]);
+    if (c + 2 >= CHUNKS) release();
 #pragma unroll
-    for (int i = 0; i < 32; ++i) acc[c][i] = fmaf(v[c & 1][i], sc, acc[c][i]);
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) acc[c + j][i] = fmaf(v[j][i], sc, acc[c + j][i]);
+      if (c + 2 < CHUNKS) tc::tmem_ld32_issue(base + 32 * (c + 2 + j), v[j]);
+    }
   }
 }
 
 // The scales of one row of A and one row block of B, loaded four groups ahead
 // and multiplied only when they are used: a load has four groups' time to
-// arrive.
+// arrive. A row's scales come as one load of four or two of two where its
+// length and start are multiples of that: the lanes' rows lie apart, and with
+// single loads their accesses took 150 cycles of a group's 1190.
 struct Scales {
   const float* a;
   const float* b;
-  int groups;
+  int groups, width;
   float cur[4], na[4], nb[4];
   __device__ __forceinline__ void load(int kb) {
+    if (width == 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(a + kb));
+      na[0] = v.x, na[1] = v.y, na[2] = v.z, na[3] = v.w;
+    } else if (width == 2) {
+      const float2 v = __ldg(reinterpret_cast<const float2*>(a + kb));
+      const float2 u = __ldg(reinterpret_cast<const float2*>(a + min(kb + 2, groups - 2)));
+      na[0] = v.x, na[1] = v.y, na[2] = u.x, na[3] = u.y;
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int k = min(kb + j, groups - 1);
-      na[j] = __ldg(a + k);
-      nb[j] = __ldg(b + k);
+      for (int j = 0; j < 4; ++j) na[j] = __ldg(a + min(kb + j, groups - 1));
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) nb[j] = __ldg(b + min(kb + j, groups - 1));
   }
-  __device__ __forceinline__ Scales(const float* pa, const float* pb, int g) : a(pa), b(pb), groups(g) {
+  // `stride`: groups of a whole row; `groups`: of the part that starts at pa.
+  __device__ __forceinline__ Scales(const float* pa, const float* pb, int g, int stride) : a(pa), b(pb), groups(g) {
+    const int bits = stride | g | (int)(reinterpret_cast<uintptr_t>(pa) >> 2);
+    width = bits & 1 ? 1 : (bits & 2 ? 2 : 4);
     if (a && g > 0) load(0);
   }
   // Call for kb = 0, 1, 2, ...
@@ -205,7 +224,7 @@ __device__ __forceinline__ void epilogue(const Args& g, uint32_t tmem, uint32_t 
 #pragma unroll
       for (int i = 0; i < 32; ++i) acc[c][i] = 0.f;
     Scales sc(SCALED ? g.a_scale + (int64_t)min(row, g.M - 1) * G + kb0 : nullptr,
-              SCALED ? g.b_scale + (int64_t)min(n0 / kGroup, (g.N - 1) / kGroup) * G + kb0 : nullptr, kb1 - kb0);
+              SCALED ? g.b_scale + (int64_t)min(n0 / kGroup, (g.N - 1) / kGroup) * G + kb0 : nullptr, kb1 - kb0, G);
     for (int kb = kb0; kb < kb1; ++kb) {
       const float scale = SCALED ? sc.at(kb - kb0) : 1.f;
       const bool got = tc::mbar_wait(done0 + 8 * st.slot, st.round, g.wait_ns);
