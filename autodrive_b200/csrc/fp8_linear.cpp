@@ -36,12 +36,13 @@ torch::Tensor bf16_operand(const torch::Tensor& x) {
 
 struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& weight,
-                               const c10::optional<torch::Tensor>& bias_, int64_t out_dtype, const torch::Tensor& status) {
+                               const c10::optional<torch::Tensor>& bias_, int64_t out_dtype, bool grad,
+                               const torch::Tensor& status) {
     at::AutoDispatchBelowADInplaceOrView below;
     const c10::DeviceGuard guard(x.device());
     const torch::Tensor bias = bias_ ? *bias_ : torch::Tensor();
     const auto x2 = fp8::as_matrix(x);
-    const bool need_x = x.requires_grad(), need_w = weight.requires_grad();
+    const bool need_x = grad && x.requires_grad(), need_w = grad && weight.requires_grad();
     const auto xq = fp8::quantize_rows(x2);
     // the input gradient reads the weight down its columns: its transposed copy is written by the same pass
     const auto wq = fp8::quantize_blocks(fp8::as_matrix(weight), need_x);
@@ -70,7 +71,7 @@ struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
     const c10::DeviceGuard guard(grads[0].device());
     const auto g = fp8::as_matrix(grads[0]);
     const auto& status = saved[3];
-    variable_list out(5);
+    variable_list out(6);
     if (ctx->needs_input_grad(0)) {
       const auto gq = fp8::quantize_rows(g);
       out[0] = fp8::matmul(gq.first, gq.second, saved[1], saved[2], {},
@@ -102,7 +103,8 @@ torch::Tensor fp8_linear(torch::Tensor x, torch::Tensor weight, c10::optional<to
                     "fp8_linear needs all of its tensors on one device");
   TORCH_CHECK(status.scalar_type() == torch::kInt32, "fp8_linear: status must be int32");
   return Fp8LinearFn::apply(x, weight, bias,
-                            static_cast<int64_t>(torch::python::detail::py_object_to_dtype(dtype)), status);
+                            static_cast<int64_t>(torch::python::detail::py_object_to_dtype(dtype)),
+                            at::GradMode::is_enabled(), status);
 }
 
 }  // namespace

@@ -11,6 +11,8 @@ import torch
 from torch import nn
 from torch.distributions import Normal
 
+from ..ops.token_logprobs import token_log_probs
+
 OBS_DIM = 35
 ACTION_DIM = 3
 STRATEGIC_OBS_DIM = 137
@@ -72,6 +74,27 @@ class ActorCritic(nn.Module):
         dist = Normal(mean, log_std.exp())
         log_prob = dist.log_prob(latent).sum(-1) - torch.log(1 - actions.square() + 1e-6).sum(-1)
         return log_prob, dist.entropy().sum(-1), value, mean
+
+    @torch.no_grad()
+    def alternatives(self, obs: torch.Tensor, top: int = 3, action_mask=None):
+        """The `top` most probable actions of a categorical policy: (actions
+        [B, top], their log-probabilities, the distributions' entropies [B]).
+        Where fewer actions are valid, -1 and -inf; a row whose mask leaves
+        none counts every action."""
+        if self.action_kind != "categorical":
+            raise ValueError("alternatives need a categorical policy")
+        return most_probable(self(obs)[0], top, action_mask)
+
+
+def most_probable(logits: torch.Tensor, top: int, action_mask=None):
+    """(actions, log-probabilities, entropies) of the `top` most probable
+    entries of categorical logits (see ``ActorCritic.alternatives``)."""
+    if action_mask is not None:
+        action_mask = action_mask.bool()
+        action_mask = action_mask | ~action_mask.any(-1, keepdim=True)
+    nobody = torch.full(logits.shape[:-1], -1, dtype=torch.long, device=logits.device)
+    r = token_log_probs(logits.detach(), nobody, mask=action_mask, top=top)
+    return r.top_token, r.top_log_prob, r.entropy
 
 
 class DDPScore(nn.Module):

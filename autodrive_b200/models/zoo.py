@@ -45,6 +45,7 @@ from torch.nn.attention import SDPBackend, sdpa_kernel
 from ..ops.attention import supported as _tc_attention_supported, varlen_attention, varlen_query_attention
 from ..ops.layernorm import FusedLayerNorm
 from ..ops.tc_linear import _TcLinearFn, tensorize
+from .actor_critic import most_probable
 
 _SDPA_BACKENDS = [SDPBackend.EFFICIENT_ATTENTION, SDPBackend.FLASH_ATTENTION, SDPBackend.MATH]
 
@@ -555,6 +556,14 @@ class PerceptionActorCritic(nn.Module):
         dist = torch.distributions.Categorical(logits=logits)
         actions = actions.long().reshape(-1)
         return dist.log_prob(actions), dist.entropy(), value, logits
+
+    @torch.no_grad()
+    def alternatives(self, inputs: dict, top: int = 3, action_mask=None):
+        """The `top` most probable actions: (actions [B, top], their
+        log-probabilities, the distributions' entropies [B])."""
+        if action_mask is None:
+            action_mask = inputs["scalars"][:, -self.action_dim:] > .5
+        return most_probable(self(inputs)[0].float(), top, action_mask)
 
 
 def make_policy(architecture: str = "baseline_mlp", tensor_cores: bool = True):

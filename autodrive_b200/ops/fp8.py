@@ -249,7 +249,9 @@ def freeze_fp8(module: nn.Module, min_features: int = GROUP) -> nn.Module:
     """Replace, in place, every plain nn.Linear of `module` (recursively) whose
     two widths are at least `min_features` with a FrozenFp8Linear of its
     current weight: narrower layers, such as the policy heads, are not bound
-    by their weights and keep their precision. Returns the module."""
+    by their weights and keep their precision. Layers that ``tensorize`` has
+    put on the bf16 GEMM stay as they are (a policy to be frozen is built with
+    ``tensor_cores=False``). Returns the module."""
     for name, child in list(module.named_children()):
         if type(child) in (nn.Linear, Fp8Linear):
             if min(child.in_features, child.out_features) >= min_features:

@@ -114,7 +114,7 @@ class _Status:
             return
         e["host"].copy_(e["word"], non_blocking=True)
         ev = torch.cuda.Event()
-        ev.record()
+        ev.record(torch.cuda.current_stream(e["word"].device))   # the copy's stream, whatever the current device
         e["event"] = ev
 
     @classmethod

@@ -373,3 +373,41 @@ def test_changes_in_place_and_second_derivatives_are_refused():
     x += 1.   # the weight gradient would read it
     with pytest.raises(RuntimeError):
         y.sum().backward()
+
+
+@pytest.mark.gpu
+def test_frozen_raster_policy_acts_as_its_dequantised_weights_would():
+    """The raster network's wide layers (16640 -> 1408 -> 256) frozen: the logits against the same network with the
+    quantised weights and inputs in fp32, 16640 terms off by at most (K + 8) 2^-23 of their magnitudes each, which
+    moves a hidden value across a rounding of the next layer at times: one step of e4m3, 2^-3, of single values among
+    hundreds, well under 5 % of the logits. size."""
+    from autodrive_b200.models.zoo import PerceptionActorCritic
+    torch.manual_seed(0)
+    policy = PerceptionActorCritic("raster_cnn_large", tensor_cores=False).cuda()
+    inputs = {"scalars": torch.randn(5, 137, device="cuda"), "field": torch.rand(5, 12, 64, 128, device="cuda")}
+    freeze_fp8(policy)
+    frozen = [m for m in policy.modules() if isinstance(m, FrozenFp8Linear)]
+    assert len(frozen) == 3
+    with torch.no_grad():
+        got = policy(inputs)[0]
+        for m in frozen:
+            m.forward = lambda x, m=m: torch.nn.functional.linear(
+                dequantize_rows(*quantize_rows(x)), dequantize_blocks(m.weight_q, m.weight_scale), m.bias)
+        want = policy(inputs)[0]
+    check_gemm_status(torch.device("cuda", 0))
+    assert got.shape == (5, 8) and (got - want).abs().max() <= .05 * want.abs().max()
+
+
+@pytest.mark.gpu
+def test_no_gradient_is_prepared_where_none_is_taken():
+    x = torch.randn(40, 300, device="cuda", requires_grad=True)
+    w = torch.randn(130, 300, device="cuda", requires_grad=True)
+    with torch.no_grad():
+        y = fp8_linear(x, w)
+    assert not y.requires_grad and torch.equal(y, fp8_linear(x, w))
+    y = fp8_linear(x, w.detach())
+    gx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert gx.shape == x.shape
+    y = fp8_linear(x.detach(), w)
+    gw, = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert gw.shape == w.shape
