@@ -234,6 +234,15 @@ class FrozenFp8Linear(nn.Module):
         self.register_buffer("weight_scale", scale)
         self.register_buffer("bias", None if bias is None else bias.detach().float().clone())
 
+    def _apply(self, fn, recurse=True):
+        """Moves the buffers with the module and keeps their types and layout: ``half()`` or ``to(dtype)`` of a
+        network change its other layers, not the 8-bit numbers and their scales."""
+        for name, t in self._buffers.items():
+            if t is not None:
+                moved = t.to(fn(t.new_empty(0, dtype=torch.float32)).device)
+                self._buffers[name] = _padded_q(moved) if name == "weight_q" and moved is not t else moved
+        return self
+
     @classmethod
     def from_linear(cls, linear: nn.Linear) -> "FrozenFp8Linear":
         return cls(linear.weight, linear.bias)

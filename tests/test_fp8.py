@@ -411,3 +411,20 @@ def test_no_gradient_is_prepared_where_none_is_taken():
     y = fp8_linear(x.detach(), w)
     gw, = torch.autograd.grad(y, w, torch.ones_like(y))
     assert gw.shape == w.shape
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_frozen_layers_keep_their_types_when_the_network_is_converted(device):
+    net = freeze_fp8(nn.Sequential(nn.Linear(300, 200), nn.Linear(200, 5)))
+    x = torch.randn(4, 300)
+    with torch.no_grad():
+        want = net[0](x)
+        net.half().to(device)
+        layer = net[0]
+        assert layer.weight_q.dtype == torch.float8_e4m3fn and layer.weight_scale.dtype == layer.bias.dtype == torch.float32
+        assert layer.weight_q.device.type == device and layer.weight_q.stride(0) % 16 == 0
+        assert net[1].weight.dtype == torch.float16
+        got = layer(x.to(device))
+        assert net(x.half().to(device)).shape == (4, 5)
+    # fp32 sums of 300 terms of size 1 on either device
+    assert (got.cpu() - want).abs().max() <= 310 * E * 40
