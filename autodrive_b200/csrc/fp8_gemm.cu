@@ -481,8 +481,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
 }
 
 // ---- few rows --------------------------------------------------------------------
-// Up to 64 rows of A: bound by reading B. The operands change places, 128 rows
-// of B against COLS = 16, 32 or 64 rows of A, so that no tensor work is spent
+// Up to 32 rows of A: bound by reading B. The operands change places, 128 rows
+// of B against COLS = 16 or 32 rows of A, so that no tensor work is spent
 // on rows that are not there, and a cluster shares a tile's groups. A thread's
 // sums are one row of B against all rows of A, with a scale for each: the
 // products of the scales of the CTA's groups lie in shared memory.
@@ -869,15 +869,20 @@ torch::Tensor matmul(const torch::Tensor& a, const torch::Tensor& a_scale, const
   const int64_t lda = M > 1 ? a.stride(0) : one_row;
   const CUtensorMap tb = tma::u8_sw128(b.data_ptr(), N, K, N > 1 ? b.stride(0) : one_row, 128);
   auto st = c10::cuda::getCurrentCUDAStream().stream();
-  const int cols = M <= 16 ? 16 : (M <= 32 ? 32 : 64), splits = splits_for((N + kBM - 1) / kBM, g.groups);
-  if (M <= 64 && (g.groups + splits - 1) / splits * cols <= kRowsScales) {
+  // By sizes alone (us measured at N = K = 4096 unless said):
+  //  * up to 32 rows the few-row kernel, 7.9 against 10.1 with 128 x 128 tiles at 16 rows, 9.9 against 12.9 for one row
+  //    of 1408 x 16640, 9.1 against 10.8 at 32 rows (at 64 there is no difference: 11.1 and 10.9);
+  //  * 128 x 128 tiles, or parts of them, while one round of CTAs has them all: 18 against 24 with pairs for
+  //    1024 x 2048, where pairs leave half of the SMs idle;
+  //  * pairs of CTAs beyond: 25 against 31 for 2048 x 2048, 85 against 111 for 9472 x 2048.
+  const int cols = M <= 16 ? 16 : 32, splits = splits_for((N + kBM - 1) / kBM, g.groups);
+  if (M <= 32 && (g.groups + splits - 1) / splits * cols <= kRowsScales) {
     if (cols == 16) launch_rows<16>(tb, a, lda, g, splits, st);
-    else if (cols == 32) launch_rows<32>(tb, a, lda, g, splits, st);
-    else launch_rows<64>(tb, a, lda, g, splits, st);
+    else launch_rows<32>(tb, a, lda, g, splits, st);
   } else {
     const CUtensorMap ta = tma::u8_sw128(a.data_ptr(), M, K, lda, kBM);
-    const int64_t pair_tiles = ((M + 255) / 256) * ((N + 255) / 256);
-    if (pair_tiles >= lm::sm_count() / 2) launch_pair<false>(ta, tb, g, pair_tiles, st);
+    const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);
+    if (tiles > lm::sm_count()) launch_pair<false>(ta, tb, g, ((M + 255) / 256) * ((N + 255) / 256), st);
     else launch<128>(ta, tb, g, st);
   }
   lm::count_launches(1);
