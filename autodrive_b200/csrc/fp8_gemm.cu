@@ -292,14 +292,32 @@ __device__ __forceinline__ void store_one(const Args& g, int row, int col, float
   else reinterpret_cast<__half*>(g.c)[off] = __float2half_rn(v);
 }
 
+// Where the second CTA of a pair leaves, in the first, the number of groups whose tiles it has asked for.
+struct PairLink {
+  uint32_t rank;
+  uint32_t* issued;   // of the second CTA
+  uint32_t through;   // barrier: it asks for no more
+};
+
 // The producer's thread: `walk` calls load(k, row of A, row of B) for one
 // group's tiles after the other, until it answers false. Before it returns,
 // every load has landed and the products of every stage are complete: the
 // CTA's shared memory must not be given away before.
-template <int STAGES, bool BF16 = false, typename F>
+//
+// In a pair both CTAs' loads complete on the first CTA's barriers, each round
+// armed by both, and the first CTA sees to the landing of all of them (neither
+// ends before the other). Where a wait ran out, one CTA may have armed up to a
+// ring's rounds that the other has not: the first CTA arms those in its place.
+template <int STAGES, bool PAIR = false, bool BF16 = false, typename F>
 __device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, const CUtensorMap* tb, uint32_t smem0,
                                         uint32_t stage_bytes, uint32_t a_bytes, uint32_t full0, uint32_t done0,
-                                        int* s_fail, F&& walk) {
+                                        const PairLink& link, int* s_fail, F&& walk) {
+  static_assert(PAIR || !BF16, "bf16 tiles are the pairs' alone");
+  const uint32_t armed0 = PAIR ? tc::cluster_map(full0, 0) : full0;
+  const auto tile = [](uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if constexpr (PAIR) tc::tma_load_2d_pair(dst, map, x, y, bar);
+    else tc::tma_load_2d(dst, map, x, y, bar);
+  };
   Ring<STAGES> st;
   uint32_t issued = 0;
   bool ok = true;
@@ -308,29 +326,41 @@ __device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, co
       give_up(g, 1, s_fail);
       return ok = false;
     }
-    const uint32_t sa = smem0 + st.slot * stage_bytes, full = full0 + 8 * st.slot;
-    tc::mbar_arrive_expect_tx(full, stage_bytes);
+    const uint32_t sa = smem0 + st.slot * stage_bytes, full = armed0 + 8 * st.slot;
+    if constexpr (PAIR) tc::mbar_arrive_expect_tx_cluster(full, stage_bytes);
+    else tc::mbar_arrive_expect_tx(full, stage_bytes);
     if constexpr (BF16) {   // 64 rows by 128 columns, as two boxes of 64 columns
-      tc::tma_load_2d(sa, ta, row_a, k, full);
-      tc::tma_load_2d(sa + 8192, ta, row_a + 64, k, full);
-      tc::tma_load_2d(sa + a_bytes, tb, row_b, k, full);
-      tc::tma_load_2d(sa + a_bytes + 8192, tb, row_b + 64, k, full);
+      tile(sa, ta, row_a, k, full);
+      tile(sa + 8192, ta, row_a + 64, k, full);
+      tile(sa + a_bytes, tb, row_b, k, full);
+      tile(sa + a_bytes + 8192, tb, row_b + 64, k, full);
     } else {
-      tc::tma_load_2d(sa, ta, k, row_a, full);
-      tc::tma_load_2d(sa + a_bytes, tb, k, row_b, full);
+      tile(sa, ta, k, row_a, full);
+      tile(sa + a_bytes, tb, k, row_b, full);
     }
     st.next();
     ++issued;
     return true;
   });
-  for (uint32_t i = issued > (uint32_t)STAGES ? issued - STAGES : 0u; i < issued; ++i) {
-    const uint32_t slot = i % STAGES, round = (i / STAGES) & 1;
-    if (ok && !tc::mbar_wait(done0 + 8 * slot, round, g.wait_ns)) {
+  if (PAIR && link.rank == 1) {
+    tc::publish_cluster(tc::cluster_map(tc::smem_u32(link.issued), 0), issued, tc::cluster_map(link.through, 0));
+    return;
+  }
+  for (uint32_t i = issued > (uint32_t)STAGES ? issued - STAGES : 0u; ok && i < issued; ++i)
+    if (!tc::mbar_wait(done0 + 8 * (i % STAGES), (i / STAGES) & 1, g.wait_ns)) {
       give_up(g, 1, s_fail);
       ok = false;
     }
-    if (!ok && !tc::mbar_wait(full0 + 8 * slot, round, kDrainNs)) atomicOr(g.status, 16);
+  if (ok) return;
+  uint32_t end = issued;   // of the groups that have been asked for
+  if constexpr (PAIR) {
+    if (!tc::mbar_wait_cluster(link.through, 0, g.wait_ns + kDrainNs)) atomicOr(g.status, 16);
+    const uint32_t other = *(volatile uint32_t*)link.issued;
+    end = max(issued, other);
+    for (uint32_t i = min(issued, other); i < end; ++i) tc::mbar_arrive(full0 + 8 * (i % STAGES));
   }
+  for (uint32_t i = end > (uint32_t)STAGES ? end - STAGES : 0u; i < end; ++i)
+    if (!tc::mbar_wait(full0 + 8 * (i % STAGES), (i / STAGES) & 1, kDrainNs)) atomicOr(g.status, 16);
 }
 
 // The product thread: for each of `count` groups, once its tiles are loaded (in
@@ -340,21 +370,20 @@ __device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, co
 // the next group's barriers are looked at between the products.
 template <int STAGES, int BUFFERS, int COLS, bool PAIR, bool BF16 = false>
 __device__ __forceinline__ void multiply(const Args& g, uint32_t count, uint32_t smem0, uint32_t stage_bytes,
-                                         uint32_t a_bytes, uint32_t tmem, uint32_t full0, uint32_t peer0,
+                                         uint32_t a_bytes, uint32_t tmem, uint32_t full0,
                                          uint32_t done0, uint32_t tempty0, uint32_t drain, int* s_fail) {
   static_assert(!BF16 || PAIR, "bf16 tiles are the pairs' alone");
   const uint32_t id = BF16 ? tc::idesc_bf16(256, COLS, true, true) : tc::idesc_e4m3(PAIR ? 256 : 128, COLS);
   const uint32_t lo = BF16 ? tc::mnmajor64_desc_lo(smem0) : tc::kmajor_desc_lo(smem0);
   Ring<STAGES> st;
   Ring<BUFFERS> buf;
-  bool loaded = false, read = true, peer = !PAIR;   // the buffers' first round needs no waiting
+  bool loaded = false, read = true;   // the buffers' first round needs no waiting
   for (uint32_t it = 0; it < count; ++it) {
     if (!read && !tc::mbar_wait(tempty0 + 8 * buf.slot, buf.round ^ 1, g.wait_ns)) {
       give_up(g, 8, s_fail);
       break;
     }
-    if ((!loaded && !tc::mbar_wait(full0 + 8 * st.slot, st.round, g.wait_ns)) ||
-        (!peer && !tc::mbar_wait(peer0 + 8 * st.slot, st.round, g.wait_ns))) {
+    if (!loaded && !tc::mbar_wait(full0 + 8 * st.slot, st.round, g.wait_ns)) {
       give_up(g, 2, s_fail);
       break;
     }
@@ -372,7 +401,6 @@ __device__ __forceinline__ void multiply(const Args& g, uint32_t count, uint32_t
       if (ks == 1) {
         read = it + 1 < (uint32_t)BUFFERS || tc::mbar_try_wait(tempty0 + 8 * buf.slot, buf.round ^ 1);
         loaded = tc::mbar_try_wait(full0 + 8 * st.slot, st.round);
-        if constexpr (PAIR) peer = tc::mbar_try_wait(peer0 + 8 * st.slot, st.round);
       }
     }
     if constexpr (PAIR) tc::mma_commit_pair(done);
@@ -434,14 +462,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
   static_assert(kBM * kStride * 4 <= C::stages * C::stage_bytes, "the sums take the stages' place");
 
   if (warp == 0 && lane == 0) {
-    produce<C::stages>(g, &ta, &tb, smem0, C::stage_bytes, C::a_bytes, full0, done0, s_fail, [&](auto&& load) {
+    produce<C::stages>(g, &ta, &tb, smem0, C::stage_bytes, C::a_bytes, full0, done0, PairLink{}, s_fail, [&](auto&& load) {
       for (int w = first; w < total; w += step)
         for (int kb = kb0; kb < kb1; ++kb)
           if (!load(kb * kGroup, (w / tiles_n) * kBM, (w % tiles_n) * BN)) return;
     });
   } else if (warp == 1 && lane == 0) {
     const uint32_t tiles = (total - 1 - first) / step + 1;   // never more CTAs than tiles
-    multiply<C::stages, C::buffers, BN, false>(g, tiles * (kb1 - kb0), smem0, C::stage_bytes, C::a_bytes, tmem, full0, 0,
+    multiply<C::stages, C::buffers, BN, false>(g, tiles * (kb1 - kb0), smem0, C::stage_bytes, C::a_bytes, tmem, full0,
                                                done0, tempty0, drain, s_fail);
   } else if (warp >= 2) {
     const int q = warp & 3, half = (warp - 2) >> 2;
@@ -535,12 +563,12 @@ fp8_gemm_rows_kernel(const __grid_constant__ CUtensorMap tb, const __grid_consta
   float* sums = reinterpret_cast<float*>(smem);
 
   if (warp == 0 && lane == 0) {
-    produce<kRowsStages>(g, &tb, &ta, smem0, kStage, kBM * kGroup, full0, done0, s_fail, [&](auto&& load) {
+    produce<kRowsStages>(g, &tb, &ta, smem0, kStage, kBM * kGroup, full0, done0, PairLink{}, s_fail, [&](auto&& load) {
       for (int kb = kb0; kb < kb1; ++kb)
         if (!load(kb * kGroup, n0, 0)) return;
     });
   } else if (warp == 1 && lane == 0) {
-    multiply<kRowsStages, kRowsBuffers, COLS, false>(g, kb1 - kb0, smem0, kStage, kBM * kGroup, tmem, full0, 0, done0,
+    multiply<kRowsStages, kRowsBuffers, COLS, false>(g, kb1 - kb0, smem0, kStage, kBM * kGroup, tmem, full0, done0,
                                                      tempty0, drain, s_fail);
   } else if (warp >= 2) {
     const int q = warp & 3;
@@ -625,11 +653,12 @@ fp8_gemm_rows_kernel(const __grid_constant__ CUtensorMap tb, const __grid_consta
 // 128 KB with two of 128 x 128.
 //   warp 0      producer of the CTA's own tiles, into its own ring;
 //   warp 1      first CTA: issues the pair's products once both CTAs' tiles are
-//               there; second CTA: tells the first when its tiles have arrived;
+//               there, for which it waits on one barrier of its own, as the
+//               loads of both complete on that;
 //   warps 4-11  epilogue, as above; warps 2 and 3 only complete the warpgroup
 //               that gives up its registers to the epilogue's 128 sums a thread.
-// Every CTA waits for its own loads before it ends, and both meet at a cluster
-// barrier before either frees its TMEM or shared memory.
+// The first CTA waits for the loads of both before it ends, and both meet at a
+// cluster barrier before either frees its TMEM or shared memory.
 constexpr int kPairThreads = 384, kPairStages = 6, kPairBuffers = 2;
 constexpr uint32_t kPairTile = 128 * kGroup, kPairStage = 2 * kPairTile;
 constexpr uint32_t kPairSmem = kPairStages * kPairStage + kEpiWarps * kStoreStage + 1024 + 256;
@@ -647,13 +676,13 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* stage0 = smem + kPairStages * kPairStage;
   uint8_t* misc = stage0 + kEpiWarps * kStoreStage;
-  const uint32_t full0 = tc::smem_u32(misc);                  // own tiles loaded
-  const uint32_t peer0 = full0 + 8 * kPairStages;             // first CTA: the second one's tiles loaded
-  const uint32_t done0 = peer0 + 8 * kPairStages;             // stage's products complete
+  const uint32_t full0 = tc::smem_u32(misc);                  // first CTA: both CTAs' tiles loaded
+  const uint32_t done0 = full0 + 8 * kPairStages;             // stage's products complete
   const uint32_t tempty0 = done0 + 8 * kPairStages;           // first CTA: TMEM buffer read out by both
-  const uint32_t drain = tempty0 + 8 * kPairBuffers;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (3 * kPairStages + kPairBuffers + 1));
+  const uint32_t drain = tempty0 + 8 * kPairBuffers, through = drain + 8;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (2 * kPairStages + kPairBuffers + 2));
   int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
+  uint32_t* s_issued = s_tmem + 2;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_rank();
@@ -672,15 +701,16 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
     tc::tma_prefetch_map(&ta);
     tc::tma_prefetch_map(&tb);
     for (int s = 0; s < kPairStages; ++s) {
-      tc::mbar_init(full0 + 8 * s, 1);
-      tc::mbar_init(peer0 + 8 * s, 1);
+      tc::mbar_init(full0 + 8 * s, 2);   // both producers
       tc::mbar_init(done0 + 8 * s, 1);
     }
     for (int b = 0; b < kPairBuffers; ++b)
       tc::mbar_init(tempty0 + 8 * b, 2 * kEpiWarps);   // one lane of every epilogue warp of both CTAs
     tc::mbar_init(drain, 1);
+    tc::mbar_init(through, 1);
     tc::mbar_init_fence();
     *s_fail = 0;
+    *s_issued = 0;
   }
   if (warp == 1) {
     tc::tmem_alloc_pair(tc::smem_u32(s_tmem), 512);
@@ -695,7 +725,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
   if (warp < 4) {
     tc::regs_dec<40>();
     if (warp == 0 && lane == 0) {
-      produce<kPairStages, BF16>(g, &ta, &tb, smem0, kPairStage, kPairTile, full0, done0, s_fail, [&](auto&& load) {
+      const PairLink link{rank, s_issued, through};
+      produce<kPairStages, true, BF16>(g, &ta, &tb, smem0, kPairStage, kPairTile, full0, done0, link, s_fail, [&](auto&& load) {
         for (int w = pair; w < total; w += pairs) {
           const int2 kb = range(w);
           const int m0 = (w % tiles / tiles_n) * 256 + (int)rank * 128, n0 = (w % tiles_n) * 256 + (int)rank * 128;
@@ -704,18 +735,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
         }
       });
     } else if (warp == 1 && lane == 0 && rank == 0) {
-      multiply<kPairStages, kPairBuffers, 256, true, BF16>(g, count, smem0, kPairStage, kPairTile, tmem, full0, peer0, done0,
+      multiply<kPairStages, kPairBuffers, 256, true, BF16>(g, count, smem0, kPairStage, kPairTile, tmem, full0, done0,
                                                            tempty0, drain, s_fail);
-    } else if (warp == 1 && lane == 0) {
-      const uint32_t peer = tc::cluster_map(peer0, 0);
-      Ring<kPairStages> st;
-      for (uint32_t it = 0; it < count; ++it, st.next()) {
-        if (!tc::mbar_wait(full0 + 8 * st.slot, st.round, g.wait_ns)) {
-          give_up(g, 2, s_fail);
-          break;
-        }
-        tc::mbar_arrive_cluster(peer + 8 * st.slot);
-      }
     }
     __syncwarp();
   } else {

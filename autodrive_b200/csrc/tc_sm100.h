@@ -276,10 +276,44 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Arrive on a barrier of any CTA of the cluster (an address from cluster_map).
-// For handing over what the tensor cores and the TMA unit read and write; with
-// cluster-scope release semantics an arrival takes 320 cycles instead of 16.
+// Nothing that this thread wrote or saw written is handed over: for TMEM that
+// it has read out (tcgen05.wait::ld is behind it), where the other CTA needs
+// to know only that the reads are over.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t mapped) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(mapped) : "memory");
+}
+// A number written into the first CTA's shared memory, and the arrival that
+// publishes it: mbar_wait_cluster's caller may read it. An arrival with
+// cluster-scope release semantics takes 320 cycles.
+__device__ __forceinline__ void publish_cluster(uint32_t mapped, uint32_t value, uint32_t mapped_bar) {
+  asm volatile(
+      "st.shared::cluster.u32 [%0], %1;\n mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%2];"
+      :: "r"(mapped), "r"(value), "r"(mapped_bar) : "memory");
+}
+// mbar_wait for what another CTA of the cluster has published.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+    if (globaltimer_ns() - t0 > limit_ns) return false;
+  }
+}
+// Loads of either CTA of a pair that complete on a barrier of the first: it is
+// armed by both (mapped address), and the loaded tiles lie in the issuing CTA.
+// The products that read both CTAs' tiles then need no other hand-over.
+__device__ __forceinline__ void mbar_arrive_expect_tx_cluster(uint32_t mapped, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" :: "r"(mapped), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* map, int x, int y, uint32_t mapped_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];"
+      :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(mapped_bar) : "memory");
 }
 // Whole-warp operations, by one warp of each CTA of the pair.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {

@@ -428,3 +428,28 @@ def test_frozen_layers_keep_their_types_when_the_network_is_converted(device):
         assert net(x.half().to(device)).shape == (4, 5)
     # fp32 sums of 300 terms of size 1 on either device
     assert (got.cpu() - want).abs().max() <= 310 * E * 40
+
+
+@pytest.mark.gpu
+def test_pairs_of_ctas_read_each_others_tiles_when_they_are_there():
+    """Two sets of operands of other sizes of value in turn, a different value in every group of 128: a tile that the
+    pair's products read before the second CTA's loads have landed would be the other call's or an earlier group's.
+    Products and weight gradients are sums of small integers, below 2^24, so every order of addition gives them exactly."""
+    def operands(seed):
+        g = _gen(seed)
+        a = torch.randint(-3 * seed, 3 * seed + 1, (2500, 1408), generator=g).float()
+        b = torch.randint(-3, 4, (1500, 1408), generator=g).float()
+        q = [t.to(fp8.E4M3).cuda() for t in (a, b)]
+        scales = (torch.arange(1, 12).float().repeat(2500, 1).cuda(), torch.ones(12, 11).cuda())
+        want = ((a * torch.arange(1, 12).repeat_interleave(128)).double() @ b.double().t()).cuda()
+        dy = torch.randint(-3 * seed, 3 * seed + 1, (5000, 520), generator=g).float().bfloat16().cuda()
+        x = torch.randint(-3, 4, (5000, 648), generator=g).float().bfloat16().cuda()
+        return q, scales, want.float(), dy, x, (dy.double().t() @ x.double()).float()
+
+    sets = [operands(1), operands(4)]
+    w = torch.zeros(520, 648, device="cuda", requires_grad=True)
+    for _ in range(40):
+        for (a, b), (a_s, b_s), want, dy, x, dw in sets:
+            assert torch.equal(fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32), want)
+            assert torch.equal(torch.autograd.grad(fp8_linear(x, w), w, dy)[0], dw)
+    check_gemm_status(torch.device("cuda", 0))
