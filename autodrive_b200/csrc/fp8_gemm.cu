@@ -18,7 +18,9 @@
 //              a whole round behind);
 //   warps 2-9  two per TMEM lane quadrant: thread = one row, half the columns.
 // Waits are bounded and reported as in the bf16 GEMM (tc_gemm.cu), with the
-// same status bits and the same drains before the CTA gives up its TMEM.
+// same status bits; whichever wait runs out, the producer sees its loads land and
+// the product thread its last products complete before the CTA gives up its
+// shared memory and TMEM.
 #include <torch/extension.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -57,12 +59,6 @@ struct Args {
   int* status;
   uint64_t wait_ns;
 };
-
-// Records that a wait of the role with this status bit ran out.
-__device__ __forceinline__ void give_up(const Args& g, int bit, int* s_fail) {
-  atomicOr(g.status, bit);
-  atomicExch(s_fail, 1);
-}
 
 // A place in a ring of N slots and the parity of its current round.
 template <int N> struct Ring {
@@ -208,7 +204,7 @@ __device__ __forceinline__ void store_rows(const Args& g, float (&acc)[CHUNKS][3
 // other; sink(sums, row, first column) gets each tile's sums. `tempty0` may
 // lie in another CTA (a mapped address).
 template <int STAGES, int BUFFERS, int COLS, bool SCALED = true, typename F, typename S>
-__device__ __forceinline__ void epilogue(const Args& g, uint32_t tmem, uint32_t done0, uint32_t tempty0, int* s_fail,
+__device__ __forceinline__ void epilogue(const Args& g, uint32_t tmem, uint32_t done0, uint32_t tempty0,
                                          int q, int half, F&& walk, S&& sink) {
   constexpr int kChunks = COLS / 64;   // 32-column chunks per warp
   const int lane = threadIdx.x & 31, G = g.groups;
@@ -229,7 +225,7 @@ __device__ __forceinline__ void epilogue(const Args& g, uint32_t tmem, uint32_t 
       const float scale = SCALED ? sc.at(kb - kb0) : 1.f;
       const bool got = tc::mbar_wait(done0 + 8 * st.slot, st.round, g.wait_ns);
       if (!__all_sync(0xffffffffu, got)) {   // the loads below are whole-warp
-        give_up(g, 4, s_fail);
+        atomicOr(g.status, 4);
         return false;
       }
       tc::tc_fence_after();
@@ -311,7 +307,7 @@ struct PairLink {
 template <int STAGES, bool PAIR = false, bool BF16 = false, typename F>
 __device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, const CUtensorMap* tb, uint32_t smem0,
                                         uint32_t stage_bytes, uint32_t a_bytes, uint32_t full0, uint32_t done0,
-                                        const PairLink& link, int* s_fail, F&& walk) {
+                                        const PairLink& link, F&& walk) {
   static_assert(PAIR || !BF16, "bf16 tiles are the pairs' alone");
   const uint32_t armed0 = PAIR ? tc::cluster_map(full0, 0) : full0;
   const auto tile = [](uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -323,7 +319,7 @@ __device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, co
   bool ok = true;
   walk([&](int k, int row_a, int row_b) {
     if (issued >= STAGES && !tc::mbar_wait(done0 + 8 * st.slot, st.round ^ 1, g.wait_ns)) {
-      give_up(g, 1, s_fail);
+      atomicOr(g.status, 1);
       return ok = false;
     }
     const uint32_t sa = smem0 + st.slot * stage_bytes, full = armed0 + 8 * st.slot;
@@ -348,7 +344,7 @@ __device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, co
   }
   for (uint32_t i = issued > (uint32_t)STAGES ? issued - STAGES : 0u; ok && i < issued; ++i)
     if (!tc::mbar_wait(done0 + 8 * (i % STAGES), (i / STAGES) & 1, g.wait_ns)) {
-      give_up(g, 1, s_fail);
+      atomicOr(g.status, 1);
       ok = false;
     }
   if (ok) return;
@@ -367,29 +363,33 @@ __device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, co
 // both CTAs of a pair) and the TMEM buffer is read out, issue its four products
 // and one commit, for the producer and the epilogue alike. Products take 48
 // cycles to issue, commits 59 and successful waits 40, one after the other, so
-// the next group's barriers are looked at between the products.
+// the next group's barriers are looked at between the products. Before it
+// returns, its last products are complete.
 template <int STAGES, int BUFFERS, int COLS, bool PAIR, bool BF16 = false>
 __device__ __forceinline__ void multiply(const Args& g, uint32_t count, uint32_t smem0, uint32_t stage_bytes,
                                          uint32_t a_bytes, uint32_t tmem, uint32_t full0,
-                                         uint32_t done0, uint32_t tempty0, uint32_t drain, int* s_fail) {
+                                         uint32_t done0, uint32_t tempty0) {
   static_assert(!BF16 || PAIR, "bf16 tiles are the pairs' alone");
   const uint32_t id = BF16 ? tc::idesc_bf16(256, COLS, true, true) : tc::idesc_e4m3(PAIR ? 256 : 128, COLS);
   const uint32_t lo = BF16 ? tc::mnmajor64_desc_lo(smem0) : tc::kmajor_desc_lo(smem0);
-  Ring<STAGES> st;
+  Ring<STAGES> st, last;
   Ring<BUFFERS> buf;
+  uint32_t issued = 0;
   bool loaded = false, read = true;   // the buffers' first round needs no waiting
   for (uint32_t it = 0; it < count; ++it) {
     if (!read && !tc::mbar_wait(tempty0 + 8 * buf.slot, buf.round ^ 1, g.wait_ns)) {
-      give_up(g, 8, s_fail);
+      atomicOr(g.status, 8);
       break;
     }
     if (!loaded && !tc::mbar_wait(full0 + 8 * st.slot, st.round, g.wait_ns)) {
-      give_up(g, 2, s_fail);
+      atomicOr(g.status, 2);
       break;
     }
     tc::tc_fence_after();
     const uint32_t la = lo + st.slot * (stage_bytes >> 4), lb = la + (a_bytes >> 4), d = tmem + buf.slot * COLS;
     const uint32_t done = done0 + 8 * st.slot;
+    last = st;
+    ++issued;
     st.next();
     buf.next();
 #pragma unroll
@@ -406,11 +406,9 @@ __device__ __forceinline__ void multiply(const Args& g, uint32_t count, uint32_t
     if constexpr (PAIR) tc::mma_commit_pair(done);
     else tc::mma_commit(done);
   }
-  if (*(volatile int*)s_fail) {   // products issued so far may still read shared memory and write TMEM
-    if constexpr (PAIR) tc::mma_commit_pair(drain);
-    else tc::mma_commit(drain);
-    if (!tc::mbar_wait(drain, 0, kDrainNs)) atomicOr(g.status, 32);
-  }
+  // The last commit covers all products: whoever's wait has run out or runs out yet, they are through with shared
+  // memory and TMEM before the CTA gives those up.
+  if (issued && !tc::mbar_wait(done0 + 8 * last.slot, last.round, kDrainNs)) atomicOr(g.status, 32);
 }
 
 template <int BN>
@@ -424,9 +422,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
   const uint32_t full0 = tc::smem_u32(misc);                    // stage loaded
   const uint32_t done0 = full0 + 8 * C::stages;                 // stage's products complete
   const uint32_t tempty0 = done0 + 8 * C::stages;               // TMEM buffer read out
-  const uint32_t drain = tempty0 + 8 * C::buffers;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (2 * C::stages + C::buffers + 1));
-  int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (2 * C::stages + C::buffers));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles_n = (g.N + BN - 1) / BN, tiles_m = (g.M + kBM - 1) / kBM;
@@ -440,9 +436,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
       tc::mbar_init(done0 + 8 * s, 1);
     }
     for (int b = 0; b < C::buffers; ++b) tc::mbar_init(tempty0 + 8 * b, kEpiWarps);   // one lane of every epilogue warp
-    tc::mbar_init(drain, 1);
     tc::mbar_init_fence();
-    *s_fail = 0;
   }
   if (warp == 1) {
     tc::tmem_alloc(tc::smem_u32(s_tmem), 512);
@@ -462,7 +456,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
   static_assert(kBM * kStride * 4 <= C::stages * C::stage_bytes, "the sums take the stages' place");
 
   if (warp == 0 && lane == 0) {
-    produce<C::stages>(g, &ta, &tb, smem0, C::stage_bytes, C::a_bytes, full0, done0, PairLink{}, s_fail, [&](auto&& load) {
+    produce<C::stages>(g, &ta, &tb, smem0, C::stage_bytes, C::a_bytes, full0, done0, PairLink{}, [&](auto&& load) {
       for (int w = first; w < total; w += step)
         for (int kb = kb0; kb < kb1; ++kb)
           if (!load(kb * kGroup, (w / tiles_n) * kBM, (w % tiles_n) * BN)) return;
@@ -470,11 +464,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
   } else if (warp == 1 && lane == 0) {
     const uint32_t tiles = (total - 1 - first) / step + 1;   // never more CTAs than tiles
     multiply<C::stages, C::buffers, BN, false>(g, tiles * (kb1 - kb0), smem0, C::stage_bytes, C::a_bytes, tmem, full0,
-                                               done0, tempty0, drain, s_fail);
+                                               done0, tempty0);
   } else if (warp >= 2) {
     const int q = warp & 3, half = (warp - 2) >> 2;
     epilogue<C::stages, C::buffers, BN>(
-        g, tmem, done0, tempty0, s_fail, q, half,
+        g, tmem, done0, tempty0, q, half,
         [&](auto&& tile) {
           for (int w = first; w < total; w += step)
             if (!tile((w / tiles_n) * kBM, (w % tiles_n) * BN, kb0, kb1)) return;
@@ -532,9 +526,7 @@ fp8_gemm_rows_kernel(const __grid_constant__ CUtensorMap tb, const __grid_consta
   float* scales = reinterpret_cast<float*>(smem + kRowsStages * kStage);   // [group][COLS]
   uint8_t* misc = reinterpret_cast<uint8_t*>(scales + kRowsScales);
   const uint32_t full0 = tc::smem_u32(misc), done0 = full0 + 8 * kRowsStages, tempty0 = done0 + 8 * kRowsStages;
-  const uint32_t drain = tempty0 + 8 * kRowsBuffers;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (2 * kRowsStages + kRowsBuffers + 1));
-  int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (2 * kRowsStages + kRowsBuffers));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = g.groups;
   const int splits = g.splits, rank = splits > 1 ? (int)tc::cluster_rank() : 0, n0 = (blockIdx.x / splits) * kBM;
@@ -548,9 +540,7 @@ fp8_gemm_rows_kernel(const __grid_constant__ CUtensorMap tb, const __grid_consta
       tc::mbar_init(done0 + 8 * s, 1);
     }
     for (int b = 0; b < kRowsBuffers; ++b) tc::mbar_init(tempty0 + 8 * b, 4);
-    tc::mbar_init(drain, 1);
     tc::mbar_init_fence();
-    *s_fail = 0;
   }
   if (warp == 1) {
     tc::tmem_alloc(tc::smem_u32(s_tmem), kTmem);
@@ -563,13 +553,13 @@ fp8_gemm_rows_kernel(const __grid_constant__ CUtensorMap tb, const __grid_consta
   float* sums = reinterpret_cast<float*>(smem);
 
   if (warp == 0 && lane == 0) {
-    produce<kRowsStages>(g, &tb, &ta, smem0, kStage, kBM * kGroup, full0, done0, PairLink{}, s_fail, [&](auto&& load) {
+    produce<kRowsStages>(g, &tb, &ta, smem0, kStage, kBM * kGroup, full0, done0, PairLink{}, [&](auto&& load) {
       for (int kb = kb0; kb < kb1; ++kb)
         if (!load(kb * kGroup, n0, 0)) return;
     });
   } else if (warp == 1 && lane == 0) {
     multiply<kRowsStages, kRowsBuffers, COLS, false>(g, kb1 - kb0, smem0, kStage, kBM * kGroup, tmem, full0, done0,
-                                                     tempty0, drain, s_fail);
+                                                     tempty0);
   } else if (warp >= 2) {
     const int q = warp & 3;
     const float* bs = g.b_scale + (int64_t)(n0 / kGroup) * G;
@@ -589,7 +579,7 @@ fp8_gemm_rows_kernel(const __grid_constant__ CUtensorMap tb, const __grid_consta
     for (int kb = kb0; kb < kb1; ++kb) {
       const bool got = tc::mbar_wait(done0 + 8 * st.slot, st.round, g.wait_ns);
       if (!__all_sync(0xffffffffu, got)) {
-        give_up(g, 4, s_fail);
+        atomicOr(g.status, 4);
         break;
       }
       tc::tc_fence_after();
@@ -679,10 +669,9 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
   const uint32_t full0 = tc::smem_u32(misc);                  // first CTA: both CTAs' tiles loaded
   const uint32_t done0 = full0 + 8 * kPairStages;             // stage's products complete
   const uint32_t tempty0 = done0 + 8 * kPairStages;           // first CTA: TMEM buffer read out by both
-  const uint32_t drain = tempty0 + 8 * kPairBuffers, through = drain + 8;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (2 * kPairStages + kPairBuffers + 2));
-  int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
-  uint32_t* s_issued = s_tmem + 2;
+  const uint32_t through = tempty0 + 8 * kPairBuffers;         // first CTA: the second one's producer is through
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (2 * kPairStages + kPairBuffers + 1));
+  uint32_t* s_issued = s_tmem + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_rank();
@@ -706,10 +695,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
     }
     for (int b = 0; b < kPairBuffers; ++b)
       tc::mbar_init(tempty0 + 8 * b, 2 * kEpiWarps);   // one lane of every epilogue warp of both CTAs
-    tc::mbar_init(drain, 1);
     tc::mbar_init(through, 1);
     tc::mbar_init_fence();
-    *s_fail = 0;
     *s_issued = 0;
   }
   if (warp == 1) {
@@ -726,7 +713,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
     tc::regs_dec<40>();
     if (warp == 0 && lane == 0) {
       const PairLink link{rank, s_issued, through};
-      produce<kPairStages, true, BF16>(g, &ta, &tb, smem0, kPairStage, kPairTile, full0, done0, link, s_fail, [&](auto&& load) {
+      produce<kPairStages, true, BF16>(g, &ta, &tb, smem0, kPairStage, kPairTile, full0, done0, link, [&](auto&& load) {
         for (int w = pair; w < total; w += pairs) {
           const int2 kb = range(w);
           const int m0 = (w % tiles / tiles_n) * 256 + (int)rank * 128, n0 = (w % tiles_n) * 256 + (int)rank * 128;
@@ -736,14 +723,14 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
       });
     } else if (warp == 1 && lane == 0 && rank == 0) {
       multiply<kPairStages, kPairBuffers, 256, true, BF16>(g, count, smem0, kPairStage, kPairTile, tmem, full0, done0,
-                                                           tempty0, drain, s_fail);
+                                                           tempty0);
     }
     __syncwarp();
   } else {
     tc::regs_inc<216>();
     Args out = g;
     epilogue<kPairStages, kPairBuffers, 256, !BF16>(
-        g, tmem, done0, tc::cluster_map(tempty0, 0), s_fail, warp & 3, (warp - 4) >> 2,
+        g, tmem, done0, tc::cluster_map(tempty0, 0), warp & 3, (warp - 4) >> 2,
         [&](auto&& tile) {
           for (int w = pair; w < total; w += pairs) {
             const int2 kb = range(w);

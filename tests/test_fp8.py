@@ -453,3 +453,24 @@ def test_pairs_of_ctas_read_each_others_tiles_when_they_are_there():
             assert torch.equal(fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32), want)
             assert torch.equal(torch.autograd.grad(fp8_linear(x, w), w, dy)[0], dw)
     check_gemm_status(torch.device("cuda", 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(20000, 512, 2048), (300, 512, 2048), (4, 512, 2048), (4, 512, 512), (40, 300, 128)])
+def test_waits_of_any_length_leave_nothing_in_flight(m, n, k):
+    """Waits that run out somewhere between the first load and the last product, or not at all: the call either reports
+    them or is right, and the next call on the same shared memory and TMEM is right in any case."""
+    dev = torch.device("cuda", 0)
+    a, a_s = quantize_rows(_values(m, k, 1, device="cuda"))
+    b, b_s = quantize_blocks(_values(n, k, 2, device="cuda"))
+    want = fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32)
+    check_gemm_status(dev)
+    for wait_ns in (0, 200, 500, 1000, 1500, 2000, 3000, 5000, 10000, 20000) * 3:
+        y = fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32, wait_ns=wait_ns)
+        z = fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32)
+        try:
+            check_gemm_status(dev)
+        except TensorCoreTimeout:
+            y = want
+        assert torch.equal(y, want) and torch.equal(z, want)
+    check_gemm_status(dev)
