@@ -379,7 +379,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ C
         atomicOr(g.status, 4);
         atomicExch(s_fail, 1);
       }
-      if (!got || *fail) break;
+      if (!__all_sync(0xffffffffu, got && !*fail)) break;   // one answer a warp: its TMEM loads are whole-warp
       tc::tc_fence_after();
       const int row = t.m0 + 32 * q + lane;
       const uint32_t base = tmem + acc * kAccCols + ((uint32_t)(32 * q) << 16);
