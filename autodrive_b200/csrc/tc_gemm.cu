@@ -246,7 +246,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ C
   const uint32_t tempty0 = tfull0 + 16;                  // 2 mbarriers: accumulator read out
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (2 * kStages + 4));
   int* s_fail = reinterpret_cast<int*>(misc + 8 * (2 * kStages + 4) + 8);
-  const uint32_t drain = tc::smem_u32(misc + 8 * (2 * kStages + 4) + 16);  // MMA drain after a failure
+  const uint32_t drain = tc::smem_u32(misc + 8 * (2 * kStages + 4) + 16);  // MMA drain
   volatile int* fail = s_fail;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -309,12 +309,11 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ C
         }
       }
     }
-    if (*fail) {
-      // `it` loads were issued; every stage's latest one may still be in
-      // flight (earlier ones were consumed). Wait for them to land.
-      for (uint32_t i = it > (uint32_t)kStages ? it - kStages : 0u; i < it; ++i)
-        if (!tc::mbar_wait(full0 + 8 * (i % kStages), (i / kStages) & 1, kDrainNs)) atomicOr(g.status, 16);
-    }
+    // `it` loads were issued; every stage's latest one may still be in flight
+    // (earlier ones were consumed). Wait for them to land, also where no wait
+    // has run out yet: one may still.
+    for (uint32_t i = it > (uint32_t)kStages ? it - kStages : 0u; i < it; ++i)
+      if (!tc::mbar_wait(full0 + 8 * (i % kStages), (i / kStages) & 1, kDrainNs)) atomicOr(g.status, 16);
   } else if (warp == 1 && lane == 0) {
     // ---- MMA issuer: tile lt accumulates into TMEM columns (lt & 1) * 128 ----
     const uint32_t id = tc::idesc_bf16(kBM, BN, A_MN, B_MN);
@@ -354,11 +353,10 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ C
       tc::mma_commit(tfull0 + 8 * acc);   // accumulator complete (or nothing issued)
       if (!ok) break;
     }
-    if (*fail) {
-      // MMAs issued so far may still read shared memory / write TMEM
-      tc::mma_commit(drain);
-      if (!tc::mbar_wait(drain, 0, kDrainNs)) atomicOr(g.status, 32);
-    }
+    // MMAs issued so far may still read shared memory / write TMEM, whether or
+    // not the epilogue's wait for them runs out
+    tc::mma_commit(drain);
+    if (!tc::mbar_wait(drain, 0, kDrainNs)) atomicOr(g.status, 32);
   }
 
   if (warp >= 2) {

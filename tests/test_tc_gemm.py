@@ -231,3 +231,26 @@ def test_gemm_wait_expiry_is_reported_and_context_survives():
     check_gemm_status()
     ref = a.float() @ b.float().T
     assert (out - ref).abs().max().item() < 1e-3 * ref.abs().max().item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(20000, 512, 1024), (300, 512, 512), (64, 128, 256), (40, 128, 64)])
+def test_gemm_waits_of_any_length_leave_nothing_in_flight(m, n, k):
+    """Wait limits that run out somewhere between the first load and the last
+    MMA, or not at all: the call reports them or is right, and the next GEMM on
+    the same shared memory and TMEM is right in any case."""
+    from autodrive_b200.ops.tc_linear import TensorCoreTimeout, check_gemm_status
+    g = torch.Generator(device="cuda").manual_seed(12)
+    a = torch.randn(m, k, device="cuda", generator=g).bfloat16()
+    b = torch.randn(n, k, device="cuda", generator=g).bfloat16()
+    want = gemm(a, b)
+    check_gemm_status()
+    for wait_ns in (0, 200, 500, 1000, 1500, 2000, 3000, 5000, 10000, 20000) * 3:
+        y = gemm(a, b, wait_ns=wait_ns)
+        z = gemm(a, b)
+        try:
+            check_gemm_status()
+        except TensorCoreTimeout:
+            y = want
+        assert torch.equal(y, want) and torch.equal(z, want)
+    check_gemm_status()
