@@ -102,6 +102,7 @@ torch::Tensor fp8_linear(torch::Tensor x, torch::Tensor weight, c10::optional<to
                         (!bias || bias->device() == x.device()),
                     "fp8_linear needs all of its tensors on one device");
   TORCH_CHECK(status.scalar_type() == torch::kInt32, "fp8_linear: status must be int32");
+  LM_CHECK_NO_TANGENT("fp8_linear", x, weight, bias);
   return Fp8LinearFn::apply(x, weight, bias,
                             static_cast<int64_t>(torch::python::detail::py_object_to_dtype(dtype)),
                             at::GradMode::is_enabled(), status);

@@ -1,6 +1,7 @@
 // Host-side helpers of the language-model operators.
 #pragma once
 
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAException.h>
 #include <cuda_runtime.h>
 #include <torch/extension.h>
@@ -32,6 +33,20 @@ std::string message(const A&... parts) {
 }
 // Raises ValueError in Python.
 #define LM_CHECK_VALUE(cond, ...) TORCH_CHECK_VALUE(cond, ::lm::message(__VA_ARGS__))
+
+// Whether `t` carries a derivative of forward-mode differentiation (which
+// neither requires_grad nor the gradient mode tells).
+inline bool has_tangent(const torch::Tensor& t) {
+  return t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined();
+}
+inline bool has_tangent(const c10::optional<torch::Tensor>& t) { return t && has_tangent(*t); }
+// Raises NotImplementedError in Python.
+#define LM_CHECK_NO_TANGENT(name, ...) \
+  TORCH_CHECK_NOT_IMPLEMENTED(!::lm::any_tangent(__VA_ARGS__), name " has no forward-mode derivative")
+template <typename... T>
+bool any_tangent(const T&... t) {
+  return (has_tangent(t) || ...);
+}
 
 // Kernels launched by the operators whose autograd lives in this extension;
 // utils/launches.py adds it to its own count.

@@ -553,6 +553,7 @@ struct RmsNormFn : torch::autograd::Function<RmsNormFn> {
 // y, or (y, h) with a residual.
 py::object rms_norm(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual, double eps) {
   check_args(x, weight, residual);
+  LM_CHECK_NO_TANGENT("rms_norm", x, weight, residual);
   const torch::Tensor res = residual ? *residual : torch::Tensor();
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || weight.requires_grad() || (res.defined() && res.requires_grad()))) {
@@ -568,8 +569,9 @@ py::object rms_norm(torch::Tensor x, torch::Tensor weight, c10::optional<torch::
 // (q, scale), or (q, scale, h) with a residual.
 py::tuple rms_norm_fp8(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual, double eps) {
   check_args(x, weight, residual);
-  LM_CHECK_VALUE(!(at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() ||
-                                                     (residual && residual->requires_grad()))),
+  LM_CHECK_VALUE(!lm::any_tangent(x, weight, residual) &&
+                     !(at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() ||
+                                                      (residual && residual->requires_grad()))),
                     "rms_norm_fp8 has no gradient: call it under torch.no_grad()");
   const Forward f = forward(as_rows(x), residual ? as_rows(*residual) : torch::Tensor(), weight.contiguous(), eps, true,
                             false);

@@ -773,6 +773,7 @@ py::tuple token_log_probs(torch::Tensor logits, torch::Tensor tokens, c10::optio
   // far enough inside fp32's range for 1 / T, and for the difference of any two logits over T to be told from zero
   LM_CHECK_VALUE(temperature >= 1e-30 && temperature <= 1e30, "the temperature must be in 1e-30..1e30, not ", temperature);
   LM_CHECK_VALUE(top >= 0 && top <= kMaxTop, "top must be in 0..", kMaxTop, ", not ", top);
+  LM_CHECK_NO_TANGENT("token_log_probs", logits);
   torch::Tensor m, t = tokens;
   if (mask) {
     LM_CHECK_VALUE(mask->scalar_type() == torch::kBool && mask->device() == logits.device(),

@@ -35,7 +35,7 @@ from torch import Tensor, nn
 from torch.autograd.function import once_differentiable
 
 from .ext import require_extension
-from .rmsnorm import from_rows
+from .rmsnorm import from_rows, wants_derivative
 from .tc_linear import _result_dtype, _Status
 
 GROUP = 128
@@ -164,7 +164,7 @@ def fp8_matmul(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Ten
         raise ValueError("fp8_matmul gives fp32, bf16 or fp16")
     if any(t is not None and t.device != a.device for t in (a_scale, b, b_scale, bias)):
         raise ValueError("fp8_matmul needs all of its tensors on one device")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (a_scale, b_scale, bias)):
+    if wants_derivative(a_scale, b_scale, bias):
         raise ValueError("fp8_matmul has no gradient: use fp8_linear, or call it under torch.no_grad()")
     rows = lead.numel()
     return reference_fp8_matmul(a.reshape(rows, k), a_scale.reshape(rows, _groups(k)), b, b_scale, bias,
@@ -248,7 +248,7 @@ class FrozenFp8Linear(nn.Module):
         return cls(linear.weight, linear.bias)
 
     def forward(self, x: Tensor) -> Tensor:
-        if torch.is_grad_enabled() and x.requires_grad:
+        if wants_derivative(x):
             raise ValueError("FrozenFp8Linear has no gradient: call it under torch.no_grad()")
         xq, xs = quantize_rows(x)
         return fp8_matmul(xq, xs, self.weight_q, self.weight_scale, self.bias, _result_dtype(x))

@@ -17,12 +17,19 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor, nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .ext import require_extension
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_WIDTH = 32768
+
+
+def wants_derivative(*tensors: Tensor | None) -> bool:
+    """Whether a derivative of what is computed from `tensors` would be expected, in reverse or forward mode."""
+    return any(t is not None and (torch.is_grad_enabled() and t.requires_grad or
+                                  forward_ad.unpack_dual(t).tangent is not None) for t in tensors)
 
 
 def _check(x: Tensor, weight: Tensor, residual: Tensor | None) -> None:
@@ -97,7 +104,7 @@ def rms_norm_fp8(x: Tensor, weight: Tensor, residual: Tensor | None = None, eps:
     if x.is_cuda:
         return require_extension().rms_norm_fp8(x, weight, residual, eps)
     _check(x, weight, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    if wants_derivative(x, weight, residual):
         raise ValueError("rms_norm_fp8 has no gradient: call it under torch.no_grad()")
     from .fp8 import reference_quantize_rows
     h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
