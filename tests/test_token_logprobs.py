@@ -352,3 +352,42 @@ def test_changes_in_place_and_second_derivatives_are_refused():
         x += 1.
     with pytest.raises(RuntimeError):
         r.entropy.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [8, 40, 900, 5000])
+@pytest.mark.parametrize("temperature", [1., .25])
+def test_peaked_rows(v, temperature):
+    """One entry holds all but d of the probability, d from 1e-7 to a half, among seven others that are valid: the sum is
+    1 + d', and its logarithm all of the answer. The 1 is rounded by three joins of lanes (seven additions by the one
+    thread that has them all, in long rows), F each as the sum stays below 2; the exponentials are off by 2^-22 + 4 F |x / T| of themselves, with |x / T| up to 20 less than 96 F; the logarithm
+    is off by 6 F of itself, and the entropy's second term by less than 100 F. No log-probability is above 0, and no
+    entropy below."""
+    g = torch.Generator().manual_seed(v)
+    rows = 3000
+    d = 10. ** (-7 + 6.7 * torch.rand(rows, generator=g, dtype=torch.float64))
+    x = torch.full((rows, v), -50.)
+    x[:, 1:8] = (temperature * ((d / 7)[:, None].log() + .3 * torch.randn(rows, 7, generator=g, dtype=torch.float64))).float()
+    x[:, 0] = 0.
+    x, t = x.cuda(), torch.zeros(rows, dtype=torch.long, device="cuda")
+    mask = torch.arange(v, device="cuda") < 8
+    z = x[:, :8].double() / temperature
+    rest = z[:, 1:].exp().sum(1)
+    lp, h = -torch.log1p(rest), torch.log1p(rest) - (z * z.exp()).sum(1) / (1 + rest)
+    r = token_log_probs(x, t, mask, temperature, top=1)
+    tol = F * ((3 if v <= 1024 else 7) + 100 * rest + 8 * lp.abs())
+    assert ((r.log_prob - lp).abs() <= tol).all(), float(((r.log_prob - lp).abs() / tol).max())
+    assert torch.equal(r.top_log_prob[:, 0], r.log_prob) and (r.log_prob <= 0).all()
+    tol = tol + 100 * F * h
+    assert ((r.entropy - h).abs() <= tol).all(), float(((r.entropy - h).abs() / tol).max())
+    assert (r.entropy >= 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [8, 1000, 9000])
+def test_equal_entries(v):
+    """n equal entries: the sum is n exactly, and the entropy its logarithm, which is off by at most six roundings."""
+    x, n = torch.full((v, v), 2.5, device="cuda"), torch.arange(1, v + 1, device="cuda")
+    r = token_log_probs(x, torch.zeros(v, dtype=torch.long, device="cuda"), torch.arange(v, device="cuda") < n[:, None])
+    want = n.double().log()
+    assert ((r.entropy - want).abs() <= 6 * F * want).all() and torch.equal(r.log_prob, -r.entropy)
