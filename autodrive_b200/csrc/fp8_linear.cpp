@@ -52,7 +52,8 @@ struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
                                fp8::kWaitNs);
     torch::Tensor keep;   // what the weight gradient reads: the caller's x where it can be read as it is
     if (need_w) keep = x2.scalar_type() == torch::kBFloat16 && x2.is_alias_of(x) ? x : x2.to(torch::kBFloat16);
-    ctx->save_for_backward({keep, need_x ? wq[2] : torch::Tensor(), need_x ? wq[3] : torch::Tensor(), status});
+    ctx->save_for_backward({keep, need_x ? wq[2] : torch::Tensor(), need_x ? wq[3] : torch::Tensor()});
+    ctx->saved_data["status"] = status;   // every call's, cleared by others: not a variable of this graph
     ctx->saved_data["x_sizes"] = x.sizes().vec();
     ctx->saved_data["n"] = weight.size(0);
     ctx->saved_data["x_type"] = static_cast<int64_t>(x.scalar_type());
@@ -70,7 +71,7 @@ struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
     const int64_t n = ctx->saved_data["n"].toInt(), k = x_sizes.back();
     const c10::DeviceGuard guard(grads[0].device());
     const auto g = fp8::as_matrix(grads[0]);
-    const auto& status = saved[3];
+    const auto status = ctx->saved_data["status"].toTensor();
     variable_list out(6);
     if (ctx->needs_input_grad(0)) {
       const auto gq = fp8::quantize_rows(g);

@@ -1,0 +1,32 @@
+"""The status word that the tensor-core kernels of a device share: who makes it,
+who clears it and who reads it."""
+import pytest
+import torch
+
+from autodrive_b200.ops.fp8 import fp8_linear, fp8_matmul, quantize_blocks, quantize_rows
+from autodrive_b200.ops.tc_linear import TensorCoreTimeout, check_gemm_status
+
+pytestmark = pytest.mark.gpu
+
+
+def _operands():
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(40, 256, device="cuda", generator=g).bfloat16().requires_grad_(True)
+    w = torch.randn(130, 256, device="cuda", generator=g).requires_grad_(True)
+    return x, w
+
+
+def _quantised():
+    x, w = _operands()
+    return (*quantize_rows(x), *quantize_blocks(w))
+
+
+def test_a_cleared_timeout_leaves_pending_backwards_alone():
+    x, w = _operands()
+    y = fp8_linear(x, w)
+    with pytest.raises(TensorCoreTimeout):
+        fp8_matmul(*_quantised(), wait_ns=0)
+        check_gemm_status()
+    y.sum().backward()
+    check_gemm_status()
+    assert x.grad is not None and w.grad is not None
