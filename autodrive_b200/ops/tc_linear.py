@@ -84,8 +84,9 @@ class _Status:
             if torch.cuda.is_current_stream_capturing():
                 # a word made here would live in the graph's memory and be cleared by its replays alone
                 raise RuntimeError("make one tensor-core call on this device before capturing a graph of them")
-            word = torch.zeros(1, dtype=torch.int32, device=device)
-            host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+            with torch.inference_mode(False):   # later calls write to them, whatever mode the first one was in
+                word = torch.zeros(1, dtype=torch.int32, device=device)
+                host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
             e = {"word": word, "host": host, "event": None, "launches": 0}
             cls._state[device] = e
         return e

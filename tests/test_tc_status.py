@@ -3,10 +3,17 @@ who clears it and who reads it."""
 import pytest
 import torch
 
+from autodrive_b200.ops import tc_linear
 from autodrive_b200.ops.fp8 import fp8_linear, fp8_matmul, quantize_blocks, quantize_rows
 from autodrive_b200.ops.tc_linear import TensorCoreTimeout, check_gemm_status
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def fresh(monkeypatch):
+    """As in a process that has made no tensor-core call yet."""
+    monkeypatch.setattr(tc_linear._Status, "_state", {})
 
 
 def _operands():
@@ -19,6 +26,19 @@ def _operands():
 def _quantised():
     x, w = _operands()
     return (*quantize_rows(x), *quantize_blocks(w))
+
+
+def test_first_call_in_inference_mode(fresh):
+    """Training and polling go on as after any other first call."""
+    with torch.inference_mode():
+        fp8_matmul(*_quantised())
+    x, w = _operands()
+    fp8_linear(x, w).sum().backward()
+    assert x.grad is not None and w.grad is not None
+    with pytest.raises(TensorCoreTimeout):
+        fp8_matmul(*_quantised(), wait_ns=0)
+        check_gemm_status()
+    check_gemm_status()
 
 
 def test_a_cleared_timeout_leaves_pending_backwards_alone():
