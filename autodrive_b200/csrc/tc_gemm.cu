@@ -35,6 +35,9 @@
 // commits its issued MMAs to a drain barrier and waits for it (each wait
 // bounded by 200 ms; a drain that gives up sets bit 16 or 32).
 #include <torch/extension.h>
+#include <c10/core/InferenceMode.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -592,9 +595,28 @@ void tc_gemm(torch::Tensor a, bool a_mn, torch::Tensor b, bool b_mn, torch::Tens
   }
 }
 
+// A device's status word, zero, for the rest of the process. Its memory is its
+// own and is cleared on a stream of its own, so that it can be made while a
+// graph is captured: from the caching allocator it would lie in the graph's
+// memory, and be cleared by the graph's replays alone.
+torch::Tensor status_word(int64_t device) {
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+  const c10::InferenceMode normal(false);
+  int* word = nullptr;
+  cudaStream_t st = nullptr;
+  TORCH_CHECK(cudaMalloc(&word, sizeof(int)) == cudaSuccess, "status word: out of memory");
+  TORCH_CHECK(cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess &&
+                  cudaMemsetAsync(word, 0, sizeof(int), st) == cudaSuccess && cudaStreamSynchronize(st) == cudaSuccess &&
+                  cudaStreamDestroy(st) == cudaSuccess,
+              "status word: not cleared");
+  return torch::from_blob(word, {1}, torch::TensorOptions().dtype(torch::kInt32).device(torch::kCUDA, (c10::DeviceIndex)device));
+}
+
 }  // namespace
 
 void register_tc_gemm_ops(py::module& m) {
+  m.def("status_word", &status_word, "a new status word (int32 [1], zero) of the tensor-core kernels", py::arg("device"));
   m.def("tc_gemm", &tc_gemm, "bf16 tcgen05 GEMM C = op(A) op(B)^T (+bias, activation), TMA-fed, fp32 accumulate",
         py::arg("a"), py::arg("a_mn"), py::arg("b"), py::arg("b_mn"), py::arg("c"), py::arg("bias"),
         py::arg("act"), py::arg("accumulate"), py::arg("status"), py::arg("wait_ns") = 2000000000ll,

@@ -81,13 +81,9 @@ class _Status:
     def _entry(cls, device):
         e = cls._state.get(device)
         if e is None:
-            if torch.cuda.is_current_stream_capturing():
-                # a word made here would live in the graph's memory and be cleared by its replays alone
-                raise RuntimeError("make one tensor-core call on this device before capturing a graph of them")
-            with torch.inference_mode(False):   # later calls write to them, whatever mode the first one was in
-                word = torch.zeros(1, dtype=torch.int32, device=device)
-                host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-            e = {"word": word, "host": host, "event": None, "launches": 0}
+            # neither an inference tensor nor in a graph's memory, whatever the first call is part of
+            word = require_extension().status_word(torch.cuda.current_device() if device.index is None else device.index)
+            e = {"word": word, "host": None, "event": None, "launches": 0}
             cls._state[device] = e
         return e
 
@@ -113,6 +109,9 @@ class _Status:
     def _post(cls, e) -> None:
         if torch.cuda.is_current_stream_capturing():
             return
+        if e["host"] is None:   # made here, where nothing is being captured
+            with torch.inference_mode(False):
+                e["host"] = torch.zeros(1, dtype=torch.int32, pin_memory=True)
         e["host"].copy_(e["word"], non_blocking=True)
         ev = torch.cuda.Event()
         ev.record(torch.cuda.current_stream(e["word"].device))   # the copy's stream, whatever the current device

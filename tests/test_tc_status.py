@@ -5,7 +5,7 @@ import torch
 
 from autodrive_b200.ops import tc_linear
 from autodrive_b200.ops.fp8 import fp8_linear, fp8_matmul, quantize_blocks, quantize_rows
-from autodrive_b200.ops.tc_linear import TensorCoreTimeout, check_gemm_status
+from autodrive_b200.ops.tc_linear import TensorCoreTimeout, check_gemm_status, gemm
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,28 @@ def test_a_cleared_timeout_leaves_pending_backwards_alone():
     y.sum().backward()
     check_gemm_status()
     assert x.grad is not None and w.grad is not None
+
+
+def test_first_call_inside_a_capture(fresh):
+    """The word lies outside the graph's memory: replays leave it alone, and a replayed call's failure is reported."""
+    ops = _quantised()
+    x, w = _operands()
+    xb, wb = x.detach(), w.detach().bfloat16()
+    want, want2 = fp8_matmul(*ops), gemm(xb, wb)         # kernels loaded; their word is forgotten below
+    torch.cuda.synchronize()
+    tc_linear._Status._state.clear()
+    graph, bad = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, y2 = fp8_matmul(*ops), gemm(xb, wb)
+    check_gemm_status()                                  # nothing has run yet
+    for _ in range(3):
+        graph.replay()
+        check_gemm_status()
+        assert torch.equal(y, want) and torch.equal(y2, want2)
+    with torch.cuda.graph(bad):
+        fp8_matmul(*ops, wait_ns=0)
+    bad.replay()
+    graph.replay()
+    with pytest.raises(TensorCoreTimeout):
+        check_gemm_status()
+    check_gemm_status()
