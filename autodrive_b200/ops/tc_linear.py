@@ -82,7 +82,7 @@ class _Status:
         e = cls._state.get(device)
         if e is None:
             # neither an inference tensor nor in a graph's memory, whatever the first call is part of
-            word = require_extension().status_word(torch.cuda.current_device() if device.index is None else device.index)
+            word = require_extension().status_word(device.index)
             e = {"word": word, "host": None, "event": None, "launches": 0}
             cls._state[device] = e
         return e
@@ -143,9 +143,10 @@ def check_gemm_status(device=None, block: bool = True) -> None:
     """Raise `TensorCoreTimeout` if a tcgen05 GEMM on `device` (default: the
     current CUDA device) reported a timed-out wait since the last check. With
     block=False only an already finished read-back is examined and a new one
-    is queued."""
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    _Status.check(dev, block)
+    is queued. Launches replayed from a CUDA graph are not counted towards the
+    automatic read-backs: call this after replaying one."""
+    dev = torch.device("cuda" if device is None else device)
+    _Status.check(torch.device("cuda", torch.cuda.current_device()) if dev.index is None else dev, block)
 
 
 def gemm(a: torch.Tensor, b: torch.Tensor, *, a_mn: bool = False, b_mn: bool = False, bias=None, act=None,

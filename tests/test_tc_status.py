@@ -75,3 +75,10 @@ def test_first_call_inside_a_capture(fresh):
     with pytest.raises(TensorCoreTimeout):
         check_gemm_status()
     check_gemm_status()
+
+
+def test_a_device_without_a_number_is_the_current_one():
+    fp8_matmul(*_quantised(), wait_ns=0)
+    with pytest.raises(TensorCoreTimeout):
+        check_gemm_status("cuda")
+    check_gemm_status()
