@@ -34,6 +34,13 @@ torch::Tensor bf16_operand(const torch::Tensor& x) {
   return y;
 }
 
+// Counts a backward's launches towards the read-backs of the status word, and
+// raises what one has found (ops/tc_linear.py), as a forward does.
+void poll_status(const c10::Device& device) {
+  const py::gil_scoped_acquire gil;
+  py::module_::import("autodrive_b200.ops.tc_linear").attr("_Status").attr("after_launch")(py::cast(device));
+}
+
 struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& weight,
                                const c10::optional<torch::Tensor>& bias_, int64_t out_dtype, bool grad,
@@ -86,6 +93,7 @@ struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
     const int64_t b_type = ctx->saved_data["b_type"].toInt();
     if (b_type >= 0 && ctx->needs_input_grad(2))
       out[2] = fp8::column_sums(g, static_cast<torch::ScalarType>(b_type));
+    if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1)) poll_status(g.device());
     return out;
   }
 };

@@ -82,3 +82,20 @@ def test_a_device_without_a_number_is_the_current_one():
     with pytest.raises(TensorCoreTimeout):
         check_gemm_status("cuda")
     check_gemm_status()
+
+
+def test_backwards_are_polled(monkeypatch):
+    """A wait that runs out is reported by the backwards that follow, as by forwards: the first queues the read-back."""
+    monkeypatch.setattr(tc_linear._Status, "poll_every", 1)
+    check_gemm_status()
+    x, w = _operands()
+    first, second = fp8_linear(x, w), fp8_linear(x, w)
+    check_gemm_status()
+    tc_linear._Status.get(x.device).fill_(2)   # as a kernel would
+    first.sum().backward()
+    torch.cuda.synchronize()
+    with pytest.raises(TensorCoreTimeout, match="stage loaded"):
+        second.sum().backward()
+    check_gemm_status()
+    fp8_linear(x, w).sum().backward()          # and the engine goes on
+    check_gemm_status()
