@@ -20,7 +20,7 @@ torch::Tensor column_sums(const torch::Tensor& x, torch::ScalarType out_type);
 torch::Tensor matmul(const torch::Tensor& a, const torch::Tensor& a_scale, const torch::Tensor& b,
                      const torch::Tensor& b_scale, const torch::Tensor& bias, torch::ScalarType out_dtype,
                      const torch::Tensor& status, int64_t wait_ns);
-// a^T b of bf16 matrices [K, M] and [K, N] with 16-byte aligned rows, fp32 sums.
+// a^T b of matrices [K, M] and [K, N], both bf16 or both fp16, with 16-byte aligned rows, fp32 sums.
 torch::Tensor weight_gradient(const torch::Tensor& a, const torch::Tensor& b, torch::ScalarType out_type,
                               const torch::Tensor& status);
 // `t` as a matrix with contiguous columns: a view where its layout allows one.

@@ -54,8 +54,9 @@ struct Args {
   void* c;
   int64_t ldc;
   int out_kind;           // 0 fp32, 1 bf16, 2 fp16
-  int splits;             // CTAs of a cluster that share one tile's groups (1: none do); bf16: parts of the rows
-  int64_t part;           // bf16: elements between the results of two parts
+  int splits;             // CTAs of a cluster that share one tile's groups (1: none do); 16 bits: parts of the rows
+  int64_t part;           // 16 bits: elements between the results of two parts
+  int half;               // 16 bits: fp16 operands, not bf16
   int* status;
   uint64_t wait_ns;
 };
@@ -304,11 +305,11 @@ struct PairLink {
 // armed by both, and the first CTA sees to the landing of all of them (neither
 // ends before the other). Where a wait ran out, one CTA may have armed up to a
 // ring's rounds that the other has not: the first CTA arms those in its place.
-template <int STAGES, bool PAIR = false, bool BF16 = false, typename F>
+template <int STAGES, bool PAIR = false, bool WIDE = false, typename F>
 __device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, const CUtensorMap* tb, uint32_t smem0,
                                         uint32_t stage_bytes, uint32_t a_bytes, uint32_t full0, uint32_t done0,
                                         const PairLink& link, F&& walk) {
-  static_assert(PAIR || !BF16, "bf16 tiles are the pairs' alone");
+  static_assert(PAIR || !WIDE, "16-bit tiles are the pairs' alone");
   const uint32_t armed0 = PAIR ? tc::cluster_map(full0, 0) : full0;
   const auto tile = [](uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     if constexpr (PAIR) tc::tma_load_2d_pair(dst, map, x, y, bar);
@@ -325,7 +326,7 @@ __device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, co
     const uint32_t sa = smem0 + st.slot * stage_bytes, full = armed0 + 8 * st.slot;
     if constexpr (PAIR) tc::mbar_arrive_expect_tx_cluster(full, stage_bytes);
     else tc::mbar_arrive_expect_tx(full, stage_bytes);
-    if constexpr (BF16) {   // 64 rows by 128 columns, as two boxes of 64 columns
+    if constexpr (WIDE) {   // 64 rows by 128 columns, as two boxes of 64 columns
       tile(sa, ta, row_a, k, full);
       tile(sa + 8192, ta, row_a + 64, k, full);
       tile(sa + a_bytes, tb, row_b, k, full);
@@ -365,13 +366,14 @@ __device__ __forceinline__ void produce(const Args& g, const CUtensorMap* ta, co
 // cycles to issue, commits 59 and successful waits 40, one after the other, so
 // the next group's barriers are looked at between the products. Before it
 // returns, its last products are complete.
-template <int STAGES, int BUFFERS, int COLS, bool PAIR, bool BF16 = false>
+template <int STAGES, int BUFFERS, int COLS, bool PAIR, bool WIDE = false>
 __device__ __forceinline__ void multiply(const Args& g, uint32_t count, uint32_t smem0, uint32_t stage_bytes,
                                          uint32_t a_bytes, uint32_t tmem, uint32_t full0,
                                          uint32_t done0, uint32_t tempty0) {
-  static_assert(!BF16 || PAIR, "bf16 tiles are the pairs' alone");
-  const uint32_t id = BF16 ? tc::idesc_bf16(256, COLS, true, true) : tc::idesc_e4m3(PAIR ? 256 : 128, COLS);
-  const uint32_t lo = BF16 ? tc::mnmajor64_desc_lo(smem0) : tc::kmajor_desc_lo(smem0);
+  static_assert(!WIDE || PAIR, "16-bit tiles are the pairs' alone");
+  uint32_t id = tc::idesc_e4m3(PAIR ? 256 : 128, COLS);
+  if (WIDE) id = g.half ? tc::idesc_f16(256, COLS, true, true) : tc::idesc_bf16(256, COLS, true, true);
+  const uint32_t lo = WIDE ? tc::mnmajor64_desc_lo(smem0) : tc::kmajor_desc_lo(smem0);
   Ring<STAGES> st, last;
   Ring<BUFFERS> buf;
   uint32_t issued = 0;
@@ -394,8 +396,8 @@ __device__ __forceinline__ void multiply(const Args& g, uint32_t count, uint32_t
     buf.next();
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      if constexpr (BF16)
-        tc::mma_bf16_pair(d, tc::kmajor_desc(la + 128 * ks), tc::kmajor_desc(lb + 128 * ks), id, ks > 0);
+      if constexpr (WIDE)
+        tc::mma_16bit_pair(d, tc::kmajor_desc(la + 128 * ks), tc::kmajor_desc(lb + 128 * ks), id, ks > 0);
       else if constexpr (PAIR) tc::mma_e4m3_pair(d, tc::kmajor_desc(la + 2 * ks), tc::kmajor_desc(lb + 2 * ks), id, ks > 0);
       else tc::mma_e4m3(d, tc::kmajor_desc(la + 2 * ks), tc::kmajor_desc(lb + 2 * ks), id, ks > 0);
       if (ks == 1) {
@@ -653,13 +655,13 @@ constexpr int kPairThreads = 384, kPairStages = 6, kPairBuffers = 2;
 constexpr uint32_t kPairTile = 128 * kGroup, kPairStage = 2 * kPairTile;
 constexpr uint32_t kPairSmem = kPairStages * kPairStage + kEpiWarps * kStoreStage + 1024 + 256;
 
-// BF16: the weight gradient's product instead, C = A^T B in fp32 of bf16 A
-// [K,M] and B [K,N]. A stage holds 64 rows of both (as many bytes), read down
+// WIDE: the weight gradient's product instead, C = A^T B in fp32 of A [K,M]
+// and B [K,N] in bf16 or fp16. A stage holds 64 rows of both (as many bytes), read down
 // their columns by the tensor cores, and without scales the epilogue adds up
 // every 64 rows in fp32 with round-to-nearest, which the tensor cores' own long
 // sums do not; g.splits parts of the rows give as many partial results, `part`
 // elements apart.
-template <bool BF16>
+template <bool WIDE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const Args g) {
   extern __shared__ uint8_t smem_raw[];
@@ -677,10 +679,10 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
   const uint32_t rank = tc::cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int tiles_n = (g.N + 255) / 256, tiles_m = (g.M + 255) / 256;
-  const int tiles = tiles_n * tiles_m, splits = BF16 ? g.splits : 1, total = tiles * splits, G = g.groups;
+  const int tiles = tiles_n * tiles_m, splits = WIDE ? g.splits : 1, total = tiles * splits, G = g.groups;
   const int share = (G + splits - 1) / splits;                // groups of a part of the rows
   const auto range = [&](int w) {
-    const int kb0 = BF16 ? w / tiles * share : 0;
+    const int kb0 = WIDE ? w / tiles * share : 0;
     return make_int2(min(G, kb0), min(G, kb0 + share));
   };
   uint32_t count = 0;                                         // of this pair's groups
@@ -713,28 +715,28 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__
     tc::regs_dec<40>();
     if (warp == 0 && lane == 0) {
       const PairLink link{rank, s_issued, through};
-      produce<kPairStages, true, BF16>(g, &ta, &tb, smem0, kPairStage, kPairTile, full0, done0, link, [&](auto&& load) {
+      produce<kPairStages, true, WIDE>(g, &ta, &tb, smem0, kPairStage, kPairTile, full0, done0, link, [&](auto&& load) {
         for (int w = pair; w < total; w += pairs) {
           const int2 kb = range(w);
           const int m0 = (w % tiles / tiles_n) * 256 + (int)rank * 128, n0 = (w % tiles_n) * 256 + (int)rank * 128;
           for (int k = kb.x; k < kb.y; ++k)
-            if (!load(k * (BF16 ? 64 : kGroup), m0, n0)) return;
+            if (!load(k * (WIDE ? 64 : kGroup), m0, n0)) return;
         }
       });
     } else if (warp == 1 && lane == 0 && rank == 0) {
-      multiply<kPairStages, kPairBuffers, 256, true, BF16>(g, count, smem0, kPairStage, kPairTile, tmem, full0, done0,
+      multiply<kPairStages, kPairBuffers, 256, true, WIDE>(g, count, smem0, kPairStage, kPairTile, tmem, full0, done0,
                                                            tempty0);
     }
     __syncwarp();
   } else {
     tc::regs_inc<216>();
     Args out = g;
-    epilogue<kPairStages, kPairBuffers, 256, !BF16>(
+    epilogue<kPairStages, kPairBuffers, 256, !WIDE>(
         g, tmem, done0, tc::cluster_map(tempty0, 0), warp & 3, (warp - 4) >> 2,
         [&](auto&& tile) {
           for (int w = pair; w < total; w += pairs) {
             const int2 kb = range(w);
-            if (BF16) out.c = reinterpret_cast<float*>(g.c) + (int64_t)(w / tiles) * g.part;
+            if (WIDE) out.c = reinterpret_cast<float*>(g.c) + (int64_t)(w / tiles) * g.part;
             if (!tile((w % tiles / tiles_n) * 256 + (int)rank * 128, (w % tiles_n) * 256, kb.x, kb.y)) return;
           }
         },
@@ -822,13 +824,13 @@ void launch_rows(const CUtensorMap& tb, const torch::Tensor& a, int64_t lda, Arg
                  st, tb, ta, g);
 }
 
-template <bool BF16>
+template <bool WIDE>
 void launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const Args& g, int64_t tiles, cudaStream_t st) {
   static size_t configured[dynsmem::kMaxDevices] = {};
-  TORCH_CHECK(dynsmem::opt_in(gemm_pair_kernel<BF16>, kPairSmem, configured) == cudaSuccess,
+  TORCH_CHECK(dynsmem::opt_in(gemm_pair_kernel<WIDE>, kPairSmem, configured) == cudaSuccess,
               "fp8_matmul shared-memory attribute");
   TORCH_CHECK(tiles < (1ll << 31), "fp8_matmul: too many output tiles");
-  gemm_pair_kernel<BF16><<<2 * (int)std::min<int64_t>(tiles, lm::sm_count() / 2), kPairThreads, kPairSmem, st>>>(ta, tb, g);
+  gemm_pair_kernel<WIDE><<<2 * (int)std::min<int64_t>(tiles, lm::sm_count() / 2), kPairThreads, kPairSmem, st>>>(ta, tb, g);
   TORCH_CHECK(cudaGetLastError() == cudaSuccess, "fp8_matmul launch failed");
 }
 
@@ -919,8 +921,11 @@ torch::Tensor weight_gradient(const torch::Tensor& a, const torch::Tensor& b, to
   const bool direct = g.splits == 1 && out_type == torch::kFloat32;
   torch::Tensor parts = direct ? out : torch::empty({g.splits, M, N}, a.options().dtype(torch::kFloat32));
   g.c = parts.data_ptr();
-  const CUtensorMap ta = tma::bf16_sw128(a.data_ptr(), K, M, a.stride(0), 64);
-  const CUtensorMap tb = tma::bf16_sw128(b.data_ptr(), K, N, b.stride(0), 64);
+  TORCH_CHECK(a.scalar_type() == b.scalar_type(), "weight gradient: operands of one type");
+  g.half = a.scalar_type() == torch::kHalf;
+  const auto type = g.half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMap ta = tma::bf16_sw128(a.data_ptr(), K, M, a.stride(0), 64, type);
+  const CUtensorMap tb = tma::bf16_sw128(b.data_ptr(), K, N, b.stride(0), 64, type);
   auto st = c10::cuda::getCurrentCUDAStream().stream();
   launch_pair<true>(ta, tb, g, tiles * g.splits, st);
   lm::count_launches(1);

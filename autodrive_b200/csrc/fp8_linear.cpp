@@ -2,8 +2,13 @@
 //
 //   y  = Q(x) Q(w)^T + b      Q: e4m3 with scales for blocks of 128
 //   dx = Q(dy) Q(w)           rounding counts as the identity
-//   dw = dy^T x               bf16 operands, fp32 sums
+//   dw = dy^T x               16-bit operands, fp32 sums
 //   db = sum of dy's rows     in fp32
+//
+// The weight gradient's operands are x and dy as they are where both are bf16
+// or both fp16. Otherwise they are rounded to bf16: the tensor cores take 16
+// bits at full rate, and what the rounding adds, 2^-8 of each term at most, is
+// a sixteenth of what the layer's own e4m3 rounding of x and dy does to y and dx.
 //
 // One call runs the quantisers and the product, and one backward its
 // kernels, so that no Python runs between the launches.
@@ -22,14 +27,14 @@ namespace {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// `x` as a bf16 operand of the weight gradient: rows that start 16 bytes apart
-// on an aligned base (a copy only where they do not).
-torch::Tensor bf16_operand(const torch::Tensor& x) {
+// `x` as an operand of the weight gradient, bf16 or fp16: rows that start 16
+// bytes apart on an aligned base (a copy only where they do not).
+torch::Tensor operand(const torch::Tensor& x, torch::ScalarType type) {
   const int64_t rows = x.size(0), k = x.size(1);
-  if (x.scalar_type() == torch::kBFloat16 && (rows <= 1 || x.stride(0) % 8 == 0) && (k <= 1 || x.stride(1) == 1) &&
+  if (x.scalar_type() == type && (rows <= 1 || x.stride(0) % 8 == 0) && (k <= 1 || x.stride(1) == 1) &&
       reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && rows != 1)
     return x;
-  auto y = torch::empty({rows, (k + 7) / 8 * 8}, x.options().dtype(torch::kBFloat16)).narrow(1, 0, k);
+  auto y = torch::empty({rows, (k + 7) / 8 * 8}, x.options().dtype(type)).narrow(1, 0, k);
   y.copy_(x);
   return y;
 }
@@ -58,7 +63,8 @@ struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
     const auto y = fp8::matmul(xq.first, xq.second, wq[0], wq[1], b, static_cast<torch::ScalarType>(out_dtype), status,
                                fp8::kWaitNs);
     torch::Tensor keep;   // what the weight gradient reads: the caller's x where it can be read as it is
-    if (need_w) keep = x2.scalar_type() == torch::kBFloat16 && x2.is_alias_of(x) ? x : x2.to(torch::kBFloat16);
+    if (need_w && x2.scalar_type() == torch::kFloat32) keep = x2.to(torch::kBFloat16);
+    else if (need_w) keep = x2.is_alias_of(x) ? x : x2;
     ctx->save_for_backward({keep, need_x ? wq[2] : torch::Tensor(), need_x ? wq[3] : torch::Tensor()});
     ctx->saved_data["status"] = status;   // every call's, cleared by others: not a variable of this graph
     ctx->saved_data["x_sizes"] = x.sizes().vec();
@@ -87,7 +93,9 @@ struct Fp8LinearFn : torch::autograd::Function<Fp8LinearFn> {
                    .view(x_sizes);
     }
     if (ctx->needs_input_grad(1)) {
-      out[1] = fp8::weight_gradient(bf16_operand(g), bf16_operand(fp8::as_matrix(saved[0])),
+      const auto rows = fp8::as_matrix(saved[0]);
+      const auto type = g.scalar_type() == torch::kHalf && rows.scalar_type() == torch::kHalf ? torch::kHalf : torch::kBFloat16;
+      out[1] = fp8::weight_gradient(operand(g, type), operand(rows, type),
                                     static_cast<torch::ScalarType>(ctx->saved_data["w_type"].toInt()), status);
     }
     const int64_t b_type = ctx->saved_data["b_type"].toInt();

@@ -31,7 +31,8 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encoder() {
 // `ld` elements; box = 64 columns x box_rows rows with 128-byte swizzle, so
 // one box lands as one 64-column block of a shared-memory SW128 image.
 // Rows past the end read as zero.
-inline CUtensorMap bf16_sw128(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+inline CUtensorMap bf16_sw128(const void* ptr, int64_t rows, int64_t cols, int64_t ld, int box_rows,
+                              CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16) {
   TORCH_CHECK(reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && (ld * 2) % 16 == 0,
               "TMA operands need 16-byte aligned bases and row strides");
   CUtensorMap m;
@@ -39,7 +40,7 @@ inline CUtensorMap bf16_sw128(const void* ptr, int64_t rows, int64_t cols, int64
   cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
   cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1u, 1u};
-  CUresult r = encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+  CUresult r = encoder()(&m, type, 2, const_cast<void*>(ptr), dims, strides, box, estr,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");

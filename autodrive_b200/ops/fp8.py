@@ -19,13 +19,16 @@ with a weight matrix, a b^T, with fp32 sums. It has no gradient.
 ``fp8_linear(x, weight, bias)`` is a linear layer for training: both operands
 are quantised on the way in; the backward takes the quantised gradient through
 the same quantised weight (rounding counts as the identity), and the weight's
-gradient as a bf16 product of the unquantised gradient and input.
+gradient as a product of the unquantised gradient and input with fp32 sums: as
+they are where both are bf16 or both fp16, otherwise rounded to bf16 (2^-8 of
+each term at most for each of the two).
 ``Fp8Linear`` is the module (a drop-in ``nn.Linear``, beside ``TcLinear``), and
 ``FrozenFp8Linear`` the one for acting and serving, which holds 8-bit weights
 only. ``freeze_fp8(module)`` swaps a module's linear layers for frozen ones.
 
-On CPU all of them compute the same values in plain PyTorch. The product's
-kernel reports timed-out waits through the status word of the bf16 GEMM
+On CPU all of them compute the same in plain PyTorch, with fp32 sums in another
+order and the weight's gradient from operands of any type as they are. The
+product's kernel reports timed-out waits through the status word of the bf16 GEMM
 (``ops.tc_linear.check_gemm_status``).
 """
 from __future__ import annotations

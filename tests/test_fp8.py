@@ -474,3 +474,35 @@ def test_waits_of_any_length_leave_nothing_in_flight(m, n, k):
             y = want
         assert torch.equal(y, want) and torch.equal(z, want)
     check_gemm_status(dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 64, 64), (257, 130, 200), (3000, 256, 521)])
+def test_operands_of_the_weight_gradient(dtype, m, n, k):
+    """Values that use all bits of their type: fp16 and bf16 operands enter the product as they are, fp32 ones rounded to
+    bf16, and the sums are fp32."""
+    x = _values(m, k, 1, dtype, "cuda")
+    w = (_values(n, k, 2, device="cuda") * k ** -.5).requires_grad_(True)
+    dy = _values(m, n, 3, dtype, "cuda")
+    dw, = torch.autograd.grad(fp8_linear(x, w), w, dy)
+    a, b = (t.bfloat16().double() if dtype == torch.float32 else t.double() for t in (dy, x))
+    assert ((dw.double() - a.t() @ b).abs() <= (m + 8) * E * (a.abs().t() @ b.abs())).all()
+    # against the unrounded gradient: 2^-8 of the terms for each bf16 operand, to first order
+    a, b = dy.double(), x.double()
+    op = 2. ** -8 if dtype == torch.float32 else 0.
+    assert ((dw.double() - a.t() @ b).abs() <= ((m + 8) * E + 2.1 * op) * (a.abs().t() @ b.abs())).all()
+
+
+@pytest.mark.gpu
+def test_weight_gradient_of_mixed_types():
+    """An fp16 input whose gradient comes in bf16 (autocast), or the reverse: both operands in bf16."""
+    for xt, out in ((torch.float16, torch.bfloat16), (torch.float32, torch.float16), (torch.bfloat16, torch.float16)):
+        x, w = _values(300, 200, 1, xt, "cuda"), _values(130, 200, 2, device="cuda").requires_grad_(True)
+        with torch.autocast("cuda", dtype=out):
+            y = fp8_linear(x, w)
+        assert y.dtype == out
+        dy = _values(300, 130, 3, out, "cuda")
+        dw, = torch.autograd.grad(y, w, dy)
+        a, b = dy.bfloat16().double(), x.bfloat16().double()
+        assert ((dw.double() - a.t() @ b).abs() <= 308 * E * (a.abs().t() @ b.abs())).all()
