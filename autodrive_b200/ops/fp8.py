@@ -60,6 +60,16 @@ def _padded_q(values: Tensor) -> Tensor:
     return buf.view(E4M3)[:, :k]
 
 
+def _rows_with_padding(q: Tensor) -> Tensor:
+    """The bytes of `q` [M, K] with its rows' padding, as ``_padded_q`` lays them out: a view, or a copy where `q` lies
+    otherwise."""
+    m, k = q.shape
+    ld = (k + 15) // 16 * 16
+    if q.stride() != (ld, 1) or q.untyped_storage().nbytes() < q.storage_offset() + m * ld:
+        q = _padded_q(q)
+    return q.view(torch.uint8).as_strided((m, ld), (ld, 1))
+
+
 def _round_e4m3(t: Tensor) -> Tensor:
     """The nearest e4m3 number of each fp64 value (ties to even), in fp64."""
     _, exponent = torch.frexp(t)
@@ -238,12 +248,18 @@ class FrozenFp8Linear(nn.Module):
         self.register_buffer("bias", None if bias is None else bias.detach().float().clone())
 
     def _apply(self, fn, recurse=True):
-        """Moves the buffers with the module and keeps their types and layout: ``half()`` or ``to(dtype)`` of a
-        network change its other layers, not the 8-bit numbers and their scales."""
+        """What is done to the tensors of a module (moved, shared, emptied, converted) is done to the buffers' bits, so
+        that they keep their types and layout: ``half()`` or ``to(dtype)`` of a network change its other layers, not the
+        8-bit numbers and their scales."""
         for name, t in self._buffers.items():
-            if t is not None:
-                moved = t.to(fn(t.new_empty(0, dtype=torch.float32)).device)
-                self._buffers[name] = _padded_q(moved) if name == "weight_q" and moved is not t else moved
+            if t is None:
+                continue
+            bits = _rows_with_padding(t) if name == "weight_q" else t.view(torch.int32)
+            moved = fn(bits)
+            if moved.dtype != bits.dtype:   # type(dst) converts whole numbers, too
+                moved = bits.to(moved.device)
+            if moved is not bits:
+                self._buffers[name] = moved.view(E4M3)[:, :t.shape[1]] if name == "weight_q" else moved.view(t.dtype)
         return self
 
     @classmethod

@@ -506,3 +506,24 @@ def test_weight_gradient_of_mixed_types():
         dw, = torch.autograd.grad(y, w, dy)
         a, b = dy.bfloat16().double(), x.bfloat16().double()
         assert ((dw.double() - a.t() @ b).abs() <= 308 * E * (a.abs().t() @ b.abs())).all()
+
+
+def test_frozen_layers_of_a_skeleton_and_in_shared_memory():
+    x = torch.randn(3, 300)
+    net = nn.Sequential(freeze_fp8(nn.Sequential(nn.Linear(300, 200))), nn.Linear(200, 5))
+    state = net.state_dict()
+    with torch.device("meta"):
+        skeleton = nn.Sequential(nn.Sequential(FrozenFp8Linear(torch.empty(200, 300), torch.empty(200))), nn.Linear(200, 5))
+    skeleton.to_empty(device="cpu").load_state_dict(state)
+    layer = skeleton[0][0]
+    assert layer.weight_q.dtype == fp8.E4M3 and layer.weight_q.stride() == (304, 1)
+    with torch.no_grad():
+        assert torch.equal(skeleton(x), net(x))
+    net.share_memory()
+    assert all(t.is_shared() for t in net.state_dict().values())
+    with torch.no_grad():
+        assert torch.equal(skeleton(x), net(x))
+    for change in (lambda n: n.half().float(), lambda n: n.type(torch.float64).float(), lambda n: n.to(torch.bfloat16).float()):
+        assert change(net)[0][0].weight_q.dtype == fp8.E4M3 and net[0][0].weight_scale.dtype == torch.float32
+        assert torch.equal(net[0][0].weight_scale, layer.weight_scale)
+        assert torch.equal(net[0][0].weight_q.float(), layer.weight_q.float())
