@@ -279,11 +279,13 @@ def freeze_fp8(module: nn.Module, min_features: int = GROUP) -> nn.Module:
     current weight: narrower layers, such as the policy heads, are not bound
     by their weights and keep their precision. Layers that ``tensorize`` has
     put on the bf16 GEMM stay as they are (a policy to be frozen is built with
-    ``tensor_cores=False``). Returns the module."""
+    ``tensor_cores=False``). Returns the module, or the frozen layer where the
+    module itself is such a layer."""
+    if type(module) in (nn.Linear, Fp8Linear):
+        wide = min(module.in_features, module.out_features) >= min_features
+        return FrozenFp8Linear.from_linear(module) if wide else module
     for name, child in list(module.named_children()):
-        if type(child) in (nn.Linear, Fp8Linear):
-            if min(child.in_features, child.out_features) >= min_features:
-                setattr(module, name, FrozenFp8Linear.from_linear(child))
-        else:
-            freeze_fp8(child, min_features)
+        frozen = freeze_fp8(child, min_features)
+        if frozen is not child:
+            setattr(module, name, frozen)
     return module

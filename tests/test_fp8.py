@@ -527,3 +527,12 @@ def test_frozen_layers_of_a_skeleton_and_in_shared_memory():
         assert change(net)[0][0].weight_q.dtype == fp8.E4M3 and net[0][0].weight_scale.dtype == torch.float32
         assert torch.equal(net[0][0].weight_scale, layer.weight_scale)
         assert torch.equal(net[0][0].weight_q.float(), layer.weight_q.float())
+
+
+def test_freeze_of_a_layer_itself():
+    lin, narrow = nn.Linear(300, 200), nn.Linear(300, 5)
+    frozen = freeze_fp8(lin)
+    x = torch.randn(3, 300)
+    with torch.no_grad():
+        assert isinstance(frozen, FrozenFp8Linear) and torch.equal(frozen(x), FrozenFp8Linear.from_linear(lin)(x))
+    assert freeze_fp8(narrow) is narrow
