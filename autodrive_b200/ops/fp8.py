@@ -281,11 +281,18 @@ def freeze_fp8(module: nn.Module, min_features: int = GROUP) -> nn.Module:
     put on the bf16 GEMM stay as they are (a policy to be frozen is built with
     ``tensor_cores=False``). Returns the module, or the frozen layer where the
     module itself is such a layer."""
-    if type(module) in (nn.Linear, Fp8Linear):
-        wide = min(module.in_features, module.out_features) >= min_features
-        return FrozenFp8Linear.from_linear(module) if wide else module
-    for name, child in list(module.named_children()):
-        frozen = freeze_fp8(child, min_features)
-        if frozen is not child:
-            setattr(module, name, frozen)
-    return module
+    return _freeze(module, min_features, {})
+
+
+def _freeze(module: nn.Module, min_features: int, done: dict) -> nn.Module:
+    """`done`: what has become of each module so far (one may stand in several places)."""
+    if module not in done:
+        done[module] = module
+        if type(module) in (nn.Linear, Fp8Linear):
+            if min(module.in_features, module.out_features) >= min_features:
+                done[module] = FrozenFp8Linear.from_linear(module)
+        else:
+            for name, child in list(module._modules.items()):
+                if child is not None and _freeze(child, min_features, done) is not child:
+                    setattr(module, name, done[child])
+    return done[module]

@@ -536,3 +536,14 @@ def test_freeze_of_a_layer_itself():
     with torch.no_grad():
         assert isinstance(frozen, FrozenFp8Linear) and torch.equal(frozen(x), FrozenFp8Linear.from_linear(lin)(x))
     assert freeze_fp8(narrow) is narrow
+
+
+def test_freeze_of_a_layer_that_stands_in_several_places():
+    class Net(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.a = nn.Linear(256, 256)
+            self.b, self.inner = self.a, nn.Sequential(self.a, nn.Linear(256, 4))
+
+    net = freeze_fp8(Net())
+    assert isinstance(net.a, FrozenFp8Linear) and net.b is net.a and net.inner[0] is net.a and type(net.inner[1]) is nn.Linear
