@@ -273,14 +273,18 @@ class FrozenFp8Linear(nn.Module):
         return fp8_matmul(xq, xs, self.weight_q, self.weight_scale, self.bias, _result_dtype(x))
 
 
+_FORWARD_HOOKS = ("_forward_hooks", "_forward_hooks_with_kwargs", "_forward_hooks_always_called", "_forward_pre_hooks",
+                  "_forward_pre_hooks_with_kwargs")
+
+
 def freeze_fp8(module: nn.Module, min_features: int = GROUP) -> nn.Module:
     """Replace, in place, every plain nn.Linear of `module` (recursively) whose
     two widths are at least `min_features` with a FrozenFp8Linear of its
     current weight: narrower layers, such as the policy heads, are not bound
     by their weights and keep their precision. Layers that ``tensorize`` has
     put on the bf16 GEMM stay as they are (a policy to be frozen is built with
-    ``tensor_cores=False``). Returns the module, or the frozen layer where the
-    module itself is such a layer."""
+    ``tensor_cores=False``). Forward hooks go with their layers. Returns the
+    module, or the frozen layer where the module itself is such a layer."""
     return _freeze(module, min_features, {})
 
 
@@ -290,7 +294,10 @@ def _freeze(module: nn.Module, min_features: int, done: dict) -> nn.Module:
         done[module] = module
         if type(module) in (nn.Linear, Fp8Linear):
             if min(module.in_features, module.out_features) >= min_features:
-                done[module] = FrozenFp8Linear.from_linear(module)
+                frozen = done[module] = FrozenFp8Linear.from_linear(module)
+                frozen.training = module.training
+                for hooks in _FORWARD_HOOKS:   # the same dictionaries, so that their handles still remove them
+                    setattr(frozen, hooks, getattr(module, hooks))
         else:
             for name, child in list(module._modules.items()):
                 if child is not None and _freeze(child, min_features, done) is not child:

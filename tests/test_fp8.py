@@ -547,3 +547,22 @@ def test_freeze_of_a_layer_that_stands_in_several_places():
 
     net = freeze_fp8(Net())
     assert isinstance(net.a, FrozenFp8Linear) and net.b is net.a and net.inner[0] is net.a and type(net.inner[1]) is nn.Linear
+
+
+def test_freeze_keeps_hooks_and_mode():
+    net = nn.Sequential(nn.Linear(256, 256), nn.Linear(256, 256)).eval()
+    seen = []
+    handle = net[0].register_forward_hook(lambda m, a, y: seen.append(("after", type(m), y.shape)))
+    net[1].register_forward_pre_hook(lambda m, a: seen.append(("before", type(m), a[0].shape)))
+    net[1].register_forward_hook(lambda m, a, k, y: y + 1., with_kwargs=True)
+    freeze_fp8(net)
+    x = torch.randn(2, 256)
+    with torch.no_grad():
+        y = net(x)
+        want = net[1].forward(net[0].forward(x)) + 1.
+    assert seen == [("after", FrozenFp8Linear, (2, 256)), ("before", FrozenFp8Linear, (2, 256))]
+    assert torch.equal(y, want) and not net[0].training
+    handle.remove()
+    with torch.no_grad():
+        net(x)
+    assert len(seen) == 3
