@@ -283,8 +283,9 @@ def freeze_fp8(module: nn.Module, min_features: int = GROUP) -> nn.Module:
     current weight: narrower layers, such as the policy heads, are not bound
     by their weights and keep their precision. Layers that ``tensorize`` has
     put on the bf16 GEMM stay as they are (a policy to be frozen is built with
-    ``tensor_cores=False``). Forward hooks go with their layers. Returns the
-    module, or the frozen layer where the module itself is such a layer."""
+    ``tensor_cores=False``), and so do those of an nn.TransformerEncoderLayer,
+    which reads their weights itself. Forward hooks go with their layers.
+    Returns the module, or the frozen layer where the module itself is such a layer."""
     return _freeze(module, min_features, {})
 
 
@@ -298,7 +299,7 @@ def _freeze(module: nn.Module, min_features: int, done: dict) -> nn.Module:
                 frozen.training = module.training
                 for hooks in _FORWARD_HOOKS:   # the same dictionaries, so that their handles still remove them
                     setattr(frozen, hooks, getattr(module, hooks))
-        else:
+        elif not isinstance(module, nn.TransformerEncoderLayer):
             for name, child in list(module._modules.items()):
                 if child is not None and _freeze(child, min_features, done) is not child:
                     setattr(module, name, done[child])

@@ -566,3 +566,12 @@ def test_freeze_keeps_hooks_and_mode():
     with torch.no_grad():
         net(x)
     assert len(seen) == 3
+
+
+def test_freeze_leaves_layers_whose_weights_others_read():
+    net = nn.Sequential(nn.TransformerEncoderLayer(256, 4, 512, batch_first=True), nn.Linear(256, 256)).eval()
+    x = torch.randn(2, 3, 256)
+    with torch.no_grad():
+        want = net[0](x)
+        freeze_fp8(net)
+        assert torch.equal(net[0](x), want) and isinstance(net[1], FrozenFp8Linear)
