@@ -8,9 +8,12 @@
 // each group's tile is read back and added, scaled, to fp32 sums in registers
 // while the next group's products run into another TMEM buffer.
 //
-// Persistent kernel, one CTA per SM, 320 threads:
+// Three kernels, chosen by the sizes (matmul() below): this one for as many 128
+// x 128 tiles as the SMs hold at once, one for few rows and one by pairs of
+// CTAs for more. A CTA has one tile, or, in a cluster, a part of one tile's
+// groups; 320 threads:
 //   warp 0     TMA producer: the 128-byte wide A and B tiles of each group into
-//              a shared-memory ring that runs on across output tiles;
+//              a shared-memory ring;
 //   warp 1     allocates TMEM; one lane issues the four K = 32 products of a
 //              group into the next buffer and commits them to one barrier, on
 //              which the producer waits for the stage and the epilogue for the
@@ -69,12 +72,10 @@ template <int N> struct Ring {
   }
 };
 
-template <int BN> struct Config {
-  static constexpr int stages = BN == 128 ? 6 : 4;
-  static constexpr uint32_t a_bytes = kBM * kGroup, stage_bytes = a_bytes + BN * kGroup;
-  static constexpr uint32_t smem_bytes = stages * stage_bytes + kEpiWarps * 4096 + 1024 + 256;   // ring, stores, barriers
-  static constexpr int buffers = 512 / BN;   // TMEM has 512 columns
-};
+// 128 x 128 tiles: the ring, the epilogue's stores and the barriers; TMEM has 512 columns.
+constexpr int kBN = 128, kStages = 6, kBuffers = 512 / kBN;
+constexpr uint32_t kTileA = kBM * kGroup, kTileStage = kTileA + kBN * kGroup;
+constexpr uint32_t kSmem = kStages * kTileStage + kEpiWarps * 4096 + 1024 + 256;
 
 // The sums of a CTA's rows over one group: acc += sc * TMEM, `CHUNKS` times 32
 // columns from `base`. Two chunks are loaded at a time, and the next ones into
@@ -413,31 +414,27 @@ __device__ __forceinline__ void multiply(const Args& g, uint32_t count, uint32_t
   if (issued && !tc::mbar_wait(done0 + 8 * last.slot, last.round, kDrainNs)) atomicOr(g.status, 32);
 }
 
-template <int BN>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const Args g) {
-  using C = Config<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* stage0 = smem + C::stages * C::stage_bytes;
+  uint8_t* stage0 = smem + kStages * kTileStage;
   uint8_t* misc = stage0 + kEpiWarps * kStoreStage;
-  const uint32_t full0 = tc::smem_u32(misc);                    // stage loaded
-  const uint32_t done0 = full0 + 8 * C::stages;                 // stage's products complete
-  const uint32_t tempty0 = done0 + 8 * C::stages;               // TMEM buffer read out
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (2 * C::stages + C::buffers));
+  const uint32_t full0 = tc::smem_u32(misc);             // stage loaded
+  const uint32_t done0 = full0 + 8 * kStages;            // stage's products complete
+  const uint32_t tempty0 = done0 + 8 * kStages;          // TMEM buffer read out
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc + 8 * (2 * kStages + kBuffers));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles_n = (g.N + BN - 1) / BN, tiles_m = (g.M + kBM - 1) / kBM;
-  const int total = tiles_n * tiles_m, G = g.groups;
 
   if (threadIdx.x == 0) {
     tc::tma_prefetch_map(&ta);
     tc::tma_prefetch_map(&tb);
-    for (int s = 0; s < C::stages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       tc::mbar_init(full0 + 8 * s, 1);
       tc::mbar_init(done0 + 8 * s, 1);
     }
-    for (int b = 0; b < C::buffers; ++b) tc::mbar_init(tempty0 + 8 * b, kEpiWarps);   // one lane of every epilogue warp
+    for (int b = 0; b < kBuffers; ++b) tc::mbar_init(tempty0 + 8 * b, kEpiWarps);   // one lane of every epilogue warp
     tc::mbar_init_fence();
   }
   if (warp == 1) {
@@ -449,43 +446,37 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ 
   tc::tc_fence_after();
   const uint32_t tmem = *s_tmem, smem0 = tc::smem_u32(smem);
 
-  // this CTA's tiles, and its part of their groups
-  const int splits = g.splits, rank = splits > 1 ? (int)tc::cluster_rank() : 0;
-  const int first = blockIdx.x / splits, step = gridDim.x / splits;
+  // this CTA's tile, and its part of the tile's groups
+  const int tiles_n = (g.N + kBN - 1) / kBN, G = g.groups;
+  const int splits = g.splits, rank = splits > 1 ? (int)tc::cluster_rank() : 0, tile = blockIdx.x / splits;
+  const int m0 = (tile / tiles_n) * kBM, n0 = (tile % tiles_n) * kBN;
   const int part = (G + splits - 1) / splits, kb0 = min(G, rank * part), kb1 = min(G, kb0 + part);
-  float* sums = reinterpret_cast<float*>(smem);   // the stages, once the one tile of a shared CTA is done
-  constexpr int kStride = sum_stride(BN);
-  static_assert(kBM * kStride * 4 <= C::stages * C::stage_bytes, "the sums take the stages' place");
+  float* sums = reinterpret_cast<float*>(smem);   // the stages, once the part of a shared tile is done
+  constexpr int kStride = sum_stride(kBN);
+  static_assert(kBM * kStride * 4 <= kStages * kTileStage, "the sums take the stages' place");
 
   if (warp == 0 && lane == 0) {
-    produce<C::stages>(g, &ta, &tb, smem0, C::stage_bytes, C::a_bytes, full0, done0, PairLink{}, [&](auto&& load) {
-      for (int w = first; w < total; w += step)
-        for (int kb = kb0; kb < kb1; ++kb)
-          if (!load(kb * kGroup, (w / tiles_n) * kBM, (w % tiles_n) * BN)) return;
+    produce<kStages>(g, &ta, &tb, smem0, kTileStage, kTileA, full0, done0, PairLink{}, [&](auto&& load) {
+      for (int kb = kb0; kb < kb1; ++kb)
+        if (!load(kb * kGroup, m0, n0)) return;
     });
   } else if (warp == 1 && lane == 0) {
-    const uint32_t tiles = (total - 1 - first) / step + 1;   // never more CTAs than tiles
-    multiply<C::stages, C::buffers, BN, false>(g, tiles * (kb1 - kb0), smem0, C::stage_bytes, C::a_bytes, tmem, full0,
-                                               done0, tempty0);
+    multiply<kStages, kBuffers, kBN, false>(g, kb1 - kb0, smem0, kTileStage, kTileA, tmem, full0, done0, tempty0);
   } else if (warp >= 2) {
     const int q = warp & 3, half = (warp - 2) >> 2;
-    epilogue<C::stages, C::buffers, BN>(
-        g, tmem, done0, tempty0, q, half,
-        [&](auto&& tile) {
-          for (int w = first; w < total; w += step)
-            if (!tile((w / tiles_n) * kBM, (w % tiles_n) * BN, kb0, kb1)) return;
-        },
-        [&](auto& acc, int row, int n0) {
-          if (splits > 1) keep_sums<BN / 64>(sums, kStride, acc, 32 * q + lane, half * (BN / 2));
-          else store_rows<BN / 64>(g, acc, row - lane, n0, stage0 + (warp - 2) * kStoreStage);
+    epilogue<kStages, kBuffers, kBN>(
+        g, tmem, done0, tempty0, q, half, [&](auto&& sum) { sum(m0, n0, kb0, kb1); },
+        [&](auto& acc, int row, int col) {
+          if (splits > 1) keep_sums<kBN / 64>(sums, kStride, acc, 32 * q + lane, half * (kBN / 2));
+          else store_rows<kBN / 64>(g, acc, row - lane, col, stage0 + (warp - 2) * kStoreStage);
         });
   }
   if (splits > 1) {
     __syncwarp();
     tc::cluster_sync();
-    const int m0 = (first / tiles_n) * kBM, n0 = (first % tiles_n) * BN, rows = kBM / splits;
-    for (int e = threadIdx.x; e < rows * (BN / 4); e += kThreads) {
-      const int r = rank * rows + e / (BN / 4), c = (e % (BN / 4)) * 4;
+    const int rows = kBM / splits;
+    for (int e = threadIdx.x; e < rows * (kBN / 4); e += kThreads) {
+      const int r = rank * rows + e / (kBN / 4), c = (e % (kBN / 4)) * 4;
       if (m0 + r >= g.M || n0 + c >= g.N) continue;
       const float4 v = cluster_sum(smem0, kStride, splits, r, c);
       store_one(g, m0 + r, n0 + c, v.x);
@@ -801,16 +792,12 @@ void launch_cluster(K* kernel, int grid, int threads, size_t smem, int cluster, 
   TORCH_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess, "fp8_matmul launch failed");
 }
 
-template <int BN>
-void launch(const CUtensorMap& ta, const CUtensorMap& tb, Args g, cudaStream_t st) {
+// At most as many tiles as SMs.
+void launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, Args g, int tiles, cudaStream_t st) {
   static size_t configured[dynsmem::kMaxDevices] = {};
-  TORCH_CHECK(dynsmem::opt_in(fp8_gemm_kernel<BN>, Config<BN>::smem_bytes, configured) == cudaSuccess,
-              "fp8_matmul shared-memory attribute");
-  const int64_t tiles = (int64_t)((g.N + BN - 1) / BN) * ((g.M + kBM - 1) / kBM);
-  TORCH_CHECK(tiles < (1ll << 31), "fp8_matmul: too many output tiles");
+  TORCH_CHECK(dynsmem::opt_in(fp8_gemm_kernel, kSmem, configured) == cudaSuccess, "fp8_matmul shared-memory attribute");
   g.splits = splits_for(tiles, g.groups);
-  const int grid = g.splits > 1 ? (int)tiles * g.splits : (int)std::min<int64_t>(tiles, lm::sm_count());
-  launch_cluster(fp8_gemm_kernel<BN>, grid, kThreads, Config<BN>::smem_bytes, g.splits, st, ta, tb, g);
+  launch_cluster(fp8_gemm_kernel, tiles * g.splits, kThreads, kSmem, g.splits, st, ta, tb, g);
 }
 
 template <int COLS>
@@ -893,7 +880,7 @@ torch::Tensor matmul(const torch::Tensor& a, const torch::Tensor& a_scale, const
     const CUtensorMap ta = tma::u8_sw128(a.data_ptr(), M, K, lda, kBM);
     const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);
     if (tiles > lm::sm_count()) launch_pair<false>(ta, tb, g, ((M + 255) / 256) * ((N + 255) / 256), st);
-    else launch<128>(ta, tb, g, st);
+    else launch_tiles(ta, tb, g, (int)tiles, st);
   }
   lm::count_launches(1);
   return c;

@@ -587,5 +587,4 @@ void register_rmsnorm_ops(py::module& m) {
         py::arg("x"), py::arg("weight"), py::arg("residual"), py::arg("eps"));
   m.def("rms_norm_fp8", &rms_norm_fp8, "RMS norm with an e4m3 result: (q, scale) or (q, scale, h)", py::arg("x"),
         py::arg("weight"), py::arg("residual"), py::arg("eps"));
-  m.attr("RMS_NORM_MAX_WIDTH") = kMaxWidth;
 }

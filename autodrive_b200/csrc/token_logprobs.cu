@@ -689,7 +689,7 @@ Results forward(const torch::Tensor& x, const torch::Tensor& tokens, const torch
     } else {
       // few rows: as many CTAs for each as give the SMs two, with a vector at least for every thread
       a.splits = 1;
-      while (a.splits < kMaxSplits && a.rows * a.splits * 2 <= 2 * lm::sm_count() && a.v / 8 >= 2 * a.splits * kThreads)
+      while (a.splits < kMaxSplits && a.rows * a.splits <= lm::sm_count() && a.v / 8 >= 2 * a.splits * kThreads)
         a.splits *= 2;
       TORCH_CHECK(a.rows * a.splits < (1ll << 31), "token_log_probs: too many rows");
       cudaLaunchConfig_t cfg = {};
@@ -830,5 +830,4 @@ void register_token_logprobs_ops(py::module& m) {
   m.def("token_log_probs", &token_log_probs,
         "log-probabilities of given tokens, with autograd: (log_prob, entropy, top_log_prob, top_token)",
         py::arg("logits"), py::arg("tokens"), py::arg("mask"), py::arg("temperature"), py::arg("top"));
-  m.attr("TOKEN_LOG_PROBS_MAX_TOP") = kMaxTop;
 }
