@@ -32,6 +32,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "fp8.h"
 #include "lm_host.h"
@@ -768,27 +769,52 @@ sum_slices_kernel(const float* __restrict__ parts, int splits, int64_t count, T*
   }
 }
 
-// CTAs that share a tile: enough to give most SMs one, a power of two that
-// divides a tile's rows, and a part of at least two groups each.
-int splits_for(int64_t tiles, int groups) {
-  int s = 1;
-  while (s < kMaxSplits && tiles * s * 2 <= lm::sm_count() + lm::sm_count() / 4 && groups >= 4 * s) s *= 2;
-  return s;
-}
-
-template <typename K, typename... A>
-void launch_cluster(K* kernel, int grid, int threads, size_t smem, int cluster, cudaStream_t st, const A&... args) {
+template <typename K>
+cudaLaunchConfig_t cluster_config(K* kernel, int grid, int threads, size_t smem, int cluster, cudaStream_t st,
+                                  cudaLaunchAttribute* attr) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = cluster;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = cluster;
+  attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
+  cfg.attrs = attr;
   cfg.numAttrs = 1;
+  return cfg;
+}
+
+// CTAs that share a tile: the largest power of two (it divides a tile's rows)
+// with which all clusters run at once and a CTA's part has at least two groups.
+// How many clusters fit is asked of the device, whose SMs come in groups that
+// clusters do not cross: 15 of eight, 33 of four and 74 of two on 148 SMs. One
+// cluster too many costs a second round: 16 rows x 8192 columns take 7.4 us for
+// 15 tiles and 13.5 for 16 in clusters of eight, against 9.4 in clusters of four.
+// `KERNEL` has opted in to its shared memory.
+template <auto* KERNEL>
+int splits_for(int64_t tiles, int groups, int threads, size_t smem) {
+  static std::atomic<int> fits[64][4];   // by device and cluster size
+  int dev = 0;
+  TORCH_CHECK(cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64, "fp8_matmul: device query failed");
+  int s = 1;
+  for (int i = 1; 2 * s <= kMaxSplits && groups >= 4 * s; ++i, s *= 2) {
+    int n = fits[dev][i].load(std::memory_order_relaxed);
+    if (n == 0) {
+      cudaLaunchAttribute attr = {};
+      const auto cfg = cluster_config(KERNEL, 2 * s, threads, smem, 2 * s, nullptr, &attr);
+      TORCH_CHECK(cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) == cudaSuccess, "fp8_matmul: occupancy query failed");
+      fits[dev][i].store(n, std::memory_order_relaxed);
+    }
+    if (tiles > n) break;
+  }
+  return s;
+}
+
+template <typename K, typename... A>
+void launch_cluster(K* kernel, int grid, int threads, size_t smem, int cluster, cudaStream_t st, const A&... args) {
+  cudaLaunchAttribute attr = {};
+  const auto cfg = cluster_config(kernel, grid, threads, smem, cluster, st, &attr);
   TORCH_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess, "fp8_matmul launch failed");
 }
 
@@ -796,19 +822,23 @@ void launch_cluster(K* kernel, int grid, int threads, size_t smem, int cluster, 
 void launch_tiles(const CUtensorMap& ta, const CUtensorMap& tb, Args g, int tiles, cudaStream_t st) {
   static size_t configured[dynsmem::kMaxDevices] = {};
   TORCH_CHECK(dynsmem::opt_in(fp8_gemm_kernel, kSmem, configured) == cudaSuccess, "fp8_matmul shared-memory attribute");
-  g.splits = splits_for(tiles, g.groups);
+  g.splits = splits_for<fp8_gemm_kernel>(tiles, g.groups, kThreads, kSmem);
   launch_cluster(fp8_gemm_kernel, tiles * g.splits, kThreads, kSmem, g.splits, st, ta, tb, g);
 }
 
+// Up to COLS rows of A; false where the scales of a CTA's groups do not fit into its shared memory.
 template <int COLS>
-void launch_rows(const CUtensorMap& tb, const torch::Tensor& a, int64_t lda, Args g, int splits, cudaStream_t st) {
+bool launch_rows(const CUtensorMap& tb, const torch::Tensor& a, int64_t lda, Args g, cudaStream_t st) {
   static size_t configured[dynsmem::kMaxDevices] = {};
   TORCH_CHECK(dynsmem::opt_in(fp8_gemm_rows_kernel<COLS>, rows_smem_bytes<COLS>(), configured) == cudaSuccess,
               "fp8_matmul shared-memory attribute");
-  g.splits = splits;
+  const int tiles = (g.N + kBM - 1) / kBM;
+  g.splits = splits_for<fp8_gemm_rows_kernel<COLS>>(tiles, g.groups, kRowsThreads, rows_smem_bytes<COLS>());
+  if ((g.groups + g.splits - 1) / g.splits * COLS > kRowsScales) return false;
   const CUtensorMap ta = tma::u8_sw128(a.data_ptr(), a.size(0), a.size(1), lda, COLS);
-  launch_cluster(fp8_gemm_rows_kernel<COLS>, (g.N + kBM - 1) / kBM * splits, kRowsThreads, rows_smem_bytes<COLS>(), splits,
-                 st, tb, ta, g);
+  launch_cluster(fp8_gemm_rows_kernel<COLS>, tiles * g.splits, kRowsThreads, rows_smem_bytes<COLS>(), g.splits, st, tb, ta,
+                 g);
+  return true;
 }
 
 template <bool WIDE>
@@ -872,11 +902,8 @@ torch::Tensor matmul(const torch::Tensor& a, const torch::Tensor& a_scale, const
   //  * 128 x 128 tiles, or parts of them, while one round of CTAs has them all: 18 against 24 with pairs for
   //    1024 x 2048, where pairs leave half of the SMs idle;
   //  * pairs of CTAs beyond: 25 against 31 for 2048 x 2048, 85 against 111 for 9472 x 2048.
-  const int cols = M <= 16 ? 16 : 32, splits = splits_for((N + kBM - 1) / kBM, g.groups);
-  if (M <= 32 && (g.groups + splits - 1) / splits * cols <= kRowsScales) {
-    if (cols == 16) launch_rows<16>(tb, a, lda, g, splits, st);
-    else launch_rows<32>(tb, a, lda, g, splits, st);
-  } else {
+  const bool few = M <= 16 ? launch_rows<16>(tb, a, lda, g, st) : M <= 32 && launch_rows<32>(tb, a, lda, g, st);
+  if (!few) {
     const CUtensorMap ta = tma::u8_sw128(a.data_ptr(), M, K, lda, kBM);
     const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);
     if (tiles > lm::sm_count()) launch_pair<false>(ta, tb, g, ((M + 255) / 256) * ((N + 255) / 256), st);

@@ -575,3 +575,13 @@ def test_freeze_leaves_layers_whose_weights_others_read():
         want = net[0](x)
         freeze_fp8(net)
         assert torch.equal(net[0](x), want) and isinstance(net[1], FrozenFp8Linear)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(16, 2048, 2048), (32, 2560, 2048), (3, 4480, 1100), (16, 9500, 700), (640, 512, 2100),
+                                   (1400, 1000, 1024)])
+def test_product_where_the_number_of_clusters_decides(m, n, k):
+    a, a_s = quantize_rows(_values(m, k, 1, device="cuda"))
+    b, b_s = quantize_blocks(_values(n, k, 2, device="cuda") * k ** -.5)
+    _check_product(fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32), a, a_s, b, b_s, None, torch.float32)
+    check_gemm_status(torch.device("cuda", 0))
