@@ -985,9 +985,10 @@ torch::Tensor fp8_matmul(torch::Tensor a, torch::Tensor a_scale, torch::Tensor b
   LM_CHECK_VALUE(!bias || bias->device() == a.device(), "fp8_matmul needs all of its tensors on one device");
   TORCH_CHECK(status.scalar_type() == torch::kInt32, "fp8_matmul: status must be int32");
   LM_CHECK_VALUE(wait_ns >= 0, "wait_ns must not be negative");
-  LM_CHECK_VALUE(!lm::any_tangent(a_scale, b_scale, bias) &&
+  LM_CHECK_VALUE(!lm::any_tangent(a, a_scale, b, b_scale, bias) &&
                      !(at::GradMode::is_enabled() &&
-                       (a_scale.requires_grad() || b_scale.requires_grad() || (bias && bias->requires_grad()))),
+                       (a.requires_grad() || a_scale.requires_grad() || b.requires_grad() || b_scale.requires_grad() ||
+                        (bias && bias->requires_grad()))),
                     "fp8_matmul has no gradient: use fp8_linear, or call it under torch.no_grad()");
   const int64_t rows = c10::multiply_integers(a.sizes().slice(0, a.dim() - 1));
   const auto a2 = a.dim() == 2 ? a : a.reshape({rows, K});

@@ -177,7 +177,7 @@ def fp8_matmul(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Ten
         raise ValueError("fp8_matmul gives fp32, bf16 or fp16")
     if any(t is not None and t.device != a.device for t in (a_scale, b, b_scale, bias)):
         raise ValueError("fp8_matmul needs all of its tensors on one device")
-    if wants_derivative(a_scale, b_scale, bias):
+    if wants_derivative(a, a_scale, b, b_scale, bias):
         raise ValueError("fp8_matmul has no gradient: use fp8_linear, or call it under torch.no_grad()")
     rows = lead.numel()
     return reference_fp8_matmul(a.reshape(rows, k), a_scale.reshape(rows, _groups(k)), b, b_scale, bias,

@@ -585,3 +585,15 @@ def test_product_where_the_number_of_clusters_decides(m, n, k):
     b, b_s = quantize_blocks(_values(n, k, 2, device="cuda") * k ** -.5)
     _check_product(fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32), a, a_s, b, b_s, None, torch.float32)
     check_gemm_status(torch.device("cuda", 0))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_product_refuses_operands_that_want_a_gradient(device):
+    q, s = quantize_rows(torch.randn(4, 256, device=device))
+    wq, ws = quantize_blocks(torch.randn(130, 256, device=device))
+    for bad in (lambda: fp8_matmul(q.clone().requires_grad_(True), s, wq, ws),
+                lambda: fp8_matmul(q, s, wq.clone().requires_grad_(True), ws)):
+        with pytest.raises(ValueError):
+            bad()
+        with torch.no_grad():
+            assert bad().shape == (4, 130)
