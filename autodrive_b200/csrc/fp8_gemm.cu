@@ -789,8 +789,8 @@ cudaLaunchConfig_t cluster_config(K* kernel, int grid, int threads, size_t smem,
 // with which all clusters run at once and a CTA's part has at least two groups.
 // How many clusters fit is asked of the device, whose SMs come in groups that
 // clusters do not cross: 15 of eight, 33 of four and 74 of two on 148 SMs. One
-// cluster too many costs a second round: 16 rows x 8192 columns take 7.4 us for
-// 15 tiles and 13.5 for 16 in clusters of eight, against 9.4 in clusters of four.
+// cluster too many costs a second round: at 16 rows and K = 8192, 15 tiles take
+// 7.4 us in clusters of eight, and 16 tiles 13.5, against 9.4 in clusters of four.
 // `KERNEL` has opted in to its shared memory.
 template <auto* KERNEL>
 int splits_for(int64_t tiles, int groups, int threads, size_t smem) {
@@ -897,11 +897,11 @@ torch::Tensor matmul(const torch::Tensor& a, const torch::Tensor& a_scale, const
   const CUtensorMap tb = tma::u8_sw128(b.data_ptr(), N, K, N > 1 ? b.stride(0) : one_row, 128);
   auto st = c10::cuda::getCurrentCUDAStream().stream();
   // By sizes alone (us measured at N = K = 4096 unless said):
-  //  * up to 32 rows the few-row kernel, 7.9 against 10.1 with 128 x 128 tiles at 16 rows, 9.9 against 12.9 for one row
-  //    of 1408 x 16640, 9.1 against 10.8 at 32 rows (at 64 there is no difference: 11.1 and 10.9);
-  //  * 128 x 128 tiles, or parts of them, while one round of CTAs has them all: 18 against 24 with pairs for
+  //  * up to 32 rows the few-row kernel, 7.0 against 9.7 with 128 x 128 tiles at 16 rows, 9.4 against 12.6 for one row
+  //    of 1408 x 16640, 8.7 against 9.7 at 32 rows;
+  //  * 128 x 128 tiles, or parts of them, while one round of CTAs has them all: 17.8 against 23.2 with pairs for
   //    1024 x 2048, where pairs leave half of the SMs idle;
-  //  * pairs of CTAs beyond: 25 against 31 for 2048 x 2048, 85 against 111 for 9472 x 2048.
+  //  * pairs of CTAs beyond: 24.4 against 33.2 for 2048 x 2048, 82.9 against 128 for 9472 x 2048.
   const bool few = M <= 16 ? launch_rows<16>(tb, a, lda, g, st) : M <= 32 && launch_rows<32>(tb, a, lda, g, st);
   if (!few) {
     const CUtensorMap ta = tma::u8_sw128(a.data_ptr(), M, K, lda, kBM);

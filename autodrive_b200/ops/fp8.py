@@ -156,7 +156,9 @@ def fp8_matmul(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Ten
                out_dtype: torch.dtype = torch.bfloat16, wait_ns: int = 2_000_000_000) -> Tensor:
     """a b^T of quantised rows `a` [..., K] and a quantised matrix `b` [N, K]
     with their scales, plus `bias` [N]: [..., N] in `out_dtype` (fp32, bf16 or
-    fp16). `wait_ns` bounds every pipeline wait inside the kernel."""
+    fp16). The product of a row's scale and a block's is taken in fp32: below
+    its normal range, 2^-126, it counts as zero, beyond its end as infinite.
+    `wait_ns` bounds every pipeline wait inside the kernel."""
     if a.is_cuda:
         y = require_extension().fp8_matmul(a, a_scale, b, b_scale, bias, out_dtype, _Status.get(a.device), wait_ns)
         _Status.after_launch(a.device)

@@ -12,8 +12,8 @@ of the valid entries that broadcasts against the logits, and returns
 * ``log_prob`` [...] and ``entropy`` [...] are fp32 and differentiable with
   respect to the logits; the log-probability of a masked token is -inf;
 * ``top_log_prob`` / ``top_token`` [..., top] are the ``top`` (at most 64) most
-  probable entries, equal ones by their index, without gradient; where a row
-  has fewer entries of positive probability they are -inf and -1;
+  probable entries, equal ones by their index (on CUDA all values below fp32's
+  normal range, 2^-126, equal zero), without gradient; where a row has fewer entries of positive probability they are -inf and -1;
 * a negative token marks a row to be ignored: log_prob 0, no gradient from it
   (its entropy and alternatives are given all the same); a token beyond the
   last entry gives NaN;

@@ -597,3 +597,14 @@ def test_product_refuses_operands_that_want_a_gradient(device):
             bad()
         with torch.no_grad():
             assert bad().shape == (4, 130)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [4, 200, 5000])
+def test_products_of_scales_at_the_end_of_the_range(m):
+    """2^-63 times 2^-62 is a normal fp32 number; 2^-64 times 2^-63 is below them and counts as zero."""
+    a, a_s = quantize_rows(_values(m, 256, 1, device="cuda"))
+    b, b_s = quantize_blocks(_values(600, 256, 2, device="cuda"))
+    a_s, b_s = torch.full_like(a_s, 2. ** -63), torch.full_like(b_s, 2. ** -62)
+    _check_product(fp8_matmul(a, a_s, b, b_s, out_dtype=torch.float32), a, a_s, b, b_s, None, torch.float32)
+    assert (fp8_matmul(a, a_s / 2, b, b_s / 2, out_dtype=torch.float32) == 0).all()

@@ -391,3 +391,12 @@ def test_equal_entries(v):
     r = token_log_probs(x, torch.zeros(v, dtype=torch.long, device="cuda"), torch.arange(v, device="cuda") < n[:, None])
     want = n.double().log()
     assert ((r.entropy - want).abs() <= 6 * F * want).all() and torch.equal(r.log_prob, -r.entropy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [8, 3000])
+def test_values_below_the_normal_range_equal_zero(v):
+    x = torch.full((2, v), -1., device="cuda")
+    x[0, 2], x[0, 5], x[1, 1], x[1, 4], x[1, 6] = 0., 1e-40, -1e-40, 1e-39, 2. ** -126
+    r = token_log_probs(x, torch.zeros(2, dtype=torch.long, device="cuda"), top=3)
+    assert r.top_token[0, :2].tolist() == [2, 5] and r.top_token[1].tolist() == [6, 1, 4]
