@@ -221,7 +221,7 @@ def _plain_sample(s):
     dev = s["logits"].device
 
     def column(value, dtype):
-        return torch.as_tensor(value, device=dev).to(dtype).expand(rows)[:, None]
+        return torch.as_tensor(value, dtype=dtype, device=dev).expand(rows)[:, None]
 
     z = s["logits"].float()
     if s["mask"] is not None:
@@ -409,7 +409,7 @@ def _exact_sample(s):
     rows, v = case["rows"], case["v"]
     dev = s["logits"].device
     step = max(1, 8_000_000 // v)
-    each = {k: torch.as_tensor(s[k], device=dev).double().expand(rows) for k in ("temperature", "top_k", "top_p", "min_p")}
+    each = {k: torch.as_tensor(s[k], dtype=torch.float64, device=dev).expand(rows) for k in ("temperature", "top_k", "top_p", "min_p")}
     for r in range(0, rows, step):
         c = slice(r, min(rows, r + step))
         value = s["logits"][c].double()
