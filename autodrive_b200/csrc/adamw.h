@@ -1,0 +1,52 @@
+// The AdamW step's kernels (adamw.cu) as the entry point (adamw_ops.cpp) calls them.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace adamw {
+
+constexpr int kBlock = 256;          // elements of a block: a warp's work, one scale of the 8-bit moments
+
+struct Entry {
+  void *p, *m, *v;
+  const void* g;
+  float *m_scale, *v_scale;
+  uint64_t n : 56;
+  uint64_t p_type : 2, g_type : 2;   // 0 fp32, 1 bf16, 2 fp16
+  uint64_t vec : 1;                  // every address allows whole-lane accesses
+  uint32_t first;                    // its first block among the launch's
+  uint32_t step;
+};
+static_assert(sizeof(Entry) == 64, "table entry");
+
+struct Header {
+  uint32_t blocks;      // of the launch
+  uint32_t block0;      // blocks of the launches before (for the random bits)
+  int tensors;
+  uint32_t seed;        // mixed seed
+  float b1, c1, b2, c2; // c = 1 - b
+  float lr, decay, eps, log_b1, log_b2;
+  const int64_t* step_at;   // the number of every tensor's step on the device, or null
+  const double* parts;  // partial sums of the gradients' squares, or null
+  int nparts;
+  float max_norm;
+  float* norm_out;
+};
+
+constexpr int kMaxTensors = 500;     // of a launch
+constexpr int kWarps = 8;            // of a CTA
+
+// 32 mixed bits of 32: two rounds of multiplication and shifted exclusive or.
+__host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
+  x = (x ^ (x >> 16)) * 0x7feb352du;
+  x = (x ^ (x >> 15)) * 0x846ca68bu;
+  return x ^ (x >> 16);
+}
+
+// `grid` CTAs over the entries of one launch, which are counted from its own first block.
+cudaError_t launch_square_sums(const Header& h, const Entry* entries, double* parts, int grid, cudaStream_t st);
+cudaError_t launch_step(const Header& h, const Entry* entries, bool bits8, int grid, cudaStream_t st);
+
+}  // namespace adamw

@@ -1,0 +1,214 @@
+// Entry point of the AdamW step over a list of tensors (adamw.cu).
+#include <torch/extension.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "adamw.h"
+#include "lm_host.h"
+
+namespace py = pybind11;
+
+namespace {
+
+using namespace adamw;
+
+int type_code(torch::ScalarType t) {
+  return t == torch::kFloat32 ? 0 : t == torch::kBFloat16 ? 1 : t == torch::kHalf ? 2 : -1;
+}
+
+bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+using List = std::vector<torch::Tensor>;
+
+void touch(const torch::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+void check(cudaError_t e) {
+  TORCH_CHECK(e == cudaSuccess, "adamw_step launch failed");
+  lm::count_launches(1);
+}
+
+// A gradient as its parameter lies in memory.
+torch::Tensor in_layout_of(const torch::Tensor& g, const torch::Tensor& p) {
+  if (g.strides() == p.strides() || p.numel() <= 1) return g;
+  auto y = torch::empty_strided(p.sizes(), p.strides(), g.options());
+  y.copy_(g);
+  return y;
+}
+
+py::object adamw_step(List params, List grads, List ms, List vs, c10::optional<List> m_scales, c10::optional<List> v_scales,
+                      py::object step, double lr, double b1, double b2, double eps, double weight_decay, double max_norm,
+                      int64_t seed) {
+  const size_t count = params.size();
+  const bool bits8 = m_scales.has_value();
+  LM_CHECK_VALUE(grads.size() == count && ms.size() == count && vs.size() == count &&
+                     m_scales.has_value() == v_scales.has_value() &&
+                     (!bits8 || (m_scales->size() == count && v_scales->size() == count)),
+                 "adamw_step needs a gradient and two moments (8-bit ones with their scales) for each of ", (int64_t)count,
+                 " parameters");
+  if (count == 0) return py::none();
+  const auto device = params[0].device();
+  const c10::cuda::CUDAGuard guard(device);
+  const auto st = c10::cuda::getCurrentCUDAStream().stream();
+
+  Header h{};
+  std::vector<int64_t> steps;
+  if (THPVariable_Check(step.ptr())) {
+    const auto s = step.cast<torch::Tensor>();
+    LM_CHECK_VALUE(s.scalar_type() == torch::kInt64 && s.numel() == 1 && s.device() == device,
+                   "adamw_step needs its step as a number, a list of numbers or one int64 on ", device);
+    h.step_at = s.data_ptr<int64_t>();
+  } else {
+    if (py::isinstance<py::int_>(step)) steps.assign(count, step.cast<int64_t>());
+    else steps = step.cast<std::vector<int64_t>>();
+    LM_CHECK_VALUE(steps.size() == count, "adamw_step needs one step for all or for each of ", (int64_t)count, " parameters");
+    for (int64_t s : steps) LM_CHECK_VALUE(s >= 1 && s <= UINT32_MAX, "adamw_step counts its steps from 1, not ", s);
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    TORCH_CHECK(cudaStreamIsCapturing(st, &capture) == cudaSuccess, "adamw_step: stream query failed");
+    TORCH_CHECK(capture == cudaStreamCaptureStatusNone,
+                "adamw_step: a captured step would be replayed under its one number; give the step as an int64 tensor on ",
+                device.str());
+  }
+
+  std::vector<Entry> all;
+  all.reserve(count);
+  List keep;   // gradients that were laid out anew
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  spans.reserve(count);
+  uint64_t blocks = 0;
+  std::vector<uint64_t> first;
+  first.reserve(count);
+  for (size_t i = 0; i < count; ++i) {
+    const torch::Tensor &p = params[i], &m = ms[i], &v = vs[i];
+    torch::Tensor g = grads[i];
+    const int pt = type_code(p.scalar_type()), gt = type_code(g.scalar_type());
+    LM_CHECK_VALUE(pt >= 0 && gt >= 0, "adamw_step takes fp32, bf16 or fp16 parameters and gradients");
+    const auto mt = bits8 ? torch::kFloat8_e4m3fn : torch::kFloat32;
+    LM_CHECK_VALUE(m.scalar_type() == mt && v.scalar_type() == mt,
+                   "adamw_step takes moments in fp32, or in e4m3 with scales");
+    LM_CHECK_VALUE(p.device() == device && g.device() == device && m.device() == device && v.device() == device,
+                   "adamw_step needs all of its tensors on one device");
+    LM_CHECK_VALUE(g.sizes() == p.sizes(), "adamw_step: gradient ", g.sizes(), " of a parameter ", p.sizes());
+    LM_CHECK_VALUE(!g.is_sparse() && p.is_non_overlapping_and_dense(),
+                   "adamw_step needs dense parameters without gaps");
+    LM_CHECK_VALUE(m.sizes() == p.sizes() && v.sizes() == p.sizes() &&
+                       (p.numel() <= 1 || (m.strides() == p.strides() && v.strides() == p.strides())),
+                   "adamw_step needs moments of their parameter's shape and strides ", p.sizes());
+    const int64_t n = p.numel(), nb = (n + kBlock - 1) / kBlock;
+    if (bits8)
+      for (const auto* s : {&(*m_scales)[i], &(*v_scales)[i]})
+        LM_CHECK_VALUE(s->scalar_type() == torch::kFloat32 && s->device() == device && s->dim() == 1 && s->size(0) == nb &&
+                           s->is_contiguous(),
+                       "adamw_step needs ", nb, " fp32 scales of 256 elements each for a parameter ", p.sizes());
+    if (n == 0) continue;
+    if (g.strides() != p.strides() && n > 1) {
+      g = in_layout_of(g, p);
+      keep.push_back(g);
+    }
+    Entry e{};
+    e.p = p.data_ptr();
+    e.g = g.data_ptr();
+    e.m = m.data_ptr();
+    e.v = v.data_ptr();
+    if (bits8) {
+      e.m_scale = (*m_scales)[i].data_ptr<float>();
+      e.v_scale = (*v_scales)[i].data_ptr<float>();
+    }
+    e.n = (uint64_t)n;
+    e.step = steps.empty() ? 0 : (uint32_t)steps[i];
+    e.p_type = (unsigned)pt;
+    e.g_type = (unsigned)gt;
+    e.vec = aligned(e.p, pt ? 16 : 32) && aligned(e.g, gt ? 16 : 32) && aligned(e.m, bits8 ? 8 : 32) &&
+            aligned(e.v, bits8 ? 8 : 32);
+    all.push_back(e);
+    first.push_back(blocks);
+    blocks += nb;
+    const auto at = reinterpret_cast<uintptr_t>(e.p);
+    spans.emplace_back(at, at + n * p.element_size());
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    LM_CHECK_VALUE(spans[i].first >= spans[i - 1].second, "adamw_step: two parameters share memory");
+
+  // launches of at most kMaxTensors tensors and 2^31 blocks
+  std::vector<std::pair<size_t, size_t>> ranges;
+  for (size_t i = 0; i < all.size();) {
+    size_t j = i;
+    while (j < all.size() && j - i < (size_t)kMaxTensors) {
+      const int64_t nb = ((int64_t)all[j].n + kBlock - 1) / kBlock;
+      LM_CHECK_VALUE(nb <= (int64_t)1 << 31, "adamw_step: a parameter has more than 2^39 elements");
+      if (j > i && first[j] + nb - first[i] > (uint64_t)1 << 31) break;
+      all[j].first = (uint32_t)(first[j] - first[i]);
+      ++j;
+    }
+    ranges.emplace_back(i, j);
+    i = j;
+  }
+
+  h.b1 = (float)b1;
+  h.c1 = (float)(1. - b1);
+  h.b2 = (float)b2;
+  h.c2 = (float)(1. - b2);
+  h.decay = (float)(1. - lr * weight_decay);
+  h.eps = (float)eps;
+  h.lr = (float)lr;
+  h.log_b1 = (float)std::log(b1);
+  h.log_b2 = (float)std::log(b2);
+  h.seed = mix((uint32_t)seed);
+  const auto grid_of = [&](size_t r) {
+    const uint64_t nb = (ranges[r].second < all.size() ? first[ranges[r].second] : blocks) - first[ranges[r].first];
+    return (int)std::min<uint64_t>((nb + kWarps - 1) / kWarps, (uint64_t)lm::sm_count() * 4);
+  };
+  const auto header_of = [&](size_t r) {
+    Header x = h;
+    x.tensors = (int)(ranges[r].second - ranges[r].first);
+    x.block0 = (uint32_t)first[ranges[r].first];
+    x.blocks = (uint32_t)((ranges[r].second < all.size() ? first[ranges[r].second] : blocks) - first[ranges[r].first]);
+    return x;
+  };
+  torch::Tensor norm, parts;
+  if (max_norm > 0.) {
+    norm = torch::empty({}, params[0].options().dtype(torch::kFloat32));
+    int total = 0;
+    for (size_t r = 0; r < ranges.size(); ++r) total += grid_of(r);
+    if (total == 0) norm.zero_();
+    parts = torch::empty({std::max(total, 1)}, params[0].options().dtype(torch::kFloat64));
+    int at = 0;
+    for (size_t r = 0; r < ranges.size(); ++r) {
+      check(launch_square_sums(header_of(r), all.data() + ranges[r].first, parts.data_ptr<double>() + at, grid_of(r), st));
+      at += grid_of(r);
+    }
+    h.parts = parts.data_ptr<double>();
+    h.nparts = total;
+    h.max_norm = (float)max_norm;
+  }
+  for (size_t r = 0; r < ranges.size(); ++r) {
+    Header x = header_of(r);
+    x.norm_out = r == 0 && norm.defined() ? norm.data_ptr<float>() : nullptr;
+    check(launch_step(x, all.data() + ranges[r].first, bits8, grid_of(r), st));
+  }
+  for (size_t i = 0; i < count; ++i) {
+    touch(params[i]);
+    touch(ms[i]);
+    touch(vs[i]);
+    if (bits8) {
+      touch((*m_scales)[i]);
+      touch((*v_scales)[i]);
+    }
+  }
+  return norm.defined() ? py::cast(norm) : py::object(py::none());
+}
+
+}  // namespace
+
+void register_adamw_ops(py::module& m) {
+  m.def("adamw_step", &adamw_step, "AdamW over a list of tensors, moments in fp32 or 8 bits", py::arg("params"),
+        py::arg("grads"), py::arg("exp_avgs"), py::arg("exp_avg_sqs"), py::arg("exp_avg_scales"),
+        py::arg("exp_avg_sq_scales"), py::arg("step"), py::arg("lr"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"),
+        py::arg("weight_decay"), py::arg("max_grad_norm"), py::arg("seed"));
+}

@@ -200,6 +200,9 @@ void register_fp8_quant_ops(py::module& m);
 void register_fp8_gemm_ops(py::module& m);
 void register_fp8_linear_ops(py::module& m);
 void register_token_logprobs_ops(py::module& m);
+void register_adamw_ops(py::module& m);
+void register_groupnorm_ops(py::module& m);
+void register_sampling_ops(py::module& m);
 void register_adstar_cpu(py::module& m);
 void register_sha256_ops(py::module& m);
 void register_plan_a_ops(py::module& m);
@@ -267,6 +270,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_fp8_gemm_ops(m);
   register_fp8_linear_ops(m);
   register_token_logprobs_ops(m);
+  register_adamw_ops(m);
+  register_groupnorm_ops(m);
+  register_sampling_ops(m);
   register_adstar_cpu(m);
   register_sha256_ops(m);
   register_plan_a_ops(m);

@@ -1,0 +1,49 @@
+// The group norm's kernels (groupnorm.cu) as the entry point (groupnorm_ops.cpp) calls them.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace groupnorm {
+
+enum Activation : int { kNone = 0, kSilu = 1, kRelu = 2, kGelu = 3 };
+
+// A tensor in channels-last memory: `n` samples of `pixels` rows of `c` channels, back to back.
+struct Shape {
+  int64_t n, pixels;
+  int c, groups;
+  int type;      // 0 fp32, 1 bf16, 2 fp16
+};
+
+// How a launch cuts the samples (see plan() in groupnorm.cu).
+struct Plan {
+  int vec;            // elements of an access
+  int threads, cols, rows;   // vectors that repeat the channels' pattern; such rows that a CTA takes at a time
+  int ctas;           // that share a sample
+  int64_t chunk;      // vectors of a CTA's part, a multiple of cols
+  int iterations;     // of a thread over its part
+  bool resident;      // a cluster holds the sample in shared memory
+  int smem;
+};
+
+struct Affine {
+  const void *w, *b;         // or null: 1, 0
+  int w_type, b_type;
+};
+
+Plan plan(const Shape& s, bool backward, bool aligned, int sms);
+
+// Floats of workspace that a launch needs.
+int64_t forward_workspace(const Shape& s, const Plan& p);
+int64_t backward_workspace(const Shape& s, const Plan& p);
+
+// y, and mean and 1 / deviation [n, groups] (or null).
+cudaError_t forward(const Shape& s, const Plan& p, const void* x, const Affine& a, float eps, Activation act, void* y,
+                    float* mean, float* rstd, float* workspace, cudaStream_t st);
+// dx, and dw and db [c] in their parameters' types (or null).
+cudaError_t backward(const Shape& s, const Plan& p, const void* dy, const void* x, const Affine& a, const float* mean,
+                     const float* rstd, Activation act, void* dx, void* dw, void* db, float* workspace, cudaStream_t st);
+int launches(const Plan& p, bool backward, bool parameters);
+
+}  // namespace groupnorm

@@ -1,0 +1,156 @@
+// Entry point and autograd of the group norm with an activation (groupnorm.cu).
+#include <torch/extension.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include "groupnorm.h"
+#include "lm_host.h"
+
+namespace py = pybind11;
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+int type_code(torch::ScalarType t) {
+  return t == torch::kFloat32 ? 0 : t == torch::kBFloat16 ? 1 : t == torch::kHalf ? 2 : -1;
+}
+
+bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// x [N, C, ...] as rows of channels [N, ..., C]: a view where it lies so in memory.
+torch::Tensor as_rows(const torch::Tensor& x) { return x.movedim(1, -1).contiguous(); }
+
+groupnorm::Shape shape_of(const torch::Tensor& rows, int64_t groups) {
+  groupnorm::Shape s{};
+  s.n = rows.size(0);
+  s.c = (int)rows.size(-1);
+  s.pixels = s.n ? rows.numel() / s.n / s.c : 0;
+  s.groups = (int)groups;
+  s.type = type_code(rows.scalar_type());
+  return s;
+}
+
+groupnorm::Affine affine_of(const torch::Tensor& w, const torch::Tensor& b) {
+  groupnorm::Affine a{};
+  if (w.defined()) {
+    a.w = w.data_ptr();
+    a.w_type = type_code(w.scalar_type());
+  }
+  if (b.defined()) {
+    a.b = b.data_ptr();
+    a.b_type = type_code(b.scalar_type());
+  }
+  return a;
+}
+
+torch::Tensor floats(int64_t n, const torch::Tensor& like) {
+  return torch::empty({n}, like.options().dtype(torch::kFloat32));
+}
+
+struct Forward {
+  torch::Tensor y, mean, rstd;   // y [N, ..., C]
+};
+
+// rows: contiguous [N, ..., C]; contiguous parameters or undefined ones.
+Forward forward(const torch::Tensor& rows, int64_t groups, const torch::Tensor& w, const torch::Tensor& b, double eps,
+                int act, bool keep) {
+  const c10::cuda::CUDAGuard guard(rows.device());
+  const auto s = shape_of(rows, groups);
+  Forward f;
+  f.y = torch::empty(rows.sizes(), rows.options());
+  if (keep) {
+    f.mean = floats(s.n * groups, rows);
+    f.rstd = floats(s.n * groups, rows);
+  }
+  if (rows.numel() == 0) return f;
+  const auto p = groupnorm::plan(s, false, aligned(rows.data_ptr()) && aligned(f.y.data_ptr()), lm::sm_count());
+  TORCH_CHECK(s.n * p.ctas <= INT32_MAX, "group_norm: too many samples for one launch");
+  torch::Tensor ws;
+  if (!p.resident) {
+    ws = floats(groupnorm::forward_workspace(s, p), rows);
+    if (!keep) {
+      f.mean = floats(s.n * groups, rows);
+      f.rstd = floats(s.n * groups, rows);
+    }
+  }
+  const cudaError_t e = groupnorm::forward(
+      s, p, rows.data_ptr(), affine_of(w, b), (float)eps, static_cast<groupnorm::Activation>(act), f.y.data_ptr(),
+      f.mean.defined() ? f.mean.data_ptr<float>() : nullptr, f.rstd.defined() ? f.rstd.data_ptr<float>() : nullptr,
+      ws.defined() ? ws.data_ptr<float>() : nullptr, c10::cuda::getCurrentCUDAStream().stream());
+  TORCH_CHECK(e == cudaSuccess, "group_norm forward launch failed");
+  lm::count_launches(groupnorm::launches(p, false, false));
+  return f;
+}
+
+struct GroupNormFn : torch::autograd::Function<GroupNormFn> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& x, const c10::optional<torch::Tensor>& weight,
+                               const c10::optional<torch::Tensor>& bias, int64_t groups, double eps, int64_t act) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const auto rows = as_rows(x);
+    const auto w = weight ? weight->contiguous() : torch::Tensor(), b = bias ? bias->contiguous() : torch::Tensor();
+    const Forward f = ::forward(rows, groups, w, b, eps, (int)act, true);
+    // x is saved as the caller's own tensor where it is read as it is, so that a change of it in place is noticed
+    ctx->save_for_backward({rows.is_alias_of(x) ? x : rows.movedim(-1, 1), w, b, f.mean, f.rstd});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    return f.y.movedim(-1, 1);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "group_norm has no second derivative (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const auto rows = as_rows(saved[0]);
+    const auto &w = saved[1], &b = saved[2];
+    const c10::cuda::CUDAGuard guard(rows.device());
+    const auto dy = as_rows(grads[0].to(rows.scalar_type()));
+    const auto s = shape_of(rows, ctx->saved_data["groups"].toInt());
+    auto dx = torch::empty(rows.sizes(), rows.options());
+    torch::Tensor dw, db;
+    if (w.defined() && ctx->needs_input_grad(1)) dw = rows.numel() ? torch::empty_like(w) : torch::zeros_like(w);
+    if (b.defined() && ctx->needs_input_grad(2)) db = rows.numel() ? torch::empty_like(b) : torch::zeros_like(b);
+    if (rows.numel()) {
+      const auto p = groupnorm::plan(
+          s, true, aligned(rows.data_ptr()) && aligned(dy.data_ptr()) && aligned(dx.data_ptr()), lm::sm_count());
+      TORCH_CHECK(s.n * p.ctas <= INT32_MAX, "group_norm: too many samples for one launch");
+      const auto ws = floats(groupnorm::backward_workspace(s, p), rows);
+      const cudaError_t e = groupnorm::backward(
+          s, p, dy.data_ptr(), rows.data_ptr(), affine_of(w, b), saved[3].data_ptr<float>(), saved[4].data_ptr<float>(),
+          static_cast<groupnorm::Activation>(ctx->saved_data["act"].toInt()), dx.data_ptr(),
+          dw.defined() ? dw.data_ptr() : nullptr, db.defined() ? db.data_ptr() : nullptr, ws.data_ptr<float>(),
+          c10::cuda::getCurrentCUDAStream().stream());
+      TORCH_CHECK(e == cudaSuccess, "group_norm backward launch failed");
+      lm::count_launches(groupnorm::launches(p, true, dw.defined() || db.defined()));
+    }
+    return {dx.movedim(-1, 1), dw, db, torch::Tensor(), torch::Tensor(), torch::Tensor()};
+  }
+};
+
+torch::Tensor group_norm(torch::Tensor x, int64_t groups, c10::optional<torch::Tensor> weight,
+                         c10::optional<torch::Tensor> bias, double eps, int64_t act) {
+  LM_CHECK_VALUE(x.is_cuda() && x.dim() >= 2 && type_code(x.scalar_type()) >= 0,
+                 "group_norm takes fp32, bf16 or fp16 tensors [N, C, ...]");
+  const int64_t c = x.size(1);
+  LM_CHECK_VALUE(c >= 1 && c <= 8192, "group_norm takes 1 to 8192 channels, not ", c);
+  LM_CHECK_VALUE(groups >= 1 && c % groups == 0, "group_norm: ", c, " channels do not make ", groups, " groups");
+  for (const auto* p : {&weight, &bias})
+    LM_CHECK_VALUE(!*p || ((*p)->dim() == 1 && (*p)->size(0) == c && type_code((*p)->scalar_type()) >= 0 &&
+                           (*p)->device() == x.device()),
+                   "group_norm needs fp32, bf16 or fp16 parameters [", c, "] on ", x.device());
+  LM_CHECK_VALUE(act >= 0 && act <= 3, "group_norm: unknown activation");
+  LM_CHECK_NO_TANGENT("group_norm", x, weight, bias);
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad())))
+    return GroupNormFn::apply(x, weight, bias, groups, eps, act);
+  const Forward f = forward(as_rows(x), groups, weight ? weight->contiguous() : torch::Tensor(),
+                            bias ? bias->contiguous() : torch::Tensor(), eps, (int)act, false);
+  return f.y.movedim(-1, 1);
+}
+
+}  // namespace
+
+void register_groupnorm_ops(py::module& m) {
+  m.def("group_norm", &group_norm, "group norm with an activation over channels-last memory, with autograd", py::arg("x"),
+        py::arg("groups"), py::arg("weight"), py::arg("bias"), py::arg("eps"), py::arg("activation"));
+}

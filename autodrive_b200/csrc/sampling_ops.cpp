@@ -1,0 +1,111 @@
+// Entry point of sampling from rows of logits (sampling.cu).
+#include <torch/extension.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include "lm_host.h"
+#include "sampling.h"
+
+namespace py = pybind11;
+
+namespace {
+
+int type_code(torch::ScalarType t) {
+  return t == torch::kFloat32 ? 0 : t == torch::kBFloat16 ? 1 : t == torch::kHalf ? 2 : -1;
+}
+
+// A parameter that is a number or a tensor of the rows' leading dimensions; `keep` holds what was laid out anew.
+bool is_tensor(const py::object& o) { return THPVariable_Check(o.ptr()); }
+
+torch::Tensor each_row(const py::object& o, c10::IntArrayRef lead, const torch::Tensor& logits, const char* name) {
+  const auto t = o.cast<torch::Tensor>();
+  LM_CHECK_VALUE(t.sizes() == lead && t.device() == logits.device(), "sample_tokens needs ", name, " as a number or ", lead,
+                 " on ", logits.device());
+  return t.contiguous();
+}
+
+sampling::Real real(const py::object& o, c10::IntArrayRef lead, const torch::Tensor& logits, const char* name, double least,
+                    double most, std::vector<torch::Tensor>& keep) {
+  sampling::Real r{};
+  if (is_tensor(o)) {
+    keep.push_back(each_row(o, lead, logits, name));
+    LM_CHECK_VALUE(keep.back().scalar_type() == torch::kFloat32, "sample_tokens needs ", name, " in fp32");
+    r.each = keep.back().data_ptr<float>();
+  } else {
+    r.all = o.cast<double>();
+    LM_CHECK_VALUE(r.all >= least && r.all <= most, "sample_tokens: ", name, " must be in ", least, "..", most, ", not ", r.all);
+  }
+  return r;
+}
+
+py::tuple sample_tokens(torch::Tensor logits, torch::Tensor uniforms, c10::optional<torch::Tensor> mask,
+                        py::object temperature, py::object top_k, py::object top_p, py::object min_p) {
+  LM_CHECK_VALUE(logits.is_cuda() && logits.dim() >= 1 && type_code(logits.scalar_type()) >= 0 && logits.size(-1) >= 1,
+                 "sample_tokens takes fp32, bf16 or fp16 logits [..., V]");
+  const int64_t v = logits.size(-1);
+  LM_CHECK_VALUE(v <= INT32_MAX, "sample_tokens: rows of at most 2^31 - 1 entries, not ", v);
+  const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+  LM_CHECK_VALUE(uniforms.sizes() == lead && uniforms.device() == logits.device() &&
+                     (uniforms.scalar_type() == torch::kFloat32 || uniforms.scalar_type() == torch::kFloat64),
+                 "sample_tokens needs fp32 or fp64 uniform numbers ", lead, " on ", logits.device());
+  std::vector<torch::Tensor> keep;
+  keep.reserve(8);
+  sampling::Args a{};
+  a.temperature = real(temperature, lead, logits, "temperature", 0., 1e30, keep);
+  LM_CHECK_VALUE(a.temperature.each || a.temperature.all == 0. || a.temperature.all >= 1e-30,
+                 "sample_tokens: the temperature must be 0 or in 1e-30..1e30, not ", a.temperature.all);
+  a.top_p = real(top_p, lead, logits, "top_p", 0., 1., keep);
+  a.min_p = real(min_p, lead, logits, "min_p", 0., 1., keep);
+  if (is_tensor(top_k)) {
+    keep.push_back(each_row(top_k, lead, logits, "top_k"));
+    const auto& t = keep.back();
+    LM_CHECK_VALUE(t.scalar_type() == torch::kInt64 || t.scalar_type() == torch::kInt32,
+                   "sample_tokens needs top_k in int64 or int32");
+    a.top_k.each = t.data_ptr();
+    a.top_k.bytes = (int)t.element_size();
+  } else {
+    a.top_k.all = top_k.cast<int64_t>();
+    LM_CHECK_VALUE(a.top_k.all >= 0, "sample_tokens: top_k must not be negative, not ", a.top_k.all);
+  }
+  const c10::cuda::CUDAGuard guard(logits.device());
+  auto x = logits.dim() == 2 ? logits : logits.reshape({lead.empty() ? 1 : c10::multiply_integers(lead), v});
+  if ((v > 1 && x.stride(1) != 1) || (x.size(0) > 1 && x.stride(0) < 0)) x = x.contiguous();
+  a.rows = x.size(0);
+  a.v = v;
+  a.ld = a.rows > 1 ? x.stride(0) : v;
+  a.logits = x.data_ptr();
+  a.type = type_code(x.scalar_type());
+  keep.push_back(uniforms.contiguous());
+  a.uniforms = keep.back().data_ptr();
+  a.u_double = uniforms.scalar_type() == torch::kFloat64;
+  if (mask) {
+    LM_CHECK_VALUE(mask->scalar_type() == torch::kBool && mask->device() == logits.device(),
+                   "the mask must be boolean (true: valid) on the logits' device");
+    LM_CHECK_VALUE(mask->dim() <= logits.dim() && at::is_expandable_to(mask->sizes(), logits.sizes()), "the mask ",
+                   mask->sizes(), " does not broadcast to ", logits.sizes());
+    auto m = mask->expand(logits.sizes());
+    if (m.dim() != 2) m = m.reshape({a.rows, v});
+    keep.push_back(m);
+    a.mask = reinterpret_cast<const uint8_t*>(m.data_ptr());
+    a.mask_row = m.stride(0);
+    a.mask_col = m.stride(1);
+  }
+  auto token = torch::empty(lead, logits.options().dtype(torch::kInt64));
+  auto log_prob = torch::empty(lead, logits.options().dtype(torch::kFloat32));
+  if (a.rows == 0) return py::make_tuple(token, log_prob);
+  LM_CHECK_VALUE(a.rows <= INT32_MAX, "sample_tokens: at most 2^31 - 1 rows, not ", a.rows);
+  a.token = token.data_ptr<int64_t>();
+  a.log_prob = log_prob.data_ptr<float>();
+  TORCH_CHECK(sampling::launch(a, lm::sm_count(), c10::cuda::getCurrentCUDAStream().stream()) == cudaSuccess,
+              "sample_tokens launch failed");
+  lm::count_launches(1);
+  return py::make_tuple(token, log_prob);
+}
+
+}  // namespace
+
+void register_sampling_ops(py::module& m) {
+  m.def("sample_tokens", &sample_tokens, "sampling with temperature, top-k, top-p and min-p from given uniform numbers",
+        py::arg("logits"), py::arg("uniforms"), py::arg("mask"), py::arg("temperature"), py::arg("top_k"),
+        py::arg("top_p"), py::arg("min_p"));
+}

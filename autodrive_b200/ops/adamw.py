@@ -1,0 +1,204 @@
+"""AdamW over a list of tensors at once, with the moments in fp32 or in 8 bits,
+on fused sm_100a kernels (``csrc/adamw.cu``).
+
+``adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None,
+exp_avg_sq_scales=None, *, step, lr, betas, eps, weight_decay, max_grad_norm,
+seed)`` updates parameters (fp32, bf16 or fp16, dense, of any shape and number)
+and their moments in place:
+
+    g = grad * min(1, max_grad_norm / (norm + 1e-6))    max_grad_norm > 0; norm over all gradients
+    m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2
+    p = p (1 - lr weight_decay) - lr / (1 - b1^step) m / (sqrt(v / (1 - b2^step)) + eps)
+
+* It returns the gradients' norm (fp32, on the device) where they are clipped,
+  otherwise None. Computation is fp32 (the norm's sum fp64); a 16-bit parameter
+  is rounded once, a NaN or infinite norm makes all parameters NaN.
+* Moments without scales are fp32 of their parameter's shape and strides. With
+  scales they are e4m3 numbers of that shape, one fp32 scale for each 256
+  elements (in memory order): m, and the root of v in `exp_avg_sqs`. Their
+  rounding up or down is decided by 16 bits mixed from (seed, step, element), so
+  that moments which move by less than their spacing move on average; the same
+  call gives the same numbers. A root that is not zero never becomes zero. A
+  block of 256 whose new moments hold a NaN or an infinity becomes NaN.
+  ``moments_8bit(p)`` makes such moments, all zero.
+* `step` counts from 1: a number, a list of one for each parameter, or one int64
+  on the device, which is read when the kernel runs. Only the last may be
+  captured into a CUDA graph; it belongs to the caller, who counts it up.
+* Parameters must not share memory, and no moment may share any.
+
+``train.optim.FusedAdamW`` is the optimizer. On CPU the same is computed in plain
+PyTorch.
+"""
+from __future__ import annotations
+
+import math
+from collections.abc import Sequence
+
+import torch
+from torch import Tensor
+
+from .ext import require_extension
+
+BLOCK = 256
+E4M3 = torch.float8_e4m3fn
+E4M3_MAX = 448.
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_MASK = 0xffffffff
+
+
+def moments_8bit(p: Tensor) -> tuple[Tensor, Tensor]:
+    """(e4m3 zeros laid out as `p`, their scales), for one moment of `p`."""
+    codes = torch.empty_like(p, dtype=torch.uint8).zero_().view(E4M3)
+    return codes, torch.zeros(-(-p.numel() // BLOCK), device=p.device)
+
+
+def _mix(x):
+    """32 mixed bits of 32 (held in 64)."""
+    x = ((x ^ (x >> 16)) * 0x7feb352d) & _MASK
+    x = ((x ^ (x >> 15)) * 0x846ca68b) & _MASK
+    return x ^ (x >> 16)
+
+
+def _in_memory_order(t: Tensor) -> Tensor:
+    """The elements of a dense tensor as they lie in memory (a view)."""
+    return t.as_strided((t.numel(),), (1,))
+
+
+def dequantize_moment(codes: Tensor, scale: Tensor) -> Tensor:
+    """The fp32 values of an 8-bit moment (of the root, for `exp_avg_sqs`), laid out as its codes."""
+    y = torch.empty_like(codes, dtype=torch.float32)
+    _in_memory_order(y).copy_(_in_memory_order(codes).float() * scale.repeat_interleave(BLOCK)[:codes.numel()])
+    return y
+
+
+def _quantize(t: Tensor, bits: Tensor, root: bool) -> tuple[Tensor, Tensor]:
+    """(e4m3 numbers as fp32, scales) of a flat moment and its elements' 16 random bits."""
+    n = t.numel()
+    padded = torch.nn.functional.pad(t, (0, -n % BLOCK)).view(-1, BLOCK)
+    amax = padded.abs().amax(-1)
+    amax = torch.where(padded.isnan().any(-1), torch.nan, amax)
+    scale = torch.where(amax.isfinite(), (amax.double().clamp_min(E4M3_MAX * 2. ** -126) / E4M3_MAX).float(), amax)
+    q = (padded.abs() / scale[:, None]).view(-1)[:n]
+    off = torch.where(q < 2. ** -6, 2. ** -6, 0.)
+    code = (((q + off).view(torch.int32) + (bits << 4)) & ~0xfffff).view(torch.float32) - off
+    code = code.clamp(max=E4M3_MAX)
+    if root:
+        code = torch.where((t > 0) & (code == 0), 2. ** -9, code)
+    code = torch.where(t < 0, -code, code)
+    return torch.where(scale.isfinite().repeat_interleave(BLOCK)[:n], code, torch.nan), scale
+
+
+def reference_adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, steps, lr, betas, eps,
+                         weight_decay, max_grad_norm, seed) -> Tensor | None:
+    """The same operation in plain PyTorch (CPU path and test oracle); `steps`: one for each parameter."""
+    b1, b2 = betas
+    norm, factor = None, 1.
+    if max_grad_norm > 0:
+        norm = torch.stack([g.double().square().sum() for g in grads]).sum().sqrt()
+        factor = (max_grad_norm / (norm + 1e-6)).clamp(max=1.).float()
+    first = 0
+    for i, (p, g) in enumerate(zip(params, grads)):
+        n = p.numel()
+        if n == 0:
+            continue
+        if g.stride() != p.stride():
+            g = torch.empty_like(p, dtype=g.dtype).copy_(g)
+        fp, fg = _in_memory_order(p), _in_memory_order(g).float() * factor
+        fm, fv = _in_memory_order(exp_avgs[i]), _in_memory_order(exp_avg_sqs[i])
+        if exp_avg_scales is None:
+            m, v = fm, fv
+        else:
+            m = fm.float() * exp_avg_scales[i].repeat_interleave(BLOCK)[:n]
+            v = (fv.float() * exp_avg_sq_scales[i].repeat_interleave(BLOCK)[:n]).square()
+        m = b1 * m + (1 - b1) * fg
+        v = b2 * v + (1 - b2) * fg * fg
+        root = v.sqrt()
+        step = steps[i]
+        fp.copy_(fp.float() * (1 - lr * weight_decay)
+                 - (lr / (1 - b1 ** step)) * (m / (root * (1 / math.sqrt(1 - b2 ** step)) + eps)))
+        if exp_avg_scales is None:
+            fm.copy_(m)
+            fv.copy_(v)
+        else:
+            at = torch.arange(first * BLOCK, first * BLOCK + n, device=p.device)
+            h = _mix((at + _mix(_mix(seed & _MASK) ^ (step & _MASK))) & _MASK).to(torch.int32)
+            for codes, scales, t, bits, is_root in ((fm, exp_avg_scales[i], m, h & 0xffff, False),
+                                                    (fv, exp_avg_sq_scales[i], root, (h >> 16) & 0xffff, True)):
+                q, scale = _quantize(t, bits, is_root)
+                codes.copy_(q)
+                scales.copy_(scale)
+        first += -(-n // BLOCK)
+    return None if norm is None else norm.float()
+
+
+def _dense(t: Tensor) -> bool:
+    """Whether the elements of `t` fill one stretch of memory."""
+    expect = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _check(params, grads, ms, vs, m_scales, v_scales) -> None:
+    device, kind = params[0].device, torch.float32 if m_scales is None else E4M3
+    spans = []
+    for i, (p, g, m, v) in enumerate(zip(params, grads, ms, vs)):
+        if p.dtype not in DTYPES or g.dtype not in DTYPES:
+            raise ValueError("adamw_step takes fp32, bf16 or fp16 parameters and gradients")
+        if m.dtype != kind or v.dtype != kind:
+            raise ValueError("adamw_step takes moments in fp32, or in e4m3 with scales")
+        if any(t.device != device for t in (p, g, m, v)):
+            raise ValueError("adamw_step needs all of its tensors on one device")
+        if g.shape != p.shape:
+            raise ValueError(f"adamw_step: gradient {tuple(g.shape)} of a parameter {tuple(p.shape)}")
+        if g.layout != torch.strided or not _dense(p):
+            raise ValueError("adamw_step needs dense parameters without gaps")
+        if any(t.shape != p.shape or (p.numel() > 1 and t.stride() != p.stride()) for t in (m, v)):
+            raise ValueError(f"adamw_step needs moments of their parameter's shape and strides {tuple(p.shape)}")
+        if m_scales is not None:
+            nb = -(-p.numel() // BLOCK)
+            if any(s.dtype != torch.float32 or s.device != device or s.shape != (nb,) or not s.is_contiguous()
+                   for s in (m_scales[i], v_scales[i])):
+                raise ValueError(f"adamw_step needs {nb} fp32 scales of 256 elements each for a parameter {tuple(p.shape)}")
+        if p.numel():
+            spans.append((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()))
+    spans.sort()
+    if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        raise ValueError("adamw_step: two parameters share memory")
+
+
+@torch.no_grad()
+def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
+               exp_avg_sqs: Sequence[Tensor], exp_avg_scales: Sequence[Tensor] | None = None,
+               exp_avg_sq_scales: Sequence[Tensor] | None = None, *, step: int | Sequence[int] | Tensor, lr: float,
+               betas: tuple[float, float] = (.9, .999), eps: float = 1e-8, weight_decay: float = .01,
+               max_grad_norm: float = 0., seed: int = 0) -> Tensor | None:
+    """One AdamW step of all `params` in place (see the module docstring)."""
+    b1, b2 = betas
+    if not (0. <= b1 < 1. and 0. <= b2 < 1.):
+        raise ValueError(f"adamw_step needs betas in [0, 1), not {betas}")
+    if not (lr >= 0. and eps >= 0. and weight_decay >= 0. and max_grad_norm >= 0.):
+        raise ValueError("adamw_step needs lr, eps, weight_decay and max_grad_norm of at least 0")
+    if len(params) and params[0].is_cuda:
+        return require_extension().adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales,
+                                              step, lr, b1, b2, eps, weight_decay, max_grad_norm, seed & _MASK)
+    lists = [grads, exp_avgs, exp_avg_sqs] + ([exp_avg_scales, exp_avg_sq_scales] if exp_avg_scales is not None else [])
+    if (exp_avg_scales is None) != (exp_avg_sq_scales is None) or any(len(x) != len(params) for x in lists):
+        raise ValueError("adamw_step needs a gradient and two moments (8-bit ones with their scales) for each of "
+                         f"{len(params)} parameters")
+    if not len(params):
+        return None
+    _check(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales)
+    if isinstance(step, Tensor):
+        if step.dtype != torch.int64 or step.numel() != 1 or step.device != params[0].device:
+            raise ValueError(f"adamw_step needs its step as a number, a list of numbers or one int64 on {params[0].device}")
+        step = int(step)
+    steps = [step] * len(params) if isinstance(step, int) else list(step)
+    if len(steps) != len(params):
+        raise ValueError(f"adamw_step needs one step for all or for each of {len(params)} parameters")
+    if any(not 1 <= s < 2 ** 32 for s in steps):
+        raise ValueError("adamw_step counts its steps from 1")
+    return reference_adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, steps, lr, betas,
+                                eps, weight_decay, max_grad_norm, seed)

@@ -1,0 +1,142 @@
+"""Group norm with an activation over channels-last memory, forward and
+backward, on fused sm_100a kernels (``csrc/groupnorm.cu``).
+
+``group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None)``
+normalises each sample's groups of channels of `x` [N, C, ...] (fp32, bf16 or
+fp16; at most 8192 channels) and applies the activation (``"silu"``, ``"relu"``,
+``"gelu"`` (by the error function) or none), with autograd. Statistics and sums
+are fp32. The result lies in channels-last memory ([N, ..., C], what PyTorch's
+``channels_last`` formats mean); an `x` in other memory is copied there first.
+
+``FusedGroupNorm`` is a drop-in ``nn.GroupNorm`` with an activation, and
+``fuse_group_norms(module)`` puts it in the place of the group norms of a module
+and of the activations that follow them. On CPU all of them are plain PyTorch.
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor, nn
+from torch.nn import functional as F
+
+from .ext import require_extension
+
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+MAX_CHANNELS = 8192
+ACTIVATIONS = (None, "silu", "relu", "gelu")
+_ACT = {"silu": F.silu, "relu": F.relu, "gelu": F.gelu}
+
+
+def _code(activation: str | None) -> int:
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"group_norm knows the activations {ACTIVATIONS}, not {activation!r}")
+    return ACTIVATIONS.index(activation)
+
+
+def reference_group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tensor | None = None,
+                         eps: float = 1e-5, activation: str | None = None) -> Tensor:
+    """The same operation in plain PyTorch, in fp32, with autograd (CPU path)."""
+    y = F.group_norm(x.float(), groups, None if weight is None else weight.float(), None if bias is None else bias.float(),
+                     eps)
+    return (y if activation is None else _ACT[activation](y)).to(x.dtype)
+
+
+def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5,
+               activation: str | None = None) -> Tensor:
+    """Group norm of `x` [N, C, ...] followed by the activation (see the module docstring)."""
+    act = _code(activation)
+    if x.is_cuda:
+        return require_extension().group_norm(x, groups, weight, bias, eps, act)
+    if x.dim() < 2 or x.dtype not in DTYPES:
+        raise ValueError("group_norm takes fp32, bf16 or fp16 tensors [N, C, ...]")
+    c = x.shape[1]
+    if not 1 <= c <= MAX_CHANNELS:
+        raise ValueError(f"group_norm takes 1 to {MAX_CHANNELS} channels, not {c}")
+    if groups < 1 or c % groups:
+        raise ValueError(f"group_norm: {c} channels do not make {groups} groups")
+    for p in (weight, bias):
+        if p is not None and (p.shape != (c,) or p.dtype not in DTYPES or p.device != x.device):
+            raise ValueError(f"group_norm needs fp32, bf16 or fp16 parameters [{c}] on {x.device}")
+    if x.numel() == 0:
+        return x.clone()
+    rows = x.movedim(1, -1).contiguous().movedim(-1, 1)   # lies as the result on a GPU does
+    y = reference_group_norm(rows if rows.dim() > 2 else rows[..., None], groups, weight, bias, eps, activation)
+    return (y if rows.dim() > 2 else y[..., 0]).movedim(1, -1).contiguous().movedim(-1, 1)
+
+
+class FusedGroupNorm(nn.GroupNorm):
+    """``nn.GroupNorm`` (same parameters and state-dict keys) followed by an activation, on the fused kernels."""
+
+    def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True,
+                 activation: str | None = None, device=None, dtype=None):
+        super().__init__(num_groups, num_channels, eps=eps, affine=affine, device=device, dtype=dtype)
+        _code(activation)
+        self.activation = activation
+
+    def forward(self, x: Tensor) -> Tensor:
+        return group_norm(x, self.num_groups, self.weight, self.bias, self.eps, self.activation)
+
+    def extra_repr(self) -> str:
+        return super().extra_repr() + f", activation={self.activation}"
+
+
+def _activation_of(module: nn.Module) -> str | None:
+    if type(module) is nn.SiLU:
+        return "silu"
+    if type(module) is nn.ReLU:
+        return "relu"
+    if type(module) is nn.GELU and module.approximate == "none":
+        return "gelu"
+    return None
+
+
+def _bare(module: nn.Module) -> bool:
+    return not (module._forward_hooks or module._forward_pre_hooks)
+
+
+def fuse_group_norms(module: nn.Module) -> nn.Module:
+    """Put a FusedGroupNorm, with the same parameters, in the place of every plain nn.GroupNorm of `module`
+    (recursively), in place. In an nn.Sequential the SiLU, ReLU or GELU behind a norm becomes its activation, with an
+    nn.Identity left in its place, so that the state dict keeps its keys; an activation that stands in several places
+    or has hooks stays, and so does a norm with hooks or of more than 8192 channels. The module's convolutions run best on
+    channels-last weights: ``module.to(memory_format=torch.channels_last)``. Returns the module, or the fused norm where
+    the module itself is a norm."""
+    return _fuse(module, {}, _places(module, {}))
+
+
+def _places(module: nn.Module, seen: dict) -> dict:
+    """How often each module stands in the tree."""
+    seen[module] = seen.get(module, 0) + 1
+    if seen[module] == 1:
+        for child in module.children():
+            _places(child, seen)
+        for child in module._modules.values():   # children() tells each once
+            if child is not None and list(module._modules.values()).count(child) > 1:
+                seen[child] += 1
+    return seen
+
+
+def _fuse(module: nn.Module, done: dict, places: dict) -> nn.Module:
+    if module in done:
+        return done[module]
+    done[module] = module
+    if type(module) is nn.GroupNorm:
+        if _bare(module) and module.num_channels <= MAX_CHANNELS:
+            fused = done[module] = FusedGroupNorm(module.num_groups, module.num_channels, module.eps, False)
+            fused.affine, fused.training = module.affine, module.training
+            fused.weight, fused.bias = module.weight, module.bias
+        return done[module]
+    names = list(module._modules)
+    for at, name in enumerate(names):
+        child = module._modules[name]
+        if child is None:
+            continue
+        fused = _fuse(child, done, places)
+        if fused is not child:
+            setattr(module, name, fused)
+            if type(module) is nn.Sequential and at + 1 < len(names) and places[child] == 1:
+                follower = module._modules[names[at + 1]]
+                act = None if follower is None else _activation_of(follower)
+                if act and _bare(follower) and places[follower] == 1:
+                    fused.activation = act
+                    setattr(module, names[at + 1], nn.Identity())
+    return done[module]

@@ -1,0 +1,121 @@
+"""Sampling of tokens (or actions) from rows of logits with temperature, top-k,
+top-p and min-p, by given uniform numbers, on fused sm_100a kernels
+(``csrc/sampling.cu``).
+
+``sample_tokens(logits, uniforms, mask=None, temperature=1., top_k=0, top_p=1.,
+min_p=0.)`` takes logits [..., V] (fp32, bf16 or fp16), one number of [0, 1) for
+each row (fp32 or fp64 [...]) and an optional boolean mask of the valid entries
+that broadcasts against the logits, and returns ``SampledTokens(token,
+log_prob)``, int64 and fp32 [...], without gradient (``ops.token_logprobs``
+scores tokens with one):
+
+* entries weigh w = exp((logit - largest) / temperature); masked ones are not
+  read, whatever they hold;
+* those with w < ``min_p`` are cut off; of the rest the first ``top_k`` by
+  their logits stay (0: all), equal ones by their index; of these the fewest,
+  in the same order, whose weights come to ``top_p`` of theirs, and always one;
+* the token is the first entry that stays, by index, at which the running sum
+  of the staying weights exceeds the row's number times their sum (a number of
+  1 or more takes the last, a negative one the first), and ``log_prob`` the
+  logarithm of its share of that sum;
+* a temperature of 0 takes the first of the largest entries;
+* a row without a valid entry above -inf gives token -1 and -inf; a NaN or
+  +inf among its valid entries, or a number or parameter that is NaN or out of
+  range, gives -1 and NaN.
+
+Each of the four parameters is a number for all rows or a tensor [...] (fp32;
+``top_k`` int64 or int32) with one for each. Weights and sums are fp64; on CUDA
+entries further than 44 temperatures below the largest count as zero. On CPU
+the same is computed in plain PyTorch.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+from torch import Tensor
+
+from .ext import require_extension
+
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class SampledTokens(NamedTuple):
+    token: Tensor
+    log_prob: Tensor
+
+
+def reference_sample_tokens(logits: Tensor, uniforms: Tensor, mask: Tensor | None, temperature: Tensor, top_k: Tensor,
+                            top_p: Tensor, min_p: Tensor) -> SampledTokens:
+    """The same operation on rows [R, V] in plain PyTorch (CPU path and test oracle); uniforms and parameters [R]."""
+    v = logits.shape[-1]
+    z = logits.float()
+    if mask is not None:
+        z = torch.where(mask, z, -torch.inf)
+    u, t, p, least = (x.double()[:, None] for x in (uniforms, temperature, top_p, min_p))
+    k = top_k.long()[:, None]
+    bad = ~((t == 0) | ((t >= 1e-30) & (t <= 1e30))) | p.isnan() | u.isnan() | ~(least <= 1) | (k < 0)
+    bad |= (z.isnan() | (z == torch.inf)).any(-1, keepdim=True)
+    z = torch.where(bad, 0., z)
+    top = z.amax(-1, keepdim=True)
+    empty = top == -torch.inf
+    top = torch.where(empty, 0., top)
+    greedy = t == 0
+    scaled = (z.double() - top) / torch.where(greedy, 1., t)
+    w = torch.where(greedy, (z == top).double(), scaled.exp())
+    w = torch.where(w >= least, w, 0.)
+    _, index = torch.sort(z, dim=-1, descending=True, stable=True)
+    ordered = w.gather(1, index)
+    rank = torch.arange(v, device=z.device)
+    k = torch.where(greedy, 1, k)
+    ordered = torch.where((k == 0) | (rank < k), ordered, 0.)
+    before = ordered.cumsum(-1)
+    before, target = torch.nn.functional.pad(before[:, :-1], (1, 0)), p * before[:, -1:]
+    ordered = torch.where((p >= 1) | (rank == 0) | (before < target), ordered, 0.)
+    w = torch.zeros_like(w).scatter_(1, index, ordered)
+    running = w.cumsum(-1)
+    total = running[:, -1:]
+    token = (running <= u * total).sum(-1, keepdim=True)
+    token = torch.minimum(token, (running < total).sum(-1, keepdim=True)).clamp(max=v - 1)
+    log_prob = torch.where(greedy, 0., scaled.gather(1, token)) - total.log()
+    log_prob = torch.where(bad, torch.nan, torch.where(empty, -torch.inf, log_prob))
+    return SampledTokens(torch.where(bad | empty, -1, token)[:, 0], log_prob[:, 0].float())
+
+
+def _each(value, lead, name, dtypes, least, most, device) -> Tensor:
+    if isinstance(value, Tensor):
+        if value.shape != lead or value.device != device or value.dtype not in dtypes:
+            raise ValueError(f"sample_tokens needs {name} as a number or {tuple(lead)} of {dtypes[0]} on {device}")
+        return value.reshape(-1)
+    if not least <= value <= most:
+        raise ValueError(f"sample_tokens: {name} must be in {least}..{most}, not {value}")
+    kind = torch.int64 if dtypes[0] == torch.int64 else torch.float64
+    return torch.full((lead.numel(),), value, dtype=kind, device=device)
+
+
+def sample_tokens(logits: Tensor, uniforms: Tensor, mask: Tensor | None = None, temperature: float | Tensor = 1.,
+                  top_k: int | Tensor = 0, top_p: float | Tensor = 1., min_p: float | Tensor = 0.) -> SampledTokens:
+    """One token of each row of `logits` by its uniform number (see the module docstring)."""
+    if logits.is_cuda:
+        return SampledTokens._make(require_extension().sample_tokens(logits, uniforms, mask, temperature, top_k, top_p,
+                                                                     min_p))
+    if logits.dim() < 1 or logits.shape[-1] < 1 or logits.dtype not in DTYPES:
+        raise ValueError("sample_tokens takes fp32, bf16 or fp16 logits [..., V]")
+    lead, v = logits.shape[:-1], logits.shape[-1]
+    if uniforms.shape != lead or uniforms.dtype not in (torch.float32, torch.float64) or uniforms.device != logits.device:
+        raise ValueError(f"sample_tokens needs fp32 or fp64 uniform numbers {tuple(lead)} on {logits.device}")
+    reals, wholes = (torch.float32,), (torch.int64, torch.int32)
+    t = _each(temperature, lead, "temperature", reals, 0., 1e30, logits.device)
+    if not isinstance(temperature, Tensor) and 0 < temperature < 1e-30:
+        raise ValueError(f"sample_tokens: the temperature must be 0 or in 1e-30..1e30, not {temperature}")
+    k = _each(top_k, lead, "top_k", wholes, 0, 2 ** 63 - 1, logits.device)
+    p, least = (_each(value, lead, name, reals, 0., 1., logits.device) for value, name in ((top_p, "top_p"), (min_p, "min_p")))
+    if mask is not None:
+        if mask.dtype != torch.bool or mask.device != logits.device:
+            raise ValueError("the mask must be boolean (true: valid) on the logits' device")
+        try:
+            mask = mask.expand(logits.shape).reshape(-1, v)
+        except RuntimeError as exc:
+            raise ValueError(f"the mask {tuple(mask.shape)} does not broadcast to {tuple(logits.shape)}") from exc
+    token, log_prob = reference_sample_tokens(logits.detach().reshape(-1, v), uniforms.reshape(-1), mask, t, k, p, least)
+    return SampledTokens(token.view(lead), log_prob.view(lead))
