@@ -13,10 +13,15 @@
 // fp64 (the device has half as many fp64 units as fp32 ones), added in an order
 // that the sizes alone give. Entries further than 44 T below the largest (they
 // hold less than 10^-13 of any row's sum) count as zero.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "lm_vec.h"
 #include "sampling.h"
+
+namespace cg = cooperative_groups;
 
 namespace sampling {
 namespace {
@@ -53,10 +58,33 @@ struct Row {
   }
 };
 
+// e^x for -64 <= x <= 0 to about 2^-47: x = k ln 2 + r, and e^r by its series
+// to r^11 (|r| <= ln 2 / 2).
+__device__ __forceinline__ double exp_of(double x) {
+  const double shift = 6755399441055744.;   // 1.5 * 2^52: adding it rounds to a whole number in the low word
+  const double t = fma(x, 1.4426950408889634, shift);
+  const int k = __double2loint(t);
+  const double r = fma(t - shift, -0.69314718055994531, x);
+  double p = 1. / 39916800.;
+  p = fma(p, r, 1. / 3628800.);
+  p = fma(p, r, 1. / 362880.);
+  p = fma(p, r, 1. / 40320.);
+  p = fma(p, r, 1. / 5040.);
+  p = fma(p, r, 1. / 720.);
+  p = fma(p, r, 1. / 120.);
+  p = fma(p, r, 1. / 24.);
+  p = fma(p, r, 1. / 6.);
+  p = fma(p, r, .5);
+  p = fma(p, r, 1.);
+  p = fma(p, r, 1.);
+  return __hiloint2double(__double2hiint(p) + (k << 20), __double2loint(p));
+}
+
 // Weights relative to the row's largest logit.
 struct Weights {
   double top, inv;        // 1 / T
   float top32, inv32, far;
+  float scale, sure;       // bins a logit (see RowOf); places below this one stay without a further look
   double least;
   __device__ __forceinline__ void set(float m, const Row& r) {
     top = m;
@@ -65,26 +93,33 @@ struct Weights {
     inv32 = (float)inv;
     least = r.min_p;
     far = least > 0. ? fminf(kRange, -(float)log(least)) : kRange;
+    if (r.t == 0.) far = -1.f;
+    scale = sure = 0.f;
   }
-  __device__ __forceinline__ double of(float l) const { return exp(((double)l - top) * inv); }
+  __device__ __forceinline__ void set_bins(int bins) {
+    if (far > 0.f) scale = (float)bins / far * inv32;
+    sure = (float)bins * (far - 1e-3f) / far;
+    if (!(far > 2e-3f)) sure = -1.f;
+  }
+  __device__ __forceinline__ float place(float l) const { return __fmul_rn(__fsub_rn(top32, l), scale); }
+  __device__ __forceinline__ double of(float l) const { return exp_of(((double)l - top) * inv); }
   // Whether an entry stays before the cut-offs by order: told in fp32 but next to the border.
   __device__ __forceinline__ bool in(float l) const {
-    const float d = (top32 - l) * inv32;
-    if (!(d <= far + 1e-3f)) return false;
+    if (place(l) < sure) return true;
+    const float d = __fmul_rn(__fsub_rn(top32, l), inv32);
+    if (!(d <= far + 1e-3f)) return far < 0.f && l == top32;   // a temperature of 0: the largest entries alone
     if (d < far - 1e-3f) return true;
-    return least > 0. && far < kRange ? of(l) >= least : d <= far;
+    return far < kRange ? of(l) >= least : d <= far;
   }
 };
-
-template <typename T>
-__device__ __forceinline__ float logit(const Args& a, int64_t row, int64_t i) {
-  if (a.mask && !a.mask[row * a.mask_row + i * a.mask_col]) return -INFINITY;
-  return lm::to_f<T>(static_cast<const T*>(a.logits)[row * a.ld + i]);
-}
 
 __device__ __forceinline__ void answer(const Args& a, int64_t row, int64_t token, float log_prob) {
   a.token[row] = token;
   a.log_prob[row] = log_prob;
+}
+// Of a row that has no answer: `bad` if a value or a parameter is to blame.
+__device__ __forceinline__ void no_answer(const Args& a, int64_t row, bool bad) {
+  answer(a, row, -1, bad ? __uint_as_float(0x7fc00000u) : -INFINITY);
 }
 
 __device__ __forceinline__ double warp_sum(double s) {
@@ -92,172 +127,933 @@ __device__ __forceinline__ double warp_sum(double s) {
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
-__device__ __forceinline__ double block_sum(double s, double* red) {
-  s = warp_sum(s);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-  __syncthreads();
-  s = 0.;
-  for (int w = 0; w < (int)blockDim.x / 32; ++w) s += red[w];
-  return s;
+
+template <typename T>
+__device__ __forceinline__ float logit(const Args& a, int64_t row, int64_t i) {
+  if (a.mask && !a.mask[row * a.mask_row + i * a.mask_col]) return -INFINITY;
+  return lm::to_f<T>(static_cast<const T*>(a.logits)[row * a.ld + i]);
 }
 
-// A CTA for a row.
-template <typename T>
-__global__ void __launch_bounds__(1024) row_kernel(const __grid_constant__ Args a) {
-  __shared__ double red[32];
-  __shared__ double parts[1024];
-  __shared__ int ties[1024];
-  __shared__ int64_t found;
-  const int64_t row = blockIdx.x;
-  const int n = blockDim.x, tid = threadIdx.x;
+// ---- short rows -------------------------------------------------------------
+// W lanes hold a row of up to W * E entries, lane l the entries l + W j. Each
+// entry compares itself with every other: its place in the order and the sum
+// of the weights before it.
+template <typename T, int W, int E>
+__global__ void __launch_bounds__(128) short_kernel(const __grid_constant__ Args a) {
+  const int lane = threadIdx.x % W;
+  const unsigned base = (threadIdx.x & 31) / W * W;   // first lane of the group
+  const unsigned group = W == 32 ? 0xffffffffu : ((1u << (W % 32)) - 1u) << base;
+  const int64_t row = (int64_t)blockIdx.x * (128 / W) + threadIdx.x / W;
+  if (row >= a.rows) return;
   const Row r(a, row);
-  // the largest entry; a NaN or +inf
-  float m = -INFINITY;
-  bool bad = false;
-  for (int64_t i = tid; i < a.v; i += n) {
-    const float l = logit<T>(a, row, i);
-    bad |= !(l < INFINITY);
-    m = fmaxf(m, l);
-  }
-  bad = __syncthreads_or(bad);
+  float l[E], m = -INFINITY;
+  bool bad = !r.good;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((tid & 31) == 0) red[tid >> 5] = m;
-  __syncthreads();
-  for (int w = 0; w < n / 32; ++w) m = fmaxf(m, (float)red[w]);
-  __syncthreads();
-  if (bad || !r.good || m == -INFINITY) {
-    if (tid == 0) answer(a, row, -1, bad || !r.good ? __uint_as_float(0x7fc00000u) : -INFINITY);
+  for (int j = 0; j < E; ++j) {
+    const int i = lane + W * j;
+    l[j] = i < a.v ? logit<T>(a, row, i) : -INFINITY;
+    bad |= !(l[j] < INFINITY);
+    m = fmaxf(m, l[j]);
+  }
+  bad = __any_sync(group, bad);
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(group, m, o));
+  if (bad || m == -INFINITY) {
+    if (lane == 0) no_answer(a, row, bad);
     return;
   }
   Weights w;
   w.set(m, r);
-  if (r.t == 0.) w.inv32 = w.far = 0.f, w.inv = 0.;
-  const auto stays = [&](float l) { return r.t == 0. ? l == m : w.in(l); };
-  // entries above `border`, and the first `most` of those on it, stay
-  uint32_t border = 0;
-  int64_t most = 0;
-  const auto count_from = [&](uint32_t key) {
-    int64_t c = 0;
-    for (int64_t i = tid; i < a.v; i += n) {
-      const float l = logit<T>(a, row, i);
-      c += key_of(l) >= key && stays(l);
-    }
-    return (int64_t)block_sum((double)c, red);
-  };
-  if (r.k > 0 && count_from(0) > r.k) {
-    uint32_t lo = 0, hi = key_of(m);
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo + 1) / 2;
-      if (count_from(mid) >= r.k) lo = mid;
-      else hi = mid - 1;
-    }
-    border = lo;
-    most = r.k - (border == key_of(m) ? 0 : count_from(border + 1));
+  double weight[E], before[E];
+  int rank[E];
+  uint32_t key[E];
+  int staying = 0;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    const bool in = w.in(l[j]);
+    weight[j] = in ? w.of(l[j]) : 0.;
+    key[j] = in ? key_of(l[j]) : 0u;   // 0: below every entry that stays
+    staying += in;
+    rank[j] = 0;
+    before[j] = 0.;
   }
-  // the sum of the staying entries from a key on (above the border)
-  const auto sum_from = [&](uint32_t key) {
-    double s = 0.;
-    for (int64_t i = tid; i < a.v; i += n) {
-      const float l = logit<T>(a, row, i);
-      const uint32_t q = key_of(l);
-      if (q >= key && q > border && stays(l)) s += w.of(l);
-    }
-    return block_sum(s, red);
-  };
-  if (r.top_p < 1.) {
-    const double on = most ? (double)most * w.of(value_of(border)) : 0.;
-    const double target = r.top_p * (sum_from(0) + on);
-    uint32_t lo = border, hi = key_of(m);
-    while (lo < hi) {   // the largest key from which on the sum reaches the target
-      const uint32_t mid = lo + (hi - lo + 1) / 2;
-      if (sum_from(mid) >= target) lo = mid;
-      else hi = mid - 1;
-    }
-    const double above = lo == key_of(m) ? 0. : sum_from(lo + 1), each = w.of(value_of(lo));
-    int64_t have = lo == border ? most : 0;
-    if (lo != border || !most) {
-      int64_t c = 0;
-      for (int64_t i = tid; i < a.v; i += n) {
-        const float l = logit<T>(a, row, i);
-        c += key_of(l) == lo && stays(l);
+  const bool ordered = r.k > 0 || r.top_p < 1.;
+  if (ordered) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+#pragma unroll 4
+      for (int o = 0; o < W; ++o) {
+        const uint32_t k = __shfl_sync(group, key[j], base + o);
+        const double x = __shfl_sync(group, weight[j], base + o);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (k > key[e] || (k == key[e] && (j < e || (j == e && o < lane)))) {
+            ++rank[e];
+            before[e] += x;
+          }
       }
-      have = (int64_t)block_sum((double)c, red);
     }
-    int64_t need = (int64_t)fmin((target - above) / each, (double)have);
-    if (need < 1) need = 1;
-    while (need > 1 && above + (double)(need - 1) * each >= target) --need;
-    while (need < have && above + (double)need * each < target) ++need;
-    border = lo;
-    most = need;
   }
-  // each thread's stretch of the row: its sum above the border, its entries on the border
-  const int64_t per = (a.v + n - 1) / n, from = min(a.v, per * tid), to = min(a.v, from + per);
-  double above = 0.;
-  int on = 0;
-  for (int64_t i = from; i < to; ++i) {
-    const float l = logit<T>(a, row, i);
-    if (!stays(l)) continue;
-    const uint32_t q = key_of(l);
-    if (q > border || (border == 0 && !most)) above += w.of(l);
-    else if (q == border) ++on;
+  if (r.k > 0) {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (rank[j] >= r.k) weight[j] = 0.;
   }
-  parts[tid] = above;
-  ties[tid] = on;
-  __syncthreads();
-  const double each = most ? w.of(value_of(border)) : 0.;
-  if (tid == 0) {
-    // the running sum at each stretch's start, and the first border entry that counts there
+  if (r.top_p < 1.) {
     double total = 0.;
+#pragma unroll
+    for (int j = 0; j < E; ++j) total += weight[j];
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) total += __shfl_xor_sync(group, total, o);
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (rank[j] > 0 && before[j] >= r.top_p * total) weight[j] = 0.;
+  }
+  // running sums in the order of the indices
+  double start = 0., run[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    run[j] = weight[j];
+#pragma unroll
+    for (int o = 1; o < W; o <<= 1) {
+      const double x = __shfl_up_sync(group, run[j], o, W);
+      if (lane >= o) run[j] += x;
+    }
+    run[j] += start;
+    start = __shfl_sync(group, run[j], base + W - 1);
+  }
+  const double target = r.u * start;
+  int token = -1, last = -1;
+#pragma unroll
+  for (int j = E - 1; j >= 0; --j) {
+    const unsigned over = __ballot_sync(group, weight[j] > 0. && run[j] > target) & group;
+    const unsigned some = __ballot_sync(group, weight[j] > 0.) & group;
+    if (over) token = W * j + __ffs(over) - 1 - (int)base;
+    if (last < 0 && some) last = W * j + 31 - __clz(some) - (int)base;
+  }
+  if (token < 0) token = last;
+#pragma unroll
+  for (int j = 0; j < E; ++j)
+    if (token == lane + W * j) answer(a, row, token, (float)(((double)l[j] - w.top) * w.inv - log(start)));
+}
+
+// ---- long rows ---------------------------------------------------------------
+constexpr int kList = 256;      // entries of a border's neighbourhood that are ordered one by one
+constexpr float kSlack = 2e-5f; // of sums of fp32 estimates of weights
+
+struct Plan {
+  int threads, ctas;    // of a row
+  int strips;           // of 32 vectors of 8 entries, of a warp
+  bool resident;        // the row is held in shared memory
+  int listed;           // entries that a warp's list holds
+};
+
+// What the threads of a CTA share; `val`, `flag` and `list` are read by the row's other CTAs.
+struct Shared {
+  double val[2][2];
+  int flag[2][2];
+  double warp_above[32];
+  int warp_ties[32];
+  int listed;
+  uint32_t list_key[kList], list_at[kList];
+  // of this CTA alone
+  uint32_t mine_key[kList], mine_at[kList], sorted[kList];
+  double red[32][2];
+  float fred[32];
+  int ired[32];
+  int first, last, under, before, all, kept;
+  int count[32];        // entries of the warps' lists
+  double mass;
+};
+
+// A row on its CTAs: the entries as strips of 256, a warp's strips one after
+// the other, eight consecutive entries to a lane, on 16-byte boundaries. Once
+// a cut-off's neighbourhood is known, the entries above it and in it are
+// copied, in order, to lists of the warps, if those hold them, and whatever
+// follows reads the lists.
+template <typename T>
+struct RowOf {
+  const Args& a;
+  Shared& s;
+  uint32_t* hist;
+  unsigned char* slots;
+  T* list_value;        // of this warp
+  uint16_t* list_index; // within this warp's strips
+  const int64_t row;
+  const int strips, capacity, tid, lane, warp, warps, rank, ctas;
+  const bool resident;
+  const T* x;
+  int shift;            // entries between the boundary below the row's start and the start
+  int64_t first;        // index of this lane's first entry in its warp's first strip
+  int phase = 0;
+  Weights w;
+  uint32_t border = 0;  // entries above `border`, and the first `most` of those on it, stay
+  int64_t most = 0;
+
+  __device__ RowOf(const Args& a_, Shared& s_, unsigned char* raw, const Plan& p)
+      : a(a_), s(s_), row(blockIdx.x / p.ctas), strips(p.strips), capacity(p.listed), tid(threadIdx.x),
+        lane(threadIdx.x & 31), warp(threadIdx.x >> 5), warps(blockDim.x >> 5), rank(blockIdx.x % p.ctas), ctas(p.ctas),
+        resident(p.resident) {
+    hist = reinterpret_cast<uint32_t*>(raw);
+    raw += sizeof(uint32_t) * 8 * blockDim.x;
+    slots = raw;
+    if (resident) raw += sizeof(T) * 8 * strips * blockDim.x;
+    list_value = reinterpret_cast<T*>(raw) + warp * capacity;
+    list_index = reinterpret_cast<uint16_t*>(raw + sizeof(T) * warps * capacity) + warp * capacity;
+    x = static_cast<const T*>(a.logits) + row * a.ld;
+    shift = (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+    first = (int64_t)(rank * warps + warp) * strips * 256 + lane * 8 - shift;
+  }
+  __device__ __forceinline__ void sync() {
+    if (ctas > 1) cg::this_cluster().sync();
+    else __syncthreads();
+  }
+  template <typename U>
+  __device__ __forceinline__ U* at(U* p, int r) {
+    return ctas > 1 ? cg::this_cluster().map_shared_rank(p, r) : p;
+  }
+
+  // ---- entries
+  __device__ __forceinline__ void load(int strip, float (&v)[8]) const {
+    const int64_t i = first + (int64_t)strip * 256;
+    if (i >= 0 && i + 8 <= a.v) {
+      lm::load8(x + i, v);
+      if (a.mask) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!a.mask[row * a.mask_row + (i + e) * a.mask_col]) v[e] = -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = i + e >= 0 && i + e < a.v ? logit<T>(a, row, i + e) : -INFINITY;
+    }
+  }
+  // A lane's vector is two slots of 16 bytes in fp32, one in 16 bits.
+  __device__ __forceinline__ void keep(int strip, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+      float4* p = reinterpret_cast<float4*>(slots) + (int64_t)strip * 2 * blockDim.x + tid;
+      p[0] = make_float4(v[0], v[1], v[2], v[3]);
+      p[blockDim.x] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      lm::store8(reinterpret_cast<T*>(slots) + ((int64_t)strip * blockDim.x + tid) * 8, v);
+    }
+  }
+  __device__ __forceinline__ void get(int strip, float (&v)[8]) const {
+    if (!resident) {
+      load(strip, v);
+    } else if constexpr (sizeof(T) == 4) {
+      const float4* p = reinterpret_cast<const float4*>(slots) + (int64_t)strip * 2 * blockDim.x + tid;
+      const float4 f = p[0], g = p[blockDim.x];
+      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = g.x, v[5] = g.y, v[6] = g.z, v[7] = g.w;
+    } else {
+      lm::load8(reinterpret_cast<const T*>(slots) + ((int64_t)strip * blockDim.x + tid) * 8, v);
+    }
+  }
+  // How a pass takes the entries: N at a time to a lane, `steps` times.
+  template <bool LIST>
+  __device__ __forceinline__ int steps() const {
+    return LIST ? (s.count[warp] + 31) >> 5 : strips;
+  }
+  template <bool LIST>
+  __device__ __forceinline__ void fetch(int k, float (&v)[(LIST ? 1 : 8)]) const {
+    if constexpr (LIST) v[0] = k * 32 + lane < s.count[warp] ? lm::to_f<T>(list_value[k * 32 + lane]) : -INFINITY;
+    else get(k, v);
+  }
+  template <bool LIST>
+  __device__ __forceinline__ uint32_t index(int k, int e) const {
+    if constexpr (LIST) return (uint32_t)(first - lane * 8 + list_index[k * 32 + lane]);
+    else return (uint32_t)(first + (int64_t)k * 256 + e);
+  }
+  // f(entry, k, e) for this thread's entries
+  template <bool LIST, typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    const int n = steps<LIST>();
+    for (int k = 0; k < n; ++k) {
+      float v[(LIST ? 1 : 8)];
+      fetch<LIST>(k, v);
+#pragma unroll
+      for (int e = 0; e < (LIST ? 1 : 8); ++e) f(v[e], k, e);
+    }
+  }
+
+  // The same with the entries one by one, for passes that few rows take: an eighth of the code.
+  template <bool LIST, typename F>
+  __device__ __forceinline__ void each_single(F&& f) const {
+    if constexpr (LIST) {
+      each<true>(f);
+    } else {
+      for (int k = 0; k < strips; ++k) {
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) f(single(k, e), k, e);
+      }
+    }
+  }
+  __device__ __forceinline__ float single(int k, int e) const {
+    if (!resident) {
+      const int64_t i = first + (int64_t)k * 256 + e;
+      return i >= 0 && i < a.v ? logit<T>(a, row, i) : -INFINITY;
+    }
+    const int64_t slot = (int64_t)k * (sizeof(T) / 2) * blockDim.x + tid;
+    if constexpr (sizeof(T) == 4) return reinterpret_cast<const float*>(slots)[(slot + e / 4 * blockDim.x) * 4 + e % 4];
+    else return lm::to_f<T>(reinterpret_cast<const T*>(slots)[slot * 8 + e]);
+  }
+
+  // ---- sums over the row, the same in every thread
+  __device__ void sums(double& p, double& q) {
+    p = warp_sum(p);
+    q = warp_sum(q);
+    __syncthreads();
+    if (lane == 0) s.red[warp][0] = p, s.red[warp][1] = q;
+    __syncthreads();
+    p = q = 0.;
+    for (int i = 0; i < warps; ++i) p += s.red[i][0], q += s.red[i][1];
+    if (ctas > 1) {
+      const int now = phase++ & 1;
+      if (tid == 0) s.val[now][0] = p, s.val[now][1] = q;
+      sync();
+      p = q = 0.;
+      for (int i = 0; i < ctas; ++i) {
+        const double* v = at(s.val[now], i);
+        p += v[0], q += v[1];
+      }
+    }
+  }
+  __device__ double sum(double p) {
+    double q = 0.;
+    sums(p, q);
+    return p;
+  }
+  // the largest entry, and whether one is NaN or +inf
+  __device__ void top(float& m, bool& bad) {
+    bad = __syncthreads_or(bad);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) s.fred[warp] = m;
+    __syncthreads();
+    for (int i = 0; i < warps; ++i) m = fmaxf(m, s.fred[i]);
+    if (ctas > 1) {
+      const int now = phase++ & 1;
+      if (tid == 0) s.flag[now][0] = __float_as_int(m), s.flag[now][1] = bad;
+      sync();
+      for (int i = 0; i < ctas; ++i) {
+        const int* f = at(s.flag[now], i);
+        m = fmaxf(m, __int_as_float(f[0]));
+        bad |= f[1];
+      }
+    }
+  }
+
+  // ---- bins of the order
+  // Entries lie in bins by (largest - l) / T, of which there are `bins` up to
+  // the furthest that stays; a window of bins is cut into as many again.
+  float step;                  // temperatures a bin
+  int bins, b1 = 0, b2 = 0;    // the window
+  float scale2 = 0.f, step2 = 0.f;
+  int c1 = 0, c2 = 0;          // the window's window, of scale2 bins a bin
+  bool fine = false;
+  __device__ __forceinline__ int bin(float l) const { return min(bins - 1, (int)w.place(l)); }
+  __device__ __forceinline__ int bin2(float l) const {
+    return min(bins - 1, (int)__fmul_rn(__fsub_rn(w.place(l), (float)b1), scale2));
+  }
+  // -1 above the window, 0 in it, 1 below
+  __device__ __forceinline__ int side(float l) const {
+    const int b = bin(l);
+    if (b < b1) return -1;
+    if (b > b2) return 1;
+    if (!fine) return 0;
+    const int c = bin2(l);
+    return c < c1 ? -1 : c > c2 ? 1 : 0;
+  }
+  __device__ __forceinline__ bool stays(float l) const { return w.in(l) && (border == 0 || key_of(l) > border); }
+
+  __device__ void clear() {
+    sync();   // the row's other CTAs have read it
+    for (int i = 0; i < 8; ++i) hist[i * blockDim.x + tid] = 0;
+    if (tid == 0) s.listed = 0;
+    __syncthreads();
+  }
+  // Joins the row's bins and finds, by weight or by number, the bins [first,
+  // last] in which the border may lie; `under`: entries
+  // in them, `before`: above them, `all`: in all bins.
+  __device__ __noinline__ void find(bool by_weight, bool second, int64_t number, float low, float high) {
+    sync();
+    uint32_t c[8];
+    const float unit = second ? step2 : step, from = second ? (float)b1 * step : 0.f;
+    float h = 0.f;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      c[i] = 0;
+      for (int k = 0; k < ctas; ++k) c[i] += at(hist, k)[tid * 8 + i];
+      n += (int)c[i];
+      h += (float)c[i] * __expf(-(from + (float)(tid * 8 + i) * unit));
+    }
+    // sums of the threads before this one
+    float hs = h;
+    int ns = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float x = __shfl_up_sync(0xffffffffu, hs, o);
+      const int y = __shfl_up_sync(0xffffffffu, ns, o);
+      if (lane >= o) hs += x, ns += y;
+    }
+    if (lane == 31) s.fred[warp] = hs, s.ired[warp] = ns;
+    if (tid == 0) s.first = s.last = bins - 1, s.under = s.before = 0;
+    __syncthreads();
+    float total = 0.f;
+    int all = 0;
+    for (int i = 0; i < warps; ++i) {
+      if (i < warp) hs += s.fred[i], ns += s.ired[i];
+      total += s.fred[i];
+      all += s.ired[i];
+    }
+    hs -= h;   // (a rounding that kSlack covers)
+    ns -= n;
+    const float shrink = __expf(-unit) * (1.f - kSlack);
+    if (by_weight && !second) low *= total * shrink, high *= total * (1.f + kSlack);
+    const int n0 = ns;
+    bool below = false, over = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ns += (int)c[i];
+      hs += (float)c[i] * __expf(-(from + (float)(tid * 8 + i) * unit));
+      const bool one = ns > 0 && (by_weight ? hs * (1.f + kSlack) >= low : ns >= number);
+      const bool two = ns > 0 && (by_weight ? hs * shrink >= high : ns >= number);
+      if (one && !below) atomicMin(&s.first, tid * 8 + i), below = true;
+      if (two && !over) atomicMin(&s.last, tid * 8 + i), over = true;
+    }
+    __syncthreads();
+    const int first = s.first, last = max(s.first, s.last);
+    int in = 0, ahead = 0;
+    ns = n0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int b = tid * 8 + i;
+      if (b >= first && b <= last) in += (int)c[i];
+      if (b < first) ahead += (int)c[i];
+    }
+    in = __reduce_add_sync(0xffffffffu, in);
+    ahead = __reduce_add_sync(0xffffffffu, ahead);
+    if (lane == 0) atomicAdd(&s.under, in), atomicAdd(&s.before, ahead);
+    __syncthreads();
+    if (tid == 0) s.last = last, s.all = all;
+    __syncthreads();
+  }
+
+  // Copies the entries of the bins up to the window's last to the warps' lists,
+  // in order, and adds up the weights of all. Whether the lists hold them.
+  template <bool WEIGH>
+  __device__ __noinline__ bool compact(double& total) {
+    const RowOf me = *this;   // a copy whose members are registers
+    double sum = 0.;
+    int n = 0;
+    const float upto = (float)(b2 + 1);
+    const bool all = b2 == bins - 1;
+    for (int k = 0; k < me.strips; ++k) {
+      float v[8];
+      me.get(k, v);
+      unsigned take = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = me.stays(v[e]);
+        if (WEIGH && in) sum += me.w.of(v[e]);
+        take |= (unsigned)(in && (all || me.w.place(v[e]) < upto)) << e;
+      }
+      const int own = __popc(take);
+      int at = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, at, o);
+        if (me.lane >= o) at += y;
+      }
+      const int strip = __shfl_sync(0xffffffffu, at, 31);
+      at += n - own;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (!(take >> e & 1)) continue;
+        if (at < me.capacity) {
+          me.list_value[at] = lm::from_f<T>(v[e]);
+          me.list_index[at] = (uint16_t)(k * 256 + me.lane * 8 + e);
+        }
+        ++at;
+      }
+      n += strip;
+    }
+    if (lane == 0) s.count[warp] = min(n, capacity);
+    double over = lane == 0 && n > capacity ? 1. : 0.;
+    sums(sum, over);
+    total = sum;
+    return over == 0.;
+  }
+
+  // Moves the border up to the first `k` of the order (by number), or to the
+  // fewest whose weights come to `p` of all of them. Whether lists hold what is left.
+  template <bool LIST>
+  __device__ __noinline__ bool cut(bool by_weight, int64_t k, double p) {
+    fine = false;
+    step = w.far / (float)bins;
+    const float on = value_of(border);
+    clear();
+    {
+      const RowOf me = *this;   // a copy whose members are registers
+      me.template each<LIST>([&](float l, int, int) {
+        if (me.stays(l)) atomicAdd(&me.hist[me.bin(l)], 1u);
+      });
+    }
+    if (most && rank == 0 && tid == 0) atomicAdd(&hist[bin(on)], (uint32_t)most);
+    find(by_weight, false, k, (float)p, (float)p);
+    b1 = s.first;
+    b2 = s.last;
+    if (!by_weight && s.all <= k) return LIST;
+    const int64_t in = s.under, before = s.before;
+    double total = 0.;
+    bool held = LIST;
+    if constexpr (!LIST) {
+      // (entries on an older border are in no list, so it has to be the first)
+      const bool small = !most && before + in <= (int64_t)capacity * warps * ctas && strips <= 256;
+      if (small) held = by_weight ? compact<true>(total) : compact<false>(total);
+      if (by_weight && !small) {
+        each_single<false>([&](float l, int, int) {
+          if (stays(l)) total += w.of(l);
+        });
+        total = sum(total);
+      }
+    } else if (by_weight) {
+      each<true>([&](float l, int, int) {
+        if (stays(l)) total += w.of(l);
+      });
+      total = sum(total);
+    }
+    if (by_weight && most) total += (double)most * w.of(on);
+    if (held) narrow<true>(by_weight, k, p * total, in, before);
+    else narrow<false>(by_weight, k, p * total, in, before);
+    return held;
+  }
+  // The border in the window of bins [b1, b2], which has `in` entries and `before` above it.
+  template <bool LIST>
+  __device__ __noinline__ void narrow(bool by_weight, int64_t k, double target, int64_t in, int64_t before) {
+    const float on = value_of(border);
+    const bool again = in > kList && step > 0.f;
+    // the sum of those above the window, and the window's own bins
+    double above = 0.;
+    if (again) {
+      scale2 = (float)bins / (float)(b2 - b1 + 1);
+      step2 = step / scale2;
+    }
+    clear();
+    if (by_weight || again) {
+      each_single<LIST>([&](float l, int, int) {
+        if (!stays(l)) return;
+        const int b = bin(l);
+        if (by_weight && b < b1) above += w.of(l);
+        if (again && b >= b1 && b <= b2) atomicAdd(&hist[bin2(l)], 1u);
+      });
+      const int b = most ? bin(on) : -1;
+      if (again && b >= b1 && b <= b2 && rank == 0 && tid == 0) atomicAdd(&hist[bin2(on)], (uint32_t)most);
+      if (by_weight) {
+        above = sum(above);
+        if (b >= 0 && b < b1) above += (double)most * w.of(on);
+      }
+    }
+    int64_t need = k - before;   // by number: of the window's
+    if (again) {
+      const float left = (float)fmax(target - above, 0.);
+      find(by_weight, true, need, left * (1.f - kSlack), left * (1.f + kSlack));
+      c1 = s.first;
+      c2 = s.last;
+      in = s.under;
+      need -= s.before;
+      fine = true;
+    }
+    // the window's entries above the border: a list, or the smallest and the largest key
+    const bool listed = in <= kList;
+    uint32_t lo = 0xffffffffu, hi = 0;
+    double more = 0.;
+    each_single<LIST>([&](float l, int k, int e) {
+      if (!stays(l)) return;
+      const int at_side = side(l);
+      if (at_side == 0) {
+        const uint32_t key = key_of(l);
+        if (listed) {
+          const int n = atomicAdd(at(&s.listed, 0), 1);
+          at(s.list_key, 0)[n] = key;
+          at(s.list_at, 0)[n] = index<LIST>(k, e);
+        }
+        lo = min(lo, key), hi = max(hi, key);
+      } else if (by_weight && again && at_side < 0 && bin(l) >= b1) {
+        more += w.of(l);
+      }
+    });
+    if (by_weight && again) above += sum(more);
+    sync();
+    const bool on_border = most && side(on) == 0;
+    if (listed) {
+      const int n = *at(&s.listed, 0);
+      for (int i = tid; i < n; i += blockDim.x) s.mine_key[i] = at(s.list_key, 0)[i], s.mine_at[i] = at(s.list_at, 0)[i];
+      __syncthreads();
+      for (int i = tid; i < n; i += blockDim.x) {
+        int place = 0;
+        const uint32_t key = s.mine_key[i], where = s.mine_at[i];
+        for (int j = 0; j < n; ++j) place += s.mine_key[j] > key || (s.mine_key[j] == key && s.mine_at[j] < where);
+        s.sorted[place] = key;
+      }
+      if (tid == 0) s.kept = 0;
+      __syncthreads();
+      if (by_weight) {
+        if (warp == 0) {   // the sums before each, 32 at a time
+          double start = above;
+          int kept = 0;
+          for (int i = 0; i < n; i += 32) {
+            double x = i + lane < n ? w.of(value_of(s.sorted[i + lane])) : 0.;
+            const double own = x;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const double y = __shfl_up_sync(0xffffffffu, x, o);
+              if (lane >= o) x += y;
+            }
+            double prior = __shfl_up_sync(0xffffffffu, x, 1);
+            prior = start + (lane ? prior : 0.);
+            kept += __popc(__ballot_sync(0xffffffffu, own > 0. && (prior == 0. || prior < target)));
+            start += __shfl_sync(0xffffffffu, x, 31);
+          }
+          if (lane == 0) s.kept = kept, s.mass = start;
+        }
+      } else if (tid == 0) {
+        s.kept = (int)min(need, (int64_t)n);
+      }
+      __syncthreads();
+      const int kept = s.kept;
+      if (kept == n && on_border) {
+        // the border's own entries follow those of the list
+        int64_t left = need - n;
+        if (by_weight) left = ties(s.mass, target, w.of(on), most);
+        if (left > 0 || kept == 0) {
+          most = min(most, max(left, (int64_t)1));
+          __syncthreads();
+          return;
+        }
+      }
+      const int last = max(kept, 1) - 1;
+      border = s.sorted[last];
+      most = 1;
+      while (most <= last && s.sorted[last - most] == border) ++most;
+      __syncthreads();
+      return;
+    }
+    // many entries: the border by halving the keys between the smallest and the largest
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    __syncthreads();
+    if (tid == 0) s.first = -1, s.last = 0;   // as whole numbers of 32 bits, by atomics that order unsigned ones
+    __syncthreads();
+    if (lane == 0) {
+      atomicMin(reinterpret_cast<uint32_t*>(&s.first), lo);
+      atomicMax(reinterpret_cast<uint32_t*>(&s.last), hi);
+    }
+    __syncthreads();
+    lo = (uint32_t)s.first, hi = (uint32_t)s.last;
+    if (ctas > 1) {
+      const int now = phase++ & 1;
+      if (tid == 0) s.flag[now][0] = (int)lo, s.flag[now][1] = (int)hi;
+      sync();
+      for (int i = 0; i < ctas; ++i) lo = min(lo, (uint32_t)at(s.flag[now], i)[0]), hi = max(hi, (uint32_t)at(s.flag[now], i)[1]);
+    }
+    const int64_t old_most = most;
+    const bool none = lo > hi;   // only the border's own entries
+    // what the window's entries from a key on come to
+    const auto from = [&](uint32_t key) {
+      double x = 0.;
+      each_single<LIST>([&](float l, int, int) {
+        if (key_of(l) >= key && stays(l) && side(l) == 0) x += by_weight ? w.of(l) : 1.;
+      });
+      return sum(x);
+    };
+    const double start = by_weight ? above : 0., aim = by_weight ? target : (double)need;
+    if (none || (on_border && start + from(lo) < aim)) {
+      const double start2 = none ? start : start + from(lo);
+      most = by_weight ? ties(start2, aim, w.of(on), old_most) : (int64_t)(aim - start2);
+      most = max((int64_t)1, min(most, old_most));
+      return;
+    }
+    uint32_t top = hi;
+    while (lo < hi) {   // the largest key from which on they reach the aim
+      const uint32_t mid = lo + (hi - lo + 1) / 2;
+      if (start + from(mid) >= aim) lo = mid;
+      else hi = mid - 1;
+    }
+    const double ahead = start + (lo == top ? 0. : from(lo + 1));
+    double x = 0.;
+    each_single<LIST>([&](float l, int, int) { x += key_of(l) == lo && stays(l) && side(l) == 0; });
+    const int64_t have = (int64_t)sum(x);
+    border = lo;
+    most = by_weight ? ties(ahead, aim, w.of(value_of(lo)), have) : (int64_t)(aim - ahead);
+    most = max((int64_t)1, min(most, have));
+  }
+  // the fewest of `have` weights `x` that bring `ahead` to `aim`, one if there is nothing ahead
+  __device__ __forceinline__ int64_t ties(double ahead, double aim, double x, int64_t have) const {
+    int64_t n = (int64_t)fmin(fmax((aim - ahead) / x, 0.), (double)have);
+    while (n > 0 && ahead + (double)(n - 1) * x >= aim) --n;
+    while (n < have && ahead + (double)n * x < aim) ++n;
+    return ahead == 0. ? max(n, (int64_t)1) : n;
+  }
+
+  // The entry that holds u of the staying ones' sum.
+  template <bool LIST>
+  __device__ __noinline__ void draw(double u) {
+    const double x_on = most ? w.of(value_of(border)) : 0.;
+    double above = 0.;
+    int on = 0;
+    const RowOf me = *this;   // a copy whose members are registers
+    me.template each<LIST>([&](float l, int, int) {
+      if (!me.w.in(l)) return;
+      if (!me.most) {
+        above += me.w.of(l);
+        return;
+      }
+      const uint32_t key = key_of(l);
+      if (key > me.border) above += me.w.of(l);
+      else if (key == me.border) ++on;
+    });
+    above = warp_sum(above);
+    on = __reduce_add_sync(0xffffffffu, on);
+    if (lane == 0) s.warp_above[warp] = above, s.warp_ties[warp] = on;
+    __syncthreads();
+    // the border's entries before this CTA, so that its own count in order
     int64_t seen = 0;
-    int last = 0;
-    for (int t = 0; t < n; ++t) {
-      const int64_t here = max((int64_t)0, min((int64_t)ties[t], most - seen));
-      const double s = parts[t] + (double)here * each;
-      if (s > 0.) last = t;
-      parts[t] = total;
-      total += s;
-      const int64_t start = seen;
-      seen += ties[t];
-      ties[t] = (int)min(start, (int64_t)INT32_MAX);
+    if (ctas > 1) {
+      const int now = phase++ & 1;
+      if (tid == 0) {
+        int n = 0;
+        for (int i = 0; i < warps; ++i) n += s.warp_ties[i];
+        s.flag[now][0] = n;
+      }
+      sync();
+      for (int i = 0; i < rank; ++i) seen += at(s.flag[now], i)[0];
     }
-    red[0] = total;
-    const double target = r.u * total;
-    int t = last;
-    while (t > 0 && parts[t] > target) --t;
-    found = t;
-  }
-  __syncthreads();
-  if (tid == found) {
-    const double total = red[0], target = r.u * total;
-    double s = parts[tid];
-    int64_t seen = ties[tid], token = -1;
-    float at = m;
-    for (int64_t i = from; i < to; ++i) {
-      const float l = logit<T>(a, row, i);
-      if (!stays(l)) continue;
-      const uint32_t q = key_of(l);
-      const bool tie = q == border && most;
-      if (tie && seen++ >= most) continue;
-      if (!tie && q < border) continue;
-      s += w.of(l);
-      token = i;
-      at = l;
-      if (s > target) break;
+    const auto sum_of = [&](int i, int64_t n) {
+      return s.warp_above[i] + (double)max((int64_t)0, min((int64_t)s.warp_ties[i], most - n)) * x_on;
+    };
+    double here = 0.;
+    int64_t n = seen;
+    for (int i = 0; i < warps; ++i) {
+      here += sum_of(i, n);
+      n += s.warp_ties[i];
     }
-    answer(a, row, token, (float)(((double)at - w.top) * w.inv - log(total)));
+    double total = here, start = 0.;
+    int chosen = 0;
+    if (ctas > 1) {   // which CTA holds the target; u of the sum beyond the last one: the last that has any
+      const int now = phase++ & 1;
+      if (tid == 0) s.val[now][0] = here;
+      sync();
+      total = 0.;
+      for (int i = 0; i < ctas; ++i) total += at(s.val[now], i)[0];
+      double run = 0.;
+      bool done = false;
+      for (int i = 0; i < ctas; ++i) {
+        const double x = at(s.val[now], i)[0];
+        if (!done && x > 0.) chosen = i, start = run, done = run + x > u * total;
+        run += x;
+      }
+    }
+    const double target = u * total - start;
+    if (rank == chosen) {
+      double run = 0., from = 0.;
+      int64_t mine = 0;
+      int held = 0;
+      bool done = false;
+      n = seen;
+      for (int i = 0; i < warps; ++i) {
+        const double x = sum_of(i, n);
+        if (!done && x > 0.) held = i, from = run, mine = n, done = run + x > target;
+        run += x;
+        n += s.warp_ties[i];
+      }
+      if (warp == held) walk<LIST>(target, total, from, mine);
+    }
+    if (ctas > 1) sync();   // no CTA ends while another reads its sums
   }
+  // The first entry of this warp at which the running sum exceeds the target, or its last that stays.
+  template <bool LIST>
+  __device__ __noinline__ void walk(double target, double total, double start, int64_t seen) {
+    constexpr int N = LIST ? 1 : 8;
+    const double x_on = most ? w.of(value_of(border)) : 0.;
+    const int n_steps = steps<LIST>();
+    uint32_t token = 0;
+    float token_logit = 0.f;
+    const auto entry = [&](int k, int e) {
+      if constexpr (LIST) {
+        float v[1];
+        fetch<true>(k, v);
+        return v[0];
+      } else {
+        return single(k, e);
+      }
+    };
+    // what an entry adds, `n` of the border's being before it
+    const auto weight = [&](float l, int64_t& n) {
+      if (!w.in(l)) return 0.;
+      const uint32_t key = key_of(l);
+      if (most && key <= border) return key == border && n++ < most ? x_on : 0.;
+      return w.of(l);
+    };
+    for (int k = 0; k < n_steps; ++k) {
+      int on = 0;
+      if (most) {
+#pragma unroll 1
+        for (int e = 0; e < N; ++e) {
+          const float l = entry(k, e);
+          on += w.in(l) && key_of(l) == border;
+        }
+      }
+      int prior = on;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, prior, o);
+        if (lane >= o) prior += y;
+      }
+      const int64_t mine = seen + prior - on;
+      seen += __shfl_sync(0xffffffffu, prior, 31);
+      int64_t n = mine;
+      double own = 0.;
+#pragma unroll 1
+      for (int e = 0; e < N; ++e) own += weight(entry(k, e), n);
+      double run = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += y;
+      }
+      const unsigned any = __ballot_sync(0xffffffffu, own > 0.);
+      const unsigned found = __ballot_sync(0xffffffffu, own > 0. && start + run > target);
+      if (any) {   // the lane that passes the target, or the last that has any so far
+        const int src = found ? __ffs(found) - 1 : 31 - __clz(any);
+        double t = start + run - own;
+        n = mine;
+        int at = 0;
+        bool past = false;
+        float l = 0.f;
+#pragma unroll 1
+        for (int e = 0; e < N; ++e) {
+          const float here = entry(k, e);
+          const double x = weight(here, n);
+          if (x > 0. && !past) {
+            t += x;
+            at = e;
+            l = here;
+            past = t > target;
+          }
+        }
+        token = __shfl_sync(0xffffffffu, index<LIST>(k, at), src);
+        token_logit = __shfl_sync(0xffffffffu, l, src);
+      }
+      if (found) break;
+      start += __shfl_sync(0xffffffffu, run, 31);
+    }
+    if (lane == 0) answer(a, row, token, (float)(((double)token_logit - w.top) * w.inv - log(total)));
+  }
+
+  __device__ void run() {
+    const Row r(a, row);
+    float m = -INFINITY;
+    bool bad = !r.good;
+    for (int k = 0; k < strips; ++k) {
+      float v[8];
+      load(k, v);
+      if (resident) keep(k, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        bad |= !(v[e] < INFINITY);
+        m = fmaxf(m, v[e]);
+      }
+    }
+    top(m, bad);
+    if (bad || m == -INFINITY) {
+      if (rank == 0 && tid == 0) no_answer(a, row, bad);
+      if (ctas > 1) sync();
+      return;
+    }
+    w.set(m, r);
+    bins = 8 * blockDim.x;
+    if (r.t == 0.) {   // the first of the largest
+      border = key_of(m);
+      most = 1;
+      draw<false>(r.u);
+      return;
+    }
+    w.set_bins(bins);
+    bool listed = false;
+    if (r.k > 0 && r.k < a.v) listed = cut<false>(false, r.k, 0.);
+    if (r.top_p < 1.) listed = listed ? cut<true>(true, 0, r.top_p) : cut<false>(true, 0, r.top_p);
+    if (listed) draw<true>(r.u);
+    else draw<false>(r.u);
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(512, 2) row_kernel(const __grid_constant__ Args a, const __grid_constant__ Plan p) {
+  __shared__ Shared s;
+  extern __shared__ __align__(16) unsigned char raw[];
+  RowOf<T> on(a, s, raw, p);
+  on.run();
+}
+
+template <typename T>
+cudaError_t launch_rows(const Args& a, const Plan& p, cudaStream_t st) {
+  const auto kernel = row_kernel<T>;
+  const int smem = 32 * p.threads + (p.resident ? p.strips * p.threads * 8 * (int)sizeof(T) : 0) +
+                   p.threads / 32 * p.listed * ((int)sizeof(T) + 2);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.rows * p.ctas));
+  cfg.blockDim = dim3(p.threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = p.ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = p.ctas > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, a, p);
+}
+
+Plan plan(const Args& a, int sms) {
+  const int size = a.type == 0 ? 4 : 2;
+  Plan p{};
+  p.threads = a.v <= 1024 ? 64 : a.v <= 2048 ? 128 : a.v <= 8192 ? 256 : 512;
+  const int64_t vectors = (a.v + 7 + 16 / size - 1) / 8;   // with what lies before a row's start
+  const auto cut = [&](int ctas) {
+    p.ctas = ctas;
+    p.strips = (int)((vectors + (int64_t)ctas * p.threads - 1) / ((int64_t)ctas * p.threads));
+    return (int64_t)p.strips * p.threads * 8 * size;
+  };
+  // few rows are shared by more CTAs; a row's part fits three times into an SM's shared memory
+  int64_t bytes = cut(1);
+  while (p.ctas < 8 && (bytes > 66 * 1024 || (a.rows * p.ctas * 2 <= sms && p.strips > 2))) bytes = cut(p.ctas * 2);
+  p.resident = bytes <= 160 * 1024;   // one CTA's part always is
+  p.listed = std::min(p.strips * 48, 512);   // three sixteenths of a warp's entries
+  return p;
+}
+
+template <typename T>
+cudaError_t launch_type(const Args& a, int sms, cudaStream_t st) {
+  if (a.v <= 128) {
+    const auto grid = [&](int w) { return (unsigned)((a.rows + 128 / w - 1) / (128 / w)); };
+    if (a.v <= 8) short_kernel<T, 8, 1><<<grid(8), 128, 0, st>>>(a);
+    else if (a.v <= 32) short_kernel<T, 32, 1><<<grid(32), 128, 0, st>>>(a);
+    else short_kernel<T, 32, 4><<<grid(32), 128, 0, st>>>(a);
+    return cudaGetLastError();
+  }
+  return launch_rows<T>(a, plan(a, sms), st);
 }
 
 }  // namespace
 
 cudaError_t launch(const Args& a, int sms, cudaStream_t st) {
-  const int threads = a.v >= 16384 ? 1024 : a.v >= 1024 ? 256 : 64;
-  if (a.type == 0) row_kernel<float><<<(unsigned)a.rows, threads, 0, st>>>(a);
-  else if (a.type == 1) row_kernel<__nv_bfloat16><<<(unsigned)a.rows, threads, 0, st>>>(a);
-  else row_kernel<__half><<<(unsigned)a.rows, threads, 0, st>>>(a);
-  return cudaGetLastError();
+  if (a.type == 0) return launch_type<float>(a, sms, st);
+  if (a.type == 1) return launch_type<__nv_bfloat16>(a, sms, st);
+  return launch_type<__half>(a, sms, st);
 }
 
 }  // namespace sampling

@@ -18,14 +18,15 @@ scores tokens with one):
   of the staying weights exceeds the row's number times their sum (a number of
   1 or more takes the last, a negative one the first), and ``log_prob`` the
   logarithm of its share of that sum;
+* entries further than 44 temperatures below the largest count as zero (they
+  hold less than 10^-13 of any row's sum);
 * a temperature of 0 takes the first of the largest entries;
 * a row without a valid entry above -inf gives token -1 and -inf; a NaN or
   +inf among its valid entries, or a number or parameter that is NaN or out of
   range, gives -1 and NaN.
 
 Each of the four parameters is a number for all rows or a tensor [...] (fp32;
-``top_k`` int64 or int32) with one for each. Weights and sums are fp64; on CUDA
-entries further than 44 temperatures below the largest count as zero. On CPU
+``top_k`` int64 or int32) with one for each. Weights and sums are fp64. On CPU
 the same is computed in plain PyTorch.
 """
 from __future__ import annotations
@@ -38,6 +39,7 @@ from torch import Tensor
 from .ext import require_extension
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+RANGE = 44.
 
 
 class SampledTokens(NamedTuple):
@@ -53,6 +55,7 @@ def reference_sample_tokens(logits: Tensor, uniforms: Tensor, mask: Tensor | Non
     if mask is not None:
         z = torch.where(mask, z, -torch.inf)
     u, t, p, least = (x.double()[:, None] for x in (uniforms, temperature, top_p, min_p))
+    u = u.clamp_min(0.)
     k = top_k.long()[:, None]
     bad = ~((t == 0) | ((t >= 1e-30) & (t <= 1e30))) | p.isnan() | u.isnan() | ~(least <= 1) | (k < 0)
     bad |= (z.isnan() | (z == torch.inf)).any(-1, keepdim=True)
@@ -63,7 +66,7 @@ def reference_sample_tokens(logits: Tensor, uniforms: Tensor, mask: Tensor | Non
     greedy = t == 0
     scaled = (z.double() - top) / torch.where(greedy, 1., t)
     w = torch.where(greedy, (z == top).double(), scaled.exp())
-    w = torch.where(w >= least, w, 0.)
+    w = torch.where((w >= least) & (scaled >= -RANGE), w, 0.)
     _, index = torch.sort(z, dim=-1, descending=True, stable=True)
     ordered = w.gather(1, index)
     rank = torch.arange(v, device=z.device)
@@ -76,7 +79,7 @@ def reference_sample_tokens(logits: Tensor, uniforms: Tensor, mask: Tensor | Non
     running = w.cumsum(-1)
     total = running[:, -1:]
     token = (running <= u * total).sum(-1, keepdim=True)
-    token = torch.minimum(token, (running < total).sum(-1, keepdim=True)).clamp(max=v - 1)
+    token = torch.minimum(token, torch.where(w > 0, rank, 0).amax(-1, keepdim=True))
     log_prob = torch.where(greedy, 0., scaled.gather(1, token)) - total.log()
     log_prob = torch.where(bad, torch.nan, torch.where(empty, -torch.inf, log_prob))
     return SampledTokens(torch.where(bad | empty, -1, token)[:, 0], log_prob[:, 0].float())
