@@ -16,6 +16,8 @@
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include <algorithm>
 
 #include "lm_vec.h"
@@ -84,33 +86,50 @@ __device__ __forceinline__ double exp_of(double x) {
 struct Weights {
   double top, inv;        // 1 / T
   float top32, inv32, far;
-  float scale, sure;       // bins a logit (see RowOf); places below this one stay without a further look
-  double least;
-  __device__ __forceinline__ void set(float m, const Row& r) {
+  float scale;             // bins a logit (see RowOf)
+  float lowest;            // the smallest logit that stays before the cut-offs by order
+  float log2_hi, log2_lo;  // log2(e) / T in two parts
+  // `cut`: the entries that min_p cuts off are told by their logits.
+  __device__ __forceinline__ void set(float m, const Row& r, bool cut) {
     top = m;
     top32 = m;
     inv = r.t == 0. ? 0. : 1. / r.t;
     inv32 = (float)inv;
-    least = r.min_p;
-    far = least > 0. ? fminf(kRange, -(float)log(least)) : kRange;
-    if (r.t == 0.) far = -1.f;
-    scale = sure = 0.f;
+    const double c = 1.4426950408889634 * inv;
+    log2_hi = (float)c;
+    log2_lo = (float)(c - (double)log2_hi);
+    far = kRange;
+    scale = 0.f;
+    if (r.t == 0.) {   // the largest entries alone
+      lowest = m;
+      far = 0.f;
+      return;
+    }
+    lowest = __double2float_ru(fmax(top - (double)kRange * r.t, -3.4e38));
+    if (cut && r.min_p > 0.) {   // by halving: a logit stays or not by its weight in fp64
+      uint32_t lo = key_of(lowest), hi = key_of(m);
+      while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (of(value_of(mid)) >= r.min_p) hi = mid;
+        else lo = mid + 1;
+      }
+      lowest = value_of(lo);
+      far = fminf(kRange, (float)((top - (double)lowest) * inv));
+    }
   }
-  __device__ __forceinline__ void set_bins(int bins) {
-    if (far > 0.f) scale = (float)bins / far * inv32;
-    sure = (float)bins * (far - 1e-3f) / far;
-    if (!(far > 2e-3f)) sure = -1.f;
-  }
+  __device__ __forceinline__ void set_bins(int bins) { scale = far > 0.f ? (float)bins / far * inv32 : 0.f; }
   __device__ __forceinline__ float place(float l) const { return __fmul_rn(__fsub_rn(top32, l), scale); }
-  __device__ __forceinline__ double of(float l) const { return exp_of(((double)l - top) * inv); }
-  // Whether an entry stays before the cut-offs by order: told in fp32 but next to the border.
-  __device__ __forceinline__ bool in(float l) const {
-    if (place(l) < sure) return true;
-    const float d = __fmul_rn(__fsub_rn(top32, l), inv32);
-    if (!(d <= far + 1e-3f)) return far < 0.f && l == top32;   // a temperature of 0: the largest entries alone
-    if (d < far - 1e-3f) return true;
-    return far < kRange ? of(l) >= least : d <= far;
+  // The weight in fp32. The product's rounding is added back, so that what is
+  // left is that of top - l, of the exponential and of the sums (see kError).
+  __device__ __forceinline__ float of32(float l) const {
+    const float d = __fsub_rn(l, top32);
+    const float p = __fmul_rn(d, log2_hi);
+    const float e = __fmaf_rn(d, log2_lo, __fmaf_rn(d, log2_hi, -p));
+    float x;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(p));
+    return __fmul_rn(x, __fmaf_rn(e, .6931471806f, 1.f));
   }
+  __device__ __forceinline__ double of(float l) const { return exp_of(((double)l - top) * inv); }
 };
 
 __device__ __forceinline__ void answer(const Args& a, int64_t row, int64_t token, float log_prob) {
@@ -163,15 +182,17 @@ __global__ void __launch_bounds__(128) short_kernel(const __grid_constant__ Args
     return;
   }
   Weights w;
-  w.set(m, r);
+  w.set(m, r, false);
   double weight[E], before[E];
   int rank[E];
   uint32_t key[E];
   int staying = 0;
 #pragma unroll
   for (int j = 0; j < E; ++j) {
-    const bool in = w.in(l[j]);
+    bool in = l[j] >= w.lowest;
     weight[j] = in ? w.of(l[j]) : 0.;
+    in = in && weight[j] >= r.min_p;
+    if (!in) weight[j] = 0.;
     key[j] = in ? key_of(l[j]) : 0u;   // 0: below every entry that stays
     staying += in;
     rank[j] = 0;
@@ -240,11 +261,16 @@ __global__ void __launch_bounds__(128) short_kernel(const __grid_constant__ Args
 // ---- long rows ---------------------------------------------------------------
 constexpr int kList = 256;      // entries of a border's neighbourhood that are ordered one by one
 constexpr float kSlack = 2e-5f; // of sums of fp32 estimates of weights
+// Relative error of a sum of of32() over at most 2^20 entries: 2^-22 of the
+// exponential, 3 * 2^-24 of sums of eight, and the rounding of top - l, 2^-24 |x|,
+// where the mean of |x| over the weights is at most the logarithm of their
+// number (it is the distribution's entropy less log S, and S >= 1): 14 * 2^-24.
+constexpr double kError = 1.4e-6;
+constexpr int64_t kMost32 = 1 << 20;
 
 struct Plan {
   int threads, ctas;    // of a row
   int strips;           // of 32 vectors of 8 entries, of a warp
-  bool resident;        // the row is held in shared memory
   int listed;           // entries that a warp's list holds
 };
 
@@ -276,12 +302,10 @@ struct RowOf {
   const Args& a;
   Shared& s;
   uint32_t* hist;
-  unsigned char* slots;
   T* list_value;        // of this warp
   uint16_t* list_index; // within this warp's strips
   const int64_t row;
   const int strips, capacity, tid, lane, warp, warps, rank, ctas;
-  const bool resident;
   const T* x;
   int shift;            // entries between the boundary below the row's start and the start
   int64_t first;        // index of this lane's first entry in its warp's first strip
@@ -289,15 +313,13 @@ struct RowOf {
   Weights w;
   uint32_t border = 0;  // entries above `border`, and the first `most` of those on it, stay
   int64_t most = 0;
+  float least = 0.f;    // the smallest logit above the border that stays
 
   __device__ RowOf(const Args& a_, Shared& s_, unsigned char* raw, const Plan& p)
       : a(a_), s(s_), row(blockIdx.x / p.ctas), strips(p.strips), capacity(p.listed), tid(threadIdx.x),
-        lane(threadIdx.x & 31), warp(threadIdx.x >> 5), warps(blockDim.x >> 5), rank(blockIdx.x % p.ctas), ctas(p.ctas),
-        resident(p.resident) {
+        lane(threadIdx.x & 31), warp(threadIdx.x >> 5), warps(blockDim.x >> 5), rank(blockIdx.x % p.ctas), ctas(p.ctas) {
     hist = reinterpret_cast<uint32_t*>(raw);
     raw += sizeof(uint32_t) * 8 * blockDim.x;
-    slots = raw;
-    if (resident) raw += sizeof(T) * 8 * strips * blockDim.x;
     list_value = reinterpret_cast<T*>(raw) + warp * capacity;
     list_index = reinterpret_cast<uint16_t*>(raw + sizeof(T) * warps * capacity) + warp * capacity;
     x = static_cast<const T*>(a.logits) + row * a.ld;
@@ -328,40 +350,24 @@ struct RowOf {
       for (int e = 0; e < 8; ++e) v[e] = i + e >= 0 && i + e < a.v ? logit<T>(a, row, i + e) : -INFINITY;
     }
   }
-  // A lane's vector is two slots of 16 bytes in fp32, one in 16 bits.
-  __device__ __forceinline__ void keep(int strip, const float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
-      float4* p = reinterpret_cast<float4*>(slots) + (int64_t)strip * 2 * blockDim.x + tid;
-      p[0] = make_float4(v[0], v[1], v[2], v[3]);
-      p[blockDim.x] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      lm::store8(reinterpret_cast<T*>(slots) + ((int64_t)strip * blockDim.x + tid) * 8, v);
-    }
-  }
-  __device__ __forceinline__ void get(int strip, float (&v)[8]) const {
-    if (!resident) {
-      load(strip, v);
-    } else if constexpr (sizeof(T) == 4) {
-      const float4* p = reinterpret_cast<const float4*>(slots) + (int64_t)strip * 2 * blockDim.x + tid;
-      const float4 f = p[0], g = p[blockDim.x];
-      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = g.x, v[5] = g.y, v[6] = g.z, v[7] = g.w;
-    } else {
-      lm::load8(reinterpret_cast<const T*>(slots) + ((int64_t)strip * blockDim.x + tid) * 8, v);
-    }
-  }
   // How a pass takes the entries: N at a time to a lane, `steps` times.
   template <bool LIST>
   __device__ __forceinline__ int steps() const {
-    return LIST ? (s.count[warp] + 31) >> 5 : strips;
+    return LIST ? (s.count[warp] + 127) >> 7 : strips;
   }
   template <bool LIST>
-  __device__ __forceinline__ void fetch(int k, float (&v)[(LIST ? 1 : 8)]) const {
-    if constexpr (LIST) v[0] = k * 32 + lane < s.count[warp] ? lm::to_f<T>(list_value[k * 32 + lane]) : -INFINITY;
-    else get(k, v);
+  __device__ __forceinline__ void fetch(int k, float (&v)[LIST ? 4 : 8]) const {
+    if constexpr (LIST) {
+      const int i = k * 128 + lane * 4, n = s.count[warp];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = i + e < n ? lm::to_f<T>(list_value[i + e]) : -INFINITY;
+    } else {
+      load(k, v);
+    }
   }
   template <bool LIST>
   __device__ __forceinline__ uint32_t index(int k, int e) const {
-    if constexpr (LIST) return (uint32_t)(first - lane * 8 + list_index[k * 32 + lane]);
+    if constexpr (LIST) return (uint32_t)(first - lane * 8 + list_index[min(k * 128 + lane * 4 + e, capacity - 1)]);
     else return (uint32_t)(first + (int64_t)k * 256 + e);
   }
   // f(entry, k, e) for this thread's entries
@@ -369,13 +375,26 @@ struct RowOf {
   __device__ __forceinline__ void each(F&& f) const {
     const int n = steps<LIST>();
     for (int k = 0; k < n; ++k) {
-      float v[(LIST ? 1 : 8)];
+      float v[(LIST ? 4 : 8)];
       fetch<LIST>(k, v);
 #pragma unroll
-      for (int e = 0; e < (LIST ? 1 : 8); ++e) f(v[e], k, e);
+      for (int e = 0; e < (LIST ? 4 : 8); ++e) f(v[e], k, e);
     }
   }
 
+  // The sum of f(entry) in fp32 over a thread's eight, and in fp64 beyond.
+  template <typename F>
+  __device__ __forceinline__ double mass(F&& f) const {
+    double s = 0.;
+    for (int k = 0; k < strips; ++k) {
+      float v[8];
+      load(k, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = f(v[e]);
+      s += (double)(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])));
+    }
+    return s;
+  }
   // The same with the entries one by one, for passes that few rows take: an eighth of the code.
   template <bool LIST, typename F>
   __device__ __forceinline__ void each_single(F&& f) const {
@@ -389,13 +408,8 @@ struct RowOf {
     }
   }
   __device__ __forceinline__ float single(int k, int e) const {
-    if (!resident) {
-      const int64_t i = first + (int64_t)k * 256 + e;
-      return i >= 0 && i < a.v ? logit<T>(a, row, i) : -INFINITY;
-    }
-    const int64_t slot = (int64_t)k * (sizeof(T) / 2) * blockDim.x + tid;
-    if constexpr (sizeof(T) == 4) return reinterpret_cast<const float*>(slots)[(slot + e / 4 * blockDim.x) * 4 + e % 4];
-    else return lm::to_f<T>(reinterpret_cast<const T*>(slots)[slot * 8 + e]);
+    const int64_t i = first + (int64_t)k * 256 + e;
+    return i >= 0 && i < a.v ? logit<T>(a, row, i) : -INFINITY;
   }
 
   // ---- sums over the row, the same in every thread
@@ -464,11 +478,17 @@ struct RowOf {
     const int c = bin2(l);
     return c < c1 ? -1 : c > c2 ? 1 : 0;
   }
-  __device__ __forceinline__ bool stays(float l) const { return w.in(l) && (border == 0 || key_of(l) > border); }
+  __device__ __forceinline__ bool stays(float l) const { return l >= least; }
+  __device__ __forceinline__ void set_border(uint32_t key) {
+    border = key;
+    // comparisons take what is below 2^-126 for zero, so the next number above zero is that one
+    const uint32_t next = key >= 0x80000000u && key < 0x80800000u ? 0x80800000u : key + 1;
+    least = key < key_of(w.top32) ? value_of(next) : INFINITY;
+  }
 
   __device__ void clear() {
     sync();   // the row's other CTAs have read it
-    for (int i = 0; i < 8; ++i) hist[i * blockDim.x + tid] = 0;
+    reinterpret_cast<uint4*>(hist)[tid] = reinterpret_cast<uint4*>(hist)[blockDim.x + tid] = make_uint4(0, 0, 0, 0);
     if (tid == 0) s.listed = 0;
     __syncthreads();
   }
@@ -482,11 +502,21 @@ struct RowOf {
     float h = 0.f;
     int n = 0;
 #pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = 0;
+#pragma unroll 4
+    for (int k = 0; k < ctas; ++k) {
+      const uint4* p = reinterpret_cast<const uint4*>(at(hist, k)) + tid * 2;
+      const uint4 x = p[0], y = p[1];
+      c[0] += x.x, c[1] += x.y, c[2] += x.z, c[3] += x.w, c[4] += y.x, c[5] += y.y, c[6] += y.z, c[7] += y.w;
+    }
+    const float head = __expf(-(from + (float)(tid * 8) * unit)), ratio = __expf(-unit);
+    float part[8], f = head;
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
-      c[i] = 0;
-      for (int k = 0; k < ctas; ++k) c[i] += at(hist, k)[tid * 8 + i];
       n += (int)c[i];
-      h += (float)c[i] * __expf(-(from + (float)(tid * 8 + i) * unit));
+      part[i] = (float)c[i] * f;
+      h += part[i];
+      f *= ratio;
     }
     // sums of the threads before this one
     float hs = h;
@@ -509,19 +539,22 @@ struct RowOf {
     }
     hs -= h;   // (a rounding that kSlack covers)
     ns -= n;
-    const float shrink = __expf(-unit) * (1.f - kSlack);
+    const float shrink = ratio * (1.f - kSlack);
     if (by_weight && !second) low *= total * shrink, high *= total * (1.f + kSlack);
     const int n0 = ns;
-    bool below = false, over = false;
+    int low_at = bins - 1, high_at = bins - 1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       ns += (int)c[i];
-      hs += (float)c[i] * __expf(-(from + (float)(tid * 8 + i) * unit));
+      hs += part[i];
       const bool one = ns > 0 && (by_weight ? hs * (1.f + kSlack) >= low : ns >= number);
       const bool two = ns > 0 && (by_weight ? hs * shrink >= high : ns >= number);
-      if (one && !below) atomicMin(&s.first, tid * 8 + i), below = true;
-      if (two && !over) atomicMin(&s.last, tid * 8 + i), over = true;
+      if (one) low_at = min(low_at, tid * 8 + i);
+      if (two) high_at = min(high_at, tid * 8 + i);
     }
+    low_at = __reduce_min_sync(0xffffffffu, low_at);
+    high_at = __reduce_min_sync(0xffffffffu, high_at);
+    if (lane == 0) atomicMin(&s.first, low_at), atomicMin(&s.last, high_at);
     __syncthreads();
     const int first = s.first, last = max(s.first, s.last);
     int in = 0, ahead = 0;
@@ -541,24 +574,26 @@ struct RowOf {
   }
 
   // Copies the entries of the bins up to the window's last to the warps' lists,
-  // in order, and adds up the weights of all. Whether the lists hold them.
-  template <bool WEIGH>
-  __device__ __noinline__ bool compact(double& total) {
+  // in order. Whether the lists hold them.
+  __device__ __noinline__ bool compact() {
     const RowOf me = *this;   // a copy whose members are registers
-    double sum = 0.;
     int n = 0;
-    const float upto = (float)(b2 + 1);
-    const bool all = b2 == bins - 1;
+    float lowest = least;   // of the window: by halving, as the bins' rounding has it
+    if (b2 < bins - 1) {
+      uint32_t lo = key_of(least), hi = key_of(w.top32);
+      while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (me.w.place(value_of(mid)) < (float)(b2 + 1)) hi = mid;
+        else lo = mid + 1;
+      }
+      lowest = value_of(lo);
+    }
     for (int k = 0; k < me.strips; ++k) {
       float v[8];
-      me.get(k, v);
+      me.load(k, v);
       unsigned take = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool in = me.stays(v[e]);
-        if (WEIGH && in) sum += me.w.of(v[e]);
-        take |= (unsigned)(in && (all || me.w.place(v[e]) < upto)) << e;
-      }
+      for (int e = 0; e < 8; ++e) take |= (unsigned)(v[e] >= lowest) << e;
       const int own = __popc(take);
       int at = own;
 #pragma unroll
@@ -568,22 +603,28 @@ struct RowOf {
       }
       const int strip = __shfl_sync(0xffffffffu, at, 31);
       at += n - own;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (!(take >> e & 1)) continue;
-        if (at < me.capacity) {
-          me.list_value[at] = lm::from_f<T>(v[e]);
-          me.list_index[at] = (uint16_t)(k * 256 + me.lane * 8 + e);
-        }
-        ++at;
+      for (; take; take &= take - 1, ++at) {
+        const int e = __ffs(take) - 1;
+        if (at >= me.capacity) break;
+        me.list_value[at] = lm::from_f<T>(me.single(k, e));
+        me.list_index[at] = (uint16_t)(k * 256 + me.lane * 8 + e);
       }
       n += strip;
     }
     if (lane == 0) s.count[warp] = min(n, capacity);
-    double over = lane == 0 && n > capacity ? 1. : 0.;
-    sums(sum, over);
-    total = sum;
-    return over == 0.;
+    return sum(lane == 0 && n > capacity ? 1. : 0.) == 0.;
+  }
+
+  // The sum of the staying entries' weights, in fp64.
+  template <bool LIST>
+  __device__ __noinline__ double total() {
+    const RowOf me = *this;   // a copy whose members are registers
+    double x = 0.;
+    me.template each_single<LIST>([&](float l, int, int) {
+      if (me.stays(l)) x += me.w.of(l);
+    });
+    x = sum(x);
+    return most ? x + (double)most * w.of(value_of(border)) : x;
   }
 
   // Moves the border up to the first `k` of the order (by number), or to the
@@ -594,11 +635,24 @@ struct RowOf {
     step = w.far / (float)bins;
     const float on = value_of(border);
     clear();
+    // a sum in fp32 will mostly do, whose error is known
+    const bool rough = !LIST && by_weight && a.v <= kMost32;
+    double sum_of = 0.;
     {
       const RowOf me = *this;   // a copy whose members are registers
-      me.template each<LIST>([&](float l, int, int) {
-        if (me.stays(l)) atomicAdd(&me.hist[me.bin(l)], 1u);
-      });
+      if constexpr (!LIST) {
+        if (rough) {
+          sum_of = me.mass([&](float l) {
+            if (!me.stays(l)) return 0.f;
+            atomicAdd(&me.hist[me.bin(l)], 1u);
+            return me.w.of32(l);
+          });
+        }
+      }
+      if (!rough)
+        me.template each<LIST>([&](float l, int, int) {
+          if (me.stays(l)) atomicAdd(&me.hist[me.bin(l)], 1u);
+        });
     }
     if (most && rank == 0 && tid == 0) atomicAdd(&hist[bin(on)], (uint32_t)most);
     find(by_weight, false, k, (float)p, (float)p);
@@ -606,32 +660,37 @@ struct RowOf {
     b2 = s.last;
     if (!by_weight && s.all <= k) return LIST;
     const int64_t in = s.under, before = s.before;
-    double total = 0.;
     bool held = LIST;
     if constexpr (!LIST) {
       // (entries on an older border are in no list, so it has to be the first)
-      const bool small = !most && before + in <= (int64_t)capacity * warps * ctas && strips <= 256;
-      if (small) held = by_weight ? compact<true>(total) : compact<false>(total);
-      if (by_weight && !small) {
-        each_single<false>([&](float l, int, int) {
-          if (stays(l)) total += w.of(l);
-        });
-        total = sum(total);
-      }
-    } else if (by_weight) {
-      each<true>([&](float l, int, int) {
-        if (stays(l)) total += w.of(l);
-      });
-      total = sum(total);
+      if (!most && before + in <= (int64_t)capacity * warps * ctas && strips <= 256) held = compact();
     }
-    if (by_weight && most) total += (double)most * w.of(on);
-    if (held) narrow<true>(by_weight, k, p * total, in, before);
-    else narrow<false>(by_weight, k, p * total, in, before);
+    Aim aim{p, 0., 0., true};
+    if (by_weight) {
+      sum_of = rough ? sum(sum_of) + (most ? (double)most * w.of(on) : 0.) : total<LIST>();
+      aim.low = p * sum_of * (1. - (rough ? kError : 0.));
+      aim.high = p * sum_of * (1. + (rough ? kError : 0.));
+      aim.exact = !rough;
+    }
+    if (held) narrow<LIST, true>(by_weight, k, aim, in, before);
+    else narrow<LIST, false>(by_weight, k, aim, in, before);
     return held;
   }
-  // The border in the window of bins [b1, b2], which has `in` entries and `before` above it.
+  // What a prefix of the order has to come to: `p` of a sum that lies in a range, or is exact.
+  struct Aim {
+    double p, low, high;
+    bool exact;
+  };
   template <bool LIST>
-  __device__ __noinline__ void narrow(bool by_weight, int64_t k, double target, int64_t in, int64_t before) {
+  __device__ void settle(Aim& aim) {
+    if (aim.exact) return;
+    aim.low = aim.high = aim.p * total<LIST>();
+    aim.exact = true;
+  }
+  // The border in the window of bins [b1, b2], which has `in` entries and `before` above it.
+  // `ALL` is whether the entries that the sum is over are in lists, `LIST` whether those of the window and above are.
+  template <bool ALL, bool LIST>
+  __device__ __noinline__ void narrow(bool by_weight, int64_t k, Aim aim, int64_t in, int64_t before) {
     const float on = value_of(border);
     const bool again = in > kList && step > 0.f;
     // the sum of those above the window, and the window's own bins
@@ -642,11 +701,12 @@ struct RowOf {
     }
     clear();
     if (by_weight || again) {
-      each_single<LIST>([&](float l, int, int) {
-        if (!stays(l)) return;
-        const int b = bin(l);
-        if (by_weight && b < b1) above += w.of(l);
-        if (again && b >= b1 && b <= b2) atomicAdd(&hist[bin2(l)], 1u);
+      const RowOf me = *this;   // a copy whose members are registers
+      me.template each_single<LIST>([&](float l, int, int) {
+        if (!me.stays(l)) return;
+        const int b = me.bin(l);
+        if (by_weight && b < me.b1) above += me.w.of(l);
+        if (again && b >= me.b1 && b <= me.b2) atomicAdd(&me.hist[me.bin2(l)], 1u);
       });
       const int b = most ? bin(on) : -1;
       if (again && b >= b1 && b <= b2 && rank == 0 && tid == 0) atomicAdd(&hist[bin2(on)], (uint32_t)most);
@@ -657,8 +717,8 @@ struct RowOf {
     }
     int64_t need = k - before;   // by number: of the window's
     if (again) {
-      const float left = (float)fmax(target - above, 0.);
-      find(by_weight, true, need, left * (1.f - kSlack), left * (1.f + kSlack));
+      find(by_weight, true, need, (float)fmax(aim.low - above, 0.) * (1.f - kSlack),
+           (float)fmax(aim.high - above, 0.) * (1.f + kSlack));
       c1 = s.first;
       c2 = s.last;
       in = s.under;
@@ -669,26 +729,33 @@ struct RowOf {
     const bool listed = in <= kList;
     uint32_t lo = 0xffffffffu, hi = 0;
     double more = 0.;
-    each_single<LIST>([&](float l, int k, int e) {
-      if (!stays(l)) return;
-      const int at_side = side(l);
-      if (at_side == 0) {
-        const uint32_t key = key_of(l);
-        if (listed) {
-          const int n = atomicAdd(at(&s.listed, 0), 1);
-          at(s.list_key, 0)[n] = key;
-          at(s.list_at, 0)[n] = index<LIST>(k, e);
+    {
+      const RowOf me = *this;   // a copy whose members are registers
+      int* number = at(&s.listed, 0);
+      uint32_t *keys = at(s.list_key, 0), *places = at(s.list_at, 0);
+      me.template each_single<LIST>([&](float l, int k, int e) {
+        if (!me.stays(l)) return;
+        const int at_side = me.side(l);
+        if (at_side == 0) {
+          const uint32_t key = key_of(l);
+          if (listed) {
+            const int n = atomicAdd(number, 1);
+            if (n < kList) {   // which the bins' numbers have said
+              keys[n] = key;
+              places[n] = me.template index<LIST>(k, e);
+            }
+          }
+          lo = min(lo, key), hi = max(hi, key);
+        } else if (by_weight && again && at_side < 0 && me.bin(l) >= me.b1) {
+          more += me.w.of(l);
         }
-        lo = min(lo, key), hi = max(hi, key);
-      } else if (by_weight && again && at_side < 0 && bin(l) >= b1) {
-        more += w.of(l);
-      }
-    });
+      });
+    }
     if (by_weight && again) above += sum(more);
     sync();
     const bool on_border = most && side(on) == 0;
     if (listed) {
-      const int n = *at(&s.listed, 0);
+      const int n = min(*at(&s.listed, 0), kList);
       for (int i = tid; i < n; i += blockDim.x) s.mine_key[i] = at(s.list_key, 0)[i], s.mine_at[i] = at(s.list_at, 0)[i];
       __syncthreads();
       for (int i = tid; i < n; i += blockDim.x) {
@@ -697,12 +764,12 @@ struct RowOf {
         for (int j = 0; j < n; ++j) place += s.mine_key[j] > key || (s.mine_key[j] == key && s.mine_at[j] < where);
         s.sorted[place] = key;
       }
-      if (tid == 0) s.kept = 0;
       __syncthreads();
-      if (by_weight) {
+      if (by_weight && on_border) settle<ALL>(aim);
+      while (by_weight) {
         if (warp == 0) {   // the sums before each, 32 at a time
           double start = above;
-          int kept = 0;
+          int kept = 0, most_kept = 0;
           for (int i = 0; i < n; i += 32) {
             double x = i + lane < n ? w.of(value_of(s.sorted[i + lane])) : 0.;
             const double own = x;
@@ -713,20 +780,22 @@ struct RowOf {
             }
             double prior = __shfl_up_sync(0xffffffffu, x, 1);
             prior = start + (lane ? prior : 0.);
-            kept += __popc(__ballot_sync(0xffffffffu, own > 0. && (prior == 0. || prior < target)));
+            kept += __popc(__ballot_sync(0xffffffffu, own > 0. && (prior == 0. || prior < aim.low)));
+            most_kept += __popc(__ballot_sync(0xffffffffu, own > 0. && (prior == 0. || prior < aim.high)));
             start += __shfl_sync(0xffffffffu, x, 31);
           }
-          if (lane == 0) s.kept = kept, s.mass = start;
+          if (lane == 0) s.kept = kept, s.last = most_kept, s.mass = start;
         }
-      } else if (tid == 0) {
-        s.kept = (int)min(need, (int64_t)n);
+        __syncthreads();
+        if (s.kept == s.last) break;
+        settle<ALL>(aim);   // a sum's end lies in the range
+        __syncthreads();
       }
-      __syncthreads();
-      const int kept = s.kept;
+      const int kept = by_weight ? s.kept : (int)min(need, (int64_t)n);
       if (kept == n && on_border) {
         // the border's own entries follow those of the list
         int64_t left = need - n;
-        if (by_weight) left = ties(s.mass, target, w.of(on), most);
+        if (by_weight) left = ties(s.mass, aim.low, w.of(on), most);
         if (left > 0 || kept == 0) {
           most = min(most, max(left, (int64_t)1));
           __syncthreads();
@@ -734,12 +803,17 @@ struct RowOf {
         }
       }
       const int last = max(kept, 1) - 1;
-      border = s.sorted[last];
+      set_border(s.sorted[last]);
       most = 1;
-      while (most <= last && s.sorted[last - most] == border) ++most;
+      for (int i = last - 1; i >= 0; i -= 32) {   // how many of the kept ones are on it
+        const unsigned same = __ballot_sync(0xffffffffu, i - lane >= 0 && s.sorted[max(i - lane, 0)] == border);
+        most += ~same ? __ffs(~same) - 1 : 32;
+        if (~same) break;
+      }
       __syncthreads();
       return;
     }
+    if (by_weight) settle<ALL>(aim);
     // many entries: the border by halving the keys between the smallest and the largest
     lo = __reduce_min_sync(0xffffffffu, lo);
     hi = __reduce_max_sync(0xffffffffu, hi);
@@ -768,25 +842,25 @@ struct RowOf {
       });
       return sum(x);
     };
-    const double start = by_weight ? above : 0., aim = by_weight ? target : (double)need;
-    if (none || (on_border && start + from(lo) < aim)) {
+    const double start = by_weight ? above : 0., goal = by_weight ? aim.low : (double)need;
+    if (none || (on_border && start + from(lo) < goal)) {
       const double start2 = none ? start : start + from(lo);
-      most = by_weight ? ties(start2, aim, w.of(on), old_most) : (int64_t)(aim - start2);
+      most = by_weight ? ties(start2, goal, w.of(on), old_most) : (int64_t)(goal - start2);
       most = max((int64_t)1, min(most, old_most));
       return;
     }
     uint32_t top = hi;
-    while (lo < hi) {   // the largest key from which on they reach the aim
+    while (lo < hi) {   // the largest key from which on they reach the goal
       const uint32_t mid = lo + (hi - lo + 1) / 2;
-      if (start + from(mid) >= aim) lo = mid;
+      if (start + from(mid) >= goal) lo = mid;
       else hi = mid - 1;
     }
     const double ahead = start + (lo == top ? 0. : from(lo + 1));
     double x = 0.;
     each_single<LIST>([&](float l, int, int) { x += key_of(l) == lo && stays(l) && side(l) == 0; });
     const int64_t have = (int64_t)sum(x);
-    border = lo;
-    most = by_weight ? ties(ahead, aim, w.of(value_of(lo)), have) : (int64_t)(aim - ahead);
+    set_border(lo);
+    most = by_weight ? ties(ahead, goal, w.of(value_of(lo)), have) : (int64_t)(goal - ahead);
     most = max((int64_t)1, min(most, have));
   }
   // the fewest of `have` weights `x` that bring `ahead` to `aim`, one if there is nothing ahead
@@ -797,26 +871,31 @@ struct RowOf {
     return ahead == 0. ? max(n, (int64_t)1) : n;
   }
 
-  // The entry that holds u of the staying ones' sum.
-  template <bool LIST>
-  __device__ __noinline__ void draw(double u) {
+  // The entry that holds u of the staying ones' sum. With EXACT unset the sums
+  // are fp32, and the answer is given only if their error cannot change it.
+  template <bool LIST, bool EXACT>
+  __device__ __noinline__ bool draw(double u) {
     const double x_on = most ? w.of(value_of(border)) : 0.;
     double above = 0.;
     int on = 0;
-    const RowOf me = *this;   // a copy whose members are registers
-    me.template each<LIST>([&](float l, int, int) {
-      if (!me.w.in(l)) return;
-      if (!me.most) {
-        above += me.w.of(l);
-        return;
+    {
+      const RowOf me = *this;   // a copy whose members are registers
+      const auto is_above = [&](float l) {
+        if (me.most) on += key_of(l) == me.border;
+        return l >= me.least;
+      };
+      if constexpr (EXACT) {
+        me.template each<LIST>([&](float l, int, int) {
+          if (is_above(l)) above += me.w.of(l);
+        });
+      } else {
+        above = me.mass([&](float l) { return is_above(l) ? me.w.of32(l) : 0.f; });
       }
-      const uint32_t key = key_of(l);
-      if (key > me.border) above += me.w.of(l);
-      else if (key == me.border) ++on;
-    });
+    }
     above = warp_sum(above);
     on = __reduce_add_sync(0xffffffffu, on);
     if (lane == 0) s.warp_above[warp] = above, s.warp_ties[warp] = on;
+    if (tid == 0) s.kept = 0;
     __syncthreads();
     // the border's entries before this CTA, so that its own count in order
     int64_t seen = 0;
@@ -868,124 +947,158 @@ struct RowOf {
         run += x;
         n += s.warp_ties[i];
       }
-      if (warp == held) walk<LIST>(target, total, from, mine);
+      if (warp == held) walk<LIST, EXACT>(target, total, from, mine);
     }
-    if (ctas > 1) sync();   // no CTA ends while another reads its sums
+    sync();
+    if constexpr (EXACT) return true;
+    const bool sure = *at(&s.kept, chosen) != 0;
+    sync();   // no CTA goes on while another reads this
+    return sure;
   }
   // The first entry of this warp at which the running sum exceeds the target, or its last that stays.
-  template <bool LIST>
+  template <bool LIST, bool EXACT>
   __device__ __noinline__ void walk(double target, double total, double start, int64_t seen) {
-    constexpr int N = LIST ? 1 : 8;
-    const double x_on = most ? w.of(value_of(border)) : 0.;
-    const int n_steps = steps<LIST>();
+    constexpr int N = LIST ? 4 : 8;
+    const RowOf me = *this;   // a copy whose members are registers
+    const double x_on = me.most ? me.w.of(value_of(me.border)) : 0.;
+    const int n_steps = me.template steps<LIST>();
     uint32_t token = 0;
     float token_logit = 0.f;
-    const auto entry = [&](int k, int e) {
-      if constexpr (LIST) {
-        float v[1];
-        fetch<true>(k, v);
-        return v[0];
-      } else {
-        return single(k, e);
-      }
-    };
-    // what an entry adds, `n` of the border's being before it
-    const auto weight = [&](float l, int64_t& n) {
-      if (!w.in(l)) return 0.;
-      const uint32_t key = key_of(l);
-      if (most && key <= border) return key == border && n++ < most ? x_on : 0.;
-      return w.of(l);
-    };
+    double end = 0., last = 0.;   // the running sum behind the token, and its weight
     for (int k = 0; k < n_steps; ++k) {
-      int on = 0;
-      if (most) {
-#pragma unroll 1
-        for (int e = 0; e < N; ++e) {
-          const float l = entry(k, e);
-          on += w.in(l) && key_of(l) == border;
-        }
-      }
-      int prior = on;
+      float v[N];
+      double x[N];
+      me.template fetch<LIST>(k, v);
+      int64_t mine = 0;
+      if (me.most) {
+        int on = 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, prior, o);
-        if (lane >= o) prior += y;
+        for (int e = 0; e < N; ++e) on += key_of(v[e]) == me.border;
+        int prior = on;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, prior, o);
+          if (me.lane >= o) prior += y;
+        }
+        mine = seen + prior - on;
+        seen += __shfl_sync(0xffffffffu, prior, 31);
       }
-      const int64_t mine = seen + prior - on;
-      seen += __shfl_sync(0xffffffffu, prior, 31);
-      int64_t n = mine;
       double own = 0.;
-#pragma unroll 1
-      for (int e = 0; e < N; ++e) own += weight(entry(k, e), n);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        x[e] = v[e] >= me.least ? me.w.of(v[e]) : 0.;
+        if (me.most && key_of(v[e]) == me.border) x[e] = mine++ < me.most ? x_on : 0.;
+        own += x[e];
+      }
       double run = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const double y = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += y;
+        if (me.lane >= o) run += y;
       }
       const unsigned any = __ballot_sync(0xffffffffu, own > 0.);
       const unsigned found = __ballot_sync(0xffffffffu, own > 0. && start + run > target);
       if (any) {   // the lane that passes the target, or the last that has any so far
         const int src = found ? __ffs(found) - 1 : 31 - __clz(any);
-        double t = start + run - own;
-        n = mine;
+        double t = start + run - own, one = 0.;
         int at = 0;
         bool past = false;
         float l = 0.f;
-#pragma unroll 1
+#pragma unroll
         for (int e = 0; e < N; ++e) {
-          const float here = entry(k, e);
-          const double x = weight(here, n);
-          if (x > 0. && !past) {
-            t += x;
+          if (x[e] > 0. && !past) {
+            t += x[e];
+            one = x[e];
             at = e;
-            l = here;
+            l = v[e];
             past = t > target;
           }
         }
-        token = __shfl_sync(0xffffffffu, index<LIST>(k, at), src);
+        token = __shfl_sync(0xffffffffu, me.template index<LIST>(k, at), src);
         token_logit = __shfl_sync(0xffffffffu, l, src);
+        end = __shfl_sync(0xffffffffu, t, src);
+        last = __shfl_sync(0xffffffffu, one, src);
       }
       if (found) break;
       start += __shfl_sync(0xffffffffu, run, 31);
     }
-    if (lane == 0) answer(a, row, token, (float)(((double)token_logit - w.top) * w.inv - log(total)));
+    const double error = 2. * kError * total;
+    const bool sure = EXACT || (end - last + error <= target && target + error < end);
+    if (lane == 0 && sure) {
+      answer(a, row, token, (float)(((double)token_logit - w.top) * w.inv - log(total)));
+      s.kept = 1;
+    }
+  }
+
+  // Reads the row and returns the thread's largest entry, NaN if it has one.
+  __device__ __forceinline__ float take() {
+    constexpr int kAhead = 4;   // strips under way
+    float m = -INFINITY;
+    const int64_t begin = first - lane * 8;   // of the warp
+    for (int k = 0; k < strips; k += kAhead) {
+      if (!a.mask && k + kAhead <= strips && begin + (int64_t)k * 256 >= 0 && begin + (int64_t)(k + kAhead) * 256 <= a.v) {
+        constexpr int W = sizeof(T) / 2;      // 16-byte words of a lane's vector
+        uint4 u[kAhead][W];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+          for (int h = 0; h < W; ++h) u[j][h] = reinterpret_cast<const uint4*>(x + first + (int64_t)(k + j) * 256)[h];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+          for (int h = 0; h < W; ++h) m = max_nan(m, largest(u[j][h]));
+      } else {
+        for (int j = k; j < min(k + kAhead, strips); ++j) {
+          float v[8];
+          load(j, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) m = max_nan(m, v[e]);
+        }
+      }
+    }
+    return m;
+  }
+  static __device__ __forceinline__ float max_nan(float p, float q) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(p), "f"(q));
+    return r;
+  }
+  static __device__ __forceinline__ float largest(const uint4& u) {
+    if constexpr (sizeof(T) == 4) {
+      return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+    } else {
+      using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+      const T2* h = reinterpret_cast<const T2*>(&u);
+      const T2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+      return max_nan(lm::to_f<T>(m.x), lm::to_f<T>(m.y));
+    }
   }
 
   __device__ void run() {
     const Row r(a, row);
-    float m = -INFINITY;
-    bool bad = !r.good;
-    for (int k = 0; k < strips; ++k) {
-      float v[8];
-      load(k, v);
-      if (resident) keep(k, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        bad |= !(v[e] < INFINITY);
-        m = fmaxf(m, v[e]);
-      }
-    }
+    float m = take();
+    bool bad = !r.good || !(m < INFINITY);
     top(m, bad);
     if (bad || m == -INFINITY) {
       if (rank == 0 && tid == 0) no_answer(a, row, bad);
       if (ctas > 1) sync();
       return;
     }
-    w.set(m, r);
+    w.set(m, r, true);
     bins = 8 * blockDim.x;
     if (r.t == 0.) {   // the first of the largest
-      border = key_of(m);
+      set_border(key_of(m));
       most = 1;
-      draw<false>(r.u);
+      draw<false, true>(r.u);
       return;
     }
     w.set_bins(bins);
+    least = w.lowest;
     bool listed = false;
     if (r.k > 0 && r.k < a.v) listed = cut<false>(false, r.k, 0.);
     if (r.top_p < 1.) listed = listed ? cut<true>(true, 0, r.top_p) : cut<false>(true, 0, r.top_p);
-    if (listed) draw<true>(r.u);
-    else draw<false>(r.u);
+    if (listed) draw<true, true>(r.u);
+    else if (a.v > kMost32 || !draw<false, false>(r.u)) draw<false, true>(r.u);
   }
 };
 
@@ -1000,8 +1113,7 @@ __global__ void __launch_bounds__(512, 2) row_kernel(const __grid_constant__ Arg
 template <typename T>
 cudaError_t launch_rows(const Args& a, const Plan& p, cudaStream_t st) {
   const auto kernel = row_kernel<T>;
-  const int smem = 32 * p.threads + (p.resident ? p.strips * p.threads * 8 * (int)sizeof(T) : 0) +
-                   p.threads / 32 * p.listed * ((int)sizeof(T) + 2);
+  const int smem = 32 * p.threads + p.threads / 32 * p.listed * ((int)sizeof(T) + 2);
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -1019,20 +1131,16 @@ cudaError_t launch_rows(const Args& a, const Plan& p, cudaStream_t st) {
 }
 
 Plan plan(const Args& a, int sms) {
-  const int size = a.type == 0 ? 4 : 2;
   Plan p{};
-  p.threads = a.v <= 1024 ? 64 : a.v <= 2048 ? 128 : a.v <= 8192 ? 256 : 512;
-  const int64_t vectors = (a.v + 7 + 16 / size - 1) / 8;   // with what lies before a row's start
-  const auto cut = [&](int ctas) {
-    p.ctas = ctas;
-    p.strips = (int)((vectors + (int64_t)ctas * p.threads - 1) / ((int64_t)ctas * p.threads));
-    return (int64_t)p.strips * p.threads * 8 * size;
-  };
-  // few rows are shared by more CTAs; a row's part fits three times into an SM's shared memory
-  int64_t bytes = cut(1);
-  while (p.ctas < 8 && (bytes > 66 * 1024 || (a.rows * p.ctas * 2 <= sms && p.strips > 2))) bytes = cut(p.ctas * 2);
-  p.resident = bytes <= 160 * 1024;   // one CTA's part always is
-  p.listed = std::min(p.strips * 48, 512);   // three sixteenths of a warp's entries
+  // Threads by the row's length: half as many cost 2047 rows of 8000 65 %, of
+  // 32003 60 % of this time and more; twice as many 40 % and 15 % more.
+  p.threads = a.v <= 2048 ? 64 : a.v <= 8192 ? 128 : 256;
+  const int64_t vectors = (a.v + 14) / 8;   // with what lies before a row's start
+  p.ctas = 1;
+  const auto strips = [&] { return (int)((vectors + (int64_t)p.ctas * p.threads - 1) / ((int64_t)p.ctas * p.threads)); };
+  while (p.ctas < 8 && a.rows * p.ctas * 2 <= sms && strips() > 2) p.ctas *= 2;   // few rows are shared by more CTAs
+  p.strips = strips();
+  p.listed = std::min(p.strips * 48, 4096);   // three sixteenths of a warp's entries
   return p;
 }
 

@@ -12,8 +12,9 @@ scores tokens with one):
 * entries weigh w = exp((logit - largest) / temperature); masked ones are not
   read, whatever they hold;
 * those with w < ``min_p`` are cut off; of the rest the first ``top_k`` by
-  their logits stay (0: all), equal ones by their index; of these the fewest,
-  in the same order, whose weights come to ``top_p`` of theirs, and always one;
+  their logits stay (0: all), equal ones by their index (on CUDA all logits
+  below fp32's normal range, 2^-126, equal zero); of these the fewest, in the
+  same order, whose weights come to ``top_p`` of theirs, and always one;
 * the token is the first entry that stays, by index, at which the running sum
   of the staying weights exceeds the row's number times their sum (a number of
   1 or more takes the last, a negative one the first), and ``log_prob`` the
