@@ -16,10 +16,11 @@
 // vectors once from memory and keeps it in a slot of shared memory that no
 // other thread reads, so only the sums need barriers.
 //
-// A cluster of CTAs holds a whole sample and joins its sums through
-// distributed shared memory: one read and one write of each value. Samples too
-// large for that take a pass for the sums and one that reads the values again.
-#include <cooperative_groups.h>
+// Where a CTA's shared memory holds a sample, one launch reads and writes each
+// value once. Larger samples are cut into parts, a CTA's each: one launch takes
+// the parts' sums, a second one reads them again, the last first, as L2 may
+// still hold those. A thread keeps its next vectors under way in a ring of its
+// own slots.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -29,12 +30,8 @@
 #include "groupnorm.h"
 #include "lm_vec.h"
 
-namespace cg = cooperative_groups;
-
 namespace groupnorm {
 namespace {
-
-constexpr int kStages = 4;            // waits among a thread's loads
 
 struct Args {
   const void *x, *dy;
@@ -42,25 +39,80 @@ struct Args {
   Affine a;
   const float *mean_in, *rstd_in;
   float *mean, *rstd;
-  float *ws;                          // partial sums of the samples' parts
-  float *sums;                        // backward: [n][2][c] sums P and Q, or null
+  float *ws;                          // sums of the samples' parts
   int64_t pixels, vectors;            // of a sample
   int64_t n;
   int64_t chunk;
-  int c, groups, cols, rows, iterations, act;
+  int c, groups, cols, rows, iterations, act, ctas;
   float eps;
 };
 
+// Two fp32 numbers that one instruction works on.
+struct Pair {
+  unsigned long long v;
+  __device__ __forceinline__ Pair() : v(0) {}
+  __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit Pair(float a) : Pair(a, a) {}
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+template <typename F>
+__device__ __forceinline__ Pair map(Pair a, F&& f) {
+  float x, y;
+  a.get(x, y);
+  return Pair(f(x), f(y));
+}
+
+// V elements as they lie in memory, and as P pairs (the last one half used where V is 1).
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
+  static constexpr int P = (V + 1) / 2;
   T e[V];
-  __device__ __forceinline__ void get(float (&f)[V]) const {
+  __device__ __forceinline__ void get(Pair (&f)[P]) const {
+    if constexpr (V == 1) {
+      f[0] = Pair(lm::to_f<T>(e[0]), 0.f);
+    } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = lm::to_f<T>(e[i]);
+      for (int i = 0; i < P; ++i) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          const uint32_t u = reinterpret_cast<const uint32_t*>(e)[i];
+          f[i] = Pair(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+        } else {
+          f[i] = Pair(lm::to_f<T>(e[2 * i]), lm::to_f<T>(e[2 * i + 1]));
+        }
+      }
+    }
   }
-  __device__ __forceinline__ void set(const float (&f)[V]) {
+  __device__ __forceinline__ void set(const Pair (&f)[P]) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = lm::from_f<T>(f[i]);
+    for (int i = 0; i < P; ++i) {
+      float a, b;
+      f[i].get(a, b);
+      if constexpr (V == 1) {
+        e[0] = lm::from_f<T>(a);
+      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        reinterpret_cast<__nv_bfloat162*>(e)[i] = __floats2bfloat162_rn(a, b);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        reinterpret_cast<__half2*>(e)[i] = __floats2half2_rn(a, b);
+      } else {
+        e[2 * i] = a;
+        e[2 * i + 1] = b;
+      }
+    }
   }
 };
 
@@ -75,14 +127,7 @@ __device__ __forceinline__ void fetch(Vec<T, V>* slot, const Vec<T, V>* from) {
   }
 }
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void wait_for(int left) {
-  switch (left) {
-    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-    default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-  }
-}
+__device__ __forceinline__ void wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
 __device__ __forceinline__ float parameter(const void* p, int type, int c, float otherwise) {
   if (!p) return otherwise;
@@ -91,62 +136,122 @@ __device__ __forceinline__ float parameter(const void* p, int type, int c, float
                                : __half2float(static_cast<const __half*>(p)[c]);
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + __expf(-z)); }
-
-template <int V>
-__device__ __forceinline__ void activate(int act, float (&z)[V]) {
-  if (act == kSilu) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) z[i] *= sigmoid(z[i]);
-  } else if (act == kRelu) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) z[i] = z[i] < 0.f ? 0.f : z[i];
-  } else if (act == kGelu) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) z[i] *= normcdff(z[i]);
-  }
+__device__ __forceinline__ float tanh_of(float x) {
+  float y;
+  asm("tanh.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-// dy times the activation's slope at z.
-template <int V>
-__device__ __forceinline__ void slope(int act, const float (&z)[V], float (&d)[V]) {
+// 1 / (1 + e^-z)
+__device__ __forceinline__ Pair sigmoid(Pair z) {
+  const Pair e = map(z * Pair(-1.4426950409f), [](float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+  });
+  return map(e + Pair(1.f), [](float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+  });
+}
+
+// For bf16 values SiLU goes by the hardware's tanh, whose 2^-11 is a quarter of
+// their rounding: one special function instead of two, of which an SM has 16 a
+// cycle. With t = tanh(z / 2) it is z / 2 (1 + t), and its slope (1 + t + z / 2
+// (1 - t^2)) / 2; z is halved in its parameters, and the slope's half is left
+// to those of what follows.
+template <typename T>
+__device__ __forceinline__ float halved(int act) {
+  return std::is_same<T, __nv_bfloat16>::value && act == kSilu ? .5f : 1.f;
+}
+
+template <typename T, int P>
+__device__ __forceinline__ void activate(int act, Pair (&z)[P]) {
   if (act == kSilu) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float s = sigmoid(z[i]);
-      d[i] *= s * (1.f + z[i] * (1.f - s));
+    for (int i = 0; i < P; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) z[i] = fma(z[i], map(z[i], tanh_of), z[i]);
+      else z[i] = z[i] * sigmoid(z[i]);
     }
   } else if (act == kRelu) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) d[i] = z[i] > 0.f ? d[i] : z[i] <= 0.f ? 0.f : z[i];
+    for (int i = 0; i < P; ++i) z[i] = map(z[i], [](float x) { return x < 0.f ? 0.f : x; });
   } else if (act == kGelu) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) d[i] *= normcdff(z[i]) + z[i] * .3989422804f * __expf(-.5f * z[i] * z[i]);
+    for (int i = 0; i < P; ++i) z[i] = map(z[i], [](float x) { return x * normcdff(x); });
+  }
+}
+// d (the gradient of y) times the activation's slope at z, over halved().
+template <typename T, int P>
+__device__ __forceinline__ void slope(int act, const Pair (&z)[P], Pair (&d)[P]) {
+  if (act == kSilu) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const Pair t = map(z[i], tanh_of);
+        d[i] = fma(d[i], fma(z[i], fma(t * Pair(-1.f), t, Pair(1.f)), t), d[i]);
+      } else {
+        const Pair s = sigmoid(z[i]);
+        d[i] = d[i] * fma(z[i], fma(s * Pair(-1.f), s, s), s);
+      }
+    }
+  } else if (act == kRelu) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const auto gate = [](float x, float g) { return x <= 0.f ? 0.f : x > 0.f ? g : x; };
+      float x, y, g, h;
+      z[i].get(x, y);
+      d[i].get(g, h);
+      d[i] = Pair(gate(x, g), gate(y, h));
+    }
+  } else if (act == kGelu) {
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      d[i] = d[i] * map(z[i], [](float x) { return normcdff(x) + x * .3989422804f * __expf(-.5f * x * x); });
   }
 }
 
 // What the threads of a CTA share.
 struct Shared {
-  float *red;       // [threads * V] (twice for the backward)
-  float *channel;   // [c] (twice)
-  float *group;     // [2][groups]
+  float *red;           // [threads * V] (twice for the backward)
+  float *channel;       // [c] (twice)
+  float *w, *b;         // [c]
   float *mean, *rstd;   // [groups]
+  float *sum_a, *sum_b; // [groups]
 };
 
 template <int V, bool BWD>
 __host__ __device__ inline int shared_floats(int threads, int c, int groups) {
-  return (BWD ? 2 : 1) * (threads * V + c) + 4 * groups;
+  return (BWD ? 2 : 1) * (threads * V + c) + 2 * c + 4 * groups;
 }
 template <int V, bool BWD>
 __device__ __forceinline__ Shared carve(float* at, int threads, int c, int groups) {
   Shared s;
   s.red = at;
-  at += (BWD ? 2 : 1) * threads * V;
-  s.channel = at;
-  at += (BWD ? 2 : 1) * c;
-  s.group = at;
-  s.mean = at + 2 * groups;
-  s.rstd = at + 3 * groups;
+  s.channel = s.red + (BWD ? 2 : 1) * threads * V;
+  s.w = s.channel + (BWD ? 2 : 1) * c;
+  s.b = s.w + c;
+  s.mean = s.b + c;
+  s.rstd = s.mean + groups;
+  s.sum_a = s.rstd + groups;
+  s.sum_b = s.sum_a + groups;
   return s;
+}
+// The parameters, and for the backward the sample's statistics, on their way while the data is.
+__device__ __forceinline__ void load_parameters(const Args& a, const Shared& s, int64_t sample) {
+  for (int c = threadIdx.x; c < a.c; c += blockDim.x) {
+    s.w[c] = parameter(a.a.w, a.a.w_type, c, 1.f);
+    s.b[c] = parameter(a.a.b, a.a.b_type, c, 0.f);
+  }
+  if (a.mean_in) {
+    for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
+      s.mean[g] = a.mean_in[sample * a.groups + g];
+      s.rstd[g] = a.rstd_in[sample * a.groups + g];
+    }
+  }
+}
+__device__ __forceinline__ void clear(float* p, int n) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) p[i] = 0.f;
 }
 
 // A thread's place: its column of the channels' pattern and its row, for the tile of columns from c0.
@@ -164,415 +269,523 @@ __device__ __forceinline__ Place place_of(const Args& a, int c0) {
   return p;
 }
 
-// Adds up v over the CTA's rows: channel[c] += the sum of the tile's values of channel c.
-template <int V>
-__device__ void join_rows(const Args& a, const Place& p, int c0, const float (&v)[V], float* red, float* channel) {
+// Adds up N numbers of each element over the CTA's rows: channel[k][c] += the
+// sum of the tile's k-th numbers of channel c. Some lanes (a power of two) share a channel.
+template <int V, int N>
+__device__ void join_rows(const Args& a, const Place& p, int c0, const Pair (&v)[N][(V + 1) / 2], float* red, float* channel) {
+  const int width = p.tile_cols * V, plane = p.tile_rows * width;
   if (p.active) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) red[(p.row * p.tile_cols + p.col) * V + i] = v[i];
-  }
-  __syncthreads();
-  const int width = p.tile_cols * V;
-  for (int left = p.tile_rows; left > 1;) {
-    const int half = (left + 1) >> 1;
-    for (int i = threadIdx.x; i < (left - half) * width; i += blockDim.x) red[i] += red[i + half * width];
-    left = half;
-    __syncthreads();
-  }
-  const int from = c0 * V;
-  for (int c = threadIdx.x; c < a.c; c += blockDim.x) {
-    float s = channel[c];
-    for (int q = c; q < from + width; q += a.c)
-      if (q >= from) s += red[q - from];
-    channel[c] = s;
-  }
-  __syncthreads();
-}
-
-// out[g] = the sum of channel[c] (times w_c) over the group's channels: a warp for each group.
-__device__ __forceinline__ void join_channels(const Args& a, const float* channel, bool weighted, float* out) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = a.c / a.groups;
-  for (int g = warp; g < a.groups; g += blockDim.x >> 5) {
-    float s = 0.f;
-    for (int i = lane; i < per; i += 32) {
-      const int c = g * per + i;
-      s += channel[c] * (weighted ? parameter(a.a.w, a.a.w_type, c, 1.f) : 1.f);
+    for (int k = 0; k < N; ++k) {
+      float* to = red + k * plane + (p.row * p.tile_cols + p.col) * V;
+#pragma unroll
+      for (int i = 0; i < (V + 1) / 2; ++i) {
+        float x, y;
+        v[k][i].get(x, y);
+        to[2 * i] = x;
+        if (V > 1) to[2 * i + 1] = y;
+      }
     }
-    s = lm::warp_sum(s);
-    if (lane == 0) out[g] = s;
   }
-}
-
-template <int V>
-__device__ __forceinline__ int channel_of(const Args& a, int c0, int col, int i) {
-  return (int)(((int64_t)(c0 + col) * V + i) % a.c);
-}
-
-// A CTA's part of a sample: vectors [begin, begin + count) and the first address.
-struct Part {
-  int64_t sample, begin, count;
-};
-__device__ __forceinline__ Part part_of(const Args& a, int ctas) {
-  Part p;
-  p.sample = blockIdx.x / ctas;
-  p.begin = (int64_t)(blockIdx.x - p.sample * ctas) * a.chunk;
-  p.count = max((int64_t)0, min(a.chunk, a.vectors - p.begin));
-  return p;
-}
-
-// f(k, i) for this thread's vectors i of its part in the tile of columns from c0, k counting its slots over all tiles.
-template <typename F>
-__device__ __forceinline__ void for_vectors(const Args& a, const Place& p, int c0, int64_t count, F&& f) {
-  if (!p.active) return;
-  const int64_t step = (int64_t)p.tile_rows * a.cols;
-  int k = c0 / (int)blockDim.x * a.iterations;
-  for (int64_t i = (int64_t)p.row * a.cols + c0 + p.col; i < count; i += step, ++k) f(k, i);
-}
-
-// Sums `v` of the group over the cluster's CTAs, in the order of their ranks.
-__device__ __forceinline__ void join_cluster(cg::cluster_group& cluster, float* mine, float* out, int n) {
-  cluster.sync();
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+  __syncthreads();
+  int share = 1;
+  while (share < 32 && share * 2 * N * a.c <= (int)blockDim.x) share *= 2;
+  const int from = c0 * V, part = threadIdx.x % share;
+  for (int at = threadIdx.x / share; at < N * a.c; at += blockDim.x / share) {
+    const int k = at / a.c, c = at - k * a.c;
     float s = 0.f;
-    for (unsigned r = 0; r < cluster.num_blocks(); ++r) s += cluster.map_shared_rank(mine, r)[i];
-    out[i] = s;
+    for (int q = c < from ? c + (from - c + a.c - 1) / a.c * a.c : c; q < from + width; q += a.c) {
+      const float* col = red + k * plane + q - from;
+#pragma unroll 4
+      for (int r = part; r < p.tile_rows; r += share) s += col[r * width];
+    }
+    for (int o = share >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(__activemask(), s, o);
+    if (part == 0) channel[at] += s;
   }
   __syncthreads();
 }
 
-// Forward. FULL: the cluster holds the sample and writes y. Otherwise a CTA
-// writes its part's (sum, sum of squares less its own mean's) of each group.
-template <typename T, int V, bool FULL>
-__global__ void __launch_bounds__(512) forward_kernel(const __grid_constant__ Args a) {
-  using Vector = Vec<T, V>;
-  extern __shared__ __align__(16) unsigned char raw[];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = FULL ? (int)cluster.num_blocks() : (int)gridDim.x / (int)a.n;
-  const Part part = part_of(a, ctas);
-  const int tiles = (a.cols + blockDim.x - 1) / blockDim.x;
-  Vector* slots = reinterpret_cast<Vector*>(raw);
-  const Shared s = carve<V, false>(reinterpret_cast<float*>(raw + sizeof(Vector) * blockDim.x * a.iterations * tiles),
-                                   blockDim.x, a.c, a.groups);
-  const Vector* x = static_cast<const Vector*>(a.x) + part.sample * a.vectors + part.begin;
+// out[g] = factor times the sum of channel[c] (times w_c) over the group's channels.
+__device__ __forceinline__ void join_channels(const Args& a, const float* channel, const float* w, float factor, float* out) {
   const int per = a.c / a.groups;
-  // all loads are under way before the first is waited for
-  for (int c0 = 0; c0 < a.cols; c0 += blockDim.x) {
-    const Place p = place_of(a, c0);
-    for_vectors(a, p, c0, part.count, [&](int k, int64_t i) { fetch(slots + k * blockDim.x + threadIdx.x, x + i); });
-  }
-  commit();
-  for (int c = threadIdx.x; c < a.c; c += blockDim.x) s.channel[c] = 0.f;
-  __syncthreads();
-  wait_for(0);
-  for (int c0 = 0; c0 < a.cols; c0 += blockDim.x) {
-    const Place p = place_of(a, c0);
-    float sum[V] = {};
-    for_vectors(a, p, c0, part.count, [&](int k, int64_t) {
-      float v[V];
-      slots[k * blockDim.x + threadIdx.x].get(v);
-#pragma unroll
-      for (int e = 0; e < V; ++e) sum[e] += v[e];
-    });
-    join_rows(a, p, c0, sum, s.red, s.channel);
-  }
-  join_channels(a, s.channel, false, s.group);
-  __syncthreads();
-  const float values = FULL ? (float)a.pixels * per : (float)((double)part.count * V / a.groups);
-  if (FULL) {
-    join_cluster(cluster, s.group, s.mean, a.groups);
-  } else {
-    for (int g = threadIdx.x; g < a.groups; g += blockDim.x) s.mean[g] = s.group[g];
-    __syncthreads();
-  }
-  for (int g = threadIdx.x; g < a.groups; g += blockDim.x) s.mean[g] = values > 0.f ? s.mean[g] / values : 0.f;
-  for (int c = threadIdx.x; c < a.c; c += blockDim.x) s.channel[c] = 0.f;
-  __syncthreads();
-  for (int c0 = 0; c0 < a.cols; c0 += blockDim.x) {
-    const Place p = place_of(a, c0);
-    float sum[V] = {}, mean[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) mean[e] = p.active ? s.mean[channel_of<V>(a, c0, p.col, e) / per] : 0.f;
-    for_vectors(a, p, c0, part.count, [&](int k, int64_t) {
-      float v[V];
-      slots[k * blockDim.x + threadIdx.x].get(v);
-#pragma unroll
-      for (int e = 0; e < V; ++e) sum[e] += (v[e] - mean[e]) * (v[e] - mean[e]);
-    });
-    join_rows(a, p, c0, sum, s.red, s.channel);
-  }
-  join_channels(a, s.channel, false, s.group + a.groups);
-  __syncthreads();
-  if (!FULL) {
-    float* to = a.ws + blockIdx.x * (int64_t)a.groups * 2;
+  if (per <= 32) {   // a thread for each group
     for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
-      to[2 * g] = s.mean[g];
-      to[2 * g + 1] = s.group[a.groups + g];
+      float s = 0.f;
+      for (int c = g * per; c < (g + 1) * per; ++c) s += w ? channel[c] * w[c] : channel[c];
+      out[g] = s * factor;
     }
     return;
   }
-  join_cluster(cluster, s.group + a.groups, s.rstd, a.groups);
+  const int lane = threadIdx.x & 31;
+  for (int g = threadIdx.x >> 5; g < a.groups; g += blockDim.x >> 5) {
+    float s = 0.f;
+    for (int c = g * per + lane; c < (g + 1) * per; c += 32) s += w ? channel[c] * w[c] : channel[c];
+    s = lm::warp_sum(s);
+    if (lane == 0) out[g] = s * factor;
+  }
+}
+
+// A CTA's part of a sample: vectors [begin, begin + count).
+struct Part {
+  int64_t sample, begin, at;   // at: the part's place among all samples' parts
+  int count;
+};
+__device__ __forceinline__ int64_t part_size(const Args& a, int64_t i) {
+  return max((int64_t)0, min(a.chunk, a.vectors - i * a.chunk));
+}
+__device__ __forceinline__ Part part_of(const Args& a, uint32_t block) {
+  Part p;
+  const uint32_t sample = block / (uint32_t)a.ctas, i = block - sample * (uint32_t)a.ctas;
+  p.sample = sample;
+  p.begin = (int64_t)i * a.chunk;
+  p.at = block;
+  p.count = (int)part_size(a, i);
+  return p;
+}
+
+// f(slot, i) for this thread's vectors i of its part in the tile of columns
+// from c0; its slots are `blockDim.x` apart, over all tiles.
+template <typename F>
+__device__ __forceinline__ void for_vectors(const Args& a, const Place& p, int c0, int count, F&& f) {
+  if (!p.active) return;
+  const int step = p.tile_rows * a.cols;
+  int slot = c0 / (int)blockDim.x * a.iterations * (int)blockDim.x + (int)threadIdx.x;
+#pragma unroll 2
+  for (int i = p.row * a.cols + c0 + p.col; i < count; i += step, slot += (int)blockDim.x) f(slot, i);
+}
+// f(vectors, i) for the same vectors of N tensors, which are under way D ahead in the thread's slots.
+template <int D, int N, typename Vector, typename F>
+__device__ __forceinline__ void for_ahead(const Args& a, const Place& p, int c0, int count, Vector* ring,
+                                          const Vector* const (&from)[N], F&& f) {
+  if (!p.active) return;
+  const int step = p.tile_rows * a.cols, start = p.row * a.cols + c0 + p.col, threads = (int)blockDim.x;
+  Vector* mine = ring + threadIdx.x;
+  int next = start;
+#pragma unroll
+  for (int k = 0; k < D - 1; ++k, next += step) {
+    if (next < count) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) fetch(mine + (k * N + n) * threads, from[n] + next);
+    }
+    commit();
+  }
+  int at = 0, to = D - 1;
+  for (int i = start; i < count; i += step, next += step) {
+    asm volatile("cp.async.wait_group %0;" :: "n"(D - 2) : "memory");
+    Vector v[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = mine[(at * N + n) * threads];
+    if (next < count) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) fetch(mine + (to * N + n) * threads, from[n] + next);
+    }
+    commit();
+    at = at + 1 == D ? 0 : at + 1;
+    to = to + 1 == D ? 0 : to + 1;
+    f(v, i);
+  }
+  wait_all();   // nothing is under way when the slots are filled anew
+}
+// f(channel, group) of each of a vector's elements, as pairs: one division for
+// the first element, the others count on.
+template <int V, typename F>
+__device__ __forceinline__ void of_channels(const Args& a, const Place& p, int c0, Pair (&out)[(V + 1) / 2], F&& f) {
+  const int per = a.c / a.groups;
+  int c = p.active ? (c0 + p.col) * V % a.c : 0, g = c / per, left = per - (c - g * per);
+  float x[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    x[i] = f(c, g);
+    ++c;
+    if (--left == 0) left = per, ++g;
+    if (c == a.c) c = 0, g = 0;
+  }
+#pragma unroll
+  for (int i = 0; i < (V + 1) / 2; ++i) out[i] = Pair(x[2 * i], V == 1 ? 0.f : x[V == 1 ? 0 : 2 * i + 1]);
+}
+
+// y of a vector, with the means and deviations of a sample's groups.
+template <typename T, int V>
+struct Normalise {
+  static constexpr int P = (V + 1) / 2;
+  Pair mean[P], scale[P], shift[P];
+  __device__ __forceinline__ Normalise(const Args& a, const Place& p, int c0, const Shared& s) {
+    const float h = halved<T>(a.act);
+    of_channels<V>(a, p, c0, mean, [&](int, int g) { return -s.mean[g]; });
+    of_channels<V>(a, p, c0, scale, [&](int c, int g) { return s.rstd[g] * s.w[c] * h; });
+    of_channels<V>(a, p, c0, shift, [&](int c, int) { return s.b[c] * h; });
+  }
+  __device__ __forceinline__ Vec<T, V> operator()(int act, const Vec<T, V>& x) const {
+    Pair v[P];
+    x.get(v);
+#pragma unroll
+    for (int e = 0; e < P; ++e) v[e] = fma(v[e] + mean[e], scale[e], shift[e]);
+    activate<T>(act, v);
+    Vec<T, V> y;
+    y.set(v);
+    return y;
+  }
+};
+
+// The means of the groups of the `count` vectors that walk() goes through, and
+// the sums of their squares about them (in s.mean and s.rstd), in one pass:
+// of each channel's values less the first that the thread meets, and of their
+// squares. Whatever that first value is, its own square is among the sums, so
+// that a thread's cancellation is at most the number of its values. (Channels
+// that take several tiles of columns are read twice, once for the means.)
+template <typename T, int V, typename F>
+__device__ __forceinline__ void statistics(const Args& a, int count, const Shared& s, F&& walk) {
+  constexpr int P = (V + 1) / 2;
+  const bool one = a.cols <= (int)blockDim.x;
+  const float inv_values = count ? (float)a.groups / ((float)count * V) : 0.f;
+  for (int pass = one ? 1 : 0; pass < 2; ++pass) {
+    clear(s.channel, a.c);
+    __syncthreads();
+    for (int c0 = 0; c0 < a.cols; c0 += blockDim.x) {
+      const Place p = place_of(a, c0);
+      Pair base[P], sum[P], square[P], v[1][P];
+      int n = 0;
+      walk(p, c0, [&](const Vec<T, V>& in) {
+        Pair x[P];
+        in.get(x);
+        if (n++ == 0) {
+#pragma unroll
+          for (int e = 0; e < P; ++e) base[e] = x[e] * Pair(-1.f);
+        }
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const Pair d = x[e] + base[e];
+          sum[e] = sum[e] + d;
+          square[e] = fma(d, d, square[e]);
+        }
+      });
+      const Pair number((float)n), inv(n ? 1.f / n : 0.f);
+      if (one || pass == 0) {   // the sums: the base n times, and the differences
+#pragma unroll
+        for (int e = 0; e < P; ++e) v[0][e] = fma(base[e] * Pair(-1.f), number, sum[e]);
+        join_rows<V, 1>(a, p, c0, v, s.red, s.channel);
+      }
+      if (one) {
+        join_channels(a, s.channel, nullptr, inv_values, s.mean);
+        __syncthreads();
+        clear(s.channel, a.c);
+        __syncthreads();
+      }
+      if (pass == 1) {   // squares about the thread's mean, and those of that mean about the part's
+        of_channels<V>(a, p, c0, v[0], [&](int, int g) { return -s.mean[g]; });
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const Pair off = fma(sum[e], inv, base[e] * Pair(-1.f)) + v[0][e];
+          v[0][e] = fma(off * off, number, fma(sum[e] * inv * Pair(-1.f), sum[e], square[e]));
+        }
+        join_rows<V, 1>(a, p, c0, v, s.red, s.channel);
+      }
+    }
+    if (pass == 0) {
+      join_channels(a, s.channel, nullptr, inv_values, s.mean);
+      __syncthreads();
+    }
+  }
+  join_channels(a, s.channel, nullptr, 1.f, s.rstd);
+  __syncthreads();
+}
+
+// A sample in a CTA's shared memory.
+template <typename T, int V>
+__global__ void __launch_bounds__(512) forward_kernel(const __grid_constant__ Args a) {
+  using Vector = Vec<T, V>;
+  extern __shared__ __align__(16) unsigned char raw[];
+  const int64_t sample = blockIdx.x;
+  const int tiles = (a.cols + blockDim.x - 1) / blockDim.x, count = (int)a.vectors;
+  Vector* slots = reinterpret_cast<Vector*>(raw);
+  const Shared s = carve<V, false>(reinterpret_cast<float*>(raw + sizeof(Vector) * blockDim.x * a.iterations * tiles),
+                                   blockDim.x, a.c, a.groups);
+  const Vector* x = static_cast<const Vector*>(a.x) + sample * a.vectors;
+  for (int c0 = 0; c0 < a.cols; c0 += blockDim.x)
+    for_vectors(a, place_of(a, c0), c0, count, [&](int slot, int i) { fetch(slots + slot, x + i); });
+  commit();
+  load_parameters(a, s, sample);
+  wait_all();
+  statistics<T, V>(a, count, s, [&](const Place& p, int c0, auto&& f) {
+    for_vectors(a, p, c0, count, [&](int slot, int) { f(slots[slot]); });
+  });
+  const float values = (float)a.pixels * (a.c / a.groups);
   for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
     s.rstd[g] = rsqrtf(s.rstd[g] / values + a.eps);
-    if (a.mean && cluster.block_rank() == 0) {
+    if (a.mean) {
+      a.mean[sample * a.groups + g] = s.mean[g];
+      a.rstd[sample * a.groups + g] = s.rstd[g];
+    }
+  }
+  __syncthreads();
+  Vector* y = static_cast<Vector*>(a.y) + sample * a.vectors;
+  for (int c0 = 0; c0 < a.cols; c0 += blockDim.x) {
+    const Place p = place_of(a, c0);
+    const Normalise<T, V> norm(a, p, c0, s);
+    for_vectors(a, p, c0, count, [&](int slot, int i) { y[i] = norm(a.act, slots[slot]); });
+  }
+}
+
+// A write that nothing here reads again.
+template <typename T, int V>
+__device__ __forceinline__ void last_write(Vec<T, V>* p, const Vec<T, V>& r) {
+  if constexpr (sizeof(r) == 16) __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&r));
+  else if constexpr (sizeof(r) == 8) __stcs(reinterpret_cast<uint2*>(p), *reinterpret_cast<const uint2*>(&r));
+  else *p = r;
+}
+// Vectors of N tensors that a thread keeps under way: 24 KB of a CTA of 256.
+template <int N>
+constexpr int kAhead = 6;
+
+// The mean and 1 / deviation of a sample's groups from its parts' means and
+// squares, some lanes for each group: the parts' means less the first one's,
+// and their squares, in one pass.
+__device__ __forceinline__ void merge_parts(const Args& a, int64_t sample, int vec, const Shared& s) {
+  const int lanes = a.groups * 32 <= (int)blockDim.x ? 32 : 8, part = threadIdx.x % lanes;
+  const float inv = 1.f / ((float)a.pixels * (float)(a.c / a.groups)), each = (float)vec / a.groups;
+  const float2* from = reinterpret_cast<const float2*>(a.ws) + sample * a.ctas * a.groups;
+  const float whole = (float)part_size(a, 0) * each, rest = (float)part_size(a, a.ctas - 1) * each;
+  for (int g0 = 0; g0 < a.groups; g0 += blockDim.x / lanes) {
+    const int g = g0 + threadIdx.x / lanes;
+    float first = 0.f, sum = 0.f, square = 0.f, own = 0.f;
+    if (g < a.groups) {
+      first = from[g].x;
+#pragma unroll 8
+      for (int i = part; i < a.ctas; i += lanes) {
+        const float2 m = from[(int64_t)i * a.groups + g];
+        const float n = i == a.ctas - 1 ? rest : whole, d = m.x - first;
+        sum += n * d;
+        square += n * d * d;
+        own += m.y;
+      }
+    }
+    for (int o = lanes >> 1; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      square += __shfl_xor_sync(0xffffffffu, square, o);
+      own += __shfl_xor_sync(0xffffffffu, own, o);
+    }
+    if (part == 0 && g < a.groups) {
+      s.mean[g] = first + sum * inv;
+      s.rstd[g] = rsqrtf(fmaxf(own + (square - sum * sum * inv), 0.f) * inv + a.eps);
+    }
+  }
+  __syncthreads();
+}
+
+// The statistics of a sample's part.
+template <typename T, int V>
+__global__ void __launch_bounds__(512) statistics_kernel(const __grid_constant__ Args a) {
+  using Vector = Vec<T, V>;
+  extern __shared__ __align__(16) unsigned char raw[];
+  Vector* ring = reinterpret_cast<Vector*>(raw);
+  const Shared s = carve<V, false>(reinterpret_cast<float*>(ring + kAhead<1> * blockDim.x), blockDim.x, a.c, a.groups);
+  const Part part = part_of(a, blockIdx.x);
+  const Vector* const x[1] = {static_cast<const Vector*>(a.x) + part.sample * a.vectors + part.begin};
+  statistics<T, V>(a, part.count, s, [&](const Place& p, int c0, auto&& f) {
+    for_ahead<kAhead<1>>(a, p, c0, part.count, ring, x, [&](const Vector (&v)[1], int) { f(v[0]); });
+  });
+  float* to = a.ws + part.at * a.groups * 2;
+  for (int g = threadIdx.x; g < a.groups; g += blockDim.x) to[2 * g] = s.mean[g], to[2 * g + 1] = s.rstd[g];
+}
+// y of a part from its sample's statistics.
+template <typename T, int V>
+__global__ void __launch_bounds__(512) apply_kernel(const __grid_constant__ Args a) {
+  using Vector = Vec<T, V>;
+  extern __shared__ __align__(16) unsigned char raw[];
+  Vector* ring = reinterpret_cast<Vector*>(raw);
+  const Shared s = carve<V, false>(reinterpret_cast<float*>(ring + kAhead<1> * blockDim.x), blockDim.x, a.c, a.groups);
+  const Part part = part_of(a, gridDim.x - 1 - blockIdx.x);
+  load_parameters(a, s, part.sample);
+  merge_parts(a, part.sample, V, s);
+  if (a.mean && part.begin == 0) {
+    for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
       a.mean[part.sample * a.groups + g] = s.mean[g];
       a.rstd[part.sample * a.groups + g] = s.rstd[g];
     }
   }
-  __syncthreads();
+  const Vector* const x[1] = {static_cast<const Vector*>(a.x) + part.sample * a.vectors + part.begin};
   Vector* y = static_cast<Vector*>(a.y) + part.sample * a.vectors + part.begin;
   for (int c0 = 0; c0 < a.cols; c0 += blockDim.x) {
     const Place p = place_of(a, c0);
-    float mean[V], scale[V], shift[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = p.active ? channel_of<V>(a, c0, p.col, e) : 0;
-      mean[e] = s.mean[c / per];
-      scale[e] = s.rstd[c / per] * parameter(a.a.w, a.a.w_type, c, 1.f);
-      shift[e] = parameter(a.a.b, a.a.b_type, c, 0.f);
-    }
-    for_vectors(a, p, c0, part.count, [&](int k, int64_t i) {
-      float v[V];
-      slots[k * blockDim.x + threadIdx.x].get(v);
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = (v[e] - mean[e]) * scale[e] + shift[e];
-      activate(a.act, v);
-      Vector o;
-      o.set(v);
-      y[i] = o;
-    });
-  }
-  cluster.sync();   // no CTA ends while another reads its sums
-}
-
-// Means and deviations of the samples from their parts' (Chan, Golub & LeVeque, 1979): a warp for each (sample, group).
-__global__ void merge_kernel(const __grid_constant__ Args a, int ctas, int vec) {
-  const int64_t at = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (at >= a.n * a.groups) return;
-  const int lane = threadIdx.x & 31, g = (int)(at % a.groups);
-  const float* from = a.ws + at / a.groups * ctas * a.groups * 2 + 2 * g;
-  const auto count = [&](int i) {
-    return (float)((double)max((int64_t)0, min(a.chunk, a.vectors - i * a.chunk)) * vec / a.groups);
-  };
-  const float all = (float)a.pixels * (float)(a.c / a.groups);
-  float s = 0.f;
-  for (int i = lane; i < ctas; i += 32) s += from[(int64_t)i * a.groups * 2] * (count(i) / all);
-  const float mean = lm::warp_sum(s);
-  s = 0.f;
-  for (int i = lane; i < ctas; i += 32) {
-    const float d = from[(int64_t)i * a.groups * 2] - mean;
-    s += from[(int64_t)i * a.groups * 2 + 1] + d * d * count(i);
-  }
-  const float var = lm::warp_sum(s) / all;
-  if (lane == 0) {
-    a.mean[at] = mean;
-    a.rstd[at] = rsqrtf(var + a.eps);
+    const Normalise<T, V> norm(a, p, c0, s);
+    for_ahead<kAhead<1>>(a, p, c0, part.count, ring, x,
+                         [&](const Vector (&v)[1], int i) { last_write(y + i, norm(a.act, v[0])); });
   }
 }
 
+// x less its mean and dz (over halved()) of a thread's vectors.
 template <typename T, int V>
-__global__ void __launch_bounds__(512) apply_kernel(const __grid_constant__ Args a) {
-  using Vector = Vec<T, V>;
-  const Part part = part_of(a, (int)gridDim.x / (int)a.n);
-  const int per = a.c / a.groups;
-  const Vector* x = static_cast<const Vector*>(a.x) + part.sample * a.vectors + part.begin;
-  Vector* y = static_cast<Vector*>(a.y) + part.sample * a.vectors + part.begin;
-  for (int c0 = 0; c0 < a.cols; c0 += blockDim.x) {
-    const Place p = place_of(a, c0);
-    float mean[V], scale[V], shift[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = p.active ? channel_of<V>(a, c0, p.col, e) : 0;
-      const int64_t g = part.sample * a.groups + c / per;
-      mean[e] = a.mean[g];
-      scale[e] = a.rstd[g] * parameter(a.a.w, a.a.w_type, c, 1.f);
-      shift[e] = parameter(a.a.b, a.a.b_type, c, 0.f);
-    }
-    for_vectors(a, p, c0, part.count, [&](int, int64_t i) {
-      const Vector in = x[i];
-      float v[V];
-      in.get(v);
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = (v[e] - mean[e]) * scale[e] + shift[e];
-      activate(a.act, v);
-      Vector o;
-      o.set(v);
-      y[i] = o;
-    });
+struct Derive {
+  static constexpr int P = (V + 1) / 2;
+  Pair mean[P], scale[P], shift[P];
+  __device__ __forceinline__ Derive(const Args& a, const Place& p, int c0, const Shared& s) {
+    const float h = halved<T>(a.act);
+    of_channels<V>(a, p, c0, mean, [&](int, int g) { return -s.mean[g]; });
+    of_channels<V>(a, p, c0, scale, [&](int c, int g) { return s.rstd[g] * s.w[c] * h; });
+    of_channels<V>(a, p, c0, shift, [&](int c, int) { return s.b[c] * h; });
   }
-}
-
-// A thread's parameters of its channels in the backward.
-template <int V>
-struct Channels {
-  float mean[V], rstd[V], w[V], b[V];
-  int c[V];
-  __device__ __forceinline__ Channels(const Args& a, const Place& p, int c0, int64_t sample) {
-    const int per = a.c / a.groups;
+  __device__ __forceinline__ void operator()(int act, const Vec<T, V>& vx, const Vec<T, V>& vd, Pair (&x)[P], Pair (&d)[P]) const {
+    vx.get(x);
+    vd.get(d);
+    Pair z[P];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      c[e] = p.active ? channel_of<V>(a, c0, p.col, e) : 0;
-      const int64_t g = sample * a.groups + c[e] / per;
-      mean[e] = a.mean_in[g];
-      rstd[e] = a.rstd_in[g];
-      w[e] = parameter(a.a.w, a.a.w_type, c[e], 1.f);
-      b[e] = parameter(a.a.b, a.a.b_type, c[e], 0.f);
+    for (int e = 0; e < P; ++e) {
+      x[e] = x[e] + mean[e];
+      z[e] = fma(x[e], scale[e], shift[e]);
     }
+    slope<T>(act, z, d);
   }
-  // x becomes x^, d (the gradient of y) becomes dz
-  __device__ __forceinline__ void derive(int act, float (&x)[V], float (&d)[V]) const {
-    float z[V];
+};
+// dx = rstd w dz - rstd A / m - (x - mean) rstd^2 B / m
+template <typename T, int V>
+struct InputGradient {
+  static constexpr int P = (V + 1) / 2;
+  Derive<T, V> derive;
+  Pair by_dz[P], by_x[P], at[P];
+  __device__ __forceinline__ InputGradient(const Args& a, const Place& p, int c0, const Shared& s) : derive(a, p, c0, s) {
+    const float inv = 1.f / ((float)a.pixels * (a.c / a.groups)), h = halved<T>(a.act);
+    of_channels<V>(a, p, c0, by_dz, [&](int c, int g) { return s.rstd[g] * s.w[c] * h; });
+    of_channels<V>(a, p, c0, by_x, [&](int, int g) { return -s.rstd[g] * s.rstd[g] * s.sum_b[g] * inv; });
+    of_channels<V>(a, p, c0, at, [&](int, int g) { return -s.rstd[g] * s.sum_a[g] * inv; });
+  }
+  __device__ __forceinline__ Vec<T, V> operator()(int act, const Vec<T, V>& vx, const Vec<T, V>& vd) const {
+    Pair x[P], d[P];
+    derive(act, vx, vd, x, d);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      x[e] = (x[e] - mean[e]) * rstd[e];
-      z[e] = x[e] * w[e] + b[e];
-    }
-    slope(act, z, d);
+    for (int e = 0; e < P; ++e) d[e] = fma(by_dz[e], d[e], fma(x[e], by_x[e], at[e]));
+    Vec<T, V> o;
+    o.set(d);
+    return o;
   }
 };
 
-// dx of a vector from its x^ and dz and the group's A / m and B / m.
-template <int V>
-__device__ __forceinline__ void input_gradient(const Channels<V>& ch, const float (&ga)[V], const float (&gb)[V],
-                                               const float (&x)[V], float (&d)[V]) {
+// The sums P and Q (in s.channel) over the vectors that walk() goes through.
+template <typename T, int V, typename F>
+__device__ __forceinline__ void channel_sums(const Args& a, const Shared& s, F&& walk) {
+  constexpr int P = (V + 1) / 2;
+  for (int c0 = 0; c0 < a.cols; c0 += blockDim.x) {
+    const Place p = place_of(a, c0);
+    Pair sums[2][P];
+    {
+      const Derive<T, V> derive(a, p, c0, s);
+      walk(p, c0, [&](const Vec<T, V>& vx, const Vec<T, V>& vd) {
+        Pair x[P], d[P];
+        derive(a.act, vx, vd, x, d);
 #pragma unroll
-  for (int e = 0; e < V; ++e) d[e] = ch.rstd[e] * (ch.w[e] * d[e] - (ga[e] + x[e] * gb[e]));
+        for (int e = 0; e < P; ++e) {
+          sums[0][e] = sums[0][e] + d[e];
+          sums[1][e] = fma(d[e], x[e], sums[1][e]);
+        }
+      });
+    }
+    const float h = halved<T>(a.act);
+    Pair rstd[P];
+    of_channels<V>(a, p, c0, rstd, [&](int, int g) { return s.rstd[g] * h; });
+#pragma unroll
+    for (int e = 0; e < P; ++e) {
+      sums[0][e] = sums[0][e] * Pair(h);
+      sums[1][e] = sums[1][e] * rstd[e];
+    }
+    join_rows<V, 2>(a, p, c0, sums, s.red, s.channel);
+  }
 }
 
-// Backward. FULL: the cluster holds the sample's x and dy and writes dx.
-// Otherwise a CTA writes its part's P and Q of each channel.
-template <typename T, int V, bool FULL>
+// A sample's x and dy in a CTA's shared memory.
+template <typename T, int V>
 __global__ void __launch_bounds__(512) backward_kernel(const __grid_constant__ Args a) {
   using Vector = Vec<T, V>;
   extern __shared__ __align__(16) unsigned char raw[];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = FULL ? (int)cluster.num_blocks() : (int)gridDim.x / (int)a.n;
-  const Part part = part_of(a, ctas);
-  const int tiles = (a.cols + blockDim.x - 1) / blockDim.x;
-  const int held = FULL ? blockDim.x * a.iterations * tiles : 0;
+  const int64_t sample = blockIdx.x;
+  const int tiles = (a.cols + blockDim.x - 1) / blockDim.x, count = (int)a.vectors;
+  const int held = blockDim.x * a.iterations * tiles;
   Vector* slots = reinterpret_cast<Vector*>(raw);
   const Shared s = carve<V, true>(reinterpret_cast<float*>(raw + 2 * sizeof(Vector) * held), blockDim.x, a.c, a.groups);
-  const Vector* x = static_cast<const Vector*>(a.x) + part.sample * a.vectors + part.begin;
-  const Vector* dy = static_cast<const Vector*>(a.dy) + part.sample * a.vectors + part.begin;
-  const int per = a.c / a.groups;
-  if (FULL) {
-    for (int c0 = 0; c0 < a.cols; c0 += blockDim.x) {
-      const Place p = place_of(a, c0);
-      for_vectors(a, p, c0, part.count, [&](int k, int64_t i) {
-        fetch(slots + k * blockDim.x + threadIdx.x, x + i);
-        fetch(slots + held + k * blockDim.x + threadIdx.x, dy + i);
-      });
-    }
-    commit();
-  }
-  for (int c = threadIdx.x; c < 2 * a.c; c += blockDim.x) s.channel[c] = 0.f;
+  const Vector* x = static_cast<const Vector*>(a.x) + sample * a.vectors;
+  const Vector* dy = static_cast<const Vector*>(a.dy) + sample * a.vectors;
+  for (int c0 = 0; c0 < a.cols; c0 += blockDim.x)
+    for_vectors(a, place_of(a, c0), c0, count, [&](int slot, int i) {
+      fetch(slots + slot, x + i);
+      fetch(slots + held + slot, dy + i);
+    });
+  commit();
+  load_parameters(a, s, sample);
+  clear(s.channel, 2 * a.c);
+  wait_all();
   __syncthreads();
-  if (FULL) wait_for(0);
+  channel_sums<T, V>(a, s, [&](const Place& p, int c0, auto&& f) {
+    for_vectors(a, p, c0, count, [&](int slot, int) { f(slots[slot], slots[held + slot]); });
+  });
+  float* to = a.ws + sample * 2 * a.c;
+  for (int c = threadIdx.x; c < 2 * a.c; c += blockDim.x) to[c] = s.channel[c];
+  join_channels(a, s.channel, s.w, 1.f, s.sum_a);
+  join_channels(a, s.channel + a.c, s.w, 1.f, s.sum_b);
+  __syncthreads();
+  Vector* dx = static_cast<Vector*>(a.y) + sample * a.vectors;
   for (int c0 = 0; c0 < a.cols; c0 += blockDim.x) {
     const Place p = place_of(a, c0);
-    const Channels<V> ch(a, p, c0, part.sample);
-    float sp[V] = {}, sq[V] = {};
-    for_vectors(a, p, c0, part.count, [&](int k, int64_t i) {
-      float v[V], d[V];
-      const Vector vx = FULL ? slots[k * blockDim.x + threadIdx.x] : x[i];
-      const Vector vd = FULL ? slots[held + k * blockDim.x + threadIdx.x] : dy[i];
-      vx.get(v);
-      vd.get(d);
-      ch.derive(a.act, v, d);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        sp[e] += d[e];
-        sq[e] += d[e] * v[e];
-      }
-    });
-    join_rows(a, p, c0, sp, s.red, s.channel);
-    join_rows(a, p, c0, sq, s.red, s.channel + a.c);
+    const InputGradient<T, V> grad(a, p, c0, s);
+    for_vectors(a, p, c0, count, [&](int slot, int i) { dx[i] = grad(a.act, slots[slot], slots[held + slot]); });
   }
-  if (!FULL) {
-    float* to = a.ws + blockIdx.x * (int64_t)a.c * 2;
-    for (int c = threadIdx.x; c < 2 * a.c; c += blockDim.x) to[c] = s.channel[c];
-    return;
-  }
-  join_channels(a, s.channel, true, s.group);
-  join_channels(a, s.channel + a.c, true, s.group + a.groups);
-  __syncthreads();
-  join_cluster(cluster, s.group, s.mean, 2 * a.groups);   // A and B lie where mean and rstd would
-  if (a.sums) {   // this CTA's share of the channels
-    for (int c = cluster.block_rank() * blockDim.x + threadIdx.x; c < 2 * a.c; c += cluster.num_blocks() * blockDim.x) {
-      float v = 0.f;
-      for (unsigned r = 0; r < cluster.num_blocks(); ++r) v += cluster.map_shared_rank(s.channel, r)[c];
-      a.sums[part.sample * 2 * a.c + c] = v;
-    }
-  }
-  const float inv = 1.f / ((float)a.pixels * per);
-  Vector* dx = static_cast<Vector*>(a.y) + part.sample * a.vectors + part.begin;
-  for (int c0 = 0; c0 < a.cols; c0 += blockDim.x) {
-    const Place p = place_of(a, c0);
-    const Channels<V> ch(a, p, c0, part.sample);
-    float ga[V], gb[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      ga[e] = s.mean[ch.c[e] / per] * inv;
-      gb[e] = s.rstd[ch.c[e] / per] * inv;
-    }
-    for_vectors(a, p, c0, part.count, [&](int k, int64_t i) {
-      float v[V], d[V];
-      slots[k * blockDim.x + threadIdx.x].get(v);
-      slots[held + k * blockDim.x + threadIdx.x].get(d);
-      ch.derive(a.act, v, d);
-      input_gradient(ch, ga, gb, v, d);
-      Vector o;
-      o.set(d);
-      dx[i] = o;
-    });
-  }
-  cluster.sync();   // no CTA ends while another reads its sums
 }
 
-// sums[n][2][c] = the sum of the sample's parts, in their order.
-__global__ void join_parts_kernel(const __grid_constant__ Args a, int ctas) {
-  const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (at >= a.n * 2 * a.c) return;
-  const int64_t n = at / (2 * a.c), c = at - n * 2 * a.c;
-  const float* from = a.ws + n * ctas * 2 * a.c + c;
-  float s = 0.f;
-  for (int i = 0; i < ctas; ++i) s += from[(int64_t)i * 2 * a.c];
-  a.sums[at] = s;
-}
-
+// A part's P and Q of each channel.
 template <typename T, int V>
-__global__ void __launch_bounds__(512) input_gradient_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(512) sums_kernel(const __grid_constant__ Args a) {
   using Vector = Vec<T, V>;
   extern __shared__ __align__(16) unsigned char raw[];
-  float* group = reinterpret_cast<float*>(raw);   // [2][groups]
-  const Part part = part_of(a, (int)gridDim.x / (int)a.n);
-  const int per = a.c / a.groups;
-  join_channels(a, a.sums + part.sample * 2 * a.c, true, group);
-  join_channels(a, a.sums + part.sample * 2 * a.c + a.c, true, group + a.groups);
+  Vector* ring = reinterpret_cast<Vector*>(raw);
+  const Shared s = carve<V, true>(reinterpret_cast<float*>(ring + 2 * kAhead<2> * blockDim.x), blockDim.x, a.c, a.groups);
+  const Part part = part_of(a, blockIdx.x);
+  const Vector* const from[2] = {static_cast<const Vector*>(a.x) + part.sample * a.vectors + part.begin,
+                                 static_cast<const Vector*>(a.dy) + part.sample * a.vectors + part.begin};
+  load_parameters(a, s, part.sample);
+  clear(s.channel, 2 * a.c);
   __syncthreads();
-  const float inv = 1.f / ((float)a.pixels * per);
-  const Vector* x = static_cast<const Vector*>(a.x) + part.sample * a.vectors + part.begin;
-  const Vector* dy = static_cast<const Vector*>(a.dy) + part.sample * a.vectors + part.begin;
+  channel_sums<T, V>(a, s, [&](const Place& p, int c0, auto&& f) {
+    for_ahead<kAhead<2>>(a, p, c0, part.count, ring, from, [&](const Vector (&v)[2], int) { f(v[0], v[1]); });
+  });
+  float* to = a.ws + part.at * 2 * a.c;
+  for (int c = threadIdx.x; c < 2 * a.c; c += blockDim.x) to[c] = s.channel[c];
+}
+// dx of a part from its sample's sums.
+template <typename T, int V>
+__global__ void __launch_bounds__(512) gradient_kernel(const __grid_constant__ Args a) {
+  using Vector = Vec<T, V>;
+  extern __shared__ __align__(16) unsigned char raw[];
+  Vector* ring = reinterpret_cast<Vector*>(raw);
+  const Shared s = carve<V, true>(reinterpret_cast<float*>(ring + 2 * kAhead<2> * blockDim.x), blockDim.x, a.c, a.groups);
+  const Part part = part_of(a, gridDim.x - 1 - blockIdx.x);
+  const Vector* const in[2] = {static_cast<const Vector*>(a.x) + part.sample * a.vectors + part.begin,
+                               static_cast<const Vector*>(a.dy) + part.sample * a.vectors + part.begin};
+  load_parameters(a, s, part.sample);
+  const float* from = a.ws + part.sample * a.ctas * 2 * a.c;
+  // the parts' sums: as many threads for each channel as there are, every one over its share of the parts
+  const int share = max(1, min(a.ctas, (int)blockDim.x / (2 * a.c)));
+  for (int at = threadIdx.x; at < share * 2 * a.c; at += blockDim.x) {
+    const int c = at % (2 * a.c);
+    float v = 0.f;
+#pragma unroll 16
+    for (int i = at / (2 * a.c); i < a.ctas; i += share) v += from[(int64_t)i * 2 * a.c + c];
+    (share == 1 ? s.channel : s.red)[at] = v;
+  }
+  __syncthreads();
+  if (share > 1) {
+    for (int c = threadIdx.x; c < 2 * a.c; c += blockDim.x) {
+      float v = 0.f;
+      for (int i = 0; i < share; ++i) v += s.red[i * 2 * a.c + c];
+      s.channel[c] = v;
+    }
+    __syncthreads();
+  }
+  join_channels(a, s.channel, s.w, 1.f, s.sum_a);
+  join_channels(a, s.channel + a.c, s.w, 1.f, s.sum_b);
+  __syncthreads();
   Vector* dx = static_cast<Vector*>(a.y) + part.sample * a.vectors + part.begin;
   for (int c0 = 0; c0 < a.cols; c0 += blockDim.x) {
     const Place p = place_of(a, c0);
-    const Channels<V> ch(a, p, c0, part.sample);
-    float ga[V], gb[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      ga[e] = group[ch.c[e] / per] * inv;
-      gb[e] = group[a.groups + ch.c[e] / per] * inv;
-    }
-    for_vectors(a, p, c0, part.count, [&](int, int64_t i) {
-      float v[V], d[V];
-      const Vector vx = x[i], vd = dy[i];
-      vx.get(v);
-      vd.get(d);
-      ch.derive(a.act, v, d);
-      input_gradient(ch, ga, gb, v, d);
-      Vector o;
-      o.set(d);
-      dx[i] = o;
-    });
+    const InputGradient<T, V> grad(a, p, c0, s);
+    for_ahead<kAhead<2>>(a, p, c0, part.count, ring, in,
+                         [&](const Vector (&v)[2], int i) { last_write(dx + i, grad(a.act, v[0], v[1])); });
   }
 }
 
@@ -605,11 +818,11 @@ __global__ void __launch_bounds__(512) parameters_kernel(const float* sums, int6
   }
 }
 
-template <typename F>
+template <bool BWD, typename F>
 void with_vector(const Shape& s, const Plan& p, F&& f) {
   const auto by = [&](auto t) {
     using T = decltype(t);
-    if constexpr (sizeof(T) == 2)
+    if constexpr (sizeof(T) == 2 && !BWD)
       if (p.vec == 8) return f(t, std::integral_constant<int, 8>{});
     if (p.vec == 4) return f(t, std::integral_constant<int, 4>{});
     return f(t, std::integral_constant<int, 1>{});
@@ -630,31 +843,21 @@ Args args_of(const Shape& s, const Plan& p) {
   a.cols = p.cols;
   a.rows = p.rows;
   a.iterations = p.iterations;
+  a.ctas = p.ctas;
   return a;
 }
 
 template <typename... A>
-cudaError_t run(void (*kernel)(A...), int64_t grid, int threads, int cluster, int smem, cudaStream_t st, A... args) {
+cudaError_t run(void (*kernel)(A...), int64_t grid, int threads, int smem, cudaStream_t st, A... args) {
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = cluster;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
+  kernel<<<(unsigned)grid, threads, smem, st>>>(args...);
+  return cudaGetLastError();
 }
 
-constexpr int kMostSmem = 200 * 1024;   // of a CTA
-constexpr int kMostCtas = 8;            // of a cluster
+constexpr int kMostSmem = 75 * 1024;              // of a CTA that holds a sample: three fit an SM
 
 int shared_bytes(const Shape& s, int vec, int threads, bool backward) {
   const int f = vec == 8 ? (backward ? shared_floats<8, true>(threads, s.c, s.groups) : shared_floats<8, false>(threads, s.c, s.groups))
@@ -667,7 +870,8 @@ int shared_bytes(const Shape& s, int vec, int threads, bool backward) {
 
 Plan plan(const Shape& s, bool backward, bool aligned, int sms) {
   Plan p{};
-  const int size = s.type == 0 ? 4 : 2, most = 16 / size;
+  // (the backward holds seven numbers for each element of an access: four elements at most)
+  const int size = s.type == 0 ? 4 : 2, most = backward ? 4 : 16 / size;
   const int64_t values = s.pixels * s.c;
   p.vec = aligned && values % most == 0 ? most : aligned && values % 4 == 0 ? 4 : 1;
   p.cols = s.c / std::gcd(s.c, p.vec);
@@ -685,36 +889,33 @@ Plan plan(const Shape& s, bool backward, bool aligned, int sms) {
   const int64_t vectors = values / p.vec;
   const int64_t all_rows = (vectors + p.cols - 1) / p.cols;   // the last may be cut
   const int fixed = shared_bytes(s, p.vec, p.threads, backward);
-  const auto cut = [&](int ctas) {
-    p.ctas = ctas;
+  const auto cut = [&](int64_t ctas) {
     const int64_t rows = (all_rows + ctas - 1) / ctas;
+    p.ctas = (int)((all_rows + rows - 1) / rows);
     p.iterations = (int)std::min<int64_t>((rows + p.rows - 1) / p.rows, 1 << 30);
     p.chunk = rows * p.cols;
-    return (int64_t)(backward ? 2 : 1) * p.vec * size * p.threads * p.iterations * tiles + fixed;
   };
-  for (int ctas = 1; ctas <= kMostCtas; ctas *= 2) {
-    const int64_t bytes = cut(ctas);
-    const bool last = ctas == kMostCtas;
-    if (bytes <= (last ? kMostSmem : 72 * 1024) && (last || s.n * ctas >= 2 * sms || bytes < 16 * 1024)) {
+  const int64_t sample = values * size * (backward ? 2 : 1);
+  if (sample <= kMostSmem) {
+    cut(1);
+    const int64_t bytes = (int64_t)(backward ? 2 : 1) * p.vec * size * p.threads * p.iterations * tiles + fixed;
+    // (few samples of any size are faster by parts, which more SMs share)
+    if (bytes <= kMostSmem && (s.n * 2 >= sms || sample <= 16 * 1024)) {
       p.resident = true;
       p.smem = (int)bytes;
       return p;
     }
   }
-  // parts that are read again: enough of them for all SMs, of at least 16 iterations
-  const int64_t most_ctas = std::max<int64_t>(1, all_rows / (p.rows * 16));
-  const int64_t fits = (kMostSmem / 2 - fixed) / ((int64_t)p.vec * size * p.threads * tiles);   // iterations that the forward's sums hold
-  const int64_t least = (all_rows + fits * p.rows - 1) / (fits * p.rows);
-  cut((int)std::max<int64_t>(least, std::min<int64_t>(most_ctas, (8 * sms + s.n - 1) / s.n)));
   p.resident = false;
-  p.smem = backward ? fixed : (int)((int64_t)p.vec * size * p.threads * p.iterations * tiles + fixed);
+  p.smem = fixed + (backward ? 2 * kAhead<2> : kAhead<1>) * p.vec * size * p.threads;
+  // parts of 64 iterations of a CTA, or fewer where that would leave SMs without three
+  const int64_t least = (all_rows + p.rows * 64 - 1) / (p.rows * 64), finest = (all_rows + p.rows * 2 - 1) / (p.rows * 2);
+  cut(std::max(least, std::min<int64_t>(finest, (3 * sms + s.n - 1) / s.n)));
   return p;
 }
 
 int64_t forward_workspace(const Shape& s, const Plan& p) { return p.resident ? 0 : s.n * p.ctas * s.groups * 2; }
-int64_t backward_workspace(const Shape& s, const Plan& p) {
-  return s.n * 2 * s.c * (p.resident ? 1 : 1 + (int64_t)p.ctas);
-}
+int64_t backward_workspace(const Shape& s, const Plan& p) { return s.n * 2 * s.c * (p.resident ? 1 : p.ctas); }
 
 cudaError_t forward(const Shape& s, const Plan& p, const void* x, const Affine& affine, float eps, Activation act, void* y,
                     float* mean, float* rstd, float* workspace, cudaStream_t st) {
@@ -728,16 +929,15 @@ cudaError_t forward(const Shape& s, const Plan& p, const void* x, const Affine& 
   a.rstd = rstd;
   a.ws = workspace;
   cudaError_t e = cudaSuccess;
-  with_vector(s, p, [&](auto t, auto v) {
+  with_vector<false>(s, p, [&](auto t, auto v) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
     if (p.resident) {
-      e = run(forward_kernel<T, V, true>, s.n * p.ctas, p.threads, p.ctas, p.smem, st, a);
+      e = run(forward_kernel<T, V>, s.n, p.threads, p.smem, st, a);
       return;
     }
-    e = run(forward_kernel<T, V, false>, s.n * p.ctas, p.threads, 1, p.smem, st, a);
-    if (e == cudaSuccess) e = run(merge_kernel, (s.n * s.groups + 7) / 8, 256, 1, 0, st, a, p.ctas, p.vec);
-    if (e == cudaSuccess) e = run(apply_kernel<T, V>, s.n * p.ctas, p.threads, 1, 0, st, a);
+    e = run(statistics_kernel<T, V>, s.n * p.ctas, p.threads, p.smem, st, a);
+    if (e == cudaSuccess) e = run(apply_kernel<T, V>, s.n * p.ctas, p.threads, p.smem, st, a);
   });
   return e;
 }
@@ -752,28 +952,26 @@ cudaError_t backward(const Shape& s, const Plan& p, const void* dy, const void* 
   a.act = act;
   a.mean_in = mean;
   a.rstd_in = rstd;
-  a.sums = workspace;
-  a.ws = workspace + s.n * 2 * s.c;
+  a.ws = workspace;
   cudaError_t e = cudaSuccess;
-  with_vector(s, p, [&](auto t, auto v) {
+  with_vector<true>(s, p, [&](auto t, auto v) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
     if (p.resident) {
-      e = run(backward_kernel<T, V, true>, s.n * p.ctas, p.threads, p.ctas, p.smem, st, a);
+      e = run(backward_kernel<T, V>, s.n, p.threads, p.smem, st, a);
       return;
     }
-    e = run(backward_kernel<T, V, false>, s.n * p.ctas, p.threads, 1, p.smem, st, a);
-    if (e == cudaSuccess) e = run(join_parts_kernel, (s.n * 2 * s.c + 255) / 256, 256, 1, 0, st, a, p.ctas);
-    if (e == cudaSuccess) e = run(input_gradient_kernel<T, V>, s.n * p.ctas, p.threads, 1, s.groups * 8, st, a);
+    e = run(sums_kernel<T, V>, s.n * p.ctas, p.threads, p.smem, st, a);
+    if (e == cudaSuccess) e = run(gradient_kernel<T, V>, s.n * p.ctas, p.threads, p.smem, st, a);
   });
   if (e == cudaSuccess && (dw || db))
-    e = run(parameters_kernel, (2 * s.c + 7) / 8, 512, 1, 0, st, (const float*)workspace, s.n, s.c, dw, affine.w_type, db,
-            affine.b_type);
+    e = run(parameters_kernel, (2 * s.c + 7) / 8, 512, 0, st, (const float*)workspace, p.resident ? s.n : s.n * p.ctas, s.c, dw,
+            affine.w_type, db, affine.b_type);
   return e;
 }
 
-int launches(const Plan& p, bool backward, bool parameters) {
-  return (p.resident ? 1 : 3) + (backward && parameters ? 1 : 0);
+int launches(const Plan& p, bool parameters) {
+  return (p.resident ? 1 : 2) + parameters;
 }
 
 }  // namespace groupnorm

@@ -20,10 +20,10 @@ struct Shape {
 struct Plan {
   int vec;            // elements of an access
   int threads, cols, rows;   // vectors that repeat the channels' pattern; such rows that a CTA takes at a time
-  int ctas;           // that share a sample
-  int64_t chunk;      // vectors of a CTA's part, a multiple of cols
+  int ctas;           // parts of a sample, a CTA's each
+  int64_t chunk;      // vectors of a part, a multiple of cols
   int iterations;     // of a thread over its part
-  bool resident;      // a cluster holds the sample in shared memory
+  bool resident;      // a CTA holds the sample in shared memory
   int smem;
 };
 
@@ -44,6 +44,6 @@ cudaError_t forward(const Shape& s, const Plan& p, const void* x, const Affine& 
 // dx, and dw and db [c] in their parameters' types (or null).
 cudaError_t backward(const Shape& s, const Plan& p, const void* dy, const void* x, const Affine& a, const float* mean,
                      const float* rstd, Activation act, void* dx, void* dw, void* db, float* workspace, cudaStream_t st);
-int launches(const Plan& p, bool backward, bool parameters);
+int launches(const Plan& p, bool parameters);
 
 }  // namespace groupnorm

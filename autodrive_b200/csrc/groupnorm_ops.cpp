@@ -70,17 +70,13 @@ Forward forward(const torch::Tensor& rows, int64_t groups, const torch::Tensor& 
   torch::Tensor ws;
   if (!p.resident) {
     ws = floats(groupnorm::forward_workspace(s, p), rows);
-    if (!keep) {
-      f.mean = floats(s.n * groups, rows);
-      f.rstd = floats(s.n * groups, rows);
-    }
   }
   const cudaError_t e = groupnorm::forward(
       s, p, rows.data_ptr(), affine_of(w, b), (float)eps, static_cast<groupnorm::Activation>(act), f.y.data_ptr(),
       f.mean.defined() ? f.mean.data_ptr<float>() : nullptr, f.rstd.defined() ? f.rstd.data_ptr<float>() : nullptr,
       ws.defined() ? ws.data_ptr<float>() : nullptr, c10::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(e == cudaSuccess, "group_norm forward launch failed");
-  lm::count_launches(groupnorm::launches(p, false, false));
+  lm::count_launches(groupnorm::launches(p, false));
   return f;
 }
 
@@ -121,7 +117,7 @@ struct GroupNormFn : torch::autograd::Function<GroupNormFn> {
           dw.defined() ? dw.data_ptr() : nullptr, db.defined() ? db.data_ptr() : nullptr, ws.data_ptr<float>(),
           c10::cuda::getCurrentCUDAStream().stream());
       TORCH_CHECK(e == cudaSuccess, "group_norm backward launch failed");
-      lm::count_launches(groupnorm::launches(p, true, dw.defined() || db.defined()));
+      lm::count_launches(groupnorm::launches(p, dw.defined() || db.defined()));
     }
     return {dx.movedim(-1, 1), dw, db, torch::Tensor(), torch::Tensor(), torch::Tensor()};
   }
