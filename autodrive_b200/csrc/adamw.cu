@@ -106,12 +106,7 @@ __device__ __forceinline__ void load_codes(const uint8_t* p, int lane, int n, bo
     v[2 * i + 1] = f.y;
   }
 }
-// `v`: numbers that e4m3 holds, or NaN.
-__device__ __forceinline__ void store_codes(uint8_t* p, int lane, int n, bool whole, const float (&v)[8]) {
-  uint32_t h[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = lm::e4m3x2(v[2 * i], v[2 * i + 1]);
-  const uint2 u = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+__device__ __forceinline__ void store_codes(uint8_t* p, int lane, int n, bool whole, uint2 u) {
   if (whole) {
     *reinterpret_cast<uint2*>(p + lane * 8) = u;
   } else {
@@ -121,49 +116,99 @@ __device__ __forceinline__ void store_codes(uint8_t* p, int lane, int n, bool wh
   }
 }
 
-// The magnitude t, at most 448 and a rounding, as an e4m3 number at or below
-// it, or the next one with the probability of its distance. Below 2^-6 the
-// numbers lie 2^-9 apart: 2^-6 is added first, where the spacing is the same.
-__device__ __forceinline__ float dithered(float t, uint32_t bits16) {
-  const float off = t < 0x1p-6f ? 0x1p-6f : 0.f;
-  const uint32_t u = (__float_as_uint(t + off) + (bits16 << 4)) & 0xfff00000u;
-  return fminf(__uint_as_float(u) - off, 448.f);
+// The magnitude of x over `scale`, as the e4m3 code at or below it, or the next
+// one with the probability of its distance: in the result's upper byte. The
+// quotient is the correctly rounded one, by a correction of the product with
+// the rounded reciprocal `inv` (Markstein, 1990). Times 2^-120 the exponents of
+// e4m3 and of fp32 are the same, down to the subnormals of both (so nothing
+// here may flush them): the code is the number's upper bits, and 16 random ones
+// (`bits`, with eight zeros below) are added to those that are cut off.
+__device__ __forceinline__ uint32_t dithered(float x, float scale, float inv, uint32_t bits) {
+  const float q = lm::mul_nf(fabsf(x), inv);
+  const float t = lm::fma_nf(lm::fma_nf(-q, scale, fabsf(x)), inv, q);
+  return min(__float_as_uint(lm::mul_nf(t, 0x1p-120f)) * 16u + bits, 0x7effffffu);
+}
+// The upper bytes of four words.
+__device__ __forceinline__ uint32_t upper_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
 }
 
 __device__ __forceinline__ uint32_t warp_max(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
 
-// Scale of a block with the largest magnitude `amax` (as bits) and what a magnitude is multiplied with.
+// Scale of a block with the largest magnitude `amax` (as bits), and its reciprocal.
 __device__ __forceinline__ float2 scale_of(uint32_t amax) {
   const float s = lm::group_scale(amax);
-  float inv;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-  return make_float2(s, amax < 0x7f800000u ? inv : __uint_as_float(0x7fffffffu));
+  return make_float2(s, __frcp_rn(s));
+}
+// The larger magnitude, NaN if one is.
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
 }
 
-// Walks the blocks of the launch that belong to this warp, last to first:
-// enter(tensor) before the first block of each tensor, f(tensor, block) for each.
-template <typename TABLE, typename E, typename F>
-__device__ __forceinline__ void for_blocks(const TABLE& t, E&& enter, F&& f) {
-  const uint32_t warp = (threadIdx.x >> 5) * gridDim.x + blockIdx.x, warps = gridDim.x * kWarps;
-  if (warp >= t.h.blocks) return;
-  uint32_t b = t.h.blocks - 1 - warp;
-  int lo = 0, hi = t.h.tensors - 1;   // the last tensor whose first block is at or before b
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.e[mid].first <= b) lo = mid;
-    else hi = mid - 1;
-  }
-  enter(t.e[lo]);
-  for (;;) {
-    f(t.e[lo], b);
-    if (b < warps) return;
-    b -= warps;
-    if (t.e[lo].first > b) {
-      do --lo;
-      while (t.e[lo].first > b);
-      enter(t.e[lo]);
+// A warp's blocks of the launch, last to first, with the tensors that they belong to.
+template <typename TABLE>
+struct Walk {
+  const TABLE& t;
+  uint32_t b, warps;
+  int lo;
+  bool more;
+  __device__ __forceinline__ explicit Walk(const TABLE& table) : t(table), warps(gridDim.x * kWarps), lo(0) {
+    const uint32_t warp = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;
+    more = warp < t.h.blocks;
+    b = t.h.blocks - 1 - warp;
+    if (!more) return;
+    int hi = t.h.tensors - 1;   // the last tensor whose first block is at or before b
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (t.e[mid].first <= b) lo = mid;
+      else hi = mid - 1;
     }
   }
+  __device__ __forceinline__ const Entry& entry() const { return t.e[lo]; }
+  __device__ __forceinline__ void next() {
+    more = b >= warps;
+    b -= warps;
+    if (more)
+      while (t.e[lo].first > b) --lo;
+  }
+};
+// Where a block lies in its tensor, and how much of it there is.
+struct Place {
+  int64_t at;
+  int n;
+  bool whole;
+  __device__ __forceinline__ Place(const Entry& e, uint32_t b) : at((int64_t)(b - e.first) * kBlock) {
+    n = (int)min((int64_t)kBlock, (int64_t)e.n - at);
+    whole = e.vec && n == kBlock;
+  }
+};
+
+// A warp's next block on its way into shared memory: every lane copies what it will read itself.
+struct Staged {
+  unsigned char p[kBlock * 4], g[kBlock * 4], m[kBlock], v[kBlock];
+  float m_scale[32], v_scale[32];
+};
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy8(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" :: "r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy4(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void stage_lane(unsigned char* to, const void* from, int type, int64_t at, int lane) {
+  const int size = type == 0 ? 32 : 16;
+  const char* p = static_cast<const char*>(from) + at * (size / 8) + lane * size;
+  copy16(to + lane * size, p);
+  if (type == 0) copy16(to + lane * 32 + 16, p + 16);
+}
+__device__ __forceinline__ void staged_lane(const unsigned char* from, int type, int lane, float (&v)[8]) {
+  if (type == 0) lm::load8(reinterpret_cast<const float*>(from) + lane * 8, v);
+  else if (type == 1) lm::load8(reinterpret_cast<const __nv_bfloat16*>(from) + lane * 8, v);
+  else lm::load8(reinterpret_cast<const __half*>(from) + lane * 8, v);
 }
 
 // parts[CTA] = sum of the gradients' squares, in fp64.
@@ -171,14 +216,14 @@ template <int CAP>
 __global__ void __launch_bounds__(kThreads) square_sums_kernel(const __grid_constant__ Table<CAP> t, double* parts) {
   const int lane = threadIdx.x & 31;
   double s = 0.;
-  for_blocks(t, [](const Entry&) {}, [&](const Entry& e, uint32_t b) {
-    const int64_t at = (int64_t)(b - e.first) * kBlock;
-    const int n = (int)min((int64_t)kBlock, (int64_t)e.n - at);
+  for (Walk w(t); w.more; w.next()) {
+    const Entry& e = w.entry();
+    const Place at(e, w.b);
     float g[8];
-    load_any(e.g, e.g_type, at, lane, n, e.vec && n == kBlock, g);
+    load_any(e.g, e.g_type, at.at, lane, at.n, at.whole, g);
 #pragma unroll
     for (int i = 0; i < 8; ++i) s += (double)g[i] * (double)g[i];
-  });
+  }
   __shared__ double red[kWarps];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -222,17 +267,57 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     root_scale = rsqrtf(-expm1f((float)step * h.log_b2));
     key = mix(h.seed ^ (uint32_t)step);
   };
-  for_blocks(t, enter, [&](const Entry& e, uint32_t b) {
-    const int64_t at = (int64_t)(b - e.first) * kBlock;
-    const int n = (int)min((int64_t)kBlock, (int64_t)e.n - at);
-    const bool whole = e.vec && n == kBlock;
+  // 8-bit moments: the next block is under way while one is worked on. (With
+  // fp32 ones four times the bytes are, and the loads of one block fill the time.)
+  __shared__ __align__(16) Staged stages[BITS8 ? 2 * kWarps : 1];
+  Staged* const mine = stages + (threadIdx.x >> 5) * 2;
+  Walk ahead(t);
+  int turn = 0;
+  const auto send = [&](int to) {
+    if (ahead.more) {
+      const Entry& e = ahead.entry();
+      const Place at(e, ahead.b);
+      if (at.whole) {
+        stage_lane(mine[to].p, e.p, e.p_type, at.at, lane);
+        stage_lane(mine[to].g, e.g, e.g_type, at.at, lane);
+        copy8(mine[to].m + lane * 8, static_cast<const uint8_t*>(e.m) + at.at + lane * 8);
+        copy8(mine[to].v + lane * 8, static_cast<const uint8_t*>(e.v) + at.at + lane * 8);
+      }
+      copy4(mine[to].m_scale + lane, e.m_scale + (ahead.b - e.first));
+      copy4(mine[to].v_scale + lane, e.v_scale + (ahead.b - e.first));
+      ahead.next();
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if constexpr (BITS8) send(0);
+  int entered = -1;
+  for (Walk walk(t); walk.more; walk.next(), turn ^= 1) {
+    const Entry& e = walk.entry();
+    const uint32_t b = walk.b;
+    if (entered != walk.lo) {
+      enter(e);
+      entered = walk.lo;
+    }
+    const Place place(e, b);
+    const int64_t at = place.at;
+    const int n = place.n;
+    const bool whole = place.whole;
     float p[8], g[8], m[8], v[8];
-    load_any(e.p, e.p_type, at, lane, n, whole, p);
-    load_any(e.g, e.g_type, at, lane, n, whole, g);
     if constexpr (BITS8) {
-      load_codes(static_cast<const uint8_t*>(e.m) + at, lane, n, whole, m);
-      load_codes(static_cast<const uint8_t*>(e.v) + at, lane, n, whole, v);
-      const float ms = e.m_scale[b - e.first], vs = e.v_scale[b - e.first];
+      send(turn ^ 1);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      const float ms = mine[turn].m_scale[lane], vs = mine[turn].v_scale[lane];
+      if (whole) {
+        staged_lane(mine[turn].p, e.p_type, lane, p);
+        staged_lane(mine[turn].g, e.g_type, lane, g);
+        load_codes(mine[turn].m, lane, n, true, m);
+        load_codes(mine[turn].v, lane, n, true, v);
+      } else {
+        load_any(e.p, e.p_type, at, lane, n, false, p);
+        load_any(e.g, e.g_type, at, lane, n, false, g);
+        load_codes(static_cast<const uint8_t*>(e.m) + at, lane, n, false, m);
+        load_codes(static_cast<const uint8_t*>(e.v) + at, lane, n, false, v);
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         m[i] *= ms;
@@ -240,6 +325,8 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
         v[i] *= v[i];
       }
     } else {
+      load_any(e.p, e.p_type, at, lane, n, whole, p);
+      load_any(e.g, e.g_type, at, lane, n, whole, g);
       load_lane(static_cast<const float*>(e.m) + at, lane, n, whole, m);
       load_lane(static_cast<const float*>(e.v) + at, lane, n, whole, v);
     }
@@ -247,31 +334,52 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float gi = g[i] * clip;
-      m[i] = h.b1 * m[i] + h.c1 * gi;
-      v[i] = h.b2 * v[i] + h.c2 * gi * gi;
-      r[i] = sqrtf(v[i]);
+      // 8-bit moments: every operation is rounded on its own, so that what
+      // decides between two codes does not hang on which of them are fused
+      if constexpr (BITS8) {
+        m[i] = __fadd_rn(__fmul_rn(h.b1, m[i]), __fmul_rn(h.c1, gi));
+        v[i] = __fadd_rn(__fmul_rn(h.b2, v[i]), __fmul_rn(__fmul_rn(h.c2, gi), gi));
+        r[i] = __fsqrt_rn(v[i]);
+      } else {
+        m[i] = h.b1 * m[i] + h.c1 * gi;
+        v[i] = h.b2 * v[i] + h.c2 * gi * gi;
+        r[i] = sqrtf(v[i]);
+      }
       p[i] = p[i] * h.decay - rate * (m[i] / (r[i] * root_scale + h.eps));
     }
     store_any(e.p, e.p_type, at, lane, n, whole, p);
     if constexpr (BITS8) {
-      uint32_t am = 0, ar = 0;
+      float am = 0.f, ar = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        am = max(am, lm::abs_bits(m[i]));
-        ar = max(ar, lm::abs_bits(r[i]));
+        am = max_abs(am, m[i]);
+        ar = max_abs(ar, r[i]);
       }
-      const float2 sm = scale_of(warp_max(am)), sr = scale_of(warp_max(ar));
+      const uint32_t tm = warp_max(lm::abs_bits(am)), tr = warp_max(lm::abs_bits(ar));
+      const float2 sm = scale_of(tm), sr = scale_of(tr);
       const uint32_t number = (h.block0 + b) * kBlock + key;
+      uint32_t cm[8], cr[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t bits = mix(number + (whole ? lane * 8 + i : i * 32 + lane));
-        const float q = dithered(fabsf(m[i]) * sm.y, bits & 0xffffu);
-        m[i] = sm.y == sm.y ? copysignf(q, m[i]) : sm.y;
-        const float z = dithered(r[i] * sr.y, bits >> 16);
-        r[i] = sr.y == sr.y ? fmaxf(z, r[i] > 0.f ? 0x1p-9f : 0.f) : sr.y;
+        cm[i] = dithered(m[i], sm.x, sm.y, __byte_perm(bits, 0, 0x4104));
+        cr[i] = max(dithered(r[i], sr.x, sr.y, __byte_perm(bits, 0, 0x4324)), min(__float_as_uint(r[i]), 1u << 24));
       }
-      store_codes(static_cast<uint8_t*>(e.m) + at, lane, n, whole, m);
-      store_codes(static_cast<uint8_t*>(e.v) + at, lane, n, whole, r);
+      uint2 um, ur;
+      um.x = upper_bytes(cm[0], cm[1], cm[2], cm[3]);
+      um.y = upper_bytes(cm[4], cm[5], cm[6], cm[7]);
+      ur.x = upper_bytes(cr[0], cr[1], cr[2], cr[3]);
+      ur.y = upper_bytes(cr[4], cr[5], cr[6], cr[7]);
+      const auto sign = [&](int i) {
+        return upper_bytes(__float_as_uint(m[i]), __float_as_uint(m[i + 1]), __float_as_uint(m[i + 2]), __float_as_uint(m[i + 3])) &
+               0x80808080u;
+      };
+      um.x |= sign(0);
+      um.y |= sign(4);
+      if (tm >= 0x7f800000u) um = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);   // a NaN or an infinity
+      if (tr >= 0x7f800000u) ur = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+      store_codes(static_cast<uint8_t*>(e.m) + at, lane, n, whole, um);
+      store_codes(static_cast<uint8_t*>(e.v) + at, lane, n, whole, ur);
       if (lane == 0) {
         e.m_scale[b - e.first] = sm.x;
         e.v_scale[b - e.first] = sr.x;
@@ -280,7 +388,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
       store_lane(static_cast<float*>(e.m) + at, lane, n, whole, m);
       store_lane(static_cast<float*>(e.v) + at, lane, n, whole, v);
     }
-  });
+  }
 }
 
 template <typename F>

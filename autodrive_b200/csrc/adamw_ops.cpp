@@ -22,7 +22,21 @@ int type_code(torch::ScalarType t) {
 
 bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-using List = std::vector<torch::Tensor>;
+// A Python sequence of tensors, read where it lies.
+struct List {
+  py::object fast;
+  PyObject** items = nullptr;
+  size_t count = 0;
+  explicit List(const py::object& o) : fast(py::reinterpret_steal<py::object>(PySequence_Fast(o.ptr(), "adamw_step takes lists of tensors"))) {
+    if (!fast) throw py::error_already_set();
+    items = PySequence_Fast_ITEMS(fast.ptr());
+    count = (size_t)PySequence_Fast_GET_SIZE(fast.ptr());
+    for (size_t i = 0; i < count; ++i)
+      if (!THPVariable_Check(items[i])) throw py::type_error("adamw_step takes lists of tensors");
+  }
+  size_t size() const { return count; }
+  const torch::Tensor& operator[](size_t i) const { return THPVariable_Unpack(items[i]); }
+};
 
 void touch(const torch::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -41,9 +55,14 @@ torch::Tensor in_layout_of(const torch::Tensor& g, const torch::Tensor& p) {
   return y;
 }
 
-py::object adamw_step(List params, List grads, List ms, List vs, c10::optional<List> m_scales, c10::optional<List> v_scales,
-                      py::object step, double lr, double b1, double b2, double eps, double weight_decay, double max_norm,
+py::object adamw_step(py::object params_, py::object grads_, py::object ms_, py::object vs_, py::object m_scales_,
+                      py::object v_scales_, py::object step, double lr, double b1, double b2, double eps, double weight_decay, double max_norm,
                       int64_t seed) {
+  const at::NoGradGuard no_grad;
+  const List params(params_), grads(grads_), ms(ms_), vs(vs_);
+  c10::optional<List> m_scales, v_scales;
+  if (!m_scales_.is_none()) m_scales.emplace(m_scales_);
+  if (!v_scales_.is_none()) v_scales.emplace(v_scales_);
   const size_t count = params.size();
   const bool bits8 = m_scales.has_value();
   LM_CHECK_VALUE(grads.size() == count && ms.size() == count && vs.size() == count &&
@@ -59,7 +78,7 @@ py::object adamw_step(List params, List grads, List ms, List vs, c10::optional<L
   Header h{};
   std::vector<int64_t> steps;
   if (THPVariable_Check(step.ptr())) {
-    const auto s = step.cast<torch::Tensor>();
+    const torch::Tensor& s = THPVariable_Unpack(step.ptr());
     LM_CHECK_VALUE(s.scalar_type() == torch::kInt64 && s.numel() == 1 && s.device() == device,
                    "adamw_step needs its step as a number, a list of numbers or one int64 on ", device);
     h.step_at = s.data_ptr<int64_t>();
@@ -77,7 +96,7 @@ py::object adamw_step(List params, List grads, List ms, List vs, c10::optional<L
 
   std::vector<Entry> all;
   all.reserve(count);
-  List keep;   // gradients that were laid out anew
+  std::vector<torch::Tensor> keep;   // gradients that were laid out anew
   std::vector<std::pair<uintptr_t, uintptr_t>> spans;
   spans.reserve(count);
   uint64_t blocks = 0;
@@ -160,9 +179,10 @@ py::object adamw_step(List params, List grads, List ms, List vs, c10::optional<L
   h.log_b1 = (float)std::log(b1);
   h.log_b2 = (float)std::log(b2);
   h.seed = mix((uint32_t)seed);
-  const auto grid_of = [&](size_t r) {
+  // as many CTAs as an SM holds; the sums' have few registers
+  const auto grid_of = [&](size_t r, int per_sm) {
     const uint64_t nb = (ranges[r].second < all.size() ? first[ranges[r].second] : blocks) - first[ranges[r].first];
-    return (int)std::min<uint64_t>((nb + kWarps - 1) / kWarps, (uint64_t)lm::sm_count() * 4);
+    return (int)std::min<uint64_t>((nb + kWarps - 1) / kWarps, (uint64_t)lm::sm_count() * per_sm);
   };
   const auto header_of = [&](size_t r) {
     Header x = h;
@@ -175,13 +195,13 @@ py::object adamw_step(List params, List grads, List ms, List vs, c10::optional<L
   if (max_norm > 0.) {
     norm = torch::empty({}, params[0].options().dtype(torch::kFloat32));
     int total = 0;
-    for (size_t r = 0; r < ranges.size(); ++r) total += grid_of(r);
+    for (size_t r = 0; r < ranges.size(); ++r) total += grid_of(r, 8);
     if (total == 0) norm.zero_();
     parts = torch::empty({std::max(total, 1)}, params[0].options().dtype(torch::kFloat64));
     int at = 0;
     for (size_t r = 0; r < ranges.size(); ++r) {
-      check(launch_square_sums(header_of(r), all.data() + ranges[r].first, parts.data_ptr<double>() + at, grid_of(r), st));
-      at += grid_of(r);
+      check(launch_square_sums(header_of(r), all.data() + ranges[r].first, parts.data_ptr<double>() + at, grid_of(r, 8), st));
+      at += grid_of(r, 8);
     }
     h.parts = parts.data_ptr<double>();
     h.nparts = total;
@@ -190,7 +210,7 @@ py::object adamw_step(List params, List grads, List ms, List vs, c10::optional<L
   for (size_t r = 0; r < ranges.size(); ++r) {
     Header x = header_of(r);
     x.norm_out = r == 0 && norm.defined() ? norm.data_ptr<float>() : nullptr;
-    check(launch_step(x, all.data() + ranges[r].first, bits8, grid_of(r), st));
+    check(launch_step(x, all.data() + ranges[r].first, bits8, grid_of(r, bits8 ? 3 : 4), st));
   }
   for (size_t i = 0; i < count; ++i) {
     touch(params[i]);

@@ -157,7 +157,7 @@ __device__ __forceinline__ Pair sigmoid(Pair z) {
 
 // For bf16 values SiLU goes by the hardware's tanh, whose 2^-11 is a quarter of
 // their rounding: one special function instead of two, of which an SM has 16 a
-// cycle. With t = tanh(z / 2) it is z / 2 (1 + t), and its slope (1 + t + z / 2
+// cycle (the sums P and Q, which are fp32, take the two). With t = tanh(z / 2) it is z / 2 (1 + t), and its slope (1 + t + z / 2
 // (1 - t^2)) / 2; z is halved in its parameters, and the slope's half is left
 // to those of what follows.
 template <typename T>
@@ -181,13 +181,13 @@ __device__ __forceinline__ void activate(int act, Pair (&z)[P]) {
     for (int i = 0; i < P; ++i) z[i] = map(z[i], [](float x) { return x * normcdff(x); });
   }
 }
-// d (the gradient of y) times the activation's slope at z, over halved().
-template <typename T, int P>
+// d (the gradient of y) times the activation's slope at z, over halved(); by `FINE` not by tanh.
+template <typename T, bool FINE, int P>
 __device__ __forceinline__ void slope(int act, const Pair (&z)[P], Pair (&d)[P]) {
   if (act == kSilu) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value && !FINE) {
         const Pair t = map(z[i], tanh_of);
         d[i] = fma(d[i], fma(z[i], fma(t * Pair(-1.f), t, Pair(1.f)), t), d[i]);
       } else {
@@ -614,12 +614,12 @@ __global__ void __launch_bounds__(512) apply_kernel(const __grid_constant__ Args
 }
 
 // x less its mean and dz (over halved()) of a thread's vectors.
-template <typename T, int V>
+template <typename T, int V, bool FINE>
 struct Derive {
   static constexpr int P = (V + 1) / 2;
   Pair mean[P], scale[P], shift[P];
   __device__ __forceinline__ Derive(const Args& a, const Place& p, int c0, const Shared& s) {
-    const float h = halved<T>(a.act);
+    const float h = FINE ? 1.f : halved<T>(a.act);
     of_channels<V>(a, p, c0, mean, [&](int, int g) { return -s.mean[g]; });
     of_channels<V>(a, p, c0, scale, [&](int c, int g) { return s.rstd[g] * s.w[c] * h; });
     of_channels<V>(a, p, c0, shift, [&](int c, int) { return s.b[c] * h; });
@@ -633,14 +633,14 @@ struct Derive {
       x[e] = x[e] + mean[e];
       z[e] = fma(x[e], scale[e], shift[e]);
     }
-    slope<T>(act, z, d);
+    slope<T, FINE>(act, z, d);
   }
 };
 // dx = rstd w dz - rstd A / m - (x - mean) rstd^2 B / m
 template <typename T, int V>
 struct InputGradient {
   static constexpr int P = (V + 1) / 2;
-  Derive<T, V> derive;
+  Derive<T, V, false> derive;
   Pair by_dz[P], by_x[P], at[P];
   __device__ __forceinline__ InputGradient(const Args& a, const Place& p, int c0, const Shared& s) : derive(a, p, c0, s) {
     const float inv = 1.f / ((float)a.pixels * (a.c / a.groups)), h = halved<T>(a.act);
@@ -667,7 +667,7 @@ __device__ __forceinline__ void channel_sums(const Args& a, const Shared& s, F&&
     const Place p = place_of(a, c0);
     Pair sums[2][P];
     {
-      const Derive<T, V> derive(a, p, c0, s);
+      const Derive<T, V, true> derive(a, p, c0, s);
       walk(p, c0, [&](const Vec<T, V>& vx, const Vec<T, V>& vd) {
         Pair x[P], d[P];
         derive(a.act, vx, vd, x, d);
@@ -678,14 +678,10 @@ __device__ __forceinline__ void channel_sums(const Args& a, const Shared& s, F&&
         }
       });
     }
-    const float h = halved<T>(a.act);
     Pair rstd[P];
-    of_channels<V>(a, p, c0, rstd, [&](int, int g) { return s.rstd[g] * h; });
+    of_channels<V>(a, p, c0, rstd, [&](int, int g) { return s.rstd[g]; });
 #pragma unroll
-    for (int e = 0; e < P; ++e) {
-      sums[0][e] = sums[0][e] * Pair(h);
-      sums[1][e] = sums[1][e] * rstd[e];
-    }
+    for (int e = 0; e < P; ++e) sums[1][e] = sums[1][e] * rstd[e];
     join_rows<V, 2>(a, p, c0, sums, s.red, s.channel);
   }
 }

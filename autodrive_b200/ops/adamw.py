@@ -169,7 +169,6 @@ def _check(params, grads, ms, vs, m_scales, v_scales) -> None:
         raise ValueError("adamw_step: two parameters share memory")
 
 
-@torch.no_grad()
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
                exp_avg_sqs: Sequence[Tensor], exp_avg_scales: Sequence[Tensor] | None = None,
                exp_avg_sq_scales: Sequence[Tensor] | None = None, *, step: int | Sequence[int] | Tensor, lr: float,
@@ -200,5 +199,6 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
         raise ValueError(f"adamw_step needs one step for all or for each of {len(params)} parameters")
     if any(not 1 <= s < 2 ** 32 for s in steps):
         raise ValueError("adamw_step counts its steps from 1")
-    return reference_adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, steps, lr, betas,
-                                eps, weight_decay, max_grad_norm, seed)
+    with torch.no_grad():
+        return reference_adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, steps, lr, betas,
+                                    eps, weight_decay, max_grad_norm, seed)
