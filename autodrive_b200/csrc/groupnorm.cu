@@ -305,14 +305,15 @@ __device__ void join_rows(const Args& a, const Place& p, int c0, const Pair (&v)
   __syncthreads();
 }
 
-// out[g] = factor times the sum of channel[c] (times w_c) over the group's channels.
-__device__ __forceinline__ void join_channels(const Args& a, const float* channel, const float* w, float factor, float* out) {
+// out[g] = the sum of channel[c] (times w_c) over the group's channels, over `values` (a quotient that is rounded once:
+// the mean of equal values is that value).
+__device__ __forceinline__ void join_channels(const Args& a, const float* channel, const float* w, float values, float* out) {
   const int per = a.c / a.groups;
   if (per <= 32) {   // a thread for each group
     for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
       float s = 0.f;
       for (int c = g * per; c < (g + 1) * per; ++c) s += w ? channel[c] * w[c] : channel[c];
-      out[g] = s * factor;
+      out[g] = __fdiv_rn(s, values);
     }
     return;
   }
@@ -321,7 +322,7 @@ __device__ __forceinline__ void join_channels(const Args& a, const float* channe
     float s = 0.f;
     for (int c = g * per + lane; c < (g + 1) * per; c += 32) s += w ? channel[c] * w[c] : channel[c];
     s = lm::warp_sum(s);
-    if (lane == 0) out[g] = s * factor;
+    if (lane == 0) out[g] = __fdiv_rn(s, values);
   }
 }
 
@@ -437,7 +438,7 @@ template <typename T, int V, typename F>
 __device__ __forceinline__ void statistics(const Args& a, int count, const Shared& s, F&& walk) {
   constexpr int P = (V + 1) / 2;
   const bool one = a.cols <= (int)blockDim.x;
-  const float inv_values = count ? (float)a.groups / ((float)count * V) : 0.f;
+  const float values = count ? (float)((double)count * V / a.groups) : 1.f;
   for (int pass = one ? 1 : 0; pass < 2; ++pass) {
     clear(s.channel, a.c);
     __syncthreads();
@@ -466,7 +467,7 @@ __device__ __forceinline__ void statistics(const Args& a, int count, const Share
         join_rows<V, 1>(a, p, c0, v, s.red, s.channel);
       }
       if (one) {
-        join_channels(a, s.channel, nullptr, inv_values, s.mean);
+        join_channels(a, s.channel, nullptr, values, s.mean);
         __syncthreads();
         clear(s.channel, a.c);
         __syncthreads();
@@ -482,7 +483,7 @@ __device__ __forceinline__ void statistics(const Args& a, int count, const Share
       }
     }
     if (pass == 0) {
-      join_channels(a, s.channel, nullptr, inv_values, s.mean);
+      join_channels(a, s.channel, nullptr, values, s.mean);
       __syncthreads();
     }
   }

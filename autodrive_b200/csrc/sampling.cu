@@ -105,7 +105,7 @@ struct Weights {
       far = 0.f;
       return;
     }
-    lowest = __double2float_ru(fmax(top - (double)kRange * r.t, -3.4e38));
+    lowest = __double2float_ru(top - (double)kRange * r.t);   // at least the lowest number, and at most the largest logit
     if (cut && r.min_p > 0.) {   // by halving: a logit stays or not by its weight in fp64
       uint32_t lo = key_of(lowest), hi = key_of(m);
       while (lo < hi) {

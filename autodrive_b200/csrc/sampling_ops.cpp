@@ -42,6 +42,8 @@ py::tuple sample_tokens(torch::Tensor logits, torch::Tensor uniforms, c10::optio
                         py::object temperature, py::object top_k, py::object top_p, py::object min_p) {
   LM_CHECK_VALUE(logits.is_cuda() && logits.dim() >= 1 && type_code(logits.scalar_type()) >= 0 && logits.size(-1) >= 1,
                  "sample_tokens takes fp32, bf16 or fp16 logits [..., V]");
+  LM_CHECK_VALUE(!lm::has_tangent(logits) && !(at::GradMode::is_enabled() && logits.requires_grad()),
+                 "sample_tokens has no gradient: call it under torch.no_grad()");
   const int64_t v = logits.size(-1);
   LM_CHECK_VALUE(v <= INT32_MAX, "sample_tokens: rows of at most 2^31 - 1 entries, not ", v);
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);

@@ -41,8 +41,10 @@ import torch
 from torch import nn
 from torch.nn import functional as F
 
+from ..ops.groupnorm import fuse_group_norms
 from ..train.curriculum import (SCENARIOS, CurriculumEnv, D2PredictivePolicy, episode_success, get_scenario,
                                 seed_partition, wilson_interval)
+from ..train.optim import OPTIMIZERS, make_optimizer
 from .inputs import CELL, build_globals, build_raster, safe_action_candidates, se2_lattice
 from .tracks import HIDDEN, DecisionRequest, ScorerOutput, candidate_policy_logits, choose_candidate, make_meco_track
 
@@ -145,9 +147,15 @@ class MecoConfig:
     seed: int = 0
     device: str = "cpu"
     output: str = ""
+    optimizer: str = "adam"        # one of train.optim.OPTIMIZERS
+    fused_norms: bool = False      # group norms with their activations on the fused kernels, channels last
 
     def identity(self) -> str:
-        return hashlib.sha256(json.dumps(asdict(self), sort_keys=True).encode()).hexdigest()[:16]
+        fields = asdict(self)
+        for name in ("optimizer", "fused_norms"):   # the defaults are what a configuration without them ran
+            if fields[name] == getattr(type(self), name):
+                del fields[name]
+        return hashlib.sha256(json.dumps(fields, sort_keys=True).encode()).hexdigest()[:16]
 
 
 # --------------------------------------------------------------------------- ledger
@@ -262,7 +270,10 @@ def train_meco(config: MecoConfig, ledger: MetricLedger | None = None) -> tuple[
     sc = get_scenario(config.scenario)
     cenv = CurriculumEnv(config.scenario, sc.required_categories[0], config.envs, dev, seed=config.seed)
     policy = MecoPolicy(config.track).to(dev)
-    opt = torch.optim.Adam(policy.parameters(), lr=config.learning_rate, eps=1e-5)
+    if config.fused_norms:
+        fuse_group_norms(policy.track)
+        policy.track.to(memory_format=torch.channels_last)
+    opt = make_optimizer(config.optimizer, policy.parameters(), config.learning_rate, eps=1e-5)
     history = []
     if config.warm_start_decisions:
         loss = supervised_warm_start(policy, cenv, opt, config.warm_start_decisions)
@@ -406,6 +417,9 @@ def _parser() -> argparse.ArgumentParser:
     t.add_argument("--warm-start-decisions", type=int, default=0)
     t.add_argument("--seed", type=int, default=0)
     t.add_argument("--device", default="cpu")
+    t.add_argument("--optimizer", choices=OPTIMIZERS, default="adam")
+    t.add_argument("--fused-norms", action="store_true",
+                   help="group norms and their activations on the fused kernels, channels last")
     t.add_argument("--output", required=True)
     e = sub.add_parser("evaluate", help="matched-seed evaluation against the scripted teacher")
     e.add_argument("--checkpoint", default=None)
@@ -427,7 +441,7 @@ def main(argv=None) -> int:
         cfg = MecoConfig(track=args.track, scenario=args.scenario, envs=args.envs, updates=args.updates,
                          epochs=args.epochs, learning_rate=args.learning_rate,
                          warm_start_decisions=args.warm_start_decisions, seed=args.seed, device=args.device,
-                         output=args.output)
+                         output=args.output, optimizer=args.optimizer, fused_norms=args.fused_norms)
         out = Path(args.output)
         out.mkdir(parents=True, exist_ok=True)
         ledger = MetricLedger(out / "metric-ledger.jsonl")

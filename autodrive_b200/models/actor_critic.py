@@ -11,6 +11,7 @@ import torch
 from torch import nn
 from torch.distributions import Normal
 
+from ..ops.sampling import sample_tokens
 from ..ops.token_logprobs import token_log_probs
 
 OBS_DIM = 35
@@ -84,6 +85,29 @@ class ActorCritic(nn.Module):
         if self.action_kind != "categorical":
             raise ValueError("alternatives need a categorical policy")
         return most_probable(self(obs)[0], top, action_mask)
+
+    @torch.no_grad()
+    def draw(self, obs: torch.Tensor, uniforms: torch.Tensor | None = None, temperature=1., top_k=0, top_p=1., min_p=0.,
+             action_mask=None):
+        """(action [B], log-probability [B], value [B]) of a categorical policy,
+        drawn by one number of [0, 1) for each row (fresh ones if none are
+        given) with a temperature and cut-offs, numbers or tensors [B] (see
+        ``ops.sampling``); the log-probability is that of the distribution that
+        was drawn from. A row whose mask leaves no action counts every one."""
+        if self.action_kind != "categorical":
+            raise ValueError("draw needs a categorical policy")
+        logits, _, value = self(obs)
+        return (*draw_actions(logits, uniforms, temperature, top_k, top_p, min_p, action_mask), value)
+
+
+def draw_actions(logits: torch.Tensor, uniforms, temperature, top_k, top_p, min_p, action_mask=None):
+    """(actions, log-probabilities) of categorical logits (see ``ActorCritic.draw``)."""
+    if action_mask is not None:
+        action_mask = action_mask.bool()
+        action_mask = action_mask | ~action_mask.any(-1, keepdim=True)
+    if uniforms is None:
+        uniforms = torch.rand(logits.shape[:-1], device=logits.device)
+    return tuple(sample_tokens(logits, uniforms, action_mask, temperature, top_k, top_p, min_p))
 
 
 def most_probable(logits: torch.Tensor, top: int, action_mask=None):

@@ -45,7 +45,7 @@ from torch.nn.attention import SDPBackend, sdpa_kernel
 from ..ops.attention import supported as _tc_attention_supported, varlen_attention, varlen_query_attention
 from ..ops.layernorm import FusedLayerNorm
 from ..ops.tc_linear import _TcLinearFn, tensorize
-from .actor_critic import most_probable
+from .actor_critic import draw_actions, most_probable
 
 _SDPA_BACKENDS = [SDPBackend.EFFICIENT_ATTENTION, SDPBackend.FLASH_ATTENTION, SDPBackend.MATH]
 
@@ -564,6 +564,19 @@ class PerceptionActorCritic(nn.Module):
         if action_mask is None:
             action_mask = inputs["scalars"][:, -self.action_dim:] > .5
         return most_probable(self(inputs)[0].float(), top, action_mask)
+
+    @torch.no_grad()
+    def draw(self, inputs: dict, uniforms: Tensor | None = None, temperature=1., top_k=0, top_p=1., min_p=0.,
+             action_mask=None):
+        """(action [B], log-probability [B], value [B]) of a categorical policy,
+        drawn by one number of [0, 1) for each row (fresh ones if none are
+        given) with a temperature and cut-offs, numbers or tensors [B] (see
+        ``ops.sampling``); the log-probability is that of the distribution that
+        was drawn from. A row whose mask leaves no action counts every one."""
+        if action_mask is None:
+            action_mask = inputs["scalars"][:, -self.action_dim:] > .5
+        logits, _, value = self(inputs)
+        return (*draw_actions(logits.float(), uniforms, temperature, top_k, top_p, min_p, action_mask), value)
 
 
 def make_policy(architecture: str = "baseline_mlp", tensor_cores: bool = True):

@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor, nn
+from torch.autograd import forward_ad
 from torch.nn import functional as F
 
 from .ext import require_extension
@@ -35,8 +36,14 @@ def _code(activation: str | None) -> int:
 def reference_group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tensor | None = None,
                          eps: float = 1e-5, activation: str | None = None) -> Tensor:
     """The same operation in plain PyTorch, in fp32, with autograd (CPU path)."""
-    y = F.group_norm(x.float(), groups, None if weight is None else weight.float(), None if bias is None else bias.float(),
-                     eps)
+    y = x.float().unflatten(1, (groups, -1)).flatten(2)
+    y = y - y.mean(-1, keepdim=True)
+    y = (y * (y.square().mean(-1, keepdim=True) + eps).rsqrt()).view(x.shape)
+    channels = (x.shape[1], *(1,) * (x.dim() - 2))
+    if weight is not None:
+        y = y * weight.float().view(channels)
+    if bias is not None:
+        y = y + bias.float().view(channels)
     return (y if activation is None else _ACT[activation](y)).to(x.dtype)
 
 
@@ -56,11 +63,10 @@ def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tenso
     for p in (weight, bias):
         if p is not None and (p.shape != (c,) or p.dtype not in DTYPES or p.device != x.device):
             raise ValueError(f"group_norm needs fp32, bf16 or fp16 parameters [{c}] on {x.device}")
-    if x.numel() == 0:
-        return x.clone()
-    rows = x.movedim(1, -1).contiguous().movedim(-1, 1)   # lies as the result on a GPU does
-    y = reference_group_norm(rows if rows.dim() > 2 else rows[..., None], groups, weight, bias, eps, activation)
-    return (y if rows.dim() > 2 else y[..., 0]).movedim(1, -1).contiguous().movedim(-1, 1)
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (x, weight, bias)):
+        raise NotImplementedError("group_norm has no forward-mode derivative")
+    y = reference_group_norm(x, groups, weight, bias, eps, activation)
+    return y.movedim(1, -1).contiguous().movedim(-1, 1)   # lies as the result on a GPU does
 
 
 class FusedGroupNorm(nn.GroupNorm):

@@ -6,7 +6,7 @@ top-p and min-p, by given uniform numbers, on fused sm_100a kernels
 min_p=0.)`` takes logits [..., V] (fp32, bf16 or fp16), one number of [0, 1) for
 each row (fp32 or fp64 [...]) and an optional boolean mask of the valid entries
 that broadcasts against the logits, and returns ``SampledTokens(token,
-log_prob)``, int64 and fp32 [...], without gradient (``ops.token_logprobs``
+log_prob)``, int64 and fp32 [...]. It has no gradient (``ops.token_logprobs``
 scores tokens with one):
 
 * entries weigh w = exp((logit - largest) / temperature); masked ones are not
@@ -38,6 +38,7 @@ import torch
 from torch import Tensor
 
 from .ext import require_extension
+from .rmsnorm import wants_derivative
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 RANGE = 44.
@@ -103,6 +104,8 @@ def sample_tokens(logits: Tensor, uniforms: Tensor, mask: Tensor | None = None, 
     if logits.is_cuda:
         return SampledTokens._make(require_extension().sample_tokens(logits, uniforms, mask, temperature, top_k, top_p,
                                                                      min_p))
+    if wants_derivative(logits):
+        raise ValueError("sample_tokens has no gradient: call it under torch.no_grad()")
     if logits.dim() < 1 or logits.shape[-1] < 1 or logits.dtype not in DTYPES:
         raise ValueError("sample_tokens takes fp32, bf16 or fp16 logits [..., V]")
     lead, v = logits.shape[:-1], logits.shape[-1]

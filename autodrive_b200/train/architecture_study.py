@@ -32,6 +32,7 @@ import torch
 
 from ..models.perception import PerceptionInputs
 from ..models.zoo import ARCHITECTURES, PerceptionActorCritic, parameter_count
+from .optim import OPTIMIZERS, make_optimizer
 from .rollout import gae_reference
 
 SCENARIOS = {
@@ -134,7 +135,7 @@ def train_case(args, architecture: str, scenario: str, seed: int, lr: float) -> 
     torch.manual_seed(seed)
     dev = torch.device(args.device)
     model = PerceptionActorCritic(architecture, tensor_cores=dev.type == "cuda").to(dev)
-    opt = torch.optim.Adam(model.parameters(), lr=lr, eps=1e-5)
+    opt = make_optimizer(args.optimizer, model.parameters(), lr, eps=1e-5)
     out = Path(args.output) / architecture / scenario / f"seed-{seed}-lr-{lr:g}"
     out.mkdir(parents=True, exist_ok=True)
     train = _Case(scenario, args.envs, dev, seed, model.field_shape)
@@ -211,6 +212,7 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--scenarios", nargs="+", choices=sorted(SCENARIOS), default=sorted(SCENARIOS))
     p.add_argument("--seeds", nargs="+", type=int, default=[7, 19, 43])
     p.add_argument("--learning-rates", nargs="+", type=float, default=[3e-4])
+    p.add_argument("--optimizer", choices=OPTIMIZERS, default="adam")
     p.add_argument("--output", type=Path, default=Path("evaluations/architecture-study"))
     p.add_argument("--device", default="cuda:0" if torch.cuda.is_available() else "cpu")
     p.add_argument("--envs", type=int, default=8)

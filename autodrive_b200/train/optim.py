@@ -1,4 +1,5 @@
-"""Flat parameter storage and the fused clip + Adam optimizer.
+"""Flat parameter storage and the fused clip + Adam optimizer, and AdamW over
+parameters that stay where they are (``FusedAdamW``).
 
 All trainable parameters of a module are re-homed into one contiguous fp32
 buffer and their gradients into a second one. The whole update is then two
@@ -13,6 +14,7 @@ import torch
 from torch import nn
 
 from ..ops import require_extension
+from ..ops.adamw import adamw_step, moments_8bit
 from ..utils import launches
 
 
@@ -103,3 +105,86 @@ class FusedAdam:
         self.m.copy_(state["m"])
         self.v.copy_(state["v"])
         self.step_count = int(state["step"])
+
+
+class FusedAdamW(torch.optim.Optimizer):
+    """AdamW over any list of parameters on the fused step of ``ops.adamw``: one launch a parameter group (two with
+    clipping), the parameters where and of what type they are (fp32, bf16 or fp16), the moments in fp32 or, with
+    ``state_bits=8``, in 8 bits with a scale for each 256 elements.
+
+    ``max_grad_norm`` clips by the norm over each parameter group's gradients (``last_norms``: those of the last step, on
+    the device). With ``capturable`` the group's step is counted on the device, for steps inside a CUDA graph; the first
+    step, which makes the moments, is then taken outside of it. `seed` is that of the 8-bit moments' rounding."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(.9, .999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                 max_grad_norm: float = 0., state_bits: int = 32, seed: int = 0, capturable: bool = False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"FusedAdamW holds its moments in 8 or 32 bits, not {state_bits}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
+                                      max_grad_norm=max_grad_norm, state_bits=state_bits, seed=seed, capturable=capturable))
+        self.last_norms: list[torch.Tensor] = []
+
+    def _moments(self, p: torch.Tensor, bits: int) -> dict:
+        state = self.state[p]
+        if not state:
+            state["step"] = 0
+            if bits == 32:
+                state["exp_avg"], state["exp_avg_sq"] = (torch.zeros_like(p, dtype=torch.float32) for _ in range(2))
+            else:
+                state["exp_avg"], state["exp_avg_scale"] = moments_8bit(p)
+                state["exp_avg_sq"], state["exp_avg_sq_scale"] = moments_8bit(p)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        self.last_norms = []
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            if not params:
+                continue
+            states = [self._moments(p, group["state_bits"]) for p in params]
+            if group["capturable"]:
+                if "step" not in group:
+                    group["step"] = torch.zeros((), dtype=torch.int64, device=params[0].device)
+                step = group["step"].add_(1)
+            else:
+                for s in states:
+                    s["step"] += 1
+                step = [s["step"] for s in states]
+            scales = [[s[name] for s in states] if group["state_bits"] == 8 else None
+                      for name in ("exp_avg_scale", "exp_avg_sq_scale")]
+            norm = adamw_step(params, [p.grad for p in params], [s["exp_avg"] for s in states],
+                              [s["exp_avg_sq"] for s in states], *scales, step=step, lr=group["lr"], betas=group["betas"],
+                              eps=group["eps"], weight_decay=group["weight_decay"], max_grad_norm=group["max_grad_norm"],
+                              seed=group["seed"])
+            if norm is not None:
+                self.last_norms.append(norm)
+        return loss
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        super().load_state_dict(state_dict)
+        # the moments keep their types, which the base class casts to the parameters'
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            for p, index in zip(group["params"], saved["params"]):
+                for name, value in state_dict["state"].get(index, {}).items():
+                    if isinstance(value, torch.Tensor):
+                        self.state[p][name] = value.detach().to(p.device, copy=True)
+            if isinstance(group.get("step"), torch.Tensor):
+                group["step"] = saved["step"].detach().to(group["params"][0].device, copy=True)
+
+
+OPTIMIZERS = ("adam", "fused", "fused8")
+
+
+def make_optimizer(kind: str, params, lr: float, eps: float = 1e-8) -> torch.optim.Optimizer:
+    """Adam of a trainer whose parameters stay where they are: PyTorch's (``adam``), or FusedAdamW without weight decay
+    with its moments in fp32 (``fused``) or 8 bits (``fused8``)."""
+    if kind not in OPTIMIZERS:
+        raise ValueError(f"unknown optimizer {kind!r}; choose from {OPTIMIZERS}")
+    if kind == "adam":
+        return torch.optim.Adam(params, lr=lr, eps=eps)
+    return FusedAdamW(params, lr=lr, eps=eps, weight_decay=0., state_bits=8 if kind == "fused8" else 32)

@@ -20,6 +20,7 @@ import torch
 from torch import nn
 
 from ..models.zoo import make_policy
+from .optim import make_optimizer
 
 
 def _logits_value(policy, obs):
@@ -77,10 +78,11 @@ class DiscreteSAC(nn.Module):
         return action, logp.gather(-1, action[:, None]).squeeze(-1), value
 
 
-def make_sac_optimizers(agent: DiscreteSAC, learning_rate: float) -> dict:
-    return {"actor": torch.optim.Adam(agent.actor.parameters(), lr=learning_rate),
-            "critic": torch.optim.Adam((*agent.q1.parameters(), *agent.q2.parameters()), lr=learning_rate),
-            "alpha": torch.optim.Adam((agent.log_alpha,), lr=learning_rate)}
+def make_sac_optimizers(agent: DiscreteSAC, learning_rate: float, optimizer: str = "adam") -> dict:
+    """`optimizer`: one of ``train.optim.OPTIMIZERS``."""
+    return {"actor": make_optimizer(optimizer, agent.actor.parameters(), learning_rate),
+            "critic": make_optimizer(optimizer, (*agent.q1.parameters(), *agent.q2.parameters()), learning_rate),
+            "alpha": make_optimizer(optimizer, (agent.log_alpha,), learning_rate)}
 
 
 def _map(value, fn):

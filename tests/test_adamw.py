@@ -1,0 +1,336 @@
+"""AdamW over a list of tensors against 64 bits, its 8-bit moments against their
+definition bit for bit, and the optimizer on it.
+
+Tolerances, with f = 2^-24: m and v take three roundings each (4 f of the sum of
+their terms' magnitudes, which bounds the rest), the root two more, the update
+six with its quotient's and root's approximations to 2^-22: 40 f of the update's
+magnitude; p itself takes three, and eps / 2 of its type. The clipping factor is
+rounded once. 8-bit moments are made of fp32 operations that are rounded one by
+one, so they equal the plain form's on the same device.
+"""
+import math
+
+import pytest
+import torch
+from torch import nn
+
+from autodrive_b200.ops.adamw import adamw_step, dequantize_moment, moments_8bit, reference_adamw_step
+from autodrive_b200.train.optim import FusedAdamW, make_optimizer
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+F = 2. ** -24
+SHAPES = [(1,), (7,), (256,), (257,), (3, 5, 2), (1000,), (64, 33), (), (0,), (4, 512), (300, 41)]
+
+
+def _make(shapes, dtype, grad, device, bits=32, seed=0):
+    g = torch.Generator().manual_seed(seed)
+
+    def rand(s, scale=1.):
+        return scale * torch.randn(s, generator=g)
+
+    params = [rand(s, .1).to(dtype).to(device) for s in shapes]
+    grads = [rand(s, math.exp(-2. * (i % 4))).to(grad).to(device) for i, s in enumerate(shapes)]
+    if bits == 32:
+        return params, grads, [rand(g_.shape, .1).to(device) for g_ in grads], \
+            [rand(g_.shape, .1).to(device).square() for g_ in grads], None, None
+    ms, vs = [moments_8bit(p) for p in params], [moments_8bit(p) for p in params]
+    return params, grads, [m[0] for m in ms], [v[0] for v in vs], [m[1] for m in ms], [v[1] for v in vs]
+
+
+def _copy(lists):
+    return [None if x is None else [t.clone() for t in x] for x in lists]
+
+
+@pytest.mark.parametrize("clip", [0., .3, 1e6])
+@pytest.mark.parametrize("dtype,grad", [(a, b) for a in TYPES for b in (torch.float32, torch.bfloat16, torch.float16)])
+@pytest.mark.parametrize("device", DEVICES)
+def test_against_64_bits(dtype, grad, clip, device):
+    lists = _make(SHAPES, dtype, grad, device)
+    before = _copy(lists)
+    lr, (b1, b2), eps, decay, step = 1e-2, (.9, .99), 1e-6, .1, 7
+    norm = adamw_step(*lists[:4], step=step, lr=lr, betas=(b1, b2), eps=eps, weight_decay=decay, max_grad_norm=clip)
+    total = torch.stack([g.double().square().sum() for g in before[1]]).sum().sqrt()
+    c = 1.
+    if clip:
+        assert norm.dtype == torch.float32 and norm.shape == () and abs(float(norm) / float(total) - 1) <= 4 * F
+        c = min(1., clip / (float(total) + 1e-6))
+    else:
+        assert norm is None
+    for p0, g, m0, v0, p, m, v in zip(*before[:4], lists[0], lists[2], lists[3]):
+        p0, g, m0, v0 = p0.double(), g.double() * c, m0.double(), v0.double()
+        m1, v1 = b1 * m0 + (1 - b1) * g, b2 * v0 + (1 - b2) * g * g
+        assert ((m.double() - m1).abs() <= 5 * F * (b1 * m0.abs() + (1 - b1) * g.abs())).all()
+        assert ((v.double() - v1).abs() <= 6 * F * v1).all()
+        up = lr / (1 - b1 ** step) * (b1 * m0.abs() + (1 - b1) * g.abs()) / ((v1 / (1 - b2 ** step)).sqrt() + eps)
+        want = p0 * (1 - lr * decay) - lr / (1 - b1 ** step) * m1 / ((v1 / (1 - b2 ** step)).sqrt() + eps)
+        # (subnormal numbers are as far apart as the smallest normal ones)
+        i = torch.finfo(dtype)
+        tol = 40 * F * up + 4 * F * p0.abs() + i.eps / 2 * want.abs().clamp_min(i.smallest_normal) + 1e-12
+        assert ((p.double() - want).abs() <= tol).all(), float(((p.double() - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dtype,clip", [(torch.float32, 0.), (torch.float32, .5), (torch.bfloat16, .5), (torch.float16, 0.)])
+@pytest.mark.parametrize("device", DEVICES)
+def test_8_bit_moments_are_those_of_the_definition(dtype, clip, device):
+    lists = _make(SHAPES, dtype, dtype, device, bits=8)
+    plain = _copy(lists)
+    for step in range(1, 5):
+        for x, y in zip(lists[1], plain[1]):
+            x.mul_(.7), y.copy_(x)
+        opts = dict(lr=1e-3, betas=(.9, .999), eps=1e-8, weight_decay=.01, max_grad_norm=clip, seed=5)
+        adamw_step(*lists, step=step, **opts)
+        reference_adamw_step(*plain, [step] * len(SHAPES), **opts)
+        for a, b, name in zip(lists[2:], plain[2:], ("m", "r", "m scale", "r scale")):
+            for x, y in zip(a, b):
+                assert torch.equal(x.float(), y.float()), name
+        for x, y in zip(lists[0], plain[0]):
+            assert torch.allclose(x.float(), y.float(), rtol=2 * torch.finfo(dtype).eps, atol=1e-6)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_8_bit_moments_move_on_average(device):
+    """A second moment that decays by a thousandth a step, next to one that holds its scale: rounded to the nearest code it
+    would never move. 4096 of them, each step a code up or down by chance: the mean's deviation after 400 steps is below
+    sqrt(400 / 4096) of a spacing's half, 2^-4 / 2 of the root."""
+    p = torch.zeros(16, 257, device=device)
+    n = p.numel()
+    grad = torch.zeros_like(p)
+    grad.view(-1)[::256] = 1.                         # one large element in each block
+    m, ms = moments_8bit(p)
+    r, rs = moments_8bit(p)
+    adamw_step([p], [torch.where(grad == 0, .5, 1.)], [m], [r], [ms], [rs], step=1, lr=0.)
+    first = dequantize_moment(r, rs)
+    for step in range(2, 402):
+        adamw_step([p], [grad], [m], [r], [ms], [rs], step=step, lr=0., seed=1)
+    held = (grad == 0)
+    ratio = (dequantize_moment(r, rs)[held] / first[held]).double().mean()
+    want = .999 ** 200                                # the root of .999^400
+    assert abs(float(ratio) / want - 1) <= math.sqrt(400 / n) / 32 + .02
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_8_bit_edges(device):
+    p = torch.ones(600, device=device)
+    m, ms = moments_8bit(p)
+    r, rs = moments_8bit(p)
+    g = torch.zeros_like(p)
+    g[0], g[1], g[300] = 1., 1e-7, torch.nan
+    adamw_step([p], [g], [m], [r], [ms], [rs], step=1, lr=.1, weight_decay=0.)
+    assert m[:256].float().isfinite().all() and m[256:512].float().isnan().all() and (m[512:].float() == 0).all()
+    assert r[1].float() == 2. ** -9 and (r[2:256].float() == 0).all()     # what is not zero does not become zero
+    assert p[300].isnan() and p[:300].isfinite().all() and (p[2:256] == 1).all()
+    # blocks that stay zero hold the smallest scale
+    assert rs[2] == 2. ** -126
+    # (the quotient is rounded once; a product with 1 / 448, which a division by a number may be on a GPU, twice)
+    assert ms[0] == (torch.tensor(.1).double() / 448).float()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layouts_steps_and_empty_lists(device):
+    torch.manual_seed(0)
+    w = torch.randn(8, 4, 3, 3, device=device).contiguous(memory_format=torch.channels_last)
+    flat = torch.randn(1000, device=device)
+    params = [w, flat[1:13].view(3, 4), flat[13:270], flat[400:400 + 35].view(5, 7).t()]
+    grads = [torch.randn(8, 4, 3, 3, device=device), torch.randn(4, 3, device=device).t(), torch.randn(257, device=device),
+             torch.randn(7, 5, device=device)]
+    ms, vs = [[torch.zeros_like(p) for p in params] for _ in range(2)]
+    want = [p.clone() for p in params]
+    steps = [1, 5, 9, 100]
+    for p, g, s in zip(want, grads, steps):
+        q = p.double()
+        m, v = .1 * g.double(), .001 * g.double() ** 2
+        p.copy_(q * (1 - 1e-3 * .01) - 1e-3 / (1 - .9 ** s) * m / ((v / (1 - .999 ** s)).sqrt() + 1e-8))
+    keep = flat.clone()
+    adamw_step(params, grads, ms, vs, step=steps, lr=1e-3)
+    for a, b in zip(params, want):
+        assert torch.allclose(a, b, rtol=1e-6, atol=1e-7)
+    assert torch.equal(flat[:1], keep[:1]) and torch.equal(flat[270:400], keep[270:400]) and torch.equal(flat[435:], keep[435:])
+    assert adamw_step([], [], [], [], step=1, lr=1.) is None
+    e = torch.zeros(0, device=device)
+    norm = adamw_step([e], [e.clone()], [e.clone()], [e.clone()], step=1, lr=1., max_grad_norm=1.)
+    assert norm == 0
+    on_device = torch.tensor(5, device=device)
+    a, b = [[t.clone() for t in params] for _ in range(2)]
+    for x, s in ((a, 5), (b, on_device)):
+        adamw_step(x, grads, [torch.zeros_like(p) for p in params], [torch.zeros_like(p) for p in params], step=s, lr=1e-3)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    leaf = torch.ones(5, device=device, requires_grad=True)
+    y = (leaf * leaf).sum()
+    adamw_step([leaf], [torch.ones(5, device=device)], [torch.zeros(5, device=device)], [torch.zeros(5, device=device)], step=1, lr=1.)
+    with pytest.raises(RuntimeError):                # what the graph holds has changed
+        y.backward()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    p = [torch.zeros(4, 6, device=device)]
+    z = [torch.zeros(4, 6, device=device)]
+    y = [torch.zeros(4, 6, device=device)]
+    q, s = moments_8bit(p[0])
+    ok = dict(params=p, grads=z, exp_avgs=y, exp_avg_sqs=[y[0].clone()], step=1, lr=.1)
+    wide = torch.zeros(4, 7, device=device)
+    for bad in (dict(params=[p[0].double()]), dict(grads=[]), dict(grads=[z[0].view(-1)]), dict(exp_avgs=[q]), dict(exp_avgs=[y[0].half()]),
+                dict(exp_avgs=[y[0].t()]), dict(params=[wide[:, :6]]), dict(params=[torch.zeros(6, device=device).expand(4, 6)]),
+                dict(exp_avgs=[q], exp_avg_sqs=[q], exp_avg_scales=[s]), dict(exp_avgs=[q], exp_avg_sqs=[q], exp_avg_scales=[s[:0]], exp_avg_sq_scales=[s]),
+                dict(step=0), dict(step=[1, 2]), dict(step=torch.ones(2, dtype=torch.int64, device=device)),
+                dict(step=torch.ones((), device=device)), dict(betas=(1., .9)), dict(lr=-1.), dict(eps=-1.), dict(weight_decay=-1.),
+                dict(max_grad_norm=-1.), dict(lr=math.nan)):
+        with pytest.raises(ValueError):
+            adamw_step(**{**ok, **bad})
+    two = torch.zeros(48, device=device)
+    shared = [two[:24], two[20:44]]
+    others = [[torch.zeros(24, device=device) for _ in range(2)] for _ in range(3)]
+    with pytest.raises(ValueError):
+        adamw_step(shared, *others, step=1, lr=.1)
+    with pytest.raises(ValueError):
+        adamw_step([two, two], *[[torch.zeros(48, device=device) for _ in range(2)] for _ in range(3)], step=1, lr=.1)
+
+
+def _net(device, dtype=torch.float32):
+    torch.manual_seed(4)
+    return nn.Sequential(nn.Conv2d(3, 6, 3), nn.Flatten(), nn.Linear(96, 20), nn.Tanh(), nn.Linear(20, 3)).to(device, dtype)
+
+
+@pytest.mark.parametrize("kind,tol", [("fused", 2e-5), ("fused8", 3e-2)])
+@pytest.mark.parametrize("device", DEVICES)
+def test_optimizer_follows_adam(kind, tol, device):
+    """The same parameters after 20 steps: in fp32 to the rounding of 20 updates of 1e-2 relative to sqrt(v), in 8 bits to
+    their spacing, 2^-4 of 20 updates of 1e-2 and a fraction that averages out."""
+    a, b = _net(device), _net(device)
+    opts = make_optimizer("adam", a.parameters(), 1e-3, 1e-5), make_optimizer(kind, b.parameters(), 1e-3, 1e-5)
+    for i in range(20):
+        x = torch.randn(8, 3, 6, 6, device=device, generator=torch.Generator(device).manual_seed(i))
+        grads = torch.autograd.grad(a(x).square().mean(), list(a.parameters()))
+        for net, opt in zip((a, b), opts):
+            for p, g in zip(net.parameters(), grads):
+                p.grad = g.clone() if not (i == 3 and p.dim() == 1) else None     # some without a gradient once
+            opt.step()
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert (p - q).abs().max() <= tol
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("device", DEVICES)
+def test_optimizer_state(bits, device, tmp_path):
+    torch.manual_seed(0)
+    a, b = _net(device, torch.bfloat16).to(memory_format=torch.channels_last), _net(device, torch.bfloat16).to(memory_format=torch.channels_last)
+    opts = [FusedAdamW(net.parameters(), lr=1e-2, max_grad_norm=.1, state_bits=bits) for net in (a, b)]
+
+    def step(net, opt, i):
+        for n, p in enumerate(net.parameters()):
+            p.grad = torch.randn(p.shape, generator=torch.Generator().manual_seed(100 * i + n)).to(p)
+        opt.step()
+        return opt.last_norms[0].clone()
+
+    for i in range(3):
+        step(a, opts[0], i)
+    torch.save({"net": a.state_dict(), "opt": opts[0].state_dict()}, tmp_path / "s.pt")
+    loaded = torch.load(tmp_path / "s.pt", map_location=device, weights_only=True)
+    b.load_state_dict(loaded["net"])
+    opts[1].load_state_dict(loaded["opt"])
+    for s, t in zip(opts[0].state.values(), opts[1].state.values()):
+        assert s.keys() == t.keys() and all(torch.equal(s[k].float(), t[k].float()) and s[k].dtype == t[k].dtype for k in s if k != "step")
+    for i in range(3, 6):
+        assert torch.equal(step(a, opts[0], i), step(b, opts[1], i))
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert torch.equal(p, q)
+    with pytest.raises(ValueError):
+        FusedAdamW(a.parameters(), state_bits=4)
+    with pytest.raises(ValueError):
+        make_optimizer("sgd", a.parameters(), 1.)
+
+
+@pytest.mark.gpu
+def test_many_tensors_and_unaligned_ones():
+    """More tensors than one launch takes, at every alignment."""
+    sizes = [int(1 + 37 * (i % 50)) for i in range(1203)]
+    buf = torch.randn(sum(sizes) + 1203 * 2, device="cuda")
+    at, params = 0, []
+    for i, n in enumerate(sizes):
+        params.append(buf[at:at + n])
+        at += n + i % 3
+    params.append(torch.randn(100_003, device="cuda"))
+    for bits in (32, 8):
+        lists = [[p.clone() if i % 2 else p for i, p in enumerate(params)], [torch.randn_like(p) for p in params]]
+        lists[0] = [p.clone() if bits == 8 else p for p in lists[0]]
+        if bits == 32:
+            lists += [[torch.randn_like(p) for p in params], [torch.rand_like(p) for p in params], None, None]
+        else:
+            m, v = [moments_8bit(p) for p in params], [moments_8bit(p) for p in params]
+            lists += [[x[0] for x in m], [x[0] for x in v], [x[1] for x in m], [x[1] for x in v]]
+        plain = _copy(lists)
+        opts = dict(lr=1e-2, betas=(.9, .999), eps=1e-8, weight_decay=.01, max_grad_norm=2., seed=3)
+        n1 = adamw_step(*lists, step=3, **opts)
+        n2 = reference_adamw_step(*plain, [3] * len(params), **opts)
+        assert abs(float(n1 / n2) - 1) <= 2 * F
+        for x, y in zip(lists[0], plain[0]):
+            assert torch.allclose(x, y, rtol=1e-6, atol=1e-6)
+        for k in (2, 3):
+            for x, y in zip(lists[k], plain[k]):
+                assert torch.equal(x.float(), y.float()) if bits == 8 else torch.allclose(x, y, rtol=1e-6, atol=1e-7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_streams_and_graphs(bits):
+    lists = _make([(1000,), (77, 5), (4096,)], torch.float32, torch.float32, "cuda", bits)
+    other, plain = _copy(lists), _copy(lists)
+    with pytest.raises(RuntimeError):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            adamw_step(*lists, step=1, lr=.1)
+    torch.cuda.synchronize()
+    step = torch.zeros((), dtype=torch.int64, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step.add_(1)
+        norm = adamw_step(*lists, step=step, lr=.1, max_grad_norm=1.)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for i in range(1, 4):
+        graph.replay()
+        with torch.cuda.stream(side):
+            n2 = adamw_step(*other, step=i, lr=.1, max_grad_norm=1.)
+        n3 = adamw_step(*plain, step=i, lr=.1, max_grad_norm=1.)
+        torch.cuda.synchronize()
+        assert torch.equal(norm, n3) and torch.equal(n2, n3)
+    for a, b, c in zip(lists, other, plain):
+        for x, y, z in zip(a or [], b or [], c or []):
+            assert torch.equal(x.float(), z.float()) and torch.equal(y.float(), z.float())
+
+
+@pytest.mark.gpu
+def test_optimizer_in_a_graph():
+    nets = [_net("cuda") for _ in range(2)]
+    x = torch.randn(8, 3, 6, 6, device="cuda")
+    opts = [FusedAdamW(nets[0].parameters(), lr=1e-2, capturable=True), FusedAdamW(nets[1].parameters(), lr=1e-2)]
+    for net in nets:
+        for p, g in zip(net.parameters(), torch.autograd.grad(nets[0](x).square().mean(), list(nets[0].parameters()))):
+            p.grad = g
+    for opt in opts:
+        opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opts[0].step()
+    for _ in range(3):
+        graph.replay()
+        opts[1].step()
+    torch.cuda.synchronize()
+    for p, q in zip(nets[0].parameters(), nets[1].parameters()):
+        assert torch.allclose(p, q, rtol=0, atol=1e-6)
+    assert int(opts[0].param_groups[0]["step"]) == 4
+
+
+@pytest.mark.gpu
+def test_elements_behind_32_bits():
+    n = (1 << 31) + 700
+    p = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    g = torch.ones(1, dtype=torch.bfloat16, device="cuda").expand(n).contiguous()
+    m, ms = moments_8bit(p)
+    r, rs = moments_8bit(p)
+    norm = adamw_step([p], [g], [m], [r], [ms], [rs], step=1, lr=.5, weight_decay=0., max_grad_norm=1e9)
+    assert abs(float(norm) / math.sqrt(n) - 1) <= 2 * F
+    at = torch.tensor([0, 1 << 30, (1 << 31) - 1, 1 << 31, n - 1], device="cuda")
+    assert torch.equal(p[at], torch.full((5,), -.5, dtype=torch.bfloat16, device="cuda"))
+    assert (m[at].float() == 448).all() and (r[at].float() == 448).all() and (ms[-1] > 0)

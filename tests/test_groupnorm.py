@@ -1,0 +1,324 @@
+"""Group norm with an activation, forward and backward, against 64 bits.
+
+Tolerances, with f = 2^-24 and eps the output type's. Sums: a thread adds up at
+most 64 (or 2^20 / C) values one after the other and joins them over at most 13 levels: S = 96 f
+of the sum of magnitudes. x^ = (x - mean) rstd then has the error of the mean,
+S times the group's mean magnitude, of the variance, S, and three roundings. z
+and the activations (special functions to 2^-21, in bf16 SiLU 2^-10 of tanh)
+have Lipschitz constants of at most 1.1, the slopes of at most 1.1 in z. What is
+added up for the parameters' gradients has the same errors in each term. An
+output is rounded once, eps / 2 of itself. The slope of ReLU jumps: where |z| is
+below its error either value is right, so those elements are set apart in the
+inputs (none lies there).
+"""
+import pytest
+import torch
+from torch import nn
+from torch.nn import functional as F
+
+from autodrive_b200.meco.tracks import make_meco_track
+from autodrive_b200.ops.groupnorm import FusedGroupNorm, fuse_group_norms, group_norm
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.fixture(autouse=True)
+def _full_convolutions():
+    """Convolutions of fp32 tensors may round their operands to 2^-11 (TF32), in one layout and not in another: not here."""
+    with torch.backends.cudnn.flags(enabled=True, benchmark=False, deterministic=True, allow_tf32=False):
+        yield
+
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+S = 96 * 2. ** -24
+ACTS = {None: lambda z: z, "silu": F.silu, "relu": F.relu, "gelu": F.gelu}
+
+
+def _make(shape, groups, dtype, device, offset=0., seed=0, affine=torch.float32):
+    g = torch.Generator().manual_seed(seed + sum(shape) * 7 + groups)
+    n, c, *space = shape
+    x = (torch.randn(n, *space, c, generator=g) * (.5 * torch.randn(c, generator=g)).exp() + offset).to(dtype).to(device).movedim(-1, 1)
+    dy = torch.randn(n, *space, c, generator=g).to(dtype).to(device).movedim(-1, 1)
+    w = (1 + .3 * torch.randn(c, generator=g)).to(affine).to(device) if affine else None
+    b = (.3 * torch.randn(c, generator=g)).to(affine).to(device) if affine else None
+    return x, dy, w, b
+
+
+def _exact(x, groups, w, b, eps, act, dy):
+    x, w, b = (None if t is None else t.detach().double().contiguous().requires_grad_(True) for t in (x, w, b))
+    rows = x.reshape(x.shape[0], groups, -1)
+    mean = rows.mean(-1, keepdim=True)
+    rstd = ((rows - mean).square().mean(-1, keepdim=True) + eps).rsqrt()
+    z = ((rows - mean) * rstd).reshape(x.shape)
+    channels = (1, -1) + (1,) * (x.dim() - 2)
+    if w is not None:
+        z = z * w.view(channels)
+    if b is not None:
+        z = z + b.view(channels)
+    y = ACTS[act](z)
+    grads = torch.autograd.grad(y, [t for t in (x, w, b) if t is not None], dy.double())
+    size = (rows.detach().abs().mean(-1, keepdim=True) * rstd.detach()).expand_as(rows).reshape(x.shape)   # mean |x| / deviation
+    return y.detach(), z.detach(), grads, size, rstd.detach().expand_as(rows).reshape(x.shape)
+
+
+def _check(shape, groups, dtype, device, act, offset=0., affine=torch.float32, eps=1e-5, seed=0):
+    x, dy, w, b = _make(shape, groups, dtype, device, offset, seed, affine)
+    y0, z, g0, size, rstd = _exact(x, groups, w, b, eps, act, dy)
+    half = torch.finfo(dtype).eps / 2
+    tanh = 2. ** -10 if act == "silu" and dtype == torch.bfloat16 else 2. ** -20
+    w1 = 1. if w is None else w.double().view(1, -1, *(1,) * (len(shape) - 2)).abs()
+    dz = (S * (size + 2) * (1 + z.abs()) + 6 * 2. ** -24) * (w1 + 1)          # error of z
+    if act == "relu":                                                          # nothing next to the jump
+        near = z.abs() <= 2 * dz
+        x, dy = x.clone(), torch.where(near, torch.zeros_like(dy), dy)
+        y0, z, g0, size, rstd = _exact(x, groups, w, b, eps, act, dy)
+    ins = [t.requires_grad_(True) for t in (x, w, b) if t is not None]
+    y = group_norm(x, groups, w, b, eps, act)
+    assert y.dtype == dtype and y.shape == x.shape and y.movedim(1, -1).is_contiguous()
+    tol = half * y0.abs() + 1.1 * dz + tanh * (z.abs() + 1)
+    assert ((y.double() - y0).abs() <= tol).all(), float(((y.double() - y0).abs() / tol).max())
+    grads = torch.autograd.grad(y, ins, dy)
+    d = dy.double().abs()
+    # the gradient of z and its error, and those of what it is multiplied with
+    each = d * (1.1 * dz + tanh * (2 + z.abs()) + 4 * 2. ** -24)
+    fine = d * (1.1 * dz + 2. ** -20 * (2 + z.abs()) + 4 * 2. ** -24)
+    dims = [i for i in range(x.dim()) if i != 1]
+    xhat = (z.abs() + 1) / w1
+    for got, want, name in zip(grads, g0, "xwb"):
+        assert got.dtype == {"x": dtype}.get(name, affine)
+        h = torch.finfo(got.dtype).eps / 2
+        if name == "x":
+            per = x.numel() // x.shape[0] // groups
+            def mean(t):
+                return t.reshape(x.shape[0], groups, per).mean(-1, keepdim=True).expand(-1, -1, per).reshape(x.shape)
+            slack = S * (2 + size) * (1 + xhat)
+            tol = h * want.abs() + rstd * w1 * (each + slack * 1.2 * d) + rstd * (
+                mean(w1 * (fine + 3 * slack * 1.2 * d)) * (1 + xhat) + xhat * mean(xhat * w1 * (fine + 3 * slack * 1.2 * d)))
+        elif name == "w":
+            tol = h * want.abs() + (fine * xhat + 1.2 * d * (dz + 3 * S * xhat * (1 + size))).sum(dims)
+        else:
+            tol = h * want.abs() + (fine + 1.2 * d * 3 * S).sum(dims)
+        off = (got.double() - want).abs()
+        assert (off <= tol + 1e-30).all(), (name, float((off / (tol + 1e-30)).max()))
+
+
+SHAPES = [((1, 24, 25, 51), 8), ((3, 24, 25, 51), 8), ((2, 64, 7, 13), 8), ((5, 1, 9, 4), 1), ((2, 3, 5, 7), 3), ((40, 6, 3, 2), 2),
+          ((2, 36, 31, 29), 4), ((3, 20, 17), 5), ((4, 16), 4), ((2, 8, 3, 4, 5), 2), ((1, 130, 11, 3), 13), ((2, 1025, 3, 5), 5),
+          ((300, 32, 2, 3), 32)]
+
+
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("shape,groups", SHAPES)
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_and_gradients(shape, groups, act, device):
+    for n, dtype in enumerate(TYPES):
+        _check(shape, groups, dtype, device, act, seed=n)
+
+
+@pytest.mark.parametrize("affine", [None, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("device", DEVICES)
+def test_parameters_of_other_types_and_none(affine, device):
+    for dtype in TYPES:
+        _check((3, 24, 10, 9), 6, dtype, device, "silu", affine=affine)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_large_means(device):
+    """A mean of many deviations, and a first pixel far from the others."""
+    _check((2, 16, 40, 41), 4, torch.float32, device, "silu", offset=300.)
+    x, dy, w, b = _make((2, 16, 40, 41), 4, torch.float32, device)
+    x[:, :, 0, 0] = 3e4
+    y0, _, _, size, _ = _exact(x, 4, w, b, 1e-5, None, dy)
+    y = group_norm(x, 4, w, b)
+    # the outlier's own square is the variance: a thread's cancellation is the number of its values, at most 64 here
+    assert ((y.double() - y0).abs() <= 64 * S * (size + 2) * (1 + y0.abs())).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_constant_groups_and_non_finite_samples(device):
+    x = torch.randn(4, 8, 6, 5, device=device).contiguous(memory_format=torch.channels_last)
+    x[1] = 2.5
+    y = group_norm(x, 2)
+    assert (y[1] == 0).all() and y.isfinite().all()
+    x[2, 1, 3, 2], x[3, 7, 0, 0] = torch.nan, torch.inf
+    y = group_norm(x, 2, activation="relu")
+    assert y[2, :4].isnan().all() and y[3, 4:].isnan().all()         # their groups
+    assert y[:2].isfinite().all() and y[2, 4:].isfinite().all() and y[3, :4].isfinite().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layouts(device):
+    x, dy, w, b = _make((3, 12, 9, 8), 4, torch.float32, device)
+    want = group_norm(x, 4, w, b, activation="silu")
+    big = torch.zeros(3, 9, 8, 16, device=device)
+    big[..., 1:13] = x.movedim(1, -1)
+    flat = torch.zeros(x.numel() + 1, device=device)
+    flat[1:] = x.movedim(1, -1).reshape(-1)
+    for y in (x.contiguous(), big[..., 1:13].movedim(-1, 1), flat[1:].view(3, 9, 8, 12).movedim(-1, 1), x.flip(0).flip(0)):
+        got = group_norm(y, 4, w, b, activation="silu")
+        assert torch.allclose(got, want, rtol=0, atol=1e-6)
+    for g in (dy, dy.contiguous(), torch.ones(1, device=device).expand_as(dy)):
+        a, c = x.clone().requires_grad_(True), x.detach().double().contiguous().requires_grad_(True)
+        da, = torch.autograd.grad(group_norm(a, 4, w, b), a, g)
+        dc, = torch.autograd.grad(F.group_norm(c, 4, w.double(), b.double()), c, g.double())
+        assert torch.allclose(da.double(), dc, rtol=1e-4, atol=1e-5)
+    none = group_norm(x[:0], 4, w, b)
+    assert none.shape == (0, 12, 9, 8)
+    wg, xe = w.clone().requires_grad_(True), x[:0].clone().requires_grad_(True)
+    dx, dw = torch.autograd.grad(group_norm(xe, 4, wg, b), (xe, wg), none)
+    assert dx.shape == none.shape and (dw == 0).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_differences(device):
+    """The gradient along a direction against the difference of the results, in 32 bits: the differences' own error is
+    the third derivative's, h^2, and the roundings over h."""
+    x, dy, w, b = _make((2, 12, 5, 6), 3, torch.float32, device)
+    for act in (None, "silu", "gelu"):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        grads = torch.autograd.grad(group_norm(leaves[0], 3, *leaves[1:], activation=act), leaves, dy)
+        for i, g in enumerate(grads):
+            v = torch.randn_like(leaves[i])
+            h = 1e-2
+            f = []
+            for sign in (1, -1):
+                moved = [t.detach() + sign * h * v if j == i else t.detach() for j, t in enumerate(leaves)]
+                f.append((group_norm(moved[0], 3, *moved[1:], activation=act).double() * dy.double()).sum())
+            want = float((f[0] - f[1]) / (2 * h))
+            scale = float(g.double().norm() * v.double().norm())
+            assert abs(want - float((g.double() * v.double()).sum())) <= 2e-3 * scale
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    x, w = torch.randn(2, 8, 3, device=device), torch.ones(8, device=device)
+    for call in (lambda: group_norm(x.double(), 2), lambda: group_norm(x[0, 0], 1), lambda: group_norm(x, 3), lambda: group_norm(x, 0),
+                 lambda: group_norm(x, 2, w[:4]), lambda: group_norm(x, 2, w.double()), lambda: group_norm(x, 2, None, w[None]),
+                 lambda: group_norm(x, 2, activation="tanh"), lambda: group_norm(torch.zeros(1, 8193, 1, device=device), 1)):
+        with pytest.raises(ValueError):
+            call()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError):
+            group_norm(dual, 2)
+
+
+@pytest.mark.gpu
+def test_no_second_derivative_and_changed_inputs():
+    x = torch.randn(2, 8, 3, device="cuda", requires_grad=True)
+    y = group_norm(x, 2)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+    a = torch.randn(2, 3, 3, 8, device="cuda").movedim(-1, 1)
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    y = group_norm(a, 2, w)
+    a.add_(1.)
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+
+
+class _Net(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.shared = nn.SiLU()
+        self.a = nn.Sequential(nn.Conv2d(4, 8, 3), nn.GroupNorm(2, 8), nn.SiLU(), nn.Conv2d(8, 6, 1), nn.GroupNorm(3, 6), nn.ReLU(),
+                               nn.GroupNorm(2, 6), nn.Tanh(), nn.GroupNorm(1, 6), nn.GELU(approximate="tanh"))
+        self.b = nn.Sequential(nn.GroupNorm(2, 6), self.shared, nn.GroupNorm(2, 6), self.shared, nn.GroupNorm(6, 6), nn.GELU())
+        self.c = nn.GroupNorm(2, 6, affine=False)
+
+    def forward(self, x):
+        return self.c(self.b(self.a(x)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_fused_modules(device):
+    torch.manual_seed(1)
+    net = _Net().to(device)
+    x = torch.randn(3, 4, 9, 8, device=device)
+    with torch.no_grad():
+        for p in net.parameters():
+            p.add_(.1 * torch.randn_like(p))
+        want = net(x)
+    state, params = {k: v.clone() for k, v in net.state_dict().items()}, list(net.parameters())
+    assert fuse_group_norms(net) is net
+    assert list(net.state_dict()) == list(state) and all(a is b for a, b in zip(net.parameters(), params))
+    assert [m.activation for m in net.modules() if isinstance(m, FusedGroupNorm)] == ["silu", "relu", None, None, None, None, "gelu", None]
+    assert isinstance(net.b[1], nn.SiLU) and isinstance(net.a[2], nn.Identity) and isinstance(net.a[7], nn.Tanh)
+    got = net(x)
+    # seven norms in a row, each with the errors of the last: 2^-24 grows by their Lipschitz constants of about 3
+    assert torch.allclose(got, want, rtol=0, atol=2e-4)
+    net.load_state_dict(state)
+    one = nn.GroupNorm(2, 6)
+    assert isinstance(fuse_group_norms(one), FusedGroupNorm) and fuse_group_norms(one).weight is one.weight
+    hooked = nn.Sequential(nn.GroupNorm(2, 6), nn.ReLU())
+    hooked[0].register_forward_hook(lambda *a: None)
+    assert type(fuse_group_norms(hooked)[0]) is nn.GroupNorm
+    twice = nn.GroupNorm(2, 6)
+    both = nn.Sequential(twice, nn.ReLU(), twice)
+    fuse_group_norms(both)
+    assert both[0] is both[2] and both[0].activation is None and isinstance(both[1], nn.ReLU)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_raster_scorer(device):
+    torch.manual_seed(2)
+    track = make_meco_track("A1").to(device)
+    raster, globals_ = torch.rand(3, 6, 25, 51, device=device), torch.rand(3, 7, device=device)
+    want = track(raster, globals_)
+    grads = torch.autograd.grad(want["utility"].square().mean() + want["penalty"].mean(), list(track.enc0.parameters()))
+    fuse_group_norms(track).to(memory_format=torch.channels_last)
+    assert sum(isinstance(m, FusedGroupNorm) and m.activation == "silu" for m in track.modules()) == 10
+    got = track(raster, globals_)
+    for name in ("utility", "penalty", "hidden"):
+        assert torch.allclose(got[name], want[name], rtol=1e-3, atol=1e-3)
+    again = torch.autograd.grad(got["utility"].square().mean() + got["penalty"].mean(), list(track.enc0.parameters()))
+    for a, b in zip(again, grads):
+        assert (a - b).norm() <= 1e-2 * b.norm() + 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups", [((300, 128, 16, 16), 32), ((3, 36, 257, 263), 4), ((1, 320, 90, 91), 32), ((2, 8192, 3, 3), 1),
+                                          ((1, 4099, 5, 4), 1), ((700, 24, 12, 13), 8), ((1, 2, 1500, 1501), 1)])
+def test_larger(shape, groups):
+    for dtype, act in ((torch.bfloat16, "silu"), (torch.float32, "gelu"), (torch.float16, None)):
+        _check(shape, groups, dtype, "cuda", act)
+
+
+@pytest.mark.gpu
+def test_streams_graphs_and_the_same_results_again():
+    x, dy, w, b = _make((64, 24, 25, 51), 8, torch.float32, "cuda")
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+
+    def step():
+        y = group_norm(*leaves[:1], 8, *leaves[1:], activation="silu")
+        return (y, *torch.autograd.grad(y, leaves, dy))
+
+    want = [t.clone() for t in step()]
+    side = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for r in got for a, b in zip(r, want))
+    x2 = x.detach().clone()
+    with torch.no_grad():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = group_norm(x2, 8, w, b, activation="silu")
+    for scale in (1., 2.):
+        x2.copy_(x.detach() * scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, group_norm(x2, 8, w.detach(), b.detach(), activation="silu"))
+
+
+@pytest.mark.gpu
+def test_samples_behind_32_bits():
+    n = (1 << 31) // (16 * 64 * 64) + 3
+    x = torch.empty(n, 64, 64, 16, dtype=torch.bfloat16, device="cuda").normal_().movedim(-1, 1)
+    y = group_norm(x, 4, activation="silu")
+    at = [0, n // 2, n - 2, n - 1]
+    want = F.silu(F.group_norm(x[at].float(), 4))
+    assert ((y[at].float() - want).abs() <= 2. ** -8 * want.abs() + 2. ** -9).all()

@@ -1,0 +1,286 @@
+"""Sampling with temperature, top-k, top-p and min-p from given numbers, against
+the definition entry by entry in 64 bits.
+
+A token is told apart from its neighbours where the row's number times the sum
+is further than 1e-9 of it from every running sum, and the sum that top_p asks
+for further than 1e-9 from every sum of the order: a sum of V fp64 weights is
+off by at most (V + 4) 2^-52 of itself, 4e-11 at the longest here, each weight by
+2^-45. log_prob: the sum in it may be one of fp32 weights, off by 1.4e-6
+(2^-22 of the exponential, 3 2^-24 of sums, 14 2^-24 of the argument), and the
+result is rounded, 2^-24 of itself.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from autodrive_b200.models.actor_critic import ActorCritic
+from autodrive_b200.models.zoo import PerceptionActorCritic
+from autodrive_b200.ops.sampling import sample_tokens
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+NEAR = 1e-9
+
+
+def _row(x, u, mask, t, k, p, least):
+    """(token, log_prob, whether both are beyond doubt) of one row of 64-bit numbers."""
+    v = len(x)
+    ok = np.ones(v, bool) if mask is None else mask.copy()
+    if (np.isnan(x[ok]) | (x[ok] == np.inf)).any() or not (t == 0 or 1e-30 <= t <= 1e30) or u != u:
+        return -1, math.nan, True
+    ok &= x > -np.inf
+    if not ok.any():
+        return -1, -math.inf, True
+    order = [i for i in np.argsort(-x, kind="stable") if ok[i]]
+    top = x[order[0]]
+    d = np.array([x[i] - top for i in order])
+    if t == 0:
+        return order[0], 0., True
+    d = d / t
+    w = np.exp(d)
+    n = int(((w >= least) & (d >= -44)).sum())     # a prefix of the order
+    sure = least == 0 or bool((abs(w - least) > NEAR * least).all()) or least == 1.
+    if k:
+        n = min(n, k)
+    w = w[:n]
+    if p < 1:
+        run = np.cumsum(w)
+        target = p * run[-1]
+        keep = 1 + int((run[:-1] < target).sum())
+        exact = len(set(w.tolist())) == 1          # sums of equal ones are exact
+        sure &= exact or bool((abs(run - target) > NEAR * run[-1]).all())
+        w, n = w[:keep], keep
+    kept = sorted(zip(order[:n], w))
+    run = np.cumsum([b for _, b in kept])
+    target = max(u, 0.) * run[-1]
+    exact = len(set(w.tolist())) == 1
+    sure &= exact or u >= 1 or u <= 0 or bool((abs(run - target) > NEAR * run[-1]).all())
+    at = min(int((run <= target).sum()), n - 1)
+    return kept[at][0], math.log(kept[at][1]) - math.log(run[-1]), sure
+
+
+def _check(x, u, mask, t, k, p, least, r):
+    rows, v = x.shape
+    each = [np.broadcast_to(z.cpu().numpy() if torch.is_tensor(z) else z, (rows,)) for z in (t, k, p, least)]
+    xs, us = x.double().cpu().numpy(), u.double().cpu().numpy()
+    ms = None if mask is None else mask.expand(rows, v).cpu().numpy()
+    token, log_prob = r.token.cpu().tolist(), r.log_prob.double().cpu().tolist()
+    assert r.token.dtype == torch.int64 and r.log_prob.dtype == torch.float32
+    told = 0
+    for i in range(rows):
+        want, lp, sure = _row(xs[i], us[i], None if ms is None else ms[i], float(each[0][i]), int(each[1][i]),
+                              float(each[2][i]), float(each[3][i]))
+        if not sure:
+            continue
+        told += 1
+        assert token[i] == want, (i, token[i], want, log_prob[i], lp)
+        assert math.isnan(lp) == math.isnan(log_prob[i])
+        if not math.isnan(lp):
+            assert lp == log_prob[i] or abs(lp - log_prob[i]) <= 1.5e-6 + 2. ** -23 * abs(lp), (i, log_prob[i], lp)
+    assert told >= rows * .9
+
+
+def _make(rows, v, dtype, device, seed=0, spread=3.):
+    g = torch.Generator().manual_seed(seed + 11 * rows + v)
+    x = (spread * torch.randn(rows, v, generator=g)).to(dtype).to(device)
+    return x, torch.rand(rows, generator=g).to(device), g
+
+
+SIZES = [(1, 1), (9, 2), (40, 8), (33, 31), (12, 33), (20, 128), (20, 129), (12, 1000), (9, 2049), (5, 8193), (3, 40001)]
+CUTS = [(1., 0, 1., 0.), (.7, 5, 1., 0.), (1., 0, .9, 0.), (1.5, 0, 1., .05), (.7, 50, .9, .01), (0., 7, .3, .5), (1., 1, 1., 0.),
+        (2., 0, 0., 0.), (1., 0, 1., 1.), (3., 700, .99, 0.)]
+
+
+@pytest.mark.parametrize("cut", CUTS)
+@pytest.mark.parametrize("rows,v", SIZES)
+@pytest.mark.parametrize("device", DEVICES)
+def test_cuts(rows, v, cut, device):
+    for n, dtype in enumerate(TYPES):
+        x, u, _ = _make(rows, v, dtype, device, seed=n)
+        _check(x, u, None, *cut, sample_tokens(x, u, None, *cut))
+
+
+@pytest.mark.parametrize("v", [3, 8, 100, 513, 5000])
+@pytest.mark.parametrize("device", DEVICES)
+def test_masks_and_layouts(v, device):
+    for n, dtype in enumerate(TYPES):
+        x, u, g = _make(28, v, dtype, device, seed=n)
+        mask = (torch.rand(28, v, generator=g) < .5).to(device)
+        mask[3::7] = False
+        x = torch.where(mask, x, torch.nan)                         # what is masked is not read
+        cut = (.8, 9, .95, 0.)
+        r = sample_tokens(x, u, mask, *cut)
+        _check(x, u, mask, *cut, r)
+        assert (r.token[3::7] == -1).all() and (r.log_prob[3::7] == -torch.inf).all()
+        assert mask[torch.arange(28, device=device), r.token.clamp_min(0)].eq(r.token >= 0).all()
+        # the type's lowest value instead of a mask: a row of them alone is a row of equals
+        low = torch.where(mask, x, torch.finfo(dtype).min)
+        _check(low, u, None, *cut, sample_tokens(low, u, None, *cut))
+        # rows of a wider matrix, every second row, a transposed matrix, a mask that broadcasts, more dimensions
+        x = _make(28, v, dtype, device, seed=9 + n)[0]
+        wide = torch.zeros(28, v + 3, dtype=dtype, device=device)
+        wide[:, 1:v + 1] = x
+        want = sample_tokens(x, u, mask[:1], *cut)
+        _check(x, u, mask[:1], *cut, want)
+        for y in (wide[:, 1:v + 1], torch.stack((x, x), 1)[:, 0], x.t().contiguous().t()):
+            got = sample_tokens(y, u, mask[:1], *cut)
+            assert torch.equal(got.token, want.token) and torch.equal(got.log_prob, want.log_prob)
+        got = sample_tokens(x.view(4, 7, v), u.view(4, 7), mask[0], *cut)
+        assert got.token.shape == (4, 7) and torch.equal(got.token.view(-1), want.token)
+        one = sample_tokens(x[4], u[4], mask[0], *cut)
+        assert one.token.shape == () and one.token == want.token[4]
+        none = sample_tokens(x[:0], u[:0])
+        assert none.token.shape == none.log_prob.shape == (0,)
+
+
+@pytest.mark.parametrize("v", [5, 40, 300, 9000])
+@pytest.mark.parametrize("device", DEVICES)
+def test_ties_and_flat_rows(v, device):
+    """Many entries on a border, which are ordered by their index, and borders among entries that nearly agree."""
+    for n, dtype in enumerate(TYPES):
+        x, u, _ = _make(16, v, dtype, device, seed=n)
+        for cut in ((1., v // 2 + 1, 1., 0.), (1., 0, .5, 0.), (.5, v // 3 + 1, .7, 0.), (1e30, 2, 1., 0.), (1e-30, 0, .9, 0.)):
+            for y in (x.round(), torch.full_like(x, -2.5), (x * 1e-3)):
+                if y is not x and y.unique().numel() == 1 and cut[2] == .7:
+                    continue                                        # .7 of a whole number of ones hangs on a rounding
+                _check(y, u, None, *cut, sample_tokens(y, u, None, *cut))
+
+
+@pytest.mark.parametrize("v", [8, 200, 3001])
+@pytest.mark.parametrize("device", DEVICES)
+def test_parameters_of_each_row_and_numbers_at_the_ends(v, device):
+    x, u, g = _make(36, v, torch.float32, device)
+    u = u.double()
+    u[::6], u[1::6], u[2::6] = 0., 1., -3.
+    t = (torch.rand(36, generator=g) + .1).to(device)
+    t[::5] = 0.
+    k = torch.randint(0, v + 2, (36,), generator=g).to(device)
+    p, least = torch.rand(36, generator=g).to(device), (.1 * torch.rand(36, generator=g)).to(device)
+    _check(x, u, None, t, k, p, least, sample_tokens(x, u, None, t, k, p, least))
+    _check(x, u, None, t, k, 1., 0., sample_tokens(x, u, None, t, k.int()))
+
+
+@pytest.mark.parametrize("v", [4, 60, 700])
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_without_an_answer(v, device):
+    x, u, _ = _make(8, v, torch.float32, device)
+    x[0, v // 2], x[1, 0], x[2] = torch.nan, torch.inf, -torch.inf
+    u[3] = torch.nan
+    t = torch.ones(8, device=device)
+    t[4], t[5], t[6] = -1., torch.nan, torch.inf
+    r = sample_tokens(x, u, None, t)
+    assert r.token[:7].tolist() == [-1] * 7 and r.token[7] >= 0
+    assert r.log_prob[[0, 1, 3, 4, 5, 6]].isnan().all() and r.log_prob[2] == -torch.inf
+    few = x.clone()
+    few[7, 1:] = -torch.inf                                          # one entry is left
+    r = sample_tokens(few, u, None, 1., 0, .5)
+    assert r.token[7] == 0 and r.log_prob[7] == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    x, u = torch.zeros(3, 5, device=device), torch.zeros(3, device=device)
+    for bad in (dict(logits=x.double()), dict(logits=x[:, :0]), dict(logits=torch.tensor(1., device=device)), dict(uniforms=u[:2]),
+                dict(uniforms=u.half()), dict(uniforms=u.long()), dict(mask=x), dict(mask=torch.ones(2, 5, dtype=torch.bool, device=device)),
+                dict(mask=torch.ones(1, 3, 5, dtype=torch.bool, device=device)), dict(temperature=-1.), dict(temperature=1e-31),
+                dict(temperature=math.nan), dict(temperature=1e31), dict(top_k=-1), dict(top_p=1.1), dict(top_p=-.1),
+                dict(min_p=2.), dict(min_p=math.nan), dict(temperature=u[:2]), dict(temperature=u.double()), dict(top_k=u),
+                dict(top_p=u.half()), dict(min_p=torch.zeros(3, 1, device=device)), dict(logits=x.clone().requires_grad_(True))):
+        with pytest.raises(ValueError):
+            sample_tokens(**{"logits": x, "uniforms": u, **bad})
+    with torch.no_grad():
+        sample_tokens(x.clone().requires_grad_(True), u)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_policies_draw(device):
+    torch.manual_seed(3)
+    policy = ActorCritic(12, 8, "categorical").to(device)
+    obs, mask = torch.randn(50, 12, device=device), torch.rand(50, 8, device=device) < .5
+    mask[7] = False
+    u = torch.rand(50, device=device)
+    action, log_prob, value = policy.draw(obs, u, temperature=.5, top_k=3, action_mask=mask)
+    logits, _, v = policy(obs)
+    used = mask | ~mask.any(-1, keepdim=True)
+    with torch.no_grad():
+        _check(logits, u, used, .5, 3, 1., 0., sample_tokens(logits, u, used, .5, 3))
+        want = sample_tokens(logits, u, used, .5, 3)
+    assert torch.equal(action, want.token) and torch.equal(log_prob, want.log_prob) and torch.allclose(value, v)
+    assert not log_prob.requires_grad
+    greedy = policy.draw(obs, temperature=0.)[0]
+    assert torch.equal(greedy, logits.argmax(-1))
+    with pytest.raises(ValueError):
+        ActorCritic(12, 3).to(device).draw(obs)
+    net = PerceptionActorCritic("deep_sets", tensor_cores=False).to(device)
+    inputs = {"scalars": torch.rand(6, 137, device=device), "entities": torch.randn(6, 5, 12, device=device),
+              "entity_mask": torch.ones(6, 5, dtype=torch.bool, device=device)}
+    action, log_prob, value = net.draw(inputs, u[:6])
+    valid = inputs["scalars"][:, -8:] > .5
+    assert (valid[torch.arange(6, device=device), action] | ~valid.any(-1)).all() and (log_prob <= 0).all()
+
+
+def test_frequencies():
+    """Evenly spread numbers meet each entry as often as its share says, to one of them for each border."""
+    x = torch.tensor([[.5, -1., 2., 0., 1.]])
+    n = 10_000
+    u = (torch.arange(n, dtype=torch.float64) + .5) / n
+    token = sample_tokens(x.expand(n, 5), u, None, .8).token
+    share = torch.softmax(x[0].double() / .8, -1)
+    assert ((torch.bincount(token, minlength=5) / n - share).abs() <= 1. / n + 1e-9).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v,k", [(200_003, 50), (131_072, 0), (70_000, 20_000)])
+def test_long_rows_shared_by_ctas(v, k):
+    for rows in (1, 2, 5, 40):
+        x, u, _ = _make(rows, v, torch.bfloat16, "cuda")
+        for cut in ((.7, k, .9, 0.), (1., k, 1., .001)):
+            _check(x, u, None, *cut, sample_tokens(x, u, None, *cut))
+
+
+@pytest.mark.gpu
+def test_rows_are_answered_alike_however_many_there_are():
+    x, u, _ = _make(600, 9001, torch.bfloat16, "cuda")
+    for cut in ((1., 0, .9, 0.), (.7, 40, 1., 0.), (1., 0, 1., 0.)):
+        many = sample_tokens(x, u, None, *cut)
+        for i in (0, 17, 599):
+            one = sample_tokens(x[i:i + 1], u[i:i + 1], None, *cut)
+            assert one.token == many.token[i] and abs(float(one.log_prob - many.log_prob[i])) <= 3e-6
+        again = sample_tokens(x, u, None, *cut)
+        assert torch.equal(again.token, many.token) and torch.equal(again.log_prob, many.log_prob)
+
+
+@pytest.mark.gpu
+def test_streams_graphs_and_two_at_once():
+    x, u, _ = _make(64, 6000, torch.float32, "cuda")
+    want = sample_tokens(x, u, None, .9, 30, .95)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append([sample_tokens(x, u, None, .9, 30, .95) for _ in range(3)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(r.token, want.token) and torch.equal(r.log_prob, want.log_prob) for rs in got for r in rs)
+    held = u.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        r = sample_tokens(x, held, None, .9, 30, .95)
+    for shift in (0., .25):
+        held.copy_((u + shift) % 1.)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = sample_tokens(x, held, None, .9, 30, .95)
+        assert torch.equal(r.token, eager.token) and torch.equal(r.log_prob, eager.log_prob)
+
+
+@pytest.mark.gpu
+def test_rows_behind_32_bits():
+    n, v = (1 << 31) // 5000 + 3, 5000
+    x = torch.empty(n, v, dtype=torch.bfloat16, device="cuda").normal_()
+    u = torch.rand(n, device="cuda")
+    r = sample_tokens(x, u, None, 1., 20, .9)
+    at = torch.tensor([0, n // 2, n - 2, n - 1], device="cuda")
+    _check(x[at], u[at], None, 1., 20, .9, 0., type(r)(r.token[at], r.log_prob[at]))
