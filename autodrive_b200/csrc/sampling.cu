@@ -262,16 +262,17 @@ __global__ void __launch_bounds__(128) short_kernel(const __grid_constant__ Args
 constexpr int kList = 256;      // entries of a border's neighbourhood that are ordered one by one
 constexpr float kSlack = 2e-5f; // of sums of fp32 estimates of weights
 // Relative error of a sum of of32() over at most 2^20 entries: 2^-22 of the
-// exponential, 3 * 2^-24 of sums of eight, and the rounding of top - l, 2^-24 |x|,
+// exponential, 8 * 2^-24 of sums of 256, and the rounding of top - l, 2^-24 |x|,
 // where the mean of |x| over the weights is at most the logarithm of their
 // number (it is the distribution's entropy less log S, and S >= 1): 14 * 2^-24.
-constexpr double kError = 1.4e-6;
+constexpr double kError = 1.7e-6;
 constexpr int64_t kMost32 = 1 << 20;
 
 struct Plan {
   int threads, ctas;    // of a row
   int strips;           // of 32 vectors of 8 entries, of a warp
   int listed;           // entries that a warp's list holds
+  int bins;             // of the order
 };
 
 // What the threads of a CTA share; `val`, `flag` and `list` are read by the row's other CTAs.
@@ -301,7 +302,8 @@ template <typename T>
 struct RowOf {
   const Args& a;
   Shared& s;
-  uint32_t* hist;
+  uint32_t *hist, *joined;   // this CTA's bins, and the row's
+  float* strip_sum;     // of this warp's strips
   T* list_value;        // of this warp
   uint16_t* list_index; // within this warp's strips
   const int64_t row;
@@ -318,8 +320,15 @@ struct RowOf {
   __device__ RowOf(const Args& a_, Shared& s_, unsigned char* raw, const Plan& p)
       : a(a_), s(s_), row(blockIdx.x / p.ctas), strips(p.strips), capacity(p.listed), tid(threadIdx.x),
         lane(threadIdx.x & 31), warp(threadIdx.x >> 5), warps(blockDim.x >> 5), rank(blockIdx.x % p.ctas), ctas(p.ctas) {
-    hist = reinterpret_cast<uint32_t*>(raw);
-    raw += sizeof(uint32_t) * 8 * blockDim.x;
+    bins = p.bins;
+    hist = joined = reinterpret_cast<uint32_t*>(raw);
+    raw += sizeof(uint32_t) * bins;
+    if (ctas > 1) {
+      joined = reinterpret_cast<uint32_t*>(raw);
+      raw += sizeof(uint32_t) * bins;
+    }
+    strip_sum = reinterpret_cast<float*>(raw) + warp * strips;
+    raw += sizeof(float) * warps * strips;
     list_value = reinterpret_cast<T*>(raw) + warp * capacity;
     list_index = reinterpret_cast<uint16_t*>(raw + sizeof(T) * warps * capacity) + warp * capacity;
     x = static_cast<const T*>(a.logits) + row * a.ld;
@@ -382,8 +391,8 @@ struct RowOf {
     }
   }
 
-  // The sum of f(entry) in fp32 over a thread's eight, and in fp64 beyond.
-  template <typename F>
+  // The sum of f(entry) in fp32 over a thread's eight, and in fp64 beyond; KEEP: and those of the strips.
+  template <bool KEEP, typename F>
   __device__ __forceinline__ double mass(F&& f) const {
     double s = 0.;
     for (int k = 0; k < strips; ++k) {
@@ -391,7 +400,12 @@ struct RowOf {
       load(k, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = f(v[e]);
-      s += (double)(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])));
+      float eight = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+      s += (double)eight;
+      if constexpr (KEEP) {
+        eight = lm::warp_sum(eight);
+        if (lane == 0) strip_sum[k] = eight;
+      }
     }
     return s;
   }
@@ -488,35 +502,35 @@ struct RowOf {
 
   __device__ void clear() {
     sync();   // the row's other CTAs have read it
-    reinterpret_cast<uint4*>(hist)[tid] = reinterpret_cast<uint4*>(hist)[blockDim.x + tid] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < bins / 4; i += blockDim.x) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
     if (tid == 0) s.listed = 0;
     __syncthreads();
   }
   // Joins the row's bins and finds, by weight or by number, the bins [first,
-  // last] in which the border may lie; `under`: entries
-  // in them, `before`: above them, `all`: in all bins.
+  // last] in which the border may lie; `under`: entries in them, `before`:
+  // above them, `all`: in all bins. A thread looks at a stretch of the bins.
   __device__ __noinline__ void find(bool by_weight, bool second, int64_t number, float low, float high) {
     sync();
-    uint32_t c[8];
+    const int per = bins / (int)blockDim.x;   // a multiple of 8
     const float unit = second ? step2 : step, from = second ? (float)b1 * step : 0.f;
-    float h = 0.f;
+    const float ratio = __expf(-unit), head = __expf(-(from + (float)(tid * per) * unit));
+    uint4* const mine = reinterpret_cast<uint4*>(joined) + tid * per / 4;
+    float h = 0.f, f = head;
     int n = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = 0;
-#pragma unroll 4
-    for (int k = 0; k < ctas; ++k) {
-      const uint4* p = reinterpret_cast<const uint4*>(at(hist, k)) + tid * 2;
-      const uint4 x = p[0], y = p[1];
-      c[0] += x.x, c[1] += x.y, c[2] += x.z, c[3] += x.w, c[4] += y.x, c[5] += y.y, c[6] += y.z, c[7] += y.w;
-    }
-    const float head = __expf(-(from + (float)(tid * 8) * unit)), ratio = __expf(-unit);
-    float part[8], f = head;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      n += (int)c[i];
-      part[i] = (float)c[i] * f;
-      h += part[i];
+    const auto add = [&](uint32_t c) {
+      n += (int)c;
+      h += (float)c * f;
       f *= ratio;
+    };
+    for (int q = 0; q < per / 4; ++q) {
+      uint4 c = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+      for (int k = 0; k < ctas; ++k) {
+        const uint4 x = reinterpret_cast<const uint4*>(at(hist, k))[tid * per / 4 + q];
+        c.x += x.x, c.y += x.y, c.z += x.z, c.w += x.w;
+      }
+      if (ctas > 1) mine[q] = c;
+      add(c.x), add(c.y), add(c.z), add(c.w);
     }
     // sums of the threads before this one
     float hs = h;
@@ -528,7 +542,7 @@ struct RowOf {
       if (lane >= o) hs += x, ns += y;
     }
     if (lane == 31) s.fred[warp] = hs, s.ired[warp] = ns;
-    if (tid == 0) s.first = s.last = bins - 1, s.under = s.before = 0;
+    if (tid == 0) s.first = s.last = bins - 1, s.under = 0;
     __syncthreads();
     float total = 0.f;
     int all = 0;
@@ -541,35 +555,39 @@ struct RowOf {
     ns -= n;
     const float shrink = ratio * (1.f - kSlack);
     if (by_weight && !second) low *= total * shrink, high *= total * (1.f + kSlack);
-    const int n0 = ns;
     int low_at = bins - 1, high_at = bins - 1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      ns += (int)c[i];
-      hs += part[i];
-      const bool one = ns > 0 && (by_weight ? hs * (1.f + kSlack) >= low : ns >= number);
-      const bool two = ns > 0 && (by_weight ? hs * shrink >= high : ns >= number);
-      if (one) low_at = min(low_at, tid * 8 + i);
-      if (two) high_at = min(high_at, tid * 8 + i);
+    f = head;
+    n = ns;
+    h = hs;
+    const auto look = [&](uint32_t c, int b) {
+      add(c);
+      const bool one = n > 0 && (by_weight ? h * (1.f + kSlack) >= low : n >= number);
+      const bool two = n > 0 && (by_weight ? h * shrink >= high : n >= number);
+      if (one) low_at = min(low_at, b);
+      if (two) high_at = min(high_at, b);
+    };
+    for (int q = 0; q < per / 4; ++q) {
+      const uint4 c = mine[q];
+      const int b = tid * per + q * 4;
+      look(c.x, b), look(c.y, b + 1), look(c.z, b + 2), look(c.w, b + 3);
     }
     low_at = __reduce_min_sync(0xffffffffu, low_at);
     high_at = __reduce_min_sync(0xffffffffu, high_at);
     if (lane == 0) atomicMin(&s.first, low_at), atomicMin(&s.last, high_at);
     __syncthreads();
     const int first = s.first, last = max(s.first, s.last);
-    int in = 0, ahead = 0;
-    ns = n0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int b = tid * 8 + i;
-      if (b >= first && b <= last) in += (int)c[i];
-      if (b < first) ahead += (int)c[i];
+    const uint32_t* bin_at = reinterpret_cast<const uint32_t*>(mine);
+    if (first / per == tid || last / per == tid) {   // the entries before the first bin, and up to the last
+      int before = ns, upto = ns;
+      for (int i = 0; i < per; ++i) {
+        if (tid * per + i < first) before += (int)bin_at[i];
+        if (tid * per + i <= last) upto += (int)bin_at[i];
+      }
+      if (first / per == tid) s.before = before;
+      if (last / per == tid) s.under = upto;
     }
-    in = __reduce_add_sync(0xffffffffu, in);
-    ahead = __reduce_add_sync(0xffffffffu, ahead);
-    if (lane == 0) atomicAdd(&s.under, in), atomicAdd(&s.before, ahead);
     __syncthreads();
-    if (tid == 0) s.last = last, s.all = all;
+    if (tid == 0) s.last = last, s.all = all, s.under -= s.before;
     __syncthreads();
   }
 
@@ -603,11 +621,13 @@ struct RowOf {
       }
       const int strip = __shfl_sync(0xffffffffu, at, 31);
       at += n - own;
-      for (; take; take &= take - 1, ++at) {
-        const int e = __ffs(take) - 1;
-        if (at >= me.capacity) break;
-        me.list_value[at] = lm::from_f<T>(me.single(k, e));
-        me.list_index[at] = (uint16_t)(k * 256 + me.lane * 8 + e);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if ((take >> e & 1) && at < me.capacity) {
+          me.list_value[at] = lm::from_f<T>(v[e]);
+          me.list_index[at] = (uint16_t)(k * 256 + me.lane * 8 + e);
+        }
+        at += take >> e & 1;
       }
       n += strip;
     }
@@ -642,7 +662,7 @@ struct RowOf {
       const RowOf me = *this;   // a copy whose members are registers
       if constexpr (!LIST) {
         if (rough) {
-          sum_of = me.mass([&](float l) {
+          sum_of = me.template mass<false>([&](float l) {
             if (!me.stays(l)) return 0.f;
             atomicAdd(&me.hist[me.bin(l)], 1u);
             return me.w.of32(l);
@@ -702,7 +722,7 @@ struct RowOf {
     clear();
     if (by_weight || again) {
       const RowOf me = *this;   // a copy whose members are registers
-      me.template each_single<LIST>([&](float l, int, int) {
+      me.template each<LIST>([&](float l, int, int) {
         if (!me.stays(l)) return;
         const int b = me.bin(l);
         if (by_weight && b < me.b1) above += me.w.of(l);
@@ -733,7 +753,7 @@ struct RowOf {
       const RowOf me = *this;   // a copy whose members are registers
       int* number = at(&s.listed, 0);
       uint32_t *keys = at(s.list_key, 0), *places = at(s.list_at, 0);
-      me.template each_single<LIST>([&](float l, int k, int e) {
+      me.template each<LIST>([&](float l, int k, int e) {
         if (!me.stays(l)) return;
         const int at_side = me.side(l);
         if (at_side == 0) {
@@ -889,7 +909,7 @@ struct RowOf {
           if (is_above(l)) above += me.w.of(l);
         });
       } else {
-        above = me.mass([&](float l) { return is_above(l) ? me.w.of32(l) : 0.f; });
+        above = me.template mass<true>([&](float l) { return is_above(l) ? me.w.of32(l) : 0.f; });
       }
     }
     above = warp_sum(above);
@@ -965,7 +985,14 @@ struct RowOf {
     uint32_t token = 0;
     float token_logit = 0.f;
     double end = 0., last = 0.;   // the running sum behind the token, and its weight
-    for (int k = 0; k < n_steps; ++k) {
+    int k = 0;
+    if constexpr (!EXACT) {   // the strip that holds the target by the strips' sums, up to their error
+      if (!me.most) {
+        __syncwarp();
+        while (k + 1 < n_steps && start + (double)me.strip_sum[k] <= target) start += (double)me.strip_sum[k++];
+      }
+    }
+    for (; k < n_steps; ++k) {
       float v[N];
       double x[N];
       me.template fetch<LIST>(k, v);
@@ -1085,7 +1112,6 @@ struct RowOf {
       return;
     }
     w.set(m, r, true);
-    bins = 8 * blockDim.x;
     if (r.t == 0.) {   // the first of the largest
       set_border(key_of(m));
       most = 1;
@@ -1113,7 +1139,7 @@ __global__ void __launch_bounds__(512, 2) row_kernel(const __grid_constant__ Arg
 template <typename T>
 cudaError_t launch_rows(const Args& a, const Plan& p, cudaStream_t st) {
   const auto kernel = row_kernel<T>;
-  const int smem = 32 * p.threads + p.threads / 32 * p.listed * ((int)sizeof(T) + 2);
+  const int smem = (p.ctas > 1 ? 8 : 4) * p.bins + p.strips * p.threads / 8 + p.threads / 32 * p.listed * ((int)sizeof(T) + 2);
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -1136,6 +1162,7 @@ Plan plan(const Args& a, int sms) {
   // 32003 60 % of this time and more; twice as many 40 % and 15 % more.
   p.threads = a.v <= 2048 ? 64 : a.v <= 8192 ? 128 : 256;
   const int64_t vectors = (a.v + 14) / 8;   // with what lies before a row's start
+  p.bins = std::max(2048, 8 * p.threads);
   p.ctas = 1;
   const auto strips = [&] { return (int)((vectors + (int64_t)p.ctas * p.threads - 1) / ((int64_t)p.ctas * p.threads)); };
   while (p.ctas < 8 && a.rows * p.ctas * 2 <= sms && strips() > 2) p.ctas *= 2;   // few rows are shared by more CTAs
