@@ -147,6 +147,11 @@ __device__ __forceinline__ double warp_sum(double s) {
   return s;
 }
 
+// What a running sum has to exceed; from 1 on no rounding of theirs does, and the last entry is taken.
+__device__ __forceinline__ double target_of(double u, double total) {
+  return u < 1. ? u * total : __longlong_as_double(0x7ff0000000000000ll);
+}
+
 template <typename T>
 __device__ __forceinline__ float logit(const Args& a, int64_t row, int64_t i) {
   if (a.mask && !a.mask[row * a.mask_row + i * a.mask_col]) return -INFINITY;
@@ -243,7 +248,7 @@ __global__ void __launch_bounds__(128) short_kernel(const __grid_constant__ Args
     run[j] += start;
     start = __shfl_sync(group, run[j], base + W - 1);
   }
-  const double target = r.u * start;
+  const double target = target_of(r.u, start);
   int token = -1, last = -1;
 #pragma unroll
   for (int j = E - 1; j >= 0; --j) {
@@ -483,14 +488,39 @@ struct RowOf {
   __device__ __forceinline__ int bin2(float l) const {
     return min(bins - 1, (int)__fmul_rn(__fsub_rn(w.place(l), (float)b1), scale2));
   }
-  // -1 above the window, 0 in it, 1 below
-  __device__ __forceinline__ int side(float l) const {
+  // The window as logits: entries from `above` on are above it, those from `within` on in it.
+  float above = 0.f, within = 0.f;
+  // The smallest logit that stays and for which f holds, as it does for all larger ones: a search of 32 ways.
+  template <typename F>
+  __device__ __forceinline__ float lowest_where(F&& f) const {
+    uint32_t lo = key_of(least), hi = key_of(w.top32);
+    while (lo < hi) {
+      const uint32_t step = (hi - lo) / 32 + 1, mine = min(lo + lane * step, hi);
+      const unsigned holds = __ballot_sync(0xffffffffu, f(value_of(mine)));
+      const int first = holds ? __ffs(holds) - 1 : 32;
+      if (first == 0) break;
+      hi = min(hi, first < 32 ? lo + first * step : hi);
+      lo = min(lo + (first - 1) * step + 1, hi);
+    }
+    return value_of(lo);
+  }
+  // Whether the border's own logit (the lowest that stays) is in the window, or above it.
+  __device__ __forceinline__ int side_of_border() const {
+    const float l = value_of(border);
     const int b = bin(l);
     if (b < b1) return -1;
     if (b > b2) return 1;
-    if (!fine) return 0;
-    const int c = bin2(l);
-    return c < c1 ? -1 : c > c2 ? 1 : 0;
+    const int c = fine ? bin2(l) : 0;
+    return fine && c < c1 ? -1 : fine && c > c2 ? 1 : 0;
+  }
+  __device__ __forceinline__ void set_window() {
+    if (fine) {
+      above = b1 == 0 && c1 == 0 ? INFINITY : lowest_where([&](float l) { return bin(l) < b1 || (bin(l) <= b2 && bin2(l) < c1); });
+      within = lowest_where([&](float l) { return bin(l) < b1 || (bin(l) <= b2 && bin2(l) <= c2); });
+    } else {
+      above = b1 == 0 ? INFINITY : lowest_where([&](float l) { return bin(l) < b1; });
+      within = b2 == bins - 1 ? least : lowest_where([&](float l) { return bin(l) <= b2; });
+    }
   }
   __device__ __forceinline__ bool stays(float l) const { return l >= least; }
   __device__ __forceinline__ void set_border(uint32_t key) {
@@ -498,6 +528,12 @@ struct RowOf {
     // comparisons take what is below 2^-126 for zero, so the next number above zero is that one
     const uint32_t next = key >= 0x80000000u && key < 0x80800000u ? 0x80800000u : key + 1;
     least = key < key_of(w.top32) ? value_of(next) : INFINITY;
+  }
+
+  // An entry's weight in fp64 if it is at least `from`, and 0 otherwise, without a branch.
+  __device__ __forceinline__ double weight_from(float l, float from) const {
+    const double x = w.of(fmaxf(l, from));
+    return l >= from ? x : 0.;
   }
 
   __device__ void clear() {
@@ -596,22 +632,12 @@ struct RowOf {
   __device__ __noinline__ bool compact() {
     const RowOf me = *this;   // a copy whose members are registers
     int n = 0;
-    float lowest = least;   // of the window: by halving, as the bins' rounding has it
-    if (b2 < bins - 1) {
-      uint32_t lo = key_of(least), hi = key_of(w.top32);
-      while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (me.w.place(value_of(mid)) < (float)(b2 + 1)) hi = mid;
-        else lo = mid + 1;
-      }
-      lowest = value_of(lo);
-    }
     for (int k = 0; k < me.strips; ++k) {
       float v[8];
       me.load(k, v);
       unsigned take = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) take |= (unsigned)(v[e] >= lowest) << e;
+      for (int e = 0; e < 8; ++e) take |= (unsigned)(v[e] >= me.within) << e;
       const int own = __popc(take);
       int at = own;
 #pragma unroll
@@ -640,8 +666,8 @@ struct RowOf {
   __device__ __noinline__ double total() {
     const RowOf me = *this;   // a copy whose members are registers
     double x = 0.;
-    me.template each_single<LIST>([&](float l, int, int) {
-      if (me.stays(l)) x += me.w.of(l);
+    me.template each<LIST>([&](float l, int, int) {
+      x += me.weight_from(l, me.least);
     });
     x = sum(x);
     return most ? x + (double)most * w.of(value_of(border)) : x;
@@ -663,9 +689,10 @@ struct RowOf {
       if constexpr (!LIST) {
         if (rough) {
           sum_of = me.template mass<false>([&](float l) {
-            if (!me.stays(l)) return 0.f;
-            atomicAdd(&me.hist[me.bin(l)], 1u);
-            return me.w.of32(l);
+            const bool in = me.stays(l);
+            if (in) atomicAdd(&me.hist[me.bin(l)], 1u);
+            const float x = me.w.of32(fmaxf(l, me.least));
+            return in ? x : 0.f;
           });
         }
       }
@@ -680,6 +707,7 @@ struct RowOf {
     b2 = s.last;
     if (!by_weight && s.all <= k) return LIST;
     const int64_t in = s.under, before = s.before;
+    set_window();
     bool held = LIST;
     if constexpr (!LIST) {
       // (entries on an older border are in no list, so it has to be the first)
@@ -712,9 +740,9 @@ struct RowOf {
   template <bool ALL, bool LIST>
   __device__ __noinline__ void narrow(bool by_weight, int64_t k, Aim aim, int64_t in, int64_t before) {
     const float on = value_of(border);
-    const bool again = in > kList && step > 0.f;
+    const bool again = in > kList && step > 0.f;   // (as it stands, all of the window stays: it is above the border)
     // the sum of those above the window, and the window's own bins
-    double above = 0.;
+    double ahead = 0.;
     if (again) {
       scale2 = (float)bins / (float)(b2 - b1 + 1);
       step2 = step / scale2;
@@ -722,23 +750,26 @@ struct RowOf {
     clear();
     if (by_weight || again) {
       const RowOf me = *this;   // a copy whose members are registers
-      me.template each<LIST>([&](float l, int, int) {
-        if (!me.stays(l)) return;
-        const int b = me.bin(l);
-        if (by_weight && b < me.b1) above += me.w.of(l);
-        if (again && b >= me.b1 && b <= me.b2) atomicAdd(&me.hist[me.bin2(l)], 1u);
-      });
-      const int b = most ? bin(on) : -1;
-      if (again && b >= b1 && b <= b2 && rank == 0 && tid == 0) atomicAdd(&hist[bin2(on)], (uint32_t)most);
       if (by_weight) {
-        above = sum(above);
-        if (b >= 0 && b < b1) above += (double)most * w.of(on);
+        me.template each<LIST>([&](float l, int, int) {
+          ahead += me.weight_from(l, me.above);
+          if (again && l >= me.within && l < me.above) atomicAdd(&me.hist[me.bin2(l)], 1u);
+        });
+      } else {
+        me.template each<LIST>([&](float l, int, int) {
+          if (l >= me.within && l < me.above) atomicAdd(&me.hist[me.bin2(l)], 1u);
+        });
+      }
+      if (again && most && side_of_border() == 0 && rank == 0 && tid == 0) atomicAdd(&hist[bin2(on)], (uint32_t)most);
+      if (by_weight) {
+        ahead = sum(ahead);
+        if (most && side_of_border() < 0) ahead += (double)most * w.of(on);
       }
     }
     int64_t need = k - before;   // by number: of the window's
     if (again) {
-      find(by_weight, true, need, (float)fmax(aim.low - above, 0.) * (1.f - kSlack),
-           (float)fmax(aim.high - above, 0.) * (1.f + kSlack));
+      find(by_weight, true, need, (float)fmax(aim.low - ahead, 0.) * (1.f - kSlack),
+           (float)fmax(aim.high - ahead, 0.) * (1.f + kSlack));
       c1 = s.first;
       c2 = s.last;
       in = s.under;
@@ -750,30 +781,32 @@ struct RowOf {
     uint32_t lo = 0xffffffffu, hi = 0;
     double more = 0.;
     {
+      const float old_above = above;
+      if (again) set_window();
       const RowOf me = *this;   // a copy whose members are registers
       int* number = at(&s.listed, 0);
       uint32_t *keys = at(s.list_key, 0), *places = at(s.list_at, 0);
       me.template each<LIST>([&](float l, int k, int e) {
-        if (!me.stays(l)) return;
-        const int at_side = me.side(l);
-        if (at_side == 0) {
-          const uint32_t key = key_of(l);
-          if (listed) {
-            const int n = atomicAdd(number, 1);
-            if (n < kList) {   // which the bins' numbers have said
-              keys[n] = key;
-              places[n] = me.template index<LIST>(k, e);
+        if (l >= me.within && l < old_above) {
+          if (l >= me.above) {
+            if (by_weight) more += me.w.of(l);
+          } else {
+            const uint32_t key = key_of(l);
+            if (listed) {
+              const int n = atomicAdd(number, 1);
+              if (n < kList) {   // which the bins' numbers have said
+                keys[n] = key;
+                places[n] = me.template index<LIST>(k, e);
+              }
             }
+            lo = min(lo, key), hi = max(hi, key);
           }
-          lo = min(lo, key), hi = max(hi, key);
-        } else if (by_weight && again && at_side < 0 && me.bin(l) >= me.b1) {
-          more += me.w.of(l);
         }
       });
     }
-    if (by_weight && again) above += sum(more);
+    if (by_weight && again) ahead += sum(more);
     sync();
-    const bool on_border = most && side(on) == 0;
+    const bool on_border = most && side_of_border() == 0;
     if (listed) {
       const int n = min(*at(&s.listed, 0), kList);
       for (int i = tid; i < n; i += blockDim.x) s.mine_key[i] = at(s.list_key, 0)[i], s.mine_at[i] = at(s.list_at, 0)[i];
@@ -788,7 +821,7 @@ struct RowOf {
       if (by_weight && on_border) settle<ALL>(aim);
       while (by_weight) {
         if (warp == 0) {   // the sums before each, 32 at a time
-          double start = above;
+          double start = ahead;
           int kept = 0, most_kept = 0;
           for (int i = 0; i < n; i += 32) {
             double x = i + lane < n ? w.of(value_of(s.sorted[i + lane])) : 0.;
@@ -858,11 +891,11 @@ struct RowOf {
     const auto from = [&](uint32_t key) {
       double x = 0.;
       each_single<LIST>([&](float l, int, int) {
-        if (key_of(l) >= key && stays(l) && side(l) == 0) x += by_weight ? w.of(l) : 1.;
+        if (key_of(l) >= key && l >= within && l < above) x += by_weight ? w.of(l) : 1.;
       });
       return sum(x);
     };
-    const double start = by_weight ? above : 0., goal = by_weight ? aim.low : (double)need;
+    const double start = by_weight ? ahead : 0., goal = by_weight ? aim.low : (double)need;
     if (none || (on_border && start + from(lo) < goal)) {
       const double start2 = none ? start : start + from(lo);
       most = by_weight ? ties(start2, goal, w.of(on), old_most) : (int64_t)(goal - start2);
@@ -875,12 +908,12 @@ struct RowOf {
       if (start + from(mid) >= goal) lo = mid;
       else hi = mid - 1;
     }
-    const double ahead = start + (lo == top ? 0. : from(lo + 1));
+    const double front = start + (lo == top ? 0. : from(lo + 1));
     double x = 0.;
-    each_single<LIST>([&](float l, int, int) { x += key_of(l) == lo && stays(l) && side(l) == 0; });
+    each_single<LIST>([&](float l, int, int) { x += key_of(l) == lo && l >= within && l < above; });
     const int64_t have = (int64_t)sum(x);
     set_border(lo);
-    most = by_weight ? ties(ahead, goal, w.of(value_of(lo)), have) : (int64_t)(goal - ahead);
+    most = by_weight ? ties(front, goal, w.of(value_of(lo)), have) : (int64_t)(goal - front);
     most = max((int64_t)1, min(most, have));
   }
   // the fewest of `have` weights `x` that bring `ahead` to `aim`, one if there is nothing ahead
@@ -900,16 +933,17 @@ struct RowOf {
     int on = 0;
     {
       const RowOf me = *this;   // a copy whose members are registers
-      const auto is_above = [&](float l) {
-        if (me.most) on += key_of(l) == me.border;
-        return l >= me.least;
-      };
       if constexpr (EXACT) {
         me.template each<LIST>([&](float l, int, int) {
-          if (is_above(l)) above += me.w.of(l);
+          if (me.most) on += key_of(l) == me.border;
+          above += me.weight_from(l, me.least);
         });
       } else {
-        above = me.template mass<true>([&](float l) { return is_above(l) ? me.w.of32(l) : 0.f; });
+        above = me.template mass<true>([&](float l) {
+          if (me.most) on += key_of(l) == me.border;
+          const float x = me.w.of32(fmaxf(l, me.least));
+          return l >= me.least ? x : 0.f;
+        });
       }
     }
     above = warp_sum(above);
@@ -950,11 +984,11 @@ struct RowOf {
       bool done = false;
       for (int i = 0; i < ctas; ++i) {
         const double x = at(s.val[now], i)[0];
-        if (!done && x > 0.) chosen = i, start = run, done = run + x > u * total;
+        if (!done && x > 0.) chosen = i, start = run, done = run + x > target_of(u, total);
         run += x;
       }
     }
-    const double target = u * total - start;
+    const double target = target_of(u, total) - start;
     if (rank == chosen) {
       double run = 0., from = 0.;
       int64_t mine = 0;
@@ -1013,7 +1047,7 @@ struct RowOf {
       double own = 0.;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        x[e] = v[e] >= me.least ? me.w.of(v[e]) : 0.;
+        x[e] = me.weight_from(v[e], me.least);
         if (me.most && key_of(v[e]) == me.border) x[e] = mine++ < me.most ? x_on : 0.;
         own += x[e];
       }
