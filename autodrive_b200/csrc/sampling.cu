@@ -638,6 +638,7 @@ struct RowOf {
       unsigned take = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) take |= (unsigned)(v[e] >= me.within) << e;
+      if (!__any_sync(0xffffffffu, take)) continue;
       const int own = __popc(take);
       int at = own;
 #pragma unroll
@@ -1163,7 +1164,7 @@ struct RowOf {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(512, 2) row_kernel(const __grid_constant__ Args a, const __grid_constant__ Plan p) {
+__global__ void __launch_bounds__(256, 4) row_kernel(const __grid_constant__ Args a, const __grid_constant__ Plan p) {
   __shared__ Shared s;
   extern __shared__ __align__(16) unsigned char raw[];
   RowOf<T> on(a, s, raw, p);
@@ -1192,11 +1193,12 @@ cudaError_t launch_rows(const Args& a, const Plan& p, cudaStream_t st) {
 
 Plan plan(const Args& a, int sms) {
   Plan p{};
-  // Threads by the row's length: half as many cost 2047 rows of 8000 65 %, of
-  // 32003 60 % of this time and more; twice as many 40 % and 15 % more.
-  p.threads = a.v <= 2048 ? 64 : a.v <= 8192 ? 128 : 256;
+  // Threads by the row's length. Twice as many cost 16384 rows of 500 (bf16, top-k 50) 15 %, 2047 rows of 8000 (top-p .9)
+  // 19 % more; half as many, 2047 rows of 2000 (top-k 50) 24 %, of 8000 38 % and of 32003 (top-p .95) 2 % more, 2 rows of
+  // 131072 28 %.
+  p.threads = a.v <= 1024 ? 64 : a.v <= 8192 ? 128 : 256;
   const int64_t vectors = (a.v + 14) / 8;   // with what lies before a row's start
-  p.bins = std::max(2048, 8 * p.threads);
+  p.bins = a.v <= 1024 ? 1024 : 2048;   // finer ones than a row has entries for cost more to go through
   p.ctas = 1;
   const auto strips = [&] { return (int)((vectors + (int64_t)p.ctas * p.threads - 1) / ((int64_t)p.ctas * p.threads)); };
   while (p.ctas < 8 && a.rows * p.ctas * 2 <= sms && strips() > 2) p.ctas *= 2;   // few rows are shared by more CTAs
