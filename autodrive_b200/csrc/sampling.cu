@@ -1203,17 +1203,19 @@ Plan plan(const Args& a, int sms) {
   const auto strips = [&] { return (int)((vectors + (int64_t)p.ctas * p.threads - 1) / ((int64_t)p.ctas * p.threads)); };
   while (p.ctas < 8 && a.rows * p.ctas * 2 <= sms && strips() > 2) p.ctas *= 2;   // few rows are shared by more CTAs
   p.strips = strips();
-  p.listed = std::min(p.strips * 48, 4096);   // three sixteenths of a warp's entries
+  // all of a warp's entries where they are few, and three sixteenths of many
+  p.listed = std::max(std::min(p.strips * 256, 768), std::min(p.strips * 48, 4096));
   return p;
 }
 
 template <typename T>
 cudaError_t launch_type(const Args& a, int sms, cudaStream_t st) {
-  if (a.v <= 128) {
+  if (a.v <= 256) {
     const auto grid = [&](int w) { return (unsigned)((a.rows + 128 / w - 1) / (128 / w)); };
     if (a.v <= 8) short_kernel<T, 8, 1><<<grid(8), 128, 0, st>>>(a);
     else if (a.v <= 32) short_kernel<T, 32, 1><<<grid(32), 128, 0, st>>>(a);
-    else short_kernel<T, 32, 4><<<grid(32), 128, 0, st>>>(a);
+    else if (a.v <= 128) short_kernel<T, 32, 4><<<grid(32), 128, 0, st>>>(a);
+    else short_kernel<T, 32, 8><<<grid(32), 128, 0, st>>>(a);
     return cudaGetLastError();
   }
   return launch_rows<T>(a, plan(a, sms), st);
