@@ -20,7 +20,16 @@
 // value once. Larger samples are cut into parts, a CTA's each: one launch takes
 // the parts' sums, a second one reads them again, the last first, as L2 may
 // still hold those. A thread keeps its next vectors under way in a ring of its
-// own slots.
+// own slots (24 KB a CTA: with two vectors in registers instead, the wide case
+// below took 490 us). Clusters that hold a sample were slower (700 us: three
+// barriers across the cluster, and no room for a second one's phases beside it).
+//
+// Measured on one B200, forward and backward: 384 x 128 channels x 32 x 64 bf16
+// 316 us (1.6 GB of traffic, 5.1 TB/s; 0.8 GB that are needed), 512 x 24 x 25 x 51
+// fp32 107 us, 3 x 36 x 257 x 263 fp16 48 us, one fp32 raster of 24 x 25 x 51
+// forward 8.3 us. The backward's sums are bound by the special functions (two an
+// element), the results by DRAM, the small ones by two launches and the chain of
+// loads, joins and barriers in each.
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -9,10 +9,29 @@
 //          the staying w exceeds u times their sum
 //
 // Which entry that is hangs on a sum's last bits: of 131072 entries one in
-// fifty rows would come out otherwise with 32-bit sums. Weights and sums are
-// fp64 (the device has half as many fp64 units as fp32 ones), added in an order
-// that the sizes alone give. Entries further than 44 T below the largest (they
-// hold less than 10^-13 of any row's sum) count as zero.
+// fifty rows would come out otherwise with 32-bit sums. So the answer is the one
+// that fp64 weights and sums give. A pass over a row in fp64 costs twice one in
+// fp32 and more (17 fp64 operations an entry), so long rows are summed up in
+// fp32, with an error that is known, and in fp64 only where that error could
+// change the answer (an eighth of the rows at 32003 entries with a top-p among
+// thousands of them, one in 200 without). All sums are added in an order that
+// the sizes alone give. Entries further than 44 T below the largest (they hold
+// less than 10^-13 of any row's sum) count as zero.
+//
+// Rows of up to 256 entries lie in a warp's registers and order themselves by
+// comparing all with all. Longer rows stay in L2 and are read by a CTA three
+// times (few rows by clusters of up to eight): for the largest, into bins of
+// (max - l) / T, and for what lies above the bins in which the cut-off must be,
+// which goes to lists in shared memory; a second, finer set of bins and an
+// ordered list of what is left in them give the border itself. Bins and not a
+// sort, as a cut-off needs no order but its own place. Holding rows in shared memory
+// was slower (three CTAs an SM instead of five: 633 against 571 us at 2047 x 32003).
+//
+// Measured on one B200: 6144 rows of 8 fp32 entries 3.9 us; 2 x 131072 bf16,
+// top-k 50, 71 us; 2047 x 32003 bf16, top-p .95, 507 us (131 MB: 20 us at the
+// copy's rate); without cut-offs 200 us. Bound by instruction issue: about 150
+// instructions an entry's warp over all passes, a tenth of them fp64; the bins'
+// atomics are bound by bank conflicts (5.5 cycles each).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -278,6 +297,7 @@ struct Plan {
   int strips;           // of 32 vectors of 8 entries, of a warp
   int listed;           // entries that a warp's list holds
   int bins;             // of the order
+  int sums;             // fp32 sums of strips that a warp holds: all, or none where the sums are fp64 ones
 };
 
 // What the threads of a CTA share; `val`, `flag` and `list` are read by the row's other CTAs.
@@ -333,7 +353,7 @@ struct RowOf {
       raw += sizeof(uint32_t) * bins;
     }
     strip_sum = reinterpret_cast<float*>(raw) + warp * strips;
-    raw += sizeof(float) * warps * strips;
+    raw += sizeof(float) * warps * p.sums;
     list_value = reinterpret_cast<T*>(raw) + warp * capacity;
     list_index = reinterpret_cast<uint16_t*>(raw + sizeof(T) * warps * capacity) + warp * capacity;
     x = static_cast<const T*>(a.logits) + row * a.ld;
@@ -1174,7 +1194,7 @@ __global__ void __launch_bounds__(256, 4) row_kernel(const __grid_constant__ Arg
 template <typename T>
 cudaError_t launch_rows(const Args& a, const Plan& p, cudaStream_t st) {
   const auto kernel = row_kernel<T>;
-  const int smem = (p.ctas > 1 ? 8 : 4) * p.bins + p.strips * p.threads / 8 + p.threads / 32 * p.listed * ((int)sizeof(T) + 2);
+  const int smem = (p.ctas > 1 ? 8 : 4) * p.bins + p.sums * p.threads / 8 + p.threads / 32 * p.listed * ((int)sizeof(T) + 2);
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -1203,6 +1223,7 @@ Plan plan(const Args& a, int sms) {
   const auto strips = [&] { return (int)((vectors + (int64_t)p.ctas * p.threads - 1) / ((int64_t)p.ctas * p.threads)); };
   while (p.ctas < 8 && a.rows * p.ctas * 2 <= sms && strips() > 2) p.ctas *= 2;   // few rows are shared by more CTAs
   p.strips = strips();
+  p.sums = a.v <= kMost32 ? p.strips : 0;
   // all of a warp's entries where they are few, and three sixteenths of many
   p.listed = std::max(std::min(p.strips * 256, 768), std::min(p.strips * 48, 4096));
   return p;

@@ -284,3 +284,16 @@ def test_rows_behind_32_bits():
     r = sample_tokens(x, u, None, 1., 20, .9)
     at = torch.tensor([0, n // 2, n - 2, n - 1], device="cuda")
     _check(x[at], u[at], None, 1., 20, .9, 0., type(r)(r.token[at], r.log_prob[at]))
+
+
+@pytest.mark.gpu
+def test_rows_beyond_the_fp32_sums():
+    for rows, v in ((1, 3_000_001), (160, 1_200_003)):
+        x, u, _ = _make(2, v, torch.bfloat16, "cuda")
+        x = x[:1].expand(rows, v).contiguous()
+        x[:, 5] = 20.
+        u = torch.linspace(.05, .95, rows, device="cuda")
+        for cut in ((1., 0, .9, 0.), (.5, 30, 1., 0.), (1., 0, 1., 0.)):
+            r = sample_tokens(x, u, None, *cut)
+            at = torch.tensor(sorted({0, rows - 1}), device="cuda")
+            _check(x[at], u[at], None, *cut, type(r)(r.token[at], r.log_prob[at]))
