@@ -3,8 +3,8 @@
 The Python entry points of the native kernels (tensor-core GEMM, fused
 LayerNorm, GAE, fused Adam, peer all-reduce) add the number of kernels each
 call launches; benchmarks read the count around a timed region. The operators
-whose autograd is in C++ (RMS norm, 8-bit products, token log-probabilities)
-count theirs in the extension. Simulator kernels are launched from C++ methods
+whose host code is in C++ (RMS norm, 8-bit products, token log-probabilities,
+sampling, group norm, AdamW) count theirs in the extension. Simulator kernels are launched from C++ methods
 and are counted by their callers.
 """
 from __future__ import annotations
