@@ -130,6 +130,8 @@ torch::Tensor group_norm(torch::Tensor x, int64_t groups, c10::optional<torch::T
   const int64_t c = x.size(1);
   LM_CHECK_VALUE(c >= 1 && c <= 8192, "group_norm takes 1 to 8192 channels, not ", c);
   LM_CHECK_VALUE(groups >= 1 && c % groups == 0, "group_norm: ", c, " channels do not make ", groups, " groups");
+  // what a CTA of the backward holds of them in shared memory beside its vectors: 16 (c + groups) bytes
+  LM_CHECK_VALUE(c + groups <= 10240, "group_norm takes at most 10240 channels and groups together, not ", c, " and ", groups);
   for (const auto* p : {&weight, &bias})
     LM_CHECK_VALUE(!*p || ((*p)->dim() == 1 && (*p)->size(0) == c && type_code((*p)->scalar_type()) >= 0 &&
                            (*p)->device() == x.device()),

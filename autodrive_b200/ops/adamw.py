@@ -12,7 +12,8 @@ and their moments in place:
 
 * It returns the gradients' norm (fp32, on the device) where they are clipped,
   otherwise None. Computation is fp32 (the norm's sum fp64); a 16-bit parameter
-  is rounded once, a NaN or infinite norm makes all parameters NaN.
+  is rounded once. Where gradients are clipped, a NaN in one of them makes all
+  parameters NaN; an infinity makes its own NaN and counts the others as zero.
 * Moments without scales are fp32 of their parameter's shape and strides. With
   scales they are e4m3 numbers of that shape, one fp32 scale for each 256
   elements (in memory order): m, and the root of v in `exp_avg_sqs`. Their

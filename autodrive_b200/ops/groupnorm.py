@@ -3,9 +3,9 @@ backward, on fused sm_100a kernels (``csrc/groupnorm.cu``).
 
 ``group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None)``
 normalises each sample's groups of channels of `x` [N, C, ...] (fp32, bf16 or
-fp16; at most 8192 channels) and applies the activation (``"silu"``, ``"relu"``,
-``"gelu"`` (by the error function) or none), with autograd. Statistics and sums
-are fp32. The result lies in channels-last memory ([N, ..., C], what PyTorch's
+fp16; at most 8192 channels, and 10240 channels and groups together) and applies
+the activation (``"silu"``, ``"relu"``, ``"gelu"`` (by the error function) or
+none), with autograd. Statistics and sums are fp32. The result lies in channels-last memory ([N, ..., C], what PyTorch's
 ``channels_last`` formats mean); an `x` in other memory is copied there first.
 
 ``FusedGroupNorm`` is a drop-in ``nn.GroupNorm`` with an activation, and
@@ -23,6 +23,7 @@ from .ext import require_extension
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_CHANNELS = 8192
+MAX_TOGETHER = 10240   # channels and groups
 ACTIVATIONS = (None, "silu", "relu", "gelu")
 _ACT = {"silu": F.silu, "relu": F.relu, "gelu": F.gelu}
 
@@ -60,6 +61,8 @@ def group_norm(x: Tensor, groups: int, weight: Tensor | None = None, bias: Tenso
         raise ValueError(f"group_norm takes 1 to {MAX_CHANNELS} channels, not {c}")
     if groups < 1 or c % groups:
         raise ValueError(f"group_norm: {c} channels do not make {groups} groups")
+    if c + groups > MAX_TOGETHER:
+        raise ValueError(f"group_norm takes at most {MAX_TOGETHER} channels and groups together, not {c} and {groups}")
     for p in (weight, bias):
         if p is not None and (p.shape != (c,) or p.dtype not in DTYPES or p.device != x.device):
             raise ValueError(f"group_norm needs fp32, bf16 or fp16 parameters [{c}] on {x.device}")
@@ -103,7 +106,7 @@ def fuse_group_norms(module: nn.Module) -> nn.Module:
     """Put a FusedGroupNorm, with the same parameters, in the place of every plain nn.GroupNorm of `module`
     (recursively), in place. In an nn.Sequential the SiLU, ReLU or GELU behind a norm becomes its activation, with an
     nn.Identity left in its place, so that the state dict keeps its keys; an activation that stands in several places
-    or has hooks stays, and so does a norm with hooks or of more than 8192 channels. The module's convolutions run best on
+    or has hooks stays, and so does a norm with hooks or of more channels or groups than ``group_norm`` takes. The module's convolutions run best on
     channels-last weights: ``module.to(memory_format=torch.channels_last)``. Returns the module, or the fused norm where
     the module itself is a norm."""
     return _fuse(module, {}, _places(module, {}))
@@ -126,7 +129,8 @@ def _fuse(module: nn.Module, done: dict, places: dict) -> nn.Module:
         return done[module]
     done[module] = module
     if type(module) is nn.GroupNorm:
-        if _bare(module) and module.num_channels <= MAX_CHANNELS:
+        if (_bare(module) and module.num_channels <= MAX_CHANNELS
+                and module.num_channels + module.num_groups <= MAX_TOGETHER):
             fused = done[module] = FusedGroupNorm(module.num_groups, module.num_channels, module.eps, False)
             fused.affine, fused.training = module.affine, module.training
             fused.weight, fused.bias = module.weight, module.bias

@@ -127,6 +127,8 @@ class FusedAdamW(torch.optim.Optimizer):
     def _moments(self, p: torch.Tensor, bits: int) -> dict:
         state = self.state[p]
         if not state:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("FusedAdamW: the first step of a parameter makes its moments and cannot be captured")
             state["step"] = 0
             if bits == 32:
                 state["exp_avg"], state["exp_avg_sq"] = (torch.zeros_like(p, dtype=torch.float32) for _ in range(2))

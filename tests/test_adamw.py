@@ -334,3 +334,33 @@ def test_elements_behind_32_bits():
     at = torch.tensor([0, 1 << 30, (1 << 31) - 1, 1 << 31, n - 1], device="cuda")
     assert torch.equal(p[at], torch.full((5,), -.5, dtype=torch.bfloat16, device="cuda"))
     assert (m[at].float() == 448).all() and (r[at].float() == 448).all() and (ms[-1] > 0)
+
+
+@pytest.mark.gpu
+def test_first_step_is_not_captured():
+    p = torch.ones(300, device="cuda", requires_grad=True)
+    p.grad = torch.ones_like(p)
+    opt = FusedAdamW([p], capturable=True)
+    x = torch.zeros(1, device="cuda")
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        x.add_(1.)
+        with pytest.raises(RuntimeError, match="moments"):
+            opt.step()
+    opt.step()
+    assert (p.detach() < 1.).all() and int(opt.param_groups[0]["step"]) == 1
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_gradients_that_are_not_finite(device, value):
+    p = torch.ones(600, device=device)
+    g, m, v = torch.ones_like(p), torch.zeros_like(p), torch.zeros_like(p)
+    g[300] = value
+    norm = adamw_step([p], [g], [m], [v], step=1, lr=.5, weight_decay=0., max_grad_norm=1.)
+    assert not norm.isfinite()
+    others = torch.arange(600, device=device) != 300
+    assert p[300].isnan() and m[300].isnan()
+    if math.isnan(value):
+        assert p.isnan().all()
+    else:   # clipped to nothing
+        assert torch.equal(p[others], torch.ones_like(p[others])) and not m[others].any()

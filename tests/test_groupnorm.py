@@ -322,3 +322,19 @@ def test_samples_behind_32_bits():
     at = [0, n // 2, n - 2, n - 1]
     want = F.silu(F.group_norm(x[at].float(), 4))
     assert ((y[at].float() - want).abs() <= 2. ** -8 * want.abs() + 2. ** -9).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("c,groups", [(8192, 4096), (6144, 6144), (5122, 5122)])
+def test_too_many_groups(device, c, groups):
+    with pytest.raises(ValueError, match="together"):
+        group_norm(torch.zeros(1, c, 1, device=device), groups)
+    kept = nn.GroupNorm(groups, c, affine=False)
+    assert fuse_group_norms(kept) is kept
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups", [((2, 8192, 3, 3), 2048), ((1, 5120, 5, 3), 5120), ((1, 5119, 4, 3), 5119), ((1, 2040, 70, 1), 2040)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_most_groups(shape, groups, dtype):
+    _check(shape, groups, dtype, "cuda", "relu")
