@@ -56,8 +56,8 @@ torch::Tensor in_layout_of(const torch::Tensor& g, const torch::Tensor& p) {
 }
 
 py::object adamw_step(py::object params_, py::object grads_, py::object ms_, py::object vs_, py::object m_scales_,
-                      py::object v_scales_, py::object step, double lr, double b1, double b2, double eps, double weight_decay, double max_norm,
-                      int64_t seed) {
+                      py::object v_scales_, py::object step, double lr, double b1, double b2, double eps,
+                      double weight_decay, double max_norm, int64_t seed) {
   const at::NoGradGuard no_grad;
   const List params(params_), grads(grads_), ms(ms_), vs(vs_);
   c10::optional<List> m_scales, v_scales;
@@ -90,8 +90,8 @@ py::object adamw_step(py::object params_, py::object grads_, py::object ms_, py:
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     TORCH_CHECK(cudaStreamIsCapturing(st, &capture) == cudaSuccess, "adamw_step: stream query failed");
     TORCH_CHECK(capture == cudaStreamCaptureStatusNone,
-                "adamw_step: a captured step would be replayed under its one number; give the step as an int64 tensor on ",
-                device.str());
+                lm::message("adamw_step: a captured step would be replayed under its one number; give the step as an int64 "
+                            "tensor on ", device));
   }
 
   std::vector<Entry> all;

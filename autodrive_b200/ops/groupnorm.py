@@ -7,6 +7,9 @@ fp16; at most 8192 channels, and 10240 channels and groups together) and applies
 the activation (``"silu"``, ``"relu"``, ``"gelu"`` (by the error function) or
 none), with autograd. Statistics and sums are fp32. The result lies in channels-last memory ([N, ..., C], what PyTorch's
 ``channels_last`` formats mean); an `x` in other memory is copied there first.
+It has no second derivative. Before a backward pass is captured into a CUDA
+graph, eager graphs of the same leaves have to be gone, as for PyTorch's own
+operators.
 
 ``FusedGroupNorm`` is a drop-in ``nn.GroupNorm`` with an activation, and
 ``fuse_group_norms(module)`` puts it in the place of the group norms of a module

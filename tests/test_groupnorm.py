@@ -338,3 +338,36 @@ def test_too_many_groups(device, c, groups):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_most_groups(shape, groups, dtype):
     _check(shape, groups, dtype, "cuda", "relu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(64, 24, 25, 51), (400, 16, 6, 7), (3, 20, 90, 91)])
+def test_captured_training_step(shape):
+    x, dy, w, b = _make(shape, 4, torch.bfloat16, "cuda")
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+
+    def step():
+        y = group_norm(x, 4, w, b, activation="silu")
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph in graphs:   # two, whose workspaces must not meet
+        with torch.cuda.graph(graph):
+            outs.append(step())
+    with torch.no_grad():
+        x.copy_(torch.randn_like(x))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    want = step()
+    for out in outs:
+        assert all(torch.equal(a, c) for a, c in zip(out, want))
