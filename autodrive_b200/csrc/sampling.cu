@@ -101,6 +101,21 @@ __device__ __forceinline__ double exp_of(double x) {
   return __hiloint2double(__double2hiint(p) + (k << 20), __double2loint(p));
 }
 
+// The first of the keys lo..hi for whose value f holds, as it does for all
+// larger ones and for hi's: a warp's search, 32 keys at a time.
+template <typename F>
+__device__ __forceinline__ uint32_t first_key(uint32_t lo, uint32_t hi, int lane, F&& f) {
+  while (lo < hi) {
+    const uint32_t step = (hi - lo) / 32 + 1, mine = min(lo + lane * step, hi);
+    const unsigned holds = __ballot_sync(0xffffffffu, f(value_of(mine)));
+    const int first = holds ? __ffs(holds) - 1 : 32;
+    if (first == 0) break;
+    hi = min(hi, first < 32 ? lo + first * step : hi);
+    lo = min(lo + (first - 1) * step + 1, hi);
+  }
+  return lo;
+}
+
 // Weights relative to the row's largest logit.
 struct Weights {
   double top, inv;        // 1 / T
@@ -125,14 +140,8 @@ struct Weights {
       return;
     }
     lowest = __double2float_ru(top - (double)kRange * r.t);   // at least the lowest number, and at most the largest logit
-    if (cut && r.min_p > 0.) {   // by halving: a logit stays or not by its weight in fp64
-      uint32_t lo = key_of(lowest), hi = key_of(m);
-      while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (of(value_of(mid)) >= r.min_p) hi = mid;
-        else lo = mid + 1;
-      }
-      lowest = value_of(lo);
+    if (cut && r.min_p > 0.) {   // a logit stays or not by its weight in fp64
+      lowest = value_of(first_key(key_of(lowest), key_of(m), threadIdx.x & 31, [&](float l) { return of(l) >= r.min_p; }));
       far = fminf(kRange, (float)((top - (double)lowest) * inv));
     }
   }
@@ -311,7 +320,7 @@ struct Shared {
   // of this CTA alone
   uint32_t mine_key[kList], mine_at[kList], sorted[kList];
   double red[32][2];
-  float fred[32];
+  float fred[32], window[2];
   int ired[32];
   int first, last, under, before, all, kept;
   int count[32];        // entries of the warps' lists
@@ -510,19 +519,10 @@ struct RowOf {
   }
   // The window as logits: entries from `above` on are above it, those from `within` on in it.
   float above = 0.f, within = 0.f;
-  // The smallest logit that stays and for which f holds, as it does for all larger ones: a search of 32 ways.
+  // The smallest logit that stays and for which f holds, as it does for all larger ones.
   template <typename F>
   __device__ __forceinline__ float lowest_where(F&& f) const {
-    uint32_t lo = key_of(least), hi = key_of(w.top32);
-    while (lo < hi) {
-      const uint32_t step = (hi - lo) / 32 + 1, mine = min(lo + lane * step, hi);
-      const unsigned holds = __ballot_sync(0xffffffffu, f(value_of(mine)));
-      const int first = holds ? __ffs(holds) - 1 : 32;
-      if (first == 0) break;
-      hi = min(hi, first < 32 ? lo + first * step : hi);
-      lo = min(lo + (first - 1) * step + 1, hi);
-    }
-    return value_of(lo);
+    return value_of(first_key(key_of(least), key_of(w.top32), lane, f));
   }
   // Whether the border's own logit (the lowest that stays) is in the window, or above it.
   __device__ __forceinline__ int side_of_border() const {
@@ -533,14 +533,23 @@ struct RowOf {
     const int c = fine ? bin2(l) : 0;
     return fine && c < c1 ? -1 : fine && c > c2 ? 1 : 0;
   }
+  // One warp looks for `above`, another for `within` (by all of them, 2 % of a long row's time more).
   __device__ __forceinline__ void set_window() {
-    if (fine) {
-      above = b1 == 0 && c1 == 0 ? INFINITY : lowest_where([&](float l) { return bin(l) < b1 || (bin(l) <= b2 && bin2(l) < c1); });
-      within = lowest_where([&](float l) { return bin(l) < b1 || (bin(l) <= b2 && bin2(l) <= c2); });
-    } else {
-      above = b1 == 0 ? INFINITY : lowest_where([&](float l) { return bin(l) < b1; });
-      within = b2 == bins - 1 ? least : lowest_where([&](float l) { return bin(l) <= b2; });
+    if (warp < 2) {
+      float l;
+      if (fine) {
+        const int c = warp ? c2 : c1 - 1;
+        l = warp || b1 > 0 || c1 > 0 ? lowest_where([&](float l) { return bin(l) < b1 || (bin(l) <= b2 && bin2(l) <= c); })
+                                     : INFINITY;
+      } else {
+        const int b = warp ? b2 : b1 - 1;
+        l = b < 0 ? INFINITY : b == bins - 1 ? least : lowest_where([&](float l) { return bin(l) <= b; });
+      }
+      if (lane == 0) s.window[warp] = l;
     }
+    __syncthreads();
+    above = s.window[0];
+    within = s.window[1];
   }
   __device__ __forceinline__ bool stays(float l) const { return l >= least; }
   __device__ __forceinline__ void set_border(uint32_t key) {
@@ -668,15 +677,16 @@ struct RowOf {
       }
       const int strip = __shfl_sync(0xffffffffu, at, 31);
       at += n - own;
+      n += strip;
+      if (n > me.capacity) continue;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if ((take >> e & 1) && at < me.capacity) {
+        if (take >> e & 1) {
           me.list_value[at] = lm::from_f<T>(v[e]);
           me.list_index[at] = (uint16_t)(k * 256 + me.lane * 8 + e);
         }
         at += take >> e & 1;
       }
-      n += strip;
     }
     if (lane == 0) s.count[warp] = min(n, capacity);
     return sum(lane == 0 && n > capacity ? 1. : 0.) == 0.;
@@ -734,7 +744,7 @@ struct RowOf {
       // (entries on an older border are in no list, so it has to be the first)
       if (!most && before + in <= (int64_t)capacity * warps * ctas && strips <= 256) held = compact();
     }
-    Aim aim{p, 0., 0., true};
+    Aim aim{p, 0., 0., true, within};
     if (by_weight) {
       sum_of = rough ? sum(sum_of) + (most ? (double)most * w.of(on) : 0.) : total<LIST>();
       aim.low = p * sum_of * (1. - (rough ? kError : 0.));
@@ -749,7 +759,27 @@ struct RowOf {
   struct Aim {
     double p, low, high;
     bool exact;
+    float within;   // what the lists hold: the entries from here on
+    bool refined = false;
   };
+  // A narrower range of the sum: those in the lists hold nearly all of it and
+  // are added up in fp64, those below in fp32. (The border is the first one,
+  // so that all that stay are at or above `least`; 2^-40: of fp64 sums in
+  // another order.)
+  __device__ __noinline__ void refine(Aim& aim) {
+    const RowOf me = *this;   // a copy whose members are registers
+    double listed = 0., rest;
+    const float end = aim.within;
+    rest = me.template mass<false>([&](float l) {
+      const float x = me.w.of32(fmaxf(l, me.least));
+      return l >= me.least && l < end ? x : 0.f;
+    });
+    me.template each<true>([&](float l, int, int) { listed += me.weight_from(l, end); });
+    sums(listed, rest);
+    aim.low = aim.p * ((listed + rest * (1. - kError)) * (1. - 0x1p-40));
+    aim.high = aim.p * ((listed + rest * (1. + kError)) * (1. + 0x1p-40));
+    aim.refined = true;
+  }
   template <bool LIST>
   __device__ void settle(Aim& aim) {
     if (aim.exact) return;
@@ -862,7 +892,15 @@ struct RowOf {
         }
         __syncthreads();
         if (s.kept == s.last) break;
-        settle<ALL>(aim);   // a sum's end lies in the range
+        // a sum's end lies in the range
+        if constexpr (LIST && !ALL) {
+          if (!aim.refined && !aim.exact) {
+            refine(aim);
+            __syncthreads();
+            continue;
+          }
+        }
+        settle<ALL>(aim);
         __syncthreads();
       }
       const int kept = by_weight ? s.kept : (int)min(need, (int64_t)n);
