@@ -13,8 +13,9 @@
 // that fp64 weights and sums give. A pass over a row in fp64 costs twice one in
 // fp32 and more (17 fp64 operations an entry), so long rows are summed up in
 // fp32, with an error that is known, and in fp64 only where that error could
-// change the answer (an eighth of the rows at 32003 entries with a top-p among
-// thousands of them, one in 200 without). All sums are added in an order that
+// change the answer (one in 200 rows of 32003 entries; of those with a top-p
+// among thousands of entries a seventh add up the entries above the cut-off in
+// fp64 and one in a hundred all of them). All sums are added in an order that
 // the sizes alone give. Entries further than 44 T below the largest (they hold
 // less than 10^-13 of any row's sum) count as zero.
 //
@@ -28,8 +29,8 @@
 // was slower (three CTAs an SM instead of five: 633 against 571 us at 2047 x 32003).
 //
 // Measured on one B200: 6144 rows of 8 fp32 entries 3.9 us; 2 x 131072 bf16,
-// top-k 50, 71 us; 2047 x 32003 bf16, top-p .95, 507 us (131 MB: 20 us at the
-// copy's rate); without cut-offs 200 us. Bound by instruction issue: about 150
+// top-k 50, 67 us; 2047 x 32003 bf16, top-p .95, 478 us (131 MB: 20 us at the
+// copy's rate); without cut-offs 200 us. Bound by instruction issue: about 130
 // instructions an entry's warp over all passes, a tenth of them fp64; the bins'
 // atomics are bound by bank conflicts (5.5 cycles each).
 #include <cooperative_groups.h>
@@ -587,14 +588,28 @@ struct RowOf {
       h += (float)c * f;
       f *= ratio;
     };
-    for (int q = 0; q < per / 4; ++q) {
-      uint4 c = make_uint4(0, 0, 0, 0);
-#pragma unroll 4
-      for (int k = 0; k < ctas; ++k) {
-        const uint4 x = reinterpret_cast<const uint4*>(at(hist, k))[tid * per / 4 + q];
-        c.x += x.x, c.y += x.y, c.z += x.z, c.w += x.w;
+    // each CTA adds up a share of the bins, which the others then read (all of them by every CTA: 70 instead of 67 us at
+    // 2 x 131072, as another CTA's memory is read at a few bytes a cycle)
+    const uint4* whole = mine;
+    bool copied = false;
+    if (ctas > 1) {
+      const int part = bins / ctas, owner = tid * per / part;
+      for (int i = tid; i < part / 4; i += blockDim.x) {
+        uint4 c = make_uint4(0, 0, 0, 0);
+#pragma unroll 8
+        for (int k = 0; k < ctas; ++k) {
+          const uint4 x = reinterpret_cast<const uint4*>(at(hist, k) + rank * part)[i];
+          c.x += x.x, c.y += x.y, c.z += x.z, c.w += x.w;
+        }
+        reinterpret_cast<uint4*>(joined + rank * part)[i] = c;
       }
-      if (ctas > 1) mine[q] = c;
+      sync();
+      whole = reinterpret_cast<const uint4*>(at(joined, owner)) + tid * per / 4;
+      copied = owner != rank;
+    }
+    for (int q = 0; q < per / 4; ++q) {
+      const uint4 c = whole[q];
+      if (copied) mine[q] = c;
       add(c.x), add(c.y), add(c.z), add(c.w);
     }
     // sums of the threads before this one
